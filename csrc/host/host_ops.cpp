@@ -12,6 +12,7 @@
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
 
+#include <algorithm>
 #include <optional>
 #include <string>
 #include <tuple>
@@ -732,6 +733,136 @@ Tensor mlp_block_bwd(const Tensor& dy, const Tensor& x, const Tensor& scale,
   return norm_backward(*dh, x, scale, rstd, dy, dscale, st);
 }
 
+// ---- the optimizer's step over trees of parameters ----
+
+// What adamw_tree has gathered of the trees.
+struct AdamwItems {
+  std::vector<t5x_adamw_item> items;
+  std::vector<std::pair<uintptr_t, uintptr_t>> written;  // [begin, end) of what the step writes
+  c10::DeviceIndex device;
+  bool small;  // moments in 8 bits
+
+  void writes(const void* p, size_t bytes) {
+    const auto at = reinterpret_cast<uintptr_t>(p);
+    if (bytes) written.emplace_back(at, at + bytes);
+  }
+  // Whether two of the tensors share memory: the parameters then have to be updated in turn.
+  bool overlap() {
+    std::sort(written.begin(), written.end());
+    for (size_t i = 1; i < written.size(); ++i)
+      if (written[i].first < written[i - 1].second) return true;
+    return false;
+  }
+};
+
+constexpr int64_t kMomentBlock = 256;  // values that share a scale in 8-bit moments
+
+// A contiguous tensor of n values on the device, or null.
+const Tensor* leaf(PyObject* o, at::ScalarType type, c10::DeviceIndex device, int64_t n) {
+  if (o == nullptr || !THPVariable_CheckExact(o)) return nullptr;
+  const Tensor& t = THPVariable_Unpack(o);
+  if (!t.defined() || !t.is_cuda() || t.scalar_type() != type || t.get_device() != device ||
+      (n >= 0 && t.numel() != n) || !t.is_contiguous())
+    return nullptr;
+  return &t;
+}
+
+// Adds the parameters of one level. False: something that the grouped step does not cover.
+bool gather(PyObject* params, PyObject* grads, PyObject* mu, PyObject* nu, PyObject* mu_most,
+            PyObject* nu_most, AdamwItems& to) {
+  PyObject* trees[5] = {grads, mu, nu, mu_most, nu_most};
+  const int count = to.small ? 5 : 3;
+  for (int i = 0; i < count; ++i)
+    if (trees[i] == nullptr || !PyDict_CheckExact(trees[i]) || PyDict_Size(trees[i]) != PyDict_Size(params))
+      return false;
+  PyObject *key, *value;
+  Py_ssize_t pos = 0;
+  while (PyDict_Next(params, &pos, &key, &value)) {
+    PyObject* at[5] = {};
+    for (int i = 0; i < count; ++i)
+      if ((at[i] = PyDict_GetItemWithError(trees[i], key)) == nullptr) {
+        PyErr_Clear();
+        return false;
+      }
+    if (PyDict_CheckExact(value)) {
+      if (!gather(value, at[0], at[1], at[2], at[3], at[4], to)) return false;
+      continue;
+    }
+    const Tensor* p = leaf(value, at::kFloat, to.device, -1);
+    if (p == nullptr) return false;
+    const int64_t n = p->numel(), blocks = (n + kMomentBlock - 1) / kMomentBlock;
+    const auto type = to.small ? at::kByte : at::kFloat;
+    const Tensor* g = leaf(at[0], at::kFloat, to.device, n);
+    const Tensor *m = leaf(at[1], type, to.device, n), *v = leaf(at[2], type, to.device, n);
+    if (g == nullptr || m == nullptr || v == nullptr) return false;
+    t5x_adamw_item item = {p->data_ptr(), g->data_ptr(), m->data_ptr(), v->data_ptr(), nullptr, nullptr,
+                           nullptr, n};
+    if (to.small) {
+      const Tensor *a = leaf(at[3], at::kFloat, to.device, blocks), *b = leaf(at[4], at::kFloat, to.device, blocks);
+      if (a == nullptr || b == nullptr) return false;
+      item.mu_absmax = a->data_ptr();
+      item.nu_absmax = b->data_ptr();
+      to.writes(item.mu_absmax, blocks * 4);
+      to.writes(item.nu_absmax, blocks * 4);
+    }
+    PyObject* attributes = PyObject_GenericGetDict(value, nullptr);
+    if (attributes == nullptr) {
+      PyErr_Clear();
+      return false;
+    }
+    PyObject* sharded = PyDict_GetItemString(attributes, "zero");
+    PyObject* copy = PyDict_GetItemString(attributes, "bf16");
+    Py_DECREF(attributes);  // (the tensor holds it)
+    if (sharded != nullptr && sharded != Py_None) return false;
+    if (copy != nullptr && copy != Py_None) {
+      const Tensor* c = leaf(copy, at::kBFloat16, to.device, n);
+      if (c == nullptr) return false;
+      item.out = c->data_ptr();
+      to.writes(item.out, n * 2);
+    }
+    to.writes(item.p, n * 4);
+    to.writes(item.mu, n * (to.small ? 1 : 4));
+    to.writes(item.nu, n * (to.small ? 1 : 4));
+    to.items.push_back(item);
+  }
+  return true;
+}
+
+// One AdamW step of all parameters of nested dicts of one structure (gradients, moments and, for
+// moments in 8 bits, their scales beside them); with max_norm >= 0 the gradients are clipped by their
+// global norm. False, before doing anything, for what is not covered.
+bool adamw_tree(py::handle params, py::handle grads, py::handle mu, py::handle nu, py::handle mu_most,
+                py::handle nu_most, double lr, double b1, double b2, double eps, double eps_root,
+                double weight_decay, int64_t step, int64_t seed, double max_norm) {
+  AdamwItems to;
+  to.device = c10::cuda::current_device();
+  to.small = !mu_most.is_none();
+  to.items.reserve(256);
+  to.written.reserve(1024);
+  if (!PyDict_CheckExact(params.ptr()) ||
+      !gather(params.ptr(), grads.ptr(), mu.ptr(), nu.ptr(), mu_most.ptr(), nu_most.ptr(), to) ||
+      to.overlap())
+    return false;
+  py::gil_scoped_release no_gil;
+  void* st = stream_of();
+  const int count = static_cast<int>(to.items.size());
+  const void* factor = nullptr;
+  Tensor scratch;
+  if (max_norm >= 0) {
+    const int64_t bytes = t5x_grad_clip_scratch_bytes(to.items.data(), count);
+    scratch = at::empty({bytes + 16},
+                        at::TensorOptions().dtype(at::kByte).device(at::Device(at::kCUDA, to.device)));
+    char* at = static_cast<char*>(scratch.data_ptr());
+    check(t5x_grad_clip_scale(to.items.data(), count, at + 16, static_cast<float>(max_norm), at, st),
+          "grad_clip_scale");
+    factor = at;
+  }
+  check(t5x_adamw_group(to.items.data(), count, to.small ? 8 : 32, lr, b1, b2, eps, eps_root, weight_decay,
+                        step, static_cast<unsigned>(seed), factor, st),
+        "adamw_group");
+  return true;
+}
+
 }  // namespace
 
 // The GIL is released for the duration of a call: a launch waits when the device's queue is full,
@@ -758,4 +889,5 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("relu_grads_ok", relu_grads_ok);
   m.def("relu_block", torch::wrap_pybind_function_no_gil(relu_block));
   m.def("relu_block_bwd", torch::wrap_pybind_function_no_gil(relu_block_bwd));
+  m.def("adamw_tree", adamw_tree);  // (it reads Python's dicts, and releases the GIL for the launches)
 }

@@ -65,6 +65,30 @@ int t5x_gemm_gated_grad(const void* dy, const void* B, void* h0, void* h1, int M
 int t5x_gated_gelu_bwd(void* dg, void* h, long long rows, int dff, long long ldh, long long ldg,
                        int write_g, void* stream);
 
+/* One parameter of t5x_adamw_group: n fp32 values p and gradients g, the moments mu and nu (fp32, or
+ * e4m3 codes with the largest magnitude of each 256 values in mu_absmax / nu_absmax), and the bf16
+ * working copy or null. No two items may share memory. */
+typedef struct {
+  void* p;
+  const void* g;
+  void* mu;
+  void* nu;
+  void* out;
+  void* mu_absmax;
+  void* nu_absmax;
+  long long n;
+} t5x_adamw_item;
+/* One AdamW step of all items. state_bits: 32 or 8 (seed: of the rounding). step >= 1 is the count after
+ * this update. clip_scale: device float that multiplies the gradients, or null. */
+int t5x_adamw_group(const t5x_adamw_item* items, int count, int state_bits, float lr, double b1, double b2,
+                    float eps, float eps_root, float weight_decay, int step, unsigned int seed,
+                    const void* clip_scale, void* stream);
+/* *clip_scale = min(1, max_norm / (norm + 1e-16)), norm over the items' gradients (the other pointers
+ * are not read). scratch: t5x_grad_clip_scratch_bytes bytes, 8-byte aligned. */
+long long t5x_grad_clip_scratch_bytes(const t5x_adamw_item* items, int count);
+int t5x_grad_clip_scale(const t5x_adamw_item* items, int count, void* scratch, float max_norm,
+                        void* clip_scale, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

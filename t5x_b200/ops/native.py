@@ -133,7 +133,8 @@ class _HostOps:
   NAMES = ("linear", "multi_linear", "multi_linear_bwd", "gated_in", "gated_in_bwd", "rmsnorm",
            "rmsnorm_bwd", "attention", "attention_bwd", "attention_block_ok", "attention_grads_ok",
            "attention_block", "attention_block_bwd", "mlp_block_ok", "mlp_grads_ok", "mlp_block",
-           "mlp_block_bwd", "relu_block_ok", "relu_grads_ok", "relu_block", "relu_block_bwd")
+           "mlp_block_bwd", "relu_block_ok", "relu_grads_ok", "relu_block", "relu_block_bwd",
+           "adamw_tree")
 
   def __init__(self, module):
     for name in self.NAMES:
@@ -1122,3 +1123,75 @@ def adamw_step_(p, g, mu, nu, bf16_out_ptrs, bf16_mc: int = 0, *, lr, b1, b2, ep
                               float(b1), float(b2), float(eps), float(eps_root),
                               float(weight_decay), int(step), ptr(clip_scale), stream_ptr()),
          "adamw_step")
+
+
+register_signature("t5x_grad_clip_scratch_bytes", [c_void_p, c_int])
+register_signature("t5x_grad_clip_scale", [c_void_p, c_int, c_void_p, c_float, c_void_p, c_void_p])
+register_signature("t5x_adamw_group", [c_void_p, c_int, c_int, c_float] + [ctypes.c_double] * 2 + [c_float] * 3 +
+                   [c_int, c_uint, c_void_p, c_void_p])
+
+MOMENT_BLOCK = 256  # values that share a scale in 8-bit moments
+
+
+class AdamwItems:
+  """The parameters of one `adamw_group_` call in the library's item layout. Keeps no reference to the
+  tensors: the caller holds them until the call has been issued."""
+  _ITEM = struct.Struct("=7Qq")
+
+  def __init__(self):
+    self._packed, self._written = [], []
+
+  def __len__(self):
+    return len(self._packed)
+
+  def add(self, p, g, mu, nu, out=None, mu_absmax=None, nu_absmax=None) -> None:
+    """p, g fp32; mu, nu fp32, or uint8 (e4m3 codes) with one fp32 scale per 256 values; out: the bf16
+    working copy or None. All contiguous on the current device."""
+    n, bits = p.numel(), 8 if mu.dtype == torch.uint8 else 32
+    moment = torch.uint8 if bits == 8 else torch.float32
+    wanted = [(p, torch.float32, n), (g, torch.float32, n), (mu, moment, n), (nu, moment, n)]
+    if out is not None:
+      wanted.append((out, torch.bfloat16, n))
+    if bits == 8:
+      wanted += [(t, torch.float32, -(-n // MOMENT_BLOCK)) for t in (mu_absmax, nu_absmax)]
+    for t, dtype, size in wanted:
+      if t is None or t.dtype != dtype or t.numel() != size or not t.is_contiguous() or t.device != p.device:
+        raise NativeError("adamw_group: operands must be contiguous tensors of one device whose types and sizes "
+                          "fit the parameter")
+    self._written += [(t.data_ptr(), t.data_ptr() + size * t.element_size())
+                      for i, (t, _, size) in enumerate(wanted) if i != 1 and size]  # (g is only read)
+    self._packed.append(self._ITEM.pack(ptr(p), ptr(g), ptr(mu), ptr(nu), ptr(out), ptr(mu_absmax),
+                                        ptr(nu_absmax), n))
+
+  def overlap(self) -> bool:
+    """Whether two of the tensors that a step writes share memory."""
+    spans = sorted(self._written)
+    return any(b[0] < a[1] for a, b in zip(spans, spans[1:]))
+
+  def buffer(self, which=None):
+    packed = self._packed if which is None else [self._packed[which]]
+    return ctypes.create_string_buffer(b"".join(packed), self._ITEM.size * max(1, len(packed)))
+
+
+def grad_clip_scale(items: AdamwItems, max_norm: float, device) -> torch.Tensor:
+  """min(1, max_norm / (global norm of the items' gradients + 1e-16)) as a device scalar [1]."""
+  buf = items.buffer()
+  lib().t5x_grad_clip_scratch_bytes.restype = c_ll
+  nbytes = lib().t5x_grad_clip_scratch_bytes(ctypes.addressof(buf), len(items))
+  scratch = torch.empty(nbytes, dtype=torch.uint8, device=device)
+  out = torch.empty(1, dtype=torch.float32, device=device)
+  _check(lib().t5x_grad_clip_scale(ctypes.addressof(buf), len(items), scratch.data_ptr(), max_norm,
+                                   out.data_ptr(), stream_ptr()), "grad_clip_scale")
+  return out
+
+
+def adamw_group_(items: AdamwItems, state_bits: int, *, lr, b1, b2, eps, eps_root, weight_decay, step: int,
+                 seed: int = 0, clip_scale: Optional[torch.Tensor] = None) -> None:
+  """One AdamW step of every item in one launch (csrc/adamw_group.cu); items that share memory are updated
+  in turn. `step` is the count after the update, `seed` that of the rounding of 8-bit moments."""
+  parts = [(i, 1) for i in range(len(items))] if items.overlap() else [(None, len(items))]
+  for which, count in parts:
+    buf = items.buffer(which)
+    _check(lib().t5x_adamw_group(ctypes.addressof(buf), count, state_bits, lr, b1, b2, eps, eps_root,
+                                 weight_decay, step, seed & 0xFFFFFFFF, ptr(clip_scale), stream_ptr()),
+           "adamw_group")

@@ -16,6 +16,7 @@ scale = _o.scale
 scale_by_learning_rate = _o.scale_by_learning_rate
 trace = _o.trace
 scale_by_adam = _o.scale_by_adam
+scale_by_adam8 = _o.scale_by_adam8  # (moments in 8 bits: no counterpart in optax)
 scale_by_belief = _o.scale_by_belief
 scale_by_yogi = _o.scale_by_yogi
 scale_by_radam = _o.scale_by_radam
@@ -35,6 +36,7 @@ def chain(*transforms):
 sgd = _o._sgd
 adam = _o._adam
 adamw = _o._adamw
+adamw8 = _o._adamw8
 lion = _o._lion
 lamb = _o._lamb
 lars = _o._lars

@@ -231,6 +231,95 @@ def scale_by_adam(b1=0.9, b2=0.999, eps=1e-8, eps_root=0.0) -> GradientTransform
                                 {"b1": b1, "b2": b2, "eps": eps, "eps_root": eps_root})
 
 
+# ---- Adam's moments in 8 bits ----
+MOMENT_BLOCK = 256  # consecutive values of a tensor that share a scale
+_E4M3_MAX = 448.0
+_NOISE = (0x9E3779B1, 0x6A09E667, 0xBB67AE85)  # leading bits of the golden ratio, sqrt 2, sqrt 3
+
+
+def _moment_blocks(n: int) -> int:
+  return -(-n // MOMENT_BLOCK)
+
+
+def _moment_noise(n: int, seed: int, step: int, device) -> torch.Tensor:
+  """32 bits for each of a tensor's n values, a function of seed, step and place alone."""
+  low = 0xFFFFFFFF
+  h = torch.arange(n, device=device) + ((seed * _NOISE[0] + step * _NOISE[2]) & low)
+  for factor, shift in zip(_NOISE, (15, 13, 16)):
+    h = (h * factor) & low
+    h = h ^ (h >> shift)
+  return h
+
+
+def _blocks_of(x: torch.Tensor) -> torch.Tensor:
+  """[blocks, 256], the last one filled up with zeros."""
+  flat = x.reshape(-1)
+  return torch.nn.functional.pad(flat, (0, -flat.numel() % MOMENT_BLOCK)).view(-1, MOMENT_BLOCK)
+
+
+def dequantize_moment(codes: torch.Tensor, absmax: torch.Tensor) -> torch.Tensor:
+  """The fp32 values that 8-bit moments stand for: e4m3 code / 448 * largest of the block."""
+  values = _blocks_of(codes).view(torch.float8_e4m3fn).float() * (1.0 / _E4M3_MAX) * absmax[:, None]
+  return values.reshape(-1)[:codes.numel()].view(codes.shape)
+
+
+def quantize_moment(x: torch.Tensor, noise: torch.Tensor, second: bool):
+  """(codes, absmax) of a moment. A value is rounded to one of the e4m3 numbers on either side of
+  x / absmax * 448, up with the probability (distance to the lower) / (distance of the two), so that
+  it keeps its mean: rounded to the nearest, a second moment that moves by a thousandth of itself per
+  step would never move. `noise`: 16 bits a value. A second moment (`second`) above zero is stored as
+  the smallest number at least: as zero it would leave the step to be divided by eps."""
+  rows = _blocks_of(x.float())
+  absmax = rows.abs().amax(dim=1) if rows.numel() else rows.new_zeros(rows.shape[0])
+  inverse = torch.where(absmax > 0, 1.0 / absmax, torch.zeros_like(absmax))
+  y = rows.abs() * inverse[:, None] * _E4M3_MAX
+  gap = torch.ldexp(torch.ones_like(y), (torch.frexp(y)[1] - 1).clamp(min=-6) - 3)
+  up = (_blocks_of(noise).to(y.dtype) + 0.5) / 65536.0
+  y = (torch.floor(y / gap + up) * gap).clamp(max=_E4M3_MAX)
+  if second:
+    y = torch.where((rows > 0) & (y == 0), torch.full_like(y, 2.0 ** -9), y)
+  codes = torch.copysign(y, rows).to(torch.float8_e4m3fn).view(torch.uint8)
+  return codes.reshape(-1)[:x.numel()].view(x.shape).contiguous(), absmax
+
+
+def scale_by_adam8(b1=0.9, b2=0.999, eps=1e-8, eps_root=0.0, seed=0) -> GradientTransformation:
+  """`scale_by_adam` with both moments in 8 bits: e4m3 codes (uint8, of the parameter's shape) under
+  'mu' and 'nu', and the largest magnitude of every 256 consecutive values in fp32 under 'mu_absmax'
+  and 'nu_absmax'. The update is taken from the moments in 32 bits, before they are rounded (see
+  `quantize_moment`; `seed` is that of the rounding). Needs whole parameters: not under a model or
+  expert axis, nor with the optimizer sharded over replicas."""
+  def init(params):
+    from t5x_b200.parallel import state as pstate
+    st = pstate.get()
+    if st.model_size > 1 or st.expert_size > 1:
+      raise ValueError("Adam moments in 8 bits need whole parameters: they are not available under a model or "
+                       "expert axis.")
+    codes = lambda: {k: torch.zeros(v.shape, dtype=torch.uint8, device=v.device)  # noqa: E731
+                     for k, v in params.items()}
+    scales = lambda: {k: torch.zeros(_moment_blocks(v.numel()), device=v.device)  # noqa: E731
+                      for k, v in params.items()}
+    return {"count": torch.zeros((), dtype=torch.int32), "mu": codes(), "nu": codes(),
+            "mu_absmax": scales(), "nu_absmax": scales()}
+
+  def update(updates, state, params=None):
+    count = state["count"] + 1
+    c = int(count)
+    new = {"count": count, "mu": {}, "nu": {}, "mu_absmax": {}, "nu_absmax": {}}
+    bc1, bc2 = 1 - b1 ** c, 1 - b2 ** c
+    out = {}
+    for k, g in updates.items():
+      mu = b1 * dequantize_moment(state["mu"][k], state["mu_absmax"][k]) + (1 - b1) * g
+      nu = b2 * dequantize_moment(state["nu"][k], state["nu_absmax"][k]) + (1 - b2) * g * g
+      out[k] = (mu / bc1) / (torch.sqrt(nu / bc2 + eps_root) + eps)
+      noise = _moment_noise(g.numel(), seed, c, g.device)
+      new["mu"][k], new["mu_absmax"][k] = quantize_moment(mu, noise & 0xFFFF, False)
+      new["nu"][k], new["nu_absmax"][k] = quantize_moment(nu, noise >> 16, True)
+    return out, new
+
+  return GradientTransformation(init, update, "scale_by_adam8",
+                                {"b1": b1, "b2": b2, "eps": eps, "eps_root": eps_root, "seed": seed})
+
+
 def scale_by_belief(b1=0.9, b2=0.999, eps=1e-16, eps_root=1e-16) -> GradientTransformation:
   def init(params):
     return {"count": torch.zeros((), dtype=torch.int32), "mu": _zeros_like_tree(params),
@@ -413,6 +502,14 @@ def _adamw(learning_rate, b1=0.9, b2=0.999, eps=1e-8, eps_root=0.0, weight_decay
                           scale_by_learning_rate(learning_rate))
 
 
+def _adamw8(learning_rate, b1=0.9, b2=0.999, eps=1e-8, eps_root=0.0, weight_decay=1e-4,
+            mask=None, seed=0):
+  """AdamW with both moments in 8 bits (`scale_by_adam8`): 2 bytes of state a parameter instead of 8."""
+  return chain_transforms(scale_by_adam8(b1, b2, eps, eps_root, seed),
+                          add_decayed_weights(weight_decay, mask),
+                          scale_by_learning_rate(learning_rate))
+
+
 def _lion(learning_rate, b1=0.9, b2=0.99, weight_decay=1e-3, mask=None):
   return chain_transforms(scale_by_lion(b1, b2), add_decayed_weights(weight_decay, mask),
                           scale_by_learning_rate(learning_rate))
@@ -478,7 +575,10 @@ class OptaxWrapper(OptimizerDef):
 
   def __init__(self, optax_optimizer: GradientTransformation):
     self.optax_optimizer = optax_optimizer
+    # fused_plan: the chain with moments in 32 bits (also inside the sharded exchange);
+    # fused_plan8: with moments in 8 bits, on whole parameters only
     self.fused_plan = _fused_adamw_plan(optax_optimizer)
+    self.fused_plan8 = _fused_adamw_plan(optax_optimizer, "scale_by_adam8")
     super().__init__(hyper_params=None)
 
   def init_state(self, params):
@@ -518,9 +618,15 @@ class OptaxWrapper(OptimizerDef):
     return {"learning_rate": hyper_param_overrides.get("learning_rate")}
 
   def apply_gradient(self, hyper_params, params, state, grads):
+    plan = self.fused_plan or self.fused_plan8
+    if plan is not None:
+      stepped = self._apply_group(plan, hyper_params, params, state, grads)
+      if stepped is not None:
+        return params, OptimizerState(step=state.step + 1, param_states=stepped)
     flat_p = tree_utils.flatten_dict(params)
-    if self.fused_plan is not None and _fused_adamw_usable(flat_p, grads):
-      return self._apply_fused_adamw(hyper_params, params, state, grads)
+    if plan is not None and _fused_adamw_usable(flat_p, grads) and (
+        plan is self.fused_plan or _whole_on_one_device(flat_p)):
+      return self._apply_fused_adamw(plan, hyper_params, params, state, grads)
     flat_g = {k: v.float() for k, v in tree_utils.flatten_dict(grads).items()}
     opt_state = self._flat(state.param_states, flat_p.keys())
     _STEP_LEARNING_RATE[0] = (hyper_params or {}).get("learning_rate")
@@ -537,16 +643,63 @@ class OptaxWrapper(OptimizerDef):
           bf.copy_(p)
     return params, OptimizerState(step=state.step + 1, param_states=self._nest(new_opt_state))
 
-  def _apply_fused_adamw(self, hyper_params, params, state, grads):
+  def _apply_group(self, plan, hyper_params, params, state, grads):
+    """The step of all parameters in one launch, from the trees as they are, through the compiled host
+    path (`adamw_tree` in csrc/host/host_ops.cpp: the walk over a few hundred tensors in Python takes
+    longer than the kernel). Returns the new states: the same moments, updated in place, beside new
+    counts. None, before doing anything, where that does not cover the call:
+    parameters sharded over replicas, tensors of other types, layouts or devices, tensors that share
+    memory, and, with moments in 32 bits, a clip by the global norm, whose factor the general path
+    takes."""
+    small = plan["bits"] == 8
+    if plan["max_norm"] is not None and not small:
+      return None
+    if type(params) is not dict or not torch.cuda.is_initialized():
+      return None
+    from t5x_b200.ops import native
+    host = native.host()
+    if host is None:
+      return None
+    stepped = dict(state.param_states)
+
+    def at(path):  # dicts of this call's own down to the node
+      node = stepped
+      for i in path:
+        below = dict(node[str(i)])
+        node[str(i)] = below
+        node = below
+      return node
+
+    adam, lr_state = at(plan["adam_path"]), at(plan["lr_path"])
+    lr, count = self._step_lr(plan, hyper_params, lr_state), int(adam["count"])
+    if not host.adamw_tree(params, grads, adam["mu"], adam["nu"], adam["mu_absmax"] if small else None,
+                           adam["nu_absmax"] if small else None, lr, plan["b1"], plan["b2"], plan["eps"],
+                           plan["eps_root"], plan["weight_decay"], count + 1, plan["seed"],
+                           -1.0 if plan["max_norm"] is None else float(plan["max_norm"])):
+      return None
+    adam["count"] = adam["count"] + 1
+    lr_state["count"] = lr_state["count"] + 1
+    return stepped
+
+  @staticmethod
+  def _step_lr(plan, hyper_params, lr_state) -> float:
+    _STEP_LEARNING_RATE[0] = (hyper_params or {}).get("learning_rate")
+    try:
+      return float(_lr(plan["learning_rate"], int(lr_state["count"])))
+    finally:
+      _STEP_LEARNING_RATE[0] = None
+
+  def _apply_fused_adamw(self, plan, hyper_params, params, state, grads):
     """[clip_by_global_norm ->] scale_by_adam [-> add_decayed_weights] -> scale_by_learning_rate
-    as one native kernel per parameter (csrc/adamw.cu), with the same state layout as the
-    generic path. With the optimizer sharded over the data axis (`parallel/zero.py`) the owner
+    as native kernels, with the same state layout as the generic path: one launch for all
+    parameters that live whole on this GPU (csrc/adamw_group.cu), one per parameter that is sharded
+    (csrc/adamw.cu). With the optimizer sharded over the data axis (`parallel/zero.py`) the owner
     of a parameter first sums the replicas' gradients over NVLink, the clip factor is taken
     from the norm of the summed gradients of all owners, and the update kernel stores the new
-    bf16 weights into every replica's working copy."""
+    bf16 weights into every replica's working copy. Moments in 8 bits (`scale_by_adam8`) are
+    covered on whole parameters."""
     from t5x_b200.ops import comm, native
     from t5x_b200.parallel import state as pstate
-    plan = self.fused_plan
     flat_p = tree_utils.flatten_dict(params)
     flat_g = tree_utils.flatten_dict(grads)
     opt_state = self._flat(state.param_states, flat_p.keys())
@@ -557,13 +710,12 @@ class OptaxWrapper(OptimizerDef):
       return node
 
     adam_state, lr_state = at(plan["adam_path"]), at(plan["lr_path"])
-    _STEP_LEARNING_RATE[0] = (hyper_params or {}).get("learning_rate")
-    try:
-      lr = float(_lr(plan["learning_rate"], int(lr_state["count"])))
-    finally:
-      _STEP_LEARNING_RATE[0] = None
+    lr = self._step_lr(plan, hyper_params, lr_state)
     step = int(adam_state["count"]) + 1
     st = pstate.get()
+    hyper = dict(lr=lr, b1=plan["b1"], b2=plan["b2"], eps=plan["eps"], eps_root=plan["eps_root"],
+                 weight_decay=plan["weight_decay"], step=step)
+    small = plan["bits"] == 8
     with torch.no_grad():
       mine, replicated = [], []
       for k, p in flat_p.items():
@@ -574,7 +726,7 @@ class OptaxWrapper(OptimizerDef):
           comm.peer_reduce_f32_(flat_g[k], z.grad_ptrs(), z.numel)
           mine.append(k)
       clip_scale = None
-      if plan["max_norm"] is not None:
+      if plan["max_norm"] is not None and not small:
         def sumsq(keys):
           if not keys:
             return torch.zeros((), dtype=torch.float32, device=st.device)
@@ -587,20 +739,24 @@ class OptaxWrapper(OptimizerDef):
         total = total + sumsq(replicated)
         gnorm = torch.sqrt(total)
         clip_scale = torch.clamp(plan["max_norm"] / (gnorm + 1e-16), max=1.0).float().reshape(1)
-      for k in mine + replicated:
-        p, g = flat_p[k], flat_g[k]
-        z = getattr(p, "zero", None)
-        bf = getattr(p, "bf16", None)
-        if z is not None:
-          outs, mc = z.bf16_ptrs(), z.bf16_mc()
-        elif bf is not None:
-          outs, mc = comm._ptr_array([bf.data_ptr()]), 0
-        else:
-          outs, mc = comm._ptr_array([]), 0
-        native.adamw_step_(p, g, adam_state["mu"][k], adam_state["nu"][k], outs, mc, lr=lr,
-                           b1=plan["b1"], b2=plan["b2"], eps=plan["eps"],
-                           eps_root=plan["eps_root"], weight_decay=plan["weight_decay"],
-                           step=step, clip_scale=clip_scale)
+      for k in mine:
+        z = flat_p[k].zero
+        native.adamw_step_(flat_p[k], flat_g[k], adam_state["mu"][k], adam_state["nu"][k], z.bf16_ptrs(),
+                           z.bf16_mc(), clip_scale=clip_scale, **hyper)
+      devices = {}  # (parameters on several devices are stepped device by device)
+      for k in replicated:
+        devices.setdefault(flat_p[k].device, []).append(k)
+      for device, keys in devices.items():
+        with torch.cuda.device(device):
+          items = native.AdamwItems()
+          for k in keys:
+            scales = [adam_state[n][k] for n in ("mu_absmax", "nu_absmax")] if small else []
+            items.add(flat_p[k], flat_g[k], adam_state["mu"][k], adam_state["nu"][k],
+                      getattr(flat_p[k], "bf16", None), *scales)
+          if small and plan["max_norm"] is not None:
+            clip_scale = native.grad_clip_scale(items, plan["max_norm"], device)
+          factor = clip_scale if clip_scale is None else clip_scale.to(device)
+          native.adamw_group_(items, plan["bits"], seed=plan["seed"], clip_scale=factor, **hyper)
     adam_state["count"] = adam_state["count"] + 1
     lr_state["count"] = lr_state["count"] + 1
     return params, OptimizerState(step=state.step + 1, param_states=self._nest(opt_state))
@@ -610,22 +766,24 @@ class OptaxWrapper(OptimizerDef):
     flat_axes = tree_utils.flatten_dict(param_logical_axes, is_leaf=lambda x: not isinstance(x, dict))
     keyset = set(flat_axes.keys())
 
-    def conv(node):
+    def conv(node, name=""):
       if isinstance(node, dict):
         fl = tree_utils.flatten_dict(node)
         if fl and set(fl.keys()) == keyset:
+          if name.endswith("_absmax"):  # one value per 256 of the parameter: whole everywhere
+            return tree_utils.unflatten_dict({k: (None,) for k in fl})
           return tree_utils.unflatten_dict({k: flat_axes[k] for k in fl})
-        return {k: conv(v) for k, v in node.items()}
+        return {k: conv(v, k) for k, v in node.items()}
       return None
 
     state_axes = OptimizerState(step=None, param_states=conv(optimizer.state.param_states))
     return Optimizer(optimizer.optimizer_def, state_axes, param_logical_axes)
 
 
-def _fused_adamw_plan(t: GradientTransformation):
-  """The hyper-parameters of an Adam / AdamW chain that the native kernel covers, or None:
-  [clip_by_global_norm,] scale_by_adam, [add_decayed_weights without a mask,]
-  scale_by_learning_rate (descending), possibly nested one level (`chain([clip, adamw(...)])`)."""
+def _fused_adamw_plan(t: GradientTransformation, adam_name: str = "scale_by_adam"):
+  """The hyper-parameters of an Adam / AdamW chain that the native kernels cover, or None:
+  [clip_by_global_norm,] scale_by_adam (or, by name, scale_by_adam8), [add_decayed_weights without a
+  mask,] scale_by_learning_rate (descending), possibly nested one level (`chain([clip, adamw(...)])`)."""
   def flatten(x):
     if x.name == "chain":
       out = []
@@ -647,8 +805,8 @@ def _fused_adamw_plan(t: GradientTransformation):
   parts, paths = flatten(t), index_paths(t)
   names = [x.name for x in parts]
   want = [n for n in names if n != "clip_by_global_norm"]
-  if want not in (["scale_by_adam", "scale_by_schedule"],
-                  ["scale_by_adam", "add_decayed_weights", "scale_by_schedule"]):
+  if want not in ([adam_name, "scale_by_schedule"],
+                  [adam_name, "add_decayed_weights", "scale_by_schedule"]):
     return None
   if names.count("clip_by_global_norm") > 1 or \
       ("clip_by_global_norm" in names and names[0] != "clip_by_global_norm"):
@@ -659,8 +817,9 @@ def _fused_adamw_plan(t: GradientTransformation):
     return None
   if not by["scale_by_schedule"].hparams.get("flip_sign", True):
     return None
-  adam = by["scale_by_adam"].hparams
-  return {"adam_path": paths[names.index("scale_by_adam")],
+  adam = by[adam_name].hparams
+  return {"adam_path": paths[names.index(adam_name)], "bits": 8 if adam_name == "scale_by_adam8" else 32,
+          "seed": adam.get("seed", 0),
           "lr_path": paths[names.index("scale_by_schedule")],
           "learning_rate": by["scale_by_schedule"].hparams["learning_rate"],
           "b1": adam["b1"], "b2": adam["b2"], "eps": adam["eps"], "eps_root": adam["eps_root"],
@@ -683,6 +842,11 @@ def _fused_adamw_usable(flat_p, grads) -> bool:
   return True
 
 
+def _whole_on_one_device(flat_p) -> bool:
+  return all(getattr(p, "zero", None) is None for p in flat_p.values()) and \
+      len({p.device for p in flat_p.values()}) <= 1
+
+
 def wrap_optax_optimizer(optax_optimizer_fn):
   """Makes `fn(*args) -> OptaxWrapper(fn(*args))` (t5x/optimizers.py:529-546)."""
   def wrapped(*args, **kwargs) -> OptimizerDef:
@@ -699,6 +863,7 @@ adabelief = wrap_optax_optimizer(_adabelief)
 adagrad = wrap_optax_optimizer(_adagrad)
 adam = wrap_optax_optimizer(_adam)
 adamw = wrap_optax_optimizer(_adamw)
+adamw8 = wrap_optax_optimizer(_adamw8)
 fromage = wrap_optax_optimizer(_fromage)
 lamb = wrap_optax_optimizer(_lamb)
 lars = wrap_optax_optimizer(_lars)
