@@ -11,8 +11,8 @@
 // model of 190 tensors spent 190 launches on it, most of them with less work than a launch costs.
 //
 // The items travel in the kernel's parameters (no table in device memory that a captured graph would
-// have to keep alive). Each CTA takes one chunk of kChunk elements of one item; it finds the item by
-// a binary search over the items' first chunks.
+// have to keep alive). Each CTA takes one chunk of one item, which it finds by a binary search over the
+// items' first chunks between two of 256 hints (over all of 300 items the search took 5 % of the time).
 //
 // Moments in 8 bits: blocks of 256 consecutive values of a tensor share a scale, the largest
 // magnitude of the block, held in 32 bits; a value is stored as the e4m3 number next to
@@ -35,11 +35,15 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kChunk = 2048;      // elements per CTA
 constexpr int kQuantBlock = 256;  // values that share a scale
-constexpr int kMaxItems = 448;    // (28 KB of the 32 KB that a launch's parameters may have)
+constexpr int kSpan = 4;          // chunks that a CTA of the norm takes in a row
+constexpr int kMaxItems = 448;    // (31 KB of the 32 KB that a launch's parameters may have)
+constexpr int kHints = 256;
 constexpr int kFewItems = 48;
 
 struct Hyper {
   float lr, b1, b2, c1, c2, eps, eps_root, weight_decay, bc1, bc2;  // c = 1 - b
+  // for moments in 8 bits: b / 448, 1 / bc2, -lr / bc1, -lr * weight_decay
+  float b1_448, b2_448, ibc2, lr_bc1, lr_decay;
   uint32_t noise_key;
 };
 
@@ -47,14 +51,18 @@ template <int kItems>
 struct Group {
   Hyper h;
   const float* clip_scale;
-  int count;
-  unsigned first[kItems];  // first chunk of each item
+  int count, shift;
+  unsigned ahead;                   // chunks from a CTA's own to the one that it has fetched into L2
+  unsigned first[kItems];           // first chunk of each item
+  bool wide[kItems];                // every pointer of the item takes the wide accesses
+  unsigned short near[kHints + 1];  // item of chunk (i << shift); behind the last chunk the last item
   t5x_adamw_item item[kItems];
 };
 
 template <int kItems>
 __device__ __forceinline__ int find_item(const Group<kItems>& grp, unsigned chunk) {
-  int lo = 0, hi = grp.count;  // first[lo] <= chunk < first[hi]
+  const unsigned hint = chunk >> grp.shift;
+  int lo = grp.near[hint], hi = grp.near[hint + 1] + 1;  // first[lo] <= chunk < first[hi]
   while (hi - lo > 1) {
     const int mid = (lo + hi) >> 1;
     if (grp.first[mid] <= chunk)
@@ -65,8 +73,7 @@ __device__ __forceinline__ int find_item(const Group<kItems>& grp, unsigned chun
   return lo;
 }
 
-// Every pointer of the item takes the wide accesses.
-__device__ __forceinline__ bool wide(const t5x_adamw_item& it) {
+bool takes_wide(const t5x_adamw_item& it) {
   return ((reinterpret_cast<uintptr_t>(it.p) | reinterpret_cast<uintptr_t>(it.g) |
            reinterpret_cast<uintptr_t>(it.mu) | reinterpret_cast<uintptr_t>(it.nu)) & 15) == 0 &&
          (reinterpret_cast<uintptr_t>(it.out) & 7) == 0;
@@ -102,7 +109,7 @@ __global__ void __launch_bounds__(kThreads)
   float* mu = static_cast<float*>(it.mu) + begin;
   float* nu = static_cast<float*>(it.nu) + begin;
   __nv_bfloat16* out = it.out != nullptr ? static_cast<__nv_bfloat16*>(it.out) + begin : nullptr;
-  if (n == kChunk && wide(it)) {
+  if (n == kChunk && grp.wide[which]) {
     constexpr int kVec = kChunk / (4 * kThreads);
     float4 gv[kVec], pv[kVec], mv[kVec], nv[kVec];
 #pragma unroll
@@ -139,26 +146,83 @@ __global__ void __launch_bounds__(kThreads)
 
 // ---- moments in 8 bits ----
 
-// 32 bits for the value at `place` of a tensor: 16 for each moment. The factors are the leading
-// bits of the golden ratio and of the square roots of 2 and 3 (all odd).
-__device__ __forceinline__ uint32_t noise(uint32_t place, uint32_t key) {
-  uint32_t h = (place + key) * 0x9E3779B1u;
+// 32 random bits for the value at a place of its tensor, 16 for each moment: a hash of (place + key),
+// with the key from seed and step, begun with the product (place + key) * kNoise1. The factors are the
+// leading bits of the golden ratio and of the square roots of 2 and 3 (all odd).
+constexpr uint32_t kNoise1 = 0x9E3779B1u;
+struct Noise {
+  uint32_t mu, nu;  // the 16 bits at bits 4 to 19
+};
+__device__ __forceinline__ Noise noise(uint32_t h) {
   h ^= h >> 15;
   h *= 0x6A09E667u;
   h ^= h >> 13;
   h *= 0xBB67AE85u;
-  return h ^ (h >> 16);
+  // the halves of h ^ (h >> 16)
+  const uint32_t high = h >> 12;
+  return {((h << 4) ^ high) & 0xffff0u, high & 0xffff0u};
 }
 
-// The e4m3 code of y in [0, 448], rounded to a neighbour by the 16 random bits r: e4m3 keeps three
-// of the 23 bits of the mantissa, so the bits that fall away are topped up by a random number below
-// one step before they are cut off. Below 2^-6 the steps are 2^-9 wide; adding 2^-6 puts y among
-// numbers whose steps are the same.
-__device__ __forceinline__ uint32_t to_e4m3(float y, uint32_t r) {
-  const bool low = y < 0.015625f;
-  const uint32_t bits = __float_as_uint(low ? y + 0.015625f : y) + (r << 4) + 8u;
-  const int code = static_cast<int>(bits >> 20) - (low ? 968 : 960);
-  return static_cast<uint32_t>(code < 126 ? code : 126);
+// ---- pairs of values: sm_100 does two 32-bit products or sums in one instruction ----
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  uint64_t d;
+  asm("fma.rn.ftz.f32x2 %0, %1, %2, %3;"
+      : "=l"(d)
+      : "l"(*reinterpret_cast<uint64_t*>(&a)), "l"(*reinterpret_cast<uint64_t*>(&b)),
+        "l"(*reinterpret_cast<uint64_t*>(&c)));
+  return *reinterpret_cast<float2*>(&d);
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  uint64_t d;
+  asm("mul.rn.ftz.f32x2 %0, %1, %2;"
+      : "=l"(d)
+      : "l"(*reinterpret_cast<uint64_t*>(&a)), "l"(*reinterpret_cast<uint64_t*>(&b)));
+  return *reinterpret_cast<float2*>(&d);
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  uint64_t d;
+  asm("add.rn.ftz.f32x2 %0, %1, %2;"
+      : "=l"(d)
+      : "l"(*reinterpret_cast<uint64_t*>(&a)), "l"(*reinterpret_cast<uint64_t*>(&b)));
+  return *reinterpret_cast<float2*>(&d);
+}
+__device__ __forceinline__ float2 both(float x) { return make_float2(x, x); }
+
+// What a step multiplies by, the same for a whole block of values.
+struct Factors {
+  float2 clip, c1, c2, mu, nu;              // mu, nu: b / 448 * largest of the old moments
+  float2 ibc2, eps_root, eps, lr, lr_decay;  // lr: -lr / bc1; lr_decay: -lr * weight_decay
+};
+__device__ __forceinline__ Factors factors(const Hyper& h, float clip, float mu_most, float nu_most) {
+  Factors f;
+  f.clip = both(clip);
+  f.c1 = both(h.c1);
+  f.c2 = both(h.c2);
+  f.mu = both(h.b1_448 * mu_most);
+  f.nu = both(h.b2_448 * nu_most);
+  f.ibc2 = both(h.ibc2);
+  f.eps_root = both(h.eps_root);
+  f.eps = both(h.eps);
+  f.lr = both(h.lr_bc1);
+  f.lr_decay = both(h.lr_decay);
+  return f;
+}
+
+__device__ __forceinline__ float reciprocal(float x) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+
+// The step of two values; m and v: e4m3 values of the old moments, then the new moments in 32 bits.
+__device__ __forceinline__ void update2(const Factors& f, float2 g, float2& p, float2& m, float2& v) {
+  g = mul2(g, f.clip);
+  m = fma2(m, f.mu, mul2(g, f.c1));
+  v = fma2(mul2(g, f.c2), g, mul2(v, f.nu));
+  float2 d = fma2(v, f.ibc2, f.eps_root);
+  d = add2(make_float2(sqrtf(d.x), sqrtf(d.y)), f.eps);
+  const float2 r = make_float2(reciprocal(d.x), reciprocal(d.y));
+  p = add2(p, fma2(mul2(m, r), f.lr, mul2(p, f.lr_decay)));
 }
 
 __device__ __forceinline__ float2 from_e4m3x2(uint32_t two) {
@@ -169,33 +233,111 @@ __device__ __forceinline__ float2 from_e4m3x2(uint32_t two) {
 
 __device__ __forceinline__ uint32_t abs_bits(float x) { return __float_as_uint(x) & 0x7fffffffu; }
 
-// 1 / largest; 0 where all are zero. (A largest that is not finite makes the whole block NaN when it
-// is read back, as the largest itself is kept.)
-__device__ __forceinline__ float inverse(float most) { return most > 0.f ? 1.f / most : 0.f; }
+// 1.75 / largest: times 256 = 448 / largest, which would overflow where the largest is tiny; 0 where
+// all are zero. (A largest that is not finite makes the whole block NaN when it is read back, as the
+// largest itself is kept.)
+__device__ __forceinline__ float inverse(float most) { return most > 0.f ? 1.75f / most : 0.f; }
 
-__device__ __forceinline__ uint32_t code_mu(float m, float inv, uint32_t r) {
-  return to_e4m3(fabsf(m) * inv * 448.f, r & 0xffffu) | ((__float_as_uint(m) >> 24) & 0x80u);
-}
-__device__ __forceinline__ uint32_t code_nu(float v, float inv, uint32_t r) {
-  const uint32_t c = to_e4m3(v * inv * 448.f, r >> 16);
-  return c == 0u && v > 0.f ? 1u : c;
+// The two e4m3 codes of x / largest * 448, each rounded to a neighbour by 16 random bits (at bits 4 to 19
+// of `noise`): e4m3 keeps three of the 23 bits of the mantissa, so the bits that fall away are topped
+// up by a random number below one step before they are cut off. Below 2^-6 the steps are 2^-9 wide;
+// with 2^-6 added the value lies among numbers whose steps are the same, and what is left when it is
+// taken off again is exact. kSecond: no sign, and nothing is stored as zero (the caller sees to zeros).
+template <bool kSecond>
+__device__ __forceinline__ uint32_t codes2(float2 x, float inv, uint32_t noise0, uint32_t noise1) {
+  const float2 y = mul2(x, both(inv));
+  auto shift = [](float v) {
+    const float by = kSecond ? 0.015625f
+                             : __uint_as_float((__float_as_uint(v) & 0x80000000u) | 0x3c800000u);
+    return fabsf(v) < 0.00006103515625f ? by : 0.f;  // (2^-14: y is x / largest * 1.75)
+  };
+  const float2 c = make_float2(shift(y.x), shift(y.y));
+  float2 z = fma2(y, both(256.f), c);
+  z.x = __uint_as_float((__float_as_uint(z.x) + noise0 + 8u) & 0xfff00000u);
+  z.y = __uint_as_float((__float_as_uint(z.y) + noise1 + 8u) & 0xfff00000u);
+  z = fma2(c, both(-1.f), z);
+  if (kSecond) {
+    z.x = fmaxf(z.x, 0.001953125f);
+    z.y = fmaxf(z.y, 0.001953125f);
+  }
+  return __nv_cvt_float2_to_fp8x2(z, __NV_SATFINITE, __NV_E4M3);
 }
 
-// A warp per block of 256 values: lane l holds values 4l .. 4l + 3 and 128 + 4l .. 128 + 4l + 3, so
-// that every access of the warp is contiguous.
+// (16-byte aligned address, size a multiple of 16 bytes)
+__device__ __forceinline__ void prefetch_l2(const void* p, uint32_t bytes) {
+  asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(p), "r"(bytes) : "memory");
+}
+
+// What a lane reads of a block: values 4l .. 4l + 3 and 128 + 4l .. 128 + 4l + 3, so that every access of
+// the warp is contiguous.
+struct Block8 {
+  float4 g[2], p[2];
+  uint32_t mu[2], nu[2];
+  float mu_most, nu_most;
+};
+
+// The step of one block by a warp, from the block's values to its new ones in their places.
+struct Result8 {
+  float2 p[4];  // pair j: values (j / 2) * 128 + 4 * lane + 2 * (j % 2) and the next
+  uint32_t mu[4], nu[4];
+  uint32_t mu_most, nu_most;
+};
+__device__ __forceinline__ Result8 step8(const Hyper& h, float clip, const Block8& in, uint32_t key, int lane) {
+  const Factors f = factors(h, clip, in.mu_most, in.nu_most);
+  Result8 r;
+  float2 m[4], v[4];
+  r.mu_most = r.nu_most = 0;
+  float nu_least = 1.f;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const int k = j >> 1, s = (j & 1) * 16;
+    const float2 g = j & 1 ? make_float2(in.g[k].z, in.g[k].w) : make_float2(in.g[k].x, in.g[k].y);
+    r.p[j] = j & 1 ? make_float2(in.p[k].z, in.p[k].w) : make_float2(in.p[k].x, in.p[k].y);
+    m[j] = from_e4m3x2(in.mu[k] >> s);
+    v[j] = from_e4m3x2(in.nu[k] >> s);
+    update2(f, g, r.p[j], m[j], v[j]);
+    // as integers NaN is above every number, so that a NaN stays the largest
+    r.mu_most = max(r.mu_most, max(abs_bits(m[j].x), abs_bits(m[j].y)));
+    r.nu_most = max(r.nu_most, max(__float_as_uint(v[j].x), __float_as_uint(v[j].y)));
+    nu_least = fminf(nu_least, fminf(v[j].x, v[j].y));
+  }
+  r.mu_most = __reduce_max_sync(0xffffffffu, r.mu_most);
+  r.nu_most = __reduce_max_sync(0xffffffffu, r.nu_most);
+  const float mi = inverse(__uint_as_float(r.mu_most)), ni = inverse(__uint_as_float(r.nu_most));
+  const uint32_t seed = (key + lane * 4) * kNoise1;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const uint32_t i = (j >> 1) * 128 + (j & 1) * 2;
+    const Noise a = noise(seed + i * kNoise1), b = noise(seed + (i + 1) * kNoise1);
+    r.mu[j] = codes2<false>(m[j], mi, a.mu, b.mu);
+    r.nu[j] = codes2<true>(v[j], ni, a.nu, b.nu);
+  }
+  if (nu_least <= 0.f) {  // rare: weights that have had no gradient yet
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      r.nu[j] &= (v[j].x > 0.f ? 0xffu : 0u) | (v[j].y > 0.f ? 0xff00u : 0u);
+  }
+  return r;
+}
+
+// A warp per block of 256 values. What bounds it: 59 instructions an element beside its 18 bytes (75 before
+// products and sums went in pairs), so that a warp spends half of its time with no load in flight, and
+// under a load of seconds the clock (the power cap takes 10 %). A CTA therefore has the chunk of a later
+// CTA fetched into L2, one wave of CTAs ahead: 77M elements in 190 tensors 246 -> 211 us (6.6 TB/s;
+// sustained 253 -> 230), half a wave 218, two 228, four 298. Four CTAs an SM 230, five (spills) 242; a
+// warp that works on several blocks in a row 276 to 316, or with the next block's loads ahead in
+// registers, which leaves room for three CTAs, as long as without.
 template <int kItems>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kThreads, 4)
     adamw8_group_kernel(const __grid_constant__ Group<kItems> grp) {
   const unsigned chunk = blockIdx.x;
   const int which = find_item(grp, chunk);
   const t5x_adamw_item it = grp.item[which];
-  const Hyper h = grp.h;
   const int lane = threadIdx.x & 31;
   const long long block = static_cast<long long>(chunk - grp.first[which]) * (kChunk / kQuantBlock) +
                           (threadIdx.x >> 5);
   const long long begin = block * kQuantBlock;
   if (begin >= it.n) return;
-  const float cs = grp.clip_scale != nullptr ? *grp.clip_scale : 1.f;
   const int n = static_cast<int>(it.n - begin < kQuantBlock ? it.n - begin : kQuantBlock);
   float* p = static_cast<float*>(it.p) + begin;
   const float* g = static_cast<const float*>(it.g) + begin;
@@ -204,100 +346,87 @@ __global__ void __launch_bounds__(kThreads)
   __nv_bfloat16* out = it.out != nullptr ? static_cast<__nv_bfloat16*>(it.out) + begin : nullptr;
   float* mu_most = static_cast<float*>(it.mu_absmax) + block;
   float* nu_most = static_cast<float*>(it.nu_absmax) + block;
-  const uint32_t place = static_cast<uint32_t>(begin);
+  const bool fast = n == kQuantBlock && grp.wide[which];
 
-  float gg[8], pp[8], mm[8], vv[8];
-  const bool fast = n == kQuantBlock && wide(it);
+  if (threadIdx.x == 0 && chunk + grp.ahead < gridDim.x) {
+    const unsigned later = chunk + grp.ahead;
+    const int w = find_item(grp, later);
+    const t5x_adamw_item& item = grp.item[w];
+    const long long at = static_cast<long long>(later - grp.first[w]) * kChunk;
+    if (at + kChunk <= item.n && grp.wide[w]) {
+      prefetch_l2(static_cast<const float*>(item.g) + at, kChunk * 4);
+      prefetch_l2(static_cast<const float*>(item.p) + at, kChunk * 4);
+      prefetch_l2(static_cast<const uint8_t*>(item.mu) + at, kChunk);
+      prefetch_l2(static_cast<const uint8_t*>(item.nu) + at, kChunk);
+    }
+  }
+  Block8 in;
+  in.mu_most = *mu_most;
+  in.nu_most = *nu_most;
   if (fast) {
-    float4 gv[2], pv[2];
-    uint32_t mc[2], nc[2];
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      const int i = k * 32 + lane;
-      gv[k] = reinterpret_cast<const float4*>(g)[i];
-      pv[k] = reinterpret_cast<const float4*>(p)[i];
-      mc[k] = reinterpret_cast<const uint32_t*>(mu)[i];
-      nc[k] = reinterpret_cast<const uint32_t*>(nu)[i];
-    }
-    const float ms = *mu_most, ns = *nu_most;
-#pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      const float2 m0 = from_e4m3x2(mc[k]), m1 = from_e4m3x2(mc[k] >> 16);
-      const float2 n0 = from_e4m3x2(nc[k]), n1 = from_e4m3x2(nc[k] >> 16);
-      mm[4 * k] = m0.x, mm[4 * k + 1] = m0.y, mm[4 * k + 2] = m1.x, mm[4 * k + 3] = m1.y;
-      vv[4 * k] = n0.x, vv[4 * k + 1] = n0.y, vv[4 * k + 2] = n1.x, vv[4 * k + 3] = n1.y;
-      gg[4 * k] = gv[k].x, gg[4 * k + 1] = gv[k].y, gg[4 * k + 2] = gv[k].z, gg[4 * k + 3] = gv[k].w;
-      pp[4 * k] = pv[k].x, pp[4 * k + 1] = pv[k].y, pp[4 * k + 2] = pv[k].z, pp[4 * k + 3] = pv[k].w;
-    }
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      mm[j] = mm[j] * (1.f / 448.f) * ms;
-      vv[j] = vv[j] * (1.f / 448.f) * ns;
+    for (int j = 0; j < 2; ++j) {
+      const int i = j * 32 + lane;
+      in.g[j] = reinterpret_cast<const float4*>(g)[i];
+      in.p[j] = reinterpret_cast<const float4*>(p)[i];
+      in.mu[j] = reinterpret_cast<const uint32_t*>(mu)[i];
+      in.nu[j] = reinterpret_cast<const uint32_t*>(nu)[i];
     }
   } else {
-    const float ms = *mu_most, ns = *nu_most;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const int i = (j >> 2) * 128 + lane * 4 + (j & 3);
-      const bool in = i < n;
-      gg[j] = in ? g[i] : 0.f;
-      pp[j] = in ? p[i] : 0.f;
-      mm[j] = in ? from_e4m3x2(mu[i]).x * (1.f / 448.f) * ms : 0.f;
-      vv[j] = in ? from_e4m3x2(nu[i]).x * (1.f / 448.f) * ns : 0.f;
+    for (int j = 0; j < 2; ++j) {  // (what lies behind the end counts as zero: it stays out of the largest)
+      in.mu[j] = in.nu[j] = 0;
+      float gs[4], ps[4];
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int i = j * 128 + lane * 4 + q;
+        gs[q] = i < n ? g[i] : 0.f;
+        ps[q] = i < n ? p[i] : 0.f;
+        in.mu[j] |= (i < n ? mu[i] : 0u) << (8 * q);
+        in.nu[j] |= (i < n ? nu[i] : 0u) << (8 * q);
+      }
+      in.g[j] = make_float4(gs[0], gs[1], gs[2], gs[3]);
+      in.p[j] = make_float4(ps[0], ps[1], ps[2], ps[3]);
     }
   }
-  uint32_t mb = 0, nb = 0;
-#pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    update(h, gg[j] * cs, pp[j], mm[j], vv[j]);
-    const int i = (j >> 2) * 128 + lane * 4 + (j & 3);
-    if (fast || i < n) {  // as integers NaN is above every number, so that a NaN stays the largest
-      mb = max(mb, abs_bits(mm[j]));
-      nb = max(nb, abs_bits(vv[j]));
-    }
-  }
-  mb = __reduce_max_sync(0xffffffffu, mb);
-  nb = __reduce_max_sync(0xffffffffu, nb);
-  const float mi = inverse(__uint_as_float(mb)), ni = inverse(__uint_as_float(nb));
+  const float clip = grp.clip_scale != nullptr ? *grp.clip_scale : 1.f;
+  const Result8 r = step8(grp.h, clip, in, grp.h.noise_key + static_cast<uint32_t>(begin), lane);
   if (lane == 0) {  // (every lane has read the old scales: the reduction is behind the reads)
-    *mu_most = __uint_as_float(mb);
-    *nu_most = __uint_as_float(nb);
+    *mu_most = __uint_as_float(r.mu_most);
+    *nu_most = __uint_as_float(r.nu_most);
   }
   if (fast) {
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      const int i = k * 32 + lane;
-      uint32_t mc = 0, nc = 0;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const uint32_t r = noise(place + 4 * i + j, h.noise_key);
-        mc |= code_mu(mm[4 * k + j], mi, r) << (8 * j);
-        nc |= code_nu(vv[4 * k + j], ni, r) << (8 * j);
-      }
-      const float4 pv = make_float4(pp[4 * k], pp[4 * k + 1], pp[4 * k + 2], pp[4 * k + 3]);
+    for (int j = 0; j < 2; ++j) {
+      const int i = j * 32 + lane;
+      const float4 pv = make_float4(r.p[2 * j].x, r.p[2 * j].y, r.p[2 * j + 1].x, r.p[2 * j + 1].y);
       reinterpret_cast<float4*>(p)[i] = pv;
-      reinterpret_cast<uint32_t*>(mu)[i] = mc;
-      reinterpret_cast<uint32_t*>(nu)[i] = nc;
+      reinterpret_cast<uint32_t*>(mu)[i] = r.mu[2 * j] | (r.mu[2 * j + 1] << 16);
+      reinterpret_cast<uint32_t*>(nu)[i] = r.nu[2 * j] | (r.nu[2 * j + 1] << 16);
       if (out != nullptr) reinterpret_cast<uint2*>(out)[i] = pack_bf16(pv);
     }
     return;
   }
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    const int i = (j >> 2) * 128 + lane * 4 + (j & 3);
-    if (i >= n) continue;
-    const uint32_t r = noise(place + i, h.noise_key);
-    p[i] = pp[j];
-    mu[i] = static_cast<uint8_t>(code_mu(mm[j], mi, r));
-    nu[i] = static_cast<uint8_t>(code_nu(vv[j], ni, r));
-    if (out != nullptr) out[i] = __float2bfloat16(pp[j]);
+  for (int j = 0; j < 4; ++j) {
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+      const int i = (j >> 1) * 128 + lane * 4 + (j & 1) * 2 + q;
+      if (i >= n) continue;
+      const float v = q ? r.p[j].y : r.p[j].x;
+      p[i] = v;
+      mu[i] = static_cast<uint8_t>(r.mu[j] >> (8 * q));
+      nu[i] = static_cast<uint8_t>(r.nu[j] >> (8 * q));
+      if (out != nullptr) out[i] = __float2bfloat16(v);
+    }
   }
 }
 
 // ---- global norm ----
 
-// Sum of squares of the chunks blockIdx.x, blockIdx.x + gridDim.x, ... in 64 bits across chunks
-// (eight values of a thread in 32). A CTA's chunks and the order of all sums depend on the grid
+// Sum of squares of every gridDim.x-th span of chunks, in 64 bits across spans (the up to 64 values of a thread
+// in a span in 32), from the last chunk to the first: the step that follows begins with those that were read last
+// and are still in L2. A CTA's chunks and the order of all sums depend on the grid
 // alone. `finish`: the CTA that arrives last adds the partial sums of this and the earlier launches of
 // the call and stores the clip factor min(1, max_norm / (norm + 1e-16)).
 template <int kItems>
@@ -308,23 +437,32 @@ __global__ void __launch_bounds__(kThreads)
   __shared__ bool s_last;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   double sum = 0.0;
-  for (unsigned chunk = blockIdx.x; chunk < chunks; chunk += gridDim.x) {
-    const int which = find_item(grp, chunk);
-    const t5x_adamw_item& it = grp.item[which];
-    const long long begin = static_cast<long long>(chunk - grp.first[which]) * kChunk;
-    const int n = static_cast<int>(it.n - begin < kChunk ? it.n - begin : kChunk);
-    const float* g = static_cast<const float*>(it.g) + begin;
-    float s = 0.f;
-    if (n == kChunk && (reinterpret_cast<uintptr_t>(it.g) & 15) == 0) {
-#pragma unroll
-      for (int k = 0; k < kChunk / (4 * kThreads); ++k) {
-        const float4 v = reinterpret_cast<const float4*>(g)[k * kThreads + threadIdx.x];
-        s += v.x * v.x + v.y * v.y + v.z * v.z + v.w * v.w;
+  const unsigned spans = (chunks + kSpan - 1) / kSpan;
+  for (unsigned at = blockIdx.x; at < spans; at += gridDim.x) {
+    unsigned chunk = (spans - 1 - at) * kSpan;
+    const unsigned end = chunk + kSpan < chunks ? chunk + kSpan : chunks;
+    int which = find_item(grp, chunk);
+    while (chunk < end) {
+      while (which + 1 < grp.count && grp.first[which + 1] <= chunk) ++which;
+      const unsigned behind = which + 1 < grp.count && grp.first[which + 1] < end ? grp.first[which + 1] : end;
+      const long long begin = static_cast<long long>(chunk - grp.first[which]) * kChunk;
+      const long long left = grp.item[which].n - begin;
+      const int n = static_cast<int>(left < (behind - chunk) * kChunk ? left : (behind - chunk) * kChunk);
+      const float* g = static_cast<const float*>(grp.item[which].g) + begin;
+      float s = 0.f;
+      if (n == kSpan * kChunk && grp.wide[which]) {
+#pragma unroll 8
+        for (int k = 0; k < kSpan * kChunk / (4 * kThreads); ++k) {
+          const float4 v = reinterpret_cast<const float4*>(g)[k * kThreads + threadIdx.x];
+          s += v.x * v.x + v.y * v.y + v.z * v.z + v.w * v.w;
+        }
+      } else {
+#pragma unroll 4
+        for (int i = threadIdx.x; i < n; i += kThreads) s += g[i] * g[i];
       }
-    } else {
-      for (int i = threadIdx.x; i < n; i += kThreads) s += g[i] * g[i];
+      sum += static_cast<double>(s);
+      chunk = behind;
     }
-    sum += static_cast<double>(s);
   }
   auto block_sum = [&](double v) {
 #pragma unroll
@@ -370,8 +508,16 @@ int fill(Group<kItems>& grp, const t5x_adamw_item* items, int from, int count, u
     if (need == 0) continue;
     if (c + need > 0x7fffffffull) break;
     grp.first[grp.count] = static_cast<unsigned>(c);
+    grp.wide[grp.count] = takes_wide(items[i]);
     grp.item[grp.count++] = items[i];
     c += need;
+  }
+  grp.shift = 0;
+  while ((c >> grp.shift) >= kHints) ++grp.shift;
+  for (int k = 0, at = 0; k <= kHints; ++k) {
+    const unsigned long long chunk_k = static_cast<unsigned long long>(k) << grp.shift;
+    while (at + 1 < grp.count && grp.first[at + 1] <= chunk_k) ++at;
+    grp.near[k] = static_cast<unsigned short>(at);
   }
   *chunks = static_cast<unsigned>(c);
   return i - from;
@@ -407,6 +553,7 @@ int step_in_groups(const t5x_adamw_item* items, int count, const Hyper& h, const
   Group<kItems> grp;
   grp.h = h;
   grp.clip_scale = clip_scale;
+  grp.ahead = static_cast<unsigned>(num_sms()) * 4;
   for (int from = 0; from < count;) {
     unsigned chunks;
     from += fill(grp, items, from, count, &chunks);
@@ -434,7 +581,8 @@ int sumsq_in_groups(const t5x_adamw_item* items, int count, void* scratch, float
     from += fill(grp, items, from, count, &chunks);
     const bool last = from >= count;
     if (chunks == 0 && !last) continue;
-    const unsigned grid = chunks == 0 ? 1 : (chunks < cap ? chunks : cap);
+    const unsigned spans = (chunks + kSpan - 1) / kSpan;
+    const unsigned grid = spans == 0 ? 1 : (spans < cap ? spans : cap);
     sumsq_group_kernel<kItems><<<grid, kThreads, 0, st>>>(grp, chunks, partial, first, arrived, max_norm,
                                                           last ? clip : nullptr);
     count_launches(1);
@@ -502,7 +650,12 @@ T5X_API int t5x_adamw_group(const t5x_adamw_item* items, int count, int state_bi
     h.bc1 = static_cast<float>(1.0 - pow(b1, step));
     h.bc2 = static_cast<float>(1.0 - pow(b2, step));
   }
-  h.noise_key = seed * 0x9E3779B1u + static_cast<unsigned>(step) * 0xBB67AE85u;
+  h.b1_448 = static_cast<float>(b1 / 448.0);
+  h.b2_448 = static_cast<float>(b2 / 448.0);
+  h.ibc2 = 1.f / h.bc2;
+  h.lr_bc1 = -lr / h.bc1;
+  h.lr_decay = -lr * weight_decay;
+  h.noise_key = seed * kNoise1 + static_cast<unsigned>(step) * 0xBB67AE85u;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const float* cs = static_cast<const float*>(clip_scale);
   if (count <= kFewItems)

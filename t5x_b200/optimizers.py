@@ -278,7 +278,8 @@ def quantize_moment(x: torch.Tensor, noise: torch.Tensor, second: bool):
   y = (torch.floor(y / gap + up) * gap).clamp(max=_E4M3_MAX)
   if second:
     y = torch.where((rows > 0) & (y == 0), torch.full_like(y, 2.0 ** -9), y)
-  codes = torch.copysign(y, rows).to(torch.float8_e4m3fn).view(torch.uint8)
+  y = torch.where(y == 0, y, torch.copysign(y, rows))  # (no negative zeros)
+  codes = y.to(torch.float8_e4m3fn).view(torch.uint8)
   return codes.reshape(-1)[:x.numel()].view(x.shape).contiguous(), absmax
 
 
