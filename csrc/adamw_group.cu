@@ -42,8 +42,7 @@ constexpr int kFewItems = 48;
 
 struct Hyper {
   float lr, b1, b2, c1, c2, eps, eps_root, weight_decay, bc1, bc2;  // c = 1 - b
-  // for moments in 8 bits: b / 448, 1 / bc2, -lr / bc1, -lr * weight_decay
-  float b1_448, b2_448, ibc2, lr_bc1, lr_decay;
+  float one, ibc2, lr_bc1, lr_decay;  // for moments in 8 bits: 1, 1 / bc2, -lr / bc1, -lr * weight_decay
   uint32_t noise_key;
 };
 
@@ -188,41 +187,30 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
 }
 __device__ __forceinline__ float2 both(float x) { return make_float2(x, x); }
 
-// What a step multiplies by, the same for a whole block of values.
-struct Factors {
-  float2 clip, c1, c2, mu, nu;              // mu, nu: b / 448 * largest of the old moments
-  float2 ibc2, eps_root, eps, lr, lr_decay;  // lr: -lr / bc1; lr_decay: -lr * weight_decay
-};
-__device__ __forceinline__ Factors factors(const Hyper& h, float clip, float mu_most, float nu_most) {
-  Factors f;
-  f.clip = both(clip);
-  f.c1 = both(h.c1);
-  f.c2 = both(h.c2);
-  f.mu = both(h.b1_448 * mu_most);
-  f.nu = both(h.b2_448 * nu_most);
-  f.ibc2 = both(h.ibc2);
-  f.eps_root = both(h.eps_root);
-  f.eps = both(h.eps);
-  f.lr = both(h.lr_bc1);
-  f.lr_decay = both(h.lr_decay);
-  return f;
+// a / b to the nearest from inv = 1 / b to the nearest: Markstein's correction (IBM J. Res. Dev. 34, 1990).
+__device__ __forceinline__ float2 divide2(float2 a, float2 b, float2 inv) {
+  const float2 q = mul2(a, inv);
+  return fma2(fma2(make_float2(-q.x, -q.y), b, a), inv, q);
 }
-
 __device__ __forceinline__ float reciprocal(float x) {
   float r;
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
   return r;
 }
 
-// The step of two values; m and v: e4m3 values of the old moments, then the new moments in 32 bits.
-__device__ __forceinline__ void update2(const Factors& f, float2 g, float2& p, float2& m, float2& v) {
-  g = mul2(g, f.clip);
-  m = fma2(m, f.mu, mul2(g, f.c1));
-  v = fma2(mul2(g, f.c2), g, mul2(v, f.nu));
-  float2 d = fma2(v, f.ibc2, f.eps_root);
-  d = add2(make_float2(sqrtf(d.x), sqrtf(d.y)), f.eps);
+// The step of two values; m and v: the old moments, then the new ones. Their products and sums are
+// rounded one by one, so that a moment before it is stored is, bit for bit, what tensor operations make
+// of it: a draw that lies next to its border would else fall on the other side of it, and a second
+// moment that is a step of e4m3 apart shows in the weights of the next step. (The assembler makes one
+// fused instruction of a paired product and the paired sum behind it; it cannot where the sum is a
+// product with a `one` that it does not know.)
+__device__ __forceinline__ void update2(const Hyper& h, float2 g, float2& p, float2& m, float2& v) {
+  m = fma2(mul2(m, both(h.b1)), both(h.one), mul2(g, both(h.c1)));
+  v = fma2(mul2(v, both(h.b2)), both(h.one), mul2(mul2(g, g), both(h.c2)));
+  float2 d = fma2(v, both(h.ibc2), both(h.eps_root));
+  d = add2(make_float2(sqrtf(d.x), sqrtf(d.y)), both(h.eps));
   const float2 r = make_float2(reciprocal(d.x), reciprocal(d.y));
-  p = add2(p, fma2(mul2(m, r), f.lr, mul2(p, f.lr_decay)));
+  p = add2(p, fma2(mul2(m, r), both(h.lr_bc1), mul2(p, both(h.lr_decay))));
 }
 
 __device__ __forceinline__ float2 from_e4m3x2(uint32_t two) {
@@ -233,26 +221,22 @@ __device__ __forceinline__ float2 from_e4m3x2(uint32_t two) {
 
 __device__ __forceinline__ uint32_t abs_bits(float x) { return __float_as_uint(x) & 0x7fffffffu; }
 
-// 1.75 / largest: times 256 = 448 / largest, which would overflow where the largest is tiny; 0 where
-// all are zero. (A largest that is not finite makes the whole block NaN when it is read back, as the
-// largest itself is kept.)
-__device__ __forceinline__ float inverse(float most) { return most > 0.f ? 1.75f / most : 0.f; }
-
 // The two e4m3 codes of x / largest * 448, each rounded to a neighbour by 16 random bits (at bits 4 to 19
 // of `noise`): e4m3 keeps three of the 23 bits of the mantissa, so the bits that fall away are topped
 // up by a random number below one step before they are cut off. Below 2^-6 the steps are 2^-9 wide;
 // with 2^-6 added the value lies among numbers whose steps are the same, and what is left when it is
 // taken off again is exact. kSecond: no sign, and nothing is stored as zero (the caller sees to zeros).
+// (A largest that is not finite makes the whole block NaN when it is read back, as it is kept itself.)
 template <bool kSecond>
-__device__ __forceinline__ uint32_t codes2(float2 x, float inv, uint32_t noise0, uint32_t noise1) {
-  const float2 y = mul2(x, both(inv));
+__device__ __forceinline__ uint32_t codes2(float2 x, float most, float inv, uint32_t noise0, uint32_t noise1) {
+  const float2 y = mul2(divide2(x, both(most), both(inv)), both(448.f));
   auto shift = [](float v) {
     const float by = kSecond ? 0.015625f
                              : __uint_as_float((__float_as_uint(v) & 0x80000000u) | 0x3c800000u);
-    return fabsf(v) < 0.00006103515625f ? by : 0.f;  // (2^-14: y is x / largest * 1.75)
+    return fabsf(v) < 0.015625f ? by : 0.f;
   };
   const float2 c = make_float2(shift(y.x), shift(y.y));
-  float2 z = fma2(y, both(256.f), c);
+  float2 z = add2(y, c);
   z.x = __uint_as_float((__float_as_uint(z.x) + noise0 + 8u) & 0xfff00000u);
   z.y = __uint_as_float((__float_as_uint(z.y) + noise1 + 8u) & 0xfff00000u);
   z = fma2(c, both(-1.f), z);
@@ -283,7 +267,9 @@ struct Result8 {
   uint32_t mu_most, nu_most;
 };
 __device__ __forceinline__ Result8 step8(const Hyper& h, float clip, const Block8& in, uint32_t key, int lane) {
-  const Factors f = factors(h, clip, in.mu_most, in.nu_most);
+  // codes stand for code * (largest / 448)
+  const float2 mu_unit = both(__fmul_rn(in.mu_most, 1.f / 448.f));
+  const float2 nu_unit = both(__fmul_rn(in.nu_most, 1.f / 448.f));
   Result8 r;
   float2 m[4], v[4];
   r.mu_most = r.nu_most = 0;
@@ -293,9 +279,9 @@ __device__ __forceinline__ Result8 step8(const Hyper& h, float clip, const Block
     const int k = j >> 1, s = (j & 1) * 16;
     const float2 g = j & 1 ? make_float2(in.g[k].z, in.g[k].w) : make_float2(in.g[k].x, in.g[k].y);
     r.p[j] = j & 1 ? make_float2(in.p[k].z, in.p[k].w) : make_float2(in.p[k].x, in.p[k].y);
-    m[j] = from_e4m3x2(in.mu[k] >> s);
-    v[j] = from_e4m3x2(in.nu[k] >> s);
-    update2(f, g, r.p[j], m[j], v[j]);
+    m[j] = mul2(from_e4m3x2(in.mu[k] >> s), mu_unit);
+    v[j] = mul2(from_e4m3x2(in.nu[k] >> s), nu_unit);
+    update2(h, mul2(g, both(clip)), r.p[j], m[j], v[j]);
     // as integers NaN is above every number, so that a NaN stays the largest
     r.mu_most = max(r.mu_most, max(abs_bits(m[j].x), abs_bits(m[j].y)));
     r.nu_most = max(r.nu_most, max(__float_as_uint(v[j].x), __float_as_uint(v[j].y)));
@@ -303,14 +289,16 @@ __device__ __forceinline__ Result8 step8(const Hyper& h, float clip, const Block
   }
   r.mu_most = __reduce_max_sync(0xffffffffu, r.mu_most);
   r.nu_most = __reduce_max_sync(0xffffffffu, r.nu_most);
-  const float mi = inverse(__uint_as_float(r.mu_most)), ni = inverse(__uint_as_float(r.nu_most));
+  const float mu_most = __uint_as_float(r.mu_most), nu_most = __uint_as_float(r.nu_most);
+  const float mu_inv = mu_most > 0.f ? __frcp_rn(mu_most) : 0.f;  // (all zeros: codes of zero)
+  const float nu_inv = nu_most > 0.f ? __frcp_rn(nu_most) : 0.f;
   const uint32_t seed = (key + lane * 4) * kNoise1;
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     const uint32_t i = (j >> 1) * 128 + (j & 1) * 2;
     const Noise a = noise(seed + i * kNoise1), b = noise(seed + (i + 1) * kNoise1);
-    r.mu[j] = codes2<false>(m[j], mi, a.mu, b.mu);
-    r.nu[j] = codes2<true>(v[j], ni, a.nu, b.nu);
+    r.mu[j] = codes2<false>(m[j], mu_most, mu_inv, a.mu, b.mu);
+    r.nu[j] = codes2<true>(v[j], nu_most, nu_inv, a.nu, b.nu);
   }
   if (nu_least <= 0.f) {  // rare: weights that have had no gradient yet
 #pragma unroll
@@ -320,13 +308,13 @@ __device__ __forceinline__ Result8 step8(const Hyper& h, float clip, const Block
   return r;
 }
 
-// A warp per block of 256 values. What bounds it: 59 instructions an element beside its 18 bytes (75 before
-// products and sums went in pairs), so that a warp spends half of its time with no load in flight, and
-// under a load of seconds the clock (the power cap takes 10 %). A CTA therefore has the chunk of a later
-// CTA fetched into L2, one wave of CTAs ahead: 77M elements in 190 tensors 246 -> 211 us (6.6 TB/s;
-// sustained 253 -> 230), half a wave 218, two 228, four 298. Four CTAs an SM 230, five (spills) 242; a
-// warp that works on several blocks in a row 276 to 316, or with the next block's loads ahead in
-// registers, which leaves room for three CTAs, as long as without.
+// A warp per block of 256 values. What bounds it: some 65 instructions an element beside its 18 bytes (80
+// before products and sums went in pairs), so that a warp spends half of its time with no load in
+// flight, and under a load of seconds the clock (the power cap takes 10 %). A CTA therefore has the chunk
+// of a later CTA fetched into L2, one wave of CTAs ahead: 77M elements in 190 tensors 246 -> 211 us,
+// sustained 253 -> 230; half a wave 218, two 228, four 298. Four CTAs an SM 230, five (spills) 242; a warp
+// that works on several blocks in a row 276 to 316. With the moments rounded as tensor operations round
+// them 247 us sustained (5.6 TB/s).
 template <int kItems>
 __global__ void __launch_bounds__(kThreads, 4)
     adamw8_group_kernel(const __grid_constant__ Group<kItems> grp) {
@@ -424,11 +412,11 @@ __global__ void __launch_bounds__(kThreads, 4)
 
 // ---- global norm ----
 
-// Sum of squares of every gridDim.x-th span of chunks, in 64 bits across spans (the up to 64 values of a thread
-// in a span in 32), from the last chunk to the first: the step that follows begins with those that were read last
-// and are still in L2. A CTA's chunks and the order of all sums depend on the grid
-// alone. `finish`: the CTA that arrives last adds the partial sums of this and the earlier launches of
-// the call and stores the clip factor min(1, max_norm / (norm + 1e-16)).
+// Sum of squares of every gridDim.x-th span of chunks, in 64 bits (the factor scales every gradient: it
+// is the one that exact arithmetic gives, rounded once), from the last span to the first: the step that
+// follows begins with those that were read last and are still in L2. A CTA's spans and the order of
+// all sums depend on the grid alone. With `clip_out` the CTA that arrives last adds the partial sums of
+// this and the earlier launches of the call and stores min(1, max_norm / (norm + 1e-16)).
 template <int kItems>
 __global__ void __launch_bounds__(kThreads)
     sumsq_group_kernel(const __grid_constant__ Group<kItems> grp, unsigned chunks, double* partial,
@@ -436,7 +424,7 @@ __global__ void __launch_bounds__(kThreads)
   __shared__ double s_sum[kThreads / 32];
   __shared__ bool s_last;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  double sum = 0.0;
+  double sum = 0.0, more = 0.0;
   const unsigned spans = (chunks + kSpan - 1) / kSpan;
   for (unsigned at = blockIdx.x; at < spans; at += gridDim.x) {
     unsigned chunk = (spans - 1 - at) * kSpan;
@@ -449,18 +437,23 @@ __global__ void __launch_bounds__(kThreads)
       const long long left = grp.item[which].n - begin;
       const int n = static_cast<int>(left < (behind - chunk) * kChunk ? left : (behind - chunk) * kChunk);
       const float* g = static_cast<const float*>(grp.item[which].g) + begin;
-      float s = 0.f;
       if (n == kSpan * kChunk && grp.wide[which]) {
-#pragma unroll 8
+#pragma unroll
         for (int k = 0; k < kSpan * kChunk / (4 * kThreads); ++k) {
           const float4 v = reinterpret_cast<const float4*>(g)[k * kThreads + threadIdx.x];
-          s += v.x * v.x + v.y * v.y + v.z * v.z + v.w * v.w;
+          const double x = v.x, y = v.y, z = v.z, w = v.w;
+          sum = fma(x, x, sum);
+          more = fma(y, y, more);
+          sum = fma(z, z, sum);
+          more = fma(w, w, more);
         }
       } else {
 #pragma unroll 4
-        for (int i = threadIdx.x; i < n; i += kThreads) s += g[i] * g[i];
+        for (int i = threadIdx.x; i < n; i += kThreads) {
+          const double x = g[i];
+          sum = fma(x, x, sum);
+        }
       }
-      sum += static_cast<double>(s);
       chunk = behind;
     }
   }
@@ -475,7 +468,7 @@ __global__ void __launch_bounds__(kThreads)
     for (int w = 0; w < kThreads / 32; ++w) t += s_sum[w];
     return t;
   };
-  sum = block_sum(sum);
+  sum = block_sum(sum + more);
   if (threadIdx.x == 0) {
     partial[partial_first + blockIdx.x] = sum;
     s_last = false;
@@ -492,8 +485,8 @@ __global__ void __launch_bounds__(kThreads)
     total += __ldcg(partial + i);
   total = block_sum(total);
   if (threadIdx.x == 0) {
-    const float f = max_norm / (static_cast<float>(sqrt(total)) + 1e-16f);
-    *clip_out = f > 1.f ? 1.f : f;  // (NaN stays)
+    const double f = static_cast<double>(max_norm) / (sqrt(total) + 1e-16);
+    *clip_out = static_cast<float>(f > 1.0 ? 1.0 : f);  // (NaN stays)
   }
 }
 
@@ -650,8 +643,7 @@ T5X_API int t5x_adamw_group(const t5x_adamw_item* items, int count, int state_bi
     h.bc1 = static_cast<float>(1.0 - pow(b1, step));
     h.bc2 = static_cast<float>(1.0 - pow(b2, step));
   }
-  h.b1_448 = static_cast<float>(b1 / 448.0);
-  h.b2_448 = static_cast<float>(b2 / 448.0);
+  h.one = 1.f;
   h.ibc2 = 1.f / h.bc2;
   h.lr_bc1 = -lr / h.bc1;
   h.lr_decay = -lr * weight_decay;

@@ -258,8 +258,8 @@ def _blocks_of(x: torch.Tensor) -> torch.Tensor:
 
 
 def dequantize_moment(codes: torch.Tensor, absmax: torch.Tensor) -> torch.Tensor:
-  """The fp32 values that 8-bit moments stand for: e4m3 code / 448 * largest of the block."""
-  values = _blocks_of(codes).view(torch.float8_e4m3fn).float() * (1.0 / _E4M3_MAX) * absmax[:, None]
+  """The fp32 values that 8-bit moments stand for: e4m3 code * (largest of the block / 448)."""
+  values = _blocks_of(codes).view(torch.float8_e4m3fn).float() * (absmax * (1.0 / _E4M3_MAX))[:, None]
   return values.reshape(-1)[:codes.numel()].view(codes.shape)
 
 
@@ -271,8 +271,7 @@ def quantize_moment(x: torch.Tensor, noise: torch.Tensor, second: bool):
   the smallest number at least: as zero it would leave the step to be divided by eps."""
   rows = _blocks_of(x.float())
   absmax = rows.abs().amax(dim=1) if rows.numel() else rows.new_zeros(rows.shape[0])
-  inverse = torch.where(absmax > 0, 1.0 / absmax, torch.zeros_like(absmax))
-  y = rows.abs() * inverse[:, None] * _E4M3_MAX
+  y = rows.abs() / torch.where(absmax == 0, torch.ones_like(absmax), absmax)[:, None] * _E4M3_MAX
   gap = torch.ldexp(torch.ones_like(y), (torch.frexp(y)[1] - 1).clamp(min=-6) - 3)
   up = (_blocks_of(noise).to(y.dtype) + 0.5) / 65536.0
   y = (torch.floor(y / gap + up) * gap).clamp(max=_E4M3_MAX)
@@ -310,7 +309,7 @@ def scale_by_adam8(b1=0.9, b2=0.999, eps=1e-8, eps_root=0.0, seed=0) -> Gradient
     out = {}
     for k, g in updates.items():
       mu = b1 * dequantize_moment(state["mu"][k], state["mu_absmax"][k]) + (1 - b1) * g
-      nu = b2 * dequantize_moment(state["nu"][k], state["nu_absmax"][k]) + (1 - b2) * g * g
+      nu = b2 * dequantize_moment(state["nu"][k], state["nu_absmax"][k]) + (1 - b2) * (g * g)
       out[k] = (mu / bc1) / (torch.sqrt(nu / bc2 + eps_root) + eps)
       noise = _moment_noise(g.numel(), seed, c, g.device)
       new["mu"][k], new["mu_absmax"][k] = quantize_moment(mu, noise & 0xFFFF, False)
