@@ -89,6 +89,34 @@ long long t5x_grad_clip_scratch_bytes(const t5x_adamw_item* items, int count);
 int t5x_grad_clip_scale(const t5x_adamw_item* items, int count, void* scratch, float max_norm,
                         void* clip_scale, void* stream);
 
+/* Losses over logits [batch, length, vocab] (fp32 or bf16; strides in values, last dimension contiguous)
+ * with their gradient in `grad` (the same strides and place of 16 bytes, or null), and over
+ * log-probabilities [batch, length] (fp32) with theirs in `slope` (or null): see token_losses.cu.
+ * targets int64, weights fp32 (or null: all 1), other inputs fp32. normalizer: device scalar that divides
+ * the loss, or null: `scale` multiplies it. scratch: the stated bytes, 16-byte aligned. policy: out = loss,
+ * kl, clipped, weight. preference: scores [batch], margins [batch / 2], out = loss, pairs. */
+long long t5x_policy_loss_scratch_bytes();
+int t5x_policy_loss(const void* logits, int fp32, void* grad, long long batch, int length, int vocab,
+                    long long stride_b, long long stride_t, const void* targets, const void* weights,
+                    const void* old_scores, const void* ref_scores, const void* advantages, long long adv_b,
+                    long long adv_t, float clip_low, float clip_high, float kl_weight, float scale,
+                    const void* normalizer, void* scratch, void* out, void* stream);
+int t5x_policy_loss_tokens(const void* logp, void* slope, long long batch, int length, const void* weights,
+                           const void* old_scores, const void* ref_scores, const void* advantages,
+                           long long adv_b, long long adv_t, float clip_low, float clip_high, float kl_weight,
+                           float scale, const void* normalizer, void* scratch, void* out, void* stream);
+long long t5x_preference_loss_scratch_bytes(long long batch, int length);
+int t5x_preference_loss(const void* logits, int fp32, void* grad, long long batch, int length, int vocab,
+                        long long stride_b, long long stride_t, const void* targets, const void* weights,
+                        const void* reference, float beta, float smoothing, float scale, const void* normalizer,
+                        void* scratch, void* scores, void* margins, void* out, void* stream);
+int t5x_preference_loss_tokens(const void* logp, void* slope, long long batch, int length, const void* weights,
+                               const void* reference, float beta, float smoothing, float scale,
+                               const void* normalizer, void* scratch, void* scores, void* margins, void* out,
+                               void* stream);
+/* dst = src * *factor (dst may be src; nothing is done where the factor is 1 then) */
+int t5x_scale_gradient(const void* src, void* dst, long long n, int fp32, const void* factor, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -156,3 +156,137 @@ def _sum_over_data_replicas(factor):
   t = torch.as_tensor(factor, dtype=torch.float32, device=st.device).detach().clone().reshape(1)
   dist.all_reduce(t, group=st.data_group)
   return t[0]
+
+
+# ----------------------------------------------------------------------------
+# Preference and policy fine-tuning
+# ----------------------------------------------------------------------------
+def _check_tokens(what: str, values: torch.Tensor, dims: int, **tokens) -> None:
+  if values.dim() != dims:
+    raise ValueError(f"{what}: expected a tensor of {dims} dimensions, got shape {tuple(values.shape)}")
+  if not values.is_floating_point():
+    raise ValueError(f"{what}: expected floating-point values, got {values.dtype}")
+  for name, t in tokens.items():
+    if t is not None and t.shape != values.shape[:2]:
+      raise ValueError(f"{what}: Incorrect shapes. Got shape {tuple(t.shape)} {name} for [batch, length] = "
+                       f"{tuple(values.shape[:2])}")
+    if t is not None and t.device != values.device:
+      raise ValueError(f"{what}: {name} are on {t.device}, the values on {values.device}")
+    if name == "targets" and (t.is_floating_point() or t.dtype == torch.bool):
+      raise ValueError(f"{what}: targets must be whole numbers, got {t.dtype}")
+
+
+def _check_factor(what: str, factor) -> None:
+  if isinstance(factor, (str, SpecialLossNormalizingFactor)):
+    raise ValueError(f"{what}: resolve a special loss_normalizing_factor with "
+                     "get_loss_normalizing_factor_and_weights first")
+
+
+def _check_preference(what, values, reference_scores, beta, label_smoothing, factor):
+  if values.shape[0] % 2 or values.shape[0] == 0:
+    raise ValueError(f"{what}: the batch must hold pairs of rows, got {values.shape[0]} rows")
+  if reference_scores.shape != values.shape[:1] or reference_scores.device != values.device:
+    raise ValueError(f"{what}: reference_scores must be [{values.shape[0]}] on {values.device}, got "
+                     f"{tuple(reference_scores.shape)} on {reference_scores.device}")
+  if not 0.0 <= label_smoothing <= 1.0 or not math.isfinite(beta):
+    raise ValueError(f"{what}: beta must be finite and label_smoothing in [0, 1], got {beta}, {label_smoothing}")
+  _check_factor(what, factor)
+
+
+def compute_preference_loss(logits: torch.Tensor, targets: torch.Tensor, weights: Optional[torch.Tensor],
+                            reference_scores: torch.Tensor, beta: float = 0.1, label_smoothing: float = 0.0,
+                            loss_normalizing_factor=None):
+  """Loss of paired answers by their log ratios against a reference model.
+
+  Rows 2j and 2j + 1 of `logits` [batch, length, vocab] are answers to one prompt, row 2j the preferred one.
+  With the score of a row, sum_t weights * log softmax(logits)[targets], and `reference_scores` [batch], the
+  scores that the reference model gives (`score_batch` of both models returns such scores),
+  margin_j = beta * ((score - reference)_2j - (score - reference)_2j+1), and the loss is the sum (not mean) of
+  (1 - label_smoothing) log(1 + exp(-margin)) + label_smoothing log(1 + exp(margin)), over
+  `loss_normalizing_factor` if one is given.
+
+  Returns (loss, scores [batch], margins [batch / 2], number of pairs); the loss alone is differentiable, and in
+  the logits alone. Tokens of weight 0 do not count, whatever their logits hold, and a pair without any
+  other is padding: it counts nowhere. A weighted target outside of the vocabulary gives a NaN loss on the GPU.
+
+  On the GPU the gradient is computed along with the loss (memory of the logits' size) for logits in bf16 or
+  fp32; see t5x_b200/ops/token_losses.py."""
+  from t5x_b200.ops import token_losses
+  what = "compute_preference_loss"
+  _check_tokens(what, logits, 3, targets=targets, weights=weights)
+  _check_preference(what, logits, reference_scores, beta, label_smoothing, loss_normalizing_factor)
+  return token_losses.preference_loss(logits, targets, weights, reference_scores, float(beta),
+                                      float(label_smoothing), loss_normalizing_factor)
+
+
+def preference_loss_from_token_scores(token_scores: torch.Tensor, weights: Optional[torch.Tensor],
+                                      reference_scores: torch.Tensor, beta: float = 0.1,
+                                      label_smoothing: float = 0.0, loss_normalizing_factor=None):
+  """`compute_preference_loss` from log-probabilities of the targets [batch, length], differentiable in them.
+  Behind the projection that is fused with its cross entropy, where no logits exist: `token_scores` is minus the
+  per-token loss of `functional.logits_cross_entropy` (z-loss and label smoothing 0)."""
+  from t5x_b200.ops import token_losses
+  what = "preference_loss_from_token_scores"
+  _check_tokens(what, token_scores, 2, weights=weights)
+  _check_preference(what, token_scores, reference_scores, beta, label_smoothing, loss_normalizing_factor)
+  return token_losses.preference_loss(token_scores, None, weights, reference_scores, float(beta),
+                                      float(label_smoothing), loss_normalizing_factor)
+
+
+def _check_policy(what, values, advantages, clip_range, clip_range_high, factor):
+  if advantages.shape not in (values.shape[:1], values.shape[:2], (values.shape[0], 1)) or \
+      advantages.device != values.device:
+    raise ValueError(f"{what}: advantages must be [batch] or [batch, length] = {tuple(values.shape[:2])} on "
+                     f"{values.device}, got {tuple(advantages.shape)} on {advantages.device}")
+  high = clip_range if clip_range_high is None else clip_range_high
+  if not (0.0 <= clip_range <= 1.0 and high >= 0.0):
+    raise ValueError(f"{what}: clip_range must lie in [0, 1] and clip_range_high must not be negative, got "
+                     f"{clip_range}, {high}")
+  _check_factor(what, factor)
+  return float(clip_range), float(high)
+
+
+def compute_policy_loss(logits: torch.Tensor, targets: torch.Tensor, weights: Optional[torch.Tensor],
+                        old_token_scores: torch.Tensor, advantages: torch.Tensor,
+                        reference_token_scores: Optional[torch.Tensor] = None, clip_range: float = 0.2,
+                        clip_range_high: Optional[float] = None, kl_weight: float = 0.0,
+                        loss_normalizing_factor=None):
+  """Clipped policy loss with a KL term over the tokens of drawn answers.
+
+  With logp = log softmax(logits)[targets] of `logits` [batch, length, vocab], ratio = exp(logp -
+  old_token_scores) against the log-probabilities [batch, length] when the answers were drawn, and `advantages`
+  ([batch], one for an answer, or [batch, length]), a token's loss is
+  -min(advantage * ratio, advantage * clip(ratio, 1 - clip_range, 1 + clip_range_high)) + kl_weight * kl with
+  kl = exp(ref - logp) - 1 - (ref - logp) against `reference_token_scores` (None: no such term);
+  clip_range_high is clip_range unless given. Log-probabilities are unweighted, as in the `token_scores` that
+  `score_batch` returns for weights of 0 and 1.
+
+  Returns (loss, kl, clipped, weight_sum): the sums (not means) of weights * loss and weights * kl, both over
+  `loss_normalizing_factor` if one is given, the weights of the tokens that the clip holds, and all weights. The
+  loss alone is differentiable, and in the logits alone. Tokens of weight 0 do not count, whatever is in
+  their places. A weighted target outside of the vocabulary gives a NaN loss on the GPU.
+
+  On the GPU loss and gradient take one pass over logits in bf16 or fp32; see t5x_b200/ops/token_losses.py."""
+  from t5x_b200.ops import token_losses
+  what = "compute_policy_loss"
+  _check_tokens(what, logits, 3, targets=targets, weights=weights, old_token_scores=old_token_scores,
+                reference_token_scores=reference_token_scores)
+  low, high = _check_policy(what, logits, advantages, clip_range, clip_range_high, loss_normalizing_factor)
+  return token_losses.policy_loss(logits, targets, weights, old_token_scores, advantages, reference_token_scores,
+                                  low, high, float(kl_weight), loss_normalizing_factor)
+
+
+def policy_loss_from_token_scores(token_scores: torch.Tensor, weights: Optional[torch.Tensor],
+                                  old_token_scores: torch.Tensor, advantages: torch.Tensor,
+                                  reference_token_scores: Optional[torch.Tensor] = None, clip_range: float = 0.2,
+                                  clip_range_high: Optional[float] = None, kl_weight: float = 0.0,
+                                  loss_normalizing_factor=None):
+  """`compute_policy_loss` from log-probabilities of the targets [batch, length], differentiable in them (see
+  `preference_loss_from_token_scores`)."""
+  from t5x_b200.ops import token_losses
+  what = "policy_loss_from_token_scores"
+  _check_tokens(what, token_scores, 2, weights=weights, old_token_scores=old_token_scores,
+                reference_token_scores=reference_token_scores)
+  low, high = _check_policy(what, token_scores, advantages, clip_range, clip_range_high, loss_normalizing_factor)
+  return token_losses.policy_loss(token_scores, None, weights, old_token_scores, advantages,
+                                  reference_token_scores, low, high, float(kl_weight), loss_normalizing_factor)

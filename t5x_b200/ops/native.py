@@ -1195,3 +1195,108 @@ def adamw_group_(items: AdamwItems, state_bits: int, *, lr, b1, b2, eps, eps_roo
     _check(lib().t5x_adamw_group(ctypes.addressof(buf), count, state_bits, lr, b1, b2, eps, eps_root,
                                  weight_decay, step, seed & 0xFFFFFFFF, ptr(clip_scale), stream_ptr()),
            "adamw_group")
+
+
+# ----------------------------------------------------------------------------
+# Losses of preference and policy fine-tuning
+# ----------------------------------------------------------------------------
+register_signature("t5x_policy_loss", [c_void_p, c_int, c_void_p, c_ll, c_int, c_int, c_ll, c_ll] + [c_void_p] * 5 +
+                   [c_ll, c_ll] + [c_float] * 4 + [c_void_p] * 4)
+register_signature("t5x_policy_loss_tokens", [c_void_p, c_void_p, c_ll, c_int] + [c_void_p] * 4 + [c_ll, c_ll] +
+                   [c_float] * 4 + [c_void_p] * 4)
+register_signature("t5x_preference_loss_scratch_bytes", [c_ll, c_int])
+register_signature("t5x_preference_loss", [c_void_p, c_int, c_void_p, c_ll, c_int, c_int, c_ll, c_ll] + [c_void_p] * 3 +
+                   [c_float] * 3 + [c_void_p] * 6)
+register_signature("t5x_preference_loss_tokens", [c_void_p, c_void_p, c_ll, c_int, c_void_p, c_void_p] +
+                   [c_float] * 3 + [c_void_p] * 6)
+register_signature("t5x_scale_gradient", [c_void_p, c_void_p, c_ll, c_int, c_void_p, c_void_p])
+
+
+class _on_device_of:
+  """Makes a tensor's device the current one for a call."""
+
+  def __new__(cls, t: torch.Tensor):
+    return torch.cuda.device(t.device)
+
+
+def _loss_inputs(what: str, values, grad, targets, weights, *more):
+  """Raises unless the operands of a loss over [B, L(, V)] fit each other."""
+  shape, dev = values.shape[:2], values.device
+  ok = values.dtype in ((torch.float32, torch.bfloat16) if targets is not None else (torch.float32,))
+  ok = ok and values.dim() == (3 if targets is not None else 2)
+  ok = ok and (targets is not None or values.is_contiguous())
+  ok = ok and (targets is None or values.shape[2] == 1 or values.stride(2) == 1)
+  for t, dtype in [(targets, torch.int64), (weights, torch.float32)] + [(m, torch.float32) for m in more]:
+    ok = ok and (t is None or (t.dtype == dtype and t.shape == shape and t.device == dev and t.is_contiguous()))
+  ok = ok and (grad is None or (grad.shape == values.shape and grad.stride() == values.stride() and
+                                grad.dtype == values.dtype and grad.device == dev))
+  if not ok:
+    raise NativeError(f"{what}: operands must be tensors of one device whose types and shapes fit")
+
+
+def _loss_strides(t: torch.Tensor):
+  """Strides of batch and length; of a dimension of one, what it would be side by side."""
+  b, l, v = t.shape
+  st = t.stride(1) if l > 1 else v
+  return (t.stride(0) if b > 1 else (l - 1) * st + v), st
+
+
+def policy_loss(values, grad, targets, weights, old, advantages, reference, clip_low, clip_high, kl_weight, scale,
+                normalizer):
+  """(loss, kl, clipped, weight) as device scalars; the gradient in `grad` unless it is None. values: logits
+  [B, L, V], or log-probabilities [B, L] with targets None; advantages: [B, L] of any strides."""
+  _loss_inputs("policy_loss", values, grad, targets, weights, old, reference)
+  if advantages.shape != values.shape[:2] or advantages.dtype != torch.float32 or advantages.device != values.device:
+    raise NativeError("policy_loss: advantages must be fp32 of the batch's shape")
+  b, l = values.shape[:2]
+  with _on_device_of(values):
+    nbytes = lib().t5x_policy_loss_scratch_bytes
+    nbytes.restype = c_ll
+    scratch = torch.empty(nbytes(), dtype=torch.uint8, device=values.device)
+    out = torch.empty(4, dtype=torch.float32, device=values.device)
+    tail = (weights, old, reference, advantages)
+    tail = (*map(ptr, tail), advantages.stride(0), advantages.stride(1), clip_low, clip_high, kl_weight, scale,
+            ptr(normalizer), scratch.data_ptr(), out.data_ptr(), stream_ptr())
+    if targets is None:
+      rc = lib().t5x_policy_loss_tokens(values.data_ptr(), ptr(grad), b, l, *tail)
+    else:
+      rc = lib().t5x_policy_loss(values.data_ptr(), int(values.dtype == torch.float32), ptr(grad), b, l,
+                                 values.shape[2], *_loss_strides(values), targets.data_ptr(), *tail)
+  _check(rc, "policy_loss")
+  return tuple(o.clone() if i == 0 else o for i, o in enumerate(out.unbind(0)))
+
+
+def preference_loss(values, grad, targets, weights, reference, beta, label_smoothing, scale, normalizer):
+  """(loss, scores [B], margins [B / 2], pairs); values and grad as in `policy_loss`."""
+  _loss_inputs("preference_loss", values, grad, targets, weights)
+  b, l = values.shape[:2]
+  if reference.shape != (b,) or reference.dtype != torch.float32 or reference.device != values.device:
+    raise NativeError("preference_loss: reference scores must be fp32, one for each sequence")
+  with _on_device_of(values):
+    nbytes = lib().t5x_preference_loss_scratch_bytes
+    nbytes.restype = c_ll
+    scratch = torch.empty(nbytes(b, l), dtype=torch.uint8, device=values.device)
+    scores = torch.empty(b, dtype=torch.float32, device=values.device)
+    margins = torch.empty(b // 2, dtype=torch.float32, device=values.device)
+    out = torch.empty(2, dtype=torch.float32, device=values.device)
+    tail = (ptr(weights), reference.data_ptr(), beta, label_smoothing, scale, ptr(normalizer), scratch.data_ptr(),
+            scores.data_ptr(), margins.data_ptr(), out.data_ptr(), stream_ptr())
+    if targets is None:
+      rc = lib().t5x_preference_loss_tokens(values.data_ptr(), ptr(grad), b, l, *tail)
+    else:
+      rc = lib().t5x_preference_loss(values.data_ptr(), int(values.dtype == torch.float32), ptr(grad), b, l,
+                                     values.shape[2], *_loss_strides(values), targets.data_ptr(), *tail)
+  _check(rc, "preference_loss")
+  return out[0].clone(), scores, margins, out[1]
+
+
+def scale_gradient(grad: torch.Tensor, factor: torch.Tensor, keep: bool) -> torch.Tensor:
+  """grad * factor (a device scalar) in place, or, with `keep`, in memory of its own."""
+  out = grad
+  span = sum((n - 1) * s for n, s in zip(grad.shape, grad.stride())) + 1
+  if keep:
+    out = torch.empty(span, dtype=grad.dtype, device=grad.device).as_strided(grad.shape, grad.stride())
+  with _on_device_of(grad):
+    _check(lib().t5x_scale_gradient(grad.data_ptr(), out.data_ptr(), span, int(grad.dtype == torch.float32),
+                                    factor.data_ptr(), stream_ptr()), "scale_gradient")
+  return out

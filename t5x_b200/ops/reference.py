@@ -246,3 +246,70 @@ def dropout(x: torch.Tensor, rate: float, training: bool, broadcast_dims=(),
   keep = 1.0 - rate
   mask = torch.rand(shape, device=x.device, generator=generator) < keep
   return torch.where(mask, x / keep, torch.zeros_like(x))
+
+
+# ----------------------------------------------------------------------------
+# Losses of preference and policy fine-tuning
+# ----------------------------------------------------------------------------
+def _wide(t: torch.Tensor) -> torch.Tensor:
+  return t if t.dtype == torch.float64 else t.float()
+
+
+def token_log_probs(logits: torch.Tensor, targets: torch.Tensor,
+                    weights: Optional[torch.Tensor] = None) -> torch.Tensor:
+  """log softmax(logits)[target] in 32 bits; 0 for tokens of weight 0, whatever their logits hold."""
+  if weights is None:
+    return _wide(logits).log_softmax(-1).gather(-1, targets[..., None].long())[..., 0]
+  seen = weights != 0
+  x = torch.where(seen[..., None], _wide(logits), torch.zeros((), dtype=_wide(logits).dtype, device=logits.device))
+  at = torch.where(seen, targets.long(), torch.zeros_like(targets, dtype=torch.long))
+  logp = x.log_softmax(-1).gather(-1, at[..., None])[..., 0]
+  return torch.where(seen, logp, torch.zeros_like(logp))
+
+
+def _over_normalizer(loss: torch.Tensor, normalizer) -> torch.Tensor:
+  if normalizer is None:
+    return loss
+  return loss / (normalizer.detach().to(loss.device) if isinstance(normalizer, torch.Tensor) else normalizer)
+
+
+def policy_loss(logp, weights, old, advantages, reference, clip_low, clip_high, kl_weight, normalizer):
+  """(loss, kl, clipped, weight) from log-probabilities [B, L]:
+  sum w (kl_weight kl - min(A rho, A clip(rho, 1 - clip_low, 1 + clip_high))) / normalizer with
+  rho = exp(logp - old) and kl = exp(reference - logp) - 1 - (reference - logp)."""
+  logp = _wide(logp)
+  w = torch.ones_like(logp) if weights is None else weights.detach().to(logp.dtype)
+  seen, zero = w != 0, torch.zeros((), dtype=logp.dtype, device=logp.device)
+  adv = advantages.detach().to(logp.dtype)
+  adv = (adv[:, None] if adv.dim() == 1 else adv).expand(logp.shape)
+  pick = lambda t: torch.where(seen, t.detach().to(logp.dtype), zero)  # noqa: E731
+  logp, adv = torch.where(seen, logp, zero), pick(adv)
+  ratio = torch.exp(logp - pick(old))
+  gain, held = adv * ratio, adv * ratio.clamp(1.0 - clip_low, 1.0 + clip_high)
+  each, kl = -torch.minimum(gain, held), torch.zeros_like(logp)
+  if reference is not None:
+    apart = pick(reference) - logp
+    kl = torch.expm1(apart) - apart
+    each = each + kl_weight * kl
+  total = lambda t: torch.where(seen, t * w, zero).sum(dtype=torch.float64)  # noqa: E731
+  back = logp.dtype
+  return (_over_normalizer(total(each), normalizer).to(back), _over_normalizer(total(kl.detach()), normalizer).to(back),
+          total((held < gain).to(back)).to(back), w.sum(dtype=torch.float64).to(back))
+
+
+def preference_loss(logp, weights, reference, beta, label_smoothing, normalizer):
+  """(loss, scores, margins, pairs) from log-probabilities [B, L], rows 2j (preferred) and 2j + 1 a pair:
+  scores = sum_t w logp, margin = beta ((s_2j - r_2j) - (s_2j+1 - r_2j+1)),
+  loss = sum (1 - e) log(1 + exp(-margin)) + e log(1 + exp(margin)), over the normalizer. Pairs without a
+  token of weight are padding."""
+  logp = _wide(logp)
+  w = torch.ones_like(logp) if weights is None else weights.detach().to(logp.dtype)
+  seen, zero = w != 0, torch.zeros((), dtype=torch.float64, device=logp.device)
+  scores = torch.where(seen, logp.double() * w, zero).sum(-1)
+  real = seen.any(-1).view(-1, 2).any(-1)
+  apart = scores - torch.where(real.repeat_interleave(2), reference.detach().double(), zero)
+  margins = torch.where(real, beta * (apart[0::2] - apart[1::2]), zero)
+  loss = (1.0 - label_smoothing) * F.softplus(-margins) + label_smoothing * F.softplus(margins)
+  back = logp.dtype
+  return (_over_normalizer(torch.where(real, loss, zero).sum(), normalizer).to(back), scores.detach().to(back),
+          margins.detach().to(back), real.sum().to(back))

@@ -1,0 +1,143 @@
+"""Losses of preference and policy fine-tuning with their gradients.
+
+On CUDA, over bf16 or fp32 logits or fp32 log-probabilities, the kernels of csrc/token_losses.cu
+compute the loss and, where a gradient will be wanted, the gradient in the same pass; backward
+multiplies it by the gradient of the loss (which leaves it alone where that is 1). Anything else
+runs the PyTorch statements in :mod:`t5x_b200.ops.reference`.
+
+The arguments are those of `t5x_b200.losses`, which checks them.
+"""
+from __future__ import annotations
+
+from typing import Optional
+
+import torch
+
+from t5x_b200.ops import functional as F
+from t5x_b200.ops import native
+from t5x_b200.ops import reference as ref
+
+
+def _native_logits(logits: torch.Tensor) -> bool:
+  return logits.is_cuda and logits.dtype in (torch.bfloat16, torch.float32) and logits.numel() > 0
+
+
+def _rows_apart(logits: torch.Tensor) -> torch.Tensor:
+  """The logits as the kernels take them: values of a row side by side, rows in order and apart."""
+  (b, l, v), (sb, st, sv) = logits.shape, logits.stride()
+  if (sv == 1 or v == 1) and (l == 1 or st >= v) and (b == 1 or sb >= (l - 1) * st + v):
+    return logits
+  return logits.contiguous()
+
+
+def _like(logits: torch.Tensor) -> torch.Tensor:
+  """Memory for the gradient of `logits`: the same strides, at the same place of 16 bytes, so that the
+  kernel's wide accesses fall on the same values of both."""
+  size = logits.element_size()
+  behind = logits.data_ptr() % 16 // size
+  span = sum((n - 1) * s for n, s in zip(logits.shape, logits.stride())) + 1
+  flat = torch.empty(span + behind, dtype=logits.dtype, device=logits.device)
+  return flat.as_strided(logits.shape, logits.stride(), behind)
+
+
+def _times(grad: torch.Tensor, factor: torch.Tensor) -> torch.Tensor:
+  """The saved gradient times the gradient of the loss."""
+  return native.scale_gradient(grad, factor.detach().float().reshape(1), keep=F._graph_is_kept())
+
+
+class _PolicyFn(torch.autograd.Function):
+
+  @staticmethod
+  def forward(ctx, values, targets, weights, old, advantages, reference, cfg):
+    want = not isinstance(ctx, F._NoGraph) and ctx.needs_input_grad[0]
+    if targets is not None:
+      values = _rows_apart(values)
+      grad = _like(values) if want else None
+    else:
+      values = values.contiguous()
+      grad = torch.empty_like(values) if want else None
+    out = native.policy_loss(values, grad, targets, weights, old, advantages, reference, *cfg)
+    ctx.save_for_backward(grad)
+    ctx.mark_non_differentiable(*out[1:])
+    return out
+
+  @staticmethod
+  @torch.autograd.function.once_differentiable
+  def backward(ctx, by, *_):
+    return (_times(ctx.saved_tensors[0], by),) + (None,) * 6
+
+
+class _PreferenceFn(torch.autograd.Function):
+
+  @staticmethod
+  def forward(ctx, values, targets, weights, reference, cfg):
+    want = not isinstance(ctx, F._NoGraph) and ctx.needs_input_grad[0]
+    if targets is not None:
+      values = _rows_apart(values)
+      grad = _like(values) if want else None
+    else:
+      values = values.contiguous()
+      grad = torch.empty_like(values) if want else None
+    out = native.preference_loss(values, grad, targets, weights, reference, *cfg)
+    ctx.save_for_backward(grad)
+    ctx.mark_non_differentiable(*out[1:])
+    return out
+
+  @staticmethod
+  @torch.autograd.function.once_differentiable
+  def backward(ctx, by, *_):
+    return (_times(ctx.saved_tensors[0], by),) + (None,) * 4
+
+
+def _plain(t: Optional[torch.Tensor], dtype=torch.float32) -> Optional[torch.Tensor]:
+  """A contiguous tensor of the type, without its graph."""
+  if t is None:
+    return None
+  if t.requires_grad:
+    t = t.detach()
+  return t if t.dtype == dtype and t.is_contiguous() else t.to(dtype).contiguous()
+
+
+def _divisor(factor, device):
+  """(1 / factor, None), or (1, the factor as a device scalar)."""
+  if factor is None:
+    return 1.0, None
+  if isinstance(factor, torch.Tensor) and factor.numel() == 1 and factor.device.type != "cpu":
+    return 1.0, _plain(factor.reshape(1).to(device))
+  return 1.0 / float(factor), None
+
+
+def policy_loss(values, targets, weights, old, advantages, reference, clip_low, clip_high, kl_weight,
+                normalizer):
+  """(loss, kl, clipped, weight); values: logits [B, L, V], or log-probabilities [B, L] with targets
+  None."""
+  if targets is None:
+    native_ok = values.is_cuda and values.dtype == torch.float32 and values.numel() > 0
+  else:
+    native_ok = _native_logits(values)
+  if not native_ok:
+    logp = values if targets is None else ref.token_log_probs(values, targets, weights)
+    return ref.policy_loss(logp, weights, old, advantages, reference, clip_low, clip_high, kl_weight,
+                           normalizer)
+  scale, divisor = _divisor(normalizer, values.device)
+  b, l = values.shape[:2]
+  advantages = _plain(advantages)
+  if advantages.dim() == 1:
+    advantages = advantages[:, None]
+  return F._apply(_PolicyFn, values, _plain(targets, torch.int64), _plain(weights), _plain(old),
+                  advantages.expand(b, l), _plain(reference),
+                  (clip_low, clip_high, kl_weight, scale, divisor))
+
+
+def preference_loss(values, targets, weights, reference, beta, label_smoothing, normalizer):
+  """(loss, scores, margins, pairs); values as in `policy_loss`, rows 2j and 2j + 1 a pair."""
+  if targets is None:
+    native_ok = values.is_cuda and values.dtype == torch.float32 and values.numel() > 0
+  else:
+    native_ok = _native_logits(values)
+  if not native_ok:
+    logp = values if targets is None else ref.token_log_probs(values, targets, weights)
+    return ref.preference_loss(logp, weights, reference, beta, label_smoothing, normalizer)
+  scale, divisor = _divisor(normalizer, values.device)
+  return F._apply(_PreferenceFn, values, _plain(targets, torch.int64), _plain(weights),
+                  _plain(reference), (beta, label_smoothing, scale, divisor))
