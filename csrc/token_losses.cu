@@ -19,6 +19,7 @@
 //
 // What bounds it: memory; the logits that count read once, the gradient written once.
 #include <cmath>
+#include <type_traits>
 
 #include "common.cuh"
 #include "t5x_ops.h"
@@ -173,54 +174,15 @@ __device__ __forceinline__ float log_prob(const T* row, int vocab, long long tar
   return (Pack<T>::one(row[target]) - s.most) - log1pf(s.sum - 1.f);
 }
 
-// The rows are walked by teams: warps for short rows, whole CTAs for long ones.
-template <int kTeam>
-struct Team {
-  int tid, id, count;
-  __device__ Team()
-      : tid(kTeam == 32 ? threadIdx.x & 31 : threadIdx.x),
-        id(kTeam == 32 ? (blockIdx.x * blockDim.x + threadIdx.x) >> 5 : blockIdx.x),
-        count(kTeam == 32 ? (gridDim.x * blockDim.x) >> 5 : gridDim.x) {}
-  // The whole row's softmax; valid in the first warp of the team.
-  __device__ Softmax reduce(Softmax s) const {
+// The softmax of what the 32 lanes have seen, in every lane.
+__device__ __forceinline__ Softmax join_lanes(Softmax s) {
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      const Softmax other = {__shfl_xor_sync(0xffffffffu, s.most, o), __shfl_xor_sync(0xffffffffu, s.sum, o)};
-      s = join(s, other);
-    }
-    if (kTeam > 32) {
-      __shared__ Softmax part[kTeam / 32];
-      if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = s;
-      __syncthreads();
-      if (threadIdx.x < 32) {
-        s = threadIdx.x < kTeam / 32 ? part[threadIdx.x] : Softmax{-INFINITY, 0.f};
-#pragma unroll
-        for (int o = kTeam / 64; o > 0; o >>= 1) {
-          const Softmax other = {__shfl_xor_sync(0xffffffffu, s.most, o), __shfl_xor_sync(0xffffffffu, s.sum, o)};
-          s = join(s, other);
-        }
-      }
-    }
-    return s;
+  for (int o = 16; o > 0; o >>= 1) {
+    const Softmax other = {__shfl_xor_sync(0xffffffffu, s.most, o), __shfl_xor_sync(0xffffffffu, s.sum, o)};
+    s = join(s, other);
   }
-  // v of the team's first thread.
-  template <typename V>
-  __device__ V broadcast(V v) const {
-    if (kTeam == 32) {
-      int w[sizeof(V) / 4];
-      memcpy(w, &v, sizeof(V));
-#pragma unroll
-      for (int i = 0; i < static_cast<int>(sizeof(V) / 4); ++i) w[i] = __shfl_sync(0xffffffffu, w[i], 0);
-      memcpy(&v, w, sizeof(V));
-      return v;
-    }
-    __shared__ V s;
-    __syncthreads();  // (the last row's is read)
-    if (threadIdx.x == 0) s = v;
-    __syncthreads();
-    return s;
-  }
-};
+  return s;
+}
 
 struct Rows {
   long long rows;  // B * L
@@ -317,45 +279,36 @@ __device__ __forceinline__ void policy_finish(double* sums, const Policy& p, dou
   }
 }
 
-template <typename T, int kTeam>
+// Short rows, a warp each.
+template <typename T>
 __global__ void __launch_bounds__(kRowThreads)
-    policy_rows_kernel(const T* __restrict__ logits, T* __restrict__ grad, const Rows r, const Policy p,
-                       double* partial, unsigned* arrived, float* out) {
-  const Team<kTeam> team;
+    policy_short_rows_kernel(const T* __restrict__ logits, T* __restrict__ grad, const Rows r, const Policy p,
+                             double* partial, unsigned* arrived, float* out) {
+  const int lane = threadIdx.x & 31;
+  const long long warps = static_cast<long long>(gridDim.x) * (kRowThreads / 32);
   const float scale = scale_of(p.normalizer, p.scale);
   double sums[4] = {0.0, 0.0, 0.0, 0.0};
-  for (long long row = team.id; row < r.rows; row += team.count) {
+  for (long long row = blockIdx.x * static_cast<long long>(kRowThreads / 32) + (threadIdx.x >> 5); row < r.rows;
+       row += warps) {
     const float w = r.weights != nullptr ? r.weights[row] : 1.f;
     const long long at = row_at(r, row);
     if (w == 0.f) {
-      if (grad != nullptr) row_zero(grad + at, r.vocab, team.tid, kTeam);
+      if (grad != nullptr) row_zero(grad + at, r.vocab, lane, 32);
       continue;
     }
-    struct Said {
-      Softmax s;
-      float by;
-      int target;
-    } said = {team.reduce(row_softmax(logits + at, r.vocab, team.tid, kTeam)), 0.f, 0};
-    if (team.tid == 0) {
-      const long long target = r.targets[row], b = row / r.length;
-      const float logp = log_prob(logits + at, r.vocab, target, said.s);
-      const PolicyToken k = policy_token(p, row, b, row - b * r.length, logp);
+    const long long target = r.targets[row], b = row / r.length;
+    const Softmax s = join_lanes(row_softmax(logits + at, r.vocab, lane, 32));
+    const float logp = log_prob(logits + at, r.vocab, target, s);
+    const PolicyToken k = policy_token(p, row, b, row - b * r.length, logp);
+    if (lane == 0) {
       sums[0] += static_cast<double>(w) * k.loss;
       sums[1] += static_cast<double>(w) * k.kl;
       sums[2] += static_cast<double>(w) * k.clipped;
       sums[3] += w;
-      said.by = w * k.slope * scale;
-      said.target = target >= 0 && target < r.vocab ? static_cast<int>(target) : -1;
     }
-    if (grad == nullptr) {
-      if (kTeam > 32) __syncthreads();  // (the partial sums are read)
-      continue;
-    }
-    said = team.broadcast(said);
-    if (said.by == 0.f)
-      row_zero(grad + at, r.vocab, team.tid, kTeam);
-    else
-      row_gradient(logits + at, grad + at, r.vocab, said.s, said.target, said.by, team.tid, kTeam);
+    if (grad != nullptr)
+      row_gradient(logits + at, grad + at, r.vocab, s,
+                   target >= 0 && target < r.vocab ? static_cast<int>(target) : -1, w * k.slope * scale, lane, 32);
   }
   policy_finish(sums, p, partial, arrived, out);
 }
@@ -391,21 +344,41 @@ struct Preference {
   const float* normalizer;
 };
 
-template <typename T, int kTeam>
+// Short rows, a warp each: softmax and log-probability.
+template <typename T>
 __global__ void __launch_bounds__(kRowThreads)
-    preference_rows_kernel(const T* __restrict__ logits, const Rows r, Softmax* __restrict__ softmax,
-                           float* __restrict__ logp) {
-  const Team<kTeam> team;
-  for (long long row = team.id; row < r.rows; row += team.count) {
+    preference_short_rows_kernel(const T* __restrict__ logits, const Rows r, Softmax* __restrict__ softmax,
+                                 float* __restrict__ logp) {
+  const int lane = threadIdx.x & 31;
+  const long long warps = static_cast<long long>(gridDim.x) * (kRowThreads / 32);
+  for (long long row = blockIdx.x * static_cast<long long>(kRowThreads / 32) + (threadIdx.x >> 5); row < r.rows;
+       row += warps) {
     if (r.weights != nullptr && r.weights[row] == 0.f) continue;
     const long long at = row_at(r, row);
-    const Softmax s = team.reduce(row_softmax(logits + at, r.vocab, team.tid, kTeam));
-    if (team.tid == 0) {
+    const Softmax s = join_lanes(row_softmax(logits + at, r.vocab, lane, 32));
+    if (lane == 0) {
       softmax[row] = s;
       logp[row] = log_prob(logits + at, r.vocab, r.targets[row], s);
     }
-    if (kTeam > 32) __syncthreads();  // (the partial sums are read)
   }
+}
+
+struct Margin {
+  double margin, loss, slope;  // slope: dloss / d(score of the preferred)
+};
+__device__ __forceinline__ Margin pair_margin(const Preference& p, bool real, double s0, double s1, float r0, float r1,
+                                              double scale) {
+  Margin m = {0.0, 0.0, 0.0};
+  if (!real) return m;
+  m.margin = p.beta * ((s0 - r0) - (s1 - r1));
+  // log(1 + exp(-d)) = log1p(exp(-|d|)) + max(-d, 0)
+  const double e = exp(-fabs(m.margin)), tail = log1p(e);
+  const double sigmoid = m.margin >= 0.0 ? 1.0 / (1.0 + e) : e / (1.0 + e);
+  m.loss = m.margin != m.margin ? m.margin
+                                : (1.0 - p.smoothing) * (tail + fmax(-m.margin, 0.0)) +
+                                      p.smoothing * (tail + fmax(m.margin, 0.0));
+  m.slope = p.beta * (sigmoid - (1.0 - p.smoothing)) * scale;
+  return m;
 }
 
 // A CTA per pair: scores, margin, the pair's loss, the slopes of its two sequences (and, from
@@ -430,26 +403,17 @@ __global__ void __launch_bounds__(kRowThreads)
     sum[side] = cta_sum<kRowThreads>(sum[side]);
   }
   const bool real = cta_sum<kRowThreads>(seen) > 0.0;
-  const double margin =
-      real ? p.beta * ((sum[0] - p.ref[2 * pair]) - (sum[1] - p.ref[2 * pair + 1])) : 0.0;
-  // log(1 + exp(-d)) = log1p(exp(-|d|)) + max(-d, 0)
-  const double e = exp(-fabs(margin)), tail = log1p(e);
-  const double sigmoid = margin >= 0.0 ? 1.0 / (1.0 + e) : e / (1.0 + e);
-  const double slope = real ? p.beta * (sigmoid - (1.0 - p.smoothing)) * scale : 0.0;
+  const Margin m = pair_margin(p, real, sum[0], sum[1], p.ref[2 * pair], p.ref[2 * pair + 1], scale);
+  const double slope = m.slope;
   if (threadIdx.x == 0) {
-    double loss = 0.0;
-    if (real)
-      loss = margin != margin ? margin
-                              : (1.0 - p.smoothing) * (tail + fmax(-margin, 0.0)) +
-                                    p.smoothing * (tail + fmax(margin, 0.0));
     scores[2 * pair] = static_cast<float>(sum[0]);
     scores[2 * pair + 1] = static_cast<float>(sum[1]);
-    margins[pair] = static_cast<float>(margin);
+    margins[pair] = static_cast<float>(m.margin);
     if (by != nullptr) {
       by[2 * pair] = static_cast<float>(slope);
       by[2 * pair + 1] = static_cast<float>(-slope);
     }
-    pair_loss[2 * pair] = loss;
+    pair_loss[2 * pair] = m.loss;
     pair_loss[2 * pair + 1] = real ? 1.0 : 0.0;
   }
   if (token_slope != nullptr) {
@@ -477,23 +441,623 @@ __global__ void __launch_bounds__(kRowThreads)
   }
 }
 
-template <typename T, int kTeam>
+template <typename T>
 __global__ void __launch_bounds__(kRowThreads)
-    preference_gradient_kernel(const T* __restrict__ logits, T* __restrict__ grad, const Rows r,
-                               const Softmax* __restrict__ softmax, const float* __restrict__ by) {
-  const Team<kTeam> team;
-  for (long long row = team.id; row < r.rows; row += team.count) {
+    preference_short_gradient_kernel(const T* __restrict__ logits, T* __restrict__ grad, const Rows r,
+                                     const Softmax* __restrict__ softmax, const float* __restrict__ by) {
+  const int lane = threadIdx.x & 31;
+  const long long warps = static_cast<long long>(gridDim.x) * (kRowThreads / 32);
+  for (long long row = blockIdx.x * static_cast<long long>(kRowThreads / 32) + (threadIdx.x >> 5); row < r.rows;
+       row += warps) {
     const float w = r.weights != nullptr ? r.weights[row] : 1.f;
     const long long at = row_at(r, row);
-    const float slope = w == 0.f ? 0.f : w * by[row / r.length];
-    if (slope == 0.f) {
-      row_zero(grad + at, r.vocab, team.tid, kTeam);
+    if (w == 0.f) {
+      row_zero(grad + at, r.vocab, lane, 32);
       continue;
     }
     const long long target = r.targets[row];
     row_gradient(logits + at, grad + at, r.vocab, softmax[row],
-                 target >= 0 && target < r.vocab ? static_cast<int>(target) : -1, slope, team.tid, kTeam);
+                 target >= 0 && target < r.vocab ? static_cast<int>(target) : -1, w * by[row / r.length], lane, 32);
   }
+}
+
+// ---- long rows ----
+// A CTA's producer thread copies the rows in tiles of 16 KB into a ring in shared memory, in the order
+// in which the worker warps take them, far ahead of them; so the loads go on while a row's sums meet.
+// Each tile goes by twice, for the softmax and for the gradient, the second time out of L2. A keeper warp
+// makes of the workers' sums what the gradient needs, so that no worker waits for a load of a single
+// value, a logarithm or another CTA.
+//
+// policy: row after row, the gradient of one behind the softmax of the next.
+// preference: the slope needs the sums of all rows of a pair. The tasks (a row's softmax, a row's gradient)
+// stand in an order in which a group of pairs is followed by the next group's softmaxes and then its own
+// gradients; a CTA takes the next task by a ticket. What a gradient waits for has smaller tickets, is
+// therefore done or under way, and waits itself for smaller tickets at most.
+constexpr int kWorkers = 256;
+constexpr int kWorkerWarps = kWorkers / 32;
+constexpr int kLongThreads = kWorkers + 64;
+constexpr int kTileBytes = 16384;
+constexpr int kStages = 6;
+constexpr int kSlots = 16;  // rows between their sums and their gradient: at most the ring's tiles and two
+
+enum Kind : int { kEnd, kStat, kGrad, kZero, kSkip };
+struct Tile {
+  long long row;
+  int kind;
+  int at, packs;  // first 16 bytes of the row's aligned part, how many
+  int last;
+};
+// What the gradient of a row needs: by * onehot(target) + k * exp(x - most) with k = -by / sum.
+struct Slope {
+  float most, by, k;
+  int target;
+};
+struct LongShared {
+  alignas(128) unsigned char data[kStages][kTileBytes];
+  uint64_t full[kStages], empty[kStages], sums[kSlots], said[kSlots];
+  Tile tile[kStages];
+  Softmax part[kSlots][kWorkerWarps];
+  Slope slope[kSlots];
+  int abort;
+};
+
+// The part of a row between 16-byte boundaries.
+template <typename T>
+__device__ __forceinline__ void aligned_part(const T* row, int vocab, int& head, int& packs) {
+  constexpr int kN = Pack<T>::kN;
+  const int off = static_cast<int>(reinterpret_cast<uintptr_t>(row) & 15) / static_cast<int>(sizeof(T));
+  head = off ? kN - off : 0;
+  packs = (vocab - head) / kN;
+}
+
+struct Order {
+  long long rows, group;  // rows of the batch, of a group of pairs
+  bool behind;            // a group's gradients follow the next group's softmaxes
+  bool gradient;
+};
+// (row, is it the gradient's turn) of a ticket below rows * (1 + gradient)
+__device__ __forceinline__ long long task_of(const Order& o, long long ticket, bool& gradient) {
+  gradient = false;
+  if (!o.gradient) return ticket;
+  const long long last = (o.rows - 1) / o.group * o.group;  // first row of the last group
+  if (!o.behind) {  // softmaxes of a group, then its gradients, those last read first
+    const long long k = ticket / (2 * o.group), first = k * o.group, at = ticket - 2 * first;
+    const long long n = o.rows - first < o.group ? o.rows - first : o.group;
+    gradient = at >= n;
+    return gradient ? first + 2 * n - 1 - at : first + at;
+  }
+  gradient = ticket >= o.rows + last;
+  if (gradient) return ticket - o.rows;  // of the last group
+  if (ticket < o.group) return ticket;
+  const long long k = (ticket - o.group) / (2 * o.group) + 1;  // softmaxes of group k, gradients of k - 1
+  const long long at = ticket - o.group - (k - 1) * 2 * o.group, first = k * o.group;
+  const long long n = o.rows - first < o.group ? o.rows - first : o.group;
+  gradient = at >= n;
+  return gradient ? first - o.group + (at - n) : first + at;
+}
+
+struct Work {
+  unsigned long long* ticket;
+  unsigned *done, *pairs_done;  // done: rows of the pair whose softmax is there (or that do not count)
+  Softmax* softmax;
+  float* logp;
+  double* pair_loss;
+  float *scores, *margins;
+  Order order;
+};
+
+// Two values at once where the arithmetic has pairs.
+__device__ __forceinline__ uint64_t pair_of(float a, float b) {
+  uint64_t d;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(a), "f"(b));
+  return d;
+}
+__device__ __forceinline__ void split(uint64_t d, float& a, float& b) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(d));
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.ftz.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("add.rn.ftz.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("mul.rn.ftz.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+
+// In the tiles an exponential exp(x - most) is exp2(x log2 e - ref), a fused product and difference, with
+// ref = most log2 e as rounded: the same factor for the sum, the target and the gradient. Where a largest
+// logit's product may overflow, it is exp2((x - most) log2 e).
+constexpr float kHuge = 1.0e38f;
+__device__ __forceinline__ bool huge(float most) { return !(fabsf(most) <= kHuge); }  // (NaN and -inf too)
+// log2 of exp(a - b); 0 for a = b = -inf
+__device__ __forceinline__ float shift(float a, float b) {
+  if (huge(a) || huge(b)) return a == b ? 0.f : (a - b) * kLog2e;
+  return __fmul_rn(a, kLog2e) - __fmul_rn(b, kLog2e);
+}
+__device__ __forceinline__ float exp_from(float x, float most) {
+  return exp2_approx(huge(most) ? (x - (most == -INFINITY ? 0.f : most)) * kLog2e
+                                : fmaf(x, kLog2e, -__fmul_rn(most, kLog2e)));
+}
+__device__ __forceinline__ Softmax join_rows(Softmax a, Softmax b) {
+  const float m = fmaxf(a.most, b.most);
+  return {m, a.sum * exp2_approx(shift(a.most, m)) + b.sum * exp2_approx(shift(b.most, m))};
+}
+__device__ __forceinline__ Softmax join_row_lanes(Softmax s) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1)
+    s = join_rows(s, {__shfl_xor_sync(0xffffffffu, s.most, o), __shfl_xor_sync(0xffffffffu, s.sum, o)});
+  return s;
+}
+__device__ __forceinline__ float log_prob_of(float x, Softmax s) {
+  if (s.most == -INFINITY) return NAN;
+  const float d = huge(s.most) ? x - s.most : fmaf(x, kLog2e, -__fmul_rn(s.most, kLog2e)) * 0.6931471805599453f;
+  return d - log1pf(s.sum - 1.f);
+}
+
+// 16 bytes of the tile, as pairs
+template <typename T>
+struct Pairs;
+template <>
+struct Pairs<float> {
+  uint64_t v[2];
+  __device__ void load(const void* p) {
+    const float4 x = *static_cast<const float4*>(p);
+    v[0] = pair_of(x.x, x.y), v[1] = pair_of(x.z, x.w);
+  }
+  __device__ float most() const {
+    float a, b, c, d;
+    split(v[0], a, b), split(v[1], c, d);
+    return fmaxf(fmaxf(a, b), fmaxf(c, d));
+  }
+};
+template <>
+struct Pairs<__nv_bfloat16> {
+  uint64_t v[4];
+  float top;
+  __device__ void load(const void* p) {
+    const uint4 x = *static_cast<const uint4*>(p);
+    const uint32_t u[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = pair_of(__uint_as_float(u[i] << 16), __uint_as_float(u[i] & 0xffff0000u));
+    const __nv_bfloat162 m = __hmax2(__hmax2(as2(u[0]), as2(u[1])), __hmax2(as2(u[2]), as2(u[3])));
+    top = fmaxf(__low2float(m), __high2float(m));
+  }
+  __device__ static __nv_bfloat162 as2(uint32_t u) { return *reinterpret_cast<__nv_bfloat162*>(&u); }
+  __device__ float most() const { return top; }
+};
+
+// Adds a thread's 16 bytes each to the softmax of what it has seen.
+template <typename T, int kPacks>
+__device__ __forceinline__ void take(Softmax& s, const Pairs<T>* x) {
+  constexpr int kPairsOf = sizeof(Pairs<T>::v) / 8;
+  float m = x[0].most();
+#pragma unroll
+  for (int i = 1; i < kPacks; ++i) m = fmaxf(m, x[i].most());
+  if (m > s.most) {
+    s.sum *= exp2_approx(shift(s.most, m));
+    s.most = m;
+  }
+  uint64_t t = pair_of(0.f, 0.f);
+  if (!huge(s.most)) {
+    const float ref = __fmul_rn(s.most, kLog2e);
+    const uint64_t l2e = pair_of(kLog2e, kLog2e), off = pair_of(-ref, -ref);
+#pragma unroll
+    for (int i = 0; i < kPacks; ++i) {
+#pragma unroll
+      for (int j = 0; j < kPairsOf; ++j) {
+        float a, b;
+        split(fma2(x[i].v[j], l2e, off), a, b);
+        t = add2(t, pair_of(exp2_approx(a), exp2_approx(b)));
+      }
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < kPacks; ++i) {
+#pragma unroll
+      for (int j = 0; j < kPairsOf; ++j) {
+        float a, b;
+        split(x[i].v[j], a, b);
+        t = add2(t, pair_of(exp_from(a, s.most), exp_from(b, s.most)));
+      }
+    }
+  }
+  float a, b;
+  split(t, a, b);
+  s.sum += a + b;
+}
+
+template <typename T, bool kPairs>
+__global__ void __launch_bounds__(kLongThreads, 2)
+    long_rows_kernel(const T* __restrict__ logits, T* __restrict__ grad, const Rows r, const Policy p,
+                     const Preference q, const Work work, double* partial, unsigned* arrived, float* out,
+                     int* status) {
+  constexpr int kN = Pack<T>::kN;
+  constexpr int kTilePacks = kTileBytes / 16;
+  extern __shared__ __align__(128) unsigned char raw[];
+  LongShared& sh = *reinterpret_cast<LongShared*>(raw);
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  if (tid == 0) {
+    for (int i = 0; i < kStages; ++i) {
+      mbar_init(&sh.full[i], 1);
+      mbar_init(&sh.empty[i], kWorkerWarps + 1);
+    }
+    for (int i = 0; i < kSlots; ++i) {
+      mbar_init(&sh.sums[i], kWorkerWarps);
+      mbar_init(&sh.said[i], 1);
+    }
+    sh.abort = 0;
+    mbar_fence_init();
+  }
+  __syncthreads();
+  volatile int* abort = &sh.abort;
+  int stage = 0;
+  uint32_t round = 0;
+  bool ok = true;
+  auto advance = [&] {
+    if (++stage == kStages) stage = 0, ++round;
+  };
+  auto wait = [&](uint64_t* bar, uint32_t parity) {  // the whole warp's
+    ok = __all_sync(0xffffffffu, mbar_wait(bar, parity, abort));
+    return ok;
+  };
+  auto give_up = [&](int code) {
+    if (lane == 0) {
+      *abort = 1;
+      report_status(status, code, 41, warp);
+    }
+  };
+
+  if (warp == kWorkerWarps) {  // ---- producer ----
+    int issued = 0;
+    auto push = [&](const Tile& t, const void* src) {  // (one thread's)
+      if (!ok || !mbar_wait(&sh.empty[stage], (round & 1) ^ 1, abort)) {
+        ok = false;
+        return;
+      }
+      sh.tile[stage] = t;
+      if (src != nullptr) {
+        mbar_expect_tx(&sh.full[stage], t.packs * 16);
+        bulk_load(sh.data[stage], src, t.packs * 16, &sh.full[stage]);
+      } else {
+        mbar_arrive(&sh.full[stage]);
+      }
+      ++issued;
+      advance();
+    };
+    auto stream = [&](int kind, long long row) {
+      const T* x = logits + row_at(r, row);
+      int head, packs;
+      aligned_part(x, r.vocab, head, packs);
+      for (int at = 0; at < packs && ok; at += kTilePacks) {
+        const int n = packs - at < kTilePacks ? packs - at : kTilePacks;
+        push({row, kind, at, n, at + n == packs}, x + head + static_cast<long long>(at) * kN);
+      }
+    };
+    if (kPairs) {
+      if (lane == 0) {
+        const unsigned long long total = work.order.rows * (work.order.gradient ? 2 : 1);
+        auto weight = [&](unsigned long long t) {
+          bool g;
+          return t < total && r.weights != nullptr ? r.weights[task_of(work.order, t, g)] : 1.f;
+        };
+        unsigned long long ticket = atomicAdd(work.ticket, 1ull);
+        float w = weight(ticket);
+        while (ok && ticket < total) {
+          const unsigned long long next = atomicAdd(work.ticket, 1ull);  // (one ahead: the answer takes its time)
+          bool gradient;
+          const long long row = task_of(work.order, ticket, gradient);
+          if (w == 0.f)
+            push({row, gradient ? kZero : kSkip, 0, 0, 1}, nullptr);
+          else
+            stream(gradient ? kGrad : kStat, row);
+          ticket = next;
+          w = weight(ticket);
+        }
+      }
+    } else {
+      long long before = -1;  // the row whose gradient is still to come
+      for (long long base = blockIdx.x; base < r.rows; base += 32ll * gridDim.x) {
+        const long long mine = base + static_cast<long long>(lane) * gridDim.x;
+        const float w = mine < r.rows && r.weights != nullptr ? r.weights[mine] : 1.f;
+        const unsigned visible = __ballot_sync(0xffffffffu, w != 0.f);
+        if (lane == 0) {
+          for (int i = 0; i < 32; ++i) {
+            const long long row = base + static_cast<long long>(i) * gridDim.x;
+            if (row >= r.rows || !ok) break;
+            if (visible >> i & 1) {
+              stream(kStat, row);
+              if (grad != nullptr && before >= 0) stream(kGrad, before);
+              before = row;
+            } else if (grad != nullptr) {
+              push({row, kZero, 0, 0, 1}, nullptr);
+            }
+          }
+        }
+        __syncwarp();
+      }
+      if (lane == 0 && grad != nullptr && before >= 0) stream(kGrad, before);
+    }
+    if (lane == 0) {
+      push({0, kEnd, 0, 0, 1}, nullptr);
+      if (!ok) {  // no copy may be under way when the shared memory is given back
+        give_up(kStatusTimeoutProducer);
+        const int n = issued < kStages ? issued : kStages;
+        for (int i = issued - n; i < issued; ++i)
+          for (uint32_t it = 0; it < kWaitLimit && !mbar_try_wait(&sh.full[i % kStages], (i / kStages) & 1); ++it) {
+          }
+      }
+    }
+    return;
+  }
+
+  unsigned rows_summed = 0, rows_turned = 0;  // softmaxes and gradients so far
+  if (warp > kWorkerWarps) {  // ---- keeper ----
+    const float scale = kPairs ? 0.f : scale_of(p.normalizer, p.scale);
+    double sums[4] = {0.0, 0.0, 0.0, 0.0};
+    float w = 0.f, x = 0.f;  // weight and target's logit of the row under way
+    long long target = -1, known = -1;
+    float slope0 = 0.f;  // of the preferred row of the known pair
+    while (wait(&sh.full[stage], round & 1)) {
+      const Tile t = sh.tile[stage];
+      if (t.kind == kEnd) break;
+      const long long b = t.row / r.length;
+      if (t.kind == kStat) {
+        if (t.at == 0 && lane == 0) {  // (asked for while the row is summed)
+          const T* row = logits + row_at(r, t.row);
+          target = r.targets[t.row];
+          w = r.weights != nullptr ? r.weights[t.row] : 1.f;
+          x = target >= 0 && target < r.vocab ? Pack<T>::one(row[target]) : NAN;
+        }
+        if (t.last) {
+          const int slot = rows_summed % kSlots;
+          if (!wait(&sh.sums[slot], rows_summed / kSlots & 1)) break;
+          const Softmax s = join_row_lanes(lane < kWorkerWarps ? sh.part[slot][lane] : Softmax{-INFINITY, 0.f});
+          if (lane == 0) {
+            const float logp = log_prob_of(x, s);
+            if (kPairs) {
+              work.softmax[t.row] = s;
+              work.logp[t.row] = logp;
+              red_release_gpu_add(work.done + b / 2, 1u);
+            } else {
+              const PolicyToken c = policy_token(p, t.row, b, t.row - b * r.length, logp);
+              sums[0] += static_cast<double>(w) * c.loss;
+              sums[1] += static_cast<double>(w) * c.kl;
+              sums[2] += static_cast<double>(w) * c.clipped;
+              sums[3] += w;
+              const float by = w * c.slope * scale;
+              sh.slope[slot] = {s.most, by, -by / s.sum,
+                                target >= 0 && target < r.vocab ? static_cast<int>(target) : -1};
+              mbar_arrive(&sh.said[slot]);
+            }
+          }
+          ++rows_summed;
+        }
+      } else if (kPairs && t.at == 0) {
+        const long long pair = b / 2;
+        if (t.kind == kSkip) {
+          if (lane == 0) red_release_gpu_add(work.done + pair, 1u);
+        } else {
+          const bool turned = t.kind == kGrad;
+          const bool writes = t.row == pair * 2 * r.length;  // one row of a pair writes what the pair gives
+          if (pair != known && (turned || writes)) {
+            uint32_t it = 0;
+            while (ld_acquire_gpu(work.done + pair) != 2u * r.length) {
+              if (++it == kWaitLimit || *abort) {
+                ok = false;
+                break;
+              }
+              __nanosleep(20);
+            }
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) break;
+            double sum[2] = {0.0, 0.0};
+            bool seen = false;
+#pragma unroll
+            for (int side = 0; side < 2; ++side) {
+              const long long first = (2 * pair + side) * r.length;
+#pragma unroll 4
+              for (int i = lane; i < r.length; i += 32) {
+                const float wt = r.weights != nullptr ? r.weights[first + i] : 1.f;
+                const float lp = __ldcg(work.logp + first + i);
+                if (wt != 0.f) {
+                  sum[side] += static_cast<double>(wt) * lp;
+                  seen = true;
+                }
+              }
+#pragma unroll
+              for (int o = 16; o > 0; o >>= 1) sum[side] += __shfl_xor_sync(0xffffffffu, sum[side], o);
+            }
+            const bool real = __any_sync(0xffffffffu, seen);
+            const Margin m = pair_margin(q, real, sum[0], sum[1], q.ref[2 * pair], q.ref[2 * pair + 1],
+                                         scale_of(q.normalizer, q.scale));
+            slope0 = static_cast<float>(m.slope);
+            known = pair;
+            if (writes) {
+              unsigned before = 0;
+              if (lane == 0) {
+                work.scores[2 * pair] = static_cast<float>(sum[0]);
+                work.scores[2 * pair + 1] = static_cast<float>(sum[1]);
+                work.margins[pair] = static_cast<float>(m.margin);
+                work.pair_loss[2 * pair] = m.loss;
+                work.pair_loss[2 * pair + 1] = real ? 1.0 : 0.0;
+                __threadfence();
+                before = atomicAdd(work.pairs_done, 1u);
+              }
+              const long long pairs = r.rows / r.length / 2;
+              if (__shfl_sync(0xffffffffu, before, 0) == pairs - 1) {
+                __threadfence();
+                double loss = 0.0, count = 0.0;
+                for (long long i = lane; i < pairs; i += 32) {
+                  loss += __ldcg(work.pair_loss + 2 * i);
+                  count += __ldcg(work.pair_loss + 2 * i + 1);
+                }
+#pragma unroll
+                for (int o = 16; o > 0; o >>= 1) {
+                  loss += __shfl_xor_sync(0xffffffffu, loss, o);
+                  count += __shfl_xor_sync(0xffffffffu, count, o);
+                }
+                if (lane == 0) {
+                  const double whole = q.normalizer != nullptr ? 1.0 / static_cast<double>(*q.normalizer) : q.scale;
+                  out[0] = static_cast<float>(loss * whole);
+                  out[1] = static_cast<float>(count);
+                }
+              }
+            }
+          }
+          if (turned) {
+            if (lane == 0) {
+              const long long at = r.targets[t.row];
+              const float wt = r.weights != nullptr ? r.weights[t.row] : 1.f;
+              const float most = __ldcg(&work.softmax[t.row].most), sum = __ldcg(&work.softmax[t.row].sum);
+              const float by = wt * (b & 1 ? -slope0 : slope0);
+              const int slot = rows_turned % kSlots;
+              sh.slope[slot] = {most, by, -by / sum, at >= 0 && at < r.vocab ? static_cast<int>(at) : -1};
+              mbar_arrive(&sh.said[slot]);
+            }
+            ++rows_turned;
+          }
+        }
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sh.empty[stage]);
+      advance();
+    }
+    if (!ok) {
+      give_up(kStatusTimeoutEpilogue);
+      return;
+    }
+    if (kPairs) return;
+    unsigned before = 0;
+    if (lane == 0) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) partial[blockIdx.x * 4 + i] = sums[i];
+      __threadfence();
+      before = atomicAdd(arrived, 1u);
+    }
+    if (__shfl_sync(0xffffffffu, before, 0) != gridDim.x - 1) return;
+    __threadfence();
+    const double whole = p.normalizer != nullptr ? 1.0 / static_cast<double>(*p.normalizer) : p.scale;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      double v = 0.0;
+      for (unsigned c = lane; c < gridDim.x; c += 32) v += __ldcg(partial + c * 4 + i);
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+      if (lane == 0) out[i] = static_cast<float>(i < 2 ? v * whole : v);
+    }
+    return;
+  }
+
+  // ---- workers ----
+  Softmax seen = {-INFINITY, 0.f};       // of the row whose softmax is under way
+  Slope now = {0.f, 0.f, 0.f, -1};       // of the row whose gradient is under way
+  while (wait(&sh.full[stage], round & 1)) {
+    const Tile t = sh.tile[stage];
+    if (t.kind == kEnd) break;
+    const unsigned char* data = sh.data[stage];
+    const T* row = logits + row_at(r, t.row);
+    int head = 0, outside = -1;  // the value outside of the aligned part that this thread sees to
+    if (t.kind == kStat || t.kind == kGrad) {
+      int packs;
+      aligned_part(row, r.vocab, head, packs);
+      if (t.at == 0) {
+        const int i = tid < head ? tid : packs * kN + tid;  // (head + packs * kN + tid - head)
+        if (i < r.vocab && (tid < head || tid < r.vocab - packs * kN)) outside = i;
+      }
+    }
+    if (t.kind == kStat) {
+      if (outside >= 0) {
+        const float v = Pack<T>::one(row[outside]);
+        seen = {v, v == -INFINITY ? 0.f : v * 0.f + 1.f};  // (NaN of +inf and NaN)
+      }
+      if (t.packs == kTilePacks) {
+        constexpr int kMine = kTilePacks / kWorkers;
+        Pairs<T> x[kMine];
+#pragma unroll
+        for (int i = 0; i < kMine; ++i) x[i].load(data + (tid + i * kWorkers) * 16);
+        take<T, kMine>(seen, x);
+      } else {
+        for (int i = tid; i < t.packs; i += kWorkers) {
+          Pairs<T> x[1];
+          x[0].load(data + i * 16);
+          take<T, 1>(seen, x);
+        }
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sh.empty[stage]);
+      if (t.last) {
+        const Softmax s = join_row_lanes(seen);
+        if (lane == 0) {
+          const int slot = rows_summed % kSlots;
+          sh.part[slot][warp] = s;
+          mbar_arrive(&sh.sums[slot]);
+        }
+        ++rows_summed;
+        seen = {-INFINITY, 0.f};
+      }
+    } else if (t.kind == kGrad) {
+      T* g = grad + row_at(r, t.row);
+      if (t.at == 0) {
+        const int slot = rows_turned % kSlots;
+        if (!wait(&sh.said[slot], rows_turned / kSlots & 1)) break;
+        now = sh.slope[slot];
+        ++rows_turned;
+        if (outside >= 0) {
+          const float v = now.k * exp_from(Pack<T>::one(row[outside]), now.most);
+          g[outside] = Pack<T>::back(outside == now.target ? v + now.by : v);
+        }
+      }
+      const int first = head + t.at * kN;
+      const float ref = __fmul_rn(now.most, kLog2e);
+      const bool far = huge(now.most);
+      const uint64_t l2e = pair_of(kLog2e, kLog2e), off = pair_of(-ref, -ref), k2 = pair_of(now.k, now.k);
+      auto one = [&](int i) {
+        Pairs<T> v;
+        v.load(data + i * 16);
+        float x[kN];
+#pragma unroll
+        for (int j = 0; j < kN / 2; ++j) {
+          float a, b;
+          if (far) {
+            split(v.v[j], a, b);
+            a = exp_from(a, now.most), b = exp_from(b, now.most);
+          } else {
+            split(fma2(v.v[j], l2e, off), a, b);
+            a = exp2_approx(a), b = exp2_approx(b);
+          }
+          split(mul2(pair_of(a, b), k2), x[2 * j], x[2 * j + 1]);
+        }
+        const int at = first + i * kN;
+        if (static_cast<unsigned>(now.target - at) < static_cast<unsigned>(kN)) {
+#pragma unroll
+          for (int j = 0; j < kN; ++j)
+            if (now.target == at + j) x[j] += now.by;
+        }
+        Pack<T>::store(g + at, x);
+      };
+      if (t.packs == kTilePacks) {
+#pragma unroll
+        for (int i = 0; i < kTilePacks / kWorkers; ++i) one(tid + i * kWorkers);
+      } else {
+        for (int i = tid; i < t.packs; i += kWorkers) one(i);
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sh.empty[stage]);
+    } else {
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sh.empty[stage]);
+      if (t.kind == kZero) row_zero(grad + row_at(r, t.row), r.vocab, tid, kWorkers);
+    }
+    advance();
+  }
+  if (!ok) give_up(kStatusTimeoutEpilogue);
 }
 
 // grad *= *factor; nothing where the factor is 1, as it is behind `loss.backward()`. dst may be src.
@@ -508,7 +1072,7 @@ __global__ void __launch_bounds__(256)
 }
 
 // ---- host ----
-constexpr int kShortRow = 2048;  // values; shorter rows are a warp's
+constexpr long long kShortRow = 4096;  // bytes; shorter rows are a warp's
 
 int check_rows(const char* what, const void* logits, int fp32, const void* grad, long long batch, int length,
                int vocab, long long stride_b, long long stride_t, const void* targets) {
@@ -525,8 +1089,8 @@ int check_rows(const char* what, const void* logits, int fp32, const void* grad,
   return 0;
 }
 
-unsigned row_grid(long long rows, bool by_warp) {
-  const long long ctas = by_warp ? (rows + kRowThreads / 32 - 1) / (kRowThreads / 32) : rows;
+unsigned row_grid(long long rows) {
+  const long long ctas = (rows + kRowThreads / 32 - 1) / (kRowThreads / 32);
   const long long cap = static_cast<long long>(num_sms()) * 4;
   return static_cast<unsigned>(ctas < 1 ? 1 : (ctas < cap ? ctas : cap));
 }
@@ -538,7 +1102,30 @@ int launched(const char* what, int n) {
   return 0;
 }
 
-constexpr size_t kHead = 16;  // bytes of scratch in front: the count of arrived CTAs
+unsigned long_grid(long long rows) {
+  const long long cap = static_cast<long long>(num_sms()) * 2;
+  return static_cast<unsigned>(rows < 1 ? 1 : (rows < cap ? rows : cap));
+}
+
+template <typename T, bool kPairs>
+int launch_long(const char* what, const void* logits, void* grad, const Rows& r, const Policy& p, const Preference& q,
+                const Work& work, double* partial, unsigned* arrived, float* out, cudaStream_t st) {
+  auto kernel = long_rows_kernel<T, kPairs>;
+  const cudaError_t e =
+      cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, sizeof(LongShared));
+  if (e != cudaSuccess) return set_error("%s: %s", what, cudaGetErrorString(e));
+  kernel<<<long_grid(r.rows), kLongThreads, sizeof(LongShared), st>>>(
+      static_cast<const T*>(logits), static_cast<T*>(grad), r, p, q, work, partial, arrived, out,
+      device_status_buffer());
+  return launched(what, 1);
+}
+
+// The order of the tasks of a preference loss: a pair of up to kBehindBytes of logits stands in a group of
+// up to kGroupBytes, whose gradients follow the next group's softmaxes; a larger pair's gradients follow
+// its own softmaxes, beginning with the rows read last.
+constexpr long long kGroupBytes = 16 << 20, kBehindBytes = 24 << 20;
+
+constexpr size_t kHead = 16;  // bytes of scratch in front: the ticket, the count of arrived CTAs or pairs done
 
 }  // namespace
 }  // namespace t5x
@@ -567,19 +1154,18 @@ T5X_API int t5x_policy_loss(const void* logits, int fp32, void* grad, long long 
   const Policy p = {static_cast<const float*>(old_scores), static_cast<const float*>(ref_scores),
                     static_cast<const float*>(advantages), adv_b, adv_t, 1.f - clip_low, 1.f + clip_high,
                     kl_weight, scale, static_cast<const float*>(normalizer)};
-  const bool by_warp = vocab < kShortRow;
-  const unsigned grid = row_grid(r.rows, by_warp);
-  auto go = [&](auto kernel, auto* x) {
-    kernel<<<grid, kRowThreads, 0, st>>>(x, static_cast<std::remove_const_t<std::remove_pointer_t<decltype(x)>>*>(grad),
-                                         r, p, partial, arrived, static_cast<float*>(out));
-  };
-  if (fp32) {
-    const float* x = static_cast<const float*>(logits);
-    by_warp ? go(policy_rows_kernel<float, 32>, x) : go(policy_rows_kernel<float, kRowThreads>, x);
-  } else {
-    const __nv_bfloat16* x = static_cast<const __nv_bfloat16*>(logits);
-    by_warp ? go(policy_rows_kernel<__nv_bfloat16, 32>, x) : go(policy_rows_kernel<__nv_bfloat16, kRowThreads>, x);
-  }
+  float* o = static_cast<float*>(out);
+  if (static_cast<long long>(vocab) * (fp32 ? 4 : 2) >= kShortRow)
+    return fp32 ? launch_long<float, false>("policy_loss", logits, grad, r, p, {}, {}, partial, arrived, o, st)
+                : launch_long<__nv_bfloat16, false>("policy_loss", logits, grad, r, p, {}, {}, partial, arrived, o, st);
+  const unsigned grid = row_grid(r.rows);
+  if (fp32)
+    policy_short_rows_kernel<<<grid, kRowThreads, 0, st>>>(static_cast<const float*>(logits),
+                                                           static_cast<float*>(grad), r, p, partial, arrived, o);
+  else
+    policy_short_rows_kernel<<<grid, kRowThreads, 0, st>>>(static_cast<const __nv_bfloat16*>(logits),
+                                                           static_cast<__nv_bfloat16*>(grad), r, p, partial, arrived,
+                                                           o);
   return launched("policy_loss", 1);
 }
 
@@ -598,7 +1184,7 @@ T5X_API int t5x_policy_loss_tokens(const void* logp, void* slope, long long batc
   const Policy p = {static_cast<const float*>(old_scores), static_cast<const float*>(ref_scores),
                     static_cast<const float*>(advantages), adv_b, adv_t, 1.f - clip_low, 1.f + clip_high,
                     kl_weight, scale, static_cast<const float*>(normalizer)};
-  policy_tokens_kernel<<<row_grid((r.rows + kRowThreads - 1) / kRowThreads, false), kRowThreads, 0, st>>>(
+  policy_tokens_kernel<<<row_grid((r.rows + 31) / 32), kRowThreads, 0, st>>>(
       static_cast<const float*>(logp), static_cast<float*>(slope), r, p,
       reinterpret_cast<double*>(static_cast<char*>(scratch) + kHead), static_cast<unsigned*>(scratch),
       static_cast<float*>(out));
@@ -606,8 +1192,9 @@ T5X_API int t5x_policy_loss_tokens(const void* logp, void* slope, long long batc
 }
 
 T5X_API long long t5x_preference_loss_scratch_bytes(long long batch, int length) {
-  // head | loss and count of each pair | largest and sum of each token | log-probability | slope of each row
-  return static_cast<long long>(kHead) + batch * 8 + batch * length * 12 + batch * 4;
+  // head | counts and flags of the pairs | loss and count of each pair | largest and sum of each token |
+  // log-probability | slope of each row
+  return static_cast<long long>(kHead) + batch / 2 * 8 + batch * 8 + batch * length * 12 + batch * 4;
 }
 
 T5X_API int t5x_preference_loss(const void* logits, int fp32, void* grad, long long batch, int length, int vocab,
@@ -617,41 +1204,55 @@ T5X_API int t5x_preference_loss(const void* logits, int fp32, void* grad, long l
                                 void* stream) {
   if (check_rows("preference_loss", logits, fp32, grad, batch, length, vocab, stride_b, stride_t, targets)) return -1;
   if (batch < 2 || batch % 2) return set_error("preference_loss: the batch must hold pairs");
+  if (length < 1 || length > (1 << 30)) return set_error("preference_loss: bad sizes");
   if (!scratch || !out || !reference || !scores || !margins) return set_error("preference_loss: null pointer");
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  cudaError_t e = cudaMemsetAsync(scratch, 0, kHead, st);
-  if (e != cudaSuccess) return set_error("preference_loss: memset: %s", cudaGetErrorString(e));
+  const long long pairs = batch / 2;
+  char* at = static_cast<char*>(scratch);
   const Rows r = {batch * length, length, vocab, stride_b, stride_t, static_cast<const long long*>(targets),
                   static_cast<const float*>(weights)};
   const Preference p = {static_cast<const float*>(reference), beta, smoothing, scale,
                         static_cast<const float*>(normalizer)};
-  char* at = static_cast<char*>(scratch);
-  unsigned* arrived = reinterpret_cast<unsigned*>(at);
-  double* pair_loss = reinterpret_cast<double*>(at + kHead);
-  Softmax* softmax = reinterpret_cast<Softmax*>(at + kHead + batch * 8);
-  float* logp = reinterpret_cast<float*>(softmax + r.rows);
-  float* by = logp + r.rows;
-  const bool by_warp = vocab < kShortRow;
-  const unsigned grid = row_grid(r.rows, by_warp);
-  auto go = [&](auto rows, auto gradient, auto* x) {
-    if (r.rows > 0) rows<<<grid, kRowThreads, 0, st>>>(x, r, softmax, logp);
-    preference_pairs_kernel<<<static_cast<unsigned>(batch / 2), kRowThreads, 0, st>>>(
-        logp, r, p, static_cast<float*>(scores), static_cast<float*>(margins), by, nullptr, pair_loss, arrived,
-        static_cast<float*>(out));
-    if (grad != nullptr && r.rows > 0)
-      gradient<<<grid, kRowThreads, 0, st>>>(
-          x, static_cast<std::remove_const_t<std::remove_pointer_t<decltype(x)>>*>(grad), r, softmax, by);
-  };
-  if (fp32) {
-    const float* x = static_cast<const float*>(logits);
-    by_warp ? go(preference_rows_kernel<float, 32>, preference_gradient_kernel<float, 32>, x)
-            : go(preference_rows_kernel<float, kRowThreads>, preference_gradient_kernel<float, kRowThreads>, x);
-  } else {
-    const __nv_bfloat16* x = static_cast<const __nv_bfloat16*>(logits);
-    by_warp ? go(preference_rows_kernel<__nv_bfloat16, 32>, preference_gradient_kernel<__nv_bfloat16, 32>, x)
-            : go(preference_rows_kernel<__nv_bfloat16, kRowThreads>,
-                 preference_gradient_kernel<__nv_bfloat16, kRowThreads>, x);
+  Work w;
+  w.ticket = reinterpret_cast<unsigned long long*>(at);
+  w.pairs_done = reinterpret_cast<unsigned*>(at + 8);
+  w.done = reinterpret_cast<unsigned*>(at + kHead);
+  w.pair_loss = reinterpret_cast<double*>(at + kHead + pairs * 8);
+  w.softmax = reinterpret_cast<Softmax*>(w.pair_loss + batch);
+  w.logp = reinterpret_cast<float*>(w.softmax + r.rows);
+  float* by = w.logp + r.rows;
+  w.scores = static_cast<float*>(scores);
+  w.margins = static_cast<float*>(margins);
+  float* o = static_cast<float*>(out);
+  const long long row_bytes = static_cast<long long>(vocab) * (fp32 ? 4 : 2);
+  const bool in_long = row_bytes >= kShortRow;
+  cudaError_t e = cudaMemsetAsync(scratch, 0, kHead + (in_long ? pairs * 8 : 0), st);
+  if (e != cudaSuccess) return set_error("preference_loss: memset: %s", cudaGetErrorString(e));
+  if (in_long) {
+    const long long pair_bytes = 2 * length * row_bytes;
+    const long long group = kGroupBytes / pair_bytes > 1 ? kGroupBytes / pair_bytes : 1;
+    w.order = {r.rows, (group < pairs ? group : pairs) * 2 * length, pair_bytes <= kBehindBytes, grad != nullptr};
+    if (fp32 ? launch_long<float, true>("preference_loss", logits, grad, r, {}, p, w, nullptr, nullptr, o, st)
+             : launch_long<__nv_bfloat16, true>("preference_loss", logits, grad, r, {}, p, w, nullptr, nullptr, o, st))
+      return -1;
+    if (grad != nullptr) return 0;
+    preference_pairs_kernel<<<static_cast<unsigned>(pairs), kRowThreads, 0, st>>>(
+        w.logp, r, p, w.scores, w.margins, nullptr, nullptr, w.pair_loss, w.pairs_done, o);
+    return launched("preference_loss", 1);
   }
+  const unsigned grid = row_grid(r.rows);
+  auto go = [&](auto* x) {
+    using T = std::remove_const_t<std::remove_pointer_t<decltype(x)>>;
+    preference_short_rows_kernel<T><<<grid, kRowThreads, 0, st>>>(x, r, w.softmax, w.logp);
+    preference_pairs_kernel<<<static_cast<unsigned>(pairs), kRowThreads, 0, st>>>(
+        w.logp, r, p, w.scores, w.margins, by, nullptr, w.pair_loss, w.pairs_done, o);
+    if (grad != nullptr)
+      preference_short_gradient_kernel<T><<<grid, kRowThreads, 0, st>>>(x, static_cast<T*>(grad), r, w.softmax, by);
+  };
+  if (fp32)
+    go(static_cast<const float*>(logits));
+  else
+    go(static_cast<const __nv_bfloat16*>(logits));
   return launched("preference_loss", 2 + (grad != nullptr));
 }
 
