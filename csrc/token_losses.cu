@@ -18,6 +18,7 @@
 // taken in an order that depends on the sizes alone.
 //
 // What bounds it: memory; the logits that count read once, the gradient written once.
+#include <atomic>
 #include <cmath>
 #include <type_traits>
 
@@ -239,10 +240,15 @@ struct PolicyToken {
   float loss, kl, clipped;  // before weight and scale
   float slope;              // dloss / dlogp
 };
-__device__ __forceinline__ PolicyToken policy_token(const Policy& p, long long row, long long b, long long t,
-                                                    float logp) {
-  const float a = p.advantages[b * p.adv_b + t * p.adv_t];
-  const float ratio = expf(logp - p.old[row]);
+struct PolicyInputs {
+  float old, ref, advantage;
+};
+__device__ __forceinline__ PolicyInputs policy_inputs(const Policy& p, long long row, long long b, long long t) {
+  return {p.old[row], p.ref != nullptr ? p.ref[row] : 0.f, p.advantages[b * p.adv_b + t * p.adv_t]};
+}
+__device__ __forceinline__ PolicyToken policy_token(const Policy& p, PolicyInputs in, float logp) {
+  const float a = in.advantage;
+  const float ratio = expf(logp - in.old);
   const float gain = a * ratio, held = a * fminf(fmaxf(ratio, p.low), p.high);
   PolicyToken k;
   k.clipped = held < gain ? 1.f : 0.f;
@@ -251,7 +257,7 @@ __device__ __forceinline__ PolicyToken policy_token(const Policy& p, long long r
   k.slope = held < gain ? 0.f : -gain;
   k.kl = 0.f;
   if (p.ref != nullptr) {
-    const float apart = p.ref[row] - logp, e = expm1f(apart);
+    const float apart = in.ref - logp, e = expm1f(apart);
     k.kl = e - apart;
     k.loss += p.kl_weight * k.kl;
     k.slope -= p.kl_weight * e;
@@ -297,9 +303,10 @@ __global__ void __launch_bounds__(kRowThreads)
       continue;
     }
     const long long target = r.targets[row], b = row / r.length;
+    const PolicyInputs in = policy_inputs(p, row, b, row - b * r.length);
     const Softmax s = join_lanes(row_softmax(logits + at, r.vocab, lane, 32));
     const float logp = log_prob(logits + at, r.vocab, target, s);
-    const PolicyToken k = policy_token(p, row, b, row - b * r.length, logp);
+    const PolicyToken k = policy_token(p, in, logp);
     if (lane == 0) {
       sums[0] += static_cast<double>(w) * k.loss;
       sums[1] += static_cast<double>(w) * k.kl;
@@ -325,7 +332,7 @@ __global__ void __launch_bounds__(kRowThreads)
     float by = 0.f;
     if (w != 0.f) {
       const long long b = row / r.length;
-      const PolicyToken k = policy_token(p, row, b, row - b * r.length, logp[row]);
+      const PolicyToken k = policy_token(p, policy_inputs(p, row, b, row - b * r.length), logp[row]);
       sums[0] += static_cast<double>(w) * k.loss;
       sums[1] += static_cast<double>(w) * k.kl;
       sums[2] += static_cast<double>(w) * k.clipped;
@@ -364,27 +371,30 @@ __global__ void __launch_bounds__(kRowThreads)
 }
 
 struct Margin {
-  double margin, loss, slope;  // slope: dloss / d(score of the preferred)
+  double margin;      // of sums of many tokens: in 64 bits; what follows of their difference in 32
+  float loss, slope;  // slope: dloss / d(score of the preferred)
 };
 __device__ __forceinline__ Margin pair_margin(const Preference& p, bool real, double s0, double s1, float r0, float r1,
-                                              double scale) {
-  Margin m = {0.0, 0.0, 0.0};
+                                              float scale) {
+  Margin m = {0.0, 0.f, 0.f};
   if (!real) return m;
   m.margin = p.beta * ((s0 - r0) - (s1 - r1));
+  const float d = static_cast<float>(m.margin);
   // log(1 + exp(-d)) = log1p(exp(-|d|)) + max(-d, 0)
-  const double e = exp(-fabs(m.margin)), tail = log1p(e);
-  const double sigmoid = m.margin >= 0.0 ? 1.0 / (1.0 + e) : e / (1.0 + e);
-  m.loss = m.margin != m.margin ? m.margin
-                                : (1.0 - p.smoothing) * (tail + fmax(-m.margin, 0.0)) +
-                                      p.smoothing * (tail + fmax(m.margin, 0.0));
-  m.slope = p.beta * (sigmoid - (1.0 - p.smoothing)) * scale;
+  const float e = expf(-fabsf(d)), tail = log1pf(e);
+  const float sigmoid = (d >= 0.f ? 1.f : e) / (1.f + e);
+  m.loss = d != d ? d : (1.f - p.smoothing) * (tail + fmaxf(-d, 0.f)) + p.smoothing * (tail + fmaxf(d, 0.f));
+  // sigmoid - 1 + e, near 0 from the side that does not cancel
+  const float under = (d >= 0.f ? e : 1.f) / (1.f + e);  // sigmoid(-d)
+  m.slope = p.beta * (p.smoothing * sigmoid - (1.f - p.smoothing) * under) * scale;
   return m;
 }
 
 // A CTA per pair: scores, margin, the pair's loss, the slopes of its two sequences (and, from
-// log-probabilities, of its tokens). The last CTA adds the losses. out: loss, pairs
+// log-probabilities, of its tokens). The last CTA adds the losses. out: loss, pairs. logp: `logp_step` floats
+// from one to the next.
 __global__ void __launch_bounds__(kRowThreads)
-    preference_pairs_kernel(const float* __restrict__ logp, const Rows r, const Preference p, float* scores,
+    preference_pairs_kernel(const float* __restrict__ logp, int logp_step, const Rows r, const Preference p, float* scores,
                             float* margins, float* __restrict__ by, float* __restrict__ token_slope,
                             double* pair_loss, unsigned* arrived, float* out) {
   const long long pair = blockIdx.x;
@@ -396,7 +406,7 @@ __global__ void __launch_bounds__(kRowThreads)
     for (int t = threadIdx.x; t < r.length; t += kRowThreads) {
       const float w = r.weights != nullptr ? r.weights[first + t] : 1.f;
       if (w != 0.f) {
-        sum[side] += static_cast<double>(w) * logp[first + t];
+        sum[side] += static_cast<double>(w) * logp[(first + t) * logp_step];
         seen = 1.0;
       }
     }
@@ -404,14 +414,14 @@ __global__ void __launch_bounds__(kRowThreads)
   }
   const bool real = cta_sum<kRowThreads>(seen) > 0.0;
   const Margin m = pair_margin(p, real, sum[0], sum[1], p.ref[2 * pair], p.ref[2 * pair + 1], scale);
-  const double slope = m.slope;
+  const float slope = m.slope;
   if (threadIdx.x == 0) {
     scores[2 * pair] = static_cast<float>(sum[0]);
     scores[2 * pair + 1] = static_cast<float>(sum[1]);
     margins[pair] = static_cast<float>(m.margin);
     if (by != nullptr) {
-      by[2 * pair] = static_cast<float>(slope);
-      by[2 * pair + 1] = static_cast<float>(-slope);
+      by[2 * pair] = slope;
+      by[2 * pair + 1] = -slope;
     }
     pair_loss[2 * pair] = m.loss;
     pair_loss[2 * pair + 1] = real ? 1.0 : 0.0;
@@ -422,7 +432,7 @@ __global__ void __launch_bounds__(kRowThreads)
       const long long first = (2 * pair + side) * r.length;
       for (int t = threadIdx.x; t < r.length; t += kRowThreads) {
         const float w = r.weights != nullptr ? r.weights[first + t] : 1.f;
-        token_slope[first + t] = w == 0.f ? 0.f : static_cast<float>((side ? -slope : slope) * w);
+        token_slope[first + t] = w == 0.f ? 0.f : (side ? -slope : slope) * w;
       }
     }
   }
@@ -462,43 +472,60 @@ __global__ void __launch_bounds__(kRowThreads)
 }
 
 // ---- long rows ----
-// A CTA's producer thread copies the rows in tiles of 16 KB into a ring in shared memory, in the order
-// in which the worker warps take them, far ahead of them; so the loads go on while a row's sums meet.
-// Each tile goes by twice, for the softmax and for the gradient, the second time out of L2. A keeper warp
-// makes of the workers' sums what the gradient needs, so that no worker waits for a load of a single
-// value, a logarithm or another CTA.
-//
-// policy: row after row, the gradient of one behind the softmax of the next.
-// preference: the slope needs the sums of all rows of a pair. The tasks (a row's softmax, a row's gradient)
-// stand in an order in which a group of pairs is followed by the next group's softmaxes and then its own
-// gradients; a CTA takes the next task by a ticket. What a gradient waits for has smaller tickets, is
-// therefore done or under way, and waits itself for smaller tickets at most.
-constexpr int kWorkers = 256;
-constexpr int kWorkerWarps = kWorkers / 32;
-constexpr int kLongThreads = kWorkers + 64;
+// What both kernels share. A CTA's producer thread copies rows in tiles of up to 16 KB into a ring in
+// shared memory, far ahead of the worker warps, so that the loads go on while a row's sums meet. A keeper
+// warp makes of the workers' sums what the gradient of the row needs, so that no worker waits for the
+// load of a single value, a logarithm or another CTA; the producer hands it a row's few values, which it
+// has asked for rows ahead.
 constexpr int kTileBytes = 16384;
-constexpr int kStages = 6;
-constexpr int kSlots = 16;  // rows between their sums and their gradient: at most the ring's tiles and two
+constexpr int kTilePacks = kTileBytes / 16;
+constexpr int kSlots = 16;  // rows that the keeper is told of ahead; more than the tiles of a ring and two
 
-enum Kind : int { kEnd, kStat, kGrad, kZero, kSkip };
+enum Kind : int { kEnd, kStat, kGrad, kZero };
 struct Tile {
-  long long row;
-  int kind;
-  int at, packs;  // first 16 bytes of the row's aligned part, how many
-  int last;
+  long long offset;  // of the row in the logits and their gradient
+  int kind, last;
+  int head;          // values in front of the row's first 16-byte boundary
+  int at, packs;     // first 16 bytes behind it, how many
+  int outside;       // 16 bytes of the whole row, on the tile whose workers see to the values outside; else -1
+  unsigned task;     // the row's place in the keeper's queue
+};
+struct Task {
+  long long row, b;
+  int kind, target;  // target: -1 outside of the vocabulary
+  float w, x;        // weight, the target's logit
+  PolicyInputs in;
 };
 // What the gradient of a row needs: by * onehot(target) + k * exp(x - most) with k = -by / sum.
 struct Slope {
   float most, by, k;
   int target;
 };
+template <int kStages, int kWarps>
 struct LongShared {
   alignas(128) unsigned char data[kStages][kTileBytes];
-  uint64_t full[kStages], empty[kStages], sums[kSlots], said[kSlots];
+  uint64_t full[kStages], empty[kStages], told[kSlots], kept[kSlots], sums[kSlots], said[kSlots], met[kSlots];
   Tile tile[kStages];
-  Softmax part[kSlots][kWorkerWarps];
+  Task task[kSlots];
+  Softmax part[kSlots][kWarps];
+  Softmax of_cta[kSlots][8];  // of the CTAs that share the row
   Slope slope[kSlots];
   int abort;
+  __device__ void init() {
+    for (int i = 0; i < kStages; ++i) {
+      mbar_init(&full[i], 1);
+      mbar_init(&empty[i], kWarps);
+    }
+    for (int i = 0; i < kSlots; ++i) {
+      mbar_init(&told[i], 1);
+      mbar_init(&kept[i], 1);
+      mbar_init(&sums[i], kWarps);
+      mbar_init(&said[i], 1);
+      mbar_init(&met[i], 1);
+    }
+    abort = 0;
+    mbar_fence_init();
+  }
 };
 
 // The part of a row between 16-byte boundaries.
@@ -509,42 +536,6 @@ __device__ __forceinline__ void aligned_part(const T* row, int vocab, int& head,
   head = off ? kN - off : 0;
   packs = (vocab - head) / kN;
 }
-
-struct Order {
-  long long rows, group;  // rows of the batch, of a group of pairs
-  bool behind;            // a group's gradients follow the next group's softmaxes
-  bool gradient;
-};
-// (row, is it the gradient's turn) of a ticket below rows * (1 + gradient)
-__device__ __forceinline__ long long task_of(const Order& o, long long ticket, bool& gradient) {
-  gradient = false;
-  if (!o.gradient) return ticket;
-  const long long last = (o.rows - 1) / o.group * o.group;  // first row of the last group
-  if (!o.behind) {  // softmaxes of a group, then its gradients, those last read first
-    const long long k = ticket / (2 * o.group), first = k * o.group, at = ticket - 2 * first;
-    const long long n = o.rows - first < o.group ? o.rows - first : o.group;
-    gradient = at >= n;
-    return gradient ? first + 2 * n - 1 - at : first + at;
-  }
-  gradient = ticket >= o.rows + last;
-  if (gradient) return ticket - o.rows;  // of the last group
-  if (ticket < o.group) return ticket;
-  const long long k = (ticket - o.group) / (2 * o.group) + 1;  // softmaxes of group k, gradients of k - 1
-  const long long at = ticket - o.group - (k - 1) * 2 * o.group, first = k * o.group;
-  const long long n = o.rows - first < o.group ? o.rows - first : o.group;
-  gradient = at >= n;
-  return gradient ? first - o.group + (at - n) : first + at;
-}
-
-struct Work {
-  unsigned long long* ticket;
-  unsigned *done, *pairs_done;  // done: rows of the pair whose softmax is there (or that do not count)
-  Softmax* softmax;
-  float* logp;
-  double* pair_loss;
-  float *scores, *margins;
-  Order order;
-};
 
 // Two values at once where the arithmetic has pairs.
 __device__ __forceinline__ uint64_t pair_of(float a, float b) {
@@ -570,6 +561,7 @@ __device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
   asm("mul.rn.ftz.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
   return d;
 }
+__device__ __forceinline__ uint64_t same2(float a) { return pair_of(a, a); }
 
 // In the tiles an exponential exp(x - most) is exp2(x log2 e - ref), a fused product and difference, with
 // ref = most log2 e as rounded: the same factor for the sum, the target and the gradient. Where a largest
@@ -601,16 +593,18 @@ __device__ __forceinline__ float log_prob_of(float x, Softmax s) {
   return d - log1pf(s.sum - 1.f);
 }
 
-// 16 bytes of the tile, as pairs
+// 16 bytes of a tile, as pairs
 template <typename T>
 struct Pairs;
 template <>
 struct Pairs<float> {
+  static constexpr int kPairs = 2;
   uint64_t v[2];
   __device__ void load(const void* p) {
     const float4 x = *static_cast<const float4*>(p);
     v[0] = pair_of(x.x, x.y), v[1] = pair_of(x.z, x.w);
   }
+  __device__ void nothing() { v[0] = v[1] = same2(-INFINITY); }
   __device__ float most() const {
     float a, b, c, d;
     split(v[0], a, b), split(v[1], c, d);
@@ -619,6 +613,7 @@ struct Pairs<float> {
 };
 template <>
 struct Pairs<__nv_bfloat16> {
+  static constexpr int kPairs = 4;
   uint64_t v[4];
   float top;
   __device__ void load(const void* p) {
@@ -629,80 +624,213 @@ struct Pairs<__nv_bfloat16> {
     const __nv_bfloat162 m = __hmax2(__hmax2(as2(u[0]), as2(u[1])), __hmax2(as2(u[2]), as2(u[3])));
     top = fmaxf(__low2float(m), __high2float(m));
   }
+  __device__ void nothing() {
+    v[0] = v[1] = v[2] = v[3] = same2(-INFINITY);
+    top = -INFINITY;
+  }
   __device__ static __nv_bfloat162 as2(uint32_t u) { return *reinterpret_cast<__nv_bfloat162*>(&u); }
   __device__ float most() const { return top; }
 };
 
-// Adds a thread's 16 bytes each to the softmax of what it has seen.
-template <typename T, int kPacks>
-__device__ __forceinline__ void take(Softmax& s, const Pairs<T>* x) {
-  constexpr int kPairsOf = sizeof(Pairs<T>::v) / 8;
+// exp2 of the two values
+__device__ __forceinline__ uint64_t exp2_pair(uint64_t x) {
+  float a, b;
+  split(x, a, b);
+  return pair_of(exp2_approx(a), exp2_approx(b));
+}
+
+// The tile's part of the row's softmax.
+template <typename T, int kWorkers>
+__device__ __forceinline__ void sum_tile(Softmax& s, const unsigned char* data, int packs, int tid) {
+  constexpr int kMine = (kTilePacks + kWorkers - 1) / kWorkers, kP = Pairs<T>::kPairs;
+  Pairs<T> x[kMine];
+#pragma unroll
+  for (int i = 0; i < kMine; ++i) {
+    if (tid + i * kWorkers < packs)
+      x[i].load(data + (tid + i * kWorkers) * 16);
+    else
+      x[i].nothing();
+  }
   float m = x[0].most();
 #pragma unroll
-  for (int i = 1; i < kPacks; ++i) m = fmaxf(m, x[i].most());
+  for (int i = 1; i < kMine; ++i) m = fmaxf(m, x[i].most());
   if (m > s.most) {
     s.sum *= exp2_approx(shift(s.most, m));
     s.most = m;
   }
-  uint64_t t = pair_of(0.f, 0.f);
+  uint64_t t[2] = {same2(0.f), same2(0.f)};
   if (!huge(s.most)) {
     const float ref = __fmul_rn(s.most, kLog2e);
-    const uint64_t l2e = pair_of(kLog2e, kLog2e), off = pair_of(-ref, -ref);
+    const uint64_t l2e = same2(kLog2e), off = same2(-ref);
 #pragma unroll
-    for (int i = 0; i < kPacks; ++i) {
+    for (int i = 0; i < kMine; ++i)
 #pragma unroll
-      for (int j = 0; j < kPairsOf; ++j) {
-        float a, b;
-        split(fma2(x[i].v[j], l2e, off), a, b);
-        t = add2(t, pair_of(exp2_approx(a), exp2_approx(b)));
-      }
-    }
+      for (int j = 0; j < kP; ++j) t[j & 1] = add2(t[j & 1], exp2_pair(fma2(x[i].v[j], l2e, off)));
   } else {
 #pragma unroll
-    for (int i = 0; i < kPacks; ++i) {
+    for (int i = 0; i < kMine; ++i)
 #pragma unroll
-      for (int j = 0; j < kPairsOf; ++j) {
+      for (int j = 0; j < kP; ++j) {
         float a, b;
         split(x[i].v[j], a, b);
-        t = add2(t, pair_of(exp_from(a, s.most), exp_from(b, s.most)));
+        t[0] = add2(t[0], pair_of(exp_from(a, s.most), exp_from(b, s.most)));
       }
-    }
   }
   float a, b;
-  split(t, a, b);
+  split(add2(t[0], t[1]), a, b);
   s.sum += a + b;
 }
 
-template <typename T, bool kPairs>
-__global__ void __launch_bounds__(kLongThreads, 2)
-    long_rows_kernel(const T* __restrict__ logits, T* __restrict__ grad, const Rows r, const Policy p,
-                     const Preference q, const Work work, double* partial, unsigned* arrived, float* out,
-                     int* status) {
-  constexpr int kN = Pack<T>::kN;
-  constexpr int kTilePacks = kTileBytes / 16;
-  extern __shared__ __align__(128) unsigned char raw[];
-  LongShared& sh = *reinterpret_cast<LongShared*>(raw);
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  if (tid == 0) {
-    for (int i = 0; i < kStages; ++i) {
-      mbar_init(&sh.full[i], 1);
-      mbar_init(&sh.empty[i], kWorkerWarps + 1);
+// The tile's part of the gradient; g: the row's.
+template <typename T, int kWorkers>
+__device__ __forceinline__ void turn_tile(T* g, const unsigned char* data, const Tile& t, const Slope& now, int tid) {
+  constexpr int kMine = (kTilePacks + kWorkers - 1) / kWorkers, kN = Pack<T>::kN;
+  const int first = t.head + t.at * kN;
+  const bool far = huge(now.most);
+  const float ref = __fmul_rn(now.most, kLog2e);
+  const uint64_t l2e = same2(kLog2e), off = same2(-ref), k2 = same2(now.k);
+  auto one = [&](int i, auto plain) {
+    Pairs<T> v;
+    v.load(data + i * 16);
+    float x[kN];
+#pragma unroll
+    for (int j = 0; j < kN / 2; ++j) {
+      uint64_t e;
+      if (plain || !far) {
+        e = exp2_pair(fma2(v.v[j], l2e, off));
+      } else {
+        float a, b;
+        split(v.v[j], a, b);
+        e = pair_of(exp_from(a, now.most), exp_from(b, now.most));
+      }
+      split(mul2(e, k2), x[2 * j], x[2 * j + 1]);
     }
-    for (int i = 0; i < kSlots; ++i) {
-      mbar_init(&sh.sums[i], kWorkerWarps);
-      mbar_init(&sh.said[i], 1);
+    const int at = first + i * kN;
+    if (!plain && static_cast<unsigned>(now.target - at) < static_cast<unsigned>(kN)) {
+#pragma unroll
+      for (int j = 0; j < kN; ++j)
+        if (now.target == at + j) x[j] += now.by;
     }
-    sh.abort = 0;
-    mbar_fence_init();
-  }
-  __syncthreads();
-  volatile int* abort = &sh.abort;
-  int stage = 0;
-  uint32_t round = 0;
-  bool ok = true;
-  auto advance = [&] {
-    if (++stage == kStages) stage = 0, ++round;
+    Pack<T>::store(g + at, x);
   };
+  // a tile without the target, of a row whose exponentials take the short way
+  if (!far && static_cast<unsigned>(now.target - first) >= static_cast<unsigned>(t.packs * kN)) {
+#pragma unroll
+    for (int i = 0; i < kMine; ++i)
+      if (tid + i * kWorkers < t.packs) one(tid + i * kWorkers, std::true_type());
+  } else {
+    for (int i = tid; i < t.packs; i += kWorkers) one(i, std::false_type());
+  }
+}
+
+// The value outside of the row's 16-byte boundaries that a thread sees to, or -1.
+template <typename T>
+__device__ __forceinline__ int outside_of(const Tile& t, int vocab, int tid) {
+  if (t.outside < 0) return -1;
+  const int behind = t.outside * Pack<T>::kN;  // head + ... - head
+  return tid < t.head ? tid : (tid < vocab - behind ? behind + tid : -1);
+}
+template <typename T>
+__device__ __forceinline__ Softmax one_value(T v) {
+  const float x = Pack<T>::one(v);
+  return {x, x == -INFINITY ? 0.f : x * 0.f + 1.f};  // (NaN of +inf and NaN)
+}
+template <typename T>
+__device__ __forceinline__ void turn_one(T* g, const T* row, int i, const Slope& now) {
+  const float v = now.k * exp_from(Pack<T>::one(row[i]), now.most);
+  g[i] = Pack<T>::back(i == now.target ? v + now.by : v);
+}
+
+// The producer's side of a ring; one thread's.
+template <typename Shared, int kStages>
+struct Ring {
+  Shared& sh;
+  volatile int* abort;
+  int stage = 0, issued = 0;
+  uint32_t round = 0;
+  unsigned tasks = 0;
+  bool ok = true;
+  __device__ Ring(Shared& s) : sh(s), abort(&s.abort) {}
+  __device__ void push(const Tile& t, const void* src) {
+    if (!ok || !mbar_wait(&sh.empty[stage], (round & 1) ^ 1, abort)) {
+      ok = false;
+      return;
+    }
+    sh.tile[stage] = t;
+    if (src != nullptr) {
+      mbar_expect_tx(&sh.full[stage], t.packs * 16);
+      bulk_load(sh.data[stage], src, t.packs * 16, &sh.full[stage]);
+    } else {
+      mbar_arrive(&sh.full[stage]);
+    }
+    ++issued;
+    if (++stage == kStages) stage = 0, ++round;
+  }
+  // The keeper, of a row ahead of its tiles. Returns the row's place in its queue.
+  __device__ unsigned tell(const Task& t) {
+    const int slot = tasks % kSlots;
+    if (!ok || !mbar_wait(&sh.kept[slot], (tasks / kSlots & 1) ^ 1, abort)) {
+      ok = false;
+      return tasks;
+    }
+    sh.task[slot] = t;
+    mbar_arrive(&sh.told[slot]);
+    return tasks++;
+  }
+  // `packs` 16 bytes of a row from `from`, in tiles of one size, so that each gives all workers something to do.
+  template <typename T>
+  __device__ void stream(Tile t, const T* logits, int from, int packs) {
+    const int tiles = (packs + kTilePacks - 1) / kTilePacks, size = (packs + tiles - 1) / tiles;
+    for (int at = 0; at < packs && ok; at += size) {
+      t.at = from + at;
+      t.packs = packs - at < size ? packs - at : size;
+      t.last = at + t.packs == packs;
+      push(t, logits + t.offset + t.head + static_cast<long long>(t.at) * Pack<T>::kN);
+      t.outside = -1;
+    }
+  }
+  // No copy may be under way when the shared memory is given back.
+  __device__ void drain() {
+    const int n = issued < kStages ? issued : kStages;
+    for (int i = issued - n; i < issued; ++i)
+      for (uint32_t it = 0; it < kWaitLimit && !mbar_try_wait(&sh.full[i % kStages], (i / kStages) & 1); ++it) {
+      }
+  }
+};
+
+// Policy. A row belongs to a cluster of CTAs, of which each takes a part that fits into its ring with room for
+// the next one: the part is read once, summed, and turned into the gradient where it lies. The parts' sums
+// meet through distributed shared memory. `behind`: a row's gradient comes behind the next row's sums, so that
+// nobody waits while the keepers make the slope. Parts that do not fit are read a second time.
+constexpr int kPolicyStages = 13;
+constexpr int kPolicyWorkers = 512;
+constexpr int kPolicyThreads = kPolicyWorkers + 64;
+using PolicyShared = LongShared<kPolicyStages, kPolicyWorkers / 32>;
+
+__device__ __forceinline__ void send_to_cta(Softmax* slot, uint64_t* bar, int cta, Softmax s) {
+  uint64_t v;
+  memcpy(&v, &s, 8);
+  asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.b64 [%0], %1, [%2];" ::"r"(
+                   mapa_shared(smem_u32(slot), cta)),
+               "l"(v), "r"(mapa_shared(smem_u32(bar), cta))
+               : "memory");
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kPolicyThreads, 1)
+    policy_rows_kernel(const T* __restrict__ logits, T* __restrict__ grad, const Rows r, const Policy p, int ctas,
+                       bool resident, bool behind, double* partial, unsigned* arrived, float* out, int* status) {
+  constexpr int kN = Pack<T>::kN, kWarps = kPolicyWorkers / 32;
+  extern __shared__ __align__(128) unsigned char raw[];
+  PolicyShared& sh = *reinterpret_cast<PolicyShared*>(raw);
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int rank = ctas > 1 ? static_cast<int>(cluster_ctarank()) : 0;
+  const long long cluster = blockIdx.x / ctas, clusters = gridDim.x / ctas;
+  if (tid == 0) sh.init();
+  __syncthreads();
+  if (ctas > 1) cluster_sync_all();  // every CTA's barriers stand before another signals one
+  volatile int* abort = &sh.abort;
+  bool ok = true;
   auto wait = [&](uint64_t* bar, uint32_t parity) {  // the whole warp's
     ok = __all_sync(0xffffffffu, mbar_wait(bar, parity, abort));
     return ok;
@@ -714,350 +842,504 @@ __global__ void __launch_bounds__(kLongThreads, 2)
     }
   };
 
-  if (warp == kWorkerWarps) {  // ---- producer ----
-    int issued = 0;
-    auto push = [&](const Tile& t, const void* src) {  // (one thread's)
-      if (!ok || !mbar_wait(&sh.empty[stage], (round & 1) ^ 1, abort)) {
-        ok = false;
-        return;
-      }
-      sh.tile[stage] = t;
-      if (src != nullptr) {
-        mbar_expect_tx(&sh.full[stage], t.packs * 16);
-        bulk_load(sh.data[stage], src, t.packs * 16, &sh.full[stage]);
-      } else {
-        mbar_arrive(&sh.full[stage]);
-      }
-      ++issued;
-      advance();
+  if (warp == kWarps) {  // ---- producer: 32 rows' values at a time, asked for while the last 32 go by ----
+    Ring<PolicyShared, kPolicyStages> ring(sh);
+    Task next = {};
+    long long next_offset = 0;
+    auto ask = [&](long long base) {
+      next.row = base + lane * clusters;
+      next.kind = kEnd;
+      if (next.row >= r.rows) return;
+      next.b = next.row / r.length;
+      const long long t = next.row - next.b * r.length;
+      next_offset = next.b * r.stride_b + t * r.stride_t;
+      next.w = r.weights != nullptr ? r.weights[next.row] : 1.f;
+      next.kind = next.w != 0.f ? kStat : kZero;
+      if (next.kind == kZero) return;
+      const long long target = r.targets[next.row];
+      next.target = target >= 0 && target < r.vocab ? static_cast<int>(target) : -1;
+      next.in = policy_inputs(p, next.row, next.b, t);
+      next.x = next.target >= 0 ? Pack<T>::one(logits[next_offset + next.target]) : NAN;
     };
-    auto stream = [&](int kind, long long row) {
-      const T* x = logits + row_at(r, row);
-      int head, packs;
-      aligned_part(x, r.vocab, head, packs);
-      for (int at = 0; at < packs && ok; at += kTilePacks) {
-        const int n = packs - at < kTilePacks ? packs - at : kTilePacks;
-        push({row, kind, at, n, at + n == packs}, x + head + static_cast<long long>(at) * kN);
-      }
-    };
-    if (kPairs) {
-      if (lane == 0) {
-        const unsigned long long total = work.order.rows * (work.order.gradient ? 2 : 1);
-        auto weight = [&](unsigned long long t) {
-          bool g;
-          return t < total && r.weights != nullptr ? r.weights[task_of(work.order, t, g)] : 1.f;
-        };
-        unsigned long long ticket = atomicAdd(work.ticket, 1ull);
-        float w = weight(ticket);
-        while (ok && ticket < total) {
-          const unsigned long long next = atomicAdd(work.ticket, 1ull);  // (one ahead: the answer takes its time)
-          bool gradient;
-          const long long row = task_of(work.order, ticket, gradient);
-          if (w == 0.f)
-            push({row, gradient ? kZero : kSkip, 0, 0, 1}, nullptr);
-          else
-            stream(gradient ? kGrad : kStat, row);
-          ticket = next;
-          w = weight(ticket);
+    ask(cluster);
+    for (long long base = cluster; base < r.rows; base += 32 * clusters) {
+      const Task mine = next;
+      const long long offset = next_offset;
+      if (base + 32 * clusters < r.rows) ask(base + 32 * clusters);
+      for (int i = 0; i < 32; ++i) {
+        Task t;
+        t.row = base + i * clusters;
+        if (t.row >= r.rows) break;
+        t.b = __shfl_sync(0xffffffffu, mine.b, i);
+        t.kind = __shfl_sync(0xffffffffu, mine.kind, i);
+        t.target = __shfl_sync(0xffffffffu, mine.target, i);
+        t.w = __shfl_sync(0xffffffffu, mine.w, i);
+        t.x = __shfl_sync(0xffffffffu, mine.x, i);
+        t.in = {__shfl_sync(0xffffffffu, mine.in.old, i), __shfl_sync(0xffffffffu, mine.in.ref, i),
+                __shfl_sync(0xffffffffu, mine.in.advantage, i)};
+        Tile tile = {__shfl_sync(0xffffffffu, offset, i), t.kind, 1, 0, 0, 0, -1, 0};
+        if (lane != 0 || (t.kind == kZero && grad == nullptr)) continue;
+        int all;
+        aligned_part(logits + tile.offset, r.vocab, tile.head, all);
+        const int part = (all + ctas - 1) / ctas, from = part * rank < all ? part * rank : all;
+        const int packs = all - from < part ? all - from : part;
+        tile.outside = rank == 0 ? all : -1;
+        tile.at = from;
+        if (t.kind == kZero) {
+          tile.packs = packs;
+          ring.push(tile, nullptr);
+          continue;
+        }
+        tile.task = ring.tell(t);
+        ring.stream(tile, logits, from, packs);
+        if (!resident && grad != nullptr) {
+          tile.kind = kGrad;
+          ring.stream(tile, logits, from, packs);
         }
       }
-    } else {
-      long long before = -1;  // the row whose gradient is still to come
-      for (long long base = blockIdx.x; base < r.rows; base += 32ll * gridDim.x) {
-        const long long mine = base + static_cast<long long>(lane) * gridDim.x;
-        const float w = mine < r.rows && r.weights != nullptr ? r.weights[mine] : 1.f;
-        const unsigned visible = __ballot_sync(0xffffffffu, w != 0.f);
-        if (lane == 0) {
-          for (int i = 0; i < 32; ++i) {
-            const long long row = base + static_cast<long long>(i) * gridDim.x;
-            if (row >= r.rows || !ok) break;
-            if (visible >> i & 1) {
-              stream(kStat, row);
-              if (grad != nullptr && before >= 0) stream(kGrad, before);
-              before = row;
-            } else if (grad != nullptr) {
-              push({row, kZero, 0, 0, 1}, nullptr);
-            }
-          }
-        }
-        __syncwarp();
-      }
-      if (lane == 0 && grad != nullptr && before >= 0) stream(kGrad, before);
     }
     if (lane == 0) {
-      push({0, kEnd, 0, 0, 1}, nullptr);
-      if (!ok) {  // no copy may be under way when the shared memory is given back
+      Task end = {};
+      end.kind = kEnd;
+      ring.tell(end);
+      ring.push({0, kEnd, 1, 0, 0, 0, -1, 0}, nullptr);
+      if (!ring.ok) {
         give_up(kStatusTimeoutProducer);
-        const int n = issued < kStages ? issued : kStages;
-        for (int i = issued - n; i < issued; ++i)
-          for (uint32_t it = 0; it < kWaitLimit && !mbar_try_wait(&sh.full[i % kStages], (i / kStages) & 1); ++it) {
-          }
+        ring.drain();
       }
     }
-    return;
-  }
-
-  unsigned rows_summed = 0, rows_turned = 0;  // softmaxes and gradients so far
-  if (warp > kWorkerWarps) {  // ---- keeper ----
-    const float scale = kPairs ? 0.f : scale_of(p.normalizer, p.scale);
+  } else if (warp > kWarps) {  // ---- keeper ----
+    const float scale = scale_of(p.normalizer, p.scale);
     double sums[4] = {0.0, 0.0, 0.0, 0.0};
-    float w = 0.f, x = 0.f;  // weight and target's logit of the row under way
-    long long target = -1, known = -1;
-    float slope0 = 0.f;  // of the preferred row of the known pair
+    for (unsigned n = 0;; ++n) {
+      const int slot = n % kSlots;
+      const uint32_t parity = n / kSlots & 1;
+      if (!wait(&sh.told[slot], parity)) break;
+      const Task t = sh.task[slot];
+      if (t.kind == kEnd) break;
+      if (!wait(&sh.sums[slot], parity)) break;
+      Softmax s = join_row_lanes(lane < kWarps ? sh.part[slot][lane] : Softmax{-INFINITY, 0.f});
+      if (ctas > 1) {
+        if (lane == 0) mbar_expect_tx(&sh.met[slot], 8 * ctas);
+        __syncwarp();
+        if (lane < ctas) send_to_cta(&sh.of_cta[slot][rank], &sh.met[slot], lane, s);
+        if (!wait(&sh.met[slot], parity)) break;
+        s = join_row_lanes(lane < ctas ? sh.of_cta[slot][lane] : Softmax{-INFINITY, 0.f});
+      }
+      if (lane == 0) {
+        const PolicyToken c = policy_token(p, t.in, log_prob_of(t.x, s));
+        const float by = t.w * c.slope * scale;
+        sh.slope[slot] = {s.most, by, -by / s.sum, t.target};
+        mbar_arrive(&sh.said[slot]);
+        mbar_arrive(&sh.kept[slot]);
+        sums[0] += static_cast<double>(t.w) * c.loss;
+        sums[1] += static_cast<double>(t.w) * c.kl;
+        sums[2] += static_cast<double>(t.w) * c.clipped;
+        sums[3] += t.w;
+      }
+      __syncwarp();
+    }
+    if (!ok) give_up(kStatusTimeoutEpilogue);
+    unsigned before = 0;
+    if (lane == 0 && rank == 0) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) partial[cluster * 4 + i] = ok ? sums[i] : NAN;
+      __threadfence();
+      before = atomicAdd(arrived, 1u) + 1;
+    }
+    if (__shfl_sync(0xffffffffu, before, 0) == clusters) {
+      __threadfence();
+      const double whole = p.normalizer != nullptr ? 1.0 / static_cast<double>(*p.normalizer) : p.scale;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        double v = 0.0;
+        for (long long c = lane; c < clusters; c += 32) v += __ldcg(partial + c * 4 + i);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+        if (lane == 0) out[i] = static_cast<float>(i < 2 ? v * whole : v);
+      }
+    }
+  } else {  // ---- workers ----
+    int stage = 0;
+    uint32_t round = 0;
+    auto advance = [&](int& s, uint32_t& n) {
+      if (++s == kPolicyStages) s = 0, ++n;
+    };
+    auto release = [&](int s) {
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sh.empty[s]);
+    };
+    const bool keep = resident && grad != nullptr;  // the sums leave the tiles where they are
+    // The gradient of the row whose tiles begin at the stage; leaves the stage behind them.
+    auto turn_row = [&](int& s, uint32_t& n) {
+      Slope now = {0.f, 0.f, 0.f, -1};
+      for (bool first = true;; first = false) {
+        if (!wait(&sh.full[s], n & 1)) return;
+        const Tile t = sh.tile[s];
+        const T* row = logits + t.offset;
+        if (first) {
+          if (!wait(&sh.said[t.task % kSlots], t.task / kSlots & 1)) return;
+          now = sh.slope[t.task % kSlots];
+          const int i = outside_of<T>(t, r.vocab, tid);
+          if (i >= 0) turn_one(grad + t.offset, row, i, now);
+        }
+        turn_tile<T, kPolicyWorkers>(grad + t.offset, sh.data[s], t, now, tid);
+        release(s);
+        advance(s, n);
+        if (t.last) return;
+      }
+    };
+    int old_stage = 0;  // of the row whose gradient is still to come
+    uint32_t old_round = 0;
+    bool old = false;
+    while (ok && wait(&sh.full[stage], round & 1)) {
+      Tile t = sh.tile[stage];
+      if (t.kind != kStat && old) {  // (a row's tiles may need the room of the one before)
+        old = false;
+        turn_row(old_stage, old_round);
+        if (!ok) break;
+      }
+      if (t.kind == kEnd) break;
+      if (t.kind == kZero) {
+        release(stage);
+        advance(stage, round);
+        T* g = grad + t.offset;
+        for (int i = tid; i < t.packs; i += kPolicyWorkers)
+          *reinterpret_cast<uint4*>(g + t.head + static_cast<long long>(t.at + i) * kN) = make_uint4(0, 0, 0, 0);
+        const int i = outside_of<T>(t, r.vocab, tid);
+        if (i >= 0) g[i] = Pack<T>::back(0.f);
+        continue;
+      }
+      if (t.kind == kGrad) {
+        turn_row(stage, round);
+        continue;
+      }
+      int first_stage = stage;
+      uint32_t first_round = round;
+      Softmax seen = {-INFINITY, 0.f};
+      const int i = outside_of<T>(t, r.vocab, tid);
+      if (i >= 0) seen = one_value(logits[t.offset + i]);
+      while (true) {
+        sum_tile<T, kPolicyWorkers>(seen, sh.data[stage], t.packs, tid);
+        if (!keep) release(stage);
+        advance(stage, round);
+        if (t.last || !wait(&sh.full[stage], round & 1)) break;
+        t = sh.tile[stage];
+      }
+      if (!ok) break;
+      const Softmax s = join_row_lanes(seen);
+      if (lane == 0) {
+        sh.part[t.task % kSlots][warp] = s;
+        mbar_arrive(&sh.sums[t.task % kSlots]);
+      }
+      if (!keep) continue;
+      if (old) turn_row(old_stage, old_round);
+      old = behind;
+      old_stage = first_stage;
+      old_round = first_round;
+      if (!behind) turn_row(first_stage, first_round);
+    }
+    if (!ok) give_up(kStatusTimeoutEpilogue);
+  }
+  if (ctas > 1) {
+    __syncwarp();
+    cluster_sync_all();  // no CTA ends while another may still write to it
+  }
+}
+
+// Preference. The slope of a row needs the sums of all rows of its pair. The tasks (a row's sums, a row's
+// gradient) stand in an order in which a group of pairs is followed by the next group's sums and then its
+// own gradients, whose logits are still in L2; a CTA takes the next task by a ticket. What a gradient waits
+// for has smaller tickets, is therefore done or under way, and waits itself for smaller tickets at most. A
+// row's results are 8-byte words, zero until they are there: who needs a pair reads its words until none
+// of those that count is zero. (Counting the rows done would need a fence a row, which takes microseconds
+// while the memory is busy: 355 us against ... for 64 x 114 x 32128.)
+constexpr int kPairStages = 6;
+constexpr int kPairWorkers = 256;
+constexpr int kPairThreads = kPairWorkers + 64;
+using PairShared = LongShared<kPairStages, kPairWorkers / 32>;
+
+struct Order {
+  long long rows, group;  // rows of the batch, of a group of pairs
+  bool behind;            // a group's gradients follow the next group's sums
+  bool gradient;
+};
+// (row, is it the gradient's turn) of a ticket below rows * (1 + gradient)
+__device__ __forceinline__ long long task_of(const Order& o, long long ticket, bool& gradient) {
+  gradient = false;
+  if (!o.gradient) return ticket;
+  const long long last = (o.rows - 1) / o.group * o.group;  // first row of the last group
+  if (!o.behind) {  // sums of a group, then its gradients, those last read first
+    const long long k = ticket / (2 * o.group), first = k * o.group, at = ticket - 2 * first;
+    const long long n = o.rows - first < o.group ? o.rows - first : o.group;
+    gradient = at >= n;
+    return gradient ? first + 2 * n - 1 - at : first + at;
+  }
+  gradient = ticket >= o.rows + last;
+  if (gradient) return ticket - o.rows;  // of the last group
+  if (ticket < o.group) return ticket;
+  const long long k = (ticket - o.group) / (2 * o.group) + 1;  // sums of group k, gradients of k - 1
+  const long long at = ticket - o.group - (k - 1) * 2 * o.group, first = k * o.group;
+  const long long n = o.rows - first < o.group ? o.rows - first : o.group;
+  gradient = at >= n;
+  return gradient ? first - o.group + (at - n) : first + at;
+}
+
+struct Work {
+  unsigned long long* ticket;
+  unsigned* pairs_done;
+  unsigned long long *softmax, *score;  // a row's {largest, sum} and {log-probability, 1}
+  double* pair_loss;
+  float *scores, *margins;
+  Order order;
+};
+
+__device__ __forceinline__ unsigned long long ld_word(const unsigned long long* p) {
+  unsigned long long v;
+  asm volatile("ld.relaxed.gpu.global.u64 %0, [%1];" : "=l"(v) : "l"(p) : "memory");
+  return v;
+}
+__device__ __forceinline__ void st_word(unsigned long long* p, unsigned long long v) {
+  asm volatile("st.relaxed.gpu.global.u64 [%0], %1;" ::"l"(p), "l"(v) : "memory");
+}
+__device__ __forceinline__ unsigned long long word_of(float low, uint32_t high) {
+  return static_cast<unsigned long long>(high) << 32 | __float_as_uint(low);
+}
+
+// A keeper's: the pair's margin, once all of its rows have their words. `writes`: stores what the pair gives
+// and, for the last pair, the loss.
+__device__ __forceinline__ bool pair_slope(const Rows& r, const Preference& q, const Work& work, long long pair,
+                                           bool writes, volatile int* abort, float* out, float& slope) {
+  const int lane = threadIdx.x & 31;
+  double sum[2];
+  bool seen;
+  for (uint32_t it = 0;; ++it) {
+    bool missing = false;
+    seen = false;
+#pragma unroll
+    for (int side = 0; side < 2; ++side) {
+      const long long first = (2 * pair + side) * r.length;
+      sum[side] = 0.0;
+#pragma unroll 8
+      for (int i = lane; i < r.length; i += 32) {
+        const float w = r.weights != nullptr ? r.weights[first + i] : 1.f;
+        const unsigned long long v = ld_word(work.score + first + i);
+        if (w != 0.f) {
+          sum[side] += static_cast<double>(w) * __uint_as_float(static_cast<uint32_t>(v));
+          seen = true;
+          missing = missing || v == 0;
+        }
+      }
+    }
+    if (!__any_sync(0xffffffffu, missing)) break;
+    if (__any_sync(0xffffffffu, it == kWaitLimit >> 4 || *abort)) return false;
+    __nanosleep(100);
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    sum[0] += __shfl_xor_sync(0xffffffffu, sum[0], o);
+    sum[1] += __shfl_xor_sync(0xffffffffu, sum[1], o);
+  }
+  const bool real = __any_sync(0xffffffffu, seen);
+  const Margin m = pair_margin(q, real, sum[0], sum[1], q.ref[2 * pair], q.ref[2 * pair + 1],
+                               scale_of(q.normalizer, q.scale));
+  slope = m.slope;
+  if (!writes) return true;
+  unsigned before = 0;
+  if (lane == 0) {
+    work.scores[2 * pair] = static_cast<float>(sum[0]);
+    work.scores[2 * pair + 1] = static_cast<float>(sum[1]);
+    work.margins[pair] = static_cast<float>(m.margin);
+    work.pair_loss[2 * pair] = m.loss;
+    work.pair_loss[2 * pair + 1] = real ? 1.0 : 0.0;
+    __threadfence();
+    before = atomicAdd(work.pairs_done, 1u);
+  }
+  const long long pairs = r.rows / r.length / 2;
+  if (__shfl_sync(0xffffffffu, before, 0) != pairs - 1) return true;
+  __threadfence();
+  double loss = 0.0, count = 0.0;
+  for (long long i = lane; i < pairs; i += 32) {
+    loss += __ldcg(work.pair_loss + 2 * i);
+    count += __ldcg(work.pair_loss + 2 * i + 1);
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    loss += __shfl_xor_sync(0xffffffffu, loss, o);
+    count += __shfl_xor_sync(0xffffffffu, count, o);
+  }
+  if (lane == 0) {
+    const double whole = q.normalizer != nullptr ? 1.0 / static_cast<double>(*q.normalizer) : q.scale;
+    out[0] = static_cast<float>(loss * whole);
+    out[1] = static_cast<float>(count);
+  }
+  return true;
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kPairThreads, 2)
+    preference_rows_kernel(const T* __restrict__ logits, T* __restrict__ grad, const Rows r, const Preference q,
+                           const Work work, float* out, int* status) {
+  constexpr int kWarps = kPairWorkers / 32;
+  extern __shared__ __align__(128) unsigned char raw[];
+  PairShared& sh = *reinterpret_cast<PairShared*>(raw);
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  if (tid == 0) sh.init();
+  __syncthreads();
+  volatile int* abort = &sh.abort;
+  bool ok = true;
+  auto wait = [&](uint64_t* bar, uint32_t parity) {  // the whole warp's
+    ok = __all_sync(0xffffffffu, mbar_wait(bar, parity, abort));
+    return ok;
+  };
+  auto give_up = [&](int code) {
+    if (lane == 0) {
+      *abort = 1;
+      report_status(status, code, 42, warp);
+    }
+  };
+
+  if (warp == kWarps) {  // ---- producer ----
+    if (lane != 0) return;
+    Ring<PairShared, kPairStages> ring(sh);
+    const long long total = work.order.rows * (work.order.gradient ? 2 : 1);
+    // Three tasks are under way: of one the ticket has been asked for, of the next the weight and the target, of
+    // the next the target's logit; nobody waits for any of these.
+    struct Asked {
+      Task t;
+      long long offset, target;
+    };
+    auto ask = [&](long long ticket) {
+      Asked a = {};
+      a.t.row = -1;
+      if (ticket >= total) return a;
+      bool gradient;
+      a.t.row = task_of(work.order, ticket, gradient);
+      a.t.b = a.t.row / r.length;
+      a.t.kind = gradient ? kGrad : kStat;
+      a.offset = a.t.b * r.stride_b + (a.t.row - a.t.b * r.length) * r.stride_t;
+      a.t.w = r.weights != nullptr ? r.weights[a.t.row] : 1.f;
+      a.target = r.targets[a.t.row];
+      return a;
+    };
+    auto ask_logit = [&](Asked& a) {
+      if (a.t.row < 0) return;
+      a.t.target = a.target >= 0 && a.target < r.vocab ? static_cast<int>(a.target) : -1;
+      a.t.x = NAN;
+      if (a.t.kind == kStat && a.t.w != 0.f && a.t.target >= 0) a.t.x = Pack<T>::one(logits[a.offset + a.t.target]);
+    };
+    Asked now = ask(static_cast<long long>(atomicAdd(work.ticket, 1ull)));
+    Asked next = ask(static_cast<long long>(atomicAdd(work.ticket, 1ull)));
+    ask_logit(now);
+    while (now.t.row >= 0 && ring.ok) {
+      const long long ticket = static_cast<long long>(atomicAdd(work.ticket, 1ull));
+      ask_logit(next);
+      Tile tile = {now.offset, now.t.kind, 1, 0, 0, 0, -1, 0};
+      int all;
+      aligned_part(logits + now.offset, r.vocab, tile.head, all);
+      if (now.t.w != 0.f) {
+        tile.outside = all;
+        tile.task = ring.tell(now.t);
+        ring.stream(tile, logits, 0, all);
+      } else if (now.t.kind == kGrad) {
+        tile.kind = now.t.kind = kZero;
+        if (now.t.row % (2 * r.length) == 0) ring.tell(now.t);  // (whose keeper writes what the pair gives)
+        ring.push(tile, nullptr);
+      }
+      now = next;
+      next = ask(ticket);
+    }
+    Task end = {};
+    end.kind = kEnd;
+    ring.tell(end);
+    ring.push({0, kEnd, 1, 0, 0, 0, -1, 0}, nullptr);
+    if (!ring.ok) {
+      give_up(kStatusTimeoutProducer);
+      ring.drain();
+    }
+  } else if (warp > kWarps) {  // ---- keeper ----
+    long long known = -1;  // a pair, and the slope of its preferred row
+    float slope = 0.f;
+    for (unsigned n = 0;; ++n) {
+      const int slot = n % kSlots;
+      const uint32_t parity = n / kSlots & 1;
+      if (!wait(&sh.told[slot], parity)) break;
+      const Task t = sh.task[slot];
+      if (t.kind == kEnd) break;
+      if (t.kind == kStat) {
+        if (!wait(&sh.sums[slot], parity)) break;
+        const Softmax s = join_row_lanes(lane < kWarps ? sh.part[slot][lane] : Softmax{-INFINITY, 0.f});
+        if (lane == 0) {
+          st_word(work.score + t.row, word_of(log_prob_of(t.x, s), 1));
+          st_word(work.softmax + t.row, word_of(s.most, __float_as_uint(s.sum)));
+        }
+      } else {
+        const long long pair = t.b / 2;
+        const bool writes = t.row == pair * 2 * r.length;
+        if (pair != known || writes) {
+          ok = pair_slope(r, q, work, pair, writes, abort, out, slope);
+          if (!ok) break;
+          known = pair;
+        }
+        if (t.kind == kGrad) {
+          // (of an own or an earlier task's row: its word stands beside the score's, which is there)
+          unsigned long long v = 0;
+          for (uint32_t it = 0; it < kWaitLimit && (v = ld_word(work.softmax + t.row)) == 0 && !*abort; ++it)
+            __nanosleep(20);
+          ok = __all_sync(0xffffffffu, v != 0);
+          if (!ok) break;
+          if (lane == 0) {
+            const float by = t.w * (t.b & 1 ? -slope : slope);
+            sh.slope[slot] = {__uint_as_float(static_cast<uint32_t>(v)), by,
+                              -by / __uint_as_float(static_cast<uint32_t>(v >> 32)), t.target};
+          }
+        }
+        if (lane == 0)  // (the phases of all of a slot's barriers go on together)
+          for (int i = 0; i < kWarps; ++i) mbar_arrive(&sh.sums[slot]);
+      }
+      if (lane == 0) {
+        mbar_arrive(&sh.said[slot]);
+        mbar_arrive(&sh.kept[slot]);
+      }
+      __syncwarp();
+    }
+    if (!ok) give_up(kStatusTimeoutPeerFlag);
+  } else {  // ---- workers ----
+    int stage = 0;
+    uint32_t round = 0;
+    Softmax seen = {-INFINITY, 0.f};  // of the row whose sums are under way
+    Slope now = {0.f, 0.f, 0.f, -1};  // of the row whose gradient is under way
     while (wait(&sh.full[stage], round & 1)) {
       const Tile t = sh.tile[stage];
       if (t.kind == kEnd) break;
-      const long long b = t.row / r.length;
+      const int outside = outside_of<T>(t, r.vocab, tid);
       if (t.kind == kStat) {
-        if (t.at == 0 && lane == 0) {  // (asked for while the row is summed)
-          const T* row = logits + row_at(r, t.row);
-          target = r.targets[t.row];
-          w = r.weights != nullptr ? r.weights[t.row] : 1.f;
-          x = target >= 0 && target < r.vocab ? Pack<T>::one(row[target]) : NAN;
+        if (outside >= 0) seen = one_value(logits[t.offset + outside]);
+        sum_tile<T, kPairWorkers>(seen, sh.data[stage], t.packs, tid);
+      } else if (t.kind == kGrad) {
+        if (t.outside >= 0) {  // the row's first tile
+          if (!wait(&sh.said[t.task % kSlots], t.task / kSlots & 1)) break;
+          now = sh.slope[t.task % kSlots];
+          if (outside >= 0) turn_one(grad + t.offset, logits + t.offset, outside, now);
         }
-        if (t.last) {
-          const int slot = rows_summed % kSlots;
-          if (!wait(&sh.sums[slot], rows_summed / kSlots & 1)) break;
-          const Softmax s = join_row_lanes(lane < kWorkerWarps ? sh.part[slot][lane] : Softmax{-INFINITY, 0.f});
-          if (lane == 0) {
-            const float logp = log_prob_of(x, s);
-            if (kPairs) {
-              work.softmax[t.row] = s;
-              work.logp[t.row] = logp;
-              red_release_gpu_add(work.done + b / 2, 1u);
-            } else {
-              const PolicyToken c = policy_token(p, t.row, b, t.row - b * r.length, logp);
-              sums[0] += static_cast<double>(w) * c.loss;
-              sums[1] += static_cast<double>(w) * c.kl;
-              sums[2] += static_cast<double>(w) * c.clipped;
-              sums[3] += w;
-              const float by = w * c.slope * scale;
-              sh.slope[slot] = {s.most, by, -by / s.sum,
-                                target >= 0 && target < r.vocab ? static_cast<int>(target) : -1};
-              mbar_arrive(&sh.said[slot]);
-            }
-          }
-          ++rows_summed;
-        }
-      } else if (kPairs && t.at == 0) {
-        const long long pair = b / 2;
-        if (t.kind == kSkip) {
-          if (lane == 0) red_release_gpu_add(work.done + pair, 1u);
-        } else {
-          const bool turned = t.kind == kGrad;
-          const bool writes = t.row == pair * 2 * r.length;  // one row of a pair writes what the pair gives
-          if (pair != known && (turned || writes)) {
-            uint32_t it = 0;
-            while (ld_acquire_gpu(work.done + pair) != 2u * r.length) {
-              if (++it == kWaitLimit || *abort) {
-                ok = false;
-                break;
-              }
-              __nanosleep(20);
-            }
-            ok = __all_sync(0xffffffffu, ok);
-            if (!ok) break;
-            double sum[2] = {0.0, 0.0};
-            bool seen = false;
-#pragma unroll
-            for (int side = 0; side < 2; ++side) {
-              const long long first = (2 * pair + side) * r.length;
-#pragma unroll 4
-              for (int i = lane; i < r.length; i += 32) {
-                const float wt = r.weights != nullptr ? r.weights[first + i] : 1.f;
-                const float lp = __ldcg(work.logp + first + i);
-                if (wt != 0.f) {
-                  sum[side] += static_cast<double>(wt) * lp;
-                  seen = true;
-                }
-              }
-#pragma unroll
-              for (int o = 16; o > 0; o >>= 1) sum[side] += __shfl_xor_sync(0xffffffffu, sum[side], o);
-            }
-            const bool real = __any_sync(0xffffffffu, seen);
-            const Margin m = pair_margin(q, real, sum[0], sum[1], q.ref[2 * pair], q.ref[2 * pair + 1],
-                                         scale_of(q.normalizer, q.scale));
-            slope0 = static_cast<float>(m.slope);
-            known = pair;
-            if (writes) {
-              unsigned before = 0;
-              if (lane == 0) {
-                work.scores[2 * pair] = static_cast<float>(sum[0]);
-                work.scores[2 * pair + 1] = static_cast<float>(sum[1]);
-                work.margins[pair] = static_cast<float>(m.margin);
-                work.pair_loss[2 * pair] = m.loss;
-                work.pair_loss[2 * pair + 1] = real ? 1.0 : 0.0;
-                __threadfence();
-                before = atomicAdd(work.pairs_done, 1u);
-              }
-              const long long pairs = r.rows / r.length / 2;
-              if (__shfl_sync(0xffffffffu, before, 0) == pairs - 1) {
-                __threadfence();
-                double loss = 0.0, count = 0.0;
-                for (long long i = lane; i < pairs; i += 32) {
-                  loss += __ldcg(work.pair_loss + 2 * i);
-                  count += __ldcg(work.pair_loss + 2 * i + 1);
-                }
-#pragma unroll
-                for (int o = 16; o > 0; o >>= 1) {
-                  loss += __shfl_xor_sync(0xffffffffu, loss, o);
-                  count += __shfl_xor_sync(0xffffffffu, count, o);
-                }
-                if (lane == 0) {
-                  const double whole = q.normalizer != nullptr ? 1.0 / static_cast<double>(*q.normalizer) : q.scale;
-                  out[0] = static_cast<float>(loss * whole);
-                  out[1] = static_cast<float>(count);
-                }
-              }
-            }
-          }
-          if (turned) {
-            if (lane == 0) {
-              const long long at = r.targets[t.row];
-              const float wt = r.weights != nullptr ? r.weights[t.row] : 1.f;
-              const float most = __ldcg(&work.softmax[t.row].most), sum = __ldcg(&work.softmax[t.row].sum);
-              const float by = wt * (b & 1 ? -slope0 : slope0);
-              const int slot = rows_turned % kSlots;
-              sh.slope[slot] = {most, by, -by / sum, at >= 0 && at < r.vocab ? static_cast<int>(at) : -1};
-              mbar_arrive(&sh.said[slot]);
-            }
-            ++rows_turned;
-          }
-        }
+        turn_tile<T, kPairWorkers>(grad + t.offset, sh.data[stage], t, now, tid);
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(&sh.empty[stage]);
-      advance();
-    }
-    if (!ok) {
-      give_up(kStatusTimeoutEpilogue);
-      return;
-    }
-    if (kPairs) return;
-    unsigned before = 0;
-    if (lane == 0) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) partial[blockIdx.x * 4 + i] = sums[i];
-      __threadfence();
-      before = atomicAdd(arrived, 1u);
-    }
-    if (__shfl_sync(0xffffffffu, before, 0) != gridDim.x - 1) return;
-    __threadfence();
-    const double whole = p.normalizer != nullptr ? 1.0 / static_cast<double>(*p.normalizer) : p.scale;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      double v = 0.0;
-      for (unsigned c = lane; c < gridDim.x; c += 32) v += __ldcg(partial + c * 4 + i);
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-      if (lane == 0) out[i] = static_cast<float>(i < 2 ? v * whole : v);
-    }
-    return;
-  }
-
-  // ---- workers ----
-  Softmax seen = {-INFINITY, 0.f};       // of the row whose softmax is under way
-  Slope now = {0.f, 0.f, 0.f, -1};       // of the row whose gradient is under way
-  while (wait(&sh.full[stage], round & 1)) {
-    const Tile t = sh.tile[stage];
-    if (t.kind == kEnd) break;
-    const unsigned char* data = sh.data[stage];
-    const T* row = logits + row_at(r, t.row);
-    int head = 0, outside = -1;  // the value outside of the aligned part that this thread sees to
-    if (t.kind == kStat || t.kind == kGrad) {
-      int packs;
-      aligned_part(row, r.vocab, head, packs);
-      if (t.at == 0) {
-        const int i = tid < head ? tid : packs * kN + tid;  // (head + packs * kN + tid - head)
-        if (i < r.vocab && (tid < head || tid < r.vocab - packs * kN)) outside = i;
-      }
-    }
-    if (t.kind == kStat) {
-      if (outside >= 0) {
-        const float v = Pack<T>::one(row[outside]);
-        seen = {v, v == -INFINITY ? 0.f : v * 0.f + 1.f};  // (NaN of +inf and NaN)
-      }
-      if (t.packs == kTilePacks) {
-        constexpr int kMine = kTilePacks / kWorkers;
-        Pairs<T> x[kMine];
-#pragma unroll
-        for (int i = 0; i < kMine; ++i) x[i].load(data + (tid + i * kWorkers) * 16);
-        take<T, kMine>(seen, x);
-      } else {
-        for (int i = tid; i < t.packs; i += kWorkers) {
-          Pairs<T> x[1];
-          x[0].load(data + i * 16);
-          take<T, 1>(seen, x);
-        }
-      }
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&sh.empty[stage]);
-      if (t.last) {
+      if (++stage == kPairStages) stage = 0, ++round;
+      if (t.kind == kStat && t.last) {
         const Softmax s = join_row_lanes(seen);
         if (lane == 0) {
-          const int slot = rows_summed % kSlots;
-          sh.part[slot][warp] = s;
-          mbar_arrive(&sh.sums[slot]);
+          sh.part[t.task % kSlots][warp] = s;
+          mbar_arrive(&sh.sums[t.task % kSlots]);
         }
-        ++rows_summed;
         seen = {-INFINITY, 0.f};
+      } else if (t.kind == kZero) {
+        row_zero(grad + t.offset, r.vocab, tid, kPairWorkers);
       }
-    } else if (t.kind == kGrad) {
-      T* g = grad + row_at(r, t.row);
-      if (t.at == 0) {
-        const int slot = rows_turned % kSlots;
-        if (!wait(&sh.said[slot], rows_turned / kSlots & 1)) break;
-        now = sh.slope[slot];
-        ++rows_turned;
-        if (outside >= 0) {
-          const float v = now.k * exp_from(Pack<T>::one(row[outside]), now.most);
-          g[outside] = Pack<T>::back(outside == now.target ? v + now.by : v);
-        }
-      }
-      const int first = head + t.at * kN;
-      const float ref = __fmul_rn(now.most, kLog2e);
-      const bool far = huge(now.most);
-      const uint64_t l2e = pair_of(kLog2e, kLog2e), off = pair_of(-ref, -ref), k2 = pair_of(now.k, now.k);
-      auto one = [&](int i) {
-        Pairs<T> v;
-        v.load(data + i * 16);
-        float x[kN];
-#pragma unroll
-        for (int j = 0; j < kN / 2; ++j) {
-          float a, b;
-          if (far) {
-            split(v.v[j], a, b);
-            a = exp_from(a, now.most), b = exp_from(b, now.most);
-          } else {
-            split(fma2(v.v[j], l2e, off), a, b);
-            a = exp2_approx(a), b = exp2_approx(b);
-          }
-          split(mul2(pair_of(a, b), k2), x[2 * j], x[2 * j + 1]);
-        }
-        const int at = first + i * kN;
-        if (static_cast<unsigned>(now.target - at) < static_cast<unsigned>(kN)) {
-#pragma unroll
-          for (int j = 0; j < kN; ++j)
-            if (now.target == at + j) x[j] += now.by;
-        }
-        Pack<T>::store(g + at, x);
-      };
-      if (t.packs == kTilePacks) {
-#pragma unroll
-        for (int i = 0; i < kTilePacks / kWorkers; ++i) one(tid + i * kWorkers);
-      } else {
-        for (int i = tid; i < t.packs; i += kWorkers) one(i);
-      }
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&sh.empty[stage]);
-    } else {
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&sh.empty[stage]);
-      if (t.kind == kZero) row_zero(grad + row_at(r, t.row), r.vocab, tid, kWorkers);
     }
-    advance();
+    if (!ok) give_up(kStatusTimeoutEpilogue);
   }
-  if (!ok) give_up(kStatusTimeoutEpilogue);
 }
 
 // grad *= *factor; nothing where the factor is 1, as it is behind `loss.backward()`. dst may be src.
@@ -1102,22 +1384,64 @@ int launched(const char* what, int n) {
   return 0;
 }
 
-unsigned long_grid(long long rows) {
-  const long long cap = static_cast<long long>(num_sms()) * 2;
-  return static_cast<unsigned>(rows < 1 ? 1 : (rows < cap ? rows : cap));
+template <typename T>
+int launch_policy(const void* logits, void* grad, const Rows& r, const Policy& p, double* partial, unsigned* arrived,
+                  float* out, cudaStream_t st) {
+  // The smallest cluster whose CTAs' parts leave room for two more in the ring (four tiles; the largest
+  // cluster's may be larger).
+  const long long bytes = static_cast<long long>(r.vocab) * sizeof(T);
+  int ctas = 1;
+  while (ctas < 8 && (bytes + ctas - 1) / ctas > 4 * kTileBytes) ctas *= 2;
+  if (grad == nullptr) ctas = 1;  // (nothing has to stay)
+  const int tiles = static_cast<int>((bytes / 16 / ctas + 1 + kTilePacks - 1) / kTilePacks);
+  const bool resident = tiles <= kPolicyStages, behind = 2 * tiles <= kPolicyStages;
+  auto kernel = policy_rows_kernel<T>;
+  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, sizeof(PolicyShared));
+  if (e != cudaSuccess) return set_error("policy_loss: %s", cudaGetErrorString(e));
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(ctas));
+  cfg.blockDim = dim3(kPolicyThreads);
+  cfg.dynamicSmemBytes = sizeof(PolicyShared);
+  cfg.stream = st;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = ctas;
+  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = ctas > 1 ? 1 : 0;
+  // As many clusters as run at once: the rows are dealt out beforehand. (A cluster lies within a group of SMs,
+  // whose size need not be a multiple of the cluster's.)
+  static std::atomic<int> at_once[64][4];
+  int dev = 0, size = ctas == 1 ? 0 : ctas == 2 ? 1 : ctas == 4 ? 2 : 3;
+  cudaGetDevice(&dev);
+  int cap = at_once[dev][size].load(std::memory_order_relaxed);
+  if (cap == 0) {
+    cap = num_sms();
+    if (ctas > 1) {
+      e = cudaOccupancyMaxActiveClusters(&cap, kernel, &cfg);
+      if (e != cudaSuccess) return set_error("policy_loss: %s", cudaGetErrorString(e));
+    }
+    if (cap < 1) cap = 1;
+    at_once[dev][size].store(cap, std::memory_order_relaxed);
+  }
+  cfg.gridDim = dim3(static_cast<unsigned>((r.rows < cap ? r.rows : cap) * ctas));
+  e = cudaLaunchKernelEx(&cfg, kernel, static_cast<const T*>(logits), static_cast<T*>(grad), r, p, ctas, resident,
+                         behind, partial, arrived, out, device_status_buffer());
+  if (e != cudaSuccess) return set_error("policy_loss: %s", cudaGetErrorString(e));
+  return launched("policy_loss", 1);
 }
 
-template <typename T, bool kPairs>
-int launch_long(const char* what, const void* logits, void* grad, const Rows& r, const Policy& p, const Preference& q,
-                const Work& work, double* partial, unsigned* arrived, float* out, cudaStream_t st) {
-  auto kernel = long_rows_kernel<T, kPairs>;
+template <typename T>
+int launch_preference(const void* logits, void* grad, const Rows& r, const Preference& p, const Work& work, float* out,
+                      cudaStream_t st) {
+  auto kernel = preference_rows_kernel<T>;
   const cudaError_t e =
-      cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, sizeof(LongShared));
-  if (e != cudaSuccess) return set_error("%s: %s", what, cudaGetErrorString(e));
-  kernel<<<long_grid(r.rows), kLongThreads, sizeof(LongShared), st>>>(
-      static_cast<const T*>(logits), static_cast<T*>(grad), r, p, q, work, partial, arrived, out,
-      device_status_buffer());
-  return launched(what, 1);
+      cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, sizeof(PairShared));
+  if (e != cudaSuccess) return set_error("preference_loss: %s", cudaGetErrorString(e));
+  const long long cap = static_cast<long long>(num_sms()) * 2;
+  kernel<<<static_cast<unsigned>(r.rows < cap ? r.rows : cap), kPairThreads, sizeof(PairShared), st>>>(
+      static_cast<const T*>(logits), static_cast<T*>(grad), r, p, work, out, device_status_buffer());
+  return launched("preference_loss", 1);
 }
 
 // The order of the tasks of a preference loss: a pair of up to kBehindBytes of logits stands in a group of
@@ -1156,8 +1480,9 @@ T5X_API int t5x_policy_loss(const void* logits, int fp32, void* grad, long long 
                     kl_weight, scale, static_cast<const float*>(normalizer)};
   float* o = static_cast<float*>(out);
   if (static_cast<long long>(vocab) * (fp32 ? 4 : 2) >= kShortRow)
-    return fp32 ? launch_long<float, false>("policy_loss", logits, grad, r, p, {}, {}, partial, arrived, o, st)
-                : launch_long<__nv_bfloat16, false>("policy_loss", logits, grad, r, p, {}, {}, partial, arrived, o, st);
+    return r.rows == 0 ? set_error("policy_loss: no rows")
+           : fp32      ? launch_policy<float>(logits, grad, r, p, partial, arrived, o, st)
+                       : launch_policy<__nv_bfloat16>(logits, grad, r, p, partial, arrived, o, st);
   const unsigned grid = row_grid(r.rows);
   if (fp32)
     policy_short_rows_kernel<<<grid, kRowThreads, 0, st>>>(static_cast<const float*>(logits),
@@ -1192,9 +1517,9 @@ T5X_API int t5x_policy_loss_tokens(const void* logp, void* slope, long long batc
 }
 
 T5X_API long long t5x_preference_loss_scratch_bytes(long long batch, int length) {
-  // head | counts and flags of the pairs | loss and count of each pair | largest and sum of each token |
-  // log-probability | slope of each row
-  return static_cast<long long>(kHead) + batch / 2 * 8 + batch * 8 + batch * length * 12 + batch * 4;
+  // head | softmax and log-probability of each token, a word each | loss and count of each pair | slope of
+  // each row
+  return static_cast<long long>(kHead) + batch * length * 16 + batch * 8 + batch * 4;
 }
 
 T5X_API int t5x_preference_loss(const void* logits, int fp32, void* grad, long long batch, int length, int vocab,
@@ -1216,38 +1541,40 @@ T5X_API int t5x_preference_loss(const void* logits, int fp32, void* grad, long l
   Work w;
   w.ticket = reinterpret_cast<unsigned long long*>(at);
   w.pairs_done = reinterpret_cast<unsigned*>(at + 8);
-  w.done = reinterpret_cast<unsigned*>(at + kHead);
-  w.pair_loss = reinterpret_cast<double*>(at + kHead + pairs * 8);
-  w.softmax = reinterpret_cast<Softmax*>(w.pair_loss + batch);
-  w.logp = reinterpret_cast<float*>(w.softmax + r.rows);
-  float* by = w.logp + r.rows;
+  w.softmax = reinterpret_cast<unsigned long long*>(at + kHead);
+  w.score = w.softmax + r.rows;
+  w.pair_loss = reinterpret_cast<double*>(w.score + r.rows);
+  float* by = reinterpret_cast<float*>(w.pair_loss + batch);
   w.scores = static_cast<float*>(scores);
   w.margins = static_cast<float*>(margins);
   float* o = static_cast<float*>(out);
   const long long row_bytes = static_cast<long long>(vocab) * (fp32 ? 4 : 2);
   const bool in_long = row_bytes >= kShortRow;
-  cudaError_t e = cudaMemsetAsync(scratch, 0, kHead + (in_long ? pairs * 8 : 0), st);
+  cudaError_t e = cudaMemsetAsync(scratch, 0, kHead + (in_long ? r.rows * 16 : 0), st);
   if (e != cudaSuccess) return set_error("preference_loss: memset: %s", cudaGetErrorString(e));
   if (in_long) {
     const long long pair_bytes = 2 * length * row_bytes;
     const long long group = kGroupBytes / pair_bytes > 1 ? kGroupBytes / pair_bytes : 1;
     w.order = {r.rows, (group < pairs ? group : pairs) * 2 * length, pair_bytes <= kBehindBytes, grad != nullptr};
-    if (fp32 ? launch_long<float, true>("preference_loss", logits, grad, r, {}, p, w, nullptr, nullptr, o, st)
-             : launch_long<__nv_bfloat16, true>("preference_loss", logits, grad, r, {}, p, w, nullptr, nullptr, o, st))
+    if (fp32 ? launch_preference<float>(logits, grad, r, p, w, o, st)
+             : launch_preference<__nv_bfloat16>(logits, grad, r, p, w, o, st))
       return -1;
     if (grad != nullptr) return 0;
     preference_pairs_kernel<<<static_cast<unsigned>(pairs), kRowThreads, 0, st>>>(
-        w.logp, r, p, w.scores, w.margins, nullptr, nullptr, w.pair_loss, w.pairs_done, o);
+        reinterpret_cast<const float*>(w.score), 2, r, p, w.scores, w.margins, nullptr, nullptr, w.pair_loss,
+        w.pairs_done, o);
     return launched("preference_loss", 1);
   }
+  Softmax* softmax = reinterpret_cast<Softmax*>(w.softmax);
+  float* logp = reinterpret_cast<float*>(w.score);
   const unsigned grid = row_grid(r.rows);
   auto go = [&](auto* x) {
     using T = std::remove_const_t<std::remove_pointer_t<decltype(x)>>;
-    preference_short_rows_kernel<T><<<grid, kRowThreads, 0, st>>>(x, r, w.softmax, w.logp);
+    preference_short_rows_kernel<T><<<grid, kRowThreads, 0, st>>>(x, r, softmax, logp);
     preference_pairs_kernel<<<static_cast<unsigned>(pairs), kRowThreads, 0, st>>>(
-        w.logp, r, p, w.scores, w.margins, by, nullptr, w.pair_loss, w.pairs_done, o);
+        logp, 1, r, p, w.scores, w.margins, by, nullptr, w.pair_loss, w.pairs_done, o);
     if (grad != nullptr)
-      preference_short_gradient_kernel<T><<<grid, kRowThreads, 0, st>>>(x, static_cast<T*>(grad), r, w.softmax, by);
+      preference_short_gradient_kernel<T><<<grid, kRowThreads, 0, st>>>(x, static_cast<T*>(grad), r, softmax, by);
   };
   if (fp32)
     go(static_cast<const float*>(logits));
@@ -1270,7 +1597,7 @@ T5X_API int t5x_preference_loss_tokens(const void* logp, void* slope, long long 
   const Preference p = {static_cast<const float*>(reference), beta, smoothing, scale,
                         static_cast<const float*>(normalizer)};
   preference_pairs_kernel<<<static_cast<unsigned>(batch / 2), kRowThreads, 0, st>>>(
-      static_cast<const float*>(logp), r, p, static_cast<float*>(scores), static_cast<float*>(margins), nullptr,
+      static_cast<const float*>(logp), 1, r, p, static_cast<float*>(scores), static_cast<float*>(margins), nullptr,
       static_cast<float*>(slope), reinterpret_cast<double*>(static_cast<char*>(scratch) + kHead),
       static_cast<unsigned*>(scratch), static_cast<float*>(out));
   return launched("preference_loss_tokens", 1);
