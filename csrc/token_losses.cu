@@ -391,10 +391,9 @@ __device__ __forceinline__ Margin pair_margin(const Preference& p, bool real, do
 }
 
 // A CTA per pair: scores, margin, the pair's loss, the slopes of its two sequences (and, from
-// log-probabilities, of its tokens). The last CTA adds the losses. out: loss, pairs. logp: `logp_step` floats
-// from one to the next.
+// log-probabilities, of its tokens). The last CTA adds the losses. out: loss, pairs
 __global__ void __launch_bounds__(kRowThreads)
-    preference_pairs_kernel(const float* __restrict__ logp, int logp_step, const Rows r, const Preference p, float* scores,
+    preference_pairs_kernel(const float* __restrict__ logp, const Rows r, const Preference p, float* scores,
                             float* margins, float* __restrict__ by, float* __restrict__ token_slope,
                             double* pair_loss, unsigned* arrived, float* out) {
   const long long pair = blockIdx.x;
@@ -406,7 +405,7 @@ __global__ void __launch_bounds__(kRowThreads)
     for (int t = threadIdx.x; t < r.length; t += kRowThreads) {
       const float w = r.weights != nullptr ? r.weights[first + t] : 1.f;
       if (w != 0.f) {
-        sum[side] += static_cast<double>(w) * logp[(first + t) * logp_step];
+        sum[side] += static_cast<double>(w) * logp[first + t];
         seen = 1.0;
       }
     }
@@ -472,37 +471,44 @@ __global__ void __launch_bounds__(kRowThreads)
 }
 
 // ---- long rows ----
-// What both kernels share. A CTA's producer thread copies rows in tiles of up to 16 KB into a ring in
-// shared memory, far ahead of the worker warps, so that the loads go on while a row's sums meet. A keeper
-// warp makes of the workers' sums what the gradient of the row needs, so that no worker waits for the
-// load of a single value, a logarithm or another CTA; the producer hands it a row's few values, which it
-// has asked for rows ahead.
-constexpr int kTileBytes = 16384;
+// What both kernels share. A CTA's producer thread copies rows in tiles of up to 8 KB into a ring in
+// shared memory, far ahead of the worker warps. A tile is one warp's, the next tile the next warp's: the
+// warps of an SM are at different places of their work, so that some load or wait while others keep the
+// units for the exponentials busy (with a tile for all warps they stood in step: 375M logits summed in
+// 283 us instead of XXX). A keeper warp makes of the warps' sums what the gradient of the row needs, so that no
+// worker waits for the load of a single value, a logarithm or another CTA; the producer hands it a row's few
+// values, which it has asked for rows ahead.
+constexpr int kTileBytes = 8192;
 constexpr int kTilePacks = kTileBytes / 16;
-constexpr int kSlots = 16;  // rows that the keeper is told of ahead; more than the tiles of a ring and two
 
 enum Kind : int { kEnd, kStat, kGrad, kZero };
-struct Tile {
-  long long offset;  // of the row in the logits and their gradient
-  int kind, last;
-  int head;          // values in front of the row's first 16-byte boundary
-  int at, packs;     // first 16 bytes behind it, how many
-  int outside;       // 16 bytes of the whole row, on the tile whose workers see to the values outside; else -1
-  unsigned task;     // the row's place in the keeper's queue
-};
-struct Task {
-  long long row, b;
-  int kind, target;  // target: -1 outside of the vocabulary
-  float w, x;        // weight, the target's logit
-  PolicyInputs in;
-};
 // What the gradient of a row needs: by * onehot(target) + k * exp(x - most) with k = -by / sum.
 struct Slope {
   float most, by, k;
   int target;
 };
-template <int kStages, int kWarps>
+struct Tile {
+  long long offset;  // of the row in the logits and their gradient
+  int kind;
+  int last;          // the warp's last tile of the row
+  int head;          // values in front of the row's first 16-byte boundary
+  int at, packs;     // first 16 bytes behind it, how many
+  int outside;       // 16 bytes of the whole row, on the tile whose warp sees to the values outside; else -1
+  unsigned task;     // the how-many-th of the CTA's rows that are summed
+  Slope now;         // of a kGrad tile
+};
+struct Task {
+  long long row, b;
+  int kind, target;  // target: -1 outside of the vocabulary
+  float w, x;        // weight, the target's logit
+  int warp;          // whose is the row's first tile
+  PolicyInputs in;
+};
+// Slots for rows between their sums and their gradient: more than the ring has tiles, so that none is written
+// again before the warps that read it have given their tiles back.
+template <int kStages_, int kWarps_, int kSlots_>
 struct LongShared {
+  static constexpr int kStages = kStages_, kWarps = kWarps_, kSlots = kSlots_;
   alignas(128) unsigned char data[kStages][kTileBytes];
   uint64_t full[kStages], empty[kStages], told[kSlots], kept[kSlots], sums[kSlots], said[kSlots], met[kSlots];
   Tile tile[kStages];
@@ -511,22 +517,34 @@ struct LongShared {
   Softmax of_cta[kSlots][8];  // of the CTAs that share the row
   Slope slope[kSlots];
   int abort;
-  __device__ void init() {
+  __device__ void init(int warps_of_row) {
     for (int i = 0; i < kStages; ++i) {
       mbar_init(&full[i], 1);
-      mbar_init(&empty[i], kWarps);
+      mbar_init(&empty[i], 1);
     }
     for (int i = 0; i < kSlots; ++i) {
       mbar_init(&told[i], 1);
       mbar_init(&kept[i], 1);
-      mbar_init(&sums[i], kWarps);
+      mbar_init(&sums[i], warps_of_row);
       mbar_init(&said[i], 1);
       mbar_init(&met[i], 1);
     }
     abort = 0;
     mbar_fence_init();
   }
+  // The sums of a row's warps, in every lane of the keeper.
+  __device__ Softmax all_parts(int slot, int first, int warps_of_row) const;
 };
+
+// A wait with a limit of a second or two (a poll may be held back for some ten microseconds).
+constexpr uint32_t kPolls = 1u << 17;
+__device__ __forceinline__ bool ring_wait(uint64_t* bar, uint32_t parity, volatile int* abort) {
+  for (uint32_t it = 0; it < kPolls; ++it) {
+    if (mbar_try_wait(bar, parity)) return true;
+    if ((it & 0xf) == 0xf && *abort) return false;
+  }
+  return false;
+}
 
 // The part of a row between 16-byte boundaries.
 template <typename T>
@@ -639,18 +657,16 @@ __device__ __forceinline__ uint64_t exp2_pair(uint64_t x) {
   return pair_of(exp2_approx(a), exp2_approx(b));
 }
 
-// The tile's part of the row's softmax.
-template <typename T, int kWorkers>
-__device__ __forceinline__ void sum_tile(Softmax& s, const unsigned char* data, int packs, int tid) {
-  constexpr int kMine = (kTilePacks + kWorkers - 1) / kWorkers, kP = Pairs<T>::kPairs;
-  Pairs<T> x[kMine];
-#pragma unroll
-  for (int i = 0; i < kMine; ++i) {
-    if (tid + i * kWorkers < packs)
-      x[i].load(data + (tid + i * kWorkers) * 16);
-    else
-      x[i].nothing();
-  }
+template <int kStages, int kWarps, int kSlots>
+__device__ Softmax LongShared<kStages, kWarps, kSlots>::all_parts(int slot, int first, int warps_of_row) const {
+  const int lane = threadIdx.x & 31;
+  return join_row_lanes(lane < warps_of_row ? part[slot][(first + lane) % kWarps] : Softmax{-INFINITY, 0.f});
+}
+
+// Adds a lane's 16 bytes each to what it has seen.
+template <typename T, int kMine>
+__device__ __forceinline__ void take(Softmax& s, const Pairs<T>* x) {
+  constexpr int kP = Pairs<T>::kPairs;
   float m = x[0].most();
 #pragma unroll
   for (int i = 1; i < kMine; ++i) m = fmaxf(m, x[i].most());
@@ -681,10 +697,34 @@ __device__ __forceinline__ void sum_tile(Softmax& s, const unsigned char* data, 
   s.sum += a + b;
 }
 
-// The tile's part of the gradient; g: the row's.
-template <typename T, int kWorkers>
-__device__ __forceinline__ void turn_tile(T* g, const unsigned char* data, const Tile& t, const Slope& now, int tid) {
-  constexpr int kMine = (kTilePacks + kWorkers - 1) / kWorkers, kN = Pack<T>::kN;
+// The tile's part of the row's softmax; a warp's.
+template <typename T>
+__device__ __forceinline__ void sum_tile(Softmax& s, const unsigned char* data, int packs, int lane) {
+  constexpr int kMine = 4;
+  Pairs<T> x[kMine];
+  int at = 0;
+#pragma unroll 1
+  for (; at + kMine * 32 <= packs; at += kMine * 32) {
+#pragma unroll
+    for (int i = 0; i < kMine; ++i) x[i].load(data + (at + i * 32 + lane) * 16);
+    take<T, kMine>(s, x);
+  }
+  if (at < packs) {
+#pragma unroll
+    for (int i = 0; i < kMine; ++i) {
+      if (at + i * 32 + lane < packs)
+        x[i].load(data + (at + i * 32 + lane) * 16);
+      else
+        x[i].nothing();
+    }
+    take<T, kMine>(s, x);
+  }
+}
+
+// The tile's part of the gradient; a warp's. g: the row's.
+template <typename T>
+__device__ __forceinline__ void turn_tile(T* g, const unsigned char* data, const Tile& t, const Slope& now, int lane) {
+  constexpr int kN = Pack<T>::kN;
   const int first = t.head + t.at * kN;
   const bool far = huge(now.most);
   const float ref = __fmul_rn(now.most, kLog2e);
@@ -715,11 +755,11 @@ __device__ __forceinline__ void turn_tile(T* g, const unsigned char* data, const
   };
   // a tile without the target, of a row whose exponentials take the short way
   if (!far && static_cast<unsigned>(now.target - first) >= static_cast<unsigned>(t.packs * kN)) {
-#pragma unroll
-    for (int i = 0; i < kMine; ++i)
-      if (tid + i * kWorkers < t.packs) one(tid + i * kWorkers, std::true_type());
+#pragma unroll 4
+    for (int i = lane; i < t.packs; i += 32) one(i, std::true_type());
   } else {
-    for (int i = tid; i < t.packs; i += kWorkers) one(i, std::false_type());
+#pragma unroll 1
+    for (int i = lane; i < t.packs; i += 32) one(i, std::false_type());
   }
 }
 
@@ -742,17 +782,18 @@ __device__ __forceinline__ void turn_one(T* g, const T* row, int i, const Slope&
 }
 
 // The producer's side of a ring; one thread's.
-template <typename Shared, int kStages>
+template <typename Shared>
 struct Ring {
+  static constexpr int kStages = Shared::kStages, kSlots = Shared::kSlots;
   Shared& sh;
   volatile int* abort;
-  int stage = 0, issued = 0;
+  int stage = 0, warp = 0, issued = 0;  // warp: whose the next tile is
   uint32_t round = 0;
   unsigned tasks = 0;
   bool ok = true;
   __device__ Ring(Shared& s) : sh(s), abort(&s.abort) {}
   __device__ void push(const Tile& t, const void* src) {
-    if (!ok || !mbar_wait(&sh.empty[stage], (round & 1) ^ 1, abort)) {
+    if (!ok || !ring_wait(&sh.empty[stage], (round & 1) ^ 1, abort)) {
       ok = false;
       return;
     }
@@ -764,48 +805,67 @@ struct Ring {
       mbar_arrive(&sh.full[stage]);
     }
     ++issued;
+    if (++warp == Shared::kWarps) warp = 0;
     if (++stage == kStages) stage = 0, ++round;
   }
-  // The keeper, of a row ahead of its tiles. Returns the row's place in its queue.
-  __device__ unsigned tell(const Task& t) {
+  // The keeper, of a row ahead of its tiles.
+  __device__ void tell(Task t) {
     const int slot = tasks % kSlots;
-    if (!ok || !mbar_wait(&sh.kept[slot], (tasks / kSlots & 1) ^ 1, abort)) {
+    if (!ok || !ring_wait(&sh.kept[slot], (tasks / kSlots & 1) ^ 1, abort)) {
       ok = false;
-      return tasks;
+      return;
     }
+    t.warp = warp;
     sh.task[slot] = t;
     mbar_arrive(&sh.told[slot]);
-    return tasks++;
+    ++tasks;
   }
-  // `packs` 16 bytes of a row from `from`, in tiles of one size, so that each gives all workers something to do.
+  // `packs` 16 bytes of a row from `from`, in `tiles` tiles of one size.
   template <typename T>
-  __device__ void stream(Tile t, const T* logits, int from, int packs) {
-    const int tiles = (packs + kTilePacks - 1) / kTilePacks, size = (packs + tiles - 1) / tiles;
-    for (int at = 0; at < packs && ok; at += size) {
-      t.at = from + at;
-      t.packs = packs - at < size ? packs - at : size;
-      t.last = at + t.packs == packs;
+  __device__ void stream(Tile t, const T* logits, int from, int packs, int tiles) {
+    const int size = (packs + tiles - 1) / tiles;
+    for (int i = 0; i < tiles && ok; ++i) {
+      t.at = from + i * size;
+      t.packs = packs - i * size < size ? packs - i * size : size;
+      t.last = i + Shared::kWarps >= tiles;
       push(t, logits + t.offset + t.head + static_cast<long long>(t.at) * Pack<T>::kN);
       t.outside = -1;
     }
+  }
+  __device__ void end() {
+    Task t = {};
+    t.kind = kEnd;
+    tell(t);
+    for (int i = 0; i < Shared::kWarps; ++i) push({0, kEnd, 1, 0, 0, 0, -1, 0, {}}, nullptr);
   }
   // No copy may be under way when the shared memory is given back.
   __device__ void drain() {
     const int n = issued < kStages ? issued : kStages;
     for (int i = issued - n; i < issued; ++i)
-      for (uint32_t it = 0; it < kWaitLimit && !mbar_try_wait(&sh.full[i % kStages], (i / kStages) & 1); ++it) {
+      for (uint32_t it = 0; it < kPolls && !mbar_try_wait(&sh.full[i % kStages], (i / kStages) & 1); ++it) {
       }
   }
 };
 
+// A worker warp's side: its tiles are every kWarps-th of the ring.
+template <typename Shared>
+struct Turn {
+  int stage;
+  uint32_t round;
+  __device__ void advance() {
+    stage += Shared::kWarps;
+    while (stage >= Shared::kStages) stage -= Shared::kStages, ++round;
+  }
+};
+
 // Policy. A row belongs to a cluster of CTAs, of which each takes a part that fits into its ring with room for
-// the next one: the part is read once, summed, and turned into the gradient where it lies. The parts' sums
-// meet through distributed shared memory. `behind`: a row's gradient comes behind the next row's sums, so that
-// nobody waits while the keepers make the slope. Parts that do not fit are read a second time.
-constexpr int kPolicyStages = 13;
-constexpr int kPolicyWorkers = 512;
-constexpr int kPolicyThreads = kPolicyWorkers + 64;
-using PolicyShared = LongShared<kPolicyStages, kPolicyWorkers / 32>;
+// the next ones: the part is read once, summed, and turned into the gradient where it lies. The parts' sums
+// meet through distributed shared memory. A warp turns a tile behind the sums of its next one, so that it does
+// not wait for the row's slope. (Tile t is turned behind the sums of its row, which end n - 1 tiles later at
+// most, and of tile t + kWarps; tile u is loaded when tile u - kStages is turned: with n and kWarps no more than
+// kStages the turning waits for smaller tiles only.)
+using PolicyShared = LongShared<26, 16, 32>;
+constexpr int kPolicyThreads = PolicyShared::kWarps * 32 + 64;
 
 __device__ __forceinline__ void send_to_cta(Softmax* slot, uint64_t* bar, int cta, Softmax s) {
   uint64_t v;
@@ -819,20 +879,21 @@ __device__ __forceinline__ void send_to_cta(Softmax* slot, uint64_t* bar, int ct
 template <typename T>
 __global__ void __launch_bounds__(kPolicyThreads, 1)
     policy_rows_kernel(const T* __restrict__ logits, T* __restrict__ grad, const Rows r, const Policy p, int ctas,
-                       bool resident, bool behind, double* partial, unsigned* arrived, float* out, int* status) {
-  constexpr int kN = Pack<T>::kN, kWarps = kPolicyWorkers / 32;
+                       int tiles, double* partial, unsigned* arrived, float* out, int* status) {
+  constexpr int kN = Pack<T>::kN, kWarps = PolicyShared::kWarps, kSlots = PolicyShared::kSlots;
   extern __shared__ __align__(128) unsigned char raw[];
   PolicyShared& sh = *reinterpret_cast<PolicyShared*>(raw);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int rank = ctas > 1 ? static_cast<int>(cluster_ctarank()) : 0;
   const long long cluster = blockIdx.x / ctas, clusters = gridDim.x / ctas;
-  if (tid == 0) sh.init();
+  const int warps_of_row = tiles < kWarps ? tiles : kWarps;
+  if (tid == 0) sh.init(warps_of_row);
   __syncthreads();
   if (ctas > 1) cluster_sync_all();  // every CTA's barriers stand before another signals one
   volatile int* abort = &sh.abort;
   bool ok = true;
   auto wait = [&](uint64_t* bar, uint32_t parity) {  // the whole warp's
-    ok = __all_sync(0xffffffffu, mbar_wait(bar, parity, abort));
+    ok = __all_sync(0xffffffffu, ring_wait(bar, parity, abort));
     return ok;
   };
   auto give_up = [&](int code) {
@@ -843,7 +904,7 @@ __global__ void __launch_bounds__(kPolicyThreads, 1)
   };
 
   if (warp == kWarps) {  // ---- producer: 32 rows' values at a time, asked for while the last 32 go by ----
-    Ring<PolicyShared, kPolicyStages> ring(sh);
+    Ring<PolicyShared> ring(sh);
     Task next = {};
     long long next_offset = 0;
     auto ask = [&](long long base) {
@@ -877,32 +938,30 @@ __global__ void __launch_bounds__(kPolicyThreads, 1)
         t.x = __shfl_sync(0xffffffffu, mine.x, i);
         t.in = {__shfl_sync(0xffffffffu, mine.in.old, i), __shfl_sync(0xffffffffu, mine.in.ref, i),
                 __shfl_sync(0xffffffffu, mine.in.advantage, i)};
-        Tile tile = {__shfl_sync(0xffffffffu, offset, i), t.kind, 1, 0, 0, 0, -1, 0};
-        if (lane != 0 || (t.kind == kZero && grad == nullptr)) continue;
+        Tile tile = {__shfl_sync(0xffffffffu, offset, i), t.kind, 1, 0, 0, 0, -1, 0, {}};
         int all;
         aligned_part(logits + tile.offset, r.vocab, tile.head, all);
         const int part = (all + ctas - 1) / ctas, from = part * rank < all ? part * rank : all;
         const int packs = all - from < part ? all - from : part;
-        tile.outside = rank == 0 ? all : -1;
-        tile.at = from;
-        if (t.kind == kZero) {
-          tile.packs = packs;
-          ring.push(tile, nullptr);
+        if (t.kind == kZero) {  // (all lanes': nothing of it is in the way of the tiles)
+          if (grad == nullptr) continue;
+          T* g = grad + tile.offset;
+          for (int k = lane; k < packs; k += 32)
+            *reinterpret_cast<uint4*>(g + tile.head + static_cast<long long>(from + k) * kN) = make_uint4(0, 0, 0, 0);
+          tile.outside = rank == 0 ? all : -1;
+          const int k = outside_of<T>(tile, r.vocab, lane);
+          if (k >= 0) g[k] = Pack<T>::back(0.f);
           continue;
         }
-        tile.task = ring.tell(t);
-        ring.stream(tile, logits, from, packs);
-        if (!resident && grad != nullptr) {
-          tile.kind = kGrad;
-          ring.stream(tile, logits, from, packs);
-        }
+        if (lane != 0) continue;
+        tile.outside = rank == 0 ? all : -1;
+        tile.task = ring.tasks;
+        ring.tell(t);
+        ring.stream(tile, logits, from, packs, tiles);
       }
     }
     if (lane == 0) {
-      Task end = {};
-      end.kind = kEnd;
-      ring.tell(end);
-      ring.push({0, kEnd, 1, 0, 0, 0, -1, 0}, nullptr);
+      ring.end();
       if (!ring.ok) {
         give_up(kStatusTimeoutProducer);
         ring.drain();
@@ -918,7 +977,7 @@ __global__ void __launch_bounds__(kPolicyThreads, 1)
       const Task t = sh.task[slot];
       if (t.kind == kEnd) break;
       if (!wait(&sh.sums[slot], parity)) break;
-      Softmax s = join_row_lanes(lane < kWarps ? sh.part[slot][lane] : Softmax{-INFINITY, 0.f});
+      Softmax s = sh.all_parts(slot, t.warp, warps_of_row);
       if (ctas > 1) {
         if (lane == 0) mbar_expect_tx(&sh.met[slot], 8 * ctas);
         __syncwarp();
@@ -960,84 +1019,45 @@ __global__ void __launch_bounds__(kPolicyThreads, 1)
       }
     }
   } else {  // ---- workers ----
-    int stage = 0;
-    uint32_t round = 0;
-    auto advance = [&](int& s, uint32_t& n) {
-      if (++s == kPolicyStages) s = 0, ++n;
-    };
-    auto release = [&](int s) {
+    Turn<PolicyShared> at = {warp, 0}, old = at;  // old: of the tile whose gradient is still to come
+    bool pending = false;
+    Softmax seen = {-INFINITY, 0.f};
+    auto turn = [&](int stage) {
+      const Tile t = sh.tile[stage];
+      if (!wait(&sh.said[t.task % kSlots], t.task / kSlots & 1)) return;
+      const Slope now = sh.slope[t.task % kSlots];
+      const int i = outside_of<T>(t, r.vocab, lane);
+      if (i >= 0) turn_one(grad + t.offset, logits + t.offset, i, now);
+      turn_tile<T>(grad + t.offset, sh.data[stage], t, now, lane);
       __syncwarp();
-      if (lane == 0) mbar_arrive(&sh.empty[s]);
+      if (lane == 0) mbar_arrive(&sh.empty[stage]);
     };
-    const bool keep = resident && grad != nullptr;  // the sums leave the tiles where they are
-    // The gradient of the row whose tiles begin at the stage; leaves the stage behind them.
-    auto turn_row = [&](int& s, uint32_t& n) {
-      Slope now = {0.f, 0.f, 0.f, -1};
-      for (bool first = true;; first = false) {
-        if (!wait(&sh.full[s], n & 1)) return;
-        const Tile t = sh.tile[s];
-        const T* row = logits + t.offset;
-        if (first) {
-          if (!wait(&sh.said[t.task % kSlots], t.task / kSlots & 1)) return;
-          now = sh.slope[t.task % kSlots];
-          const int i = outside_of<T>(t, r.vocab, tid);
-          if (i >= 0) turn_one(grad + t.offset, row, i, now);
+    while (wait(&sh.full[at.stage], at.round & 1)) {
+      const Tile t = sh.tile[at.stage];
+      if (t.kind == kStat) {
+        const int i = outside_of<T>(t, r.vocab, lane);
+        if (i >= 0) seen = one_value(logits[t.offset + i]);
+        sum_tile<T>(seen, sh.data[at.stage], t.packs, lane);
+        if (t.last) {
+          const Softmax s = join_row_lanes(seen);
+          if (lane == 0) {
+            sh.part[t.task % kSlots][warp] = s;
+            mbar_arrive(&sh.sums[t.task % kSlots]);
+          }
+          seen = {-INFINITY, 0.f};
         }
-        turn_tile<T, kPolicyWorkers>(grad + t.offset, sh.data[s], t, now, tid);
-        release(s);
-        advance(s, n);
-        if (t.last) return;
+        if (grad == nullptr) {
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&sh.empty[at.stage]);
+          at.advance();
+          continue;
+        }
       }
-    };
-    int old_stage = 0;  // of the row whose gradient is still to come
-    uint32_t old_round = 0;
-    bool old = false;
-    while (ok && wait(&sh.full[stage], round & 1)) {
-      Tile t = sh.tile[stage];
-      if (t.kind != kStat && old) {  // (a row's tiles may need the room of the one before)
-        old = false;
-        turn_row(old_stage, old_round);
-        if (!ok) break;
-      }
-      if (t.kind == kEnd) break;
-      if (t.kind == kZero) {
-        release(stage);
-        advance(stage, round);
-        T* g = grad + t.offset;
-        for (int i = tid; i < t.packs; i += kPolicyWorkers)
-          *reinterpret_cast<uint4*>(g + t.head + static_cast<long long>(t.at + i) * kN) = make_uint4(0, 0, 0, 0);
-        const int i = outside_of<T>(t, r.vocab, tid);
-        if (i >= 0) g[i] = Pack<T>::back(0.f);
-        continue;
-      }
-      if (t.kind == kGrad) {
-        turn_row(stage, round);
-        continue;
-      }
-      int first_stage = stage;
-      uint32_t first_round = round;
-      Softmax seen = {-INFINITY, 0.f};
-      const int i = outside_of<T>(t, r.vocab, tid);
-      if (i >= 0) seen = one_value(logits[t.offset + i]);
-      while (true) {
-        sum_tile<T, kPolicyWorkers>(seen, sh.data[stage], t.packs, tid);
-        if (!keep) release(stage);
-        advance(stage, round);
-        if (t.last || !wait(&sh.full[stage], round & 1)) break;
-        t = sh.tile[stage];
-      }
-      if (!ok) break;
-      const Softmax s = join_row_lanes(seen);
-      if (lane == 0) {
-        sh.part[t.task % kSlots][warp] = s;
-        mbar_arrive(&sh.sums[t.task % kSlots]);
-      }
-      if (!keep) continue;
-      if (old) turn_row(old_stage, old_round);
-      old = behind;
-      old_stage = first_stage;
-      old_round = first_round;
-      if (!behind) turn_row(first_stage, first_round);
+      if (pending) turn(old.stage);
+      pending = t.kind == kStat;
+      old = at;
+      if (!ok || t.kind == kEnd) break;
+      at.advance();
     }
     if (!ok) give_up(kStatusTimeoutEpilogue);
   }
@@ -1047,149 +1067,30 @@ __global__ void __launch_bounds__(kPolicyThreads, 1)
   }
 }
 
-// Preference. The slope of a row needs the sums of all rows of its pair. The tasks (a row's sums, a row's
-// gradient) stand in an order in which a group of pairs is followed by the next group's sums and then its
-// own gradients, whose logits are still in L2; a CTA takes the next task by a ticket. What a gradient waits
-// for has smaller tickets, is therefore done or under way, and waits itself for smaller tickets at most. A
-// row's results are 8-byte words, zero until they are there: who needs a pair reads its words until none
-// of those that count is zero. (Counting the rows done would need a fence a row, which takes microseconds
-// while the memory is busy: 355 us against ... for 64 x 114 x 32128.)
-constexpr int kPairStages = 6;
-constexpr int kPairWorkers = 256;
-constexpr int kPairThreads = kPairWorkers + 64;
-using PairShared = LongShared<kPairStages, kPairWorkers / 32>;
+// Preference. The slope of a row needs the sums of all rows of its pair: one kernel makes the rows' softmaxes
+// and log-probabilities, another (above) the pairs' slopes, a third, beginning with the rows read last, which
+// are still in L2, the gradients. (One kernel for all of it, whose gradients waited for the rows of their pair,
+// would read most logits from L2 the second time, but its CTAs wait for one another.) Two CTAs an SM.
+using PairShared = LongShared<12, 8, 16>;
+constexpr int kPairThreads = PairShared::kWarps * 32 + 64;
 
-struct Order {
-  long long rows, group;  // rows of the batch, of a group of pairs
-  bool behind;            // a group's gradients follow the next group's sums
-  bool gradient;
-};
-// (row, is it the gradient's turn) of a ticket below rows * (1 + gradient)
-__device__ __forceinline__ long long task_of(const Order& o, long long ticket, bool& gradient) {
-  gradient = false;
-  if (!o.gradient) return ticket;
-  const long long last = (o.rows - 1) / o.group * o.group;  // first row of the last group
-  if (!o.behind) {  // sums of a group, then its gradients, those last read first
-    const long long k = ticket / (2 * o.group), first = k * o.group, at = ticket - 2 * first;
-    const long long n = o.rows - first < o.group ? o.rows - first : o.group;
-    gradient = at >= n;
-    return gradient ? first + 2 * n - 1 - at : first + at;
-  }
-  gradient = ticket >= o.rows + last;
-  if (gradient) return ticket - o.rows;  // of the last group
-  if (ticket < o.group) return ticket;
-  const long long k = (ticket - o.group) / (2 * o.group) + 1;  // sums of group k, gradients of k - 1
-  const long long at = ticket - o.group - (k - 1) * 2 * o.group, first = k * o.group;
-  const long long n = o.rows - first < o.group ? o.rows - first : o.group;
-  gradient = at >= n;
-  return gradient ? first - o.group + (at - n) : first + at;
-}
-
-struct Work {
-  unsigned long long* ticket;
-  unsigned* pairs_done;
-  unsigned long long *softmax, *score;  // a row's {largest, sum} and {log-probability, 1}
-  double* pair_loss;
-  float *scores, *margins;
-  Order order;
-};
-
-__device__ __forceinline__ unsigned long long ld_word(const unsigned long long* p) {
-  unsigned long long v;
-  asm volatile("ld.relaxed.gpu.global.u64 %0, [%1];" : "=l"(v) : "l"(p) : "memory");
-  return v;
-}
-__device__ __forceinline__ void st_word(unsigned long long* p, unsigned long long v) {
-  asm volatile("st.relaxed.gpu.global.u64 [%0], %1;" ::"l"(p), "l"(v) : "memory");
-}
-__device__ __forceinline__ unsigned long long word_of(float low, uint32_t high) {
-  return static_cast<unsigned long long>(high) << 32 | __float_as_uint(low);
-}
-
-// A keeper's: the pair's margin, once all of its rows have their words. `writes`: stores what the pair gives
-// and, for the last pair, the loss.
-__device__ __forceinline__ bool pair_slope(const Rows& r, const Preference& q, const Work& work, long long pair,
-                                           bool writes, volatile int* abort, float* out, float& slope) {
-  const int lane = threadIdx.x & 31;
-  double sum[2];
-  bool seen;
-  for (uint32_t it = 0;; ++it) {
-    bool missing = false;
-    seen = false;
-#pragma unroll
-    for (int side = 0; side < 2; ++side) {
-      const long long first = (2 * pair + side) * r.length;
-      sum[side] = 0.0;
-#pragma unroll 8
-      for (int i = lane; i < r.length; i += 32) {
-        const float w = r.weights != nullptr ? r.weights[first + i] : 1.f;
-        const unsigned long long v = ld_word(work.score + first + i);
-        if (w != 0.f) {
-          sum[side] += static_cast<double>(w) * __uint_as_float(static_cast<uint32_t>(v));
-          seen = true;
-          missing = missing || v == 0;
-        }
-      }
-    }
-    if (!__any_sync(0xffffffffu, missing)) break;
-    if (__any_sync(0xffffffffu, it == kWaitLimit >> 4 || *abort)) return false;
-    __nanosleep(100);
-  }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    sum[0] += __shfl_xor_sync(0xffffffffu, sum[0], o);
-    sum[1] += __shfl_xor_sync(0xffffffffu, sum[1], o);
-  }
-  const bool real = __any_sync(0xffffffffu, seen);
-  const Margin m = pair_margin(q, real, sum[0], sum[1], q.ref[2 * pair], q.ref[2 * pair + 1],
-                               scale_of(q.normalizer, q.scale));
-  slope = m.slope;
-  if (!writes) return true;
-  unsigned before = 0;
-  if (lane == 0) {
-    work.scores[2 * pair] = static_cast<float>(sum[0]);
-    work.scores[2 * pair + 1] = static_cast<float>(sum[1]);
-    work.margins[pair] = static_cast<float>(m.margin);
-    work.pair_loss[2 * pair] = m.loss;
-    work.pair_loss[2 * pair + 1] = real ? 1.0 : 0.0;
-    __threadfence();
-    before = atomicAdd(work.pairs_done, 1u);
-  }
-  const long long pairs = r.rows / r.length / 2;
-  if (__shfl_sync(0xffffffffu, before, 0) != pairs - 1) return true;
-  __threadfence();
-  double loss = 0.0, count = 0.0;
-  for (long long i = lane; i < pairs; i += 32) {
-    loss += __ldcg(work.pair_loss + 2 * i);
-    count += __ldcg(work.pair_loss + 2 * i + 1);
-  }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    loss += __shfl_xor_sync(0xffffffffu, loss, o);
-    count += __shfl_xor_sync(0xffffffffu, count, o);
-  }
-  if (lane == 0) {
-    const double whole = q.normalizer != nullptr ? 1.0 / static_cast<double>(*q.normalizer) : q.scale;
-    out[0] = static_cast<float>(loss * whole);
-    out[1] = static_cast<float>(count);
-  }
-  return true;
-}
-
-template <typename T>
+// kTurn: the gradients, from `softmax` and the slopes `by` of the sequences; else the softmaxes.
+template <typename T, bool kTurn>
 __global__ void __launch_bounds__(kPairThreads, 2)
-    preference_rows_kernel(const T* __restrict__ logits, T* __restrict__ grad, const Rows r, const Preference q,
-                           const Work work, float* out, int* status) {
-  constexpr int kWarps = kPairWorkers / 32;
+    preference_rows_kernel(const T* __restrict__ logits, T* __restrict__ grad, const Rows r, int tiles,
+                           Softmax* __restrict__ softmax, float* __restrict__ logp, const float* __restrict__ by,
+                           int* status) {
+  constexpr int kWarps = PairShared::kWarps, kSlots = PairShared::kSlots;
+  const int warps_of_row = tiles < kWarps ? tiles : kWarps;
   extern __shared__ __align__(128) unsigned char raw[];
   PairShared& sh = *reinterpret_cast<PairShared*>(raw);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  if (tid == 0) sh.init();
+  if (tid == 0) sh.init(warps_of_row);
   __syncthreads();
   volatile int* abort = &sh.abort;
   bool ok = true;
   auto wait = [&](uint64_t* bar, uint32_t parity) {  // the whole warp's
-    ok = __all_sync(0xffffffffu, mbar_wait(bar, parity, abort));
+    ok = __all_sync(0xffffffffu, ring_wait(bar, parity, abort));
     return ok;
   };
   auto give_up = [&](int code) {
@@ -1199,143 +1100,111 @@ __global__ void __launch_bounds__(kPairThreads, 2)
     }
   };
 
-  if (warp == kWarps) {  // ---- producer ----
-    if (lane != 0) return;
-    Ring<PairShared, kPairStages> ring(sh);
-    const long long total = work.order.rows * (work.order.gradient ? 2 : 1);
-    // Three tasks are under way: of one the ticket has been asked for, of the next the weight and the target, of
-    // the next the target's logit; nobody waits for any of these.
-    struct Asked {
-      Task t;
-      long long offset, target;
-    };
-    auto ask = [&](long long ticket) {
-      Asked a = {};
-      a.t.row = -1;
-      if (ticket >= total) return a;
-      bool gradient;
-      a.t.row = task_of(work.order, ticket, gradient);
-      a.t.b = a.t.row / r.length;
-      a.t.kind = gradient ? kGrad : kStat;
-      a.offset = a.t.b * r.stride_b + (a.t.row - a.t.b * r.length) * r.stride_t;
-      a.t.w = r.weights != nullptr ? r.weights[a.t.row] : 1.f;
-      a.target = r.targets[a.t.row];
-      return a;
-    };
-    auto ask_logit = [&](Asked& a) {
-      if (a.t.row < 0) return;
-      a.t.target = a.target >= 0 && a.target < r.vocab ? static_cast<int>(a.target) : -1;
-      a.t.x = NAN;
-      if (a.t.kind == kStat && a.t.w != 0.f && a.t.target >= 0) a.t.x = Pack<T>::one(logits[a.offset + a.t.target]);
-    };
-    Asked now = ask(static_cast<long long>(atomicAdd(work.ticket, 1ull)));
-    Asked next = ask(static_cast<long long>(atomicAdd(work.ticket, 1ull)));
-    ask_logit(now);
-    while (now.t.row >= 0 && ring.ok) {
-      const long long ticket = static_cast<long long>(atomicAdd(work.ticket, 1ull));
-      ask_logit(next);
-      Tile tile = {now.offset, now.t.kind, 1, 0, 0, 0, -1, 0};
-      int all;
-      aligned_part(logits + now.offset, r.vocab, tile.head, all);
-      if (now.t.w != 0.f) {
-        tile.outside = all;
-        tile.task = ring.tell(now.t);
-        ring.stream(tile, logits, 0, all);
-      } else if (now.t.kind == kGrad) {
-        tile.kind = now.t.kind = kZero;
-        if (now.t.row % (2 * r.length) == 0) ring.tell(now.t);  // (whose keeper writes what the pair gives)
-        ring.push(tile, nullptr);
+  if (warp == kWarps) {  // ---- producer: 32 rows' values at a time, asked for while the last 32 go by ----
+    Ring<PairShared> ring(sh);
+    Task next = {};
+    Slope next_slope = {};
+    long long next_offset = 0;
+    auto ask = [&](long long base) {
+      const long long at = base + static_cast<long long>(lane) * gridDim.x;
+      next.kind = kEnd;
+      if (at >= r.rows) return;
+      next.row = kTurn ? r.rows - 1 - at : at;
+      next.b = next.row / r.length;
+      next_offset = next.b * r.stride_b + (next.row - next.b * r.length) * r.stride_t;
+      next.w = r.weights != nullptr ? r.weights[next.row] : 1.f;
+      next.kind = next.w != 0.f ? (kTurn ? kGrad : kStat) : kZero;
+      if (next.kind == kZero) return;
+      const long long target = r.targets[next.row];
+      next.target = target >= 0 && target < r.vocab ? static_cast<int>(target) : -1;
+      if (kTurn) {
+        const Softmax s = softmax[next.row];
+        const float slope = next.w * by[next.b];
+        next_slope = {s.most, slope, -slope / s.sum, next.target};
+      } else {
+        next.x = next.target >= 0 ? Pack<T>::one(logits[next_offset + next.target]) : NAN;
       }
-      now = next;
-      next = ask(ticket);
+    };
+    ask(blockIdx.x);
+    for (long long base = blockIdx.x; base < r.rows; base += 32ll * gridDim.x) {
+      const Task mine = next;
+      const Slope slope = next_slope;
+      const long long offset = next_offset;
+      if (base + 32ll * gridDim.x < r.rows) ask(base + 32ll * gridDim.x);
+      for (int i = 0; i < 32; ++i) {
+        if (base + static_cast<long long>(i) * gridDim.x >= r.rows) break;
+        Task t;
+        t.row = __shfl_sync(0xffffffffu, mine.row, i);
+        t.b = 0;
+        t.kind = __shfl_sync(0xffffffffu, mine.kind, i);
+        t.target = 0;
+        t.w = 0.f;
+        t.x = __shfl_sync(0xffffffffu, mine.x, i);
+        t.in = {};
+        Tile tile = {__shfl_sync(0xffffffffu, offset, i), t.kind, 1, 0, 0, 0, -1, 0, {}};
+        tile.now = {__shfl_sync(0xffffffffu, slope.most, i), __shfl_sync(0xffffffffu, slope.by, i),
+                    __shfl_sync(0xffffffffu, slope.k, i), __shfl_sync(0xffffffffu, slope.target, i)};
+        int all;
+        aligned_part(logits + tile.offset, r.vocab, tile.head, all);
+        if (t.kind == kZero) {  // (all lanes')
+          if (kTurn) row_zero(grad + tile.offset, r.vocab, lane, 32);
+          continue;
+        }
+        if (lane != 0) continue;
+        tile.outside = all;
+        tile.task = ring.tasks;
+        if (!kTurn) ring.tell(t);
+        ring.stream(tile, logits, 0, all, tiles);
+      }
     }
-    Task end = {};
-    end.kind = kEnd;
-    ring.tell(end);
-    ring.push({0, kEnd, 1, 0, 0, 0, -1, 0}, nullptr);
-    if (!ring.ok) {
-      give_up(kStatusTimeoutProducer);
-      ring.drain();
+    if (lane == 0) {
+      ring.end();
+      if (!ring.ok) {
+        give_up(kStatusTimeoutProducer);
+        ring.drain();
+      }
     }
   } else if (warp > kWarps) {  // ---- keeper ----
-    long long known = -1;  // a pair, and the slope of its preferred row
-    float slope = 0.f;
     for (unsigned n = 0;; ++n) {
       const int slot = n % kSlots;
       const uint32_t parity = n / kSlots & 1;
       if (!wait(&sh.told[slot], parity)) break;
       const Task t = sh.task[slot];
       if (t.kind == kEnd) break;
-      if (t.kind == kStat) {
-        if (!wait(&sh.sums[slot], parity)) break;
-        const Softmax s = join_row_lanes(lane < kWarps ? sh.part[slot][lane] : Softmax{-INFINITY, 0.f});
-        if (lane == 0) {
-          st_word(work.score + t.row, word_of(log_prob_of(t.x, s), 1));
-          st_word(work.softmax + t.row, word_of(s.most, __float_as_uint(s.sum)));
-        }
-      } else {
-        const long long pair = t.b / 2;
-        const bool writes = t.row == pair * 2 * r.length;
-        if (pair != known || writes) {
-          ok = pair_slope(r, q, work, pair, writes, abort, out, slope);
-          if (!ok) break;
-          known = pair;
-        }
-        if (t.kind == kGrad) {
-          // (of an own or an earlier task's row: its word stands beside the score's, which is there)
-          unsigned long long v = 0;
-          for (uint32_t it = 0; it < kWaitLimit && (v = ld_word(work.softmax + t.row)) == 0 && !*abort; ++it)
-            __nanosleep(20);
-          ok = __all_sync(0xffffffffu, v != 0);
-          if (!ok) break;
-          if (lane == 0) {
-            const float by = t.w * (t.b & 1 ? -slope : slope);
-            sh.slope[slot] = {__uint_as_float(static_cast<uint32_t>(v)), by,
-                              -by / __uint_as_float(static_cast<uint32_t>(v >> 32)), t.target};
-          }
-        }
-        if (lane == 0)  // (the phases of all of a slot's barriers go on together)
-          for (int i = 0; i < kWarps; ++i) mbar_arrive(&sh.sums[slot]);
-      }
+      if (!wait(&sh.sums[slot], parity)) break;
+      const Softmax s = sh.all_parts(slot, t.warp, warps_of_row);
       if (lane == 0) {
-        mbar_arrive(&sh.said[slot]);
+        softmax[t.row] = s;
+        logp[t.row] = log_prob_of(t.x, s);
         mbar_arrive(&sh.kept[slot]);
       }
       __syncwarp();
     }
-    if (!ok) give_up(kStatusTimeoutPeerFlag);
+    if (!ok) give_up(kStatusTimeoutEpilogue);
   } else {  // ---- workers ----
-    int stage = 0;
-    uint32_t round = 0;
-    Softmax seen = {-INFINITY, 0.f};  // of the row whose sums are under way
-    Slope now = {0.f, 0.f, 0.f, -1};  // of the row whose gradient is under way
-    while (wait(&sh.full[stage], round & 1)) {
-      const Tile t = sh.tile[stage];
+    Turn<PairShared> at = {warp, 0};
+    Softmax seen = {-INFINITY, 0.f};
+    while (wait(&sh.full[at.stage], at.round & 1)) {
+      const Tile t = sh.tile[at.stage];
       if (t.kind == kEnd) break;
-      const int outside = outside_of<T>(t, r.vocab, tid);
-      if (t.kind == kStat) {
+      const int outside = outside_of<T>(t, r.vocab, lane);
+      if (kTurn) {
+        if (outside >= 0) turn_one(grad + t.offset, logits + t.offset, outside, t.now);
+        turn_tile<T>(grad + t.offset, sh.data[at.stage], t, t.now, lane);
+      } else {
         if (outside >= 0) seen = one_value(logits[t.offset + outside]);
-        sum_tile<T, kPairWorkers>(seen, sh.data[stage], t.packs, tid);
-      } else if (t.kind == kGrad) {
-        if (t.outside >= 0) {  // the row's first tile
-          if (!wait(&sh.said[t.task % kSlots], t.task / kSlots & 1)) break;
-          now = sh.slope[t.task % kSlots];
-          if (outside >= 0) turn_one(grad + t.offset, logits + t.offset, outside, now);
-        }
-        turn_tile<T, kPairWorkers>(grad + t.offset, sh.data[stage], t, now, tid);
+        sum_tile<T>(seen, sh.data[at.stage], t.packs, lane);
       }
       __syncwarp();
-      if (lane == 0) mbar_arrive(&sh.empty[stage]);
-      if (++stage == kPairStages) stage = 0, ++round;
-      if (t.kind == kStat && t.last) {
+      if (lane == 0) mbar_arrive(&sh.empty[at.stage]);
+      at.advance();
+      if (!kTurn && t.last) {
         const Softmax s = join_row_lanes(seen);
         if (lane == 0) {
           sh.part[t.task % kSlots][warp] = s;
           mbar_arrive(&sh.sums[t.task % kSlots]);
         }
         seen = {-INFINITY, 0.f};
-      } else if (t.kind == kZero) {
-        row_zero(grad + t.offset, r.vocab, tid, kPairWorkers);
       }
     }
     if (!ok) give_up(kStatusTimeoutEpilogue);
@@ -1354,7 +1223,13 @@ __global__ void __launch_bounds__(256)
 }
 
 // ---- host ----
-constexpr long long kShortRow = 4096;  // bytes; shorter rows are a warp's
+// Rows of these bytes go through the ring; shorter ones are a warp's each, and so are longer ones (a vocabulary
+// of 400,000 in 32 bits: more than eight CTAs hold), which no model here has.
+constexpr long long kRingRow = 4096, kRingRowMost = 1600 << 10;
+bool by_ring(long long vocab, int fp32) {
+  const long long bytes = vocab * (fp32 ? 4 : 2);
+  return bytes >= kRingRow && bytes <= kRingRowMost;
+}
 
 int check_rows(const char* what, const void* logits, int fp32, const void* grad, long long batch, int length,
                int vocab, long long stride_b, long long stride_t, const void* targets) {
@@ -1384,17 +1259,23 @@ int launched(const char* what, int n) {
   return 0;
 }
 
+// Tiles of a CTA's part of a row, the same for all rows wherever their 16-byte boundaries lie (none is empty:
+// a part of n tiles has more than 512 (n - 1) times 16 bytes, or, for n = 1, 250).
+int tiles_of(long long vocab, int size, int ctas) {
+  const long long packs = (vocab * size / 16 + ctas - 1) / ctas;
+  return static_cast<int>((packs + kTilePacks - 1) / kTilePacks);
+}
+
 template <typename T>
 int launch_policy(const void* logits, void* grad, const Rows& r, const Policy& p, double* partial, unsigned* arrived,
                   float* out, cudaStream_t st) {
-  // The smallest cluster whose CTAs' parts leave room for two more in the ring (four tiles; the largest
-  // cluster's may be larger).
+  // The smallest cluster whose CTAs' parts leave room for two more in the ring (the largest cluster's parts
+  // may be larger).
   const long long bytes = static_cast<long long>(r.vocab) * sizeof(T);
   int ctas = 1;
-  while (ctas < 8 && (bytes + ctas - 1) / ctas > 4 * kTileBytes) ctas *= 2;
+  while (ctas < 8 && (bytes + ctas - 1) / ctas > 8 * kTileBytes) ctas *= 2;
   if (grad == nullptr) ctas = 1;  // (nothing has to stay)
-  const int tiles = static_cast<int>((bytes / 16 / ctas + 1 + kTilePacks - 1) / kTilePacks);
-  const bool resident = tiles <= kPolicyStages, behind = 2 * tiles <= kPolicyStages;
+  const int tiles = tiles_of(r.vocab, sizeof(T), ctas);
   auto kernel = policy_rows_kernel<T>;
   cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, sizeof(PolicyShared));
   if (e != cudaSuccess) return set_error("policy_loss: %s", cudaGetErrorString(e));
@@ -1425,31 +1306,27 @@ int launch_policy(const void* logits, void* grad, const Rows& r, const Policy& p
     at_once[dev][size].store(cap, std::memory_order_relaxed);
   }
   cfg.gridDim = dim3(static_cast<unsigned>((r.rows < cap ? r.rows : cap) * ctas));
-  e = cudaLaunchKernelEx(&cfg, kernel, static_cast<const T*>(logits), static_cast<T*>(grad), r, p, ctas, resident,
-                         behind, partial, arrived, out, device_status_buffer());
+  e = cudaLaunchKernelEx(&cfg, kernel, static_cast<const T*>(logits), static_cast<T*>(grad), r, p, ctas, tiles, partial,
+                         arrived, out, device_status_buffer());
   if (e != cudaSuccess) return set_error("policy_loss: %s", cudaGetErrorString(e));
   return launched("policy_loss", 1);
 }
 
-template <typename T>
-int launch_preference(const void* logits, void* grad, const Rows& r, const Preference& p, const Work& work, float* out,
+template <typename T, bool kTurn>
+int launch_preference(const void* logits, void* grad, const Rows& r, Softmax* softmax, float* logp, const float* by,
                       cudaStream_t st) {
-  auto kernel = preference_rows_kernel<T>;
+  auto kernel = preference_rows_kernel<T, kTurn>;
   const cudaError_t e =
       cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, sizeof(PairShared));
   if (e != cudaSuccess) return set_error("preference_loss: %s", cudaGetErrorString(e));
   const long long cap = static_cast<long long>(num_sms()) * 2;
   kernel<<<static_cast<unsigned>(r.rows < cap ? r.rows : cap), kPairThreads, sizeof(PairShared), st>>>(
-      static_cast<const T*>(logits), static_cast<T*>(grad), r, p, work, out, device_status_buffer());
+      static_cast<const T*>(logits), static_cast<T*>(grad), r, tiles_of(r.vocab, sizeof(T), 1), softmax, logp, by,
+      device_status_buffer());
   return launched("preference_loss", 1);
 }
 
-// The order of the tasks of a preference loss: a pair of up to kBehindBytes of logits stands in a group of
-// up to kGroupBytes, whose gradients follow the next group's softmaxes; a larger pair's gradients follow
-// its own softmaxes, beginning with the rows read last.
-constexpr long long kGroupBytes = 16 << 20, kBehindBytes = 24 << 20;
-
-constexpr size_t kHead = 16;  // bytes of scratch in front: the ticket, the count of arrived CTAs or pairs done
+constexpr size_t kHead = 16;  // bytes of scratch in front: the count of arrived CTAs
 
 }  // namespace
 }  // namespace t5x
@@ -1479,7 +1356,7 @@ T5X_API int t5x_policy_loss(const void* logits, int fp32, void* grad, long long 
                     static_cast<const float*>(advantages), adv_b, adv_t, 1.f - clip_low, 1.f + clip_high,
                     kl_weight, scale, static_cast<const float*>(normalizer)};
   float* o = static_cast<float*>(out);
-  if (static_cast<long long>(vocab) * (fp32 ? 4 : 2) >= kShortRow)
+  if (by_ring(vocab, fp32))
     return r.rows == 0 ? set_error("policy_loss: no rows")
            : fp32      ? launch_policy<float>(logits, grad, r, p, partial, arrived, o, st)
                        : launch_policy<__nv_bfloat16>(logits, grad, r, p, partial, arrived, o, st);
@@ -1517,9 +1394,8 @@ T5X_API int t5x_policy_loss_tokens(const void* logp, void* slope, long long batc
 }
 
 T5X_API long long t5x_preference_loss_scratch_bytes(long long batch, int length) {
-  // head | softmax and log-probability of each token, a word each | loss and count of each pair | slope of
-  // each row
-  return static_cast<long long>(kHead) + batch * length * 16 + batch * 8 + batch * 4;
+  // head | loss and count of each pair | softmax of each token | log-probability | slope of each row
+  return static_cast<long long>(kHead) + batch * 8 + batch * length * 12 + batch * 4;
 }
 
 T5X_API int t5x_preference_loss(const void* logits, int fp32, void* grad, long long batch, int length, int vocab,
@@ -1538,49 +1414,34 @@ T5X_API int t5x_preference_loss(const void* logits, int fp32, void* grad, long l
                   static_cast<const float*>(weights)};
   const Preference p = {static_cast<const float*>(reference), beta, smoothing, scale,
                         static_cast<const float*>(normalizer)};
-  Work w;
-  w.ticket = reinterpret_cast<unsigned long long*>(at);
-  w.pairs_done = reinterpret_cast<unsigned*>(at + 8);
-  w.softmax = reinterpret_cast<unsigned long long*>(at + kHead);
-  w.score = w.softmax + r.rows;
-  w.pair_loss = reinterpret_cast<double*>(w.score + r.rows);
-  float* by = reinterpret_cast<float*>(w.pair_loss + batch);
-  w.scores = static_cast<float*>(scores);
-  w.margins = static_cast<float*>(margins);
-  float* o = static_cast<float*>(out);
-  const long long row_bytes = static_cast<long long>(vocab) * (fp32 ? 4 : 2);
-  const bool in_long = row_bytes >= kShortRow;
-  cudaError_t e = cudaMemsetAsync(scratch, 0, kHead + (in_long ? r.rows * 16 : 0), st);
+  unsigned* arrived = reinterpret_cast<unsigned*>(at);
+  double* pair_loss = reinterpret_cast<double*>(at + kHead);
+  Softmax* softmax = reinterpret_cast<Softmax*>(pair_loss + batch);
+  float* logp = reinterpret_cast<float*>(softmax + r.rows);
+  float* by = logp + r.rows;
+  cudaError_t e = cudaMemsetAsync(scratch, 0, kHead, st);
   if (e != cudaSuccess) return set_error("preference_loss: memset: %s", cudaGetErrorString(e));
-  if (in_long) {
-    const long long pair_bytes = 2 * length * row_bytes;
-    const long long group = kGroupBytes / pair_bytes > 1 ? kGroupBytes / pair_bytes : 1;
-    w.order = {r.rows, (group < pairs ? group : pairs) * 2 * length, pair_bytes <= kBehindBytes, grad != nullptr};
-    if (fp32 ? launch_preference<float>(logits, grad, r, p, w, o, st)
-             : launch_preference<__nv_bfloat16>(logits, grad, r, p, w, o, st))
-      return -1;
-    if (grad != nullptr) return 0;
-    preference_pairs_kernel<<<static_cast<unsigned>(pairs), kRowThreads, 0, st>>>(
-        reinterpret_cast<const float*>(w.score), 2, r, p, w.scores, w.margins, nullptr, nullptr, w.pair_loss,
-        w.pairs_done, o);
-    return launched("preference_loss", 1);
-  }
-  Softmax* softmax = reinterpret_cast<Softmax*>(w.softmax);
-  float* logp = reinterpret_cast<float*>(w.score);
-  const unsigned grid = row_grid(r.rows);
   auto go = [&](auto* x) {
     using T = std::remove_const_t<std::remove_pointer_t<decltype(x)>>;
-    preference_short_rows_kernel<T><<<grid, kRowThreads, 0, st>>>(x, r, softmax, logp);
+    const bool ring = by_ring(vocab, fp32);
+    const unsigned grid = row_grid(r.rows);
+    int rc = 0;
+    if (ring)
+      rc = launch_preference<T, false>(x, nullptr, r, softmax, logp, nullptr, st);
+    else
+      preference_short_rows_kernel<T><<<grid, kRowThreads, 0, st>>>(x, r, softmax, logp);
+    if (rc != 0) return rc;
     preference_pairs_kernel<<<static_cast<unsigned>(pairs), kRowThreads, 0, st>>>(
-        logp, 1, r, p, w.scores, w.margins, by, nullptr, w.pair_loss, w.pairs_done, o);
-    if (grad != nullptr)
+        logp, r, p, static_cast<float*>(scores), static_cast<float*>(margins), by, nullptr, pair_loss, arrived,
+        static_cast<float*>(out));
+    if (grad == nullptr) return launched("preference_loss", 2 - ring);
+    if (ring)
+      rc = launch_preference<T, true>(x, grad, r, softmax, logp, by, st);
+    else
       preference_short_gradient_kernel<T><<<grid, kRowThreads, 0, st>>>(x, static_cast<T*>(grad), r, softmax, by);
+    return rc != 0 ? rc : launched("preference_loss", ring ? 1 : 3);
   };
-  if (fp32)
-    go(static_cast<const float*>(logits));
-  else
-    go(static_cast<const __nv_bfloat16*>(logits));
-  return launched("preference_loss", 2 + (grad != nullptr));
+  return fp32 ? go(static_cast<const float*>(logits)) : go(static_cast<const __nv_bfloat16*>(logits));
 }
 
 T5X_API int t5x_preference_loss_tokens(const void* logp, void* slope, long long batch, int length,
@@ -1597,7 +1458,7 @@ T5X_API int t5x_preference_loss_tokens(const void* logp, void* slope, long long 
   const Preference p = {static_cast<const float*>(reference), beta, smoothing, scale,
                         static_cast<const float*>(normalizer)};
   preference_pairs_kernel<<<static_cast<unsigned>(batch / 2), kRowThreads, 0, st>>>(
-      static_cast<const float*>(logp), 1, r, p, static_cast<float*>(scores), static_cast<float*>(margins), nullptr,
+      static_cast<const float*>(logp), r, p, static_cast<float*>(scores), static_cast<float*>(margins), nullptr,
       static_cast<float*>(slope), reinterpret_cast<double*>(static_cast<char*>(scratch) + kHead),
       static_cast<unsigned*>(scratch), static_cast<float*>(out));
   return launched("preference_loss_tokens", 1);

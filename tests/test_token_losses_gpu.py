@@ -103,8 +103,8 @@ def check(kind, out, grad, d, factor):
 
 
 SHAPES = [(2, 1, 1), (2, 1, 2), (2, 3, 7), (4, 5, 31), (2, 2, 33), (6, 9, 384), (4, 3, 385), (2, 4, 2047), (2, 3, 2048),
-          (4, 3, 2049), (2, 5, 4099), (2, 7, 32128), (4, 2, 32101), (2, 2, 65537), (2, 1, 250112), (2, 600, 40),
-          (40, 33, 100), (2, 40, 12345)]
+          (4, 3, 2049), (2, 5, 4099), (2, 7, 32128), (4, 2, 32101), (2, 2, 65537), (2, 1, 250112), (2, 3, 530000), (10, 2, 8193), (6, 50, 16390), (2, 2, 131071), (2, 600, 40),
+          (40, 33, 100), (2, 40, 12345), (8, 150, 4100), (4, 300, 9001), (6, 120, 32101), (10, 100, 20000), (4, 25, 250112)]
 
 
 @pytest.mark.parametrize("kind", ["preference", "policy"])
