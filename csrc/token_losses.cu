@@ -30,6 +30,7 @@ namespace {
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kRowThreads = 512;
+constexpr int kCtasPerSm = 8;  // at most, of every grid here whose CTAs leave sums in the scratch
 
 __device__ __forceinline__ float exp2_approx(float x) {
   float r;
@@ -471,89 +472,13 @@ __global__ void __launch_bounds__(kRowThreads)
 }
 
 // ---- long rows ----
-// What both kernels share. A CTA's producer thread copies rows in tiles of up to 8 KB into a ring in
-// shared memory, far ahead of the worker warps. A tile is one warp's, the next tile the next warp's: the
-// warps of an SM are at different places of their work, so that some load or wait while others keep the
-// units for the exponentials busy (with a tile for all warps they stood in step: 375M logits summed in
-// 283 us instead of XXX). A keeper warp makes of the warps' sums what the gradient of the row needs, so that no
-// worker waits for the load of a single value, a logarithm or another CTA; the producer hands it a row's few
-// values, which it has asked for rows ahead.
-constexpr int kTileBytes = 8192;
-constexpr int kTilePacks = kTileBytes / 16;
-
-enum Kind : int { kEnd, kStat, kGrad, kZero };
-// What the gradient of a row needs: by * onehot(target) + k * exp(x - most) with k = -by / sum.
-struct Slope {
-  float most, by, k;
-  int target;
-};
-struct Tile {
-  long long offset;  // of the row in the logits and their gradient
-  int kind;
-  int last;          // the warp's last tile of the row
-  int head;          // values in front of the row's first 16-byte boundary
-  int at, packs;     // first 16 bytes behind it, how many
-  int outside;       // 16 bytes of the whole row, on the tile whose warp sees to the values outside; else -1
-  unsigned task;     // the how-many-th of the CTA's rows that are summed
-  Slope now;         // of a kGrad tile
-};
-struct Task {
-  long long row, b;
-  int kind, target;  // target: -1 outside of the vocabulary
-  float w, x;        // weight, the target's logit
-  int warp;          // whose is the row's first tile
-  PolicyInputs in;
-};
-// Slots for rows between their sums and their gradient: more than the ring has tiles, so that none is written
-// again before the warps that read it have given their tiles back.
-template <int kStages_, int kWarps_, int kSlots_>
-struct LongShared {
-  static constexpr int kStages = kStages_, kWarps = kWarps_, kSlots = kSlots_;
-  alignas(128) unsigned char data[kStages][kTileBytes];
-  uint64_t full[kStages], empty[kStages], told[kSlots], kept[kSlots], sums[kSlots], said[kSlots], met[kSlots];
-  Tile tile[kStages];
-  Task task[kSlots];
-  Softmax part[kSlots][kWarps];
-  Softmax of_cta[kSlots][8];  // of the CTAs that share the row
-  Slope slope[kSlots];
-  int abort;
-  __device__ void init(int warps_of_row) {
-    for (int i = 0; i < kStages; ++i) {
-      mbar_init(&full[i], 1);
-      mbar_init(&empty[i], 1);
-    }
-    for (int i = 0; i < kSlots; ++i) {
-      mbar_init(&told[i], 1);
-      mbar_init(&kept[i], 1);
-      mbar_init(&sums[i], warps_of_row);
-      mbar_init(&said[i], 1);
-      mbar_init(&met[i], 1);
-    }
-    abort = 0;
-    mbar_fence_init();
-  }
-  // The sums of a row's warps, in every lane of the keeper.
-  __device__ Softmax all_parts(int slot, int first, int warps_of_row) const;
-};
-
-// A wait with a limit of a second or two (a poll may be held back for some ten microseconds).
-constexpr uint32_t kPolls = 1u << 17;
-__device__ __forceinline__ bool ring_wait(uint64_t* bar, uint32_t parity, volatile int* abort) {
-  for (uint32_t it = 0; it < kPolls; ++it) {
-    if (mbar_try_wait(bar, parity)) return true;
-    if ((it & 0xf) == 0xf && *abort) return false;
-  }
-  return false;
-}
-
-// The part of a row between 16-byte boundaries.
-template <typename T>
-__device__ __forceinline__ void aligned_part(const T* row, int vocab, int& head, int& packs) {
-  constexpr int kN = Pack<T>::kN;
-  const int off = static_cast<int>(reinterpret_cast<uintptr_t>(row) & 15) / static_cast<int>(sizeof(T));
-  head = off ? kN - off : 0;
-  packs = (vocab - head) / kN;
-}
+// A CTA takes a row, or its part of a row that a cluster of CTAs shares, into registers: kPacks times 16 bytes
+// a thread, all loads in flight at once, while the SM's other CTAs are at other places of their rows. The
+// row's softmax and its gradient are both made from there, so that logits are read once. Larger rows than
+// eight CTAs hold go by in chunks, which are read a second time for the gradient.
+//
+// What bounds it: memory (read once, written once); the exponentials take 0.4 of its time for bf16 logits.
+constexpr int kPacks = 8;
 
 // Two values at once where the arithmetic has pairs.
 __device__ __forceinline__ uint64_t pair_of(float a, float b) {
@@ -581,9 +506,9 @@ __device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
 }
 __device__ __forceinline__ uint64_t same2(float a) { return pair_of(a, a); }
 
-// In the tiles an exponential exp(x - most) is exp2(x log2 e - ref), a fused product and difference, with
-// ref = most log2 e as rounded: the same factor for the sum, the target and the gradient. Where a largest
-// logit's product may overflow, it is exp2((x - most) log2 e).
+// An exponential exp(x - most) is exp2(x log2 e - ref) here, a fused product and difference, with ref =
+// most log2 e as rounded: the same factor for the sum, the target and the gradient. Where a largest logit's
+// product may overflow, it is exp2((x - most) log2 e).
 constexpr float kHuge = 1.0e38f;
 __device__ __forceinline__ bool huge(float most) { return !(fabsf(most) <= kHuge); }  // (NaN and -inf too)
 // log2 of exp(a - b); 0 for a = b = -inf
@@ -599,9 +524,11 @@ __device__ __forceinline__ Softmax join_rows(Softmax a, Softmax b) {
   const float m = fmaxf(a.most, b.most);
   return {m, a.sum * exp2_approx(shift(a.most, m)) + b.sum * exp2_approx(shift(b.most, m))};
 }
+// of `kLanes` lanes of a warp
+template <int kLanes>
 __device__ __forceinline__ Softmax join_row_lanes(Softmax s) {
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1)
+  for (int o = kLanes / 2; o > 0; o >>= 1)
     s = join_rows(s, {__shfl_xor_sync(0xffffffffu, s.most, o), __shfl_xor_sync(0xffffffffu, s.sum, o)});
   return s;
 }
@@ -611,603 +538,304 @@ __device__ __forceinline__ float log_prob_of(float x, Softmax s) {
   return d - log1pf(s.sum - 1.f);
 }
 
-// 16 bytes of a tile, as pairs
+// What the gradient of a row needs: by * onehot(target) + k * exp(x - most) with k = -by / sum.
+struct Slope {
+  float most, by, k;
+  int target;  // -1: outside of the vocabulary
+};
+
+// 16 bytes of logits as pairs.
 template <typename T>
-struct Pairs;
+struct Unpack;
 template <>
-struct Pairs<float> {
+struct Unpack<float> {
   static constexpr int kPairs = 2;
-  uint64_t v[2];
-  __device__ void load(const void* p) {
-    const float4 x = *static_cast<const float4*>(p);
-    v[0] = pair_of(x.x, x.y), v[1] = pair_of(x.z, x.w);
+  __device__ static void pairs(uint4 u, uint64_t* v) {
+    v[0] = pair_of(__uint_as_float(u.x), __uint_as_float(u.y));
+    v[1] = pair_of(__uint_as_float(u.z), __uint_as_float(u.w));
   }
-  __device__ void nothing() { v[0] = v[1] = same2(-INFINITY); }
-  __device__ float most() const {
-    float a, b, c, d;
-    split(v[0], a, b), split(v[1], c, d);
-    return fmaxf(fmaxf(a, b), fmaxf(c, d));
+  __device__ static uint4 nothing() { return make_uint4(0xff800000u, 0xff800000u, 0xff800000u, 0xff800000u); }
+  __device__ static float most(uint4 u) {
+    return fmaxf(fmaxf(__uint_as_float(u.x), __uint_as_float(u.y)), fmaxf(__uint_as_float(u.z), __uint_as_float(u.w)));
   }
 };
 template <>
-struct Pairs<__nv_bfloat16> {
+struct Unpack<__nv_bfloat16> {
   static constexpr int kPairs = 4;
-  uint64_t v[4];
-  float top;
-  __device__ void load(const void* p) {
-    const uint4 x = *static_cast<const uint4*>(p);
+  __device__ static void pairs(uint4 x, uint64_t* v) {
     const uint32_t u[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
     for (int i = 0; i < 4; ++i) v[i] = pair_of(__uint_as_float(u[i] << 16), __uint_as_float(u[i] & 0xffff0000u));
-    const __nv_bfloat162 m = __hmax2(__hmax2(as2(u[0]), as2(u[1])), __hmax2(as2(u[2]), as2(u[3])));
-    top = fmaxf(__low2float(m), __high2float(m));
   }
-  __device__ void nothing() {
-    v[0] = v[1] = v[2] = v[3] = same2(-INFINITY);
-    top = -INFINITY;
-  }
+  __device__ static uint4 nothing() { return make_uint4(0xff80ff80u, 0xff80ff80u, 0xff80ff80u, 0xff80ff80u); }
   __device__ static __nv_bfloat162 as2(uint32_t u) { return *reinterpret_cast<__nv_bfloat162*>(&u); }
-  __device__ float most() const { return top; }
-};
-
-// exp2 of the two values
-__device__ __forceinline__ uint64_t exp2_pair(uint64_t x) {
-  float a, b;
-  split(x, a, b);
-  return pair_of(exp2_approx(a), exp2_approx(b));
-}
-
-template <int kStages, int kWarps, int kSlots>
-__device__ Softmax LongShared<kStages, kWarps, kSlots>::all_parts(int slot, int first, int warps_of_row) const {
-  const int lane = threadIdx.x & 31;
-  return join_row_lanes(lane < warps_of_row ? part[slot][(first + lane) % kWarps] : Softmax{-INFINITY, 0.f});
-}
-
-// Adds a lane's 16 bytes each to what it has seen.
-template <typename T, int kMine>
-__device__ __forceinline__ void take(Softmax& s, const Pairs<T>* x) {
-  constexpr int kP = Pairs<T>::kPairs;
-  float m = x[0].most();
-#pragma unroll
-  for (int i = 1; i < kMine; ++i) m = fmaxf(m, x[i].most());
-  if (m > s.most) {
-    s.sum *= exp2_approx(shift(s.most, m));
-    s.most = m;
-  }
-  uint64_t t[2] = {same2(0.f), same2(0.f)};
-  if (!huge(s.most)) {
-    const float ref = __fmul_rn(s.most, kLog2e);
-    const uint64_t l2e = same2(kLog2e), off = same2(-ref);
-#pragma unroll
-    for (int i = 0; i < kMine; ++i)
-#pragma unroll
-      for (int j = 0; j < kP; ++j) t[j & 1] = add2(t[j & 1], exp2_pair(fma2(x[i].v[j], l2e, off)));
-  } else {
-#pragma unroll
-    for (int i = 0; i < kMine; ++i)
-#pragma unroll
-      for (int j = 0; j < kP; ++j) {
-        float a, b;
-        split(x[i].v[j], a, b);
-        t[0] = add2(t[0], pair_of(exp_from(a, s.most), exp_from(b, s.most)));
-      }
-  }
-  float a, b;
-  split(add2(t[0], t[1]), a, b);
-  s.sum += a + b;
-}
-
-// The tile's part of the row's softmax; a warp's.
-template <typename T>
-__device__ __forceinline__ void sum_tile(Softmax& s, const unsigned char* data, int packs, int lane) {
-  constexpr int kMine = 4;
-  Pairs<T> x[kMine];
-  int at = 0;
-#pragma unroll 1
-  for (; at + kMine * 32 <= packs; at += kMine * 32) {
-#pragma unroll
-    for (int i = 0; i < kMine; ++i) x[i].load(data + (at + i * 32 + lane) * 16);
-    take<T, kMine>(s, x);
-  }
-  if (at < packs) {
-#pragma unroll
-    for (int i = 0; i < kMine; ++i) {
-      if (at + i * 32 + lane < packs)
-        x[i].load(data + (at + i * 32 + lane) * 16);
-      else
-        x[i].nothing();
-    }
-    take<T, kMine>(s, x);
-  }
-}
-
-// The tile's part of the gradient; a warp's. g: the row's.
-template <typename T>
-__device__ __forceinline__ void turn_tile(T* g, const unsigned char* data, const Tile& t, const Slope& now, int lane) {
-  constexpr int kN = Pack<T>::kN;
-  const int first = t.head + t.at * kN;
-  const bool far = huge(now.most);
-  const float ref = __fmul_rn(now.most, kLog2e);
-  const uint64_t l2e = same2(kLog2e), off = same2(-ref), k2 = same2(now.k);
-  auto one = [&](int i, auto plain) {
-    Pairs<T> v;
-    v.load(data + i * 16);
-    float x[kN];
-#pragma unroll
-    for (int j = 0; j < kN / 2; ++j) {
-      uint64_t e;
-      if (plain || !far) {
-        e = exp2_pair(fma2(v.v[j], l2e, off));
-      } else {
-        float a, b;
-        split(v.v[j], a, b);
-        e = pair_of(exp_from(a, now.most), exp_from(b, now.most));
-      }
-      split(mul2(e, k2), x[2 * j], x[2 * j + 1]);
-    }
-    const int at = first + i * kN;
-    if (!plain && static_cast<unsigned>(now.target - at) < static_cast<unsigned>(kN)) {
-#pragma unroll
-      for (int j = 0; j < kN; ++j)
-        if (now.target == at + j) x[j] += now.by;
-    }
-    Pack<T>::store(g + at, x);
-  };
-  // a tile without the target, of a row whose exponentials take the short way
-  if (!far && static_cast<unsigned>(now.target - first) >= static_cast<unsigned>(t.packs * kN)) {
-#pragma unroll 4
-    for (int i = lane; i < t.packs; i += 32) one(i, std::true_type());
-  } else {
-#pragma unroll 1
-    for (int i = lane; i < t.packs; i += 32) one(i, std::false_type());
-  }
-}
-
-// The value outside of the row's 16-byte boundaries that a thread sees to, or -1.
-template <typename T>
-__device__ __forceinline__ int outside_of(const Tile& t, int vocab, int tid) {
-  if (t.outside < 0) return -1;
-  const int behind = t.outside * Pack<T>::kN;  // head + ... - head
-  return tid < t.head ? tid : (tid < vocab - behind ? behind + tid : -1);
-}
-template <typename T>
-__device__ __forceinline__ Softmax one_value(T v) {
-  const float x = Pack<T>::one(v);
-  return {x, x == -INFINITY ? 0.f : x * 0.f + 1.f};  // (NaN of +inf and NaN)
-}
-template <typename T>
-__device__ __forceinline__ void turn_one(T* g, const T* row, int i, const Slope& now) {
-  const float v = now.k * exp_from(Pack<T>::one(row[i]), now.most);
-  g[i] = Pack<T>::back(i == now.target ? v + now.by : v);
-}
-
-// The producer's side of a ring; one thread's.
-template <typename Shared>
-struct Ring {
-  static constexpr int kStages = Shared::kStages, kSlots = Shared::kSlots;
-  Shared& sh;
-  volatile int* abort;
-  int stage = 0, warp = 0, issued = 0;  // warp: whose the next tile is
-  uint32_t round = 0;
-  unsigned tasks = 0;
-  bool ok = true;
-  __device__ Ring(Shared& s) : sh(s), abort(&s.abort) {}
-  __device__ void push(const Tile& t, const void* src) {
-    if (!ok || !ring_wait(&sh.empty[stage], (round & 1) ^ 1, abort)) {
-      ok = false;
-      return;
-    }
-    sh.tile[stage] = t;
-    if (src != nullptr) {
-      mbar_expect_tx(&sh.full[stage], t.packs * 16);
-      bulk_load(sh.data[stage], src, t.packs * 16, &sh.full[stage]);
-    } else {
-      mbar_arrive(&sh.full[stage]);
-    }
-    ++issued;
-    if (++warp == Shared::kWarps) warp = 0;
-    if (++stage == kStages) stage = 0, ++round;
-  }
-  // The keeper, of a row ahead of its tiles.
-  __device__ void tell(Task t) {
-    const int slot = tasks % kSlots;
-    if (!ok || !ring_wait(&sh.kept[slot], (tasks / kSlots & 1) ^ 1, abort)) {
-      ok = false;
-      return;
-    }
-    t.warp = warp;
-    sh.task[slot] = t;
-    mbar_arrive(&sh.told[slot]);
-    ++tasks;
-  }
-  // `packs` 16 bytes of a row from `from`, in `tiles` tiles of one size.
-  template <typename T>
-  __device__ void stream(Tile t, const T* logits, int from, int packs, int tiles) {
-    const int size = (packs + tiles - 1) / tiles;
-    for (int i = 0; i < tiles && ok; ++i) {
-      t.at = from + i * size;
-      t.packs = packs - i * size < size ? packs - i * size : size;
-      t.last = i + Shared::kWarps >= tiles;
-      push(t, logits + t.offset + t.head + static_cast<long long>(t.at) * Pack<T>::kN);
-      t.outside = -1;
-    }
-  }
-  __device__ void end() {
-    Task t = {};
-    t.kind = kEnd;
-    tell(t);
-    for (int i = 0; i < Shared::kWarps; ++i) push({0, kEnd, 1, 0, 0, 0, -1, 0, {}}, nullptr);
-  }
-  // No copy may be under way when the shared memory is given back.
-  __device__ void drain() {
-    const int n = issued < kStages ? issued : kStages;
-    for (int i = issued - n; i < issued; ++i)
-      for (uint32_t it = 0; it < kPolls && !mbar_try_wait(&sh.full[i % kStages], (i / kStages) & 1); ++it) {
-      }
+  __device__ static float most(uint4 x) {
+    const __nv_bfloat162 m = __hmax2(__hmax2(as2(x.x), as2(x.y)), __hmax2(as2(x.z), as2(x.w)));
+    return fmaxf(__low2float(m), __high2float(m));
   }
 };
 
-// A worker warp's side: its tiles are every kWarps-th of the ring.
-template <typename Shared>
-struct Turn {
-  int stage;
-  uint32_t round;
-  __device__ void advance() {
-    stage += Shared::kWarps;
-    while (stage >= Shared::kStages) stage -= Shared::kStages, ++round;
+// A thread's share of a chunk of a row.
+template <typename T, int kThreads>
+struct Share {
+  static constexpr int kN = Pack<T>::kN;
+  uint4 x[kPacks];
+
+  // 16 bytes number tid, tid + kThreads, ... of `packs` at p
+  __device__ __forceinline__ void load(const T* p, int packs, int tid) {
+#pragma unroll
+    for (int i = 0; i < kPacks; ++i) {
+      const int at = i * kThreads + tid;
+      x[i] = at < packs ? reinterpret_cast<const uint4*>(p)[at] : Unpack<T>::nothing();
+    }
   }
-};
-
-// Policy. A row belongs to a cluster of CTAs, of which each takes a part that fits into its ring with room for
-// the next ones: the part is read once, summed, and turned into the gradient where it lies. The parts' sums
-// meet through distributed shared memory. A warp turns a tile behind the sums of its next one, so that it does
-// not wait for the row's slope. (Tile t is turned behind the sums of its row, which end n - 1 tiles later at
-// most, and of tile t + kWarps; tile u is loaded when tile u - kStages is turned: with n and kWarps no more than
-// kStages the turning waits for smaller tiles only.)
-using PolicyShared = LongShared<26, 16, 32>;
-constexpr int kPolicyThreads = PolicyShared::kWarps * 32 + 64;
-
-__device__ __forceinline__ void send_to_cta(Softmax* slot, uint64_t* bar, int cta, Softmax s) {
-  uint64_t v;
-  memcpy(&v, &s, 8);
-  asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.b64 [%0], %1, [%2];" ::"r"(
-                   mapa_shared(smem_u32(slot), cta)),
-               "l"(v), "r"(mapa_shared(smem_u32(bar), cta))
-               : "memory");
-}
-
-template <typename T>
-__global__ void __launch_bounds__(kPolicyThreads, 1)
-    policy_rows_kernel(const T* __restrict__ logits, T* __restrict__ grad, const Rows r, const Policy p, int ctas,
-                       int tiles, double* partial, unsigned* arrived, float* out, int* status) {
-  constexpr int kN = Pack<T>::kN, kWarps = PolicyShared::kWarps, kSlots = PolicyShared::kSlots;
-  extern __shared__ __align__(128) unsigned char raw[];
-  PolicyShared& sh = *reinterpret_cast<PolicyShared*>(raw);
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int rank = ctas > 1 ? static_cast<int>(cluster_ctarank()) : 0;
-  const long long cluster = blockIdx.x / ctas, clusters = gridDim.x / ctas;
-  const int warps_of_row = tiles < kWarps ? tiles : kWarps;
-  if (tid == 0) sh.init(warps_of_row);
-  __syncthreads();
-  if (ctas > 1) cluster_sync_all();  // every CTA's barriers stand before another signals one
-  volatile int* abort = &sh.abort;
-  bool ok = true;
-  auto wait = [&](uint64_t* bar, uint32_t parity) {  // the whole warp's
-    ok = __all_sync(0xffffffffu, ring_wait(bar, parity, abort));
-    return ok;
-  };
-  auto give_up = [&](int code) {
-    if (lane == 0) {
-      *abort = 1;
-      report_status(status, code, 41, warp);
-    }
-  };
-
-  if (warp == kWarps) {  // ---- producer: 32 rows' values at a time, asked for while the last 32 go by ----
-    Ring<PolicyShared> ring(sh);
-    Task next = {};
-    long long next_offset = 0;
-    auto ask = [&](long long base) {
-      next.row = base + lane * clusters;
-      next.kind = kEnd;
-      if (next.row >= r.rows) return;
-      next.b = next.row / r.length;
-      const long long t = next.row - next.b * r.length;
-      next_offset = next.b * r.stride_b + t * r.stride_t;
-      next.w = r.weights != nullptr ? r.weights[next.row] : 1.f;
-      next.kind = next.w != 0.f ? kStat : kZero;
-      if (next.kind == kZero) return;
-      const long long target = r.targets[next.row];
-      next.target = target >= 0 && target < r.vocab ? static_cast<int>(target) : -1;
-      next.in = policy_inputs(p, next.row, next.b, t);
-      next.x = next.target >= 0 ? Pack<T>::one(logits[next_offset + next.target]) : NAN;
-    };
-    ask(cluster);
-    for (long long base = cluster; base < r.rows; base += 32 * clusters) {
-      const Task mine = next;
-      const long long offset = next_offset;
-      if (base + 32 * clusters < r.rows) ask(base + 32 * clusters);
-      for (int i = 0; i < 32; ++i) {
-        Task t;
-        t.row = base + i * clusters;
-        if (t.row >= r.rows) break;
-        t.b = __shfl_sync(0xffffffffu, mine.b, i);
-        t.kind = __shfl_sync(0xffffffffu, mine.kind, i);
-        t.target = __shfl_sync(0xffffffffu, mine.target, i);
-        t.w = __shfl_sync(0xffffffffu, mine.w, i);
-        t.x = __shfl_sync(0xffffffffu, mine.x, i);
-        t.in = {__shfl_sync(0xffffffffu, mine.in.old, i), __shfl_sync(0xffffffffu, mine.in.ref, i),
-                __shfl_sync(0xffffffffu, mine.in.advantage, i)};
-        Tile tile = {__shfl_sync(0xffffffffu, offset, i), t.kind, 1, 0, 0, 0, -1, 0, {}};
-        int all;
-        aligned_part(logits + tile.offset, r.vocab, tile.head, all);
-        const int part = (all + ctas - 1) / ctas, from = part * rank < all ? part * rank : all;
-        const int packs = all - from < part ? all - from : part;
-        if (t.kind == kZero) {  // (all lanes': nothing of it is in the way of the tiles)
-          if (grad == nullptr) continue;
-          T* g = grad + tile.offset;
-          for (int k = lane; k < packs; k += 32)
-            *reinterpret_cast<uint4*>(g + tile.head + static_cast<long long>(from + k) * kN) = make_uint4(0, 0, 0, 0);
-          tile.outside = rank == 0 ? all : -1;
-          const int k = outside_of<T>(tile, r.vocab, lane);
-          if (k >= 0) g[k] = Pack<T>::back(0.f);
-          continue;
-        }
-        if (lane != 0) continue;
-        tile.outside = rank == 0 ? all : -1;
-        tile.task = ring.tasks;
-        ring.tell(t);
-        ring.stream(tile, logits, from, packs, tiles);
-      }
-    }
-    if (lane == 0) {
-      ring.end();
-      if (!ring.ok) {
-        give_up(kStatusTimeoutProducer);
-        ring.drain();
-      }
-    }
-  } else if (warp > kWarps) {  // ---- keeper ----
-    const float scale = scale_of(p.normalizer, p.scale);
-    double sums[4] = {0.0, 0.0, 0.0, 0.0};
-    for (unsigned n = 0;; ++n) {
-      const int slot = n % kSlots;
-      const uint32_t parity = n / kSlots & 1;
-      if (!wait(&sh.told[slot], parity)) break;
-      const Task t = sh.task[slot];
-      if (t.kind == kEnd) break;
-      if (!wait(&sh.sums[slot], parity)) break;
-      Softmax s = sh.all_parts(slot, t.warp, warps_of_row);
-      if (ctas > 1) {
-        if (lane == 0) mbar_expect_tx(&sh.met[slot], 8 * ctas);
-        __syncwarp();
-        if (lane < ctas) send_to_cta(&sh.of_cta[slot][rank], &sh.met[slot], lane, s);
-        if (!wait(&sh.met[slot], parity)) break;
-        s = join_row_lanes(lane < ctas ? sh.of_cta[slot][lane] : Softmax{-INFINITY, 0.f});
-      }
-      if (lane == 0) {
-        const PolicyToken c = policy_token(p, t.in, log_prob_of(t.x, s));
-        const float by = t.w * c.slope * scale;
-        sh.slope[slot] = {s.most, by, -by / s.sum, t.target};
-        mbar_arrive(&sh.said[slot]);
-        mbar_arrive(&sh.kept[slot]);
-        sums[0] += static_cast<double>(t.w) * c.loss;
-        sums[1] += static_cast<double>(t.w) * c.kl;
-        sums[2] += static_cast<double>(t.w) * c.clipped;
-        sums[3] += t.w;
-      }
-      __syncwarp();
-    }
-    if (!ok) give_up(kStatusTimeoutEpilogue);
-    unsigned before = 0;
-    if (lane == 0 && rank == 0) {
+  __device__ __forceinline__ void add_to(Softmax& s, int packs) const {
+    float m = s.most;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) partial[cluster * 4 + i] = ok ? sums[i] : NAN;
-      __threadfence();
-      before = atomicAdd(arrived, 1u) + 1;
+    for (int i = 0; i < kPacks; ++i)
+      if (i * kThreads < packs) m = fmaxf(m, Unpack<T>::most(x[i]));
+    if (m > s.most) {
+      s.sum *= exp2_approx(shift(s.most, m));
+      s.most = m;
     }
-    if (__shfl_sync(0xffffffffu, before, 0) == clusters) {
-      __threadfence();
-      const double whole = p.normalizer != nullptr ? 1.0 / static_cast<double>(*p.normalizer) : p.scale;
+    uint64_t t[2] = {same2(0.f), same2(0.f)};
+    if (!huge(s.most)) {
+      const uint64_t l2e = same2(kLog2e), off = same2(-__fmul_rn(s.most, kLog2e));
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        double v = 0.0;
-        for (long long c = lane; c < clusters; c += 32) v += __ldcg(partial + c * 4 + i);
+      for (int i = 0; i < kPacks; ++i)
+        if (i * kThreads < packs) {
+          uint64_t v[Unpack<T>::kPairs];
+          Unpack<T>::pairs(x[i], v);
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-        if (lane == 0) out[i] = static_cast<float>(i < 2 ? v * whole : v);
-      }
-    }
-  } else {  // ---- workers ----
-    Turn<PolicyShared> at = {warp, 0}, old = at;  // old: of the tile whose gradient is still to come
-    bool pending = false;
-    Softmax seen = {-INFINITY, 0.f};
-    auto turn = [&](int stage) {
-      const Tile t = sh.tile[stage];
-      if (!wait(&sh.said[t.task % kSlots], t.task / kSlots & 1)) return;
-      const Slope now = sh.slope[t.task % kSlots];
-      const int i = outside_of<T>(t, r.vocab, lane);
-      if (i >= 0) turn_one(grad + t.offset, logits + t.offset, i, now);
-      turn_tile<T>(grad + t.offset, sh.data[stage], t, now, lane);
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&sh.empty[stage]);
-    };
-    while (wait(&sh.full[at.stage], at.round & 1)) {
-      const Tile t = sh.tile[at.stage];
-      if (t.kind == kStat) {
-        const int i = outside_of<T>(t, r.vocab, lane);
-        if (i >= 0) seen = one_value(logits[t.offset + i]);
-        sum_tile<T>(seen, sh.data[at.stage], t.packs, lane);
-        if (t.last) {
-          const Softmax s = join_row_lanes(seen);
-          if (lane == 0) {
-            sh.part[t.task % kSlots][warp] = s;
-            mbar_arrive(&sh.sums[t.task % kSlots]);
+          for (int j = 0; j < Unpack<T>::kPairs; ++j) {
+            float a, b;
+            split(fma2(v[j], l2e, off), a, b);
+            t[j & 1] = add2(t[j & 1], pair_of(exp2_approx(a), exp2_approx(b)));
           }
-          seen = {-INFINITY, 0.f};
         }
-        if (grad == nullptr) {
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&sh.empty[at.stage]);
-          at.advance();
-          continue;
+    } else {
+#pragma unroll 1
+      for (int i = 0; i < kPacks; ++i) {
+        uint64_t v[Unpack<T>::kPairs];
+        Unpack<T>::pairs(pick(i), v);
+#pragma unroll
+        for (int j = 0; j < Unpack<T>::kPairs; ++j) {
+          float a, b;
+          split(v[j], a, b);
+          t[0] = add2(t[0], pair_of(exp_from(a, s.most), exp_from(b, s.most)));
         }
       }
-      if (pending) turn(old.stage);
-      pending = t.kind == kStat;
-      old = at;
-      if (!ok || t.kind == kEnd) break;
-      at.advance();
     }
-    if (!ok) give_up(kStatusTimeoutEpilogue);
+    float a, b;
+    split(add2(t[0], t[1]), a, b);
+    s.sum += a + b;
   }
-  if (ctas > 1) {
-    __syncwarp();
-    cluster_sync_all();  // no CTA ends while another may still write to it
+  // x[i] for an i that the compiler does not know, without the array leaving the registers
+  __device__ __forceinline__ uint4 pick(int i) const {
+    uint4 v = x[0];
+#pragma unroll
+    for (int k = 1; k < kPacks; ++k)
+      if (k == i) v = x[k];
+    return v;
   }
-}
-
-// Preference. The slope of a row needs the sums of all rows of its pair: one kernel makes the rows' softmaxes
-// and log-probabilities, another (above) the pairs' slopes, a third, beginning with the rows read last, which
-// are still in L2, the gradients. (One kernel for all of it, whose gradients waited for the rows of their pair,
-// would read most logits from L2 the second time, but its CTAs wait for one another.) Two CTAs an SM.
-using PairShared = LongShared<12, 8, 16>;
-constexpr int kPairThreads = PairShared::kWarps * 32 + 64;
-
-// kTurn: the gradients, from `softmax` and the slopes `by` of the sequences; else the softmaxes.
-template <typename T, bool kTurn>
-__global__ void __launch_bounds__(kPairThreads, 2)
-    preference_rows_kernel(const T* __restrict__ logits, T* __restrict__ grad, const Rows r, int tiles,
-                           Softmax* __restrict__ softmax, float* __restrict__ logp, const float* __restrict__ by,
-                           int* status) {
-  constexpr int kWarps = PairShared::kWarps, kSlots = PairShared::kSlots;
-  const int warps_of_row = tiles < kWarps ? tiles : kWarps;
-  extern __shared__ __align__(128) unsigned char raw[];
-  PairShared& sh = *reinterpret_cast<PairShared*>(raw);
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  if (tid == 0) sh.init(warps_of_row);
-  __syncthreads();
-  volatile int* abort = &sh.abort;
-  bool ok = true;
-  auto wait = [&](uint64_t* bar, uint32_t parity) {  // the whole warp's
-    ok = __all_sync(0xffffffffu, ring_wait(bar, parity, abort));
-    return ok;
-  };
-  auto give_up = [&](int code) {
-    if (lane == 0) {
-      *abort = 1;
-      report_status(status, code, 42, warp);
-    }
-  };
-
-  if (warp == kWarps) {  // ---- producer: 32 rows' values at a time, asked for while the last 32 go by ----
-    Ring<PairShared> ring(sh);
-    Task next = {};
-    Slope next_slope = {};
-    long long next_offset = 0;
-    auto ask = [&](long long base) {
-      const long long at = base + static_cast<long long>(lane) * gridDim.x;
-      next.kind = kEnd;
-      if (at >= r.rows) return;
-      next.row = kTurn ? r.rows - 1 - at : at;
-      next.b = next.row / r.length;
-      next_offset = next.b * r.stride_b + (next.row - next.b * r.length) * r.stride_t;
-      next.w = r.weights != nullptr ? r.weights[next.row] : 1.f;
-      next.kind = next.w != 0.f ? (kTurn ? kGrad : kStat) : kZero;
-      if (next.kind == kZero) return;
-      const long long target = r.targets[next.row];
-      next.target = target >= 0 && target < r.vocab ? static_cast<int>(target) : -1;
-      if (kTurn) {
-        const Softmax s = softmax[next.row];
-        const float slope = next.w * by[next.b];
-        next_slope = {s.most, slope, -slope / s.sum, next.target};
-      } else {
-        next.x = next.target >= 0 ? Pack<T>::one(logits[next_offset + next.target]) : NAN;
+  // Stores the gradient at g; `first`: the index in the row of the chunk's first value.
+  __device__ __forceinline__ void turn(T* g, int packs, int first, const Slope& now, int tid) const {
+    const uint64_t l2e = same2(kLog2e), off = same2(-__fmul_rn(now.most, kLog2e)), k2 = same2(now.k);
+    const bool far = huge(now.most);
+    auto one = [&](uint4 u, int at, auto plain) {
+      uint64_t v[Unpack<T>::kPairs];
+      Unpack<T>::pairs(u, v);
+      float y[kN];
+#pragma unroll
+      for (int j = 0; j < kN / 2; ++j) {
+        float a, b;
+        if (plain || !far) {
+          split(fma2(v[j], l2e, off), a, b);
+          a = exp2_approx(a), b = exp2_approx(b);
+        } else {
+          split(v[j], a, b);
+          a = exp_from(a, now.most), b = exp_from(b, now.most);
+        }
+        split(mul2(pair_of(a, b), k2), y[2 * j], y[2 * j + 1]);
       }
+      if (!plain) {
+        const int off_target = now.target - (first + at * kN);
+#pragma unroll
+        for (int j = 0; j < kN; ++j)
+          if (off_target == j) y[j] += now.by;
+      }
+      Pack<T>::store(g + at * kN, y);
     };
-    ask(blockIdx.x);
-    for (long long base = blockIdx.x; base < r.rows; base += 32ll * gridDim.x) {
-      const Task mine = next;
-      const Slope slope = next_slope;
-      const long long offset = next_offset;
-      if (base + 32ll * gridDim.x < r.rows) ask(base + 32ll * gridDim.x);
-      for (int i = 0; i < 32; ++i) {
-        if (base + static_cast<long long>(i) * gridDim.x >= r.rows) break;
-        Task t;
-        t.row = __shfl_sync(0xffffffffu, mine.row, i);
-        t.b = 0;
-        t.kind = __shfl_sync(0xffffffffu, mine.kind, i);
-        t.target = 0;
-        t.w = 0.f;
-        t.x = __shfl_sync(0xffffffffu, mine.x, i);
-        t.in = {};
-        Tile tile = {__shfl_sync(0xffffffffu, offset, i), t.kind, 1, 0, 0, 0, -1, 0, {}};
-        tile.now = {__shfl_sync(0xffffffffu, slope.most, i), __shfl_sync(0xffffffffu, slope.by, i),
-                    __shfl_sync(0xffffffffu, slope.k, i), __shfl_sync(0xffffffffu, slope.target, i)};
-        int all;
-        aligned_part(logits + tile.offset, r.vocab, tile.head, all);
-        if (t.kind == kZero) {  // (all lanes')
-          if (kTurn) row_zero(grad + tile.offset, r.vocab, lane, 32);
-          continue;
-        }
-        if (lane != 0) continue;
-        tile.outside = all;
-        tile.task = ring.tasks;
-        if (!kTurn) ring.tell(t);
-        ring.stream(tile, logits, 0, all, tiles);
-      }
+    // a chunk without the target, of a row whose exponentials take the short way
+    if (!far && static_cast<unsigned>(now.target - first) >= static_cast<unsigned>(packs * kN)) {
+#pragma unroll
+      for (int i = 0; i < kPacks; ++i)
+        if (i * kThreads + tid < packs) one(x[i], i * kThreads + tid, std::true_type());
+    } else {
+#pragma unroll 1
+      for (int i = 0; i < kPacks; ++i)
+        if (i * kThreads + tid < packs) one(pick(i), i * kThreads + tid, std::false_type());
     }
-    if (lane == 0) {
-      ring.end();
-      if (!ring.ok) {
-        give_up(kStatusTimeoutProducer);
-        ring.drain();
+  }
+};
+
+enum Mode : int { kPolicy, kSum, kTurn };  // all of the policy loss; a preference loss' softmaxes; its gradients
+
+struct LongArgs {
+  int ctas, chunks;  // CTAs that share a row, chunks of a CTA's part
+  Policy policy;
+  double* partial;
+  unsigned* arrived;
+  float* out;
+  Softmax* softmax;
+  float* logp;
+  const float* by;  // of the sequences
+};
+
+template <typename T, int kThreads, int kMode>
+__global__ void __launch_bounds__(kThreads, 1024 / kThreads)
+    long_rows_kernel(const T* __restrict__ logits, T* __restrict__ grad, const Rows r, const LongArgs a) {
+  constexpr int kN = Pack<T>::kN, kWarps = kThreads / 32, kChunk = kThreads * kPacks;
+  __shared__ Softmax part[kWarps], of_cta[2][8];
+  __shared__ Slope said;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int rank = a.ctas > 1 ? static_cast<int>(cluster_ctarank()) : 0;
+  const long long cluster = blockIdx.x / a.ctas, clusters = gridDim.x / a.ctas;
+  const float scale = kMode == kPolicy ? scale_of(a.policy.normalizer, a.policy.scale) : 0.f;
+  double sums[4] = {0.0, 0.0, 0.0, 0.0};
+  int turn = 0;
+  // The gradients begin with the rows read last, which are still in L2.
+  auto row_of = [&](long long i) { return kMode == kTurn ? r.rows - 1 - i : i; };
+  auto weight_of = [&](long long i) {
+    return i < r.rows && r.weights != nullptr ? r.weights[row_of(i)] : 1.f;
+  };
+  float next_w = weight_of(cluster);
+  for (long long i = cluster; i < r.rows; i += clusters) {
+    const float w = next_w;
+    next_w = weight_of(i + clusters);  // (asked for a row ahead)
+    const long long row = row_of(i), b = row / r.length, t = row - b * r.length;
+    const long long offset = b * r.stride_b + t * r.stride_t;
+    const T* x = logits + offset;
+    T* g = grad + offset;
+    // The row's part between 16-byte boundaries, and of that this CTA's.
+    const int off = static_cast<int>(reinterpret_cast<uintptr_t>(x) & 15) / static_cast<int>(sizeof(T));
+    const int head = off ? kN - off : 0, all = (r.vocab - head) / kN;
+    const int size = (all + a.ctas - 1) / a.ctas, from = size * rank < all ? size * rank : all;
+    const int packs = all - from < size ? all - from : size, first = head + from * kN;
+    // The value outside of the boundaries that the thread sees to, or -1.
+    int outside = -1;
+    if (rank == 0) outside = tid < head ? tid : (tid < r.vocab - all * kN ? all * kN + tid : -1);
+    if (w == 0.f) {
+      if (kMode != kSum && grad != nullptr) {
+        for (int k = tid; k < packs; k += kThreads)
+          *reinterpret_cast<uint4*>(g + first + k * kN) = make_uint4(0, 0, 0, 0);
+        if (outside >= 0) g[outside] = Pack<T>::back(0.f);
       }
+      continue;
     }
-  } else if (warp > kWarps) {  // ---- keeper ----
-    for (unsigned n = 0;; ++n) {
-      const int slot = n % kSlots;
-      const uint32_t parity = n / kSlots & 1;
-      if (!wait(&sh.told[slot], parity)) break;
-      const Task t = sh.task[slot];
-      if (t.kind == kEnd) break;
-      if (!wait(&sh.sums[slot], parity)) break;
-      const Softmax s = sh.all_parts(slot, t.warp, warps_of_row);
-      if (lane == 0) {
-        softmax[t.row] = s;
-        logp[t.row] = log_prob_of(t.x, s);
-        mbar_arrive(&sh.kept[slot]);
-      }
-      __syncwarp();
-    }
-    if (!ok) give_up(kStatusTimeoutEpilogue);
-  } else {  // ---- workers ----
-    Turn<PairShared> at = {warp, 0};
-    Softmax seen = {-INFINITY, 0.f};
-    while (wait(&sh.full[at.stage], at.round & 1)) {
-      const Tile t = sh.tile[at.stage];
-      if (t.kind == kEnd) break;
-      const int outside = outside_of<T>(t, r.vocab, lane);
-      if (kTurn) {
-        if (outside >= 0) turn_one(grad + t.offset, logits + t.offset, outside, t.now);
-        turn_tile<T>(grad + t.offset, sh.data[at.stage], t, t.now, lane);
+    Share<T, kThreads> mine;
+    mine.load(x + first, packs, tid);
+    // A row's few values: asked for behind its logits, needed when those are summed.
+    int target = -1;
+    float xt = NAN;
+    PolicyInputs in = {0.f, 0.f, 0.f};
+    Slope now = {0.f, 0.f, 0.f, -1};
+    if (kMode == kTurn || tid == 0) {
+      const long long at = r.targets[row];
+      target = at >= 0 && at < r.vocab ? static_cast<int>(at) : -1;
+      if (kMode == kTurn) {
+        const Softmax s = a.softmax[row];
+        const float by = w * a.by[b];
+        now = {s.most, by, -by / s.sum, target};
       } else {
-        if (outside >= 0) seen = one_value(logits[t.offset + outside]);
-        sum_tile<T>(seen, sh.data[at.stage], t.packs, lane);
-      }
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&sh.empty[at.stage]);
-      at.advance();
-      if (!kTurn && t.last) {
-        const Softmax s = join_row_lanes(seen);
-        if (lane == 0) {
-          sh.part[t.task % kSlots][warp] = s;
-          mbar_arrive(&sh.sums[t.task % kSlots]);
-        }
-        seen = {-INFINITY, 0.f};
+        if (kMode == kPolicy) in = policy_inputs(a.policy, row, b, t);
+        if (target >= 0) xt = Pack<T>::one(x[target]);
       }
     }
-    if (!ok) give_up(kStatusTimeoutEpilogue);
+    if (kMode != kTurn) {
+      Softmax s = {-INFINITY, 0.f};
+      if (outside >= 0) {
+        const float v = Pack<T>::one(x[outside]);
+        s = {v, v == -INFINITY ? 0.f : v * 0.f + 1.f};  // (NaN of +inf and NaN)
+      }
+      mine.add_to(s, packs);
+      for (int c = 1; c < a.chunks; ++c) {
+        mine.load(x + first + c * kChunk * kN, packs - c * kChunk, tid);
+        mine.add_to(s, packs - c * kChunk);
+      }
+      s = join_row_lanes<32>(s);
+      if (lane == 0) part[warp] = s;
+      __syncthreads();
+      if (warp == 0) {
+        s = join_row_lanes<32>(lane < kWarps ? part[lane] : Softmax{-INFINITY, 0.f});
+        if (a.ctas > 1 && lane < a.ctas)  // (two places in turn: a CTA may be at the next row already)
+          asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(
+                           mapa_shared(smem_u32(&of_cta[turn][rank]), lane)),
+                       "f"(s.most), "f"(s.sum)
+                       : "memory");
+      }
+      if (a.ctas > 1) {
+        __syncwarp();
+        cluster_sync_all();
+        if (warp == 0) s = join_row_lanes<32>(lane < a.ctas ? of_cta[turn][lane] : Softmax{-INFINITY, 0.f});
+        turn ^= 1;
+      }
+      if (tid == 0) {
+        const float logp = log_prob_of(xt, s);
+        if (kMode == kSum) {
+          if (rank == 0) {
+            a.softmax[row] = s;
+            a.logp[row] = logp;
+          }
+        } else {
+          const PolicyToken c = policy_token(a.policy, in, logp);
+          sums[0] += static_cast<double>(w) * c.loss;
+          sums[1] += static_cast<double>(w) * c.kl;
+          sums[2] += static_cast<double>(w) * c.clipped;
+          sums[3] += w;
+          const float by = w * c.slope * scale;
+          said = {s.most, by, -by / s.sum, target};
+        }
+      }
+      __syncthreads();  // (`part` is read, `said` is there; nobody writes it before all are past the next row's first)
+      if (kMode == kSum || grad == nullptr) continue;
+      now = said;
+      if (a.chunks > 1) mine.load(x + first, packs, tid);
+    }
+    if (outside >= 0) {
+      const float v = now.k * exp_from(Pack<T>::one(x[outside]), now.most);
+      g[outside] = Pack<T>::back(outside == now.target ? v + now.by : v);
+    }
+    mine.turn(g + first, packs < kChunk ? packs : kChunk, first, now, tid);
+    for (int c = 1; c < a.chunks; ++c) {
+      const int left = packs - c * kChunk, at = first + c * kChunk * kN;
+      mine.load(x + at, left, tid);
+      mine.turn(g + at, left < kChunk ? left : kChunk, at, now, tid);
+    }
+  }
+  __syncwarp();
+  if (a.ctas > 1) cluster_sync_all();  // no CTA ends while another may still write to it
+  if (kMode != kPolicy) return;
+  // Every cluster's sums, and behind the last cluster's those of all.
+  if (warp != 0 || rank != 0) return;
+  unsigned before = 0;
+  if (lane == 0) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) a.partial[cluster * 4 + k] = sums[k];
+    __threadfence();
+    before = atomicAdd(a.arrived, 1u) + 1;
+  }
+  if (__shfl_sync(0xffffffffu, before, 0) != clusters) return;
+  __threadfence();
+  const double whole =
+      a.policy.normalizer != nullptr ? 1.0 / static_cast<double>(*a.policy.normalizer) : a.policy.scale;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    double v = 0.0;
+    for (long long c = lane; c < clusters; c += 32) v += __ldcg(a.partial + c * 4 + k);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    if (lane == 0) a.out[k] = static_cast<float>(k < 2 ? v * whole : v);
   }
 }
 
@@ -1223,13 +851,8 @@ __global__ void __launch_bounds__(256)
 }
 
 // ---- host ----
-// Rows of these bytes go through the ring; shorter ones are a warp's each, and so are longer ones (a vocabulary
-// of 400,000 in 32 bits: more than eight CTAs hold), which no model here has.
-constexpr long long kRingRow = 4096, kRingRowMost = 1600 << 10;
-bool by_ring(long long vocab, int fp32) {
-  const long long bytes = vocab * (fp32 ? 4 : 2);
-  return bytes >= kRingRow && bytes <= kRingRowMost;
-}
+// Shorter rows are a warp's each.
+constexpr long long kLongRow = 4096;
 
 int check_rows(const char* what, const void* logits, int fp32, const void* grad, long long batch, int length,
                int vocab, long long stride_b, long long stride_t, const void* targets) {
@@ -1259,71 +882,56 @@ int launched(const char* what, int n) {
   return 0;
 }
 
-// Tiles of a CTA's part of a row, the same for all rows wherever their 16-byte boundaries lie (none is empty:
-// a part of n tiles has more than 512 (n - 1) times 16 bytes, or, for n = 1, 250).
-int tiles_of(long long vocab, int size, int ctas) {
-  const long long packs = (vocab * size / 16 + ctas - 1) / ctas;
-  return static_cast<int>((packs + kTilePacks - 1) / kTilePacks);
-}
-
-template <typename T>
-int launch_policy(const void* logits, void* grad, const Rows& r, const Policy& p, double* partial, unsigned* arrived,
-                  float* out, cudaStream_t st) {
-  // The smallest cluster whose CTAs' parts leave room for two more in the ring (the largest cluster's parts
-  // may be larger).
+template <typename T, int kThreads, int kMode>
+int launch_long(const char* what, const void* logits, void* grad, const Rows& r, LongArgs a, cudaStream_t st) {
+  auto kernel = long_rows_kernel<T, kThreads, kMode>;
+  const long long held = static_cast<long long>(kThreads) * kPacks * 16;  // bytes that a CTA holds
   const long long bytes = static_cast<long long>(r.vocab) * sizeof(T);
-  int ctas = 1;
-  while (ctas < 8 && (bytes + ctas - 1) / ctas > 8 * kTileBytes) ctas *= 2;
-  if (grad == nullptr) ctas = 1;  // (nothing has to stay)
-  const int tiles = tiles_of(r.vocab, sizeof(T), ctas);
-  auto kernel = policy_rows_kernel<T>;
-  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, sizeof(PolicyShared));
-  if (e != cudaSuccess) return set_error("policy_loss: %s", cudaGetErrorString(e));
+  a.ctas = 1;
+  while (a.ctas < 8 && held * a.ctas < bytes) a.ctas *= 2;
+  a.chunks = static_cast<int>(((bytes / 16 + a.ctas - 1) / a.ctas * 16 + held - 1) / held);
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(ctas));
-  cfg.blockDim = dim3(kPolicyThreads);
-  cfg.dynamicSmemBytes = sizeof(PolicyShared);
+  cfg.gridDim = dim3(static_cast<unsigned>(a.ctas));
+  cfg.blockDim = dim3(kThreads);
   cfg.stream = st;
   cudaLaunchAttribute attr;
   attr.id = cudaLaunchAttributeClusterDimension;
-  attr.val.clusterDim.x = ctas;
+  attr.val.clusterDim.x = a.ctas;
   attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
   cfg.attrs = &attr;
-  cfg.numAttrs = ctas > 1 ? 1 : 0;
+  cfg.numAttrs = a.ctas > 1 ? 1 : 0;
   // As many clusters as run at once: the rows are dealt out beforehand. (A cluster lies within a group of SMs,
   // whose size need not be a multiple of the cluster's.)
   static std::atomic<int> at_once[64][4];
-  int dev = 0, size = ctas == 1 ? 0 : ctas == 2 ? 1 : ctas == 4 ? 2 : 3;
-  cudaGetDevice(&dev);
+  int dev = 0, size = a.ctas == 1 ? 0 : a.ctas == 2 ? 1 : a.ctas == 4 ? 2 : 3;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return set_error("%s: %s", what, cudaGetErrorString(e));
   int cap = at_once[dev][size].load(std::memory_order_relaxed);
   if (cap == 0) {
-    cap = num_sms();
-    if (ctas > 1) {
+    if (a.ctas > 1) {
       e = cudaOccupancyMaxActiveClusters(&cap, kernel, &cfg);
-      if (e != cudaSuccess) return set_error("policy_loss: %s", cudaGetErrorString(e));
+    } else {
+      e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&cap, kernel, kThreads, 0);
+      cap *= num_sms();
     }
+    if (e != cudaSuccess) return set_error("%s: %s", what, cudaGetErrorString(e));
     if (cap < 1) cap = 1;
+    if (cap > kCtasPerSm * num_sms()) cap = kCtasPerSm * num_sms();
     at_once[dev][size].store(cap, std::memory_order_relaxed);
   }
-  cfg.gridDim = dim3(static_cast<unsigned>((r.rows < cap ? r.rows : cap) * ctas));
-  e = cudaLaunchKernelEx(&cfg, kernel, static_cast<const T*>(logits), static_cast<T*>(grad), r, p, ctas, tiles, partial,
-                         arrived, out, device_status_buffer());
-  if (e != cudaSuccess) return set_error("policy_loss: %s", cudaGetErrorString(e));
-  return launched("policy_loss", 1);
+  cfg.gridDim = dim3(static_cast<unsigned>((r.rows < cap ? r.rows : cap) * a.ctas));
+  e = cudaLaunchKernelEx(&cfg, kernel, static_cast<const T*>(logits), static_cast<T*>(grad), r, a);
+  if (e != cudaSuccess) return set_error("%s: %s", what, cudaGetErrorString(e));
+  return launched(what, 1);
 }
 
-template <typename T, bool kTurn>
-int launch_preference(const void* logits, void* grad, const Rows& r, Softmax* softmax, float* logp, const float* by,
-                      cudaStream_t st) {
-  auto kernel = preference_rows_kernel<T, kTurn>;
-  const cudaError_t e =
-      cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, sizeof(PairShared));
-  if (e != cudaSuccess) return set_error("preference_loss: %s", cudaGetErrorString(e));
-  const long long cap = static_cast<long long>(num_sms()) * 2;
-  kernel<<<static_cast<unsigned>(r.rows < cap ? r.rows : cap), kPairThreads, sizeof(PairShared), st>>>(
-      static_cast<const T*>(logits), static_cast<T*>(grad), r, tiles_of(r.vocab, sizeof(T), 1), softmax, logp, by,
-      device_status_buffer());
-  return launched("preference_loss", 1);
+// The smallest CTA that holds the row, so that short ones leave the SM room for many.
+template <typename T, int kMode>
+int launch_long(const char* what, const void* logits, void* grad, const Rows& r, const LongArgs& a, cudaStream_t st) {
+  const long long bytes = static_cast<long long>(r.vocab) * sizeof(T);
+  if (bytes <= 128 * kPacks * 16) return launch_long<T, 128, kMode>(what, logits, grad, r, a, st);
+  if (bytes <= 256 * kPacks * 16) return launch_long<T, 256, kMode>(what, logits, grad, r, a, st);
+  return launch_long<T, 512, kMode>(what, logits, grad, r, a, st);
 }
 
 constexpr size_t kHead = 16;  // bytes of scratch in front: the count of arrived CTAs
@@ -1334,7 +942,7 @@ constexpr size_t kHead = 16;  // bytes of scratch in front: the count of arrived
 using namespace t5x;
 
 T5X_API long long t5x_policy_loss_scratch_bytes() {
-  return static_cast<long long>(kHead) + 4ll * 8 * num_sms() * 4;
+  return static_cast<long long>(kHead) + 4ll * 8 * num_sms() * kCtasPerSm;  // (four sums of each CTA)
 }
 
 T5X_API int t5x_policy_loss(const void* logits, int fp32, void* grad, long long batch, int length, int vocab,
@@ -1356,10 +964,15 @@ T5X_API int t5x_policy_loss(const void* logits, int fp32, void* grad, long long 
                     static_cast<const float*>(advantages), adv_b, adv_t, 1.f - clip_low, 1.f + clip_high,
                     kl_weight, scale, static_cast<const float*>(normalizer)};
   float* o = static_cast<float*>(out);
-  if (by_ring(vocab, fp32))
-    return r.rows == 0 ? set_error("policy_loss: no rows")
-           : fp32      ? launch_policy<float>(logits, grad, r, p, partial, arrived, o, st)
-                       : launch_policy<__nv_bfloat16>(logits, grad, r, p, partial, arrived, o, st);
+  if (static_cast<long long>(vocab) * (fp32 ? 4 : 2) >= kLongRow && r.rows > 0) {
+    LongArgs a = {};
+    a.policy = p;
+    a.partial = partial;
+    a.arrived = arrived;
+    a.out = o;
+    return fp32 ? launch_long<float, kPolicy>("policy_loss", logits, grad, r, a, st)
+                : launch_long<__nv_bfloat16, kPolicy>("policy_loss", logits, grad, r, a, st);
+  }
   const unsigned grid = row_grid(r.rows);
   if (fp32)
     policy_short_rows_kernel<<<grid, kRowThreads, 0, st>>>(static_cast<const float*>(logits),
@@ -1423,23 +1036,27 @@ T5X_API int t5x_preference_loss(const void* logits, int fp32, void* grad, long l
   if (e != cudaSuccess) return set_error("preference_loss: memset: %s", cudaGetErrorString(e));
   auto go = [&](auto* x) {
     using T = std::remove_const_t<std::remove_pointer_t<decltype(x)>>;
-    const bool ring = by_ring(vocab, fp32);
+    const bool in_long = static_cast<long long>(vocab) * static_cast<int>(sizeof(T)) >= kLongRow;
+    LongArgs a = {};
+    a.softmax = softmax;
+    a.logp = logp;
+    a.by = by;
     const unsigned grid = row_grid(r.rows);
     int rc = 0;
-    if (ring)
-      rc = launch_preference<T, false>(x, nullptr, r, softmax, logp, nullptr, st);
+    if (in_long)
+      rc = launch_long<T, kSum>("preference_loss", x, nullptr, r, a, st);
     else
       preference_short_rows_kernel<T><<<grid, kRowThreads, 0, st>>>(x, r, softmax, logp);
     if (rc != 0) return rc;
     preference_pairs_kernel<<<static_cast<unsigned>(pairs), kRowThreads, 0, st>>>(
         logp, r, p, static_cast<float*>(scores), static_cast<float*>(margins), by, nullptr, pair_loss, arrived,
         static_cast<float*>(out));
-    if (grad == nullptr) return launched("preference_loss", 2 - ring);
-    if (ring)
-      rc = launch_preference<T, true>(x, grad, r, softmax, logp, by, st);
+    if (grad == nullptr) return launched("preference_loss", in_long ? 1 : 2);
+    if (in_long)
+      rc = launch_long<T, kTurn>("preference_loss", x, grad, r, a, st);
     else
       preference_short_gradient_kernel<T><<<grid, kRowThreads, 0, st>>>(x, static_cast<T*>(grad), r, softmax, by);
-    return rc != 0 ? rc : launched("preference_loss", ring ? 1 : 3);
+    return rc != 0 ? rc : launched("preference_loss", in_long ? 1 : 3);
   };
   return fp32 ? go(static_cast<const float*>(logits)) : go(static_cast<const __nv_bfloat16*>(logits));
 }
