@@ -575,19 +575,38 @@ struct Unpack<__nv_bfloat16> {
   }
 };
 
-// A thread's share of a chunk of a row.
+// A thread's share of a chunk of a row: 16 bytes number tid, tid + kThreads, ... of `packs` at p.
 template <typename T, int kThreads>
 struct Share {
   static constexpr int kN = Pack<T>::kN;
   uint4 x[kPacks];
 
-  // 16 bytes number tid, tid + kThreads, ... of `packs` at p
-  __device__ __forceinline__ void load(const T* p, int packs, int tid) {
+  // On its way to the thread's own places in shared memory, which no other thread reads or writes.
+  __device__ __forceinline__ static void ask(uint4* slots, const T* p, int packs, int tid) {
+    const uint32_t to = smem_u32(slots + tid);
 #pragma unroll
-    for (int i = 0; i < kPacks; ++i) {
-      const int at = i * kThreads + tid;
-      x[i] = at < packs ? reinterpret_cast<const uint4*>(p)[at] : Unpack<T>::nothing();
-    }
+    for (int i = 0; i < kPacks; ++i)
+      if (i * kThreads + tid < packs)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to + i * kThreads * 16),
+                     "l"(reinterpret_cast<const uint4*>(p) + i * kThreads + tid)
+                     : "memory");
+  }
+  // All that the thread has asked for is there.
+  __device__ __forceinline__ void take(const uint4* slots, int packs, int tid) {
+    asm volatile("cp.async.wait_all;" ::: "memory");
+#pragma unroll
+    for (int i = 0; i < kPacks; ++i)
+      x[i] = i * kThreads + tid < packs ? slots[i * kThreads + tid] : Unpack<T>::nothing();
+  }
+  // The value behind 16 bytes number `at`, by its thread.
+  __device__ __forceinline__ float value(int at) const {
+    const uint4 u = pick(at / kN / kThreads);
+    const uint32_t w = (at % kN) * sizeof(T) / 4 == 0   ? u.x
+                       : (at % kN) * sizeof(T) / 4 == 1 ? u.y
+                       : (at % kN) * sizeof(T) / 4 == 2 ? u.z
+                                                        : u.w;
+    if (sizeof(T) == 4) return __uint_as_float(w);
+    return __uint_as_float(at & 1 ? w & 0xffff0000u : w << 16);
   }
   __device__ __forceinline__ void add_to(Softmax& s, int packs) const {
     float m = s.most;
@@ -682,7 +701,7 @@ struct Share {
 enum Mode : int { kPolicy, kSum, kTurn };  // all of the policy loss; a preference loss' softmaxes; its gradients
 
 struct LongArgs {
-  int ctas, chunks;  // CTAs that share a row, chunks of a CTA's part
+  int shift, chunks;  // 1 << shift CTAs share a row; chunks of a CTA's part
   Policy policy;
   double* partial;
   unsigned* arrived;
@@ -692,96 +711,170 @@ struct LongArgs {
   const float* by;  // of the sequences
 };
 
+// Where row t of sequence b lies, and which of it is this CTA's.
+template <typename T>
+struct Part {
+  long long offset;
+  int first, packs;  // its first value, its number of 16 bytes
+  int outside;       // the value in front of the first 16-byte boundary or behind the last that a thread sees to; -1
+
+  __device__ __forceinline__ Part(const T* logits, const Rows& r, long long b, int t, int shift, int rank, int tid) {
+    constexpr int kN = Pack<T>::kN;
+    offset = b * r.stride_b + t * r.stride_t;
+    const int off = static_cast<int>(reinterpret_cast<uintptr_t>(logits + offset) & 15) / static_cast<int>(sizeof(T));
+    const int head = off ? kN - off : 0, all = (r.vocab - head) / kN;
+    const int size = (all + (1 << shift) - 1) >> shift, from = min(size * rank, all);
+    packs = min(all - from, size);
+    first = head + from * kN;
+    outside = -1;
+    if (rank == 0) outside = tid < head ? tid : (tid < r.vocab - all * kN ? all * kN + tid : -1);
+  }
+};
+
 template <typename T, int kThreads, int kMode>
 __global__ void __launch_bounds__(kThreads, 1024 / kThreads)
     long_rows_kernel(const T* __restrict__ logits, T* __restrict__ grad, const Rows r, const LongArgs a) {
   constexpr int kN = Pack<T>::kN, kWarps = kThreads / 32, kChunk = kThreads * kPacks;
-  __shared__ Softmax part[kWarps], of_cta[2][8];
+  extern __shared__ uint4 slots[];  // a chunk
+  __shared__ float4 part[kWarps], of_cta[2][8];  // softmax and target's logit (0 where it is not among the values)
   __shared__ Slope said;
+  using Chunk = Share<T, kThreads>;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int rank = a.ctas > 1 ? static_cast<int>(cluster_ctarank()) : 0;
-  const long long cluster = blockIdx.x / a.ctas, clusters = gridDim.x / a.ctas;
+  const int ctas = 1 << a.shift, rank = a.shift ? static_cast<int>(cluster_ctarank()) : 0;
+  const long long cluster = blockIdx.x >> a.shift, clusters = gridDim.x >> a.shift;
   const float scale = kMode == kPolicy ? scale_of(a.policy.normalizer, a.policy.scale) : 0.f;
   double sums[4] = {0.0, 0.0, 0.0, 0.0};
   int turn = 0;
-  // The gradients begin with the rows read last, which are still in L2.
+  // Row i, i + clusters, ... The gradients begin with the rows read last, which are still in L2.
   auto row_of = [&](long long i) { return kMode == kTurn ? r.rows - 1 - i : i; };
   auto weight_of = [&](long long i) {
-    return i < r.rows && r.weights != nullptr ? r.weights[row_of(i)] : 1.f;
+    return i < r.rows ? (r.weights != nullptr ? r.weights[row_of(i)] : 1.f) : 0.f;
   };
-  float next_w = weight_of(cluster);
+  long long b = row_of(cluster) / r.length;
+  int t = static_cast<int>(row_of(cluster) - b * r.length);
+  const long long step_b = clusters / r.length;
+  const int step_t = static_cast<int>(clusters - step_b * r.length);
+  // What a row needs is asked for a row ahead: its first chunk, its values outside of that, its weight.
+  struct Ahead {
+    float weight;
+    long long target;
+    Softmax softmax;
+    float by;
+  };
+  auto ahead_of = [&](long long i, long long b_of) {
+    Ahead n = {};
+    if (i < r.rows) {
+      n.target = r.targets[row_of(i)];
+      if (kMode == kTurn) {
+        n.softmax = a.softmax[row_of(i)];
+        n.by = a.by[b_of];
+      }
+    }
+    return n;
+  };
+  float w_next = weight_of(cluster), w_after = weight_of(cluster + clusters);
+  Ahead next = ahead_of(cluster, b);
+  if (w_next != 0.f) {
+    const Part<T> p(logits, r, b, t, a.shift, rank, tid);
+    Chunk::ask(slots, logits + p.offset + p.first, p.packs, tid);
+  }
   for (long long i = cluster; i < r.rows; i += clusters) {
-    const float w = next_w;
-    next_w = weight_of(i + clusters);  // (asked for a row ahead)
-    const long long row = row_of(i), b = row / r.length, t = row - b * r.length;
-    const long long offset = b * r.stride_b + t * r.stride_t;
-    const T* x = logits + offset;
-    T* g = grad + offset;
-    // The row's part between 16-byte boundaries, and of that this CTA's.
-    const int off = static_cast<int>(reinterpret_cast<uintptr_t>(x) & 15) / static_cast<int>(sizeof(T));
-    const int head = off ? kN - off : 0, all = (r.vocab - head) / kN;
-    const int size = (all + a.ctas - 1) / a.ctas, from = size * rank < all ? size * rank : all;
-    const int packs = all - from < size ? all - from : size, first = head + from * kN;
-    // The value outside of the boundaries that the thread sees to, or -1.
-    int outside = -1;
-    if (rank == 0) outside = tid < head ? tid : (tid < r.vocab - all * kN ? all * kN + tid : -1);
+    const float w = w_next;
+    w_next = w_after;
+    w_after = weight_of(i + 2 * clusters);
+    const long long row = row_of(i), b_now = b;
+    const int t_now = t;
+    if (kMode == kTurn) {
+      b -= step_b, t -= step_t;
+      if (t < 0) t += r.length, --b;
+    } else {
+      b += step_b, t += step_t;
+      if (t >= r.length) t -= r.length, ++b;
+    }
+    const Ahead now_of = next;
+    next = ahead_of(i + clusters, b);
+    auto ask_next = [&] {
+      if (w_next == 0.f) return;
+      const Part<T> p(logits, r, b, t, a.shift, rank, tid);
+      Chunk::ask(slots, logits + p.offset + p.first, p.packs, tid);
+    };
+    const Part<T> p(logits, r, b_now, t_now, a.shift, rank, tid);
+    const T* x = logits + p.offset;
+    T* g = grad + p.offset;
     if (w == 0.f) {
+      ask_next();
       if (kMode != kSum && grad != nullptr) {
-        for (int k = tid; k < packs; k += kThreads)
-          *reinterpret_cast<uint4*>(g + first + k * kN) = make_uint4(0, 0, 0, 0);
-        if (outside >= 0) g[outside] = Pack<T>::back(0.f);
+        for (int k = tid; k < p.packs; k += kThreads)
+          *reinterpret_cast<uint4*>(g + p.first + k * kN) = make_uint4(0, 0, 0, 0);
+        if (p.outside >= 0) g[p.outside] = Pack<T>::back(0.f);
       }
       continue;
     }
-    Share<T, kThreads> mine;
-    mine.load(x + first, packs, tid);
-    // A row's few values: asked for behind its logits, needed when those are summed.
-    int target = -1;
-    float xt = NAN;
-    PolicyInputs in = {0.f, 0.f, 0.f};
-    Slope now = {0.f, 0.f, 0.f, -1};
-    if (kMode == kTurn || tid == 0) {
-      const long long at = r.targets[row];
-      target = at >= 0 && at < r.vocab ? static_cast<int>(at) : -1;
-      if (kMode == kTurn) {
-        const Softmax s = a.softmax[row];
-        const float by = w * a.by[b];
-        now = {s.most, by, -by / s.sum, target};
-      } else {
-        if (kMode == kPolicy) in = policy_inputs(a.policy, row, b, t);
-        if (target >= 0) xt = Pack<T>::one(x[target]);
+    const int target = now_of.target >= 0 && now_of.target < r.vocab ? static_cast<int>(now_of.target) : -1;
+    float x_outside = 0.f;
+    if (p.outside >= 0) x_outside = Pack<T>::one(x[p.outside]);
+    auto ask = [&](int c) { Chunk::ask(slots, x + p.first + c * kChunk * kN, p.packs - c * kChunk, tid); };
+    Chunk mine;
+    Slope now;
+    if (kMode == kTurn) {
+      const float by = w * now_of.by;
+      now = {now_of.softmax.most, by, -by / now_of.softmax.sum, target};
+      for (int c = 0; c < a.chunks; ++c) {
+        const int left = p.packs - c * kChunk, at = p.first + c * kChunk * kN;
+        mine.take(slots, left, tid);
+        if (c + 1 < a.chunks)
+          ask(c + 1);
+        else
+          ask_next();
+        mine.turn(g + at, min(left, kChunk), at, now, tid);
       }
-    }
-    if (kMode != kTurn) {
+    } else {
+      PolicyInputs in = {0.f, 0.f, 0.f};
+      if (kMode == kPolicy && tid == 0) in = policy_inputs(a.policy, row, b_now, t_now);
       Softmax s = {-INFINITY, 0.f};
-      if (outside >= 0) {
-        const float v = Pack<T>::one(x[outside]);
-        s = {v, v == -INFINITY ? 0.f : v * 0.f + 1.f};  // (NaN of +inf and NaN)
+      float xt = 0.f;
+      for (int c = 0; c < a.chunks; ++c) {
+        const int left = p.packs - c * kChunk;
+        mine.take(slots, left, tid);
+        if (c + 1 < a.chunks)
+          ask(c + 1);
+        else if (kMode == kPolicy && grad != nullptr && c > 0)
+          ask(c - 1);
+        else
+          ask_next();
+        mine.add_to(s, left);
+        const int at = target - p.first - c * kChunk * kN;
+        if (target >= 0 && at >= 0 && at < min(left, kChunk) * kN && at / kN % kThreads == tid) xt = mine.value(at);
       }
-      mine.add_to(s, packs);
-      for (int c = 1; c < a.chunks; ++c) {
-        mine.load(x + first + c * kChunk * kN, packs - c * kChunk, tid);
-        mine.add_to(s, packs - c * kChunk);
+      if (p.outside >= 0) {
+        s = join_rows(s, {x_outside, x_outside == -INFINITY ? 0.f : x_outside * 0.f + 1.f});  // (NaN of +inf, NaN)
+        if (p.outside == target) xt = x_outside;
       }
-      s = join_row_lanes<32>(s);
-      if (lane == 0) part[warp] = s;
+      auto joined = [&](float4 v) {
+        const Softmax m = join_row_lanes<32>({v.x, v.y});
+        return make_float4(m.most, m.sum, warp_sum(v.z), 0.f);
+      };
+      const float4 none = make_float4(-INFINITY, 0.f, 0.f, 0.f);
+      float4 v = joined(make_float4(s.most, s.sum, xt, 0.f));
+      if (lane == 0) part[warp] = v;
       __syncthreads();
       if (warp == 0) {
-        s = join_row_lanes<32>(lane < kWarps ? part[lane] : Softmax{-INFINITY, 0.f});
-        if (a.ctas > 1 && lane < a.ctas)  // (two places in turn: a CTA may be at the next row already)
-          asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(
+        v = joined(lane < kWarps ? part[lane] : none);
+        if (a.shift && lane < ctas)  // (two places in turn: a CTA may be at the next row already)
+          asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(
                            mapa_shared(smem_u32(&of_cta[turn][rank]), lane)),
-                       "f"(s.most), "f"(s.sum)
+                       "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w)
                        : "memory");
-      }
-      if (a.ctas > 1) {
         __syncwarp();
+      }
+      if (a.shift) {
         cluster_sync_all();
-        if (warp == 0) s = join_row_lanes<32>(lane < a.ctas ? of_cta[turn][lane] : Softmax{-INFINITY, 0.f});
+        if (warp == 0) v = joined(lane < ctas ? of_cta[turn][lane] : none);
         turn ^= 1;
       }
       if (tid == 0) {
-        const float logp = log_prob_of(xt, s);
+        s = {v.x, v.y};
+        const float logp = log_prob_of(target >= 0 ? v.z : NAN, s);
         if (kMode == kSum) {
           if (rank == 0) {
             a.softmax[row] = s;
@@ -800,21 +893,25 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads)
       __syncthreads();  // (`part` is read, `said` is there; nobody writes it before all are past the next row's first)
       if (kMode == kSum || grad == nullptr) continue;
       now = said;
-      if (a.chunks > 1) mine.load(x + first, packs, tid);
+      for (int c = a.chunks - 1; c >= 0; --c) {  // (the last is still held)
+        const int left = p.packs - c * kChunk, at = p.first + c * kChunk * kN;
+        if (c + 1 < a.chunks) {
+          mine.take(slots, left, tid);
+          if (c > 0)
+            ask(c - 1);
+          else
+            ask_next();
+        }
+        mine.turn(g + at, min(left, kChunk), at, now, tid);
+      }
     }
-    if (outside >= 0) {
-      const float v = now.k * exp_from(Pack<T>::one(x[outside]), now.most);
-      g[outside] = Pack<T>::back(outside == now.target ? v + now.by : v);
-    }
-    mine.turn(g + first, packs < kChunk ? packs : kChunk, first, now, tid);
-    for (int c = 1; c < a.chunks; ++c) {
-      const int left = packs - c * kChunk, at = first + c * kChunk * kN;
-      mine.load(x + at, left, tid);
-      mine.turn(g + at, left < kChunk ? left : kChunk, at, now, tid);
+    if (kMode != kSum && p.outside >= 0) {
+      const float v = now.k * exp_from(x_outside, now.most);
+      g[p.outside] = Pack<T>::back(p.outside == now.target ? v + now.by : v);
     }
   }
   __syncwarp();
-  if (a.ctas > 1) cluster_sync_all();  // no CTA ends while another may still write to it
+  if (a.shift) cluster_sync_all();  // no CTA ends while another may still write to it
   if (kMode != kPolicy) return;
   // Every cluster's sums, and behind the last cluster's those of all.
   if (warp != 0 || rank != 0) return;
@@ -887,39 +984,41 @@ int launch_long(const char* what, const void* logits, void* grad, const Rows& r,
   auto kernel = long_rows_kernel<T, kThreads, kMode>;
   const long long held = static_cast<long long>(kThreads) * kPacks * 16;  // bytes that a CTA holds
   const long long bytes = static_cast<long long>(r.vocab) * sizeof(T);
-  a.ctas = 1;
-  while (a.ctas < 8 && held * a.ctas < bytes) a.ctas *= 2;
-  a.chunks = static_cast<int>(((bytes / 16 + a.ctas - 1) / a.ctas * 16 + held - 1) / held);
+  a.shift = 0;
+  while (a.shift < 3 && held << a.shift < bytes) ++a.shift;
+  const long long packs = ((bytes / 16 - 1) >> a.shift) + 1;  // of a CTA, at most
+  a.chunks = static_cast<int>((packs * 16 + held - 1) / held);
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(a.ctas));
+  cfg.gridDim = dim3(1u << a.shift);
   cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = held;
   cfg.stream = st;
   cudaLaunchAttribute attr;
   attr.id = cudaLaunchAttributeClusterDimension;
-  attr.val.clusterDim.x = a.ctas;
+  attr.val.clusterDim.x = 1u << a.shift;
   attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
   cfg.attrs = &attr;
-  cfg.numAttrs = a.ctas > 1 ? 1 : 0;
+  cfg.numAttrs = a.shift ? 1 : 0;
   // As many clusters as run at once: the rows are dealt out beforehand. (A cluster lies within a group of SMs,
   // whose size need not be a multiple of the cluster's.)
   static std::atomic<int> at_once[64][4];
-  int dev = 0, size = a.ctas == 1 ? 0 : a.ctas == 2 ? 1 : a.ctas == 4 ? 2 : 3;
+  int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return set_error("%s: %s", what, cudaGetErrorString(e));
-  int cap = at_once[dev][size].load(std::memory_order_relaxed);
+  int cap = at_once[dev][a.shift].load(std::memory_order_relaxed);
   if (cap == 0) {
-    if (a.ctas > 1) {
-      e = cudaOccupancyMaxActiveClusters(&cap, kernel, &cfg);
-    } else {
-      e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&cap, kernel, kThreads, 0);
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(held));
+    if (e == cudaSuccess && a.shift) e = cudaOccupancyMaxActiveClusters(&cap, kernel, &cfg);
+    if (e == cudaSuccess && !a.shift) {
+      e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&cap, kernel, kThreads, held);
       cap *= num_sms();
     }
     if (e != cudaSuccess) return set_error("%s: %s", what, cudaGetErrorString(e));
-    if (cap < 1) cap = 1;
+    if (cap < 1) return set_error("%s: the device has no room for the kernel", what);
     if (cap > kCtasPerSm * num_sms()) cap = kCtasPerSm * num_sms();
-    at_once[dev][size].store(cap, std::memory_order_relaxed);
+    at_once[dev][a.shift].store(cap, std::memory_order_relaxed);
   }
-  cfg.gridDim = dim3(static_cast<unsigned>((r.rows < cap ? r.rows : cap) * a.ctas));
+  cfg.gridDim = dim3(static_cast<unsigned>((r.rows < cap ? r.rows : cap) << a.shift));
   e = cudaLaunchKernelEx(&cfg, kernel, static_cast<const T*>(logits), static_cast<T*>(grad), r, a);
   if (e != cudaSuccess) return set_error("%s: %s", what, cudaGetErrorString(e));
   return launched(what, 1);
