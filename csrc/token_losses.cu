@@ -524,13 +524,10 @@ __device__ __forceinline__ Softmax join_rows(Softmax a, Softmax b) {
   const float m = fmaxf(a.most, b.most);
   return {m, a.sum * exp2_approx(shift(a.most, m)) + b.sum * exp2_approx(shift(b.most, m))};
 }
-// of `kLanes` lanes of a warp
-template <int kLanes>
-__device__ __forceinline__ Softmax join_row_lanes(Softmax s) {
-#pragma unroll
-  for (int o = kLanes / 2; o > 0; o >>= 1)
-    s = join_rows(s, {__shfl_xor_sync(0xffffffffu, s.most, o), __shfl_xor_sync(0xffffffffu, s.sum, o)});
-  return s;
+// of a warp's lanes
+__device__ __forceinline__ Softmax row_of_lanes(Softmax s) {
+  const float m = warp_max(s.most);
+  return {m, warp_sum(s.sum * exp2_approx(shift(s.most, m)))};
 }
 __device__ __forceinline__ float log_prob_of(float x, Softmax s) {
   if (s.most == -INFINITY) return NAN;
@@ -555,9 +552,14 @@ struct Unpack<float> {
     v[1] = pair_of(__uint_as_float(u.z), __uint_as_float(u.w));
   }
   __device__ static uint4 nothing() { return make_uint4(0xff800000u, 0xff800000u, 0xff800000u, 0xff800000u); }
-  __device__ static float most(uint4 u) {
-    return fmaxf(fmaxf(__uint_as_float(u.x), __uint_as_float(u.y)), fmaxf(__uint_as_float(u.z), __uint_as_float(u.w)));
+  // The largest value so far, in a form of the type's own.
+  using Most = float;
+  __device__ static Most least() { return -INFINITY; }
+  __device__ static void raise(Most& m, uint4 u) {
+    m = fmaxf(m, fmaxf(fmaxf(__uint_as_float(u.x), __uint_as_float(u.y)),
+                       fmaxf(__uint_as_float(u.z), __uint_as_float(u.w))));
   }
+  __device__ static float most(Most m) { return m; }
 };
 template <>
 struct Unpack<__nv_bfloat16> {
@@ -569,10 +571,12 @@ struct Unpack<__nv_bfloat16> {
   }
   __device__ static uint4 nothing() { return make_uint4(0xff80ff80u, 0xff80ff80u, 0xff80ff80u, 0xff80ff80u); }
   __device__ static __nv_bfloat162 as2(uint32_t u) { return *reinterpret_cast<__nv_bfloat162*>(&u); }
-  __device__ static float most(uint4 x) {
-    const __nv_bfloat162 m = __hmax2(__hmax2(as2(x.x), as2(x.y)), __hmax2(as2(x.z), as2(x.w)));
-    return fmaxf(__low2float(m), __high2float(m));
+  using Most = __nv_bfloat162;
+  __device__ static Most least() { return as2(0xff80ff80u); }
+  __device__ static void raise(Most& m, uint4 x) {
+    m = __hmax2(m, __hmax2(__hmax2(as2(x.x), as2(x.y)), __hmax2(as2(x.z), as2(x.w))));
   }
+  __device__ static float most(Most m) { return fmaxf(__low2float(m), __high2float(m)); }
 };
 
 // A thread's share of a chunk of a row: 16 bytes number tid, tid + kThreads, ... of `packs` at p.
@@ -584,19 +588,24 @@ struct Share {
   // On its way to the thread's own places in shared memory, which no other thread reads or writes.
   __device__ __forceinline__ static void ask(uint4* slots, const T* p, int packs, int tid) {
     const uint32_t to = smem_u32(slots + tid);
+    const uint4* from = reinterpret_cast<const uint4*>(p) + tid;
 #pragma unroll
     for (int i = 0; i < kPacks; ++i)
-      if (i * kThreads + tid < packs)
+      if ((i + 1) * kThreads <= packs || i * kThreads + tid < packs)
         asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to + i * kThreads * 16),
-                     "l"(reinterpret_cast<const uint4*>(p) + i * kThreads + tid)
+                     "l"(from + i * kThreads)
                      : "memory");
   }
   // All that the thread has asked for is there.
   __device__ __forceinline__ void take(const uint4* slots, int packs, int tid) {
     asm volatile("cp.async.wait_all;" ::: "memory");
 #pragma unroll
-    for (int i = 0; i < kPacks; ++i)
-      x[i] = i * kThreads + tid < packs ? slots[i * kThreads + tid] : Unpack<T>::nothing();
+    for (int i = 0; i < kPacks; ++i) {
+      if ((i + 1) * kThreads <= packs)  // (the same for all threads: no selects)
+        x[i] = slots[i * kThreads + tid];
+      else
+        x[i] = i * kThreads + tid < packs ? slots[i * kThreads + tid] : Unpack<T>::nothing();
+    }
   }
   // The value behind 16 bytes number `at`, by its thread.
   __device__ __forceinline__ float value(int at) const {
@@ -609,10 +618,10 @@ struct Share {
     return __uint_as_float(at & 1 ? w & 0xffff0000u : w << 16);
   }
   __device__ __forceinline__ void add_to(Softmax& s, int packs) const {
-    float m = s.most;
+    typename Unpack<T>::Most most = Unpack<T>::least();
 #pragma unroll
-    for (int i = 0; i < kPacks; ++i)
-      if (i * kThreads < packs) m = fmaxf(m, Unpack<T>::most(x[i]));
+    for (int i = 0; i < kPacks; ++i) Unpack<T>::raise(most, x[i]);
+    const float m = Unpack<T>::most(most);
     if (m > s.most) {
       s.sum *= exp2_approx(shift(s.most, m));
       s.most = m;
@@ -657,44 +666,46 @@ struct Share {
       if (k == i) v = x[k];
     return v;
   }
-  // Stores the gradient at g; `first`: the index in the row of the chunk's first value.
-  __device__ __forceinline__ void turn(T* g, int packs, int first, const Slope& now, int tid) const {
-    const uint64_t l2e = same2(kLog2e), off = same2(-__fmul_rn(now.most, kLog2e)), k2 = same2(now.k);
-    const bool far = huge(now.most);
-    auto one = [&](uint4 u, int at, auto plain) {
-      uint64_t v[Unpack<T>::kPairs];
-      Unpack<T>::pairs(u, v);
-      float y[kN];
-#pragma unroll
-      for (int j = 0; j < kN / 2; ++j) {
-        float a, b;
-        if (plain || !far) {
-          split(fma2(v[j], l2e, off), a, b);
-          a = exp2_approx(a), b = exp2_approx(b);
-        } else {
-          split(v[j], a, b);
-          a = exp_from(a, now.most), b = exp_from(b, now.most);
-        }
-        split(mul2(pair_of(a, b), k2), y[2 * j], y[2 * j + 1]);
-      }
-      if (!plain) {
-        const int off_target = now.target - (first + at * kN);
-#pragma unroll
-        for (int j = 0; j < kN; ++j)
-          if (off_target == j) y[j] += now.by;
-      }
-      Pack<T>::store(g + at * kN, y);
-    };
-    // a chunk without the target, of a row whose exponentials take the short way
-    if (!far && static_cast<unsigned>(now.target - first) >= static_cast<unsigned>(packs * kN)) {
+  // Stores the gradient at g; `at`: where the target lies, counted from the chunk's first value.
+  __device__ __forceinline__ void turn(T* g, int packs, int at, const Slope& now, int tid) const {
+    uint4* to = reinterpret_cast<uint4*>(g) + tid;
+    if (!huge(now.most)) {
+      const uint64_t l2e = same2(kLog2e), off = same2(-__fmul_rn(now.most, kLog2e)), k2 = same2(now.k);
 #pragma unroll
       for (int i = 0; i < kPacks; ++i)
-        if (i * kThreads + tid < packs) one(x[i], i * kThreads + tid, std::true_type());
+        if ((i + 1) * kThreads <= packs || i * kThreads + tid < packs) {
+          uint64_t v[Unpack<T>::kPairs];
+          Unpack<T>::pairs(x[i], v);
+          float y[kN];
+#pragma unroll
+          for (int j = 0; j < kN / 2; ++j) {
+            float a, b;
+            split(fma2(v[j], l2e, off), a, b);
+            split(mul2(pair_of(exp2_approx(a), exp2_approx(b)), k2), y[2 * j], y[2 * j + 1]);
+          }
+          Pack<T>::store(reinterpret_cast<T*>(to + i * kThreads), y);
+        }
     } else {
 #pragma unroll 1
       for (int i = 0; i < kPacks; ++i)
-        if (i * kThreads + tid < packs) one(pick(i), i * kThreads + tid, std::false_type());
+        if (i * kThreads + tid < packs) {
+          float y[kN];
+          uint64_t v[Unpack<T>::kPairs];
+          Unpack<T>::pairs(pick(i), v);
+#pragma unroll
+          for (int j = 0; j < kN / 2; ++j) {
+            split(v[j], y[2 * j], y[2 * j + 1]);
+            y[2 * j] = now.k * exp_from(y[2 * j], now.most);
+            y[2 * j + 1] = now.k * exp_from(y[2 * j + 1], now.most);
+          }
+          Pack<T>::store(reinterpret_cast<T*>(to + i * kThreads), y);
+        }
     }
+    if (holds(at, packs, tid)) g[at] = Pack<T>::back(now.k * exp_from(value(at), now.most) + now.by);
+  }
+  // Whether value number `at` of the chunk is this thread's.
+  __device__ __forceinline__ static bool holds(int at, int packs, int tid) {
+    return at >= 0 && at < min(packs, kThreads * kPacks) * kN && at / kN % kThreads == tid;
   }
 };
 
@@ -718,7 +729,7 @@ struct Part {
   int first, packs;  // its first value, its number of 16 bytes
   int outside;       // the value in front of the first 16-byte boundary or behind the last that a thread sees to; -1
 
-  __device__ __forceinline__ Part(const T* logits, const Rows& r, long long b, int t, int shift, int rank, int tid) {
+  __device__ __forceinline__ Part(const T* logits, const Rows& r, int b, int t, int shift, int rank, int tid) {
     constexpr int kN = Pack<T>::kN;
     offset = b * r.stride_b + t * r.stride_t;
     const int off = static_cast<int>(reinterpret_cast<uintptr_t>(logits + offset) & 15) / static_cast<int>(sizeof(T));
@@ -736,34 +747,32 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads)
     long_rows_kernel(const T* __restrict__ logits, T* __restrict__ grad, const Rows r, const LongArgs a) {
   constexpr int kN = Pack<T>::kN, kWarps = kThreads / 32, kChunk = kThreads * kPacks;
   extern __shared__ uint4 slots[];  // a chunk
-  __shared__ float4 part[kWarps], of_cta[2][8];  // softmax and target's logit (0 where it is not among the values)
+  __shared__ Softmax part[kWarps], of_cta[2][8];
+  __shared__ float of_target[2];
   __shared__ Slope said;
   using Chunk = Share<T, kThreads>;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int ctas = 1 << a.shift, rank = a.shift ? static_cast<int>(cluster_ctarank()) : 0;
-  const long long cluster = blockIdx.x >> a.shift, clusters = gridDim.x >> a.shift;
+  const int cluster = blockIdx.x >> a.shift, clusters = gridDim.x >> a.shift, rows = static_cast<int>(r.rows);
   const float scale = kMode == kPolicy ? scale_of(a.policy.normalizer, a.policy.scale) : 0.f;
   double sums[4] = {0.0, 0.0, 0.0, 0.0};
   int turn = 0;
   // Row i, i + clusters, ... The gradients begin with the rows read last, which are still in L2.
-  auto row_of = [&](long long i) { return kMode == kTurn ? r.rows - 1 - i : i; };
-  auto weight_of = [&](long long i) {
-    return i < r.rows ? (r.weights != nullptr ? r.weights[row_of(i)] : 1.f) : 0.f;
+  auto row_of = [&](int i) { return kMode == kTurn ? rows - 1 - i : i; };
+  auto weight_of = [&](int i) {
+    return i < rows ? (r.weights != nullptr ? r.weights[row_of(i)] : 1.f) : 0.f;
   };
-  long long b = row_of(cluster) / r.length;
-  int t = static_cast<int>(row_of(cluster) - b * r.length);
-  const long long step_b = clusters / r.length;
-  const int step_t = static_cast<int>(clusters - step_b * r.length);
+  int b = row_of(cluster) / r.length, t = row_of(cluster) % r.length;
+  const int step_b = clusters / r.length, step_t = clusters % r.length;
   // What a row needs is asked for a row ahead: its first chunk, its values outside of that, its weight.
   struct Ahead {
-    float weight;
     long long target;
     Softmax softmax;
     float by;
   };
-  auto ahead_of = [&](long long i, long long b_of) {
+  auto ahead_of = [&](int i, int b_of) {
     Ahead n = {};
-    if (i < r.rows) {
+    if (i < rows) {
       n.target = r.targets[row_of(i)];
       if (kMode == kTurn) {
         n.softmax = a.softmax[row_of(i)];
@@ -778,12 +787,12 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads)
     const Part<T> p(logits, r, b, t, a.shift, rank, tid);
     Chunk::ask(slots, logits + p.offset + p.first, p.packs, tid);
   }
-  for (long long i = cluster; i < r.rows; i += clusters) {
+  if (a.shift) cluster_sync_all();  // all CTAs have begun before any writes to another
+  for (int i = cluster; i < rows; i += clusters) {
     const float w = w_next;
     w_next = w_after;
     w_after = weight_of(i + 2 * clusters);
-    const long long row = row_of(i), b_now = b;
-    const int t_now = t;
+    const int row = row_of(i), b_now = b, t_now = t;
     if (kMode == kTurn) {
       b -= step_b, t -= step_t;
       if (t < 0) t += r.length, --b;
@@ -813,6 +822,17 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads)
     const int target = now_of.target >= 0 && now_of.target < r.vocab ? static_cast<int>(now_of.target) : -1;
     float x_outside = 0.f;
     if (p.outside >= 0) x_outside = Pack<T>::one(x[p.outside]);
+    // The target's logit, by the thread that holds it, for all of the cluster. (Two places in turn here and with
+    // the parts' softmaxes: a CTA may be at the next row already.)
+    auto tell_target = [&](float v) {
+      if (a.shift == 0) {
+        of_target[turn] = v;
+        return;
+      }
+      for (int k = 0; k < ctas; ++k)
+        asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(mapa_shared(smem_u32(&of_target[turn]), k)), "f"(v)
+                     : "memory");
+    };
     auto ask = [&](int c) { Chunk::ask(slots, x + p.first + c * kChunk * kN, p.packs - c * kChunk, tid); };
     Chunk mine;
     Slope now;
@@ -826,13 +846,12 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads)
           ask(c + 1);
         else
           ask_next();
-        mine.turn(g + at, min(left, kChunk), at, now, tid);
+        mine.turn(g + at, left, now.target - at, now, tid);
       }
     } else {
       PolicyInputs in = {0.f, 0.f, 0.f};
       if (kMode == kPolicy && tid == 0) in = policy_inputs(a.policy, row, b_now, t_now);
       Softmax s = {-INFINITY, 0.f};
-      float xt = 0.f;
       for (int c = 0; c < a.chunks; ++c) {
         const int left = p.packs - c * kChunk;
         mine.take(slots, left, tid);
@@ -843,38 +862,31 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads)
         else
           ask_next();
         mine.add_to(s, left);
-        const int at = target - p.first - c * kChunk * kN;
-        if (target >= 0 && at >= 0 && at < min(left, kChunk) * kN && at / kN % kThreads == tid) xt = mine.value(at);
+        const int at = target - (p.first + c * kChunk * kN);
+        if (Chunk::holds(at, left, tid)) tell_target(mine.value(at));
       }
       if (p.outside >= 0) {
         s = join_rows(s, {x_outside, x_outside == -INFINITY ? 0.f : x_outside * 0.f + 1.f});  // (NaN of +inf, NaN)
-        if (p.outside == target) xt = x_outside;
+        if (p.outside == target) tell_target(x_outside);
       }
-      auto joined = [&](float4 v) {
-        const Softmax m = join_row_lanes<32>({v.x, v.y});
-        return make_float4(m.most, m.sum, warp_sum(v.z), 0.f);
-      };
-      const float4 none = make_float4(-INFINITY, 0.f, 0.f, 0.f);
-      float4 v = joined(make_float4(s.most, s.sum, xt, 0.f));
-      if (lane == 0) part[warp] = v;
+      s = row_of_lanes(s);
+      if (lane == 0) part[warp] = s;
       __syncthreads();
       if (warp == 0) {
-        v = joined(lane < kWarps ? part[lane] : none);
-        if (a.shift && lane < ctas)  // (two places in turn: a CTA may be at the next row already)
-          asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(
+        s = row_of_lanes(lane < kWarps ? part[lane] : Softmax{-INFINITY, 0.f});
+        if (a.shift && lane < ctas)
+          asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(
                            mapa_shared(smem_u32(&of_cta[turn][rank]), lane)),
-                       "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w)
+                       "f"(s.most), "f"(s.sum)
                        : "memory");
         __syncwarp();
       }
       if (a.shift) {
         cluster_sync_all();
-        if (warp == 0) v = joined(lane < ctas ? of_cta[turn][lane] : none);
-        turn ^= 1;
+        if (warp == 0) s = row_of_lanes(lane < ctas ? of_cta[turn][lane] : Softmax{-INFINITY, 0.f});
       }
       if (tid == 0) {
-        s = {v.x, v.y};
-        const float logp = log_prob_of(target >= 0 ? v.z : NAN, s);
+        const float logp = log_prob_of(target >= 0 ? of_target[turn] : NAN, s);
         if (kMode == kSum) {
           if (rank == 0) {
             a.softmax[row] = s;
@@ -891,8 +903,10 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads)
         }
       }
       __syncthreads();  // (`part` is read, `said` is there; nobody writes it before all are past the next row's first)
+      turn ^= 1;
       if (kMode == kSum || grad == nullptr) continue;
       now = said;
+#pragma unroll 1
       for (int c = a.chunks - 1; c >= 0; --c) {  // (the last is still held)
         const int left = p.packs - c * kChunk, at = p.first + c * kChunk * kN;
         if (c + 1 < a.chunks) {
@@ -902,7 +916,7 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads)
           else
             ask_next();
         }
-        mine.turn(g + at, min(left, kChunk), at, now, tid);
+        mine.turn(g + at, left, now.target - at, now, tid);
       }
     }
     if (kMode != kSum && p.outside >= 0) {
@@ -929,7 +943,7 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads)
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
     double v = 0.0;
-    for (long long c = lane; c < clusters; c += 32) v += __ldcg(a.partial + c * 4 + k);
+    for (int c = lane; c < clusters; c += 32) v += __ldcg(a.partial + c * 4 + k);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
     if (lane == 0) a.out[k] = static_cast<float>(k < 2 ? v * whole : v);
@@ -981,6 +995,7 @@ int launched(const char* what, int n) {
 
 template <typename T, int kThreads, int kMode>
 int launch_long(const char* what, const void* logits, void* grad, const Rows& r, LongArgs a, cudaStream_t st) {
+  if (r.rows > (1 << 30)) return set_error("%s: too many rows", what);
   auto kernel = long_rows_kernel<T, kThreads, kMode>;
   const long long held = static_cast<long long>(kThreads) * kPacks * 16;  // bytes that a CTA holds
   const long long bytes = static_cast<long long>(r.vocab) * sizeof(T);
