@@ -473,38 +473,13 @@ __global__ void __launch_bounds__(kRowThreads)
 
 // ---- long rows ----
 // A CTA takes a row, or its part of a row that a cluster of CTAs shares, into registers: kPacks times 16 bytes
-// a thread, all loads in flight at once, while the SM's other CTAs are at other places of their rows. The
-// row's softmax and its gradient are both made from there, so that logits are read once. Larger rows than
-// eight CTAs hold go by in chunks, which are read a second time for the gradient.
+// a thread. The row's softmax and its gradient are both made from there, so that logits are read once, and the
+// next row is on its way into shared memory meanwhile. Larger rows than eight CTAs hold go by in chunks, which
+// are read a second time for the gradient.
 //
-// What bounds it: memory (read once, written once); the exponentials take 0.4 of its time for bf16 logits.
+// What bounds it: memory, and close behind that the instructions. So one thread finds out about the rows, a
+// few of them ahead, and leaves that for all in shared memory.
 constexpr int kPacks = 8;
-
-// Two values at once where the arithmetic has pairs.
-__device__ __forceinline__ uint64_t pair_of(float a, float b) {
-  uint64_t d;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(a), "f"(b));
-  return d;
-}
-__device__ __forceinline__ void split(uint64_t d, float& a, float& b) {
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(d));
-}
-__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
-  uint64_t d;
-  asm("fma.rn.ftz.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
-  return d;
-}
-__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
-  uint64_t d;
-  asm("add.rn.ftz.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-  return d;
-}
-__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
-  uint64_t d;
-  asm("mul.rn.ftz.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-  return d;
-}
-__device__ __forceinline__ uint64_t same2(float a) { return pair_of(a, a); }
 
 // An exponential exp(x - most) is exp2(x log2 e - ref) here, a fused product and difference, with ref =
 // most log2 e as rounded: the same factor for the sum, the target and the gradient. Where a largest logit's
@@ -541,15 +516,13 @@ struct Slope {
   int target;  // -1: outside of the vocabulary
 };
 
-// 16 bytes of logits as pairs.
+// 16 bytes of logits.
 template <typename T>
 struct Unpack;
 template <>
 struct Unpack<float> {
-  static constexpr int kPairs = 2;
-  __device__ static void pairs(uint4 u, uint64_t* v) {
-    v[0] = pair_of(__uint_as_float(u.x), __uint_as_float(u.y));
-    v[1] = pair_of(__uint_as_float(u.z), __uint_as_float(u.w));
+  __device__ static void floats(uint4 u, float* v) {
+    v[0] = __uint_as_float(u.x), v[1] = __uint_as_float(u.y), v[2] = __uint_as_float(u.z), v[3] = __uint_as_float(u.w);
   }
   __device__ static uint4 nothing() { return make_uint4(0xff800000u, 0xff800000u, 0xff800000u, 0xff800000u); }
   // The largest value so far, in a form of the type's own.
@@ -563,11 +536,13 @@ struct Unpack<float> {
 };
 template <>
 struct Unpack<__nv_bfloat16> {
-  static constexpr int kPairs = 4;
-  __device__ static void pairs(uint4 x, uint64_t* v) {
+  __device__ static void floats(uint4 x, float* v) {
     const uint32_t u[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = pair_of(__uint_as_float(u[i] << 16), __uint_as_float(u[i] & 0xffff0000u));
+    for (int i = 0; i < 4; ++i) {
+      v[2 * i] = __uint_as_float(u[i] << 16);
+      v[2 * i + 1] = __uint_as_float(u[i] & 0xffff0000u);
+    }
   }
   __device__ static uint4 nothing() { return make_uint4(0xff80ff80u, 0xff80ff80u, 0xff80ff80u, 0xff80ff80u); }
   __device__ static __nv_bfloat162 as2(uint32_t u) { return *reinterpret_cast<__nv_bfloat162*>(&u); }
@@ -578,6 +553,15 @@ struct Unpack<__nv_bfloat16> {
   }
   __device__ static float most(Most m) { return fmaxf(__low2float(m), __high2float(m)); }
 };
+
+template <int kBytes>
+__device__ __forceinline__ void fetch(uint32_t to, const void* from) {
+  if (kBytes == 16)
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
+  else
+    asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(to), "l"(from), "n"(kBytes) : "memory");
+}
+__device__ __forceinline__ void fetched() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 
 // A thread's share of a chunk of a row: 16 bytes number tid, tid + kThreads, ... of `packs` at p.
 template <typename T, int kThreads>
@@ -592,13 +576,11 @@ struct Share {
 #pragma unroll
     for (int i = 0; i < kPacks; ++i)
       if ((i + 1) * kThreads <= packs || i * kThreads + tid < packs)
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to + i * kThreads * 16),
-                     "l"(from + i * kThreads)
-                     : "memory");
+        fetch<16>(to + i * kThreads * 16, from + i * kThreads);
   }
   // All that the thread has asked for is there.
   __device__ __forceinline__ void take(const uint4* slots, int packs, int tid) {
-    asm volatile("cp.async.wait_all;" ::: "memory");
+    fetched();
 #pragma unroll
     for (int i = 0; i < kPacks; ++i) {
       if ((i + 1) * kThreads <= packs)  // (the same for all threads: no selects)
@@ -626,37 +608,27 @@ struct Share {
       s.sum *= exp2_approx(shift(s.most, m));
       s.most = m;
     }
-    uint64_t t[2] = {same2(0.f), same2(0.f)};
+    float t[4] = {0.f, 0.f, 0.f, 0.f};
     if (!huge(s.most)) {
-      const uint64_t l2e = same2(kLog2e), off = same2(-__fmul_rn(s.most, kLog2e));
+      const float off = -__fmul_rn(s.most, kLog2e);
 #pragma unroll
       for (int i = 0; i < kPacks; ++i)
         if (i * kThreads < packs) {
-          uint64_t v[Unpack<T>::kPairs];
-          Unpack<T>::pairs(x[i], v);
+          float v[kN];
+          Unpack<T>::floats(x[i], v);
 #pragma unroll
-          for (int j = 0; j < Unpack<T>::kPairs; ++j) {
-            float a, b;
-            split(fma2(v[j], l2e, off), a, b);
-            t[j & 1] = add2(t[j & 1], pair_of(exp2_approx(a), exp2_approx(b)));
-          }
+          for (int j = 0; j < kN; ++j) t[j % 4] += exp2_approx(fmaf(v[j], kLog2e, off));
         }
     } else {
 #pragma unroll 1
       for (int i = 0; i < kPacks; ++i) {
-        uint64_t v[Unpack<T>::kPairs];
-        Unpack<T>::pairs(pick(i), v);
+        float v[kN];
+        Unpack<T>::floats(pick(i), v);
 #pragma unroll
-        for (int j = 0; j < Unpack<T>::kPairs; ++j) {
-          float a, b;
-          split(v[j], a, b);
-          t[0] = add2(t[0], pair_of(exp_from(a, s.most), exp_from(b, s.most)));
-        }
+        for (int j = 0; j < kN; ++j) t[j % 4] += exp_from(v[j], s.most);
       }
     }
-    float a, b;
-    split(add2(t[0], t[1]), a, b);
-    s.sum += a + b;
+    s.sum += (t[0] + t[1]) + (t[2] + t[3]);
   }
   // x[i] for an i that the compiler does not know, without the array leaving the registers
   __device__ __forceinline__ uint4 pick(int i) const {
@@ -670,19 +642,14 @@ struct Share {
   __device__ __forceinline__ void turn(T* g, int packs, int at, const Slope& now, int tid) const {
     uint4* to = reinterpret_cast<uint4*>(g) + tid;
     if (!huge(now.most)) {
-      const uint64_t l2e = same2(kLog2e), off = same2(-__fmul_rn(now.most, kLog2e)), k2 = same2(now.k);
+      const float off = -__fmul_rn(now.most, kLog2e);
 #pragma unroll
       for (int i = 0; i < kPacks; ++i)
         if ((i + 1) * kThreads <= packs || i * kThreads + tid < packs) {
-          uint64_t v[Unpack<T>::kPairs];
-          Unpack<T>::pairs(x[i], v);
           float y[kN];
+          Unpack<T>::floats(x[i], y);
 #pragma unroll
-          for (int j = 0; j < kN / 2; ++j) {
-            float a, b;
-            split(fma2(v[j], l2e, off), a, b);
-            split(mul2(pair_of(exp2_approx(a), exp2_approx(b)), k2), y[2 * j], y[2 * j + 1]);
-          }
+          for (int j = 0; j < kN; ++j) y[j] = now.k * exp2_approx(fmaf(y[j], kLog2e, off));
           Pack<T>::store(reinterpret_cast<T*>(to + i * kThreads), y);
         }
     } else {
@@ -690,14 +657,9 @@ struct Share {
       for (int i = 0; i < kPacks; ++i)
         if (i * kThreads + tid < packs) {
           float y[kN];
-          uint64_t v[Unpack<T>::kPairs];
-          Unpack<T>::pairs(pick(i), v);
+          Unpack<T>::floats(pick(i), y);
 #pragma unroll
-          for (int j = 0; j < kN / 2; ++j) {
-            split(v[j], y[2 * j], y[2 * j + 1]);
-            y[2 * j] = now.k * exp_from(y[2 * j], now.most);
-            y[2 * j + 1] = now.k * exp_from(y[2 * j + 1], now.most);
-          }
+          for (int j = 0; j < kN; ++j) y[j] = now.k * exp_from(y[j], now.most);
           Pack<T>::store(reinterpret_cast<T*>(to + i * kThreads), y);
         }
     }
@@ -722,24 +684,14 @@ struct LongArgs {
   const float* by;  // of the sequences
 };
 
-// Where row t of sequence b lies, and which of it is this CTA's.
-template <typename T>
-struct Part {
-  long long offset;
-  int first, packs;  // its first value, its number of 16 bytes
-  int outside;       // the value in front of the first 16-byte boundary or behind the last that a thread sees to; -1
-
-  __device__ __forceinline__ Part(const T* logits, const Rows& r, int b, int t, int shift, int rank, int tid) {
-    constexpr int kN = Pack<T>::kN;
-    offset = b * r.stride_b + t * r.stride_t;
-    const int off = static_cast<int>(reinterpret_cast<uintptr_t>(logits + offset) & 15) / static_cast<int>(sizeof(T));
-    const int head = off ? kN - off : 0, all = (r.vocab - head) / kN;
-    const int size = (all + (1 << shift) - 1) >> shift, from = min(size * rank, all);
-    packs = min(all - from, size);
-    first = head + from * kN;
-    outside = -1;
-    if (rank == 0) outside = tid < head ? tid : (tid < r.vocab - all * kN ? all * kN + tid : -1);
-  }
+// What there is to know of a row.
+struct alignas(16) RowFacts {
+  long long offset;   // of its first value
+  int first, packs;   // the CTA's part: its first value, its number of 16 bytes
+  long long target;
+  float weight;
+  int row;
+  float more[4];  // policy: old score, reference score, advantage; gradients: softmax, slope of the sequence
 };
 
 template <typename T, int kThreads, int kMode>
@@ -747,6 +699,7 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads)
     long_rows_kernel(const T* __restrict__ logits, T* __restrict__ grad, const Rows r, const LongArgs a) {
   constexpr int kN = Pack<T>::kN, kWarps = kThreads / 32, kChunk = kThreads * kPacks;
   extern __shared__ uint4 slots[];  // a chunk
+  __shared__ RowFacts facts[4];
   __shared__ Softmax part[kWarps], of_cta[2][8];
   __shared__ float of_target[2];
   __shared__ Slope said;
@@ -756,72 +709,91 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads)
   const int cluster = blockIdx.x >> a.shift, clusters = gridDim.x >> a.shift, rows = static_cast<int>(r.rows);
   const float scale = kMode == kPolicy ? scale_of(a.policy.normalizer, a.policy.scale) : 0.f;
   double sums[4] = {0.0, 0.0, 0.0, 0.0};
-  int turn = 0;
-  // Row i, i + clusters, ... The gradients begin with the rows read last, which are still in L2.
-  auto row_of = [&](int i) { return kMode == kTurn ? rows - 1 - i : i; };
-  auto weight_of = [&](int i) {
-    return i < rows ? (r.weights != nullptr ? r.weights[row_of(i)] : 1.f) : 0.f;
-  };
-  int b = row_of(cluster) / r.length, t = row_of(cluster) % r.length;
-  const int step_b = clusters / r.length, step_t = clusters % r.length;
-  // What a row needs is asked for a row ahead: its first chunk, its values outside of that, its weight.
-  struct Ahead {
-    long long target;
-    Softmax softmax;
-    float by;
-  };
-  auto ahead_of = [&](int i, int b_of) {
-    Ahead n = {};
-    if (i < rows) {
-      n.target = r.targets[row_of(i)];
-      if (kMode == kTurn) {
-        n.softmax = a.softmax[row_of(i)];
-        n.by = a.by[b_of];
-      }
+
+  // The cluster's rows are number cluster, cluster + clusters, ... The gradients begin with the rows read last,
+  // which are still in L2. The facts of row k + 3 are asked for when row k has been taken, are there when row
+  // k + 1 is, and are read, behind a barrier, when row k + 3 is asked for.
+  const bool clerk = tid == kThreads - 32;
+  const int mine_of_all = (rows - cluster + clusters - 1) / clusters;
+  int ahead = cluster, described = 0;
+  int b = (kMode == kTurn ? rows - 1 - ahead : ahead) / r.length;
+  int t = (kMode == kTurn ? rows - 1 - ahead : ahead) - b * r.length;
+  const int step_b = clusters / r.length, step_t = clusters - step_b * r.length;
+  auto describe = [&] {  // (the clerk's)
+    RowFacts& f = facts[described++ & 3];
+    const int row = kMode == kTurn ? rows - 1 - ahead : ahead;
+    if (ahead >= rows) {
+      f.weight = 0.f;
+      return;
     }
-    return n;
-  };
-  float w_next = weight_of(cluster), w_after = weight_of(cluster + clusters);
-  Ahead next = ahead_of(cluster, b);
-  if (w_next != 0.f) {
-    const Part<T> p(logits, r, b, t, a.shift, rank, tid);
-    Chunk::ask(slots, logits + p.offset + p.first, p.packs, tid);
-  }
-  if (a.shift) cluster_sync_all();  // all CTAs have begun before any writes to another
-  for (int i = cluster; i < rows; i += clusters) {
-    const float w = w_next;
-    w_next = w_after;
-    w_after = weight_of(i + 2 * clusters);
-    const int row = row_of(i), b_now = b, t_now = t;
+    const long long offset = b * r.stride_b + t * r.stride_t;
+    // the row's part between 16-byte boundaries, and of that this CTA's
+    const int off = static_cast<int>(reinterpret_cast<uintptr_t>(logits + offset) & 15) / static_cast<int>(sizeof(T));
+    const int head = off ? kN - off : 0, all = (r.vocab - head) / kN;
+    const int size = (all + ctas - 1) >> a.shift, from = min(size * rank, all);
+    f.offset = offset;
+    f.first = head + from * kN;
+    f.packs = min(all - from, size);
+    f.row = row;
+    fetch<8>(smem_u32(&f.target), r.targets + row);
+    if (r.weights != nullptr)
+      fetch<4>(smem_u32(&f.weight), r.weights + row);
+    else
+      f.weight = 1.f;
     if (kMode == kTurn) {
+      fetch<8>(smem_u32(f.more), a.softmax + row);
+      fetch<4>(smem_u32(f.more + 2), a.by + b);
       b -= step_b, t -= step_t;
       if (t < 0) t += r.length, --b;
     } else {
+      if (kMode == kPolicy) {
+        fetch<4>(smem_u32(f.more), a.policy.old + row);
+        if (a.policy.ref != nullptr) fetch<4>(smem_u32(f.more + 1), a.policy.ref + row);
+        fetch<4>(smem_u32(f.more + 2), a.policy.advantages + b * a.policy.adv_b + t * a.policy.adv_t);
+      }
       b += step_b, t += step_t;
       if (t >= r.length) t -= r.length, ++b;
     }
-    const Ahead now_of = next;
-    next = ahead_of(i + clusters, b);
-    auto ask_next = [&] {
-      if (w_next == 0.f) return;
-      const Part<T> p(logits, r, b, t, a.shift, rank, tid);
-      Chunk::ask(slots, logits + p.offset + p.first, p.packs, tid);
-    };
-    const Part<T> p(logits, r, b_now, t_now, a.shift, rank, tid);
-    const T* x = logits + p.offset;
-    T* g = grad + p.offset;
+    ahead += clusters;
+  };
+  if (clerk) {
+    describe(), describe(), describe();
+    fetched();
+  }
+  __syncthreads();
+  if (a.shift) cluster_sync_all();  // all CTAs have begun before any writes to another
+  auto ask_row = [&](const RowFacts& f) {
+    if (f.weight != 0.f) Chunk::ask(slots, logits + f.offset + f.first, f.packs, tid);
+  };
+  ask_row(facts[0]);
+  for (int k = 0; k < mine_of_all; ++k) {
+    const RowFacts& f = facts[k & 3];
+    const float w = f.weight;
+    const long long offset = f.offset;
+    const int first = f.first, packs = f.packs, turn = k & 1;
+    const T* x = logits + offset;
+    T* g = grad + offset;
+    // The value in front of the first 16-byte boundary or behind the last that the thread sees to, or -1.
+    int outside = -1;
+    if (warp == 0 && rank == 0) {
+      const int rest = first + (r.vocab - first) / kN * kN;
+      outside = tid < first ? tid : (tid - first < r.vocab - rest ? rest + tid - first : -1);
+    }
     if (w == 0.f) {
-      ask_next();
+      fetched();  // (the clerk's)
+      ask_row(facts[(k + 1) & 3]);
+      if (clerk) describe();
       if (kMode != kSum && grad != nullptr) {
-        for (int k = tid; k < p.packs; k += kThreads)
-          *reinterpret_cast<uint4*>(g + p.first + k * kN) = make_uint4(0, 0, 0, 0);
-        if (p.outside >= 0) g[p.outside] = Pack<T>::back(0.f);
+        for (int i = tid; i < packs; i += kThreads)
+          *reinterpret_cast<uint4*>(g + first + i * kN) = make_uint4(0, 0, 0, 0);
+        if (outside >= 0) g[outside] = Pack<T>::back(0.f);
       }
+      __syncthreads();
       continue;
     }
-    const int target = now_of.target >= 0 && now_of.target < r.vocab ? static_cast<int>(now_of.target) : -1;
+    const int target = f.target >= 0 && f.target < r.vocab ? static_cast<int>(f.target) : -1;
     float x_outside = 0.f;
-    if (p.outside >= 0) x_outside = Pack<T>::one(x[p.outside]);
+    if (outside >= 0) x_outside = Pack<T>::one(x[outside]);
     // The target's logit, by the thread that holds it, for all of the cluster. (Two places in turn here and with
     // the parts' softmaxes: a CTA may be at the next row already.)
     auto tell_target = [&](float v) {
@@ -829,46 +801,49 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads)
         of_target[turn] = v;
         return;
       }
-      for (int k = 0; k < ctas; ++k)
-        asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(mapa_shared(smem_u32(&of_target[turn]), k)), "f"(v)
+      for (int c = 0; c < ctas; ++c)
+        asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(mapa_shared(smem_u32(&of_target[turn]), c)), "f"(v)
                      : "memory");
     };
-    auto ask = [&](int c) { Chunk::ask(slots, x + p.first + c * kChunk * kN, p.packs - c * kChunk, tid); };
+    auto ask = [&](int c) { Chunk::ask(slots, x + first + c * kChunk * kN, packs - c * kChunk, tid); };
     Chunk mine;
     Slope now;
     if (kMode == kTurn) {
-      const float by = w * now_of.by;
-      now = {now_of.softmax.most, by, -by / now_of.softmax.sum, target};
+      const float by = w * f.more[2];
+      now = {f.more[0], by, -by / f.more[1], target};
       for (int c = 0; c < a.chunks; ++c) {
-        const int left = p.packs - c * kChunk, at = p.first + c * kChunk * kN;
+        const int left = packs - c * kChunk, at = first + c * kChunk * kN;
         mine.take(slots, left, tid);
-        if (c + 1 < a.chunks)
+        if (c + 1 < a.chunks) {
           ask(c + 1);
-        else
-          ask_next();
+        } else {
+          ask_row(facts[(k + 1) & 3]);
+          if (clerk) describe();
+          __syncthreads();
+        }
         mine.turn(g + at, left, now.target - at, now, tid);
       }
     } else {
-      PolicyInputs in = {0.f, 0.f, 0.f};
-      if (kMode == kPolicy && tid == 0) in = policy_inputs(a.policy, row, b_now, t_now);
       Softmax s = {-INFINITY, 0.f};
       for (int c = 0; c < a.chunks; ++c) {
-        const int left = p.packs - c * kChunk;
+        const int left = packs - c * kChunk;
         mine.take(slots, left, tid);
         if (c + 1 < a.chunks)
           ask(c + 1);
         else if (kMode == kPolicy && grad != nullptr && c > 0)
           ask(c - 1);
         else
-          ask_next();
+          ask_row(facts[(k + 1) & 3]);
+        if (clerk && c == 0) describe();
         mine.add_to(s, left);
-        const int at = target - (p.first + c * kChunk * kN);
+        const int at = target - (first + c * kChunk * kN);
         if (Chunk::holds(at, left, tid)) tell_target(mine.value(at));
       }
-      if (p.outside >= 0) {
+      if (outside >= 0) {
         s = join_rows(s, {x_outside, x_outside == -INFINITY ? 0.f : x_outside * 0.f + 1.f});  // (NaN of +inf, NaN)
-        if (p.outside == target) tell_target(x_outside);
+        if (outside == target) tell_target(x_outside);
       }
+      __syncwarp();
       s = row_of_lanes(s);
       if (lane == 0) part[warp] = s;
       __syncthreads();
@@ -889,11 +864,11 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads)
         const float logp = log_prob_of(target >= 0 ? of_target[turn] : NAN, s);
         if (kMode == kSum) {
           if (rank == 0) {
-            a.softmax[row] = s;
-            a.logp[row] = logp;
+            a.softmax[f.row] = s;
+            a.logp[f.row] = logp;
           }
         } else {
-          const PolicyToken c = policy_token(a.policy, in, logp);
+          const PolicyToken c = policy_token(a.policy, {f.more[0], f.more[1], f.more[2]}, logp);
           sums[0] += static_cast<double>(w) * c.loss;
           sums[1] += static_cast<double>(w) * c.kl;
           sums[2] += static_cast<double>(w) * c.clipped;
@@ -903,25 +878,24 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads)
         }
       }
       __syncthreads();  // (`part` is read, `said` is there; nobody writes it before all are past the next row's first)
-      turn ^= 1;
       if (kMode == kSum || grad == nullptr) continue;
       now = said;
 #pragma unroll 1
       for (int c = a.chunks - 1; c >= 0; --c) {  // (the last is still held)
-        const int left = p.packs - c * kChunk, at = p.first + c * kChunk * kN;
+        const int left = packs - c * kChunk, at = first + c * kChunk * kN;
         if (c + 1 < a.chunks) {
           mine.take(slots, left, tid);
           if (c > 0)
             ask(c - 1);
           else
-            ask_next();
+            ask_row(facts[(k + 1) & 3]);
         }
         mine.turn(g + at, left, now.target - at, now, tid);
       }
     }
-    if (kMode != kSum && p.outside >= 0) {
+    if (kMode != kSum && outside >= 0) {
       const float v = now.k * exp_from(x_outside, now.most);
-      g[p.outside] = Pack<T>::back(p.outside == now.target ? v + now.by : v);
+      g[outside] = Pack<T>::back(outside == now.target ? v + now.by : v);
     }
   }
   __syncwarp();
