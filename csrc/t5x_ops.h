@@ -105,7 +105,7 @@ int t5x_policy_loss_tokens(const void* logp, void* slope, long long batch, int l
                            const void* old_scores, const void* ref_scores, const void* advantages,
                            long long adv_b, long long adv_t, float clip_low, float clip_high, float kl_weight,
                            float scale, const void* normalizer, void* scratch, void* out, void* stream);
-long long t5x_preference_loss_scratch_bytes(long long batch, int length);
+long long t5x_preference_loss_scratch_bytes(long long batch, int length, int vocab, int fp32);
 int t5x_preference_loss(const void* logits, int fp32, void* grad, long long batch, int length, int vocab,
                         long long stride_b, long long stride_t, const void* targets, const void* weights,
                         const void* reference, float beta, float smoothing, float scale, const void* normalizer,

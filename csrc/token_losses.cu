@@ -20,6 +20,7 @@
 // What bounds it: memory; the logits that count read once, the gradient written once.
 #include <atomic>
 #include <cmath>
+#include <cstddef>
 #include <type_traits>
 
 #include "common.cuh"
@@ -391,66 +392,6 @@ __device__ __forceinline__ Margin pair_margin(const Preference& p, bool real, do
   return m;
 }
 
-// A CTA per pair: scores, margin, the pair's loss, the slopes of its two sequences (and, from
-// log-probabilities, of its tokens). The last CTA adds the losses. out: loss, pairs
-__global__ void __launch_bounds__(kRowThreads)
-    preference_pairs_kernel(const float* __restrict__ logp, const Rows r, const Preference p, float* scores,
-                            float* margins, float* __restrict__ by, float* __restrict__ token_slope,
-                            double* pair_loss, unsigned* arrived, float* out) {
-  const long long pair = blockIdx.x;
-  const float scale = scale_of(p.normalizer, p.scale);
-  double sum[2] = {0.0, 0.0}, seen = 0.0;
-#pragma unroll
-  for (int side = 0; side < 2; ++side) {
-    const long long first = (2 * pair + side) * r.length;
-    for (int t = threadIdx.x; t < r.length; t += kRowThreads) {
-      const float w = r.weights != nullptr ? r.weights[first + t] : 1.f;
-      if (w != 0.f) {
-        sum[side] += static_cast<double>(w) * logp[first + t];
-        seen = 1.0;
-      }
-    }
-    sum[side] = cta_sum<kRowThreads>(sum[side]);
-  }
-  const bool real = cta_sum<kRowThreads>(seen) > 0.0;
-  const Margin m = pair_margin(p, real, sum[0], sum[1], p.ref[2 * pair], p.ref[2 * pair + 1], scale);
-  const float slope = m.slope;
-  if (threadIdx.x == 0) {
-    scores[2 * pair] = static_cast<float>(sum[0]);
-    scores[2 * pair + 1] = static_cast<float>(sum[1]);
-    margins[pair] = static_cast<float>(m.margin);
-    if (by != nullptr) {
-      by[2 * pair] = slope;
-      by[2 * pair + 1] = -slope;
-    }
-    pair_loss[2 * pair] = m.loss;
-    pair_loss[2 * pair + 1] = real ? 1.0 : 0.0;
-  }
-  if (token_slope != nullptr) {
-#pragma unroll
-    for (int side = 0; side < 2; ++side) {
-      const long long first = (2 * pair + side) * r.length;
-      for (int t = threadIdx.x; t < r.length; t += kRowThreads) {
-        const float w = r.weights != nullptr ? r.weights[first + t] : 1.f;
-        token_slope[first + t] = w == 0.f ? 0.f : (side ? -slope : slope) * w;
-      }
-    }
-  }
-  if (!last_cta(arrived)) return;
-  const double whole = p.normalizer != nullptr ? 1.0 / static_cast<double>(*p.normalizer) : p.scale;
-  double loss = 0.0, pairs = 0.0;
-  for (int k = threadIdx.x; k < static_cast<int>(gridDim.x); k += kRowThreads) {
-    loss += __ldcg(pair_loss + 2 * k);
-    pairs += __ldcg(pair_loss + 2 * k + 1);
-  }
-  loss = cta_sum<kRowThreads>(loss);
-  pairs = cta_sum<kRowThreads>(pairs);
-  if (threadIdx.x == 0) {
-    out[0] = static_cast<float>(loss * whole);
-    out[1] = static_cast<float>(pairs);
-  }
-}
-
 template <typename T>
 __global__ void __launch_bounds__(kRowThreads)
     preference_short_gradient_kernel(const T* __restrict__ logits, T* __restrict__ grad, const Rows r,
@@ -487,7 +428,7 @@ constexpr int kPacks = 8;
 constexpr float kHuge = 1.0e38f;
 __device__ __forceinline__ bool huge(float most) { return !(fabsf(most) <= kHuge); }  // (NaN and -inf too)
 // log2 of exp(a - b); 0 for a = b = -inf
-__device__ __forceinline__ float shift(float a, float b) {
+__device__ __forceinline__ float shift_of(float a, float b) {
   if (huge(a) || huge(b)) return a == b ? 0.f : (a - b) * kLog2e;
   return __fmul_rn(a, kLog2e) - __fmul_rn(b, kLog2e);
 }
@@ -497,12 +438,12 @@ __device__ __forceinline__ float exp_from(float x, float most) {
 }
 __device__ __forceinline__ Softmax join_rows(Softmax a, Softmax b) {
   const float m = fmaxf(a.most, b.most);
-  return {m, a.sum * exp2_approx(shift(a.most, m)) + b.sum * exp2_approx(shift(b.most, m))};
+  return {m, a.sum * exp2_approx(shift_of(a.most, m)) + b.sum * exp2_approx(shift_of(b.most, m))};
 }
 // of a warp's lanes
 __device__ __forceinline__ Softmax row_of_lanes(Softmax s) {
   const float m = warp_max(s.most);
-  return {m, warp_sum(s.sum * exp2_approx(shift(s.most, m)))};
+  return {m, warp_sum(s.sum * exp2_approx(shift_of(s.most, m)))};
 }
 __device__ __forceinline__ float log_prob_of(float x, Softmax s) {
   if (s.most == -INFINITY) return NAN;
@@ -578,6 +519,13 @@ struct Share {
       if ((i + 1) * kThreads <= packs || i * kThreads + tid < packs)
         fetch<16>(to + i * kThreads * 16, from + i * kThreads);
   }
+  // From where it lies.
+  __device__ __forceinline__ void load(const T* p, int packs, int lane) {
+    const uint4* from = reinterpret_cast<const uint4*>(p) + lane;
+#pragma unroll
+    for (int i = 0; i < kPacks; ++i)
+      x[i] = i * kThreads + lane < packs ? from[i * kThreads] : Unpack<T>::nothing();
+  }
   // All that the thread has asked for is there.
   __device__ __forceinline__ void take(const uint4* slots, int packs, int tid) {
     fetched();
@@ -605,7 +553,7 @@ struct Share {
     for (int i = 0; i < kPacks; ++i) Unpack<T>::raise(most, x[i]);
     const float m = Unpack<T>::most(most);
     if (m > s.most) {
-      s.sum *= exp2_approx(shift(s.most, m));
+      s.sum *= exp2_approx(shift_of(s.most, m));
       s.most = m;
     }
     float t[4] = {0.f, 0.f, 0.f, 0.f};
@@ -671,7 +619,139 @@ struct Share {
   }
 };
 
-enum Mode : int { kPolicy, kSum, kTurn };  // all of the policy loss; a preference loss' softmaxes; its gradients
+// Long rows in pieces of a row, a warp each: their softmaxes and the target's logit. Warps at different places
+// of their pieces keep the reads going, and none waits for another: 82 us for 64 x 114 x 32128 bf16 logits of
+// which 80% count, 4.6 TB/s, and 135 us for 14 x 509 x 32101 fp32, 5.4 TB/s; a CTA a row, as for the gradient
+// below, took 109 and 184 us.
+struct Pieces {
+  Softmax* of_piece;  // of row and piece
+  int shift;          // 1 << shift pieces a row
+  float* of_target;   // NaN: outside of the vocabulary
+  Softmax* of_row;
+
+  // The row's softmax, kept, and its target's log-probability.
+  __device__ __forceinline__ float log_prob(long long row) const {
+    const Softmax* of = of_piece + (row << shift);
+    Softmax s = {-INFINITY, 0.f};
+#pragma unroll 4
+    for (int k = 0; k < 1 << shift; ++k) s.most = fmaxf(s.most, of[k].most);
+#pragma unroll 4
+    for (int k = 0; k < 1 << shift; ++k) s.sum += of[k].sum * exp2_approx(shift_of(of[k].most, s.most));
+    of_row[row] = s;
+    return log_prob_of(of_target[row], s);
+  }
+};
+
+constexpr int kPieceThreads = 256, kPieceCtas = 4;  // CTAs of an SM
+
+template <typename T>
+__global__ void __launch_bounds__(kPieceThreads, kPieceCtas)
+    preference_pieces_kernel(const T* __restrict__ logits, const Rows r, const Pieces p) {
+  constexpr int kN = Pack<T>::kN, kChunk = 32 * kPacks;
+  const int lane = threadIdx.x & 31;
+  const long long warps = static_cast<long long>(gridDim.x) * (kPieceThreads / 32);
+  const long long pieces = r.rows << p.shift;
+  auto weight_of = [&](long long i) {
+    return i < pieces ? (r.weights != nullptr ? r.weights[i >> p.shift] : 1.f) : 0.f;
+  };
+  long long i = blockIdx.x * static_cast<long long>(kPieceThreads / 32) + (threadIdx.x >> 5);
+  float next = weight_of(i);
+  for (; i < pieces; i += warps) {
+    const float w = next;
+    next = weight_of(i + warps);
+    if (w == 0.f) continue;
+    const long long row = i >> p.shift;
+    const int piece = static_cast<int>(i - (row << p.shift)), b = static_cast<int>(row) / r.length;
+    const T* x = logits + b * r.stride_b + (static_cast<int>(row) - b * r.length) * r.stride_t;
+    const int off = static_cast<int>(reinterpret_cast<uintptr_t>(x) & 15) / static_cast<int>(sizeof(T));
+    const int head = off ? kN - off : 0, all = (r.vocab - head) / kN;
+    const int size = (all + (1 << p.shift) - 1) >> p.shift, from = min(size * piece, all);
+    const int packs = min(all - from, size);
+    Softmax s = {-INFINITY, 0.f};
+    if (piece == 0) {
+      // the values in front of the first 16-byte boundary and behind the last
+      const int outside = lane < head ? lane : all * kN + lane;
+      if (outside < r.vocab) {
+        const float v = Pack<T>::one(x[outside]);
+        s = {v, v == -INFINITY ? 0.f : v * 0.f + 1.f};  // (NaN of +inf and NaN)
+      }
+      if (lane == 0) {
+        const long long target = r.targets[row];
+        p.of_target[row] = target >= 0 && target < r.vocab ? Pack<T>::one(x[target]) : NAN;
+      }
+    }
+    Share<T, 32> mine;
+    for (int at = 0; at < packs; at += kChunk) {
+      mine.load(x + head + (from + at) * kN, packs - at, lane);
+      mine.add_to(s, packs - at);
+    }
+    __syncwarp();
+    s = row_of_lanes(s);
+    if (lane == 0) p.of_piece[i] = s;
+  }
+}
+
+// A CTA per pair: scores, margin, the pair's loss, the slopes of its two sequences (and, from
+// log-probabilities, of its tokens). The last CTA adds the losses. out: loss, pairs
+__global__ void __launch_bounds__(kRowThreads)
+    preference_pairs_kernel(const float* __restrict__ logp, const Pieces pieces, const Rows r, const Preference p,
+                            float* scores, float* margins, float* __restrict__ by, float* __restrict__ token_slope,
+                            double* pair_loss, unsigned* arrived, float* out) {
+  const long long pair = blockIdx.x;
+  const float scale = scale_of(p.normalizer, p.scale);
+  double sum[2] = {0.0, 0.0}, seen = 0.0;
+#pragma unroll
+  for (int side = 0; side < 2; ++side) {
+    const long long first = (2 * pair + side) * r.length;
+    for (int t = threadIdx.x; t < r.length; t += kRowThreads) {
+      const float w = r.weights != nullptr ? r.weights[first + t] : 1.f;
+      if (w != 0.f) {
+        sum[side] += static_cast<double>(w) * (logp != nullptr ? logp[first + t] : pieces.log_prob(first + t));
+        seen = 1.0;
+      }
+    }
+    sum[side] = cta_sum<kRowThreads>(sum[side]);
+  }
+  const bool real = cta_sum<kRowThreads>(seen) > 0.0;
+  const Margin m = pair_margin(p, real, sum[0], sum[1], p.ref[2 * pair], p.ref[2 * pair + 1], scale);
+  const float slope = m.slope;
+  if (threadIdx.x == 0) {
+    scores[2 * pair] = static_cast<float>(sum[0]);
+    scores[2 * pair + 1] = static_cast<float>(sum[1]);
+    margins[pair] = static_cast<float>(m.margin);
+    if (by != nullptr) {
+      by[2 * pair] = slope;
+      by[2 * pair + 1] = -slope;
+    }
+    pair_loss[2 * pair] = m.loss;
+    pair_loss[2 * pair + 1] = real ? 1.0 : 0.0;
+  }
+  if (token_slope != nullptr) {
+#pragma unroll
+    for (int side = 0; side < 2; ++side) {
+      const long long first = (2 * pair + side) * r.length;
+      for (int t = threadIdx.x; t < r.length; t += kRowThreads) {
+        const float w = r.weights != nullptr ? r.weights[first + t] : 1.f;
+        token_slope[first + t] = w == 0.f ? 0.f : (side ? -slope : slope) * w;
+      }
+    }
+  }
+  if (!last_cta(arrived)) return;
+  const double whole = p.normalizer != nullptr ? 1.0 / static_cast<double>(*p.normalizer) : p.scale;
+  double loss = 0.0, pairs = 0.0;
+  for (int k = threadIdx.x; k < static_cast<int>(gridDim.x); k += kRowThreads) {
+    loss += __ldcg(pair_loss + 2 * k);
+    pairs += __ldcg(pair_loss + 2 * k + 1);
+  }
+  loss = cta_sum<kRowThreads>(loss);
+  pairs = cta_sum<kRowThreads>(pairs);
+  if (threadIdx.x == 0) {
+    out[0] = static_cast<float>(loss * whole);
+    out[1] = static_cast<float>(pairs);
+  }
+}
+
+enum Mode : int { kPolicy, kTurn };  // all of the policy loss; the gradients of a preference loss
 
 struct LongArgs {
   int shift, chunks;  // 1 << shift CTAs share a row; chunks of a CTA's part
@@ -679,9 +759,8 @@ struct LongArgs {
   double* partial;
   unsigned* arrived;
   float* out;
-  Softmax* softmax;
-  float* logp;
-  const float* by;  // of the sequences
+  const Softmax* softmax;  // of the rows
+  const float* by;         // of the sequences
 };
 
 // What there is to know of a row.
@@ -690,8 +769,7 @@ struct alignas(16) RowFacts {
   int first, packs;   // the CTA's part: its first value, its number of 16 bytes
   long long target;
   float weight;
-  int row;
-  float more[4];  // policy: old score, reference score, advantage; gradients: softmax, slope of the sequence
+  alignas(16) float more[4];  // policy: old score, reference score, advantage; gradients: softmax, slope of the sequence
 };
 
 template <typename T, int kThreads, int kMode>
@@ -704,6 +782,7 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads)
   __shared__ float of_target[2];
   __shared__ Slope said;
   using Chunk = Share<T, kThreads>;
+  static_assert(offsetof(RowFacts, target) % 8 == 0 && offsetof(RowFacts, more) % 16 == 0, "places of cp.async");
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int ctas = 1 << a.shift, rank = a.shift ? static_cast<int>(cluster_ctarank()) : 0;
   const int cluster = blockIdx.x >> a.shift, clusters = gridDim.x >> a.shift, rows = static_cast<int>(r.rows);
@@ -734,7 +813,6 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads)
     f.offset = offset;
     f.first = head + from * kN;
     f.packs = min(all - from, size);
-    f.row = row;
     fetch<8>(smem_u32(&f.target), r.targets + row);
     if (r.weights != nullptr)
       fetch<4>(smem_u32(&f.weight), r.weights + row);
@@ -746,11 +824,9 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads)
       b -= step_b, t -= step_t;
       if (t < 0) t += r.length, --b;
     } else {
-      if (kMode == kPolicy) {
-        fetch<4>(smem_u32(f.more), a.policy.old + row);
-        if (a.policy.ref != nullptr) fetch<4>(smem_u32(f.more + 1), a.policy.ref + row);
-        fetch<4>(smem_u32(f.more + 2), a.policy.advantages + b * a.policy.adv_b + t * a.policy.adv_t);
-      }
+      fetch<4>(smem_u32(f.more), a.policy.old + row);
+      if (a.policy.ref != nullptr) fetch<4>(smem_u32(f.more + 1), a.policy.ref + row);
+      fetch<4>(smem_u32(f.more + 2), a.policy.advantages + b * a.policy.adv_b + t * a.policy.adv_t);
       b += step_b, t += step_t;
       if (t >= r.length) t -= r.length, ++b;
     }
@@ -783,7 +859,7 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads)
       fetched();  // (the clerk's)
       ask_row(facts[(k + 1) & 3]);
       if (clerk) describe();
-      if (kMode != kSum && grad != nullptr) {
+      if (grad != nullptr) {
         for (int i = tid; i < packs; i += kThreads)
           *reinterpret_cast<uint4*>(g + first + i * kN) = make_uint4(0, 0, 0, 0);
         if (outside >= 0) g[outside] = Pack<T>::back(0.f);
@@ -830,7 +906,7 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads)
         mine.take(slots, left, tid);
         if (c + 1 < a.chunks)
           ask(c + 1);
-        else if (kMode == kPolicy && grad != nullptr && c > 0)
+        else if (grad != nullptr && c > 0)
           ask(c - 1);
         else
           ask_row(facts[(k + 1) & 3]);
@@ -862,23 +938,16 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads)
       }
       if (tid == 0) {
         const float logp = log_prob_of(target >= 0 ? of_target[turn] : NAN, s);
-        if (kMode == kSum) {
-          if (rank == 0) {
-            a.softmax[f.row] = s;
-            a.logp[f.row] = logp;
-          }
-        } else {
-          const PolicyToken c = policy_token(a.policy, {f.more[0], f.more[1], f.more[2]}, logp);
-          sums[0] += static_cast<double>(w) * c.loss;
-          sums[1] += static_cast<double>(w) * c.kl;
-          sums[2] += static_cast<double>(w) * c.clipped;
-          sums[3] += w;
-          const float by = w * c.slope * scale;
-          said = {s.most, by, -by / s.sum, target};
-        }
+        const PolicyToken c = policy_token(a.policy, {f.more[0], f.more[1], f.more[2]}, logp);
+        sums[0] += static_cast<double>(w) * c.loss;
+        sums[1] += static_cast<double>(w) * c.kl;
+        sums[2] += static_cast<double>(w) * c.clipped;
+        sums[3] += w;
+        const float by = w * c.slope * scale;
+        said = {s.most, by, -by / s.sum, target};
       }
       __syncthreads();  // (`part` is read, `said` is there; nobody writes it before all are past the next row's first)
-      if (kMode == kSum || grad == nullptr) continue;
+      if (grad == nullptr) continue;
       now = said;
 #pragma unroll 1
       for (int c = a.chunks - 1; c >= 0; --c) {  // (the last is still held)
@@ -893,7 +962,7 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads)
         mine.turn(g + at, left, now.target - at, now, tid);
       }
     }
-    if (kMode != kSum && outside >= 0) {
+    if (outside >= 0) {
       const float v = now.k * exp_from(x_outside, now.most);
       g[outside] = Pack<T>::back(outside == now.target ? v + now.by : v);
     }
@@ -1022,6 +1091,24 @@ int launch_long(const char* what, const void* logits, void* grad, const Rows& r,
   return launch_long<T, 512, kMode>(what, logits, grad, r, a, st);
 }
 
+// Pieces of 24 to 48 KB. (Of 8 KB they are better balanced, but a pair's CTA has more of them to join: 80 and 10 us
+// in the place of 82 and 8.5 at 64 KB a row, 145 and 29 in the place of 135 and 9 at 128 KB.)
+int piece_shift(long long bytes) {
+  int shift = 0;
+  while (shift < 4 && bytes >> shift >= 49152) ++shift;
+  return shift;
+}
+
+template <typename T>
+int launch_pieces(const T* logits, const Rows& r, const Pieces& p, cudaStream_t st) {
+  if (r.rows > (1 << 30)) return set_error("preference_loss: too many rows");
+  const long long ctas = ((r.rows << p.shift) * 32 + kPieceThreads - 1) / kPieceThreads;
+  const long long cap = static_cast<long long>(num_sms()) * kPieceCtas;  // as many as run at once
+  preference_pieces_kernel<T>
+      <<<static_cast<unsigned>(ctas < cap ? ctas : cap), kPieceThreads, 0, st>>>(logits, r, p);
+  return launched("preference_loss", 1);
+}
+
 constexpr size_t kHead = 16;  // bytes of scratch in front: the count of arrived CTAs
 
 }  // namespace
@@ -1094,9 +1181,12 @@ T5X_API int t5x_policy_loss_tokens(const void* logp, void* slope, long long batc
   return launched("policy_loss_tokens", 1);
 }
 
-T5X_API long long t5x_preference_loss_scratch_bytes(long long batch, int length) {
-  // head | loss and count of each pair | softmax of each token | log-probability | slope of each row
-  return static_cast<long long>(kHead) + batch * 8 + batch * length * 12 + batch * 4;
+T5X_API long long t5x_preference_loss_scratch_bytes(long long batch, int length, int vocab, int fp32) {
+  // head | loss and count of each pair | softmax of each token | of its pieces | log-probability or logit of the
+  // target | slope of each row
+  const long long bytes = static_cast<long long>(vocab) * (fp32 ? 4 : 2);
+  const long long pieces = bytes >= kLongRow ? 1 << piece_shift(bytes) : 0;
+  return static_cast<long long>(kHead) + batch * 8 + batch * length * (12 + 8 * pieces) + batch * 4;
 }
 
 T5X_API int t5x_preference_loss(const void* logits, int fp32, void* grad, long long batch, int length, int vocab,
@@ -1118,27 +1208,29 @@ T5X_API int t5x_preference_loss(const void* logits, int fp32, void* grad, long l
   unsigned* arrived = reinterpret_cast<unsigned*>(at);
   double* pair_loss = reinterpret_cast<double*>(at + kHead);
   Softmax* softmax = reinterpret_cast<Softmax*>(pair_loss + batch);
-  float* logp = reinterpret_cast<float*>(softmax + r.rows);
+  const long long bytes = static_cast<long long>(vocab) * (fp32 ? 4 : 2);
+  const bool in_long = bytes >= kLongRow;
+  Pieces pieces = {softmax + r.rows, in_long ? piece_shift(bytes) : 0, nullptr, softmax};
+  float* logp = reinterpret_cast<float*>(pieces.of_piece + (in_long ? r.rows << pieces.shift : 0));
+  pieces.of_target = logp;
   float* by = logp + r.rows;
   cudaError_t e = cudaMemsetAsync(scratch, 0, kHead, st);
   if (e != cudaSuccess) return set_error("preference_loss: memset: %s", cudaGetErrorString(e));
   auto go = [&](auto* x) {
     using T = std::remove_const_t<std::remove_pointer_t<decltype(x)>>;
-    const bool in_long = static_cast<long long>(vocab) * static_cast<int>(sizeof(T)) >= kLongRow;
     LongArgs a = {};
     a.softmax = softmax;
-    a.logp = logp;
     a.by = by;
     const unsigned grid = row_grid(r.rows);
     int rc = 0;
     if (in_long)
-      rc = launch_long<T, kSum>("preference_loss", x, nullptr, r, a, st);
+      rc = launch_pieces<T>(x, r, pieces, st);
     else
       preference_short_rows_kernel<T><<<grid, kRowThreads, 0, st>>>(x, r, softmax, logp);
     if (rc != 0) return rc;
     preference_pairs_kernel<<<static_cast<unsigned>(pairs), kRowThreads, 0, st>>>(
-        logp, r, p, static_cast<float*>(scores), static_cast<float*>(margins), by, nullptr, pair_loss, arrived,
-        static_cast<float*>(out));
+        in_long ? nullptr : logp, pieces, r, p, static_cast<float*>(scores), static_cast<float*>(margins), by, nullptr,
+        pair_loss, arrived, static_cast<float*>(out));
     if (grad == nullptr) return launched("preference_loss", in_long ? 1 : 2);
     if (in_long)
       rc = launch_long<T, kTurn>("preference_loss", x, grad, r, a, st);
@@ -1163,8 +1255,8 @@ T5X_API int t5x_preference_loss_tokens(const void* logp, void* slope, long long 
   const Preference p = {static_cast<const float*>(reference), beta, smoothing, scale,
                         static_cast<const float*>(normalizer)};
   preference_pairs_kernel<<<static_cast<unsigned>(batch / 2), kRowThreads, 0, st>>>(
-      static_cast<const float*>(logp), r, p, static_cast<float*>(scores), static_cast<float*>(margins), nullptr,
-      static_cast<float*>(slope), reinterpret_cast<double*>(static_cast<char*>(scratch) + kHead),
+      static_cast<const float*>(logp), Pieces(), r, p, static_cast<float*>(scores), static_cast<float*>(margins),
+      nullptr, static_cast<float*>(slope), reinterpret_cast<double*>(static_cast<char*>(scratch) + kHead),
       static_cast<unsigned*>(scratch), static_cast<float*>(out));
   return launched("preference_loss_tokens", 1);
 }

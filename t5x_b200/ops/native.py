@@ -1204,7 +1204,7 @@ register_signature("t5x_policy_loss", [c_void_p, c_int, c_void_p, c_ll, c_int, c
                    [c_ll, c_ll] + [c_float] * 4 + [c_void_p] * 4)
 register_signature("t5x_policy_loss_tokens", [c_void_p, c_void_p, c_ll, c_int] + [c_void_p] * 4 + [c_ll, c_ll] +
                    [c_float] * 4 + [c_void_p] * 4)
-register_signature("t5x_preference_loss_scratch_bytes", [c_ll, c_int])
+register_signature("t5x_preference_loss_scratch_bytes", [c_ll, c_int, c_int, c_int])
 register_signature("t5x_preference_loss", [c_void_p, c_int, c_void_p, c_ll, c_int, c_int, c_ll, c_ll] + [c_void_p] * 3 +
                    [c_float] * 3 + [c_void_p] * 6)
 register_signature("t5x_preference_loss_tokens", [c_void_p, c_void_p, c_ll, c_int, c_void_p, c_void_p] +
@@ -1275,7 +1275,8 @@ def preference_loss(values, grad, targets, weights, reference, beta, label_smoot
   with _on_device_of(values):
     nbytes = lib().t5x_preference_loss_scratch_bytes
     nbytes.restype = c_ll
-    scratch = torch.empty(nbytes(b, l), dtype=torch.uint8, device=values.device)
+    vocab = 1 if targets is None else values.shape[2]
+    scratch = torch.empty(nbytes(b, l, vocab, int(values.dtype == torch.float32)), dtype=torch.uint8, device=values.device)
     scores = torch.empty(b, dtype=torch.float32, device=values.device)
     margins = torch.empty(b // 2, dtype=torch.float32, device=values.device)
     out = torch.empty(2, dtype=torch.float32, device=values.device)
