@@ -863,6 +863,129 @@ bool adamw_tree(py::handle params, py::handle grads, py::handle mu, py::handle n
   return true;
 }
 
+// ---- losses of preference and policy fine-tuning ----
+
+// The operands of a loss over logits [B, L, V] with targets, or over log-probabilities [B, L] without.
+struct LossValues {
+  int64_t b = 0, l = 0, v = 1, stride_b = 0, stride_t = 0;
+  bool fp32 = true, ok = false;
+
+  LossValues(const Tensor& x, const optional<Tensor>& targets) {
+    if (!x.is_cuda() || x.get_device() != c10::cuda::current_device() || x.numel() == 0) return;
+    fp32 = x.scalar_type() == at::kFloat;
+    if (!fp32 && !(targets && x.scalar_type() == at::kBFloat16)) return;
+    if (x.dim() != (targets ? 3 : 2)) return;
+    b = x.size(0), l = x.size(1);
+    if (!fits(l)) return;
+    if (!targets) {
+      ok = x.is_contiguous();
+      return;
+    }
+    v = x.size(2);
+    // (the stride of a dimension of one: what it would be side by side)
+    stride_t = l > 1 ? x.stride(1) : v;
+    stride_b = b > 1 ? x.stride(0) : (l - 1) * stride_t + v;
+    ok = fits(v) && (x.stride(2) == 1 || v == 1) && stride_t >= v && stride_b >= (l - 1) * stride_t + v &&
+         of(x, *targets, at::kLong);
+  }
+  // Whether t holds a value for each token.
+  bool of(const Tensor& x, const Tensor& t, at::ScalarType type) const {
+    return t.scalar_type() == type && t.dim() == 2 && t.size(0) == b && t.size(1) == l && t.is_contiguous() &&
+           t.device() == x.device();
+  }
+  bool of(const Tensor& x, const optional<Tensor>& t) const { return !t || of(x, *t, at::kFloat); }
+};
+
+const void* data_of(const optional<Tensor>& t) { return t ? t->data_ptr() : nullptr; }
+
+bool scalar(const Tensor& x, const optional<Tensor>& t) {
+  return !t || (t->scalar_type() == at::kFloat && t->numel() == 1 && t->device() == x.device());
+}
+
+// Memory for the gradient: the same strides, at the same place of 16 bytes.
+Tensor gradient_like(const Tensor& x) {
+  const int64_t behind = static_cast<int64_t>(reinterpret_cast<uintptr_t>(x.data_ptr()) % 16 / x.element_size());
+  int64_t span = 1;
+  for (int64_t i = 0; i < x.dim(); ++i) span += (x.size(i) - 1) * x.stride(i);
+  return at::empty({span + behind}, x.options()).as_strided(x.sizes(), x.strides(), behind);
+}
+
+Tensor bytes_like(const Tensor& x, int64_t n) { return at::empty({n}, x.options().dtype(at::kByte)); }
+
+// loss, kl, clipped, weight, gradient (undefined unless wanted); nothing where the call is not covered
+std::vector<Tensor> policy_loss(const Tensor& x, const optional<Tensor>& targets, const optional<Tensor>& weights,
+                                const Tensor& old, const Tensor& advantages, const optional<Tensor>& reference,
+                                double clip_low, double clip_high, double kl_weight, double scale,
+                                const optional<Tensor>& normalizer, bool wanted) {
+  const LossValues s(x, targets);
+  if (!s.ok || !s.of(x, weights) || !s.of(x, old, at::kFloat) || !s.of(x, reference) || !scalar(x, normalizer) ||
+      advantages.scalar_type() != at::kFloat || advantages.device() != x.device() || advantages.dim() < 1 ||
+      advantages.dim() > 2 || advantages.size(0) != s.b)
+    return {};
+  int64_t adv_t = 0;
+  if (advantages.dim() == 2 && advantages.size(1) != 1) {
+    if (advantages.size(1) != s.l) return {};
+    adv_t = advantages.stride(1);
+  }
+  Tensor grad = wanted ? gradient_like(x) : Tensor();
+  void* g = wanted ? grad.data_ptr() : nullptr;
+  Tensor scratch = bytes_like(x, t5x_policy_loss_scratch_bytes());
+  Tensor out = at::empty({4}, x.options().dtype(at::kFloat));
+  const float low = clip_low, high = clip_high, kl = kl_weight, by = scale;
+  void* st = stream_of();
+  check(targets ? t5x_policy_loss(x.data_ptr(), s.fp32, g, s.b, s.l, s.v, s.stride_b, s.stride_t, targets->data_ptr(),
+                                  data_of(weights), old.data_ptr(), data_of(reference), advantages.data_ptr(),
+                                  advantages.stride(0), adv_t, low, high, kl, by, data_of(normalizer),
+                                  scratch.data_ptr(), out.data_ptr(), st)
+                : t5x_policy_loss_tokens(x.data_ptr(), g, s.b, s.l, data_of(weights), old.data_ptr(),
+                                         data_of(reference), advantages.data_ptr(), advantages.stride(0), adv_t, low,
+                                         high, kl, by, data_of(normalizer), scratch.data_ptr(), out.data_ptr(), st),
+        "policy_loss");
+  // (the loss, which users add to in place, is not a view to autograd)
+  return {out.select(0, 0).variable_data(), out.select(0, 1), out.select(0, 2), out.select(0, 3), grad};
+}
+
+// loss, scores, margins, pairs, gradient (undefined unless wanted); nothing where the call is not covered
+std::vector<Tensor> preference_loss(const Tensor& x, const optional<Tensor>& targets, const optional<Tensor>& weights,
+                                    const Tensor& reference, double beta, double smoothing, double scale,
+                                    const optional<Tensor>& normalizer, bool wanted) {
+  const LossValues s(x, targets);
+  if (!s.ok || !s.of(x, weights) || !scalar(x, normalizer) || reference.scalar_type() != at::kFloat ||
+      reference.device() != x.device() || reference.dim() != 1 || reference.size(0) != s.b ||
+      !reference.is_contiguous())
+    return {};
+  Tensor grad = wanted ? gradient_like(x) : Tensor();
+  void* g = wanted ? grad.data_ptr() : nullptr;
+  Tensor scratch = bytes_like(x, t5x_preference_loss_scratch_bytes(s.b, s.l, s.v, s.fp32));
+  const auto floats = x.options().dtype(at::kFloat);
+  Tensor out = at::empty({2}, floats), scores = at::empty({s.b}, floats), margins = at::empty({s.b / 2}, floats);
+  const float b = beta, e = smoothing, by = scale;
+  void* st = stream_of();
+  check(targets ? t5x_preference_loss(x.data_ptr(), s.fp32, g, s.b, s.l, s.v, s.stride_b, s.stride_t,
+                                      targets->data_ptr(), data_of(weights), reference.data_ptr(), b, e, by,
+                                      data_of(normalizer), scratch.data_ptr(), scores.data_ptr(), margins.data_ptr(),
+                                      out.data_ptr(), st)
+                : t5x_preference_loss_tokens(x.data_ptr(), g, s.b, s.l, data_of(weights), reference.data_ptr(), b, e,
+                                             by, data_of(normalizer), scratch.data_ptr(), scores.data_ptr(),
+                                             margins.data_ptr(), out.data_ptr(), st),
+        "preference_loss");
+  return {out.select(0, 0).variable_data(), scores, margins, out.select(0, 1), grad};
+}
+
+// grad * factor, in place or, with `keep`, in memory of its own
+optional<Tensor> scale_gradient(const Tensor& grad, const Tensor& factor, bool keep) {
+  if (!grad.is_cuda() || grad.get_device() != c10::cuda::current_device() || !scalar(grad, factor) ||
+      grad.numel() == 0)
+    return std::nullopt;
+  Tensor to = keep ? gradient_like(grad) : grad;
+  int64_t span = 1;
+  for (int64_t i = 0; i < grad.dim(); ++i) span += (grad.size(i) - 1) * grad.stride(i);
+  check(t5x_scale_gradient(grad.data_ptr(), to.data_ptr(), span, grad.scalar_type() == at::kFloat,
+                           factor.data_ptr(), stream_of()),
+        "scale_gradient");
+  return to;
+}
+
 }  // namespace
 
 // The GIL is released for the duration of a call: a launch waits when the device's queue is full,
@@ -889,5 +1012,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("relu_grads_ok", relu_grads_ok);
   m.def("relu_block", torch::wrap_pybind_function_no_gil(relu_block));
   m.def("relu_block_bwd", torch::wrap_pybind_function_no_gil(relu_block_bwd));
+  m.def("policy_loss", torch::wrap_pybind_function_no_gil(policy_loss));
+  m.def("preference_loss", torch::wrap_pybind_function_no_gil(preference_loss));
+  m.def("scale_gradient", torch::wrap_pybind_function_no_gil(scale_gradient));
   m.def("adamw_tree", adamw_tree);  // (it reads Python's dicts, and releases the GIL for the launches)
 }

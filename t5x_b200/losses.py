@@ -166,12 +166,15 @@ def _check_tokens(what: str, values: torch.Tensor, dims: int, **tokens) -> None:
     raise ValueError(f"{what}: expected a tensor of {dims} dimensions, got shape {tuple(values.shape)}")
   if not values.is_floating_point():
     raise ValueError(f"{what}: expected floating-point values, got {values.dtype}")
+  shape, device = values.shape[:2], values.device
   for name, t in tokens.items():
-    if t is not None and t.shape != values.shape[:2]:
+    if t is None:
+      continue
+    if t.shape != shape:
       raise ValueError(f"{what}: Incorrect shapes. Got shape {tuple(t.shape)} {name} for [batch, length] = "
-                       f"{tuple(values.shape[:2])}")
-    if t is not None and t.device != values.device:
-      raise ValueError(f"{what}: {name} are on {t.device}, the values on {values.device}")
+                       f"{tuple(shape)}")
+    if t.device != device:
+      raise ValueError(f"{what}: {name} are on {t.device}, the values on {device}")
     if name == "targets" and (t.is_floating_point() or t.dtype == torch.bool):
       raise ValueError(f"{what}: targets must be whole numbers, got {t.dtype}")
 

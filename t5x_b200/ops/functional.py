@@ -61,6 +61,9 @@ class _NoGraph:
   def mark_non_differentiable(self, *tensors):
     pass
 
+  def set_materialize_grads(self, value):
+    pass
+
 
 def _apply(fn, *args):
   """fn.apply(*args). Where nothing can record or transform the call (no gradients, no function

@@ -134,7 +134,7 @@ class _HostOps:
            "rmsnorm_bwd", "attention", "attention_bwd", "attention_block_ok", "attention_grads_ok",
            "attention_block", "attention_block_bwd", "mlp_block_ok", "mlp_grads_ok", "mlp_block",
            "mlp_block_bwd", "relu_block_ok", "relu_grads_ok", "relu_block", "relu_block_bwd",
-           "adamw_tree")
+           "adamw_tree", "policy_loss", "preference_loss", "scale_gradient")
 
   def __init__(self, module):
     for name in self.NAMES:
@@ -1244,9 +1244,10 @@ def _loss_strides(t: torch.Tensor):
 def policy_loss(values, grad, targets, weights, old, advantages, reference, clip_low, clip_high, kl_weight, scale,
                 normalizer):
   """(loss, kl, clipped, weight) as device scalars; the gradient in `grad` unless it is None. values: logits
-  [B, L, V], or log-probabilities [B, L] with targets None; advantages: [B, L] of any strides."""
+  [B, L, V], or log-probabilities [B, L] with targets None; advantages: [B], [B, 1] or [B, L] of any strides."""
   _loss_inputs("policy_loss", values, grad, targets, weights, old, reference)
-  if advantages.shape != values.shape[:2] or advantages.dtype != torch.float32 or advantages.device != values.device:
+  advantages = (advantages[:, None] if advantages.dim() == 1 else advantages).expand(values.shape[:2])
+  if advantages.dtype != torch.float32 or advantages.device != values.device:
     raise NativeError("policy_loss: advantages must be fp32 of the batch's shape")
   b, l = values.shape[:2]
   with _on_device_of(values):
@@ -1263,7 +1264,8 @@ def policy_loss(values, grad, targets, weights, old, advantages, reference, clip
       rc = lib().t5x_policy_loss(values.data_ptr(), int(values.dtype == torch.float32), ptr(grad), b, l,
                                  values.shape[2], *_loss_strides(values), targets.data_ptr(), *tail)
   _check(rc, "policy_loss")
-  return tuple(o.clone() if i == 0 else o for i, o in enumerate(out.unbind(0)))
+  loss, *more = out.unbind(0)
+  return (loss.data, *more)  # (the loss, which users add to in place, is not a view to autograd)
 
 
 def preference_loss(values, grad, targets, weights, reference, beta, label_smoothing, scale, normalizer):
@@ -1288,7 +1290,7 @@ def preference_loss(values, grad, targets, weights, reference, beta, label_smoot
       rc = lib().t5x_preference_loss(values.data_ptr(), int(values.dtype == torch.float32), ptr(grad), b, l,
                                      values.shape[2], *_loss_strides(values), targets.data_ptr(), *tail)
   _check(rc, "preference_loss")
-  return out[0].clone(), scores, margins, out[1]
+  return out[0].data, scores, margins, out[1]
 
 
 def scale_gradient(grad: torch.Tensor, factor: torch.Tensor, keep: bool) -> torch.Tensor:

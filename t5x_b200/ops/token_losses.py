@@ -40,53 +40,57 @@ def _like(logits: torch.Tensor) -> torch.Tensor:
   return flat.as_strided(logits.shape, logits.stride(), behind)
 
 
-def _times(grad: torch.Tensor, factor: torch.Tensor) -> torch.Tensor:
-  """The saved gradient times the gradient of the loss."""
-  return native.scale_gradient(grad, factor.detach().float().reshape(1), keep=F._graph_is_kept())
+def _times(grad: torch.Tensor, factor: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
+  """The saved gradient times the gradient of the loss; None where there is none."""
+  if factor is None:
+    return None
+  keep, host = F._graph_is_kept(), native.host()
+  if host is not None:
+    out = host.scale_gradient(grad, factor, keep)
+    if out is not None:
+      return out
+  return native.scale_gradient(grad, factor.detach().float().reshape(1), keep=keep)
+
+
+def _loss(ctx, name, values, targets, *args):
+  """The outputs of the kernels' loss `name`; its gradient is kept with the graph where it will be wanted."""
+  want = not isinstance(ctx, F._NoGraph) and ctx.needs_input_grad[0]
+  host = native.host()
+  out = host and getattr(host, name)(values, targets, *args, want)
+  if out:
+    *out, grad = out
+  else:
+    values = values.contiguous() if targets is None else _rows_apart(values)
+    grad = _like(values) if want else None
+    out = getattr(native, name)(values, grad, targets, *args)
+  ctx.save_for_backward(grad)
+  ctx.mark_non_differentiable(*out[1:])
+  ctx.set_materialize_grads(False)
+  return tuple(out)
 
 
 class _PolicyFn(torch.autograd.Function):
 
   @staticmethod
-  def forward(ctx, values, targets, weights, old, advantages, reference, cfg):
-    want = not isinstance(ctx, F._NoGraph) and ctx.needs_input_grad[0]
-    if targets is not None:
-      values = _rows_apart(values)
-      grad = _like(values) if want else None
-    else:
-      values = values.contiguous()
-      grad = torch.empty_like(values) if want else None
-    out = native.policy_loss(values, grad, targets, weights, old, advantages, reference, *cfg)
-    ctx.save_for_backward(grad)
-    ctx.mark_non_differentiable(*out[1:])
-    return out
+  def forward(ctx, values, *args):
+    return _loss(ctx, "policy_loss", values, *args)
 
   @staticmethod
   @torch.autograd.function.once_differentiable
   def backward(ctx, by, *_):
-    return (_times(ctx.saved_tensors[0], by),) + (None,) * 6
+    return (_times(ctx.saved_tensors[0], by),) + (None,) * 10
 
 
 class _PreferenceFn(torch.autograd.Function):
 
   @staticmethod
-  def forward(ctx, values, targets, weights, reference, cfg):
-    want = not isinstance(ctx, F._NoGraph) and ctx.needs_input_grad[0]
-    if targets is not None:
-      values = _rows_apart(values)
-      grad = _like(values) if want else None
-    else:
-      values = values.contiguous()
-      grad = torch.empty_like(values) if want else None
-    out = native.preference_loss(values, grad, targets, weights, reference, *cfg)
-    ctx.save_for_backward(grad)
-    ctx.mark_non_differentiable(*out[1:])
-    return out
+  def forward(ctx, values, *args):
+    return _loss(ctx, "preference_loss", values, *args)
 
   @staticmethod
   @torch.autograd.function.once_differentiable
   def backward(ctx, by, *_):
-    return (_times(ctx.saved_tensors[0], by),) + (None,) * 4
+    return (_times(ctx.saved_tensors[0], by),) + (None,) * 7
 
 
 def _plain(t: Optional[torch.Tensor], dtype=torch.float32) -> Optional[torch.Tensor]:
@@ -120,13 +124,8 @@ def policy_loss(values, targets, weights, old, advantages, reference, clip_low, 
     return ref.policy_loss(logp, weights, old, advantages, reference, clip_low, clip_high, kl_weight,
                            normalizer)
   scale, divisor = _divisor(normalizer, values.device)
-  b, l = values.shape[:2]
-  advantages = _plain(advantages)
-  if advantages.dim() == 1:
-    advantages = advantages[:, None]
   return F._apply(_PolicyFn, values, _plain(targets, torch.int64), _plain(weights), _plain(old),
-                  advantages.expand(b, l), _plain(reference),
-                  (clip_low, clip_high, kl_weight, scale, divisor))
+                  _plain(advantages), _plain(reference), clip_low, clip_high, kl_weight, scale, divisor)
 
 
 def preference_loss(values, targets, weights, reference, beta, label_smoothing, normalizer):
@@ -140,4 +139,4 @@ def preference_loss(values, targets, weights, reference, beta, label_smoothing, 
     return ref.preference_loss(logp, weights, reference, beta, label_smoothing, normalizer)
   scale, divisor = _divisor(normalizer, values.device)
   return F._apply(_PreferenceFn, values, _plain(targets, torch.int64), _plain(weights),
-                  _plain(reference), (beta, label_smoothing, scale, divisor))
+                  _plain(reference), beta, label_smoothing, scale, divisor)
