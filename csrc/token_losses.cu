@@ -504,42 +504,53 @@ __device__ __forceinline__ void fetch(uint32_t to, const void* from) {
 }
 __device__ __forceinline__ void fetched() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 
-// A thread's share of a chunk of a row: 16 bytes number tid, tid + kThreads, ... of `packs` at p.
-template <typename T, int kThreads>
+// A thread's share of a chunk of a row, of which `packs` times 16 bytes at p are there: a warp has kWarpPacks of
+// them side by side, a thread every 32nd of those. So all warps but one have them all or none, and need not ask
+// for each.
+constexpr int kWarpPacks = 32 * kPacks;
+
+template <typename T>
 struct Share {
   static constexpr int kN = Pack<T>::kN;
   uint4 x[kPacks];
 
+  // visit(i, offset) for those of the thread's that are there; `offset` counts 16 bytes from the chunk's first.
+  template <typename Visit>
+  __device__ __forceinline__ static void each(int packs, int tid, Visit visit) {
+    const int first = (tid >> 5) * kWarpPacks, at = first + (tid & 31);
+    if (first + kWarpPacks <= packs) {
+#pragma unroll
+      for (int i = 0; i < kPacks; ++i) visit(i, at + i * 32);
+    } else if (first < packs) {
+#pragma unroll
+      for (int i = 0; i < kPacks; ++i)
+        if (at + i * 32 < packs) visit(i, at + i * 32);
+    }
+  }
   // On its way to the thread's own places in shared memory, which no other thread reads or writes.
   __device__ __forceinline__ static void ask(uint4* slots, const T* p, int packs, int tid) {
-    const uint32_t to = smem_u32(slots + tid);
-    const uint4* from = reinterpret_cast<const uint4*>(p) + tid;
+    const uint32_t to = smem_u32(slots);
+    each(packs, tid, [&](int, int k) { fetch<16>(to + k * 16, reinterpret_cast<const uint4*>(p) + k); });
+  }
+  __device__ __forceinline__ void get(const uint4* from, int packs, int tid) {
+    if (((tid >> 5) + 1) * kWarpPacks > packs) {
 #pragma unroll
-    for (int i = 0; i < kPacks; ++i)
-      if ((i + 1) * kThreads <= packs || i * kThreads + tid < packs)
-        fetch<16>(to + i * kThreads * 16, from + i * kThreads);
+      for (int i = 0; i < kPacks; ++i) x[i] = Unpack<T>::nothing();
+    }
+    each(packs, tid, [&](int i, int k) { x[i] = from[k]; });
   }
   // From where it lies.
-  __device__ __forceinline__ void load(const T* p, int packs, int lane) {
-    const uint4* from = reinterpret_cast<const uint4*>(p) + lane;
-#pragma unroll
-    for (int i = 0; i < kPacks; ++i)
-      x[i] = i * kThreads + lane < packs ? from[i * kThreads] : Unpack<T>::nothing();
+  __device__ __forceinline__ void load(const T* p, int packs, int tid) {
+    get(reinterpret_cast<const uint4*>(p), packs, tid);
   }
   // All that the thread has asked for is there.
   __device__ __forceinline__ void take(const uint4* slots, int packs, int tid) {
     fetched();
-#pragma unroll
-    for (int i = 0; i < kPacks; ++i) {
-      if ((i + 1) * kThreads <= packs)  // (the same for all threads: no selects)
-        x[i] = slots[i * kThreads + tid];
-      else
-        x[i] = i * kThreads + tid < packs ? slots[i * kThreads + tid] : Unpack<T>::nothing();
-    }
+    get(slots, packs, tid);
   }
-  // The value behind 16 bytes number `at`, by its thread.
+  // Value number `at` of the chunk, by its thread.
   __device__ __forceinline__ float value(int at) const {
-    const uint4 u = pick(at / kN / kThreads);
+    const uint4 u = pick(at / kN / 32 % kPacks);
     const uint32_t w = (at % kN) * sizeof(T) / 4 == 0   ? u.x
                        : (at % kN) * sizeof(T) / 4 == 1 ? u.y
                        : (at % kN) * sizeof(T) / 4 == 2 ? u.z
@@ -547,7 +558,11 @@ struct Share {
     if (sizeof(T) == 4) return __uint_as_float(w);
     return __uint_as_float(at & 1 ? w & 0xffff0000u : w << 16);
   }
-  __device__ __forceinline__ void add_to(Softmax& s, int packs) const {
+  // Whether it is this thread's.
+  __device__ __forceinline__ static bool holds(int at, int packs, int tid) {
+    return at >= 0 && at < packs * kN && at / (kN * kWarpPacks) == tid >> 5 && at / kN % 32 == (tid & 31);
+  }
+  __device__ __forceinline__ void add_to(Softmax& s) const {
     typename Unpack<T>::Most most = Unpack<T>::least();
 #pragma unroll
     for (int i = 0; i < kPacks; ++i) Unpack<T>::raise(most, x[i]);
@@ -560,13 +575,12 @@ struct Share {
     if (!huge(s.most)) {
       const float off = -__fmul_rn(s.most, kLog2e);
 #pragma unroll
-      for (int i = 0; i < kPacks; ++i)
-        if (i * kThreads < packs) {
-          float v[kN];
-          Unpack<T>::floats(x[i], v);
+      for (int i = 0; i < kPacks; ++i) {
+        float v[kN];
+        Unpack<T>::floats(x[i], v);
 #pragma unroll
-          for (int j = 0; j < kN; ++j) t[j % 4] += exp2_approx(fmaf(v[j], kLog2e, off));
-        }
+        for (int j = 0; j < kN; ++j) t[j % 4] += exp2_approx(fmaf(v[j], kLog2e, off));
+      }
     } else {
 #pragma unroll 1
       for (int i = 0; i < kPacks; ++i) {
@@ -588,34 +602,28 @@ struct Share {
   }
   // Stores the gradient at g; `at`: where the target lies, counted from the chunk's first value.
   __device__ __forceinline__ void turn(T* g, int packs, int at, const Slope& now, int tid) const {
-    uint4* to = reinterpret_cast<uint4*>(g) + tid;
     if (!huge(now.most)) {
       const float off = -__fmul_rn(now.most, kLog2e);
+      each(packs, tid, [&](int i, int k) {
+        float y[kN];
+        Unpack<T>::floats(x[i], y);
 #pragma unroll
-      for (int i = 0; i < kPacks; ++i)
-        if ((i + 1) * kThreads <= packs || i * kThreads + tid < packs) {
-          float y[kN];
-          Unpack<T>::floats(x[i], y);
-#pragma unroll
-          for (int j = 0; j < kN; ++j) y[j] = now.k * exp2_approx(fmaf(y[j], kLog2e, off));
-          Pack<T>::store(reinterpret_cast<T*>(to + i * kThreads), y);
-        }
+        for (int j = 0; j < kN; ++j) y[j] = now.k * exp2_approx(fmaf(y[j], kLog2e, off));
+        Pack<T>::store(g + k * kN, y);
+      });
     } else {
+      const int first = (tid >> 5) * kWarpPacks + (tid & 31);
 #pragma unroll 1
       for (int i = 0; i < kPacks; ++i)
-        if (i * kThreads + tid < packs) {
+        if (first + i * 32 < packs) {
           float y[kN];
           Unpack<T>::floats(pick(i), y);
 #pragma unroll
           for (int j = 0; j < kN; ++j) y[j] = now.k * exp_from(y[j], now.most);
-          Pack<T>::store(reinterpret_cast<T*>(to + i * kThreads), y);
+          Pack<T>::store(g + (first + i * 32) * kN, y);
         }
     }
     if (holds(at, packs, tid)) g[at] = Pack<T>::back(now.k * exp_from(value(at), now.most) + now.by);
-  }
-  // Whether value number `at` of the chunk is this thread's.
-  __device__ __forceinline__ static bool holds(int at, int packs, int tid) {
-    return at >= 0 && at < min(packs, kThreads * kPacks) * kN && at / kN % kThreads == tid;
   }
 };
 
@@ -680,10 +688,10 @@ __global__ void __launch_bounds__(kPieceThreads, kPieceCtas)
         p.of_target[row] = target >= 0 && target < r.vocab ? Pack<T>::one(x[target]) : NAN;
       }
     }
-    Share<T, 32> mine;
+    Share<T> mine;
     for (int at = 0; at < packs; at += kChunk) {
       mine.load(x + head + (from + at) * kN, packs - at, lane);
-      mine.add_to(s, packs - at);
+      mine.add_to(s);
     }
     __syncwarp();
     s = row_of_lanes(s);
@@ -781,7 +789,7 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads)
   __shared__ Softmax part[kWarps], of_cta[2][8];
   __shared__ float of_target[2];
   __shared__ Slope said;
-  using Chunk = Share<T, kThreads>;
+  using Chunk = Share<T>;
   static_assert(offsetof(RowFacts, target) % 8 == 0 && offsetof(RowFacts, more) % 16 == 0, "places of cp.async");
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int ctas = 1 << a.shift, rank = a.shift ? static_cast<int>(cluster_ctarank()) : 0;
@@ -839,7 +847,7 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads)
   __syncthreads();
   if (a.shift) cluster_sync_all();  // all CTAs have begun before any writes to another
   auto ask_row = [&](const RowFacts& f) {
-    if (f.weight != 0.f) Chunk::ask(slots, logits + f.offset + f.first, f.packs, tid);
+    if (f.weight != 0.f) Chunk::ask(slots, logits + f.offset + f.first, min(f.packs, kChunk), tid);
   };
   ask_row(facts[0]);
   for (int k = 0; k < mine_of_all; ++k) {
@@ -881,14 +889,16 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads)
         asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(mapa_shared(smem_u32(&of_target[turn]), c)), "f"(v)
                      : "memory");
     };
-    auto ask = [&](int c) { Chunk::ask(slots, x + first + c * kChunk * kN, packs - c * kChunk, tid); };
+    auto ask = [&](int c) {
+      Chunk::ask(slots, x + first + c * kChunk * kN, min(packs - c * kChunk, kChunk), tid);
+    };
     Chunk mine;
     Slope now;
     if (kMode == kTurn) {
       const float by = w * f.more[2];
       now = {f.more[0], by, -by / f.more[1], target};
       for (int c = 0; c < a.chunks; ++c) {
-        const int left = packs - c * kChunk, at = first + c * kChunk * kN;
+        const int left = min(packs - c * kChunk, kChunk), at = first + c * kChunk * kN;
         mine.take(slots, left, tid);
         if (c + 1 < a.chunks) {
           ask(c + 1);
@@ -902,7 +912,7 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads)
     } else {
       Softmax s = {-INFINITY, 0.f};
       for (int c = 0; c < a.chunks; ++c) {
-        const int left = packs - c * kChunk;
+        const int left = min(packs - c * kChunk, kChunk);
         mine.take(slots, left, tid);
         if (c + 1 < a.chunks)
           ask(c + 1);
@@ -911,7 +921,7 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads)
         else
           ask_row(facts[(k + 1) & 3]);
         if (clerk && c == 0) describe();
-        mine.add_to(s, left);
+        if (warp * kWarpPacks < left) mine.add_to(s);
         const int at = target - (first + c * kChunk * kN);
         if (Chunk::holds(at, left, tid)) tell_target(mine.value(at));
       }
@@ -951,7 +961,7 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads)
       now = said;
 #pragma unroll 1
       for (int c = a.chunks - 1; c >= 0; --c) {  // (the last is still held)
-        const int left = packs - c * kChunk, at = first + c * kChunk * kN;
+        const int left = min(packs - c * kChunk, kChunk), at = first + c * kChunk * kN;
         if (c + 1 < a.chunks) {
           mine.take(slots, left, tid);
           if (c > 0)
