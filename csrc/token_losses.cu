@@ -442,7 +442,8 @@ __device__ __forceinline__ Softmax join_rows(Softmax a, Softmax b) {
 }
 // of a warp's lanes
 __device__ __forceinline__ Softmax row_of_lanes(Softmax s) {
-  const float m = warp_max(s.most);
+  float m;
+  asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(m) : "f"(s.most));
   return {m, warp_sum(s.sum * exp2_approx(shift_of(s.most, m)))};
 }
 __device__ __forceinline__ float log_prob_of(float x, Softmax s) {
@@ -946,17 +947,20 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads)
         cluster_sync_all();
         if (warp == 0) s = row_of_lanes(lane < ctas ? of_cta[turn][lane] : Softmax{-INFINITY, 0.f});
       }
+      PolicyToken token = {};
       if (tid == 0) {
         const float logp = log_prob_of(target >= 0 ? of_target[turn] : NAN, s);
-        const PolicyToken c = policy_token(a.policy, {f.more[0], f.more[1], f.more[2]}, logp);
-        sums[0] += static_cast<double>(w) * c.loss;
-        sums[1] += static_cast<double>(w) * c.kl;
-        sums[2] += static_cast<double>(w) * c.clipped;
-        sums[3] += w;
-        const float by = w * c.slope * scale;
+        token = policy_token(a.policy, {f.more[0], f.more[1], f.more[2]}, logp);
+        const float by = w * token.slope * scale;
         said = {s.most, by, -by / s.sum, target};
       }
       __syncthreads();  // (`part` is read, `said` is there; nobody writes it before all are past the next row's first)
+      if (tid == 0) {
+        sums[0] += static_cast<double>(w) * token.loss;
+        sums[1] += static_cast<double>(w) * token.kl;
+        sums[2] += static_cast<double>(w) * token.clipped;
+        sums[3] += w;
+      }
       if (grad == nullptr) continue;
       now = said;
 #pragma unroll 1
