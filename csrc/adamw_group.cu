@@ -185,6 +185,13 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
       : "l"(*reinterpret_cast<uint64_t*>(&a)), "l"(*reinterpret_cast<uint64_t*>(&b)));
   return *reinterpret_cast<float2*>(&d);
 }
+__device__ __forceinline__ float2 add2_down(float2 a, float2 b) {  // (rounded toward zero)
+  uint64_t d;
+  asm("add.rz.ftz.f32x2 %0, %1, %2;"
+      : "=l"(d)
+      : "l"(*reinterpret_cast<uint64_t*>(&a)), "l"(*reinterpret_cast<uint64_t*>(&b)));
+  return *reinterpret_cast<float2*>(&d);
+}
 __device__ __forceinline__ float2 both(float x) { return make_float2(x, x); }
 
 // a / b to the nearest from inv = 1 / b to the nearest: Markstein's correction (IBM J. Res. Dev. 34, 1990).
@@ -225,7 +232,8 @@ __device__ __forceinline__ uint32_t abs_bits(float x) { return __float_as_uint(x
 // of `noise`): e4m3 keeps three of the 23 bits of the mantissa, so the bits that fall away are topped
 // up by a random number below one step before they are cut off. Below 2^-6 the steps are 2^-9 wide;
 // with 2^-6 added the value lies among numbers whose steps are the same, and what is left when it is
-// taken off again is exact. kSecond: no sign, and nothing is stored as zero (the caller sees to zeros).
+// taken off again is exact. (That sum drops bits below those of the draw, which cannot carry: rounded to the
+// nearest it moved one in 60 million values across a border.) kSecond: no sign, and nothing is stored as zero (the caller sees to zeros).
 // (A largest that is not finite makes the whole block NaN when it is read back, as it is kept itself.)
 template <bool kSecond>
 __device__ __forceinline__ uint32_t codes2(float2 x, float most, float inv, uint32_t noise0, uint32_t noise1) {
@@ -236,7 +244,7 @@ __device__ __forceinline__ uint32_t codes2(float2 x, float most, float inv, uint
     return fabsf(v) < 0.015625f ? by : 0.f;
   };
   const float2 c = make_float2(shift(y.x), shift(y.y));
-  float2 z = add2(y, c);
+  float2 z = add2_down(y, c);
   z.x = __uint_as_float((__float_as_uint(z.x) + noise0 + 8u) & 0xfff00000u);
   z.y = __uint_as_float((__float_as_uint(z.y) + noise1 + 8u) & 0xfff00000u);
   z = fma2(c, both(-1.f), z);

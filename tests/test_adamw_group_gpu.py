@@ -255,3 +255,20 @@ def test_another_stream_and_a_captured_step():
   graph.replay()
   for a, b in zip(leaves(replayed.target), leaves(want.target)):
     assert torch.equal(a, b)
+
+
+def test_draws_next_to_their_border():
+  """First moments among the numbers whose steps are the same, each some 2^-22 of a step below the place from which
+  its draw rounds it up: every code is that of the formula, whose sum of value and draw is exact in 64 bits."""
+  n, seed = 64 * 256, 9
+  up = ((optimizers._moment_noise(n, seed, 1, "cuda") & 0xFFFF).double() + 0.5) / 65536
+  g = ((2 - up - 2.0 ** -22) * 2.0 ** -9 / 448).float()
+  g[::256] = 1.0
+  opt = optimizers.chain([optimizers._adamw8(1e-3, seed=seed)]).create({"a": {"w": torch.zeros(n, device="cuda")}})
+  got = leaves(adam_of(opt.apply_gradient({"a": {"w": g}}))["mu"])[0]
+  m = ((1 - 0.9) * g).view(-1, 256)
+  y = m / m.amax(1, keepdim=True) * 448  # (rounded as before the draw)
+  small = y < 2.0 ** -6
+  want = torch.floor(y.double() * 2.0 ** 9 + up.view(-1, 256)) * 2.0 ** -9
+  assert int(small.sum()) == 64 * 255 and float((want[small] == 2.0 ** -9).double().mean()) > 0.2
+  assert torch.equal(got.view(torch.float8_e4m3fn).double().view(-1, 256)[small], want[small])
