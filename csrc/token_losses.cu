@@ -638,16 +638,23 @@ struct Pieces {
   float* of_target;   // NaN: outside of the vocabulary
   Softmax* of_row;
 
-  // The row's softmax, kept, and its target's log-probability.
-  __device__ __forceinline__ float log_prob(long long row) const {
+  // The row's softmax, kept, and its target's log-probability: in 64 bits, as the margin is a difference of two
+  // differences of sums of hundreds of them.
+  __device__ __forceinline__ double log_prob(long long row) const {
     const Softmax* of = of_piece + (row << shift);
-    Softmax s = {-INFINITY, 0.f};
+    float most = -INFINITY;
 #pragma unroll 4
-    for (int k = 0; k < 1 << shift; ++k) s.most = fmaxf(s.most, of[k].most);
+    for (int k = 0; k < 1 << shift; ++k) most = fmaxf(most, of[k].most);
+    double sum = 0.0;
 #pragma unroll 4
-    for (int k = 0; k < 1 << shift; ++k) s.sum += of[k].sum * exp2_approx(shift_of(of[k].most, s.most));
-    of_row[row] = s;
-    return log_prob_of(of_target[row], s);
+    for (int k = 0; k < 1 << shift; ++k)
+      sum += static_cast<double>(of[k].sum) * exp2_approx(shift_of(of[k].most, most));
+    of_row[row] = {most, static_cast<float>(sum)};
+    const double x = of_target[row];
+    if (most == -INFINITY) return NAN;
+    // (with the same reference as the exponentials in the sum)
+    const double d = huge(most) ? x - most : (x * kLog2e - __fmul_rn(most, kLog2e)) * 0.69314718055994531;
+    return d - log1p(sum - 1.0);
   }
 };
 
@@ -715,7 +722,7 @@ __global__ void __launch_bounds__(kRowThreads)
     for (int t = threadIdx.x; t < r.length; t += kRowThreads) {
       const float w = r.weights != nullptr ? r.weights[first + t] : 1.f;
       if (w != 0.f) {
-        sum[side] += static_cast<double>(w) * (logp != nullptr ? logp[first + t] : pieces.log_prob(first + t));
+        sum[side] += w * (logp != nullptr ? static_cast<double>(logp[first + t]) : pieces.log_prob(first + t));
         seen = 1.0;
       }
     }
