@@ -10,9 +10,12 @@
 // doing anything; the Python wrappers then take their general path, which handles or rejects the call.
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/extension.h>
 
 #include <algorithm>
+#include <functional>
+#include <memory>
 #include <optional>
 #include <string>
 #include <tuple>
@@ -912,66 +915,6 @@ Tensor gradient_like(const Tensor& x) {
 
 Tensor bytes_like(const Tensor& x, int64_t n) { return at::empty({n}, x.options().dtype(at::kByte)); }
 
-// loss, kl, clipped, weight, gradient (undefined unless wanted); nothing where the call is not covered
-std::vector<Tensor> policy_loss(const Tensor& x, const optional<Tensor>& targets, const optional<Tensor>& weights,
-                                const Tensor& old, const Tensor& advantages, const optional<Tensor>& reference,
-                                double clip_low, double clip_high, double kl_weight, double scale,
-                                const optional<Tensor>& normalizer, bool wanted) {
-  const LossValues s(x, targets);
-  if (!s.ok || !s.of(x, weights) || !s.of(x, old, at::kFloat) || !s.of(x, reference) || !scalar(x, normalizer) ||
-      advantages.scalar_type() != at::kFloat || advantages.device() != x.device() || advantages.dim() < 1 ||
-      advantages.dim() > 2 || advantages.size(0) != s.b)
-    return {};
-  int64_t adv_t = 0;
-  if (advantages.dim() == 2 && advantages.size(1) != 1) {
-    if (advantages.size(1) != s.l) return {};
-    adv_t = advantages.stride(1);
-  }
-  Tensor grad = wanted ? gradient_like(x) : Tensor();
-  void* g = wanted ? grad.data_ptr() : nullptr;
-  Tensor scratch = bytes_like(x, t5x_policy_loss_scratch_bytes());
-  Tensor out = at::empty({4}, x.options().dtype(at::kFloat));
-  const float low = clip_low, high = clip_high, kl = kl_weight, by = scale;
-  void* st = stream_of();
-  check(targets ? t5x_policy_loss(x.data_ptr(), s.fp32, g, s.b, s.l, s.v, s.stride_b, s.stride_t, targets->data_ptr(),
-                                  data_of(weights), old.data_ptr(), data_of(reference), advantages.data_ptr(),
-                                  advantages.stride(0), adv_t, low, high, kl, by, data_of(normalizer),
-                                  scratch.data_ptr(), out.data_ptr(), st)
-                : t5x_policy_loss_tokens(x.data_ptr(), g, s.b, s.l, data_of(weights), old.data_ptr(),
-                                         data_of(reference), advantages.data_ptr(), advantages.stride(0), adv_t, low,
-                                         high, kl, by, data_of(normalizer), scratch.data_ptr(), out.data_ptr(), st),
-        "policy_loss");
-  // (the loss, which users add to in place, is not a view to autograd)
-  return {out.select(0, 0).variable_data(), out.select(0, 1), out.select(0, 2), out.select(0, 3), grad};
-}
-
-// loss, scores, margins, pairs, gradient (undefined unless wanted); nothing where the call is not covered
-std::vector<Tensor> preference_loss(const Tensor& x, const optional<Tensor>& targets, const optional<Tensor>& weights,
-                                    const Tensor& reference, double beta, double smoothing, double scale,
-                                    const optional<Tensor>& normalizer, bool wanted) {
-  const LossValues s(x, targets);
-  if (!s.ok || !s.of(x, weights) || !scalar(x, normalizer) || reference.scalar_type() != at::kFloat ||
-      reference.device() != x.device() || reference.dim() != 1 || reference.size(0) != s.b ||
-      !reference.is_contiguous())
-    return {};
-  Tensor grad = wanted ? gradient_like(x) : Tensor();
-  void* g = wanted ? grad.data_ptr() : nullptr;
-  Tensor scratch = bytes_like(x, t5x_preference_loss_scratch_bytes(s.b, s.l, s.v, s.fp32));
-  const auto floats = x.options().dtype(at::kFloat);
-  Tensor out = at::empty({2}, floats), scores = at::empty({s.b}, floats), margins = at::empty({s.b / 2}, floats);
-  const float b = beta, e = smoothing, by = scale;
-  void* st = stream_of();
-  check(targets ? t5x_preference_loss(x.data_ptr(), s.fp32, g, s.b, s.l, s.v, s.stride_b, s.stride_t,
-                                      targets->data_ptr(), data_of(weights), reference.data_ptr(), b, e, by,
-                                      data_of(normalizer), scratch.data_ptr(), scores.data_ptr(), margins.data_ptr(),
-                                      out.data_ptr(), st)
-                : t5x_preference_loss_tokens(x.data_ptr(), g, s.b, s.l, data_of(weights), reference.data_ptr(), b, e,
-                                             by, data_of(normalizer), scratch.data_ptr(), scores.data_ptr(),
-                                             margins.data_ptr(), out.data_ptr(), st),
-        "preference_loss");
-  return {out.select(0, 0).variable_data(), scores, margins, out.select(0, 1), grad};
-}
-
 // grad * factor, in place or, with `keep`, in memory of its own
 optional<Tensor> scale_gradient(const Tensor& grad, const Tensor& factor, bool keep) {
   if (!grad.is_cuda() || grad.get_device() != c10::cuda::current_device() || !scalar(grad, factor) ||
@@ -984,6 +927,113 @@ optional<Tensor> scale_gradient(const Tensor& grad, const Tensor& factor, bool k
                            factor.data_ptr(), stream_of()),
         "scale_gradient");
   return to;
+}
+
+// The node of a loss in the autograd graph: the kernels have made the gradient along with the loss, backward
+// multiplies it by the gradient of the loss. In C++ the backward pass of a small loss need not wait for the GIL.
+struct LossNode : torch::autograd::Function<LossNode> {
+  using List = torch::autograd::variable_list;
+  using Run = std::function<std::vector<Tensor>(bool)>;  // (gradient wanted?) -> loss, three values, gradient
+
+  static List forward(torch::autograd::AutogradContext* ctx, const Tensor& values, const Run* run) {
+    std::vector<Tensor> out = (*run)(true);
+    ctx->save_for_backward({out[4]});
+    ctx->mark_non_differentiable({out[1], out[2], out[3]});
+    ctx->set_materialize_grads(false);
+    out.resize(4);
+    return out;
+  }
+  static List backward(torch::autograd::AutogradContext* ctx, List by) {
+    if (!by[0].defined()) return {Tensor(), Tensor()};
+    const Tensor grad = ctx->get_saved_variables()[0];
+    const bool twice = at::GradMode::is_enabled() && by[0].requires_grad();
+    optional<Tensor> out;
+    {
+      at::NoGradGuard no_grad;
+      const Tensor factor = by[0].to(grad.options().dtype(at::kFloat));
+      out = scale_gradient(grad, factor, torch::autograd::get_current_graph_task_keep_graph());
+    }
+    if (!out) throw std::runtime_error("backward of a loss on another device than its values");
+    if (!twice) return {*out, Tensor()};
+    // (a second derivative is refused where it is asked for)
+    Tensor refused = out->detach();
+    refused.set_requires_grad(true);
+    auto error = std::make_shared<torch::autograd::DelayedError>(
+        "trying to differentiate twice a loss whose gradient is made along with it", 1);
+    return {(*error)({refused})[0], Tensor()};
+  }
+};
+
+// loss and three values; nothing where the call is not covered
+std::vector<Tensor> run_loss(const Tensor& x, const LossNode::Run& run) {
+  if (at::GradMode::is_enabled() && x.requires_grad()) return LossNode::apply(x, &run);
+  std::vector<Tensor> out = run(false);
+  out.resize(4);
+  return out;
+}
+
+// loss, kl, clipped, weight; nothing where the call is not covered
+std::vector<Tensor> policy_loss(const Tensor& x, const optional<Tensor>& targets, const optional<Tensor>& weights,
+                                const Tensor& old, const Tensor& advantages, const optional<Tensor>& reference,
+                                double clip_low, double clip_high, double kl_weight, double scale,
+                                const optional<Tensor>& normalizer) {
+  const LossValues s(x, targets);
+  if (!s.ok || !s.of(x, weights) || !s.of(x, old, at::kFloat) || !s.of(x, reference) || !scalar(x, normalizer) ||
+      advantages.scalar_type() != at::kFloat || advantages.device() != x.device() || advantages.dim() < 1 ||
+      advantages.dim() > 2 || advantages.size(0) != s.b)
+    return {};
+  int64_t adv_t = 0;
+  if (advantages.dim() == 2 && advantages.size(1) != 1) {
+    if (advantages.size(1) != s.l) return {};
+    adv_t = advantages.stride(1);
+  }
+  return run_loss(x, [&](bool wanted) -> std::vector<Tensor> {
+    Tensor grad = wanted ? gradient_like(x) : Tensor();
+    void* g = wanted ? grad.data_ptr() : nullptr;
+    Tensor scratch = bytes_like(x, t5x_policy_loss_scratch_bytes());
+    Tensor out = at::empty({4}, x.options().dtype(at::kFloat));
+    const float low = clip_low, high = clip_high, kl = kl_weight, by = scale;
+    void* st = stream_of();
+    check(targets ? t5x_policy_loss(x.data_ptr(), s.fp32, g, s.b, s.l, s.v, s.stride_b, s.stride_t, targets->data_ptr(),
+                                    data_of(weights), old.data_ptr(), data_of(reference), advantages.data_ptr(),
+                                    advantages.stride(0), adv_t, low, high, kl, by, data_of(normalizer),
+                                    scratch.data_ptr(), out.data_ptr(), st)
+                  : t5x_policy_loss_tokens(x.data_ptr(), g, s.b, s.l, data_of(weights), old.data_ptr(),
+                                           data_of(reference), advantages.data_ptr(), advantages.stride(0), adv_t, low,
+                                           high, kl, by, data_of(normalizer), scratch.data_ptr(), out.data_ptr(), st),
+          "policy_loss");
+    // (the loss, which users add to in place, is not a view to autograd)
+    return {out.select(0, 0).variable_data(), out.select(0, 1), out.select(0, 2), out.select(0, 3), grad};
+  });
+}
+
+// loss, scores, margins, pairs; nothing where the call is not covered
+std::vector<Tensor> preference_loss(const Tensor& x, const optional<Tensor>& targets, const optional<Tensor>& weights,
+                                    const Tensor& reference, double beta, double smoothing, double scale,
+                                    const optional<Tensor>& normalizer) {
+  const LossValues s(x, targets);
+  if (!s.ok || !s.of(x, weights) || !scalar(x, normalizer) || reference.scalar_type() != at::kFloat ||
+      reference.device() != x.device() || reference.dim() != 1 || reference.size(0) != s.b ||
+      !reference.is_contiguous())
+    return {};
+  return run_loss(x, [&](bool wanted) -> std::vector<Tensor> {
+    Tensor grad = wanted ? gradient_like(x) : Tensor();
+    void* g = wanted ? grad.data_ptr() : nullptr;
+    Tensor scratch = bytes_like(x, t5x_preference_loss_scratch_bytes(s.b, s.l, s.v, s.fp32));
+    const auto floats = x.options().dtype(at::kFloat);
+    Tensor out = at::empty({2}, floats), scores = at::empty({s.b}, floats), margins = at::empty({s.b / 2}, floats);
+    const float b = beta, e = smoothing, by = scale;
+    void* st = stream_of();
+    check(targets ? t5x_preference_loss(x.data_ptr(), s.fp32, g, s.b, s.l, s.v, s.stride_b, s.stride_t,
+                                        targets->data_ptr(), data_of(weights), reference.data_ptr(), b, e, by,
+                                        data_of(normalizer), scratch.data_ptr(), scores.data_ptr(), margins.data_ptr(),
+                                        out.data_ptr(), st)
+                  : t5x_preference_loss_tokens(x.data_ptr(), g, s.b, s.l, data_of(weights), reference.data_ptr(), b, e,
+                                               by, data_of(normalizer), scratch.data_ptr(), scores.data_ptr(),
+                                               margins.data_ptr(), out.data_ptr(), st),
+          "preference_loss");
+    return {out.select(0, 0).variable_data(), scores, margins, out.select(0, 1), grad};
+  });
 }
 
 }  // namespace
@@ -1014,6 +1064,5 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("relu_block_bwd", torch::wrap_pybind_function_no_gil(relu_block_bwd));
   m.def("policy_loss", torch::wrap_pybind_function_no_gil(policy_loss));
   m.def("preference_loss", torch::wrap_pybind_function_no_gil(preference_loss));
-  m.def("scale_gradient", torch::wrap_pybind_function_no_gil(scale_gradient));
   m.def("adamw_tree", adamw_tree);  // (it reads Python's dicts, and releases the GIL for the launches)
 }

@@ -134,7 +134,7 @@ class _HostOps:
            "rmsnorm_bwd", "attention", "attention_bwd", "attention_block_ok", "attention_grads_ok",
            "attention_block", "attention_block_bwd", "mlp_block_ok", "mlp_grads_ok", "mlp_block",
            "mlp_block_bwd", "relu_block_ok", "relu_grads_ok", "relu_block", "relu_block_bwd",
-           "adamw_tree", "policy_loss", "preference_loss", "scale_gradient")
+           "adamw_tree", "policy_loss", "preference_loss")
 
   def __init__(self, module):
     for name in self.NAMES:

@@ -44,29 +44,29 @@ def _times(grad: torch.Tensor, factor: Optional[torch.Tensor]) -> Optional[torch
   """The saved gradient times the gradient of the loss; None where there is none."""
   if factor is None:
     return None
-  keep, host = F._graph_is_kept(), native.host()
-  if host is not None:
-    out = host.scale_gradient(grad, factor, keep)
-    if out is not None:
-      return out
-  return native.scale_gradient(grad, factor.detach().float().reshape(1), keep=keep)
+  return native.scale_gradient(grad, factor.detach().float().reshape(1), keep=F._graph_is_kept())
 
 
 def _loss(ctx, name, values, targets, *args):
   """The outputs of the kernels' loss `name`; its gradient is kept with the graph where it will be wanted."""
   want = not isinstance(ctx, F._NoGraph) and ctx.needs_input_grad[0]
-  host = native.host()
-  out = host and getattr(host, name)(values, targets, *args, want)
-  if out:
-    *out, grad = out
-  else:
-    values = values.contiguous() if targets is None else _rows_apart(values)
-    grad = _like(values) if want else None
-    out = getattr(native, name)(values, grad, targets, *args)
+  values = values.contiguous() if targets is None else _rows_apart(values)
+  grad = _like(values) if want else None
+  out = getattr(native, name)(values, grad, targets, *args)
   ctx.save_for_backward(grad)
   ctx.mark_non_differentiable(*out[1:])
   ctx.set_materialize_grads(False)
-  return tuple(out)
+  return out
+
+
+def _run(fn, name, *args):
+  """The loss by the compiled host path, which makes its own node of the graph, or else by `fn`."""
+  host = native.host()
+  if host is not None and not F._transformed():
+    out = getattr(host, name)(*args)
+    if out:
+      return tuple(out)
+  return F._apply(fn, *args)
 
 
 class _PolicyFn(torch.autograd.Function):
@@ -124,8 +124,8 @@ def policy_loss(values, targets, weights, old, advantages, reference, clip_low, 
     return ref.policy_loss(logp, weights, old, advantages, reference, clip_low, clip_high, kl_weight,
                            normalizer)
   scale, divisor = _divisor(normalizer, values.device)
-  return F._apply(_PolicyFn, values, _plain(targets, torch.int64), _plain(weights), _plain(old),
-                  _plain(advantages), _plain(reference), clip_low, clip_high, kl_weight, scale, divisor)
+  return _run(_PolicyFn, "policy_loss", values, _plain(targets, torch.int64), _plain(weights), _plain(old),
+              _plain(advantages), _plain(reference), clip_low, clip_high, kl_weight, scale, divisor)
 
 
 def preference_loss(values, targets, weights, reference, beta, label_smoothing, normalizer):
@@ -138,5 +138,5 @@ def preference_loss(values, targets, weights, reference, beta, label_smoothing, 
     logp = values if targets is None else ref.token_log_probs(values, targets, weights)
     return ref.preference_loss(logp, weights, reference, beta, label_smoothing, normalizer)
   scale, divisor = _divisor(normalizer, values.device)
-  return F._apply(_PreferenceFn, values, _plain(targets, torch.int64), _plain(weights),
-                  _plain(reference), beta, label_smoothing, scale, divisor)
+  return _run(_PreferenceFn, "preference_loss", values, _plain(targets, torch.int64), _plain(weights),
+              _plain(reference), beta, label_smoothing, scale, divisor)

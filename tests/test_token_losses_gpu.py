@@ -341,3 +341,40 @@ def test_offsets_beyond_32_bits():
     leaf = view.detach().requires_grad_()
     out = call(kind, leaf, d, None)
     check(kind, out, torch.autograd.grad(out[0], leaf)[0], d, 1.0)
+
+
+@pytest.mark.parametrize("host", ["1", "0"])
+@pytest.mark.parametrize("kind", ["preference", "policy"])
+def test_loss_in_a_larger_graph(kind, host, monkeypatch):
+  """Added to in place, used twice, scaled by something that has a gradient itself; a second derivative is refused."""
+  from t5x_b200.ops import native
+  monkeypatch.setenv("T5X_B200_HOST_OPS", host)
+  monkeypatch.setattr(native, "_host", None)
+  d = data(4, 6, 700, torch.float32, 5)
+  x = d["x"].clone().requires_grad_()
+  base = torch.autograd.grad(call(kind, x, d, 2.0)[0], x)[0]
+  scale = torch.tensor(3.0, device="cuda", requires_grad=True)
+  out = call(kind, x, d, 2.0)
+  value = float(out[0])
+  loss = out[0]
+  loss += 1.0
+  gx, gs = torch.autograd.grad(loss * scale + 0.5 * loss, (x, scale))
+  # (two products of 32 bits a value: 2^-23)
+  assert torch.allclose(gx, base * 3.5, rtol=2 ** -22, atol=0) and float(gs) == pytest.approx(value + 1, rel=1e-6)
+  assert not any(o.requires_grad for o in out[1:])
+  gx = torch.autograd.grad(call(kind, x, d, 2.0)[0] * scale, x, create_graph=True)[0]
+  with pytest.raises(RuntimeError, match="twice"):
+    gx.sum().backward()
+
+
+@pytest.mark.parametrize("kind", ["preference", "policy"])
+def test_frozen_logits_and_inputs_with_gradients(kind):
+  """Without a gradient of the logits no graph is built, and inputs beside them get none."""
+  d = data(2, 5, 1500, torch.bfloat16, 6)
+  out = call(kind, d["x"], d, None)
+  assert not any(o.requires_grad for o in out)
+  e = dict(d, w=d["w"].clone().requires_grad_(), r=d["r"].clone().requires_grad_(), old=d["old"].clone().requires_grad_())
+  assert not any(o.requires_grad for o in call(kind, d["x"], e, None))
+  x = d["x"].clone().requires_grad_()
+  got = torch.autograd.grad(call(kind, x, e, None)[0], [x, e["w"]], allow_unused=True)
+  assert got[1] is None and torch.equal(got[0], torch.autograd.grad(call(kind, x, d, None)[0], x)[0])
