@@ -31,7 +31,7 @@ namespace {
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kRowThreads = 512;
-constexpr int kCtasPerSm = 8;  // at most, of every grid here whose CTAs leave sums in the scratch
+constexpr int kCtasPerSm = 16;  // at most, of every grid here whose CTAs leave sums in the scratch
 
 __device__ __forceinline__ float exp2_approx(float x) {
   float r;
@@ -418,8 +418,14 @@ __global__ void __launch_bounds__(kRowThreads)
 // next row is on its way into shared memory meanwhile. Larger rows than eight CTAs hold go by in chunks, which
 // are read a second time for the gradient.
 //
-// What bounds it: memory, and close behind that the instructions. So one thread finds out about the rows, a
-// few of them ahead, and leaves that for all in shared memory.
+// What bounds it: memory. Policy, 128 x 114 x 32128 bf16 of which 80% count: 315 us, 5.4 TB/s of what has to be read
+// and written; 7 x 189 x 250112 fp32: 419 us, 5.7 TB/s; the gradients of a preference loss, 64 x 114 x 32128 bf16: 137
+// us, 6.2 TB/s. Close behind come the instructions (60% of the issue slots, the exponentials' unit 54%), and a policy
+// row has a chain from its last part to its slope that the SM's other CTA has to fill. So one thread finds out about
+// the rows, a few of them ahead, and leaves that for all in shared memory (488 us where all of them did), a warp's
+// share lies side by side, and what the loss itself needs is added behind the slope. Tried without effect: 256
+// threads with twice the registers; the next row asked for in four groups; a quarter of the exponentials as
+// polynomials (325).
 constexpr int kPacks = 8;
 
 // An exponential exp(x - most) is exp2(x log2 e - ref) here, a fused product and difference, with ref =
@@ -785,7 +791,8 @@ struct alignas(16) RowFacts {
   int first, packs;   // the CTA's part: its first value, its number of 16 bytes
   long long target;
   float weight;
-  alignas(16) float more[4];  // policy: old score, reference score, advantage; gradients: softmax, slope of the sequence
+  // policy: old score, reference score, advantage; gradients: softmax, slope of the sequence
+  alignas(16) float more[4];
 };
 
 template <typename T, int kThreads, int kMode>
@@ -1026,12 +1033,15 @@ __global__ void __launch_bounds__(256)
 }
 
 // ---- host ----
-// Shorter rows are a warp's each.
-constexpr long long kLongRow = 4096;
+// Shorter rows are a warp's each. Policy, a warp and a CTA a row, us: 403 and 531 for 262144 rows of 4 KB fp32, 302
+// and 300 for 131072 of 6 KB, 425 and 403 of 8 KB, 242 and 221 for 65536 of 8 KB bf16, 333 and 249 of 10 KB fp32.
+// Preference, whose three launches do not wait for a row's slope: 542 and 541 for 4 KB, 409 and 398 for 6 KB, 314 and
+// 231 for 65536 of 6 KB bf16, 541 and 532 for 131072 of 8 KB fp32; 604 and 1032 for 524288 of 2 KB.
+constexpr long long kLongPolicyRow = 6144, kLongRow = 4096;
 
 int check_rows(const char* what, const void* logits, int fp32, const void* grad, long long batch, int length,
                int vocab, long long stride_b, long long stride_t, const void* targets) {
-  if (batch < 0 || length < 0 || vocab < 1) return set_error("%s: bad sizes", what);
+  if (batch < 0 || length < 0 || vocab < 1 || vocab > (1 << 30)) return set_error("%s: bad sizes", what);
   if (batch > 0 && length > 0 && (logits == nullptr || targets == nullptr))
     return set_error("%s: null pointer", what);
   const uintptr_t size = fp32 ? 4 : 2;
@@ -1103,10 +1113,15 @@ int launch_long(const char* what, const void* logits, void* grad, const Rows& r,
   return launched(what, 1);
 }
 
-// The smallest CTA that holds the row, so that short ones leave the SM room for many.
+// The smallest CTA that holds the row, so that short ones leave the SM room for many (512 threads for all of them:
+// 1237 in the place of 383 us for 131072 policy rows of 8 KB, 636 and not 403 for 65536 of 16 KB). 64 threads for the
+// policy alone: 221 and not 283 us for 65536 rows of 8 KB bf16; gradients alone lose by it, 353 and 360 us for 262144
+// rows of 4 KB.
 template <typename T, int kMode>
 int launch_long(const char* what, const void* logits, void* grad, const Rows& r, const LongArgs& a, cudaStream_t st) {
   const long long bytes = static_cast<long long>(r.vocab) * sizeof(T);
+  if constexpr (kMode == kPolicy)
+    if (bytes <= 64 * kPacks * 16) return launch_long<T, 64, kMode>(what, logits, grad, r, a, st);
   if (bytes <= 128 * kPacks * 16) return launch_long<T, 128, kMode>(what, logits, grad, r, a, st);
   if (bytes <= 256 * kPacks * 16) return launch_long<T, 256, kMode>(what, logits, grad, r, a, st);
   return launch_long<T, 512, kMode>(what, logits, grad, r, a, st);
@@ -1160,7 +1175,7 @@ T5X_API int t5x_policy_loss(const void* logits, int fp32, void* grad, long long 
                     static_cast<const float*>(advantages), adv_b, adv_t, 1.f - clip_low, 1.f + clip_high,
                     kl_weight, scale, static_cast<const float*>(normalizer)};
   float* o = static_cast<float*>(out);
-  if (static_cast<long long>(vocab) * (fp32 ? 4 : 2) >= kLongRow && r.rows > 0) {
+  if (static_cast<long long>(vocab) * (fp32 ? 4 : 2) >= kLongPolicyRow && r.rows > 0) {
     LongArgs a = {};
     a.policy = p;
     a.partial = partial;

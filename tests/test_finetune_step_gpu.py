@@ -1,5 +1,5 @@
-"""A step of preference and of policy fine-tuning as a user writes it: reference scores from `score_batch`, the loss over
-the model's logits or behind the fused projection, its backward pass, clipping and AdamW with 8-bit moments."""
+"""A step of preference and of policy fine-tuning as a user writes it: reference scores from `score_batch`, the loss
+over the model's logits or behind the fused projection, its backward pass, clipping and AdamW with 8-bit moments."""
 import pytest
 import torch
 
@@ -18,7 +18,8 @@ def build():
       vocab_size=2112, dtype="bfloat16", emb_dim=128, num_heads=2, num_encoder_layers=1, num_decoder_layers=1,
       head_dim=64, mlp_dim=256, mlp_activations=("gelu", "linear"), dropout_rate=0.0), device="cuda")
   vocab = vocabularies.PassThroughVocabulary(2112)
-  definition = optimizers.chain([optimizers.clip_by_global_norm(0.5), optax_api.adamw8(1e-3, weight_decay=0.01, seed=3)])
+  definition = optimizers.chain([optimizers.clip_by_global_norm(0.5),
+                                 optax_api.adamw8(1e-3, weight_decay=0.01, seed=3)])
   model = models.EncoderDecoderModel(module, vocab, vocab, definition)
   params = base.module_param_tree(module)
   trainer.attach_compute_buffers(params, bf16_copy=True, main_grad=True)

@@ -103,8 +103,10 @@ def check(kind, out, grad, d, factor):
 
 
 SHAPES = [(2, 1, 1), (2, 1, 2), (2, 3, 7), (4, 5, 31), (2, 2, 33), (6, 9, 384), (4, 3, 385), (2, 4, 2047), (2, 3, 2048),
-          (4, 3, 2049), (2, 5, 4099), (2, 7, 32128), (4, 2, 32101), (2, 2, 65537), (2, 1, 250112), (2, 3, 530000), (10, 2, 8193), (6, 50, 16390), (2, 2, 131071), (2, 600, 40),
-          (40, 33, 100), (2, 40, 12345), (8, 150, 4100), (4, 300, 9001), (6, 120, 32101), (10, 100, 20000), (4, 25, 250112)]
+          (4, 3, 2049), (2, 5, 4099), (2, 7, 32128), (4, 2, 32101), (2, 2, 65537), (2, 1, 250112), (2, 3, 530000),
+          (10, 2, 8193), (6, 50, 16390), (2, 2, 131071), (2, 600, 40),
+          (40, 33, 100), (2, 40, 12345), (8, 150, 4100), (4, 300, 9001), (6, 120, 32101), (10, 100, 20000),
+          (4, 25, 250112)]
 
 
 @pytest.mark.parametrize("kind", ["preference", "policy"])
@@ -373,8 +375,28 @@ def test_frozen_logits_and_inputs_with_gradients(kind):
   d = data(2, 5, 1500, torch.bfloat16, 6)
   out = call(kind, d["x"], d, None)
   assert not any(o.requires_grad for o in out)
-  e = dict(d, w=d["w"].clone().requires_grad_(), r=d["r"].clone().requires_grad_(), old=d["old"].clone().requires_grad_())
+  e = dict(d, **{k: d[k].clone().requires_grad_() for k in ("w", "r", "old")})
   assert not any(o.requires_grad for o in call(kind, d["x"], e, None))
   x = d["x"].clone().requires_grad_()
   got = torch.autograd.grad(call(kind, x, e, None)[0], [x, e["w"]], allow_unused=True)
   assert got[1] is None and torch.equal(got[0], torch.autograd.grad(call(kind, x, d, None)[0], x)[0])
+
+
+def test_inference_mode():
+  d = data(2, 4, 2000, torch.bfloat16, 7)
+  want = call("policy", d["x"], d, None)
+  with torch.inference_mode():
+    got = call("policy", d["x"], d, None)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    assert torch.isfinite(call("preference", d["x"].clone(), d, None)[0])
+
+
+@pytest.mark.parametrize("kind", ["preference", "policy"])
+@pytest.mark.parametrize("dtype, vocab", [(torch.float32, 1800), (torch.bfloat16, 3501), (torch.float32, 1537),
+                                          (torch.bfloat16, 4096), (torch.float32, 2049)])
+def test_many_rows_of_some_kilobytes(kind, dtype, vocab):
+  """More rows than run at once, about the sizes at which a row passes from a warp to the smallest blocks."""
+  d = data(20, 150, vocab, dtype, seed=vocab)
+  x = d["x"].requires_grad_()
+  out = call(kind, x, d, 7.0)
+  check(kind, out, torch.autograd.grad(out[0], x)[0], d, 7.0)
