@@ -424,7 +424,7 @@ __global__ void __launch_bounds__(kRowThreads)
 // row has a chain from its last part to its slope that the SM's other CTA has to fill. So one thread finds out about
 // the rows, a few of them ahead, and leaves that for all in shared memory (488 us where all of them did), a warp's
 // share lies side by side, and what the loss itself needs is added behind the slope. Tried without effect: 256
-// threads with twice the registers; the next row asked for in four groups; a quarter of the exponentials as
+// threads with twice the registers; the next row asked for in four groups; an eighth of the exponentials as
 // polynomials (325).
 constexpr int kPacks = 8;
 
