@@ -418,14 +418,15 @@ __global__ void __launch_bounds__(kRowThreads)
 // next row is on its way into shared memory meanwhile. Larger rows than eight CTAs hold go by in chunks, which
 // are read a second time for the gradient.
 //
-// What bounds it: memory. Policy, 128 x 114 x 32128 bf16 of which 80% count: 315 us, 5.4 TB/s of what has to be read
-// and written; 7 x 189 x 250112 fp32: 419 us, 5.7 TB/s; the gradients of a preference loss, 64 x 114 x 32128 bf16: 137
+// What bounds it: memory. Policy, 128 x 114 x 32128 bf16 of which 80% count: 310 us, 5.4 TB/s of what has to be read
+// and written; 7 x 189 x 250112 fp32: 416 us, 5.7 TB/s; the gradients of a preference loss, 64 x 114 x 32128 bf16: 137
 // us, 6.2 TB/s. Close behind come the instructions (60% of the issue slots, the exponentials' unit 54%), and a policy
 // row has a chain from its last part to its slope that the SM's other CTA has to fill. So one thread finds out about
 // the rows, a few of them ahead, and leaves that for all in shared memory (488 us where all of them did), a warp's
 // share lies side by side, and what the loss itself needs is added behind the slope. Tried without effect: 256
 // threads with twice the registers; the next row asked for in four groups; an eighth of the exponentials as
-// polynomials (325).
+// polynomials (325); a row over two blocks of 256 threads (327); no second barrier, each warp joining the parts by
+// itself (332); exponentials kept for the gradient, by which one block of 512 threads fills an SM (370).
 constexpr int kPacks = 8;
 
 // An exponential exp(x - most) is exp2(x log2 e - ref) here, a fused product and difference, with ref =
@@ -929,6 +930,8 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads)
       for (int c = 0; c < a.chunks; ++c) {
         const int left = min(packs - c * kChunk, kChunk);
         mine.take(slots, left, tid);
+        const int at = target - (first + c * kChunk * kN);
+        if (Chunk::holds(at, left, tid)) tell_target(mine.value(at));
         if (c + 1 < a.chunks)
           ask(c + 1);
         else if (grad != nullptr && c > 0)
@@ -937,8 +940,6 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads)
           ask_row(facts[(k + 1) & 3]);
         if (clerk && c == 0) describe();
         if (warp * kWarpPacks < left) mine.add_to(s);
-        const int at = target - (first + c * kChunk * kN);
-        if (Chunk::holds(at, left, tid)) tell_target(mine.value(at));
       }
       if (outside >= 0) {
         s = join_rows(s, {x_outside, x_outside == -INFINITY ? 0.f : x_outside * 0.f + 1.f});  // (NaN of +inf, NaN)
