@@ -199,19 +199,30 @@ __device__ __forceinline__ long long row_at(const Rows& r, long long row) {
   return b * r.stride_b + (row - b * r.length) * r.stride_t;
 }
 
-// Sum over the threads of the CTA, in every thread, in a fixed order.
-template <int kThreads>
-__device__ __forceinline__ double cta_sum(double v) {
-  __shared__ double part[kThreads / 32];
+// Sums over the threads of the CTA, in every thread, in a fixed order.
+template <int kThreads, int kSums>
+__device__ __forceinline__ void cta_sums(double (&v)[kSums]) {
+  constexpr int kWarps = kThreads / 32;
+  __shared__ double part[kSums][kWarps];
+  const int lane = threadIdx.x & 31;
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  __syncthreads();
-  if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = v;
-  __syncthreads();
-  double t = 0.0;
+  for (int o = 16; o > 0; o >>= 1) {
 #pragma unroll
-  for (int i = 0; i < kThreads / 32; ++i) t += part[i];
-  return t;
+    for (int i = 0; i < kSums; ++i) v[i] += __shfl_xor_sync(0xffffffffu, v[i], o);
+  }
+  __syncthreads();
+  if (lane == 0) {
+#pragma unroll
+    for (int i = 0; i < kSums; ++i) part[i][threadIdx.x >> 5] = v[i];
+  }
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < kSums; ++i) v[i] = part[i][lane % kWarps];
+#pragma unroll
+  for (int o = kWarps / 2; o > 0; o >>= 1) {
+#pragma unroll
+    for (int i = 0; i < kSums; ++i) v[i] += __shfl_xor_sync(0xffffffffu, v[i], o);
+  }
 }
 
 // Whether this CTA is the last of the grid to come here; what the others wrote before is then visible.
@@ -268,23 +279,24 @@ __device__ __forceinline__ PolicyToken policy_token(const Policy& p, PolicyInput
 }
 
 // out: loss, kl, clipped, weight
-__device__ __forceinline__ void policy_finish(double* sums, const Policy& p, double* partial, unsigned* arrived,
+__device__ __forceinline__ void policy_finish(double (&sums)[4], const Policy& p, double* partial, unsigned* arrived,
                                               float* out) {
   constexpr int kThreads = kRowThreads;
+  cta_sums<kThreads>(sums);
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const double v = cta_sum<kThreads>(sums[i]);
-    if (threadIdx.x == 0) partial[blockIdx.x * 4 + i] = v;
-  }
+  for (int i = 0; i < 4; ++i)
+    if (threadIdx.x == 0) partial[blockIdx.x * 4 + i] = sums[i];
   if (!last_cta(arrived)) return;
   const double scale = p.normalizer != nullptr ? 1.0 / static_cast<double>(*p.normalizer) : p.scale;
+  double v[4] = {0.0, 0.0, 0.0, 0.0};
+  for (int k = threadIdx.x; k < static_cast<int>(gridDim.x); k += kThreads) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    double v = 0.0;
-    for (int k = threadIdx.x; k < static_cast<int>(gridDim.x); k += kThreads) v += __ldcg(partial + k * 4 + i);
-    v = cta_sum<kThreads>(v);
-    if (threadIdx.x == 0) out[i] = static_cast<float>(i < 2 ? v * scale : v);
+    for (int i = 0; i < 4; ++i) v[i] += __ldcg(partial + k * 4 + i);
   }
+  cta_sums<kThreads>(v);
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (threadIdx.x == 0) out[i] = static_cast<float>(i < 2 ? v[i] * scale : v[i]);
 }
 
 // Short rows, a warp each.
@@ -722,20 +734,21 @@ __global__ void __launch_bounds__(kRowThreads)
                             double* pair_loss, unsigned* arrived, float* out) {
   const long long pair = blockIdx.x;
   const float scale = scale_of(p.normalizer, p.scale);
-  double sum[2] = {0.0, 0.0}, seen = 0.0;
-#pragma unroll
-  for (int side = 0; side < 2; ++side) {
-    const long long first = (2 * pair + side) * r.length;
-    for (int t = threadIdx.x; t < r.length; t += kRowThreads) {
-      const float w = r.weights != nullptr ? r.weights[first + t] : 1.f;
-      if (w != 0.f) {
-        sum[side] += w * (logp != nullptr ? static_cast<double>(logp[first + t]) : pieces.log_prob(first + t));
-        seen = 1.0;
-      }
-    }
-    sum[side] = cta_sum<kRowThreads>(sum[side]);
+  double sum[3] = {0.0, 0.0, 0.0};  // of either answer, and whether any token counts
+  const long long first = 2 * pair * r.length;
+  const unsigned length = r.length;  // (at most 2^30)
+  for (unsigned t = threadIdx.x; t < 2 * length; t += kRowThreads) {
+    const float w = r.weights != nullptr ? r.weights[first + t] : 1.f;
+    if (w == 0.f) continue;
+    const double v = w * (logp != nullptr ? static_cast<double>(logp[first + t]) : pieces.log_prob(first + t));
+    if (t < length)
+      sum[0] += v;
+    else
+      sum[1] += v;
+    sum[2] = 1.0;
   }
-  const bool real = cta_sum<kRowThreads>(seen) > 0.0;
+  cta_sums<kRowThreads>(sum);
+  const bool real = sum[2] > 0.0;
   const Margin m = pair_margin(p, real, sum[0], sum[1], p.ref[2 * pair], p.ref[2 * pair + 1], scale);
   const float slope = m.slope;
   if (threadIdx.x == 0) {
@@ -761,16 +774,15 @@ __global__ void __launch_bounds__(kRowThreads)
   }
   if (!last_cta(arrived)) return;
   const double whole = p.normalizer != nullptr ? 1.0 / static_cast<double>(*p.normalizer) : p.scale;
-  double loss = 0.0, pairs = 0.0;
+  double all[2] = {0.0, 0.0};
   for (int k = threadIdx.x; k < static_cast<int>(gridDim.x); k += kRowThreads) {
-    loss += __ldcg(pair_loss + 2 * k);
-    pairs += __ldcg(pair_loss + 2 * k + 1);
+    all[0] += __ldcg(pair_loss + 2 * k);
+    all[1] += __ldcg(pair_loss + 2 * k + 1);
   }
-  loss = cta_sum<kRowThreads>(loss);
-  pairs = cta_sum<kRowThreads>(pairs);
+  cta_sums<kRowThreads>(all);
   if (threadIdx.x == 0) {
-    out[0] = static_cast<float>(loss * whole);
-    out[1] = static_cast<float>(pairs);
+    out[0] = static_cast<float>(all[0] * whole);
+    out[1] = static_cast<float>(all[1]);
   }
 }
 
@@ -1282,7 +1294,8 @@ T5X_API int t5x_preference_loss_tokens(const void* logp, void* slope, long long 
                                        const void* weights, const void* reference, float beta, float smoothing,
                                        float scale, const void* normalizer, void* scratch, void* scores,
                                        void* margins, void* out, void* stream) {
-  if (batch < 2 || batch % 2 || length < 0) return set_error("preference_loss_tokens: the batch must hold pairs");
+  if (batch < 2 || batch % 2) return set_error("preference_loss_tokens: the batch must hold pairs");
+  if (length < 0 || length > (1 << 30)) return set_error("preference_loss_tokens: bad sizes");
   if (!scratch || !out || !reference || !scores || !margins || (length > 0 && !logp))
     return set_error("preference_loss_tokens: null pointer");
   cudaStream_t st = static_cast<cudaStream_t>(stream);
