@@ -369,8 +369,9 @@ struct Preference {
 template <typename T>
 __global__ void __launch_bounds__(kRowThreads)
     preference_short_rows_kernel(const T* __restrict__ logits, const Rows r, Softmax* __restrict__ softmax,
-                                 float* __restrict__ logp) {
+                                 float* __restrict__ logp, unsigned* arrived) {
   const int lane = threadIdx.x & 31;
+  if (blockIdx.x == 0 && threadIdx.x == 0) *arrived = 0;  // for the launch of the pairs
   const long long warps = static_cast<long long>(gridDim.x) * (kRowThreads / 32);
   for (long long row = blockIdx.x * static_cast<long long>(kRowThreads / 32) + (threadIdx.x >> 5); row < r.rows;
        row += warps) {
@@ -681,9 +682,10 @@ constexpr int kPieceThreads = 256, kPieceCtas = 4;  // CTAs of an SM
 
 template <typename T>
 __global__ void __launch_bounds__(kPieceThreads, kPieceCtas)
-    preference_pieces_kernel(const T* __restrict__ logits, const Rows r, const Pieces p) {
+    preference_pieces_kernel(const T* __restrict__ logits, const Rows r, const Pieces p, unsigned* arrived) {
   constexpr int kN = Pack<T>::kN, kChunk = 32 * kPacks;
   const int lane = threadIdx.x & 31;
+  if (blockIdx.x == 0 && threadIdx.x == 0) *arrived = 0;  // for the launch of the pairs
   const long long warps = static_cast<long long>(gridDim.x) * (kPieceThreads / 32);
   const long long pieces = r.rows << p.shift;
   auto weight_of = [&](long long i) {
@@ -1149,12 +1151,12 @@ int piece_shift(long long bytes) {
 }
 
 template <typename T>
-int launch_pieces(const T* logits, const Rows& r, const Pieces& p, cudaStream_t st) {
+int launch_pieces(const T* logits, const Rows& r, const Pieces& p, unsigned* arrived, cudaStream_t st) {
   if (r.rows > (1 << 30)) return set_error("preference_loss: too many rows");
   const long long ctas = ((r.rows << p.shift) * 32 + kPieceThreads - 1) / kPieceThreads;
   const long long cap = static_cast<long long>(num_sms()) * kPieceCtas;  // as many as run at once
   preference_pieces_kernel<T>
-      <<<static_cast<unsigned>(ctas < cap ? ctas : cap), kPieceThreads, 0, st>>>(logits, r, p);
+      <<<static_cast<unsigned>(ctas < cap ? ctas : cap), kPieceThreads, 0, st>>>(logits, r, p, arrived);
   return launched("preference_loss", 1);
 }
 
@@ -1263,8 +1265,6 @@ T5X_API int t5x_preference_loss(const void* logits, int fp32, void* grad, long l
   float* logp = reinterpret_cast<float*>(pieces.of_piece + (in_long ? r.rows << pieces.shift : 0));
   pieces.of_target = logp;
   float* by = logp + r.rows;
-  cudaError_t e = cudaMemsetAsync(scratch, 0, kHead, st);
-  if (e != cudaSuccess) return set_error("preference_loss: memset: %s", cudaGetErrorString(e));
   auto go = [&](auto* x) {
     using T = std::remove_const_t<std::remove_pointer_t<decltype(x)>>;
     LongArgs a = {};
@@ -1273,9 +1273,9 @@ T5X_API int t5x_preference_loss(const void* logits, int fp32, void* grad, long l
     const unsigned grid = row_grid(r.rows);
     int rc = 0;
     if (in_long)
-      rc = launch_pieces<T>(x, r, pieces, st);
+      rc = launch_pieces<T>(x, r, pieces, arrived, st);
     else
-      preference_short_rows_kernel<T><<<grid, kRowThreads, 0, st>>>(x, r, softmax, logp);
+      preference_short_rows_kernel<T><<<grid, kRowThreads, 0, st>>>(x, r, softmax, logp, arrived);
     if (rc != 0) return rc;
     preference_pairs_kernel<<<static_cast<unsigned>(pairs), kRowThreads, 0, st>>>(
         in_long ? nullptr : logp, pieces, r, p, static_cast<float*>(scores), static_cast<float*>(margins), by, nullptr,
