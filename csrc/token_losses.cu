@@ -880,11 +880,12 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads)
     if (f.weight != 0.f) Chunk::ask(slots, logits + f.offset + f.first, min(f.packs, kChunk), tid);
   };
   ask_row(facts[0]);
+  int turn = 0;
   for (int k = 0; k < mine_of_all; ++k) {
     const RowFacts& f = facts[k & 3];
     const float w = f.weight;
     const long long offset = f.offset;
-    const int first = f.first, packs = f.packs, turn = k & 1;
+    const int first = f.first, packs = f.packs;
     const T* x = logits + offset;
     T* g = grad + offset;
     // The value in front of the first 16-byte boundary or behind the last that the thread sees to, or -1.
@@ -909,7 +910,8 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads)
     float x_outside = 0.f;
     if (outside >= 0) x_outside = Pack<T>::one(x[outside]);
     // The target's logit, by the thread that holds it, for all of the cluster. (Two places in turn here and with
-    // the parts' softmaxes: a CTA may be at the next row already.)
+    // the parts' softmaxes: a CTA may be at the next row that counts already, but not at the one behind that, as it
+    // has to meet the others in between. At rows that do not count CTAs do not meet: those do not change places.)
     auto tell_target = [&](float v) {
       if (a.shift == 0) {
         of_target[turn] = v;
@@ -990,6 +992,7 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads)
         sums[2] += static_cast<double>(w) * token.clipped;
         sums[3] += w;
       }
+      turn ^= 1;
       if (grad == nullptr) continue;
       now = said;
 #pragma unroll 1

@@ -400,3 +400,18 @@ def test_many_rows_of_some_kilobytes(kind, dtype, vocab):
   x = d["x"].requires_grad_()
   out = call(kind, x, d, 7.0)
   check(kind, out, torch.autograd.grad(out[0], x)[0], d, 7.0)
+
+
+@pytest.mark.parametrize("vocab", [40000, 65537, 140001])
+def test_rows_of_several_blocks_between_masked_ones(vocab):
+  """Blocks that share a row do not meet at rows of weight 0: most rows here, so that a block may run ahead by several."""
+  d = data(12, 60, vocab, torch.float32, seed=vocab, hidden=0.8)
+  x = d["x"].requires_grad_()
+  first = None
+  for _ in range(10):
+    out = call("policy", x, d, 7.0)
+    grad = torch.autograd.grad(out[0], x)[0]
+    if first is None:
+      first = out, grad
+      check("policy", out, grad, d, 7.0)
+    assert torch.equal(grad, first[1]) and all(torch.equal(a, b) for a, b in zip(out, first[0]))
