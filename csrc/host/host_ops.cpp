@@ -740,21 +740,36 @@ Tensor mlp_block_bwd(const Tensor& dy, const Tensor& x, const Tensor& scale,
 
 // What adamw_tree has gathered of the trees.
 struct AdamwItems {
+  enum Kind : int { kParam, kMu, kNu, kMuMost, kNuMost, kCopy, kKinds };
+  using Spans = std::vector<std::pair<uintptr_t, uintptr_t>>;  // [begin, end)
   std::vector<t5x_adamw_item> items;
-  std::vector<std::pair<uintptr_t, uintptr_t>> written;  // [begin, end) of what the step writes
+  Spans written[kKinds];  // of what the step writes
   c10::DeviceIndex device;
   bool small;  // moments in 8 bits
 
-  void writes(const void* p, size_t bytes) {
+  void writes(Kind kind, const void* p, size_t bytes) {
     const auto at = reinterpret_cast<uintptr_t>(p);
-    if (bytes) written.emplace_back(at, at + bytes);
+    if (bytes) written[kind].emplace_back(at, at + bytes);
   }
-  // Whether two of the tensors share memory: the parameters then have to be updated in turn.
+  static bool apart(Spans& spans) {
+    if (!std::is_sorted(spans.begin(), spans.end())) std::sort(spans.begin(), spans.end());
+    for (size_t i = 1; i < spans.size(); ++i)
+      if (spans[i].first < spans[i - 1].second) return false;
+    return true;
+  }
+  // Whether two of the tensors share memory: the parameters then have to be updated in turn. (Tensors of a kind
+  // mostly lie in the order of the tree, and often apart from those of other kinds: nothing is sorted then. 3300
+  // spans sorted as one list took a third of a step of 560 small tensors.)
   bool overlap() {
-    std::sort(written.begin(), written.end());
-    for (size_t i = 1; i < written.size(); ++i)
-      if (written[i].first < written[i - 1].second) return true;
-    return false;
+    Spans whole;
+    for (Spans& spans : written) {
+      if (!apart(spans)) return true;
+      if (!spans.empty()) whole.emplace_back(spans.front().first, spans.back().second);
+    }
+    if (apart(whole)) return false;
+    Spans all;
+    for (const Spans& spans : written) all.insert(all.end(), spans.begin(), spans.end());
+    return !apart(all);
   }
 };
 
@@ -773,6 +788,8 @@ const Tensor* leaf(PyObject* o, at::ScalarType type, c10::DeviceIndex device, in
 // Adds the parameters of one level. False: something that the grouped step does not cover.
 bool gather(PyObject* params, PyObject* grads, PyObject* mu, PyObject* nu, PyObject* mu_most,
             PyObject* nu_most, AdamwItems& to) {
+  static PyObject* const zero_name = PyUnicode_InternFromString("zero");  // (under the GIL)
+  static PyObject* const bf16_name = PyUnicode_InternFromString("bf16");
   PyObject* trees[5] = {grads, mu, nu, mu_most, nu_most};
   const int count = to.small ? 5 : 3;
   for (int i = 0; i < count; ++i)
@@ -805,27 +822,27 @@ bool gather(PyObject* params, PyObject* grads, PyObject* mu, PyObject* nu, PyObj
       if (a == nullptr || b == nullptr) return false;
       item.mu_absmax = a->data_ptr();
       item.nu_absmax = b->data_ptr();
-      to.writes(item.mu_absmax, blocks * 4);
-      to.writes(item.nu_absmax, blocks * 4);
+      to.writes(to.kMuMost, item.mu_absmax, blocks * 4);
+      to.writes(to.kNuMost, item.nu_absmax, blocks * 4);
     }
     PyObject* attributes = PyObject_GenericGetDict(value, nullptr);
     if (attributes == nullptr) {
       PyErr_Clear();
       return false;
     }
-    PyObject* sharded = PyDict_GetItemString(attributes, "zero");
-    PyObject* copy = PyDict_GetItemString(attributes, "bf16");
+    PyObject* sharded = PyDict_GetItemWithError(attributes, zero_name);
+    PyObject* copy = PyDict_GetItemWithError(attributes, bf16_name);
     Py_DECREF(attributes);  // (the tensor holds it)
     if (sharded != nullptr && sharded != Py_None) return false;
     if (copy != nullptr && copy != Py_None) {
       const Tensor* c = leaf(copy, at::kBFloat16, to.device, n);
       if (c == nullptr) return false;
       item.out = c->data_ptr();
-      to.writes(item.out, n * 2);
+      to.writes(to.kCopy, item.out, n * 2);
     }
-    to.writes(item.p, n * 4);
-    to.writes(item.mu, n * (to.small ? 1 : 4));
-    to.writes(item.nu, n * (to.small ? 1 : 4));
+    to.writes(to.kParam, item.p, n * 4);
+    to.writes(to.kMu, item.mu, n * (to.small ? 1 : 4));
+    to.writes(to.kNu, item.nu, n * (to.small ? 1 : 4));
     to.items.push_back(item);
   }
   return true;
@@ -841,7 +858,6 @@ bool adamw_tree(py::handle params, py::handle grads, py::handle mu, py::handle n
   to.device = c10::cuda::current_device();
   to.small = !mu_most.is_none();
   to.items.reserve(256);
-  to.written.reserve(1024);
   if (!PyDict_CheckExact(params.ptr()) ||
       !gather(params.ptr(), grads.ptr(), mu.ptr(), nu.ptr(), mu_most.ptr(), nu_most.ptr(), to) ||
       to.overlap())
