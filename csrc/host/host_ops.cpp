@@ -14,6 +14,7 @@
 #include <torch/extension.h>
 
 #include <algorithm>
+#include <cstring>
 #include <functional>
 #include <memory>
 #include <optional>
@@ -785,6 +786,28 @@ const Tensor* leaf(PyObject* o, at::ScalarType type, c10::DeviceIndex device, in
   return &t;
 }
 
+// The values of a dict for keys that mostly come in its own order: the entry whose turn it is, or a lookup.
+struct Entries {
+  PyObject* dict;
+  Py_ssize_t pos = 0;
+
+  static bool same(PyObject* a, PyObject* b) {
+    if (a == b) return true;
+    if (!PyUnicode_CheckExact(a) || !PyUnicode_CheckExact(b)) return false;
+    const Py_ssize_t n = PyUnicode_GET_LENGTH(a);
+    const auto kind = PyUnicode_KIND(a);
+    return n == PyUnicode_GET_LENGTH(b) && kind == PyUnicode_KIND(b) &&
+           std::memcmp(PyUnicode_DATA(a), PyUnicode_DATA(b), n * kind) == 0;
+  }
+  PyObject* operator[](PyObject* key) {
+    PyObject *k, *v;
+    if (PyDict_Next(dict, &pos, &k, &v) && same(k, key)) return v;
+    v = PyDict_GetItemWithError(dict, key);
+    if (v == nullptr) PyErr_Clear();
+    return v;
+  }
+};
+
 // Adds the parameters of one level. False: something that the grouped step does not cover.
 bool gather(PyObject* params, PyObject* grads, PyObject* mu, PyObject* nu, PyObject* mu_most,
             PyObject* nu_most, AdamwItems& to) {
@@ -795,15 +818,13 @@ bool gather(PyObject* params, PyObject* grads, PyObject* mu, PyObject* nu, PyObj
   for (int i = 0; i < count; ++i)
     if (trees[i] == nullptr || !PyDict_CheckExact(trees[i]) || PyDict_Size(trees[i]) != PyDict_Size(params))
       return false;
+  Entries entries[5] = {{trees[0]}, {trees[1]}, {trees[2]}, {trees[3]}, {trees[4]}};
   PyObject *key, *value;
   Py_ssize_t pos = 0;
   while (PyDict_Next(params, &pos, &key, &value)) {
     PyObject* at[5] = {};
     for (int i = 0; i < count; ++i)
-      if ((at[i] = PyDict_GetItemWithError(trees[i], key)) == nullptr) {
-        PyErr_Clear();
-        return false;
-      }
+      if ((at[i] = entries[i][key]) == nullptr) return false;
     if (PyDict_CheckExact(value)) {
       if (!gather(value, at[0], at[1], at[2], at[3], at[4], to)) return false;
       continue;
