@@ -743,6 +743,10 @@ Tensor mlp_block_bwd(const Tensor& dy, const Tensor& x, const Tensor& scale,
 struct AdamwItems {
   enum Kind : int { kParam, kMu, kNu, kMuMost, kNuMost, kCopy, kKinds };
   using Spans = std::vector<std::pair<uintptr_t, uintptr_t>>;  // [begin, end)
+  struct Objects {
+    PyObject *p, *copy, *of[5];  // the parameter, its bf16 copy or null; its entry in each of the other trees
+  };
+  std::vector<Objects> objects;  // (borrowed, under the GIL)
   std::vector<t5x_adamw_item> items;
   Spans written[kKinds];  // of what the step writes
   c10::DeviceIndex device;
@@ -808,7 +812,7 @@ struct Entries {
   }
 };
 
-// Adds the parameters of one level. False: something that the grouped step does not cover.
+// Gathers the objects of the parameters of one level. False: something that the grouped step does not cover.
 bool gather(PyObject* params, PyObject* grads, PyObject* mu, PyObject* nu, PyObject* mu_most,
             PyObject* nu_most, AdamwItems& to) {
   static PyObject* const zero_name = PyUnicode_InternFromString("zero");  // (under the GIL)
@@ -822,41 +826,79 @@ bool gather(PyObject* params, PyObject* grads, PyObject* mu, PyObject* nu, PyObj
   PyObject *key, *value;
   Py_ssize_t pos = 0;
   while (PyDict_Next(params, &pos, &key, &value)) {
-    PyObject* at[5] = {};
-    for (int i = 0; i < count; ++i)
-      if ((at[i] = entries[i][key]) == nullptr) return false;
+    AdamwItems::Objects at = {};
+    for (int i = 0; i < count; ++i) {
+      if ((at.of[i] = entries[i][key]) == nullptr) return false;
+      __builtin_prefetch(at.of[i]);
+    }
     if (PyDict_CheckExact(value)) {
-      if (!gather(value, at[0], at[1], at[2], at[3], at[4], to)) return false;
+      if (!gather(value, at.of[0], at.of[1], at.of[2], at.of[3], at.of[4], to)) return false;
       continue;
     }
-    const Tensor* p = leaf(value, at::kFloat, to.device, -1);
-    if (p == nullptr) return false;
-    const int64_t n = p->numel(), blocks = (n + kMomentBlock - 1) / kMomentBlock;
-    const auto type = to.small ? at::kByte : at::kFloat;
-    const Tensor* g = leaf(at[0], at::kFloat, to.device, n);
-    const Tensor *m = leaf(at[1], type, to.device, n), *v = leaf(at[2], type, to.device, n);
-    if (g == nullptr || m == nullptr || v == nullptr) return false;
-    t5x_adamw_item item = {p->data_ptr(), g->data_ptr(), m->data_ptr(), v->data_ptr(), nullptr, nullptr,
-                           nullptr, n};
-    if (to.small) {
-      const Tensor *a = leaf(at[3], at::kFloat, to.device, blocks), *b = leaf(at[4], at::kFloat, to.device, blocks);
-      if (a == nullptr || b == nullptr) return false;
-      item.mu_absmax = a->data_ptr();
-      item.nu_absmax = b->data_ptr();
-      to.writes(to.kMuMost, item.mu_absmax, blocks * 4);
-      to.writes(to.kNuMost, item.nu_absmax, blocks * 4);
-    }
+    if (!THPVariable_CheckExact(value)) return false;
+    at.p = value;
     PyObject* attributes = PyObject_GenericGetDict(value, nullptr);
     if (attributes == nullptr) {
       PyErr_Clear();
       return false;
     }
     PyObject* sharded = PyDict_GetItemWithError(attributes, zero_name);
-    PyObject* copy = PyDict_GetItemWithError(attributes, bf16_name);
+    at.copy = PyDict_GetItemWithError(attributes, bf16_name);
     Py_DECREF(attributes);  // (the tensor holds it)
     if (sharded != nullptr && sharded != Py_None) return false;
-    if (copy != nullptr && copy != Py_None) {
-      const Tensor* c = leaf(copy, at::kBFloat16, to.device, n);
+    if (at.copy == Py_None) at.copy = nullptr;
+    if (at.copy != nullptr) __builtin_prefetch(at.copy);
+    to.objects.push_back(at);
+  }
+  return true;
+}
+
+// The lines of a tensor that its checks read. (A few thousand tensors do not stay in the core's first cache:
+// waiting for them in turn took a quarter of the walk: 558 small
+// tensors 179 -> 156 us a step with moments in 8 bits, 109 -> 93 in 32.)
+void prefetch(PyObject* o) {
+  if (o == nullptr || !THPVariable_CheckExact(o)) return;
+  const char* impl = reinterpret_cast<const char*>(THPVariable_Unpack(o).unsafeGetTensorImpl());
+  for (int i = 0; i < 4; ++i) __builtin_prefetch(impl + 64 * i);
+}
+
+// The items of the objects. False: something that the grouped step does not cover.
+bool to_items(AdamwItems& to) {
+  constexpr size_t kAhead = 4;
+  const auto type = to.small ? at::kByte : at::kFloat;
+  const int count = to.small ? 5 : 3;
+  const size_t n_objects = to.objects.size();
+  auto ahead = [&](size_t i) {
+    if (i >= n_objects) return;
+    const AdamwItems::Objects& o = to.objects[i];
+    prefetch(o.p);
+    prefetch(o.copy);
+    for (int k = 0; k < count; ++k) prefetch(o.of[k]);
+  };
+  for (size_t i = 0; i < kAhead; ++i) ahead(i);
+  to.items.reserve(n_objects);
+  for (auto& spans : to.written) spans.reserve(n_objects);
+  for (size_t i = 0; i < n_objects; ++i) {
+    ahead(i + kAhead);
+    const AdamwItems::Objects& o = to.objects[i];
+    const Tensor* p = leaf(o.p, at::kFloat, to.device, -1);
+    if (p == nullptr) return false;
+    const int64_t n = p->numel(), blocks = (n + kMomentBlock - 1) / kMomentBlock;
+    const Tensor* g = leaf(o.of[0], at::kFloat, to.device, n);
+    const Tensor *m = leaf(o.of[1], type, to.device, n), *v = leaf(o.of[2], type, to.device, n);
+    if (g == nullptr || m == nullptr || v == nullptr) return false;
+    t5x_adamw_item item = {p->data_ptr(), g->data_ptr(), m->data_ptr(), v->data_ptr(), nullptr, nullptr,
+                           nullptr, n};
+    if (to.small) {
+      const Tensor *a = leaf(o.of[3], at::kFloat, to.device, blocks), *b = leaf(o.of[4], at::kFloat, to.device, blocks);
+      if (a == nullptr || b == nullptr) return false;
+      item.mu_absmax = a->data_ptr();
+      item.nu_absmax = b->data_ptr();
+      to.writes(to.kMuMost, item.mu_absmax, blocks * 4);
+      to.writes(to.kNuMost, item.nu_absmax, blocks * 4);
+    }
+    if (o.copy != nullptr) {
+      const Tensor* c = leaf(o.copy, at::kBFloat16, to.device, n);
       if (c == nullptr) return false;
       item.out = c->data_ptr();
       to.writes(to.kCopy, item.out, n * 2);
@@ -878,10 +920,10 @@ bool adamw_tree(py::handle params, py::handle grads, py::handle mu, py::handle n
   AdamwItems to;
   to.device = c10::cuda::current_device();
   to.small = !mu_most.is_none();
-  to.items.reserve(256);
+  to.objects.reserve(256);
   if (!PyDict_CheckExact(params.ptr()) ||
       !gather(params.ptr(), grads.ptr(), mu.ptr(), nu.ptr(), mu_most.ptr(), nu_most.ptr(), to) ||
-      to.overlap())
+      !to_items(to) || to.overlap())
     return false;
   py::gil_scoped_release no_gil;
   void* st = stream_of();
