@@ -36,7 +36,9 @@ constexpr int kThreads = 256;
 constexpr int kChunk = 2048;      // elements per CTA
 constexpr int kQuantBlock = 256;  // values that share a scale
 constexpr int kSpan = 4;          // chunks that a CTA of the norm takes in a row
-constexpr int kMaxItems = 448;    // (31 KB of the 32 KB that a launch's parameters may have)
+// Of a launch: what fits in 31 KB of the 32 KB that its parameters may have. (All with the items of 8 bits: 558 small
+// tensors took two launches where one is enough.)
+constexpr int kMaxItems = 576, kMaxItems8 = 448, kMaxNorms = 1408;
 constexpr int kHints = 256;
 constexpr int kFewItems = 48;
 
@@ -46,7 +48,24 @@ struct Hyper {
   uint32_t noise_key;
 };
 
-template <int kItems>
+// Of an item, what the kernel of moments in 32 bits, in 8, and the norm need.
+struct Item32 {
+  void* p;
+  const void* g;
+  void *mu, *nu, *out;
+  long long n;
+  static Item32 of(const t5x_adamw_item& i) { return {i.p, i.g, i.mu, i.nu, i.out, i.n}; }
+};
+struct Item8 : t5x_adamw_item {
+  static Item8 of(const t5x_adamw_item& i) { return {i}; }
+};
+struct ItemNorm {
+  const void* g;
+  long long n;
+  static ItemNorm of(const t5x_adamw_item& i) { return {i.g, i.n}; }
+};
+
+template <typename Item, int kItems>
 struct Group {
   Hyper h;
   const float* clip_scale;
@@ -55,11 +74,20 @@ struct Group {
   unsigned first[kItems];           // first chunk of each item
   bool wide[kItems];                // every pointer of the item takes the wide accesses
   unsigned short near[kHints + 1];  // item of chunk (i << shift); behind the last chunk the last item
-  t5x_adamw_item item[kItems];
+  Item item[kItems];
 };
-
 template <int kItems>
-__device__ __forceinline__ int find_item(const Group<kItems>& grp, unsigned chunk) {
+using Group32 = Group<Item32, kItems>;
+template <int kItems>
+using Group8 = Group<Item8, kItems>;
+template <int kItems>
+using GroupNorm = Group<ItemNorm, kItems>;
+static_assert(sizeof(Group32<kMaxItems>) < 32700 && sizeof(Group8<kMaxItems8>) < 32700 &&
+                  sizeof(GroupNorm<kMaxNorms>) < 32700 - 64,
+              "parameters of a launch");
+
+template <typename Items>
+__device__ __forceinline__ int find_item(const Items& grp, unsigned chunk) {
   const unsigned hint = chunk >> grp.shift;
   int lo = grp.near[hint], hi = grp.near[hint + 1] + 1;  // first[lo] <= chunk < first[hi]
   while (hi - lo > 1) {
@@ -95,10 +123,10 @@ __device__ __forceinline__ uint2 pack_bf16(float4 v) {
 
 template <int kItems>
 __global__ void __launch_bounds__(kThreads)
-    adamw_group_kernel(const __grid_constant__ Group<kItems> grp) {
+    adamw_group_kernel(const __grid_constant__ Group32<kItems> grp) {
   const unsigned chunk = blockIdx.x;
   const int which = find_item(grp, chunk);
-  const t5x_adamw_item it = grp.item[which];
+  const auto it = grp.item[which];
   const Hyper h = grp.h;
   const float cs = grp.clip_scale != nullptr ? *grp.clip_scale : 1.f;
   const long long begin = static_cast<long long>(chunk - grp.first[which]) * kChunk;
@@ -233,7 +261,8 @@ __device__ __forceinline__ uint32_t abs_bits(float x) { return __float_as_uint(x
 // up by a random number below one step before they are cut off. Below 2^-6 the steps are 2^-9 wide;
 // with 2^-6 added the value lies among numbers whose steps are the same, and what is left when it is
 // taken off again is exact. (That sum drops bits below those of the draw, which cannot carry: rounded to the
-// nearest it moved one in 60 million values across a border.) kSecond: no sign, and nothing is stored as zero (the caller sees to zeros).
+// nearest it moved one in 60 million values across a border.) kSecond: no sign, and nothing is stored as
+// zero (the caller sees to zeros).
 // (A largest that is not finite makes the whole block NaN when it is read back, as it is kept itself.)
 template <bool kSecond>
 __device__ __forceinline__ uint32_t codes2(float2 x, float most, float inv, uint32_t noise0, uint32_t noise1) {
@@ -325,10 +354,10 @@ __device__ __forceinline__ Result8 step8(const Hyper& h, float clip, const Block
 // them 247 us sustained (5.6 TB/s).
 template <int kItems>
 __global__ void __launch_bounds__(kThreads, 4)
-    adamw8_group_kernel(const __grid_constant__ Group<kItems> grp) {
+    adamw8_group_kernel(const __grid_constant__ Group8<kItems> grp) {
   const unsigned chunk = blockIdx.x;
   const int which = find_item(grp, chunk);
-  const t5x_adamw_item it = grp.item[which];
+  const auto it = grp.item[which];
   const int lane = threadIdx.x & 31;
   const long long block = static_cast<long long>(chunk - grp.first[which]) * (kChunk / kQuantBlock) +
                           (threadIdx.x >> 5);
@@ -347,7 +376,7 @@ __global__ void __launch_bounds__(kThreads, 4)
   if (threadIdx.x == 0 && chunk + grp.ahead < gridDim.x) {
     const unsigned later = chunk + grp.ahead;
     const int w = find_item(grp, later);
-    const t5x_adamw_item& item = grp.item[w];
+    const Item8& item = grp.item[w];
     const long long at = static_cast<long long>(later - grp.first[w]) * kChunk;
     if (at + kChunk <= item.n && grp.wide[w]) {
       prefetch_l2(static_cast<const float*>(item.g) + at, kChunk * 4);
@@ -427,7 +456,7 @@ __global__ void __launch_bounds__(kThreads, 4)
 // this and the earlier launches of the call and stores min(1, max_norm / (norm + 1e-16)).
 template <int kItems>
 __global__ void __launch_bounds__(kThreads)
-    sumsq_group_kernel(const __grid_constant__ Group<kItems> grp, unsigned chunks, double* partial,
+    sumsq_group_kernel(const __grid_constant__ GroupNorm<kItems> grp, unsigned chunks, double* partial,
                        int partial_first, unsigned* arrived, float max_norm, float* clip_out) {
   __shared__ double s_sum[kThreads / 32];
   __shared__ bool s_last;
@@ -499,8 +528,8 @@ __global__ void __launch_bounds__(kThreads)
 }
 
 // Fills `grp` with items [from, ...) up to its capacity; returns how many it took and the chunks.
-template <int kItems>
-int fill(Group<kItems>& grp, const t5x_adamw_item* items, int from, int count, unsigned* chunks) {
+template <typename Item, int kItems>
+int fill(Group<Item, kItems>& grp, const t5x_adamw_item* items, int from, int count, unsigned* chunks) {
   grp.count = 0;
   unsigned long long c = 0;
   int i = from;
@@ -510,7 +539,7 @@ int fill(Group<kItems>& grp, const t5x_adamw_item* items, int from, int count, u
     if (c + need > 0x7fffffffull) break;
     grp.first[grp.count] = static_cast<unsigned>(c);
     grp.wide[grp.count] = takes_wide(items[i]);
-    grp.item[grp.count++] = items[i];
+    grp.item[grp.count++] = Item::of(items[i]);
     c += need;
   }
   grp.shift = 0;
@@ -549,9 +578,18 @@ int validate(const char* what, const t5x_adamw_item* items, int count, int bits)
 }
 
 template <int kItems>
-int step_in_groups(const t5x_adamw_item* items, int count, const Hyper& h, const float* clip_scale, int bits,
-                   cudaStream_t st) {
-  Group<kItems> grp;
+void launch(const Group32<kItems>& grp, unsigned chunks, cudaStream_t st) {
+  adamw_group_kernel<kItems><<<chunks, kThreads, 0, st>>>(grp);
+}
+template <int kItems>
+void launch(const Group8<kItems>& grp, unsigned chunks, cudaStream_t st) {
+  adamw8_group_kernel<kItems><<<chunks, kThreads, 0, st>>>(grp);
+}
+
+template <typename Items>
+void step_in_groups(const t5x_adamw_item* items, int count, const Hyper& h, const float* clip_scale,
+                    cudaStream_t st) {
+  Items grp;
   grp.h = h;
   grp.clip_scale = clip_scale;
   grp.ahead = static_cast<unsigned>(num_sms()) * 4;
@@ -559,19 +597,15 @@ int step_in_groups(const t5x_adamw_item* items, int count, const Hyper& h, const
     unsigned chunks;
     from += fill(grp, items, from, count, &chunks);
     if (chunks == 0) continue;
-    if (bits == 8)
-      adamw8_group_kernel<kItems><<<chunks, kThreads, 0, st>>>(grp);
-    else
-      adamw_group_kernel<kItems><<<chunks, kThreads, 0, st>>>(grp);
+    launch(grp, chunks, st);
     count_launches(1);
   }
-  return 0;
 }
 
 template <int kItems>
 int sumsq_in_groups(const t5x_adamw_item* items, int count, void* scratch, float max_norm, float* clip,
                     cudaStream_t st) {
-  Group<kItems> grp;
+  GroupNorm<kItems> grp;
   grp.clip_scale = nullptr;
   unsigned* arrived = static_cast<unsigned*>(scratch);
   double* partial = reinterpret_cast<double*>(static_cast<char*>(scratch) + 16);
@@ -592,7 +626,7 @@ int sumsq_in_groups(const t5x_adamw_item* items, int count, void* scratch, float
   return 0;
 }
 
-int launches_for(int count) { return count <= kMaxItems ? 1 : (count + kMaxItems - 1) / kMaxItems; }
+int launches_for(int count) { return count <= kMaxNorms ? 1 : (count + kMaxNorms - 1) / kMaxNorms; }
 
 }  // namespace
 }  // namespace t5x
@@ -620,7 +654,7 @@ T5X_API int t5x_grad_clip_scale(const t5x_adamw_item* items, int count, void* sc
   if (count <= kFewItems)
     sumsq_in_groups<kFewItems>(items, count, scratch, max_norm, clip, st);
   else
-    sumsq_in_groups<kMaxItems>(items, count, scratch, max_norm, clip, st);
+    sumsq_in_groups<kMaxNorms>(items, count, scratch, max_norm, clip, st);
   e = cudaGetLastError();
   if (e != cudaSuccess) return set_error("grad_clip_scale: %s", cudaGetErrorString(e));
   return 0;
@@ -658,10 +692,14 @@ T5X_API int t5x_adamw_group(const t5x_adamw_item* items, int count, int state_bi
   h.noise_key = seed * kNoise1 + static_cast<unsigned>(step) * 0xBB67AE85u;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const float* cs = static_cast<const float*>(clip_scale);
-  if (count <= kFewItems)
-    step_in_groups<kFewItems>(items, count, h, cs, state_bits, st);
+  if (state_bits == 32 && count <= kFewItems)
+    step_in_groups<Group32<kFewItems>>(items, count, h, cs, st);
+  else if (state_bits == 32)
+    step_in_groups<Group32<kMaxItems>>(items, count, h, cs, st);
+  else if (count <= kFewItems)
+    step_in_groups<Group8<kFewItems>>(items, count, h, cs, st);
   else
-    step_in_groups<kMaxItems>(items, count, h, cs, state_bits, st);
+    step_in_groups<Group8<kMaxItems8>>(items, count, h, cs, st);
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return set_error("adamw_group: %s", cudaGetErrorString(e));
   return 0;

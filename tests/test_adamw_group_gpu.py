@@ -84,7 +84,7 @@ def test_many_tensors_against_64_bits(bits, host, monkeypatch):
   before = [p.clone() for p in leaves(opt.target)]
   count = native.launch_count()
   opt = opt.apply_gradient(g)
-  assert native.launch_count() - count == 3  # 448 a launch
+  assert native.launch_count() - count == (2 if bits == 32 else 3)  # 576 or 448 a launch
   zero = torch.zeros((), device="cuda")
   for p, p0, gg in zip(leaves(opt.target), before, leaves(g)):
     want, _, _ = reference_step(p0, gg, zero, zero, 1, lr, wd)
@@ -153,7 +153,7 @@ def test_host_path_and_its_stand_in_agree(bits, monkeypatch):
     assert torch.equal(a, b)
 
 
-@pytest.mark.parametrize("sizes", [[1], [7, 2048, 5000], [3] * 500, [1 << 22, 12345]])
+@pytest.mark.parametrize("sizes", [[1], [7, 2048, 5000], [3] * 500, [1 << 22, 12345], [5] * 3000])
 @pytest.mark.parametrize("max_norm", [0.1, 1e9])
 def test_clip_factor(sizes, max_norm):
   from t5x_b200.ops import native
