@@ -442,14 +442,20 @@ __global__ void __launch_bounds__(kRowThreads)
 // itself (332); exponentials kept for the gradient, by which one block of 512 threads fills an SM (370).
 constexpr int kPacks = 8;
 
-// An exponential exp(x - most) is exp2(x log2 e - ref) here, a fused product and difference, with ref =
-// most log2 e as rounded: the same factor for the sum, the target and the gradient. Where a largest logit's
-// product may overflow, it is exp2((x - most) log2 e).
-constexpr float kHuge = 1.0e38f;
-__device__ __forceinline__ bool huge(float most) { return !(fabsf(most) <= kHuge); }  // (NaN and -inf too)
-// log2 of exp(a - b); 0 for a = b = -inf
+// An exponential exp(x - most) is exp2(x log2 e - ref) here, a fused product and difference, with ref = most log2 e
+// as rounded: the same factor, 2^(most log2 e - ref), for the sum, the target and the gradient. Up to 65536 that factor
+// is within 2^(1/256) of 1. From there on it grows until it overflows (at 1e10, a usual value for masked
+// places, 2^440), and the exponential is exp2((x - most) log2 e). So each part of a row is held against its own
+// largest in one of two ways, and joining parts puts their sums on one reference (see shift_of).
+constexpr float kFused = 65536.f;
+__device__ __forceinline__ bool huge(float most) { return !(fabsf(most) <= kFused); }  // (NaN and the infinities too)
+// What the reference of a largest is rounded by: ref = most log2 e - rounded_off(most).
+__device__ __forceinline__ float rounded_off(float most) {
+  return huge(most) ? 0.f : fmaf(most, kLog2e, -__fmul_rn(most, kLog2e));
+}
+// log2 of the factor that takes a sum held against a to one held against b; 0 for a = b = -inf
 __device__ __forceinline__ float shift_of(float a, float b) {
-  if (huge(a) || huge(b)) return a == b ? 0.f : (a - b) * kLog2e;
+  if (huge(a) || huge(b)) return a == b ? 0.f : fmaf(a - b, kLog2e, rounded_off(b) - rounded_off(a));
   return __fmul_rn(a, kLog2e) - __fmul_rn(b, kLog2e);
 }
 __device__ __forceinline__ float exp_from(float x, float most) {
@@ -466,10 +472,10 @@ __device__ __forceinline__ Softmax row_of_lanes(Softmax s) {
   asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(m) : "f"(s.most));
   return {m, warp_sum(s.sum * exp2_approx(shift_of(s.most, m)))};
 }
+// (with the reference of the sum; the difference first, as a product with the lowest value overflows)
 __device__ __forceinline__ float log_prob_of(float x, Softmax s) {
   if (s.most == -INFINITY) return NAN;
-  const float d = huge(s.most) ? x - s.most : fmaf(x, kLog2e, -__fmul_rn(s.most, kLog2e)) * 0.6931471805599453f;
-  return d - log1pf(s.sum - 1.f);
+  return fmaf(rounded_off(s.most), 0.6931471805599453f, x - s.most) - log1pf(s.sum - 1.f);
 }
 
 // What the gradient of a row needs: by * onehot(target) + k * exp(x - most) with k = -by / sum.

@@ -1,0 +1,90 @@
+"""The ends of the range of the fine-tuning losses and of AdamW with 8-bit moments on the GPU: large logits and masks of
+large values, terms of weight 0 that overflow, answers that cannot be, factors of 0, blocks of the largest and smallest
+moments, memory and places of gradients, function transforms."""
+import math
+
+import pytest
+import torch
+
+from t5x_b200 import losses
+from tests.test_token_losses_gpu import call, check, data, oracle_logp
+
+pytestmark = pytest.mark.gpu
+
+
+LIMIT = 65536.0  # up to here a largest logit's product with log2 e is rounded once for the whole row
+
+
+def large_rows(vocab, dtype):
+  """Rows [18, vocab] and targets: parts of the vocabulary, or all of it, under masks of large negative values; large
+  largest values, several of them the same; values on either side of the limit, so that parts of a row lie on both."""
+  gen = torch.Generator(device="cuda").manual_seed(vocab)
+  rand = lambda n: torch.randn(n, device="cuda", generator=gen)  # noqa: E731
+  few = min(300, vocab // 2)
+  rows, targets = [], []
+
+  def add(x, t):
+    rows.append(x.to(dtype))
+    targets.append(t)
+
+  for mask in (-1e7, -1e9, -1e10, -1e20, -1e30):
+    x = rand(vocab) * 2
+    x[few:] = mask
+    add(x, few // 2)  # (in the part that counts)
+  for mask in (-1e7, -1e10, -1e30):
+    add(torch.full((vocab,), mask, device="cuda"), vocab - 1)
+  for big in (1e7, 1e9, 1e10, 1e30):
+    x = rand(vocab) * 2
+    x[few:few + 5] = big
+    add(x, few + 3)
+  for middle in (LIMIT, -LIMIT, 1e5, -1e6):
+    x = middle + rand(vocab) * 3
+    add(x, int(x.argmax()))
+  x = rand(vocab) * 2  # parts of several sizes
+  for i, v in enumerate((-1e10, -LIMIT, -7e4, -1e6, -1e38)):
+    x[vocab * (i + 1) // 7:vocab * (i + 2) // 7] = v
+  add(x, 0)
+  x = -70000 + rand(vocab) * 3  # lanes of a warp below the limit, the largest above it
+  x[vocab // 2] = -65530.0
+  add(x, vocab // 2)
+  return torch.stack(rows).view(6, 3, vocab), torch.tensor(targets, device="cuda").view(6, 3)
+
+
+@pytest.mark.parametrize("kind", ["preference", "policy"])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("vocab", [64, 4000, 32128, 140001, 250112, 530000])
+def test_large_logits(kind, dtype, vocab):
+  """Of a warp a row, a block, a cluster, several chunks."""
+  d = data(6, 3, vocab, dtype, hidden=0.0)
+  d["x"], d["t"] = large_rows(vocab, dtype)
+  logp = oracle_logp(d["x"], d["t"])
+  assert float(logp.min()) > -40  # (as the tolerances take it)
+  d["old"], d["ref"], d["r"] = (logp - 0.1).float(), (logp + 0.1).float(), (logp * d["w"]).sum(1).float() - 1
+  x = d["x"].clone().requires_grad_()
+  out = call(kind, x, d, None)
+  check(kind, out, torch.autograd.grad(out[0], x)[0], d, 1.0)
+  with torch.no_grad():
+    check(kind, call(kind, d["x"], d, None), None, d, 1.0)
+
+
+@pytest.mark.parametrize("vocab", [4000, 32128, 250112])
+def test_unlikely_targets_among_large_logits(vocab):
+  """A target far below the largest logit: its log-probability is their difference, exact in 32 bits here."""
+  for big in (1e5, 1e7, 1e10):
+    x = torch.zeros(2, 1, vocab, device="cuda")
+    x[:, :, vocab // 3] = big
+    t = torch.full((2, 1), vocab - 1, device="cuda")
+    out = losses.compute_preference_loss(x, t, None, torch.zeros(2, device="cuda"), beta=1e-8)
+    assert out[1].tolist() == pytest.approx([-big, -big], rel=2.0 ** -22)
+
+
+@pytest.mark.parametrize("vocab", [64, 4000, 32128, 250112])
+def test_targets_of_the_lowest_logit(vocab):
+  """A target at -3e38 among ordinary logits, as likely as it was when it was drawn: ratio 1."""
+  x = torch.zeros(2, 1, vocab, device="cuda")
+  x[..., 5] = -3e38
+  t, old = torch.full((2, 1), 5, device="cuda"), torch.full((2, 1), -3e38, device="cuda")
+  x.requires_grad_()
+  out = losses.compute_policy_loss(x, t, None, old, torch.ones(2, device="cuda"))
+  assert out[0].item() == -2.0
+  assert torch.all(torch.autograd.grad(out[0], x)[0][..., 5] == -1.0)
