@@ -271,9 +271,11 @@ __device__ __forceinline__ PolicyToken policy_token(const Policy& p, PolicyInput
   k.kl = 0.f;
   if (p.ref != nullptr) {
     const float apart = in.ref - logp, e = expm1f(apart);
-    k.kl = e - apart;
-    k.loss += p.kl_weight * k.kl;
-    k.slope -= p.kl_weight * e;
+    k.kl = apart == INFINITY ? apart : e - apart;
+    if (p.kl_weight != 0.f) {  // (of a term that only is reported an overflow stays out of the loss)
+      k.loss += p.kl_weight * k.kl;
+      k.slope -= p.kl_weight * e;
+    }
   }
   return k;
 }

@@ -260,9 +260,9 @@ def compute_policy_loss(logits: torch.Tensor, targets: torch.Tensor, weights: Op
   old_token_scores) against the log-probabilities [batch, length] when the answers were drawn, and `advantages`
   ([batch], one for an answer, or [batch, length]), a token's loss is
   -min(advantage * ratio, advantage * clip(ratio, 1 - clip_range, 1 + clip_range_high)) + kl_weight * kl with
-  kl = exp(ref - logp) - 1 - (ref - logp) against `reference_token_scores` (None: no such term);
-  clip_range_high is clip_range unless given. Log-probabilities are unweighted, as in the `token_scores` that
-  `score_batch` returns for weights of 0 and 1.
+  kl = exp(ref - logp) - 1 - (ref - logp) against `reference_token_scores` (None: no such term; with kl_weight 0 it
+  is returned and is not part of the loss, whatever its size); clip_range_high is clip_range unless given.
+  Log-probabilities are unweighted, as in the `token_scores` that `score_batch` returns for weights of 0 and 1.
 
   Returns (loss, kl, clipped, weight_sum): the sums (not means) of weights * loss and weights * kl, both over
   `loss_normalizing_factor` if one is given, the weights of the tokens that the clip holds, and all weights. The

@@ -289,8 +289,9 @@ def policy_loss(logp, weights, old, advantages, reference, clip_low, clip_high, 
   each, kl = -torch.minimum(gain, held), torch.zeros_like(logp)
   if reference is not None:
     apart = pick(reference) - logp
-    kl = torch.expm1(apart) - apart
-    each = each + kl_weight * kl
+    kl = torch.where(torch.isposinf(apart), apart, torch.expm1(apart) - apart)
+    if kl_weight != 0:  # (of a term that only is reported an overflow stays out of the loss)
+      each = each + kl_weight * kl
   total = lambda t: torch.where(seen, t * w, zero).sum(dtype=torch.float64)  # noqa: E731
   back = logp.dtype
   return (_over_normalizer(total(each), normalizer).to(back), _over_normalizer(total(kl.detach()), normalizer).to(back),

@@ -88,3 +88,58 @@ def test_targets_of_the_lowest_logit(vocab):
   out = losses.compute_policy_loss(x, t, None, old, torch.ones(2, device="cuda"))
   assert out[0].item() == -2.0
   assert torch.all(torch.autograd.grad(out[0], x)[0][..., 5] == -1.0)
+
+
+@pytest.mark.parametrize("kl_weight", [0.0, 0.1])
+@pytest.mark.parametrize("vocab", [0, 2, 3000, 40000])
+@pytest.mark.parametrize("host", ["1", "0"])
+def test_policy_reference_far_above(kl_weight, vocab, host, monkeypatch):
+  """exp(ref - logp) overflows: with weight 0 the term is not part of the loss. (vocab 0: from log-probabilities)"""
+  from t5x_b200.ops import native
+  monkeypatch.setattr(native, "_host", None if host == "1" else False)
+  f = lambda *v: torch.tensor(v, device="cuda").view(2, 1)  # noqa: E731
+  rest = (None, f(-100.0, -1.0), torch.ones(2, device="cuda"), f(-1.0, -1.0))
+  if vocab:
+    x = torch.full((2, 1, vocab), -1000.0, device="cuda")
+    x[..., 0], x[..., 1] = 0.0, 100.0
+    x[1, 0, 0], x[1, 0, 1] = 100.0, 101.0
+    x.requires_grad_()
+    out = losses.compute_policy_loss(x, torch.zeros(2, 1, dtype=torch.long, device="cuda"), *rest, kl_weight=kl_weight)
+  else:
+    x = f(-100.0, -1.0).requires_grad_()
+    out = losses.policy_loss_from_token_scores(x, *rest, kl_weight=kl_weight)
+  assert out[1].item() == math.inf
+  if kl_weight:
+    assert out[0].item() == math.inf
+    return
+  # ratios: 1 (a few roundings of 100 at most), and, with logits, exp(logp + 1) with logp = -log(1 + e)
+  second = math.exp(1 - math.log(1 + math.e)) if vocab else 1.0
+  assert out[0].item() == pytest.approx(-1.0 - second, abs=6e-5)
+  grad = torch.autograd.grad(out[0], x)[0]
+  assert torch.all(torch.isfinite(grad))
+  if vocab:
+    assert grad[0, 0, :2].tolist() == pytest.approx([-1.0, 1.0], abs=6e-5) and torch.all(grad[..., 2:] == 0)
+  else:
+    assert grad.flatten().tolist() == pytest.approx([-1.0, -1.0], abs=6e-5)
+
+
+@pytest.mark.parametrize("vocab", [0, 5, 3000, 40000])
+def test_policy_of_an_impossible_token(vocab):
+  """A token that the model now rules out: ratio 0, and a KL term of infinity where it is asked for."""
+  full = lambda v: torch.full((1, 2), v, device="cuda")  # noqa: E731
+  rest = (None, full(-1.0), torch.ones(1, device="cuda"), full(-2.0))
+  x = torch.zeros(1, 2, max(vocab, 5), device="cuda")
+  x[0, 0, 3] = -math.inf
+  t = torch.full((1, 2), 3, device="cuda")
+  if vocab:
+    f = lambda **kw: losses.compute_policy_loss(x, t, *rest, **kw)  # noqa: E731
+  else:
+    x = x.log_softmax(-1)[..., 3]
+    f = lambda **kw: losses.policy_loss_from_token_scores(x, *rest, **kw)  # noqa: E731
+  x.requires_grad_()
+  out = f()
+  other = -min(math.exp(1 - math.log(max(vocab, 5))), 1.2)
+  assert out[0].item() == pytest.approx(other, rel=1e-5) and out[1].item() == math.inf
+  grad = torch.autograd.grad(out[0], x)[0]
+  assert torch.all(grad[0, 0] == 0) and torch.all(torch.isfinite(grad))
+  assert f(kl_weight=0.1)[0].item() == math.inf
