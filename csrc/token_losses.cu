@@ -400,10 +400,14 @@ __device__ __forceinline__ Margin pair_margin(const Preference& p, bool real, do
   // log(1 + exp(-d)) = log1p(exp(-|d|)) + max(-d, 0)
   const float e = expf(-fabsf(d)), tail = log1pf(e);
   const float sigmoid = (d >= 0.f ? 1.f : e) / (1.f + e);
-  m.loss = d != d ? d : (1.f - p.smoothing) * (tail + fmaxf(-d, 0.f)) + p.smoothing * (tail + fmaxf(d, 0.f));
+  // (a side of weight 0 may be infinite: the answer that is not preferred cannot be)
+  const float weight = 1.f - p.smoothing;
+  m.loss = d != d ? d
+                  : (weight > 0.f ? weight * (tail + fmaxf(-d, 0.f)) : 0.f) +
+                        (p.smoothing > 0.f ? p.smoothing * (tail + fmaxf(d, 0.f)) : 0.f);
   // sigmoid - 1 + e, near 0 from the side that does not cancel
   const float under = (d >= 0.f ? e : 1.f) / (1.f + e);  // sigmoid(-d)
-  m.slope = p.beta * (p.smoothing * sigmoid - (1.f - p.smoothing) * under) * scale;
+  m.slope = p.beta * (p.smoothing * sigmoid - weight * under) * scale;
   return m;
 }
 

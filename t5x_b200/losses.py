@@ -210,7 +210,8 @@ def compute_preference_loss(logits: torch.Tensor, targets: torch.Tensor, weights
 
   Returns (loss, scores [batch], margins [batch / 2], number of pairs); the loss alone is differentiable, and in
   the logits alone. Tokens of weight 0 do not count, whatever their logits hold, and a pair without any
-  other is padding: it counts nowhere. A weighted target outside of the vocabulary gives a NaN loss on the GPU.
+  other is padding: it counts nowhere. A weighted target outside of the vocabulary gives a NaN loss on the GPU. An
+  answer with a target of logit -inf has a score of -inf: rejected, its pair's loss is 0 (without smoothing).
 
   On the GPU the gradient is computed along with the loss (memory of the logits' size) for logits in bf16 or
   fp32; see t5x_b200/ops/token_losses.py."""

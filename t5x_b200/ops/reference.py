@@ -310,7 +310,9 @@ def preference_loss(logp, weights, reference, beta, label_smoothing, normalizer)
   real = seen.any(-1).view(-1, 2).any(-1)
   apart = scores - torch.where(real.repeat_interleave(2), reference.detach().double(), zero)
   margins = torch.where(real, beta * (apart[0::2] - apart[1::2]), zero)
-  loss = (1.0 - label_smoothing) * F.softplus(-margins) + label_smoothing * F.softplus(margins)
+  # (a side of weight 0 may be infinite: the answer that is not preferred cannot be)
+  sides = [w * F.softplus(m) for w, m in ((1.0 - label_smoothing, -margins), (label_smoothing, margins)) if w != 0]
+  loss = sum(sides[1:], sides[0])
   back = logp.dtype
   return (_over_normalizer(torch.where(real, loss, zero).sum(), normalizer).to(back), scores.detach().to(back),
           margins.detach().to(back), real.sum().to(back))

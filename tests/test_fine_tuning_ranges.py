@@ -33,3 +33,36 @@ def test_policy_of_an_impossible_token():
   out = call(0.0)
   assert out[0].item() == 0 and out[1].item() == math.inf and call(0.1)[0].item() == math.inf
   assert torch.all(torch.autograd.grad(out[0], x)[0] == 0)
+
+
+def impossible(row):
+  """Two pairs over a vocabulary of 3; the target of one token of `row` has a logit of -inf."""
+  x = torch.tensor([[[1.0, 2.0, 0.5], [0.0, -1.0, 3.0]], [[0.3, 0.2, 0.1], [2.0, 2.0, 2.0]],
+                    [[0.1, 0.2, 0.9], [0.5, 0.6, 0.1]], [[0.7, 0.1, 0.3], [0.2, 1.0, 0.4]]], dtype=torch.float64)
+  t = torch.tensor([[1, 2], [0, 1], [2, 0], [1, 1]])
+  x[row, 1, t[row, 1]] = -math.inf
+  return x.requires_grad_(), t
+
+
+@pytest.mark.parametrize("from_scores", [False, True])
+def test_preference_of_an_impossible_answer(from_scores):
+  """Rejected: margin +inf, log(1 + exp(-inf)) = 0 and no gradient; preferred: margin -inf, an infinite loss."""
+  r = torch.zeros(4)
+
+  def call(x, t, **kw):
+    if not from_scores:
+      return losses.compute_preference_loss(x, t, None, r, **kw)
+    logp = x.log_softmax(-1).gather(-1, t[..., None])[..., 0]
+    return losses.preference_loss_from_token_scores(logp, None, r, **kw)
+
+  x, t = impossible(1)
+  loss, scores, margins, pairs = call(x, t)
+  other = losses.compute_preference_loss(x[2:].detach(), t[2:], None, r[2:])[0]
+  assert loss.item() == pytest.approx(other.item(), rel=1e-12) and pairs.item() == 2
+  assert scores[1].item() == -math.inf and margins[0].item() == math.inf
+  grad = torch.autograd.grad(loss, x)[0]
+  assert torch.all(grad[:2] == 0) and torch.all(torch.isfinite(grad)) and torch.all(grad[2:] != 0)
+  assert call(x, t, label_smoothing=0.1)[0].item() == math.inf
+  x, t = impossible(0)
+  assert call(x, t)[0].item() == math.inf and call(x, t)[2][0].item() == -math.inf
+  assert call(x, t, label_smoothing=1.0)[0].item() < math.inf

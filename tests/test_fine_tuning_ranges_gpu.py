@@ -143,3 +143,35 @@ def test_policy_of_an_impossible_token(vocab):
   grad = torch.autograd.grad(out[0], x)[0]
   assert torch.all(grad[0, 0] == 0) and torch.all(torch.isfinite(grad))
   assert f(kl_weight=0.1)[0].item() == math.inf
+
+
+@pytest.mark.parametrize("vocab", [0, 5, 700, 2000, 40000])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_preference_of_an_impossible_answer(vocab, dtype):
+  """Rejected: margin +inf, loss log(1 + exp(-inf)) = 0, no gradient; preferred: an infinite loss. (vocab 0: from
+  log-probabilities)"""
+  if vocab == 0 and dtype == torch.bfloat16:
+    pytest.skip("log-probabilities are fp32")
+  d = data(4, 3, max(vocab, 5), dtype, hidden=0.0)
+  r = d["r"]
+
+  def run(row, **kw):
+    x = d["x"].detach().clone()
+    x[row, 1, d["t"][row, 1]] = -math.inf
+    if vocab:
+      x.requires_grad_()
+      return x, losses.compute_preference_loss(x, d["t"], d["w"], r, **kw)
+    x = x.float().log_softmax(-1).gather(-1, d["t"][..., None])[..., 0].requires_grad_()
+    return x, losses.preference_loss_from_token_scores(x, d["w"], r, **kw)
+
+  x, (loss, scores, margins, pairs) = run(1)
+  clean = losses.compute_preference_loss(d["x"][2:].contiguous(), d["t"][2:], d["w"][2:], r[2:])[0]
+  assert loss.item() == pytest.approx(clean.item(), rel=1e-5) and pairs.item() == 2
+  assert scores[1].item() == -math.inf and margins[0].item() == math.inf and math.isfinite(margins[1].item())
+  grad = torch.autograd.grad(loss, x)[0]
+  assert torch.all(grad[:2] == 0) and torch.all(torch.isfinite(grad)) and torch.any(grad[2:] != 0)
+  assert run(1, label_smoothing=0.1)[1][0].item() == math.inf
+  x, out = run(0)
+  assert out[0].item() == math.inf and out[2][0].item() == -math.inf
+  assert torch.all(torch.isfinite(torch.autograd.grad(out[0], x)[0]))
+  assert math.isfinite(run(0, label_smoothing=1.0)[1][0].item())
