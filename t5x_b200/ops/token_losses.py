@@ -9,6 +9,7 @@ The arguments are those of `t5x_b200.losses`, which checks them.
 """
 from __future__ import annotations
 
+import math
 from typing import Optional
 
 import torch
@@ -108,7 +109,8 @@ def _divisor(factor, device):
     return 1.0, None
   if isinstance(factor, torch.Tensor) and factor.numel() == 1 and factor.device.type != "cpu":
     return 1.0, _plain(factor.reshape(1).to(device))
-  return 1.0 / float(factor), None
+  factor = float(factor)
+  return 1.0 / factor if factor else math.copysign(math.inf, factor), None
 
 
 def policy_loss(values, targets, weights, old, advantages, reference, clip_low, clip_high, kl_weight,

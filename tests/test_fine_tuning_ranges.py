@@ -66,3 +66,12 @@ def test_preference_of_an_impossible_answer(from_scores):
   x, t = impossible(0)
   assert call(x, t)[0].item() == math.inf and call(x, t)[2][0].item() == -math.inf
   assert call(x, t, label_smoothing=1.0)[0].item() < math.inf
+
+
+def test_normalizing_factor_of_zero():
+  """No tokens in the batch: the quotient that tensor operations give, no exception."""
+  x, t, one = torch.randn(2, 3, 5), torch.zeros(2, 3, dtype=torch.long), torch.ones(2, 3)
+  for factor in (0.0, torch.tensor(0.0)):
+    assert losses.compute_preference_loss(x, t, one, torch.zeros(2), loss_normalizing_factor=factor)[0].item() == math.inf
+    assert math.isnan(losses.compute_policy_loss(x, t, 0 * one, -one, torch.ones(2),
+                                                 loss_normalizing_factor=factor)[0].item())

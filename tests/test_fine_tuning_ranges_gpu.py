@@ -175,3 +175,14 @@ def test_preference_of_an_impossible_answer(vocab, dtype):
   assert out[0].item() == math.inf and out[2][0].item() == -math.inf
   assert torch.all(torch.isfinite(torch.autograd.grad(out[0], x)[0]))
   assert math.isfinite(run(0, label_smoothing=1.0)[1][0].item())
+
+
+@pytest.mark.parametrize("host", ["1", "0"])
+def test_normalizing_factor_of_zero(host, monkeypatch):
+  """What tensor operations give, whether the factor lies on the host or on the device."""
+  from t5x_b200.ops import native
+  monkeypatch.setattr(native, "_host", None if host == "1" else False)
+  d = data(2, 3, 50, torch.float32, hidden=0.0)
+  for factor in (0.0, 0, torch.tensor(0.0), torch.tensor(0.0, device="cuda")):
+    assert call("preference", d["x"], d, factor)[0].item() == math.inf
+    assert math.isnan(call("policy", d["x"], dict(d, w=0 * d["w"]), factor)[0].item())
