@@ -21,7 +21,9 @@
 // with b2 = 0.999 a second moment moves by 0.1 % of itself per step, half a step of e4m3 is up to
 // 6 %, and rounding to nearest would never move it (it stops below a hundredth of the true value).
 // The draw is a hash of (seed, step, place in the tensor): a step repeated gives the same bits. A
-// second moment that is not zero is never stored as zero, which would divide by eps.
+// second moment that is not zero is never stored as zero, which would divide by eps. For that the scale of a
+// block with anything in it is 2^-100 at least: the smallest number of such a block is 2^-118, and arithmetic
+// here takes what lies below 2^-126 for zero.
 #include <cuda_fp8.h>
 
 #include <cmath>
@@ -35,6 +37,7 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kChunk = 2048;      // elements per CTA
 constexpr int kQuantBlock = 256;  // values that share a scale
+constexpr uint32_t kLeastScale = (127u - 100) << 23;  // the bits of 2^-100
 constexpr int kSpan = 4;          // chunks that a CTA of the norm takes in a row
 // Of a launch: what fits in 31 KB of the 32 KB that its parameters may have. (All with the items of 8 bits: 558 small
 // tensors took two launches where one is enough.)
@@ -263,10 +266,12 @@ __device__ __forceinline__ uint32_t abs_bits(float x) { return __float_as_uint(x
 // taken off again is exact. (That sum drops bits below those of the draw, which cannot carry: rounded to the
 // nearest it moved one in 60 million values across a border.) kSecond: no sign, and nothing is stored as
 // zero (the caller sees to zeros).
+// `quarter`: a quarter of the largest, inv: its reciprocal, which is a normal number for any largest (that of a largest
+// above 2^126 itself is not, and was zero).
 // (A largest that is not finite makes the whole block NaN when it is read back, as it is kept itself.)
 template <bool kSecond>
-__device__ __forceinline__ uint32_t codes2(float2 x, float most, float inv, uint32_t noise0, uint32_t noise1) {
-  const float2 y = mul2(divide2(x, both(most), both(inv)), both(448.f));
+__device__ __forceinline__ uint32_t codes2(float2 x, float quarter, float inv, uint32_t noise0, uint32_t noise1) {
+  const float2 y = mul2(divide2(x, both(quarter), both(inv)), both(112.f));
   auto shift = [](float v) {
     const float by = kSecond ? 0.015625f
                              : __uint_as_float((__float_as_uint(v) & 0x80000000u) | 0x3c800000u);
@@ -326,16 +331,18 @@ __device__ __forceinline__ Result8 step8(const Hyper& h, float clip, const Block
   }
   r.mu_most = __reduce_max_sync(0xffffffffu, r.mu_most);
   r.nu_most = __reduce_max_sync(0xffffffffu, r.nu_most);
-  const float mu_most = __uint_as_float(r.mu_most), nu_most = __uint_as_float(r.nu_most);
-  const float mu_inv = mu_most > 0.f ? __frcp_rn(mu_most) : 0.f;  // (all zeros: codes of zero)
-  const float nu_inv = nu_most > 0.f ? __frcp_rn(nu_most) : 0.f;
+  r.mu_most = r.mu_most != 0 ? max(r.mu_most, kLeastScale) : 0;
+  r.nu_most = r.nu_most != 0 ? max(r.nu_most, kLeastScale) : 0;
+  const float mu_quarter = 0.25f * __uint_as_float(r.mu_most), nu_quarter = 0.25f * __uint_as_float(r.nu_most);
+  const float mu_inv = mu_quarter > 0.f ? __frcp_rn(mu_quarter) : 0.f;  // (all zeros: codes of zero)
+  const float nu_inv = nu_quarter > 0.f ? __frcp_rn(nu_quarter) : 0.f;
   const uint32_t seed = (key + lane * 4) * kNoise1;
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     const uint32_t i = (j >> 1) * 128 + (j & 1) * 2;
     const Noise a = noise(seed + i * kNoise1), b = noise(seed + (i + 1) * kNoise1);
-    r.mu[j] = codes2<false>(m[j], mu_most, mu_inv, a.mu, b.mu);
-    r.nu[j] = codes2<true>(v[j], nu_most, nu_inv, a.nu, b.nu);
+    r.mu[j] = codes2<false>(m[j], mu_quarter, mu_inv, a.mu, b.mu);
+    r.nu[j] = codes2<true>(v[j], nu_quarter, nu_inv, a.nu, b.nu);
   }
   if (nu_least <= 0.f) {  // rare: weights that have had no gradient yet
 #pragma unroll

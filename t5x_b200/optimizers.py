@@ -234,6 +234,7 @@ def scale_by_adam(b1=0.9, b2=0.999, eps=1e-8, eps_root=0.0) -> GradientTransform
 # ---- Adam's moments in 8 bits ----
 MOMENT_BLOCK = 256  # consecutive values of a tensor that share a scale
 _E4M3_MAX = 448.0
+_LEAST_SCALE = 2.0 ** -100  # of a block with anything in it: its smallest number, 2^-118, is far from where 32 bits end
 _NOISE = (0x9E3779B1, 0x6A09E667, 0xBB67AE85)  # leading bits of the golden ratio, sqrt 2, sqrt 3
 
 
@@ -263,14 +264,16 @@ def dequantize_moment(codes: torch.Tensor, absmax: torch.Tensor) -> torch.Tensor
   return values.reshape(-1)[:codes.numel()].view(codes.shape)
 
 
-def quantize_moment(x: torch.Tensor, noise: torch.Tensor, second: bool):
+def quantize_moment(x: torch.Tensor, noise: torch.Tensor, second: bool, least_scale: float = 0.0):
   """(codes, absmax) of a moment. A value is rounded to one of the e4m3 numbers on either side of
   x / absmax * 448, up with the probability (distance to the lower) / (distance of the two), so that
   it keeps its mean: rounded to the nearest, a second moment that moves by a thousandth of itself per
   step would never move. `noise`: 16 bits a value. A second moment (`second`) above zero is stored as
-  the smallest number at least: as zero it would leave the step to be divided by eps."""
+  the smallest number at least: as zero it would leave the step to be divided by eps. `least_scale`: of blocks that
+  hold more than zeros."""
   rows = _blocks_of(x.float())
   absmax = rows.abs().amax(dim=1) if rows.numel() else rows.new_zeros(rows.shape[0])
+  absmax = torch.where(absmax == 0, absmax, absmax.clamp(min=least_scale))
   y = rows.abs() / torch.where(absmax == 0, torch.ones_like(absmax), absmax)[:, None] * _E4M3_MAX
   gap = torch.ldexp(torch.ones_like(y), (torch.frexp(y)[1] - 1).clamp(min=-6) - 3)
   up = (_blocks_of(noise).to(y.dtype) + 0.5) / 65536.0
@@ -285,7 +288,7 @@ def quantize_moment(x: torch.Tensor, noise: torch.Tensor, second: bool):
 def scale_by_adam8(b1=0.9, b2=0.999, eps=1e-8, eps_root=0.0, seed=0) -> GradientTransformation:
   """`scale_by_adam` with both moments in 8 bits: e4m3 codes (uint8, of the parameter's shape) under
   'mu' and 'nu', and the largest magnitude of every 256 consecutive values in fp32 under 'mu_absmax'
-  and 'nu_absmax'. The update is taken from the moments in 32 bits, before they are rounded (see
+  and 'nu_absmax' (2^-100 at least where there is one). The update is taken from the moments in 32 bits, before they are rounded (see
   `quantize_moment`; `seed` is that of the rounding). Needs whole parameters: not under a model or
   expert axis, nor with the optimizer sharded over replicas."""
   def init(params):
@@ -312,8 +315,8 @@ def scale_by_adam8(b1=0.9, b2=0.999, eps=1e-8, eps_root=0.0, seed=0) -> Gradient
       nu = b2 * dequantize_moment(state["nu"][k], state["nu_absmax"][k]) + (1 - b2) * (g * g)
       out[k] = (mu / bc1) / (torch.sqrt(nu / bc2 + eps_root) + eps)
       noise = _moment_noise(g.numel(), seed, c, g.device)
-      new["mu"][k], new["mu_absmax"][k] = quantize_moment(mu, noise & 0xFFFF, False)
-      new["nu"][k], new["nu_absmax"][k] = quantize_moment(nu, noise >> 16, True)
+      new["mu"][k], new["mu_absmax"][k] = quantize_moment(mu, noise & 0xFFFF, False, _LEAST_SCALE)
+      new["nu"][k], new["nu_absmax"][k] = quantize_moment(nu, noise >> 16, True, _LEAST_SCALE)
     return out, new
 
   return GradientTransformation(init, update, "scale_by_adam8",

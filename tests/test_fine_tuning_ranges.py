@@ -6,7 +6,7 @@ import math
 import pytest
 import torch
 
-from t5x_b200 import losses
+from t5x_b200 import losses, optimizers
 
 
 @pytest.mark.parametrize("kl_weight", [0.0, 0.1])
@@ -75,3 +75,35 @@ def test_normalizing_factor_of_zero():
     assert losses.compute_preference_loss(x, t, one, torch.zeros(2), loss_normalizing_factor=factor)[0].item() == math.inf
     assert math.isnan(losses.compute_policy_loss(x, t, 0 * one, -one, torch.ones(2),
                                                  loss_normalizing_factor=factor)[0].item())
+
+
+# ---- moments in 8 bits ----
+@pytest.mark.parametrize("second", [False, True])
+@pytest.mark.parametrize("largest", [1.2e-38, 1e-37, 5e-36, 1e-33, 1e-30, 1.0, 8e37, 9e37, 3.4e38])
+def test_moments_at_the_ends_of_the_range(largest, second):
+  gen = torch.Generator().manual_seed(1)
+  x = torch.rand(600, generator=gen, dtype=torch.float64) ** 4 * (1 if second else -1)
+  x[::7] *= 1 if second else -1
+  x[::50] = 0
+  x[1::256] = 1
+  x = (x * largest).float()
+  codes, absmax = optimizers.quantize_moment(x, optimizers._moment_noise(600, 3, 9, "cpu") & 0xFFFF, second,
+                                             2.0 ** -100)  # (as the step stores them)
+  back = optimizers.dequantize_moment(codes, absmax)
+  assert torch.all(torch.isfinite(back))
+  # one step of e4m3 at most: an eighth of the value, or 2^-9 / 448 of the scale
+  step = x.abs().double() / 8 + max(largest, 2.0 ** -100) / (448 * 512) * 1.001
+  assert torch.all((back.double() - x.double()).abs() <= step)
+  assert torch.all((back > 0) == (x > 0)) if second else torch.all(back.sign() * x.sign() >= 0)
+  if second:
+    assert float(back[x > 0].min()) >= 2.0 ** -118
+
+
+def test_zero_gradients_behind_smallest_ones():
+  """A second moment of 8e-44 is not zero when no gradient follows: the next steps are bounded by it, not by eps."""
+  g = {"w": torch.full((300,), 4e-22)}
+  t = optimizers.scale_by_adam8(b2=0.5, eps=1e-30)
+  state = t.init(g)
+  for i in range(60):
+    out, state = t.update(g if i == 0 else {"w": torch.zeros(300)}, state)
+    assert float(out["w"].abs().max()) < 100

@@ -6,7 +6,8 @@ import math
 import pytest
 import torch
 
-from t5x_b200 import losses
+from t5x_b200 import losses, optimizers
+from tests.test_adamw_group_gpu import adam_of, leaves, to_cpu
 from tests.test_token_losses_gpu import call, check, data, oracle_logp
 
 pytestmark = pytest.mark.gpu
@@ -186,3 +187,62 @@ def test_normalizing_factor_of_zero(host, monkeypatch):
   for factor in (0.0, 0, torch.tensor(0.0), torch.tensor(0.0, device="cuda")):
     assert call("preference", d["x"], d, factor)[0].item() == math.inf
     assert math.isnan(call("policy", d["x"], dict(d, w=0 * d["w"]), factor)[0].item())
+
+
+def chain8(**kw):
+  return optimizers.chain([optimizers._adamw8(1e-2, weight_decay=0.0, **kw)])
+
+
+def same_step(gpu, g, **kw):
+  """A step on the GPU and, from the same state, by the tensor operations on the CPU: the same weights, scales, and
+  codes but for draws beside their border (a few in 2^16, see test_8_bits_match_the_tensor_operations)."""
+  cpu = chain8(**kw).create(to_cpu(gpu.target))
+  cpu.state.param_states = to_cpu(gpu.state.param_states)
+  gpu, cpu = gpu.apply_gradient(g), cpu.apply_gradient(to_cpu(g))
+  for p, q in zip(leaves(gpu.target), leaves(cpu.target)):
+    assert torch.allclose(p.cpu(), q, rtol=2 ** -22, atol=1e-2 * 2 ** -18)
+  a, b = adam_of(gpu), adam_of(cpu)
+  for name in ("mu", "nu"):
+    for x, y in zip(leaves(a[name + "_absmax"]), leaves(b[name + "_absmax"])):
+      assert torch.allclose(x.cpu(), y, rtol=2 ** -20, atol=0, equal_nan=True)
+    for x, y in zip(leaves(a[name]), leaves(b[name])):
+      d = (x.cpu().int() - y.int()).abs()
+      assert int(d.max()) <= 1 and int((d > 0).sum()) <= 4
+  return gpu
+
+
+@pytest.mark.parametrize("host", ["1", "0"])
+@pytest.mark.parametrize("largest", [1.8e19, 1.2e19, 1e10, 1.0, 1e-10, 1e-15, 3e-18, 1e-18, 4e-19])
+def test_moments_at_the_ends_of_the_range(largest, host, monkeypatch):
+  """nu = g^2 / 2 up to 1.6e38 and down to 8e-38; every value of it is a normal number of 32 bits. Steps with no gradient
+  follow: what was stored is read back, and never as zero where it was above zero."""
+  from t5x_b200.ops import native
+  monkeypatch.setattr(native, "_host", None if host == "1" else False)
+  gen = torch.Generator(device="cuda").manual_seed(1)
+  g = torch.rand(5000, device="cuda", generator=gen) * 0.5 + 0.5
+  g = g * torch.where(torch.rand(5000, device="cuda", generator=gen) < 0.5, -1.0, 1.0) * largest
+  kw = dict(b2=0.5, eps=1e-30, seed=4)
+  gpu = chain8(**kw).create({"a": {"w": torch.zeros(5000, device="cuda"), "v": torch.zeros(5000, device="cuda")}})
+  gpu = same_step(gpu, {"a": {"w": g, "v": g.flip(0).contiguous()}}, **kw)
+  nu = leaves(adam_of(gpu)["nu"])[0]
+  # (a quarter of the largest or more, and 56, an eighth, is 0x66; the scale is 2^-100 at least)
+  assert int(nu.min()) >= (0x66 if largest > 1.3e-15 else 1)
+  none = torch.zeros(5000, device="cuda")
+  for _ in range(3):
+    before = [p.clone() for p in leaves(gpu.target)]
+    gpu = same_step(gpu, {"a": {"w": none, "v": none}}, **kw)
+    assert all(float((p - b).abs().max()) < 0.02 for p, b in zip(leaves(gpu.target), before))
+
+
+def test_small_moments_beside_a_small_largest():
+  """A block whose smallest code stands for less than a normal number of 32 bits: nothing in it reads as zero."""
+  g = torch.full((2000,), 4.5e-18, device="cuda")  # nu 2e-38
+  g[::256] = 1e-15  # nu 1e-33, a code of 1 is 4e-39
+  kw = dict(eps=1e-30, seed=4)
+  gpu = chain8(**kw).create({"w": torch.zeros(2000, device="cuda")})
+  gpu = same_step(gpu, {"w": g}, **kw)
+  for _ in range(3):
+    before = gpu.target["w"].clone()
+    gpu = same_step(gpu, {"w": torch.zeros(2000, device="cuda")}, **kw)
+    assert int(adam_of(gpu)["nu"]["w"].min()) > 0
+    assert float((gpu.target["w"] - before).abs().max()) < 0.05
