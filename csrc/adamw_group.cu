@@ -37,7 +37,8 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kChunk = 2048;      // elements per CTA
 constexpr int kQuantBlock = 256;  // values that share a scale
-constexpr uint32_t kLeastScale = (127u - 100) << 23;  // the bits of 2^-100
+// The bits of 2^-100, of infinity and of NaN.
+constexpr uint32_t kLeastScale = (127u - 100) << 23, kInfinity = 0x7f800000u, kNan = 0x7fffffffu;
 constexpr int kSpan = 4;          // chunks that a CTA of the norm takes in a row
 // Of a launch: what fits in 31 KB of the 32 KB that its parameters may have. (All with the items of 8 bits: 558 small
 // tensors took two launches where one is enough.)
@@ -268,7 +269,8 @@ __device__ __forceinline__ uint32_t abs_bits(float x) { return __float_as_uint(x
 // zero (the caller sees to zeros).
 // `quarter`: a quarter of the largest, inv: its reciprocal, which is a normal number for any largest (that of a largest
 // above 2^126 itself is not, and was zero).
-// (A largest that is not finite makes the whole block NaN when it is read back, as it is kept itself.)
+// (A largest that is not finite makes the whole block NaN when it is read back: infinity is kept as NaN, as codes other
+// than zero times infinity would be infinite second moments, steps of 0 for good.)
 template <bool kSecond>
 __device__ __forceinline__ uint32_t codes2(float2 x, float quarter, float inv, uint32_t noise0, uint32_t noise1) {
   const float2 y = mul2(divide2(x, both(quarter), both(inv)), both(112.f));
@@ -333,6 +335,8 @@ __device__ __forceinline__ Result8 step8(const Hyper& h, float clip, const Block
   r.nu_most = __reduce_max_sync(0xffffffffu, r.nu_most);
   r.mu_most = r.mu_most != 0 ? max(r.mu_most, kLeastScale) : 0;
   r.nu_most = r.nu_most != 0 ? max(r.nu_most, kLeastScale) : 0;
+  if (r.mu_most == kInfinity) r.mu_most = kNan;
+  if (r.nu_most == kInfinity) r.nu_most = kNan;
   const float mu_quarter = 0.25f * __uint_as_float(r.mu_most), nu_quarter = 0.25f * __uint_as_float(r.nu_most);
   const float mu_inv = mu_quarter > 0.f ? __frcp_rn(mu_quarter) : 0.f;  // (all zeros: codes of zero)
   const float nu_inv = nu_quarter > 0.f ? __frcp_rn(nu_quarter) : 0.f;

@@ -270,10 +270,11 @@ def quantize_moment(x: torch.Tensor, noise: torch.Tensor, second: bool, least_sc
   it keeps its mean: rounded to the nearest, a second moment that moves by a thousandth of itself per
   step would never move. `noise`: 16 bits a value. A second moment (`second`) above zero is stored as
   the smallest number at least: as zero it would leave the step to be divided by eps. `least_scale`: of blocks that
-  hold more than zeros."""
+  hold more than zeros. A block with a value that is not finite is NaN when it is read back."""
   rows = _blocks_of(x.float())
   absmax = rows.abs().amax(dim=1) if rows.numel() else rows.new_zeros(rows.shape[0])
   absmax = torch.where(absmax == 0, absmax, absmax.clamp(min=least_scale))
+  absmax = torch.where(torch.isinf(absmax), math.nan, absmax)
   y = rows.abs() / torch.where(absmax == 0, torch.ones_like(absmax), absmax)[:, None] * _E4M3_MAX
   gap = torch.ldexp(torch.ones_like(y), (torch.frexp(y)[1] - 1).clamp(min=-6) - 3)
   up = (_blocks_of(noise).to(y.dtype) + 0.5) / 65536.0
@@ -288,9 +289,10 @@ def quantize_moment(x: torch.Tensor, noise: torch.Tensor, second: bool, least_sc
 def scale_by_adam8(b1=0.9, b2=0.999, eps=1e-8, eps_root=0.0, seed=0) -> GradientTransformation:
   """`scale_by_adam` with both moments in 8 bits: e4m3 codes (uint8, of the parameter's shape) under
   'mu' and 'nu', and the largest magnitude of every 256 consecutive values in fp32 under 'mu_absmax'
-  and 'nu_absmax' (2^-100 at least where there is one). The update is taken from the moments in 32 bits, before they are rounded (see
-  `quantize_moment`; `seed` is that of the rounding). Needs whole parameters: not under a model or
-  expert axis, nor with the optimizer sharded over replicas."""
+  and 'nu_absmax' (2^-100 at least where a block holds more than zeros, NaN where it is not finite). The
+  update is taken from the moments in 32 bits, before they are rounded (see `quantize_moment`; `seed` is
+  that of the rounding). Needs whole parameters: not under a model or expert axis, nor with the optimizer
+  sharded over replicas."""
   def init(params):
     from t5x_b200.parallel import state as pstate
     st = pstate.get()

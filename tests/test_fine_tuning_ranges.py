@@ -107,3 +107,16 @@ def test_zero_gradients_behind_smallest_ones():
   for i in range(60):
     out, state = t.update(g if i == 0 else {"w": torch.zeros(300)}, state)
     assert float(out["w"].abs().max()) < 100
+
+
+def test_overflowing_second_moment_shows():
+  """A square beyond 32 bits: its block is NaN when it is read back, as behind a NaN, not a step of 0 for good."""
+  w = {"w": torch.ones(600)}
+  opt = optimizers.adamw8(1e-2, weight_decay=0.0).create(w)
+  g = torch.ones(600)
+  g[300] = 1e20
+  opt = opt.apply_gradient({"w": g})
+  assert torch.all(torch.isfinite(opt.target["w"]))
+  assert torch.isnan(opt.state.param_states["0"]["nu_absmax"]["w"]).tolist() == [False, True, False]
+  opt = opt.apply_gradient({"w": torch.ones(600)})
+  assert torch.isnan(opt.target["w"]).nonzero().flatten().tolist() == list(range(256, 512))

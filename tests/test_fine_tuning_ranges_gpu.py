@@ -246,3 +246,17 @@ def test_small_moments_beside_a_small_largest():
     gpu = same_step(gpu, {"w": torch.zeros(2000, device="cuda")}, **kw)
     assert int(adam_of(gpu)["nu"]["w"].min()) > 0
     assert float((gpu.target["w"] - before).abs().max()) < 0.05
+
+
+@pytest.mark.parametrize("size", [600, 601])
+def test_overflowing_second_moment_shows(size):
+  """A square beyond 32 bits: its block is NaN when it is read back, as behind a NaN, not a step of 0 for good."""
+  w = {"w": torch.ones(size, device="cuda")}
+  opt = optimizers.adamw8(1e-2, weight_decay=0.0).create(w)
+  g = torch.ones(size, device="cuda")
+  g[300] = 1e20
+  opt = opt.apply_gradient({"w": g})
+  assert torch.all(torch.isfinite(opt.target["w"]))
+  assert torch.isnan(adam_of(opt)["nu_absmax"]["w"]).tolist() == [False, True, False]
+  opt = opt.apply_gradient({"w": torch.ones(size, device="cuda")})
+  assert torch.isnan(opt.target["w"]).nonzero().flatten().tolist() == list(range(256, 512))
