@@ -984,12 +984,20 @@ bool scalar(const Tensor& x, const optional<Tensor>& t) {
   return !t || (t->scalar_type() == at::kFloat && t->numel() == 1 && t->device() == x.device());
 }
 
-// Memory for the gradient: the same strides, at the same place of 16 bytes.
-Tensor gradient_like(const Tensor& x) {
+// Memory of x's type and sizes, of those strides, at the same place of 16 bytes.
+Tensor at_place_of(const Tensor& x, c10::IntArrayRef strides) {
   const int64_t behind = static_cast<int64_t>(reinterpret_cast<uintptr_t>(x.data_ptr()) % 16 / x.element_size());
   int64_t span = 1;
-  for (int64_t i = 0; i < x.dim(); ++i) span += (x.size(i) - 1) * x.stride(i);
-  return at::empty({span + behind}, x.options()).as_strided(x.sizes(), x.strides(), behind);
+  for (int64_t i = 0; i < x.dim(); ++i) span += (x.size(i) - 1) * strides[i];
+  return at::empty({span + behind}, x.options()).as_strided(x.sizes(), strides, behind);
+}
+
+// Memory for the gradient of a loss's values.
+Tensor gradient_of(const Tensor& x, const LossValues& s) {
+  if (x.dim() == 2) return at_place_of(x, x.strides());
+  long long strides[2];
+  t5x_loss_gradient_strides(s.l, s.v, s.fp32, s.stride_b, s.stride_t, strides);
+  return at_place_of(x, {strides[0], strides[1], 1});
 }
 
 Tensor bytes_like(const Tensor& x, int64_t n) { return at::empty({n}, x.options().dtype(at::kByte)); }
@@ -999,7 +1007,7 @@ optional<Tensor> scale_gradient(const Tensor& grad, const Tensor& factor, bool k
   if (!grad.is_cuda() || grad.get_device() != c10::cuda::current_device() || !scalar(grad, factor) ||
       grad.numel() == 0)
     return std::nullopt;
-  Tensor to = keep ? gradient_like(grad) : grad;
+  Tensor to = keep ? at_place_of(grad, grad.strides()) : grad;
   int64_t span = 1;
   for (int64_t i = 0; i < grad.dim(); ++i) span += (grad.size(i) - 1) * grad.stride(i);
   check(t5x_scale_gradient(grad.data_ptr(), to.data_ptr(), span, grad.scalar_type() == at::kFloat,
@@ -1067,7 +1075,7 @@ std::vector<Tensor> policy_loss(const Tensor& x, const optional<Tensor>& targets
     adv_t = advantages.stride(1);
   }
   return run_loss(x, [&](bool wanted) -> std::vector<Tensor> {
-    Tensor grad = wanted ? gradient_like(x) : Tensor();
+    Tensor grad = wanted ? gradient_of(x, s) : Tensor();
     void* g = wanted ? grad.data_ptr() : nullptr;
     Tensor scratch = bytes_like(x, t5x_policy_loss_scratch_bytes());
     Tensor out = at::empty({4}, x.options().dtype(at::kFloat));
@@ -1096,7 +1104,7 @@ std::vector<Tensor> preference_loss(const Tensor& x, const optional<Tensor>& tar
       !reference.is_contiguous())
     return {};
   return run_loss(x, [&](bool wanted) -> std::vector<Tensor> {
-    Tensor grad = wanted ? gradient_like(x) : Tensor();
+    Tensor grad = wanted ? gradient_of(x, s) : Tensor();
     void* g = wanted ? grad.data_ptr() : nullptr;
     Tensor scratch = bytes_like(x, t5x_preference_loss_scratch_bytes(s.b, s.l, s.v, s.fp32));
     const auto floats = x.options().dtype(at::kFloat);

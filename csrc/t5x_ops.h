@@ -90,11 +90,15 @@ int t5x_grad_clip_scale(const t5x_adamw_item* items, int count, void* scratch, f
                         void* clip_scale, void* stream);
 
 /* Losses over logits [batch, length, vocab] (fp32 or bf16; strides in values, last dimension contiguous)
- * with their gradient in `grad` (the same strides and place of 16 bytes, or null), and over
+ * with their gradient in `grad` (of the strides of t5x_loss_gradient_strides, that is the logits' own where their
+ * rows lie side by side, and at the same place of 16 bytes; or null), and over
  * log-probabilities [batch, length] (fp32) with theirs in `slope` (or null): see token_losses.cu.
  * targets int64, weights fp32 (or null: all 1), other inputs fp32. normalizer: device scalar that divides
  * the loss, or null: `scale` multiplies it. scratch: the stated bytes, 16-byte aligned. policy: out = loss,
  * kl, clipped, weight. preference: scores [batch], margins [batch / 2], out = loss, pairs. */
+/* strides: of batch and length */
+void t5x_loss_gradient_strides(int length, int vocab, int fp32, long long stride_b, long long stride_t,
+                               long long* strides);
 long long t5x_policy_loss_scratch_bytes();
 int t5x_policy_loss(const void* logits, int fp32, void* grad, long long batch, int length, int vocab,
                     long long stride_b, long long stride_t, const void* targets, const void* weights,

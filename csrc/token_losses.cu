@@ -190,13 +190,18 @@ __device__ __forceinline__ Softmax join_lanes(Softmax s) {
 struct Rows {
   long long rows;  // B * L
   int length, vocab;
-  long long stride_b, stride_t;  // in values, of the logits and of their gradient
+  long long stride_b, stride_t;  // in values, of the logits
+  long long grad_b, grad_t;      // of their gradient
   const long long* targets;
   const float* weights;  // null: all 1
 };
-__device__ __forceinline__ long long row_at(const Rows& r, long long row) {
-  const long long b = row / r.length;
-  return b * r.stride_b + (row - b * r.length) * r.stride_t;
+// Where a row of the logits and of their gradient begins.
+struct RowAt {
+  long long b, logits, grad;
+};
+__device__ __forceinline__ RowAt row_at(const Rows& r, long long row) {
+  const long long b = row / r.length, t = row - b * r.length;
+  return {b, b * r.stride_b + t * r.stride_t, b * r.grad_b + t * r.grad_t};
 }
 
 // Sums over the threads of the CTA, in every thread, in a fixed order.
@@ -313,15 +318,15 @@ __global__ void __launch_bounds__(kRowThreads)
   for (long long row = blockIdx.x * static_cast<long long>(kRowThreads / 32) + (threadIdx.x >> 5); row < r.rows;
        row += warps) {
     const float w = r.weights != nullptr ? r.weights[row] : 1.f;
-    const long long at = row_at(r, row);
+    const RowAt at = row_at(r, row);
     if (w == 0.f) {
-      if (grad != nullptr) row_zero(grad + at, r.vocab, lane, 32);
+      if (grad != nullptr) row_zero(grad + at.grad, r.vocab, lane, 32);
       continue;
     }
-    const long long target = r.targets[row], b = row / r.length;
-    const PolicyInputs in = policy_inputs(p, row, b, row - b * r.length);
-    const Softmax s = join_lanes(row_softmax(logits + at, r.vocab, lane, 32));
-    const float logp = log_prob(logits + at, r.vocab, target, s);
+    const long long target = r.targets[row];
+    const PolicyInputs in = policy_inputs(p, row, at.b, row - at.b * r.length);
+    const Softmax s = join_lanes(row_softmax(logits + at.logits, r.vocab, lane, 32));
+    const float logp = log_prob(logits + at.logits, r.vocab, target, s);
     const PolicyToken k = policy_token(p, in, logp);
     if (lane == 0) {
       sums[0] += static_cast<double>(w) * k.loss;
@@ -330,7 +335,7 @@ __global__ void __launch_bounds__(kRowThreads)
       sums[3] += w;
     }
     if (grad != nullptr)
-      row_gradient(logits + at, grad + at, r.vocab, s,
+      row_gradient(logits + at.logits, grad + at.grad, r.vocab, s,
                    target >= 0 && target < r.vocab ? static_cast<int>(target) : -1, w * k.slope * scale, lane, 32);
   }
   policy_finish(sums, p, partial, arrived, out);
@@ -378,11 +383,11 @@ __global__ void __launch_bounds__(kRowThreads)
   for (long long row = blockIdx.x * static_cast<long long>(kRowThreads / 32) + (threadIdx.x >> 5); row < r.rows;
        row += warps) {
     if (r.weights != nullptr && r.weights[row] == 0.f) continue;
-    const long long at = row_at(r, row);
-    const Softmax s = join_lanes(row_softmax(logits + at, r.vocab, lane, 32));
+    const T* x = logits + row_at(r, row).logits;
+    const Softmax s = join_lanes(row_softmax(x, r.vocab, lane, 32));
     if (lane == 0) {
       softmax[row] = s;
-      logp[row] = log_prob(logits + at, r.vocab, r.targets[row], s);
+      logp[row] = log_prob(x, r.vocab, r.targets[row], s);
     }
   }
 }
@@ -420,14 +425,14 @@ __global__ void __launch_bounds__(kRowThreads)
   for (long long row = blockIdx.x * static_cast<long long>(kRowThreads / 32) + (threadIdx.x >> 5); row < r.rows;
        row += warps) {
     const float w = r.weights != nullptr ? r.weights[row] : 1.f;
-    const long long at = row_at(r, row);
+    const RowAt at = row_at(r, row);
     if (w == 0.f) {
-      row_zero(grad + at, r.vocab, lane, 32);
+      row_zero(grad + at.grad, r.vocab, lane, 32);
       continue;
     }
     const long long target = r.targets[row];
-    row_gradient(logits + at, grad + at, r.vocab, softmax[row],
-                 target >= 0 && target < r.vocab ? static_cast<int>(target) : -1, w * by[row / r.length], lane, 32);
+    row_gradient(logits + at.logits, grad + at.grad, r.vocab, softmax[row],
+                 target >= 0 && target < r.vocab ? static_cast<int>(target) : -1, w * by[at.b], lane, 32);
   }
 }
 
@@ -814,8 +819,9 @@ struct LongArgs {
 
 // What there is to know of a row.
 struct alignas(16) RowFacts {
-  long long offset;   // of its first value
-  int first, packs;   // the CTA's part: its first value, its number of 16 bytes
+  const void* x;     // its first value
+  void* g;           // its gradient's
+  int first, packs;  // the CTA's part: its first value, its number of 16 bytes
   long long target;
   float weight;
   // policy: old score, reference score, advantage; gradients: softmax, slope of the sequence
@@ -855,12 +861,13 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads)
       f.weight = 0.f;
       return;
     }
-    const long long offset = b * r.stride_b + t * r.stride_t;
+    const T* x = logits + (b * r.stride_b + t * r.stride_t);
     // the row's part between 16-byte boundaries, and of that this CTA's
-    const int off = static_cast<int>(reinterpret_cast<uintptr_t>(logits + offset) & 15) / static_cast<int>(sizeof(T));
+    const int off = static_cast<int>(reinterpret_cast<uintptr_t>(x) & 15) / static_cast<int>(sizeof(T));
     const int head = off ? kN - off : 0, all = (r.vocab - head) / kN;
     const int size = (all + ctas - 1) >> a.shift, from = min(size * rank, all);
-    f.offset = offset;
+    f.x = x;
+    f.g = grad + (b * r.grad_b + t * r.grad_t);
     f.first = head + from * kN;
     f.packs = min(all - from, size);
     fetch<8>(smem_u32(&f.target), r.targets + row);
@@ -889,17 +896,16 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads)
   __syncthreads();
   if (a.shift) cluster_sync_all();  // all CTAs have begun before any writes to another
   auto ask_row = [&](const RowFacts& f) {
-    if (f.weight != 0.f) Chunk::ask(slots, logits + f.offset + f.first, min(f.packs, kChunk), tid);
+    if (f.weight != 0.f) Chunk::ask(slots, static_cast<const T*>(f.x) + f.first, min(f.packs, kChunk), tid);
   };
   ask_row(facts[0]);
   int turn = 0;
   for (int k = 0; k < mine_of_all; ++k) {
     const RowFacts& f = facts[k & 3];
     const float w = f.weight;
-    const long long offset = f.offset;
     const int first = f.first, packs = f.packs;
-    const T* x = logits + offset;
-    T* g = grad + offset;
+    const T* x = static_cast<const T*>(f.x);
+    T* g = static_cast<T*>(f.g);
     // The value in front of the first 16-byte boundary or behind the last that the thread sees to, or -1.
     int outside = -1;
     if (warp == 0 && rank == 0) {
@@ -1084,6 +1090,15 @@ int check_rows(const char* what, const void* logits, int fp32, const void* grad,
   return 0;
 }
 
+// The gradient's strides: rows side by side, but for the few values that put each at its logits' place of 16 bytes.
+void gradient_strides(int length, int vocab, int fp32, long long stride_b, long long stride_t, long long* grad_b,
+                      long long* grad_t) {
+  const long long pack = fp32 ? 4 : 8;
+  auto fill = [&](long long like, long long least) { return least + ((like - least) % pack + pack) % pack; };
+  *grad_t = fill(stride_t, vocab);
+  *grad_b = fill(stride_b, (length - 1) * *grad_t + vocab);
+}
+
 unsigned row_grid(long long rows) {
   const long long ctas = (rows + kRowThreads / 32 - 1) / (kRowThreads / 32);
   const long long cap = static_cast<long long>(num_sms()) * 4;
@@ -1182,6 +1197,11 @@ constexpr size_t kHead = 16;  // bytes of scratch in front: the count of arrived
 
 using namespace t5x;
 
+T5X_API void t5x_loss_gradient_strides(int length, int vocab, int fp32, long long stride_b, long long stride_t,
+                                       long long* strides) {
+  gradient_strides(length, vocab, fp32, stride_b, stride_t, strides, strides + 1);
+}
+
 T5X_API long long t5x_policy_loss_scratch_bytes() {
   return static_cast<long long>(kHead) + 4ll * 8 * num_sms() * kCtasPerSm;  // (four sums of each CTA)
 }
@@ -1199,8 +1219,9 @@ T5X_API int t5x_policy_loss(const void* logits, int fp32, void* grad, long long 
   if (e != cudaSuccess) return set_error("policy_loss: memset: %s", cudaGetErrorString(e));
   unsigned* arrived = static_cast<unsigned*>(scratch);
   double* partial = reinterpret_cast<double*>(static_cast<char*>(scratch) + kHead);
-  const Rows r = {batch * length, length, vocab, stride_b, stride_t, static_cast<const long long*>(targets),
-                  static_cast<const float*>(weights)};
+  Rows r = {batch * length, length, vocab, stride_b, stride_t, 0, 0, static_cast<const long long*>(targets),
+            static_cast<const float*>(weights)};
+  gradient_strides(length, vocab, fp32, stride_b, stride_t, &r.grad_b, &r.grad_t);
   const Policy p = {static_cast<const float*>(old_scores), static_cast<const float*>(ref_scores),
                     static_cast<const float*>(advantages), adv_b, adv_t, 1.f - clip_low, 1.f + clip_high,
                     kl_weight, scale, static_cast<const float*>(normalizer)};
@@ -1236,7 +1257,7 @@ T5X_API int t5x_policy_loss_tokens(const void* logp, void* slope, long long batc
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   cudaError_t e = cudaMemsetAsync(scratch, 0, kHead, st);
   if (e != cudaSuccess) return set_error("policy_loss_tokens: memset: %s", cudaGetErrorString(e));
-  const Rows r = {batch * length, length, 1, 0, 0, nullptr, static_cast<const float*>(weights)};
+  const Rows r = {batch * length, length, 1, 0, 0, 0, 0, nullptr, static_cast<const float*>(weights)};
   const Policy p = {static_cast<const float*>(old_scores), static_cast<const float*>(ref_scores),
                     static_cast<const float*>(advantages), adv_b, adv_t, 1.f - clip_low, 1.f + clip_high,
                     kl_weight, scale, static_cast<const float*>(normalizer)};
@@ -1267,8 +1288,9 @@ T5X_API int t5x_preference_loss(const void* logits, int fp32, void* grad, long l
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const long long pairs = batch / 2;
   char* at = static_cast<char*>(scratch);
-  const Rows r = {batch * length, length, vocab, stride_b, stride_t, static_cast<const long long*>(targets),
-                  static_cast<const float*>(weights)};
+  Rows r = {batch * length, length, vocab, stride_b, stride_t, 0, 0, static_cast<const long long*>(targets),
+            static_cast<const float*>(weights)};
+  gradient_strides(length, vocab, fp32, stride_b, stride_t, &r.grad_b, &r.grad_t);
   const Preference p = {static_cast<const float*>(reference), beta, smoothing, scale,
                         static_cast<const float*>(normalizer)};
   unsigned* arrived = reinterpret_cast<unsigned*>(at);
@@ -1316,7 +1338,7 @@ T5X_API int t5x_preference_loss_tokens(const void* logp, void* slope, long long 
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   cudaError_t e = cudaMemsetAsync(scratch, 0, kHead, st);
   if (e != cudaSuccess) return set_error("preference_loss_tokens: memset: %s", cudaGetErrorString(e));
-  const Rows r = {batch * length, length, 1, 0, 0, nullptr, static_cast<const float*>(weights)};
+  const Rows r = {batch * length, length, 1, 0, 0, 0, 0, nullptr, static_cast<const float*>(weights)};
   const Preference p = {static_cast<const float*>(reference), beta, smoothing, scale,
                         static_cast<const float*>(normalizer)};
   preference_pairs_kernel<<<static_cast<unsigned>(batch / 2), kRowThreads, 0, st>>>(

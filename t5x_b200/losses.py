@@ -213,8 +213,8 @@ def compute_preference_loss(logits: torch.Tensor, targets: torch.Tensor, weights
   other is padding: it counts nowhere. A weighted target outside of the vocabulary gives a NaN loss on the GPU. An
   answer with a target of logit -inf has a score of -inf: rejected, its pair's loss is 0 (without smoothing).
 
-  On the GPU the gradient is computed along with the loss (memory of the logits' size) for logits in bf16 or
-  fp32; see t5x_b200/ops/token_losses.py."""
+  On the GPU the gradient is computed along with the loss (memory of the logits' size, also where they are a view of
+  something larger) for logits in bf16 or fp32; see t5x_b200/ops/token_losses.py."""
   from t5x_b200.ops import token_losses
   what = "compute_preference_loss"
   _check_tokens(what, logits, 3, targets=targets, weights=weights)

@@ -1209,6 +1209,7 @@ register_signature("t5x_preference_loss", [c_void_p, c_int, c_void_p, c_ll, c_in
                    [c_float] * 3 + [c_void_p] * 6)
 register_signature("t5x_preference_loss_tokens", [c_void_p, c_void_p, c_ll, c_int, c_void_p, c_void_p] +
                    [c_float] * 3 + [c_void_p] * 6)
+register_signature("t5x_loss_gradient_strides", [c_int, c_int, c_int, c_ll, c_ll, c_void_p])
 register_signature("t5x_scale_gradient", [c_void_p, c_void_p, c_ll, c_int, c_void_p, c_void_p])
 
 
@@ -1228,8 +1229,9 @@ def _loss_inputs(what: str, values, grad, targets, weights, *more):
   ok = ok and (targets is None or values.shape[2] == 1 or values.stride(2) == 1)
   for t, dtype in [(targets, torch.int64), (weights, torch.float32)] + [(m, torch.float32) for m in more]:
     ok = ok and (t is None or (t.dtype == dtype and t.shape == shape and t.device == dev and t.is_contiguous()))
-  ok = ok and (grad is None or (grad.shape == values.shape and grad.stride() == values.stride() and
-                                grad.dtype == values.dtype and grad.device == dev))
+  ok = ok and (grad is None or (grad.shape == values.shape and grad.dtype == values.dtype and grad.device == dev))
+  if ok and grad is not None:
+    ok = grad.stride() == (values.stride() if targets is None else loss_gradient_strides(values))
   if not ok:
     raise NativeError(f"{what}: operands must be tensors of one device whose types and shapes fit")
 
@@ -1239,6 +1241,15 @@ def _loss_strides(t: torch.Tensor):
   b, l, v = t.shape
   st = t.stride(1) if l > 1 else v
   return (t.stride(0) if b > 1 else (l - 1) * st + v), st
+
+
+def loss_gradient_strides(logits: torch.Tensor):
+  """The strides that the losses give the gradient of `logits` [B, L, V]: rows side by side, but for the few values that
+  put each at its logits' place of 16 bytes."""
+  out = (c_ll * 2)()
+  _, l, v = logits.shape
+  lib().t5x_loss_gradient_strides(l, v, int(logits.dtype == torch.float32), *_loss_strides(logits), out)
+  return out[0], out[1], 1
 
 
 def policy_loss(values, grad, targets, weights, old, advantages, reference, clip_low, clip_high, kl_weight, scale,

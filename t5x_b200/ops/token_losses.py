@@ -31,14 +31,14 @@ def _rows_apart(logits: torch.Tensor) -> torch.Tensor:
   return logits.contiguous()
 
 
-def _like(logits: torch.Tensor) -> torch.Tensor:
-  """Memory for the gradient of `logits`: the same strides, at the same place of 16 bytes, so that the
-  kernel's wide accesses fall on the same values of both."""
-  size = logits.element_size()
-  behind = logits.data_ptr() % 16 // size
-  span = sum((n - 1) * s for n, s in zip(logits.shape, logits.stride())) + 1
-  flat = torch.empty(span + behind, dtype=logits.dtype, device=logits.device)
-  return flat.as_strided(logits.shape, logits.stride(), behind)
+def _like(values: torch.Tensor) -> torch.Tensor:
+  """Memory for the gradient of `values`: of their size, whatever their strides, at the same place of 16 bytes, so that
+  the kernel's wide accesses fall on the same values of both."""
+  strides = native.loss_gradient_strides(values) if values.dim() == 3 else values.stride()
+  behind = values.data_ptr() % 16 // values.element_size()
+  span = sum((n - 1) * s for n, s in zip(values.shape, strides)) + 1
+  flat = torch.empty(span + behind, dtype=values.dtype, device=values.device)
+  return flat.as_strided(values.shape, strides, behind)
 
 
 def _times(grad: torch.Tensor, factor: Optional[torch.Tensor]) -> Optional[torch.Tensor]:

@@ -260,3 +260,51 @@ def test_overflowing_second_moment_shows(size):
   assert torch.isnan(adam_of(opt)["nu_absmax"]["w"]).tolist() == [False, True, False]
   opt = opt.apply_gradient({"w": torch.ones(size, device="cuda")})
   assert torch.isnan(opt.target["w"]).nonzero().flatten().tolist() == list(range(256, 512))
+
+
+@pytest.mark.parametrize("host", ["1", "0"])
+@pytest.mark.parametrize("kind", ["preference", "policy"])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("vocab", [501, 4001, 40003])
+def test_gradient_of_a_view_takes_the_memory_of_its_values(kind, dtype, vocab, host, monkeypatch):
+  """The last tokens of much longer rows, a part of a much larger vocabulary: values as those of a copy, memory of the
+  values' own size (and up to 16 bytes a row)."""
+  from t5x_b200.ops import native
+  monkeypatch.setattr(native, "_host", None if host == "1" else False)
+  d = data(4, 5, vocab, dtype)
+  big = torch.empty(4, 60, 2 * vocab + 3, dtype=dtype, device="cuda")
+  big[:, 50:55, 7:7 + vocab] = d["x"]
+  for view in (big[:, 50:55, 7:7 + vocab].detach(), big[:, 50:55, 7:7 + vocab].detach()[::2], d["x"].detach()):
+    e = d if view.shape[0] == 4 else {k: v[::2].contiguous() for k, v in d.items()}
+    e = dict(e, x=view.contiguous())
+    leaf = view.requires_grad_()
+    call(kind, leaf, e, None)  # (what is allocated once)
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    torch.cuda.reset_peak_memory_stats()
+    out = call(kind, leaf, e, None)
+    grad = torch.autograd.grad(out[0], leaf, retain_graph=True)[0]
+    peak = torch.cuda.max_memory_allocated() - before
+    # twice (the graph is kept), 16 bytes a row, each rounded up by the allocator; scratch
+    rows = view.shape[0] * 5
+    assert peak <= 2 * (view.numel() * view.element_size() + 16 * rows + 16) + (4 << 20) and grad.shape == view.shape
+    check(kind, out, grad, e, 1.0)
+    assert torch.equal(torch.autograd.grad(out[0], leaf)[0], grad)
+
+
+def test_gradient_beyond_32_bits():
+  """More than 2^31 values; the tokens that count lie at the end."""
+  length, vocab, few = 34000, 32128, 3
+  d = data(2, few, vocab, torch.bfloat16, hidden=0.0)
+  x = torch.empty(2, length, vocab, dtype=torch.bfloat16, device="cuda")
+  assert x[1].storage_offset() + (length - few) * vocab > 2 ** 31
+  x[:, -few:] = d["x"]
+  pad = lambda v, fill=0.0: torch.nn.functional.pad(v, (length - few, 0), value=fill)  # noqa: E731
+  for kind in ("preference", "policy"):
+    e = dict(d, **{k: pad(d[k]) for k in ("w", "old", "adv", "ref")}, t=pad(d["t"], 0))
+    leaf = x.detach().requires_grad_()
+    out = call(kind, leaf, e, None)
+    grad = torch.autograd.grad(out[0], leaf)[0]
+    check(kind, out, grad[:, -few:], d, 1.0)
+    assert not torch.any(grad[0, :-few]) and not torch.any(grad[1, :-few])
+    del leaf, out, grad
