@@ -3,7 +3,7 @@
 On CUDA, over bf16 or fp32 logits or fp32 log-probabilities, the kernels of csrc/token_losses.cu
 compute the loss and, where a gradient will be wanted, the gradient in the same pass; backward
 multiplies it by the gradient of the loss (which leaves it alone where that is 1). Anything else
-runs the PyTorch statements in :mod:`t5x_b200.ops.reference`.
+runs the PyTorch statements in :mod:`t5x_b200.ops.reference`, as do calls under a function transform.
 
 The arguments are those of `t5x_b200.losses`, which checks them.
 """
@@ -19,8 +19,11 @@ from t5x_b200.ops import native
 from t5x_b200.ops import reference as ref
 
 
-def _native_logits(logits: torch.Tensor) -> bool:
-  return logits.is_cuda and logits.dtype in (torch.bfloat16, torch.float32) and logits.numel() > 0
+def _native_ok(values: torch.Tensor, targets: Optional[torch.Tensor]) -> bool:
+  """Whether the kernels take the values. (A function transform, a forward-mode level or a trace sees into the statements,
+  not into the kernels.)"""
+  types = (torch.float32,) if targets is None else (torch.bfloat16, torch.float32)
+  return values.is_cuda and values.dtype in types and values.numel() > 0 and not F._transformed()
 
 
 def _rows_apart(logits: torch.Tensor) -> torch.Tensor:
@@ -63,7 +66,7 @@ def _loss(ctx, name, values, targets, *args):
 def _run(fn, name, *args):
   """The loss by the compiled host path, which makes its own node of the graph, or else by `fn`."""
   host = native.host()
-  if host is not None and not F._transformed():
+  if host is not None:
     out = getattr(host, name)(*args)
     if out:
       return tuple(out)
@@ -117,11 +120,7 @@ def policy_loss(values, targets, weights, old, advantages, reference, clip_low, 
                 normalizer):
   """(loss, kl, clipped, weight); values: logits [B, L, V], or log-probabilities [B, L] with targets
   None."""
-  if targets is None:
-    native_ok = values.is_cuda and values.dtype == torch.float32 and values.numel() > 0
-  else:
-    native_ok = _native_logits(values)
-  if not native_ok:
+  if not _native_ok(values, targets):
     logp = values if targets is None else ref.token_log_probs(values, targets, weights)
     return ref.policy_loss(logp, weights, old, advantages, reference, clip_low, clip_high, kl_weight,
                            normalizer)
@@ -132,11 +131,7 @@ def policy_loss(values, targets, weights, old, advantages, reference, clip_low, 
 
 def preference_loss(values, targets, weights, reference, beta, label_smoothing, normalizer):
   """(loss, scores, margins, pairs); values as in `policy_loss`, rows 2j and 2j + 1 a pair."""
-  if targets is None:
-    native_ok = values.is_cuda and values.dtype == torch.float32 and values.numel() > 0
-  else:
-    native_ok = _native_logits(values)
-  if not native_ok:
+  if not _native_ok(values, targets):
     logp = values if targets is None else ref.token_log_probs(values, targets, weights)
     return ref.preference_loss(logp, weights, reference, beta, label_smoothing, normalizer)
   scale, divisor = _divisor(normalizer, values.device)

@@ -77,6 +77,18 @@ def test_normalizing_factor_of_zero():
                                                  loss_normalizing_factor=factor)[0].item())
 
 
+def test_function_transforms():
+  gen = torch.Generator().manual_seed(0)
+  x = torch.randn(4, 3, 7, generator=gen, dtype=torch.float64)
+  t = torch.randint(0, 7, (4, 3), generator=gen)
+  r, old = torch.randn(4, generator=gen), -2 + torch.randn(4, 3, generator=gen)
+  for loss in (lambda v: losses.compute_preference_loss(v, t, None, r)[0],
+               lambda v: losses.compute_policy_loss(v, t, None, old, r)[0]):
+    leaf = x.clone().requires_grad_()
+    want = torch.autograd.grad(loss(leaf), leaf)[0]
+    assert torch.allclose(torch.func.grad(loss)(x), want, rtol=1e-12, atol=1e-15)
+
+
 # ---- moments in 8 bits ----
 @pytest.mark.parametrize("second", [False, True])
 @pytest.mark.parametrize("largest", [1.2e-38, 1e-37, 5e-36, 1e-33, 1e-30, 1.0, 8e37, 9e37, 3.4e38])

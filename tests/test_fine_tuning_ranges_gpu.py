@@ -308,3 +308,20 @@ def test_gradient_beyond_32_bits():
     check(kind, out, grad[:, -few:], d, 1.0)
     assert not torch.any(grad[0, :-few]) and not torch.any(grad[1, :-few])
     del leaf, out, grad
+
+
+@pytest.mark.parametrize("host", ["1", "0"])
+def test_function_transforms(host, monkeypatch):
+  """Under `torch.func` the statements run, which can be transformed."""
+  from t5x_b200.ops import native
+  monkeypatch.setattr(native, "_host", None if host == "1" else False)
+  d = data(4, 3, 50, torch.float32)
+  for kind in ("preference", "policy"):
+    loss = lambda v: call(kind, v, d, 2.0)[0]  # noqa: E731
+    leaf = d["x"].clone().requires_grad_()
+    want = torch.autograd.grad(loss(leaf), leaf)[0]
+    got = torch.func.grad(loss)(d["x"])
+    assert torch.allclose(got, want, rtol=1e-4, atol=1e-6)
+    along = torch.randn_like(d["x"])
+    slope = torch.func.jvp(loss, (d["x"],), (along,))[1]
+    assert float(slope) == pytest.approx(float((want * along).sum()), rel=1e-4, abs=1e-5)
