@@ -95,8 +95,8 @@ __device__ __forceinline__ void over_row(const T* row, int vocab, int tid, int t
   for (int i = head + packs * kN + tid; i < vocab; i += threads) one(i);
 }
 
-// Largest logit and sum of exp(x - largest).
-struct Softmax {
+// Largest logit and sum of exp(x - largest). (8 bytes that one instruction copies or stores.)
+struct alignas(8) Softmax {
   float most, sum;
 };
 // (-inf where nothing has been seen: the difference of two such is not taken)
@@ -839,6 +839,7 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads)
   __shared__ Slope said;
   using Chunk = Share<T>;
   static_assert(offsetof(RowFacts, target) % 8 == 0 && offsetof(RowFacts, more) % 16 == 0, "places of cp.async");
+  static_assert(alignof(Softmax) == 8, "a store of both values");
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int ctas = 1 << a.shift, rank = a.shift ? static_cast<int>(cluster_ctarank()) : 0;
   const int cluster = blockIdx.x >> a.shift, clusters = gridDim.x >> a.shift, rows = static_cast<int>(r.rows);
