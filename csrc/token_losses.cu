@@ -21,6 +21,7 @@
 #include <atomic>
 #include <cmath>
 #include <cstddef>
+#include <initializer_list>
 #include <type_traits>
 
 #include "common.cuh"
@@ -1076,6 +1077,12 @@ __global__ void __launch_bounds__(256)
 // 231 for 65536 of 6 KB bf16, 541 and 532 for 131072 of 8 KB fp32; 604 and 1032 for 524288 of 2 KB.
 constexpr long long kLongPolicyRow = 6144, kLongRow = 4096;
 
+bool at_multiple(size_t of, std::initializer_list<const void*> pointers) {
+  for (const void* p : pointers)
+    if (reinterpret_cast<uintptr_t>(p) % of) return false;
+  return true;
+}
+
 int check_rows(const char* what, const void* logits, int fp32, const void* grad, long long batch, int length,
                int vocab, long long stride_b, long long stride_t, const void* targets) {
   if (batch < 0 || length < 0 || vocab < 1 || vocab > (1 << 30)) return set_error("%s: bad sizes", what);
@@ -1215,6 +1222,9 @@ T5X_API int t5x_policy_loss(const void* logits, int fp32, void* grad, long long 
   if (check_rows("policy_loss", logits, fp32, grad, batch, length, vocab, stride_b, stride_t, targets)) return -1;
   if (scratch == nullptr || out == nullptr || (batch * length > 0 && (!old_scores || !advantages)))
     return set_error("policy_loss: null pointer");
+  if (!at_multiple(16, {scratch}) || !at_multiple(8, {targets}) ||
+      !at_multiple(4, {weights, old_scores, ref_scores, advantages, normalizer, out}))
+    return set_error("policy_loss: misaligned pointer");
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   cudaError_t e = cudaMemsetAsync(scratch, 0, kHead, st);
   if (e != cudaSuccess) return set_error("policy_loss: memset: %s", cudaGetErrorString(e));
@@ -1255,6 +1265,9 @@ T5X_API int t5x_policy_loss_tokens(const void* logp, void* slope, long long batc
   if (batch < 0 || length < 0) return set_error("policy_loss_tokens: bad sizes");
   if (scratch == nullptr || out == nullptr || (batch * length > 0 && (!logp || !old_scores || !advantages)))
     return set_error("policy_loss_tokens: null pointer");
+  if (!at_multiple(16, {scratch}) ||
+      !at_multiple(4, {logp, slope, weights, old_scores, ref_scores, advantages, normalizer, out}))
+    return set_error("policy_loss_tokens: misaligned pointer");
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   cudaError_t e = cudaMemsetAsync(scratch, 0, kHead, st);
   if (e != cudaSuccess) return set_error("policy_loss_tokens: memset: %s", cudaGetErrorString(e));
@@ -1286,6 +1299,9 @@ T5X_API int t5x_preference_loss(const void* logits, int fp32, void* grad, long l
   if (batch < 2 || batch % 2) return set_error("preference_loss: the batch must hold pairs");
   if (length < 1 || length > (1 << 30)) return set_error("preference_loss: bad sizes");
   if (!scratch || !out || !reference || !scores || !margins) return set_error("preference_loss: null pointer");
+  if (!at_multiple(16, {scratch}) || !at_multiple(8, {targets}) ||
+      !at_multiple(4, {weights, reference, normalizer, scores, margins, out}))
+    return set_error("preference_loss: misaligned pointer");
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const long long pairs = batch / 2;
   char* at = static_cast<char*>(scratch);
@@ -1336,6 +1352,9 @@ T5X_API int t5x_preference_loss_tokens(const void* logp, void* slope, long long 
   if (length < 0 || length > (1 << 30)) return set_error("preference_loss_tokens: bad sizes");
   if (!scratch || !out || !reference || !scores || !margins || (length > 0 && !logp))
     return set_error("preference_loss_tokens: null pointer");
+  if (!at_multiple(16, {scratch}) ||
+      !at_multiple(4, {logp, slope, weights, reference, normalizer, scores, margins, out}))
+    return set_error("preference_loss_tokens: misaligned pointer");
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   cudaError_t e = cudaMemsetAsync(scratch, 0, kHead, st);
   if (e != cudaSuccess) return set_error("preference_loss_tokens: memset: %s", cudaGetErrorString(e));
@@ -1352,6 +1371,8 @@ T5X_API int t5x_preference_loss_tokens(const void* logp, void* slope, long long 
 T5X_API int t5x_scale_gradient(const void* src, void* dst, long long n, int fp32, const void* factor, void* stream) {
   if (n <= 0) return 0;
   if (!src || !dst || !factor) return set_error("scale_gradient: null pointer");
+  if (!at_multiple(fp32 ? 4 : 2, {src, dst}) || !at_multiple(4, {factor}))
+    return set_error("scale_gradient: misaligned pointer");
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const long long need = (n + 1023) / 1024, cap = static_cast<long long>(num_sms()) * 8;
   const unsigned grid = static_cast<unsigned>(need < cap ? need : cap);

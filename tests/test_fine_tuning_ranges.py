@@ -132,3 +132,32 @@ def test_overflowing_second_moment_shows():
   assert torch.isnan(opt.state.param_states["0"]["nu_absmax"]["w"]).tolist() == [False, True, False]
   opt = opt.apply_gradient({"w": torch.ones(600)})
   assert torch.isnan(opt.target["w"]).nonzero().flatten().tolist() == list(range(256, 512))
+
+
+# ---- refusals of the C entry points, with made-up addresses: nothing is launched ----
+A = 1 << 20
+
+
+@pytest.mark.parametrize("at,bytes_of", [(0, 16), (1, 8), (2, 4), (3, 4), (4, 4), (5, 4), (6, 4)])
+def test_misaligned_pointers_are_refused(at, bytes_of):
+  """Scratch, targets and values of 32 bits; with the middle of them an access would fault."""
+  from t5x_b200.ops import native
+  lib = native.lib()
+  p = [A] * 7
+  p[at] += bytes_of // 2
+  scratch, targets, weights, old, ref, adv, out = p
+  calls = [lambda: lib.t5x_policy_loss(A, 1, A, 4, 3, 8, 24, 8, targets, weights, old, ref, adv, 3, 1, 0.2, 0.2, 0.1, 1.0,
+                                       None, scratch, out, None),
+           lambda: lib.t5x_policy_loss_tokens(A, A, 4, 3, weights, old, ref, adv, 3, 1, 0.2, 0.2, 0.1, 1.0, None, scratch,
+                                              out, None),
+           lambda: lib.t5x_preference_loss(A, 1, A, 4, 3, 8, 24, 8, targets, weights, ref, 0.1, 0.0, 1.0, old, scratch, adv,
+                                           A, out, None),
+           lambda: lib.t5x_preference_loss_tokens(A, A, 4, 3, weights, ref, 0.1, 0.0, 1.0, old, scratch, A, adv, out,
+                                                  None)]
+  for i, call in enumerate(calls):
+    if at == 1 and i % 2:
+      continue  # (no targets)
+    assert call() != 0, i
+    assert "misaligned" in lib.t5x_last_error().decode()
+  assert lib.t5x_scale_gradient(A + 2, A, 4, 1, A, None) != 0 and lib.t5x_scale_gradient(A, A + 1, 4, 0, A, None) != 0
+  assert lib.t5x_scale_gradient(A, A, 4, 1, A + 2, None) != 0
