@@ -679,7 +679,7 @@ class OptaxWrapper(OptimizerDef):
     lr, count = self._step_lr(plan, hyper_params, lr_state), int(adam["count"])
     if not host.adamw_tree(params, grads, adam["mu"], adam["nu"], adam["mu_absmax"] if small else None,
                            adam["nu_absmax"] if small else None, lr, plan["b1"], plan["b2"], plan["eps"],
-                           plan["eps_root"], plan["weight_decay"], count + 1, plan["seed"],
+                           plan["eps_root"], plan["weight_decay"], count + 1, plan["seed"] & 0xFFFFFFFF,
                            -1.0 if plan["max_norm"] is None else float(plan["max_norm"])):
       return None
     adam["count"] = adam["count"] + 1

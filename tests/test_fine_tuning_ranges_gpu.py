@@ -325,3 +325,19 @@ def test_function_transforms(host, monkeypatch):
     along = torch.randn_like(d["x"])
     slope = torch.func.jvp(loss, (d["x"],), (along,))[1]
     assert float(slope) == pytest.approx(float((want * along).sum()), rel=1e-4, abs=1e-5)
+
+
+@pytest.mark.parametrize("host", ["1", "0"])
+@pytest.mark.parametrize("seed", [2 ** 64 - 3, 2 ** 63, -7, 2 ** 32 + 1])
+def test_seeds_of_any_size(seed, host, monkeypatch):
+  """The rounding depends on the seed modulo 2^32; seeds of 64 bits without a sign are common."""
+  from t5x_b200.ops import native
+  monkeypatch.setattr(native, "_host", None if host == "1" else False)
+  g = torch.randn(3000, device="cuda", generator=torch.Generator(device="cuda").manual_seed(0))
+  states = []
+  for s in (seed, seed % 2 ** 32, seed % 2 ** 32 + 1):
+    opt = optimizers.adamw8(1e-2, seed=s).create({"w": torch.ones(3000, device="cuda")})
+    states.append(adam_of(opt.apply_gradient({"w": g}))["mu"]["w"])
+  assert torch.equal(states[0], states[1]) and not torch.equal(states[0], states[2])
+  cpu = optimizers.adamw8(1e-2, seed=seed).create({"w": torch.ones(3000)}).apply_gradient({"w": g.cpu()})
+  assert int((adam_of(cpu)["mu"]["w"] != states[0].cpu()).sum()) <= 4
