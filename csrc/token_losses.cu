@@ -474,6 +474,8 @@ __device__ __forceinline__ float exp_from(float x, float most) {
   return exp2_approx(huge(most) ? (x - (most == -INFINITY ? 0.f : most)) * kLog2e
                                 : fmaf(x, kLog2e, -__fmul_rn(most, kLog2e)));
 }
+// of a single value: NaN of +inf and NaN, a sum of zero of -inf
+__device__ __forceinline__ Softmax row_of_one(float x) { return {x, exp_from(x, x)}; }
 __device__ __forceinline__ Softmax join_rows(Softmax a, Softmax b) {
   const float m = fmaxf(a.most, b.most);
   return {m, a.sum * exp2_approx(shift_of(a.most, m)) + b.sum * exp2_approx(shift_of(b.most, m))};
@@ -727,8 +729,7 @@ __global__ void __launch_bounds__(kPieceThreads, kPieceCtas)
       // the values in front of the first 16-byte boundary and behind the last
       const int outside = lane < head ? lane : all * kN + lane;
       if (outside < r.vocab) {
-        const float v = Pack<T>::one(x[outside]);
-        s = {v, v == -INFINITY ? 0.f : v * 0.f + 1.f};  // (NaN of +inf and NaN)
+        s = row_of_one(Pack<T>::one(x[outside]));
       }
       if (lane == 0) {
         const long long target = r.targets[row];
@@ -978,7 +979,7 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads)
         if (warp * kWarpPacks < left) mine.add_to(s);
       }
       if (outside >= 0) {
-        s = join_rows(s, {x_outside, x_outside == -INFINITY ? 0.f : x_outside * 0.f + 1.f});  // (NaN of +inf, NaN)
+        s = join_rows(s, row_of_one(x_outside));
         if (outside == target) tell_target(x_outside);
       }
       __syncwarp();

@@ -91,6 +91,31 @@ def test_targets_of_the_lowest_logit(vocab):
   assert torch.all(torch.autograd.grad(out[0], x)[0][..., 5] == -1.0)
 
 
+@pytest.mark.parametrize("kind", ["preference", "policy"])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("vocab", [101, 4001, 32131, 140005])
+def test_large_logits_at_the_ends_of_a_row(kind, dtype, vocab):
+  """The values in front of a row's first 16-byte boundary and behind its last, which are added one by one, are its
+  largest; the target is one of them, or another."""
+  d = data(6, 3, vocab, dtype, hidden=0.0)
+  big = torch.zeros(6, 3, vocab + 3, dtype=dtype, device="cuda")
+  x = big[..., 3:]
+  x.copy_(d["x"])
+  middles = torch.tensor([300.3, 1006.7, 30003.7, 60000.3, -30000.6, 65533.9], device="cuda").view(6, 1, 1)
+  x.copy_(x.float() + middles)
+  for t, at in ((0, 0), (1, vocab - 1), (2, 1)):
+    x[:, t, at] = (middles[:, 0, 0] + 9.3).to(dtype)
+  d["t"][:, 0], d["t"][:, 1] = 0, vocab - 1
+  d["t"][:, 2] = x[:, 2, 2:].argmax(-1) + 2
+  d["x"] = x.contiguous()
+  logp = oracle_logp(d["x"], d["t"])
+  assert float(logp.min()) > -40
+  d["old"], d["ref"], d["r"] = (logp - 0.1).float(), (logp + 0.1).float(), (logp * d["w"]).sum(1).float() - 1
+  leaf = x.detach().requires_grad_()
+  out = call(kind, leaf, d, None)
+  check(kind, out, torch.autograd.grad(out[0], leaf)[0], d, 1.0)
+
+
 @pytest.mark.parametrize("kl_weight", [0.0, 0.1])
 @pytest.mark.parametrize("vocab", [0, 2, 3000, 40000])
 @pytest.mark.parametrize("host", ["1", "0"])
