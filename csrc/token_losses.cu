@@ -443,9 +443,9 @@ __global__ void __launch_bounds__(kRowThreads)
 // next row is on its way into shared memory meanwhile. Larger rows than eight CTAs hold go by in chunks, which
 // are read a second time for the gradient.
 //
-// What bounds it: memory. Policy, 128 x 114 x 32128 bf16 of which 80% count: 310 us, 5.4 TB/s of what has to be read
-// and written; 7 x 189 x 250112 fp32: 416 us, 5.7 TB/s; the gradients of a preference loss, 64 x 114 x 32128 bf16: 137
-// us, 6.2 TB/s. Close behind come the instructions (60% of the issue slots, the exponentials' unit 54%), and a policy
+// What bounds it: memory. Policy, 128 x 114 x 32128 bf16 of which 80% count: 313 us, 5.4 TB/s of what has to be read
+// and written; 7 x 189 x 250112 fp32: 431 us, 5.5 TB/s; the gradients of a preference loss, 64 x 114 x 32128 bf16: 133
+// us, 6.3 TB/s. Close behind come the instructions (60% of the issue slots, the exponentials' unit 54%), and a policy
 // row has a chain from its last part to its slope that the SM's other CTA has to fill. So one thread finds out about
 // the rows, a few of them ahead, and leaves that for all in shared memory (488 us where all of them did), a warp's
 // share lies side by side, and what the loss itself needs is added behind the slope. Tried without effect: 256
@@ -669,8 +669,8 @@ struct Share {
 };
 
 // Long rows in pieces of a row, a warp each: their softmaxes and the target's logit. Warps at different places
-// of their pieces keep the reads going, and none waits for another: 82 us for 64 x 114 x 32128 bf16 logits of
-// which 80% count, 4.6 TB/s, and 135 us for 14 x 509 x 32101 fp32, 5.4 TB/s; a CTA a row, as for the gradient
+// of their pieces keep the reads going, and none waits for another: 80 us for 64 x 114 x 32128 bf16 logits of
+// which 80% count, 4.7 TB/s, and 133 us for 14 x 509 x 32101 fp32, 5.5 TB/s; a CTA a row, as for the gradient
 // below, took 109 and 184 us.
 struct Pieces {
   Softmax* of_piece;  // of row and piece

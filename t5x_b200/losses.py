@@ -214,7 +214,9 @@ def compute_preference_loss(logits: torch.Tensor, targets: torch.Tensor, weights
   answer with a target of logit -inf has a score of -inf: rejected, its pair's loss is 0 (without smoothing).
 
   On the GPU the gradient is computed along with the loss (memory of the logits' size, also where they are a view of
-  something larger) for logits in bf16 or fp32; see t5x_b200/ops/token_losses.py."""
+  something larger) for logits in bf16 or fp32, and rounded to their type. A loss that is scaled behind the call has
+  its bf16 gradient rounded once more, a `loss_normalizing_factor` comes before the rounding; see
+  t5x_b200/ops/token_losses.py."""
   from t5x_b200.ops import token_losses
   what = "compute_preference_loss"
   _check_tokens(what, logits, 3, targets=targets, weights=weights)
@@ -270,7 +272,9 @@ def compute_policy_loss(logits: torch.Tensor, targets: torch.Tensor, weights: Op
   loss alone is differentiable, and in the logits alone. Tokens of weight 0 do not count, whatever is in
   their places. A weighted target outside of the vocabulary gives a NaN loss on the GPU.
 
-  On the GPU loss and gradient take one pass over logits in bf16 or fp32; see t5x_b200/ops/token_losses.py."""
+  On the GPU loss and gradient take one pass over logits in bf16 or fp32. A loss that is scaled behind the call has its
+  bf16 gradient rounded once more, a `loss_normalizing_factor` comes before the rounding; see
+  t5x_b200/ops/token_losses.py."""
   from t5x_b200.ops import token_losses
   what = "compute_policy_loss"
   _check_tokens(what, logits, 3, targets=targets, weights=weights, old_token_scores=old_token_scores,
