@@ -121,6 +121,60 @@ int t5x_preference_loss_tokens(const void* logp, void* slope, long long batch, i
 /* dst = src * *factor (dst may be src; nothing is done where the factor is 1 then) */
 int t5x_scale_gradient(const void* src, void* dst, long long n, int fp32, const void* factor, void* stream);
 
+/* A key/value cache in 8 bits (cache8.cuh). codes: int8 [batch, heads, slots, dim] of keys and values; absmax: fp32
+ * [batch, heads, slots >> block_log2]; index: int32, tokens held (index_stride 1: by row; 0: one for all); weight: fp32
+ * [batch, heads, slots] or null; position: int32 [batch, heads, slots] or null (slots are positions then), with dropped:
+ * int32 [batch]. All contiguous. */
+typedef struct {
+  void* codes[2];
+  void* absmax[2];
+  const void* index;
+  void* weight;
+  void* position;
+  const void* dropped;
+  int index_stride, batch, heads, slots, dim, block_log2;
+} T5xCache8;
+/* Keys and values [batch, count, heads, dim], channels side by side, other strides in values; type 0 bf16, 1 fp16,
+ * 2 fp32; lengths: int32 [batch], or null where every row gets `count` tokens. */
+typedef struct {
+  const void* x[2];
+  const void* lengths;
+  long long stride_batch[2], stride_token[2], stride_head[2];
+  int count, type;
+} T5xNewTokens;
+/* One attention over the cache. query, out: [batch, count, heads * group, dim] of `type`, out contiguous. table: fp32
+ * [heads * group, table_stride] with `buckets`: bytes [distances] in the host's memory, the column of each distance (the
+ * last one's beyond; at most 1024), or null. key_mask: bytes [batch, mask_len] (slots behind are hidden) or null. causal: query i sees the slots up to
+ * that of the (count - i)-th token from the end. new_tokens: appended first, or null. */
+typedef struct {
+  const void* query;
+  void* out;
+  const void* table;
+  const unsigned char* buckets;
+  const void* key_mask;
+  long long stride_batch, stride_token, stride_head, table_stride, mask_stride;
+  int count, group, type, distances, mask_len, causal;
+  float scale;
+} T5xCache8Query;
+int t5x_cache8_append(const T5xCache8* cache, const T5xNewTokens* tokens, void* stream);
+/* workspace: that many bytes, 16-byte aligned; -1 for a call that is refused */
+long long t5x_cache8_attention_bytes(const T5xCache8* cache, const T5xCache8Query* query, const T5xNewTokens* new_tokens);
+int t5x_cache8_attention(const T5xCache8* cache, const T5xCache8Query* query, const T5xNewTokens* new_tokens,
+                         void* workspace, void* stream);
+/* kept: int32 [batch, heads, keep], slots that stay in order, -1 behind them; index_out, dropped_out: int32 [batch] */
+int t5x_cache8_evict(const T5xCache8* cache, const T5xCache8* into, int keep, int recent, void* kept, void* index_out,
+                     void* dropped_out, void* stream);
+
+/* Rows of `k` values (type 0 bf16, 1 fp16, 2 fp32; rows `stride` apart) as codes int8 [rows, ld] (zeros behind k) and
+ * their largest absolute values. */
+int t5x_quantize_rows(const void* x, int type, long long rows, int k, long long stride, void* codes, int ld, void* absmax,
+                      void* stream);
+/* y [rows, n] = x [rows, k] times weights in 8 bits (codes [n, k filled up to whole 16 with zeros], fp32 [n]), plus
+ * residual [rows, n] (rows ld_res apart) or null; x, residual and y of one type. workspace: 16-byte aligned. */
+long long t5x_linear8_workspace_bytes(int rows, int k);
+int t5x_linear8(const void* x, int type, int rows, int k, long long stride, const void* w, const void* w_absmax, int n,
+                const void* residual, long long ld_res, void* y, void* workspace, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

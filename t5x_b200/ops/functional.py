@@ -13,7 +13,7 @@ the train state:
 """
 from __future__ import annotations
 
-from typing import Optional, Sequence
+from typing import NamedTuple, Optional, Sequence
 
 import torch
 
@@ -248,6 +248,53 @@ def linear(x: torch.Tensor, weight: torch.Tensor, residual: Optional[torch.Tenso
   w = compute_weight(weight, dt).reshape(x.shape[-1], -1)
   y = x.to(dt) @ w
   return y if residual is None else y + residual
+
+
+class Weight8(NamedTuple):
+  """A kernel [in, out] in 8 bits: codes int8 [out, in filled up to whole 16 with zeros] and the largest |value| of each
+  output channel, fp32 [out]; a code c stands for c * absmax / 127."""
+  codes: torch.Tensor
+  absmax: torch.Tensor
+  in_features: int
+
+
+def quantize_weight(weight: torch.Tensor) -> Weight8:
+  """W [in, out...] (T5X kernel layout; bf16, fp16 or fp32) for `linear8`. A channel with a value that is not finite is NaN."""
+  w = weight.detach().reshape(weight.shape[0], -1).t()
+  k = w.shape[1]
+  if not w.dtype.is_floating_point or k < 1 or w.shape[0] < 1 or k > 131072:
+    raise ValueError(f"quantize_weight: a kernel of 1 to 131072 rows; got {tuple(weight.shape)} {weight.dtype}")
+  ld = -(-k // 16) * 16
+  if w.is_cuda and w.dtype in native.CACHE8_TYPES:
+    return Weight8(*native.quantize_rows(w.contiguous(), ld), k)
+  codes, absmax = ref.quantize_rows(w.contiguous())
+  return Weight8(torch.nn.functional.pad(codes, (0, ld - k)).contiguous(), absmax, k)
+
+
+def linear8(x: torch.Tensor, weight: Weight8, residual: Optional[torch.Tensor] = None) -> torch.Tensor:
+  """y = x @ W (+ residual) in 8-bit integers: x [..., in] is scaled by its rows' largest values, W by its channels', the
+  products are added exactly and the sum is rounded once, to x's type. A row with a value that is not finite is NaN. For
+  serving: there is no backward pass."""
+  codes, absmax, k = weight
+  n = codes.shape[0]
+  if torch.is_grad_enabled() and (x.requires_grad or (residual is not None and residual.requires_grad)):
+    raise ValueError("linear8 has no backward pass: detach its inputs or call it under torch.no_grad()")
+  if x.dim() < 1 or x.shape[-1] != k or not x.dtype.is_floating_point:
+    raise ValueError(f"linear8: x [..., {k}]; got {tuple(x.shape)} {x.dtype}")
+  if codes.dtype != torch.int8 or codes.shape != (n, -(-k // 16) * 16) or absmax.dtype != torch.float32 or \
+      absmax.shape != (n,) or not codes.is_contiguous() or not absmax.is_contiguous() or codes.device != x.device or \
+      absmax.device != x.device or not 1 <= k <= 131072:
+    raise ValueError("linear8: the weight is one of quantize_weight on the device of x")
+  if residual is not None and (residual.shape != (*x.shape[:-1], n) or residual.dtype != x.dtype or
+                               residual.device != x.device):
+    raise ValueError(f"linear8: a residual {(*x.shape[:-1], n)} of x's type; got {tuple(residual.shape)} {residual.dtype}")
+  flat = x.reshape(-1, k)
+  res = None if residual is None else residual.reshape(-1, n)
+  if x.is_cuda and x.dtype in native.CACHE8_TYPES and x.numel() > 0 and not _transformed():
+    y = native.linear8(flat, codes, absmax, res)
+  else:
+    y = ref.linear8(flat, codes[:, :k], absmax, res)
+  return y.view(*x.shape[:-1], n)
 
 
 class _BatchedLinearFn(torch.autograd.Function):

@@ -1314,3 +1314,156 @@ def scale_gradient(grad: torch.Tensor, factor: torch.Tensor, keep: bool) -> torc
     _check(lib().t5x_scale_gradient(grad.data_ptr(), out.data_ptr(), span, int(grad.dtype == torch.float32),
                                     factor.data_ptr(), stream_ptr()), "scale_gradient")
   return out
+
+
+# ----------------------------------------------------------------------------
+# Decoding in 8 bits
+# ----------------------------------------------------------------------------
+class _Cache8(ctypes.Structure):
+  _fields_ = [("codes", c_void_p * 2), ("absmax", c_void_p * 2), ("index", c_void_p), ("weight", c_void_p),
+              ("position", c_void_p), ("dropped", c_void_p)] + \
+      [(n, c_int) for n in ("index_stride", "batch", "heads", "slots", "dim", "block_log2")]
+
+
+class _NewTokens(ctypes.Structure):
+  _fields_ = [("x", c_void_p * 2), ("lengths", c_void_p), ("stride_batch", c_ll * 2), ("stride_token", c_ll * 2),
+              ("stride_head", c_ll * 2), ("count", c_int), ("type", c_int)]
+
+
+class _Cache8Query(ctypes.Structure):
+  _fields_ = [(n, c_void_p) for n in ("query", "out", "table", "buckets", "key_mask")] + \
+      [(n, c_ll) for n in ("stride_batch", "stride_token", "stride_head", "table_stride", "mask_stride")] + \
+      [(n, c_int) for n in ("count", "group", "type", "distances", "mask_len", "causal")] + [("scale", c_float)]
+
+
+register_signature("t5x_cache8_append", [c_void_p] * 3)
+register_signature("t5x_cache8_attention_bytes", [c_void_p] * 3)
+register_signature("t5x_cache8_attention", [c_void_p] * 5)
+register_signature("t5x_cache8_evict", [c_void_p] * 2 + [c_int] * 2 + [c_void_p] * 4)
+register_signature("t5x_quantize_rows", [c_void_p, c_int, c_ll, c_int, c_ll, c_void_p, c_int, c_void_p, c_void_p])
+register_signature("t5x_linear8_workspace_bytes", [c_int, c_int])
+register_signature("t5x_linear8", [c_void_p, c_int, c_int, c_int, c_ll, c_void_p, c_void_p, c_int, c_void_p, c_ll] +
+                   [c_void_p] * 3)
+
+CACHE8_TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+CACHE8_DISTANCES, CACHE8_BIASES = 1024, 40000  # distances of a bias table; distances times heads that share keys
+_cache8_buckets: dict = {}
+
+
+def _cache8(cache) -> _Cache8:
+  codes = cache["cached_key"]
+  b, h, slots, dim = codes.shape
+  index = cache["cache_index"]
+  c = _Cache8(index=index.data_ptr(), weight=ptr(cache.get("token_weight")), position=ptr(cache.get("token_position")),
+              dropped=ptr(cache.get("dropped")), index_stride=int(index.numel() == b and b > 1), batch=b, heads=h,
+              slots=slots, dim=dim, block_log2=(slots // cache["key_absmax"].shape[2]).bit_length() - 1)
+  c.codes[0], c.codes[1] = codes.data_ptr(), cache["cached_value"].data_ptr()
+  c.absmax[0], c.absmax[1] = cache["key_absmax"].data_ptr(), cache["value_absmax"].data_ptr()
+  return c
+
+
+def _channels_last(t: torch.Tensor) -> torch.Tensor:
+  return t if t.stride(-1) == 1 else t.contiguous()
+
+
+def _new_tokens(key, value, lengths=None) -> _NewTokens:
+  n = _NewTokens(lengths=ptr(lengths), count=key.shape[1], type=CACHE8_TYPES[key.dtype])
+  for i, t in enumerate((key, value)):
+    n.x[i] = t.data_ptr()
+    n.stride_batch[i], n.stride_token[i], n.stride_head[i] = t.stride()[:3]
+  return n
+
+
+def cache8_append(cache, key, value, lengths=None) -> None:
+  """Tokens [B, L, H, D] into a cache in 8 bits (csrc/cache8.cu)."""
+  key, value = _channels_last(key), _channels_last(value)
+  lengths = None if lengths is None else lengths.to(torch.int32).contiguous()
+  with _on_device_of(key):
+    c, n = _cache8(cache), _new_tokens(key, value, lengths)
+    _check(lib().t5x_cache8_append(ctypes.byref(c), ctypes.byref(n), stream_ptr()), "cache8_append")
+
+
+def _buckets_of(num_buckets: int, max_distance: int):
+  """The bucket of each distance up to `max_distance`, from where on all share the last: bytes on the host."""
+  table = _cache8_buckets.get((num_buckets, max_distance))
+  if table is None:
+    from t5x_b200.ops import reference
+    back = -torch.arange(max_distance + 1, device="cpu")
+    table = bytes(reference.relative_position_bucket(back, False, num_buckets, max_distance).tolist())
+    _cache8_buckets[num_buckets, max_distance] = table
+  return table
+
+
+def cache8_attention(query, cache, key, value, bias_table, num_buckets, max_distance, key_mask, causal, scale):
+  """Attention of a few queries over a cache in 8 bits (csrc/cache8_attention.cu), the new tokens appended first."""
+  query = _channels_last(query)
+  b, count, heads, dim = query.shape
+  h = cache["cached_key"].shape[1]
+  out = torch.empty(query.shape, dtype=query.dtype, device=query.device)
+  q = _Cache8Query(query=query.data_ptr(), out=out.data_ptr(), count=count, group=heads // h, type=CACHE8_TYPES[query.dtype],
+                   causal=int(causal), scale=scale)
+  q.stride_batch, q.stride_token, q.stride_head = query.stride()[:3]
+  if bias_table is not None:
+    bias_table = bias_table.detach().float().contiguous()
+    buckets = _buckets_of(num_buckets, max_distance)
+    q.table, q.table_stride, q.distances = bias_table.data_ptr(), bias_table.shape[1], len(buckets)
+    q.buckets = ctypes.cast(ctypes.c_char_p(buckets), c_void_p)
+  if key_mask is not None:
+    key_mask = (key_mask.contiguous().view(torch.uint8) if key_mask.dtype == torch.bool else
+                (key_mask != 0).to(torch.uint8).contiguous())
+    # (a mask of no slots has no memory; none of it is read)
+    q.key_mask = key_mask.data_ptr() or query.data_ptr()
+    q.mask_stride = q.mask_len = key_mask.shape[1]
+  if key is not None:
+    key, value = _channels_last(key), _channels_last(value)
+  with _on_device_of(query):
+    c, l = _cache8(cache), lib()
+    n = None if key is None else ctypes.byref(_new_tokens(key, value))
+    l.t5x_cache8_attention_bytes.restype = c_ll
+    nbytes = l.t5x_cache8_attention_bytes(ctypes.byref(c), ctypes.byref(q), n)
+    if nbytes < 0:
+      _check(-1, "cache8_attention")
+    workspace = torch.empty(nbytes, dtype=torch.uint8, device=query.device) if nbytes else None
+    _check(l.t5x_cache8_attention(ctypes.byref(c), ctypes.byref(q), n, ptr(workspace), stream_ptr()), "cache8_attention")
+  return out
+
+
+def cache8_evict(cache, into, keep: int, recent: int) -> torch.Tensor:
+  """Kept slots [B, H, keep]; the tokens go into `into` (csrc/cache8.cu)."""
+  b, h = cache["cached_key"].shape[:2]
+  with _on_device_of(cache["cached_key"]):
+    kept = torch.empty(b, h, keep, dtype=torch.int32, device=cache["cached_key"].device)
+    c, to = _cache8(cache), _cache8(into)
+    _check(lib().t5x_cache8_evict(ctypes.byref(c), ctypes.byref(to), keep, recent, kept.data_ptr(),
+                                  into["cache_index"].data_ptr(), into["dropped"].data_ptr(), stream_ptr()), "cache8_evict")
+  return kept
+
+
+def quantize_rows(x: torch.Tensor, ld: int):
+  """(codes int8 [rows, ld], zeros behind the values; fp32 largest |x| by row) of x [rows, k] (csrc/linear8.cu)."""
+  x = _channels_last(x)
+  codes = torch.empty(x.shape[0], ld, dtype=torch.int8, device=x.device)
+  most = torch.empty(x.shape[0], dtype=torch.float32, device=x.device)
+  with _on_device_of(x):
+    _check(lib().t5x_quantize_rows(x.data_ptr(), CACHE8_TYPES[x.dtype], x.shape[0], x.shape[1], x.stride(0),
+                                   codes.data_ptr(), ld, most.data_ptr(), stream_ptr()), "quantize_rows")
+  return codes, most
+
+
+def linear8(x: torch.Tensor, codes: torch.Tensor, absmax: torch.Tensor, residual: Optional[torch.Tensor]) -> torch.Tensor:
+  """x [rows, k] times weights in 8 bits (codes [n, k filled up to whole 16], absmax [n]) plus residual [rows, n]
+  (csrc/linear8.cu)."""
+  x = _channels_last(x)
+  rows, k = x.shape
+  n = codes.shape[0]
+  y = torch.empty(rows, n, dtype=x.dtype, device=x.device)
+  if residual is not None:
+    residual = _channels_last(residual)
+  with _on_device_of(x):
+    l = lib()
+    l.t5x_linear8_workspace_bytes.restype = c_ll
+    workspace = torch.empty(l.t5x_linear8_workspace_bytes(rows, k), dtype=torch.uint8, device=x.device)
+    _check(l.t5x_linear8(x.data_ptr(), CACHE8_TYPES[x.dtype], rows, k, x.stride(0), codes.data_ptr(), absmax.data_ptr(), n,
+                         ptr(residual), 0 if residual is None else residual.stride(0), y.data_ptr(), workspace.data_ptr(),
+                         stream_ptr()), "linear8")
+  return y

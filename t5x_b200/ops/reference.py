@@ -316,3 +316,157 @@ def preference_loss(logp, weights, reference, beta, label_smoothing, normalizer)
   back = logp.dtype
   return (_over_normalizer(torch.where(real, loss, zero).sum(), normalizer).to(back), scores.detach().to(back),
           margins.detach().to(back), real.sum().to(back))
+
+
+# ----------------------------------------------------------------------------
+# Numbers in 8 bits
+# ----------------------------------------------------------------------------
+def codes_of(real: torch.Tensor, whole, most: torch.Tensor) -> torch.Tensor:
+  """The code of real * whole / most: the exact quotient rounded to the nearest whole number (ties to even; in 64 bits it
+  cannot round to the other side of a border), 0 where it is none."""
+  q = torch.round(real.double() * whole / most.double())
+  return torch.nan_to_num(q, nan=0.0, posinf=127.0, neginf=-127.0).clamp(-127, 127).to(torch.int8)
+
+
+def quantize_rows(x: torch.Tensor):
+  """(codes int8, fp32 largest |x|) of each row of x [rows, k]; a code c stands for c * largest / 127."""
+  x = x.float()
+  most = x.abs().amax(1) if x.shape[0] else x.new_zeros(0)
+  return codes_of(x, 127, most[:, None]), most
+
+
+def linear8(x, codes, absmax, residual=None):
+  """x [rows, k] times weights in 8 bits [n, k]: x in 8 bits too, scaled by row; sums of whole numbers, rounded once."""
+  cx, most = quantize_rows(x)
+  y = cx.double() @ codes.double().t()  # (exact)
+  y = y * (most.double() / 127)[:, None] * (absmax.double() / 127)
+  return (y if residual is None else y + residual.double()).to(x.dtype)
+
+
+def _cache8_block(cache) -> int:
+  return cache["cached_key"].shape[2] // cache["key_absmax"].shape[2]
+
+
+def _cache8_index(cache) -> torch.Tensor:
+  """Tokens held, by row."""
+  b, _, slots, _ = cache["cached_key"].shape
+  return cache["cache_index"].long().clamp(0, slots).expand(b)
+
+
+def cache8_append(cache, key, value, lengths=None) -> None:
+  """Tokens key, value [B, L, H, D] behind those that the rows hold (lengths [B]: so many of the L). A block of tokens
+  that gets some has the largest absolute value of what it holds and gets, and its codes are rounded again."""
+  b, h, slots, dim = cache["cached_key"].shape
+  block, count, at = _cache8_block(cache), key.shape[1], _cache8_index(cache)
+  slot = torch.arange(slots, device=at.device)
+  place = slot - at[:, None]  # of the new token, for each slot [B, slots]
+  fresh = count if lengths is None else lengths.long().clamp(0, count)[:, None]
+  new, old = (place >= 0) & (place < fresh), place < 0
+  by_block = lambda t: t.view(b, -1, block).any(2)[:, None]  # noqa: E731
+  spread = lambda t: t.repeat_interleave(block, 2)[..., None]  # noqa: E731
+  touched, keeps = by_block(new), by_block(old)
+  for name, x in (("key", key), ("value", value)):
+    codes, most = cache["cached_" + name], cache[name + "_absmax"]
+    x = x.float().transpose(1, 2).gather(2, place.clamp(0, count - 1)[:, None, :, None].expand(b, h, slots, dim))
+    x = torch.where(new[:, None, :, None], x, torch.zeros_like(x))
+    before = torch.where(keeps, most, torch.zeros_like(most))
+    after = torch.maximum(before, x.abs().reshape(b, h, -1, block * dim).amax(3))
+    again = torch.where(spread(before == after), codes, codes_of(spread(before), codes, spread(after)))
+    again = torch.where((old[:, None] & touched.repeat_interleave(block, 2))[..., None], again, codes)
+    codes.copy_(torch.where(new[:, None, :, None], codes_of(x, 127, spread(after)), again))
+    most.copy_(torch.where(touched, after, most))
+  if "token_weight" in cache:
+    cache["token_weight"].masked_fill_(new[:, None], 0.0)
+  if "token_position" in cache:
+    where = (slot + cache["dropped"].long()[:, None]).to(torch.int32)
+    cache["token_position"].copy_(torch.where(new[:, None], where[:, None], cache["token_position"]))
+
+
+def cache8_values(cache, name: str, dtype=torch.float32) -> torch.Tensor:
+  """What the codes of "key" or "value" stand for, [B, H, slots, D]."""
+  scale = (cache[name + "_absmax"].to(dtype) / 127).repeat_interleave(_cache8_block(cache), 2)
+  return cache["cached_" + name].to(dtype) * scale[..., None]
+
+
+def cache8_attention(query, cache, appended=0, bias_table=None, num_buckets=32, max_distance=128, key_mask=None,
+                     causal=True, scale=1.0):
+  """softmax(scale q k + bias) v over a cache in 8 bits; query [B, L, heads * group, D]. Of the tokens that a row holds the
+  last `appended` are this call's; with `causal` the queries are the last L of all. A query that sees nothing has zeros."""
+  wide = torch.promote_types(query.dtype, torch.float32)
+  b, h, slots, dim = cache["cached_key"].shape
+  count, group = query.shape[1], query.shape[2] // h
+  index = _cache8_index(cache)
+  end = (index + appended).clamp(max=slots)[:, None, None]
+  slot = torch.arange(slots, device=query.device)
+  own = (index + appended - count)[:, None] + torch.arange(count, device=query.device)  # slots of the queries [B, L]
+  seen = (slot < end).expand(b, count, slots)
+  if causal:
+    seen = seen & (slot <= own[..., None])
+  if key_mask is not None:
+    shown = F.pad(key_mask.bool(), (0, slots - key_mask.shape[1]))
+    seen = seen & shown[:, None]
+  seen = seen[:, None, None]  # [B, 1, 1, L, slots]
+  q = query.to(wide).view(b, count, h, group, dim)
+  s = torch.einsum("blhgd,bhsd->bhgls", q, cache8_values(cache, "key", wide)) * scale
+  if bias_table is not None:
+    place, at = slot.expand(b, h, slots), own
+    if "token_position" in cache:
+      place, at = cache["token_position"].long(), own + cache["dropped"].long()[:, None]
+    buckets = relative_position_bucket(place[:, :, None] - at[:, None, :, None], False, num_buckets, max_distance)
+    table = bias_table.to(wide)[:h * group].view(h, 1, group, -1)
+    s = s + table.expand(h, count, group, -1)[None].expand(b, -1, -1, -1, -1).transpose(2, 3).gather(
+        4, buckets[:, :, None].expand(b, h, group, count, slots))
+  s = s.masked_fill(~seen, -math.inf)
+  top = s.amax(4, keepdim=True)
+  p = torch.exp(s - torch.where(torch.isneginf(top), torch.zeros_like(top), top))
+  p = torch.where(seen, p, torch.zeros_like(p))
+  total = p.sum(4, keepdim=True)
+  p = torch.where(total == 0, torch.zeros_like(p), p / total)
+  if "token_weight" in cache:
+    cache["token_weight"] += p.sum((2, 3)).to(torch.float32)
+  v = cache8_values(cache, "value", wide)[:, :, None, None]
+  # (what is hidden counts for nothing, whatever its block holds)
+  visible = seen.expand_as(p)
+  out = torch.einsum("bhgls,bhsd->blhgd", p, torch.nan_to_num(v[:, :, 0, 0], nan=0.0, posinf=0.0, neginf=0.0))
+  broken = ~torch.isfinite(v[:, :, 0, 0, :, :1])  # whole blocks
+  poisoned = (visible & broken[:, :, None, None, :, 0]).any(4)  # [B, H, group, L]
+  out = torch.where(poisoned.permute(0, 3, 1, 2)[..., None], torch.full_like(out, math.nan), out)
+  return out.reshape(query.shape).to(query.dtype)
+
+
+def cache8_evict(cache, into, keep: int, recent: int):
+  """Kept slots [B, H, keep] (-1 behind them): the last `recent` tokens and those of the largest weight (NaN above all, ties
+  to the lowest slot), in order; `into` gets them, its tokens behind them stay as they were."""
+  b, h, slots, dim = cache["cached_key"].shape
+  held = _cache8_index(cache)[:, None, None]
+  slot = torch.arange(slots, device=held.device)
+  rank = torch.argsort(torch.argsort(torch.where(slot < held - recent, cache["token_weight"].double(), -math.inf), dim=2,
+                                     descending=True, stable=True), dim=2)
+  # where a weight is -inf itself, places before the last ones still come first by the stable order
+  stays = (slot < held) & ((held <= keep) | (slot >= held - recent) | (rank < keep - recent))
+  kept = torch.where(stays, slot, slots).sort(2).values
+  kept = F.pad(kept, (0, max(0, keep - slots)), value=slots)[..., :keep]
+  there, source = kept < slots, kept.clamp(max=slots - 1)
+  block, old_block = _cache8_block(into), _cache8_block(cache)
+  blocks = -(-keep // block)
+  grown = lambda t, v: F.pad(t, (0, blocks * block - keep), value=v).view(b, h, blocks, block)  # noqa: E731
+  for name in ("key", "value"):
+    most = cache[name + "_absmax"].gather(2, source // old_block)
+    after = grown(torch.where(there, most, torch.zeros_like(most)), 0.0).amax(3)
+    each = after.repeat_interleave(block, 2)[..., :keep, None]
+    codes = cache["cached_" + name].gather(2, source[..., None].expand(-1, -1, -1, dim))
+    codes = torch.where(most[..., None] == each, codes, codes_of(most[..., None], codes, each))
+    to = into["cached_" + name][:, :, :keep]
+    to.copy_(torch.where(there[..., None], codes, to))
+    to = into[name + "_absmax"][:, :, :blocks]
+    to.copy_(torch.where(grown(there, False).any(3), after, to))
+  positions = cache.get("token_position", slot.to(torch.int32).expand(b, h, slots))
+  for name, t in (("token_weight", cache["token_weight"]), ("token_position", positions)):
+    to = into[name][:, :, :keep]
+    to.copy_(torch.where(there, t.gather(2, source), to))
+  index = cache["cache_index"].clamp(min=0).expand(b)
+  left = index.clamp(max=min(keep, slots))
+  before = cache["dropped"] if "token_position" in cache else torch.zeros_like(index)
+  into["cache_index"].copy_(left)
+  into["dropped"].copy_(before + index - left)
+  return torch.where(there, kept, -1).to(torch.int32)

@@ -1,0 +1,259 @@
+"""Kernels of decoding in 8 bits: against loops in 64 bits (test_cache8.py) at the borders of blocks, tiles, rows and masks;
+strides, streams, captures; long caches against the statements in tensor operations."""
+import math
+
+import pytest
+import torch
+
+import test_cache8 as plain
+from t5x_b200.ops import cache8
+from t5x_b200.ops import functional as F
+from t5x_b200.ops import native
+from t5x_b200.ops import reference as ref
+
+pytestmark = pytest.mark.gpu
+TYPES = [torch.bfloat16, torch.float16, torch.float32]
+
+MORE = [
+    dict(b=2, h=2, group=5, dim=128, slots=128, block=16, starts=[0, 99], count=7, bias=True, weights=True, positions=True),
+    dict(b=2, h=1, group=1, dim=64, slots=608, block=32, starts=[560, 13], count=40, bias=True, weights=True),
+    dict(b=1, h=3, group=1, dim=128, slots=640, block=128, starts=[517], count=1, weights=True, mask=True),
+    dict(b=1, h=1, group=40, dim=64, slots=528, block=16, starts=[511], count=1, bias=True),
+    dict(b=2, h=1, group=1, dim=128, slots=64, block=64, starts=[63, 64], count=33, cross=True, weights=True),
+    dict(b=2, h=2, group=2, dim=64, slots=1040, block=16, starts=[1000, 257], count=1, weights=True, positions=True, bias=True),
+    dict(b=2, h=1, group=3, dim=128, slots=32, block=32, starts=[2, 30], count=5, own=True, weights=True),
+]
+
+
+def launches(call):
+  before = native.launch_count()
+  out = call()
+  assert native.launch_count() > before
+  return out
+
+
+@pytest.mark.parametrize("c", plain.CASES + MORE, ids=range(len(plain.CASES + MORE)))
+@pytest.mark.parametrize("dtype", TYPES)
+def test_attention(c, dtype):
+  launches(lambda: plain.check_attention(c, "cuda", dtype))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("dim,block", [(64, 16), (128, 128)])
+@pytest.mark.parametrize("lengths", [None, [0, 1, 33], [-4, 90, 2]])
+def test_append(dtype, dim, block, lengths):
+  cache = plain.make(3, 2, 128, dim, block, [0, 17, 120], device="cuda")
+  before = {k: v.clone() for k, v in cache.items()}
+  key, value = [t.cuda() for t in plain.tokens(3, 33, 2, dim, dtype=dtype)]
+  given = None if lengths is None else torch.tensor(lengths).cuda()
+  launches(lambda: cache8.append_(cache, key, value, given))
+  for n, x in (("key", key), ("value", value)):
+    codes, most = plain.append_oracle(before, n, x, [0, 17, 120], [min(max(v, 0), 33) for v in lengths or [33] * 3])
+    assert torch.equal(cache["cached_" + n].cpu(), codes) and torch.equal(cache[n + "_absmax"].cpu(), most)
+
+
+def test_codes_at_every_border():
+  """Values whose quotient lies on a border between two codes, or next to it, in 32 bits."""
+  most = torch.tensor([1.0, 127.0, 2.5390625, 0.7071068286895752, 3.0e-39, 2.0e38])
+  x = torch.zeros(6, 4096)
+  for i, m in enumerate(most.tolist()):
+    at = (torch.arange(-127, 127) + 0.5).double() * m / 127
+    near = torch.stack([at.float(), torch.nextafter(at.float(), torch.tensor(math.inf)),
+                        torch.nextafter(at.float(), torch.tensor(-math.inf))]).flatten()
+    x[i, :near.numel()] = near.clamp(-m, m)
+    x[i, -1] = m
+  codes, absmax = native.quantize_rows(x.cuda(), 4096)
+  want, size = ref.quantize_rows(x)
+  assert torch.equal(codes.cpu(), want) and torch.equal(absmax.cpu(), size)
+
+
+@pytest.mark.parametrize("bad", [math.inf, -math.inf, math.nan])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_values_that_are_not_finite(bad, dtype):
+  c = dict(b=1, h=1, group=1, dim=64, slots=64, block=16, starts=[20], count=1)
+  cache, query, key, value, _ = plain.inputs(c, "cuda", dtype)
+  hide = torch.ones(1, 64, dtype=torch.bool, device="cuda")
+  hide[0, 16:32] = False  # the block that gets it
+  new = [t.cuda().to(dtype) for t in plain.tokens(1, 1, 1, 64)]
+  want = cache8.attention(query, {k: v.clone() for k, v in cache.items()}, *new, key_mask=hide)
+  for which in (key, value):
+    worse = {k: v.clone() for k, v in cache.items()}
+    which[0, 0, 0, 3] = bad
+    assert torch.equal(cache8.attention(query, worse, key, value, key_mask=hide), want)
+    assert cache8.attention(query, worse, key, value).isnan().all()
+    which[0, 0, 0, 3] = 1
+
+
+def test_biases_of_the_lowest_value_and_of_minus_infinity():
+  c = dict(b=1, h=2, group=1, dim=64, slots=64, block=16, starts=[12], count=1)
+  cache, query, key, value, _ = plain.inputs(c, "cuda", torch.float32)
+  low = torch.full((2, 32), torch.finfo(torch.float32).min, device="cuda")
+  out = cache8.attention(query * 0, cache, key, value, bias_table=low)
+  v = ref.cache8_values(cache, "value", torch.float64)[0, :, :13].mean(1)
+  assert torch.allclose(out[0, 0].double(), v, rtol=0, atol=2.0 ** -20 * v.abs().max().item() * 16)
+  assert (cache8.attention(query, cache, key, value, bias_table=torch.full_like(low, -math.inf)) == 0).all()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_strides_and_pieces_of_wider_tensors(dtype):
+  c = dict(b=2, h=2, group=1, dim=64, slots=64, block=16, starts=[9, 30], count=3)
+  cache, query, key, value, _ = plain.inputs(c, "cuda", dtype)
+  want = cache8.attention(query, {k: v.clone() for k, v in cache.items()}, key, value)
+  qkv = torch.cat([t.reshape(2, 3, 128) for t in (query, key, value)] + [torch.zeros(2, 3, 1, device="cuda", dtype=dtype)], 2)
+  for parts in (
+      [p.unflatten(2, (2, 64)) for p in qkv[..., :384].split(128, 2)],  # rows of an odd length
+      [t.permute(0, 2, 1, 3).contiguous().permute(0, 2, 1, 3) for t in (query, key, value)],
+      [t.permute(3, 0, 1, 2).contiguous().permute(1, 2, 3, 0) for t in (query, key, value)],  # channels far apart
+      [torch.cat([t.flatten(), t.flatten()[:1]])[1:].roll(1).view_as(t) for t in (query, key, value)]):
+    again = {k: v.clone() for k, v in cache.items()}
+    assert torch.equal(cache8.attention(*[parts[0], again, *parts[1:]]), want)
+
+
+def test_mask_types_and_widths():
+  c = dict(b=2, h=1, group=1, dim=64, slots=64, block=16, starts=[40, 30], count=2, cross=True)
+  cache, query, _, _, _ = plain.inputs(c, "cuda", torch.float32)
+  mask = torch.rand(2, 33, device="cuda") > 0.5
+  want = cache8.attention(query, cache, key_mask=mask, causal=False)
+  wide = torch.zeros(2, 64, device="cuda", dtype=torch.bool)
+  wide[:, :33] = mask
+  for m in (mask.int() * 256, mask.float(), wide, wide.t().contiguous().t()):
+    assert torch.equal(cache8.attention(query, cache, key_mask=m, causal=False), want)
+  assert (cache8.attention(query, cache, key_mask=mask[:, :0], causal=False) == 0).all()
+
+
+@pytest.mark.parametrize("c", plain.EVICT, ids=range(len(plain.EVICT)))
+@pytest.mark.parametrize("special", [False, True])
+def test_evict(c, special):
+  launches(lambda: plain.check_evict(c, "cuda", special))
+
+
+@pytest.mark.parametrize("rows,k,n", [(1, 16, 8), (3, 17, 5), (5, 1, 3), (2, 300, 130), (33, 129, 257), (257, 64, 40),
+                                      (130, 513, 300)])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_linear8(rows, k, n, dtype):
+  launches(lambda: plain.check_linear(rows, k, n, dtype, rows % 2 == 1, "cuda"))
+
+
+def test_linear8_strides():
+  weight = F.quantize_weight(torch.randn(48, 40).cuda())
+  x, r = torch.randn(9, 7, 48).cuda().bfloat16(), torch.randn(9, 7, 40).cuda().bfloat16()
+  want = F.linear8(x, weight, r)
+  wide = torch.zeros(9, 7, 99, device="cuda", dtype=torch.bfloat16)
+  wide[..., 1:49], wide[..., 50:90] = x, r
+  assert torch.equal(F.linear8(wide[..., 1:49], weight, wide[..., 50:90]), want)
+  assert torch.equal(F.linear8(x.transpose(0, 1).contiguous().transpose(0, 1), weight, r), want)
+  assert torch.equal(F.linear8(x[0, 0], weight, r[0, 0]), want[0, 0])
+
+
+def test_linear8_rows_that_are_not_finite():
+  weight = F.quantize_weight(torch.randn(64, 40).cuda())
+  x = torch.randn(5, 64).cuda()
+  want = F.linear8(x, weight)
+  x[1, 3], x[3, 0] = math.nan, -math.inf
+  y = F.linear8(x, weight)
+  assert y[1].isnan().all() and y[3].isnan().all() and torch.equal(y[::2], want[::2])
+
+
+def test_another_stream_and_two_captures():
+  """Two graphs of the same cache's steps, replayed in turn, and a call on another stream."""
+  c = dict(b=2, h=2, group=1, dim=64, slots=640, block=32, starts=[300, 500], count=1, weights=True, bias=True)
+  cache, query, key, value, kw = plain.inputs(c, "cuda", torch.bfloat16)
+  want = cache8.attention(query, {k: v.clone() for k, v in cache.items()}, key, value, **kw)
+  torch.cuda.synchronize()
+  graphs, outs, caches = [], [], []
+  for _ in range(2):
+    mine = {k: v.clone() for k, v in cache.items()}
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+      outs.append(cache8.attention(query, mine, key, value, **kw))
+    graphs.append(g)
+    caches.append(mine)
+  side = torch.cuda.Stream()
+  side.wait_stream(torch.cuda.current_stream())
+  with torch.cuda.stream(side):
+    beside = cache8.attention(query, {k: v.clone() for k, v in cache.items()}, key, value, **kw)
+  for _ in range(3):
+    for g in graphs:
+      g.replay()
+  torch.cuda.synchronize()
+  assert torch.equal(beside, want) and all(torch.equal(o, want) for o in outs)
+  assert torch.equal(caches[0]["token_weight"], caches[1]["token_weight"])
+
+
+def test_decode_evict_decode():
+  """A run as a server makes it: prompts, tokens one at a time, an eviction, more tokens; beside the statements."""
+  b, heads, kv, dim, slots = 3, 6, 2, 64, 160
+  table = torch.randn(heads, 32)
+  gen = torch.Generator().manual_seed(0)
+  both = [cache8.init_cache(b, slots, kv, dim, d, block=16, weights=True, positions=True) for d in ("cuda", "cpu")]
+  lengths = torch.tensor([90, 3, 41], dtype=torch.int32)
+  prompt = [torch.randn(b, 90, kv, dim, generator=gen).bfloat16() for _ in range(2)]
+  for cache in both:
+    d = cache["cached_key"].device
+    cache8.append_(cache, *[t.to(d) for t in prompt], lengths.to(d))
+    cache["cache_index"] += lengths.to(d)
+  w = torch.nn.Parameter(torch.randn(heads * dim, heads * dim, generator=gen) / 20)
+  weights = [F.quantize_weight(w.cuda()), F.quantize_weight(w)]
+  for step in range(60):
+    q = (torch.randn(b, 1, heads, dim, generator=gen) / 4).bfloat16()
+    k, v = [torch.randn(b, 1, kv, dim, generator=gen).bfloat16() for _ in range(2)]
+    outs = []
+    for i, cache in enumerate(both):
+      d = cache["cached_key"].device
+      x = cache8.attention(q.to(d), cache, k.to(d), v.to(d), bias_table=table.to(d))
+      cache["cache_index"] += 1
+      outs.append((x.cpu(), F.linear8(x.flatten(2), weights[i]).cpu()))
+    assert torch.allclose(outs[0][0].float(), outs[1][0].float(), rtol=2.0 ** -7, atol=2.0 ** -8)
+    assert torch.equal(both[0]["cached_key"].cpu(), both[1]["cached_key"])
+    if step in (20, 45):
+      # (weights of 32 bits may differ in the last place: both go by the same ones)
+      both[0]["token_weight"].copy_(both[1]["token_weight"])
+      both = [cache8.evict(c, 40, recent=8, out=cache8.init_cache(b, 96, kv, dim, c["cached_key"].device, block=16,
+                                                                  weights=True, positions=True))[0] for c in both]
+      assert all(torch.equal(both[0][n].cpu(), both[1][n]) for n in both[0])
+
+
+@pytest.mark.parametrize("c", [
+    dict(b=2, h=2, group=4, dim=128, slots=8192, block=64, starts=[8000, 4097], count=1, weights=True),
+    dict(b=1, h=1, group=1, dim=64, slots=70000 // 16 * 16, block=16, starts=[69000], count=1, bias=True),
+    dict(b=2, h=1, group=2, dim=128, slots=4096, block=32, starts=[2048, 3901], count=150, bias=True, weights=True),
+], ids=range(3))
+@pytest.mark.parametrize("dtype", TYPES)
+def test_long(c, dtype):
+  cache, query, key, value, kw = plain.inputs(c, "cuda", dtype)
+  other = {k: v.clone() for k, v in cache.items()}
+  out = launches(lambda: cache8.attention(query, cache, key, value, **kw))
+  ref.cache8_append(other, key, value)
+  wide = {k: kw[k] for k in ("bias_table", "key_mask", "causal", "scale")}
+  want = ref.cache8_attention(query.double(), other, c["count"], **wide)
+  assert torch.equal(cache["cached_key"], other["cached_key"]) and torch.equal(cache["value_absmax"], other["value_absmax"])
+  # |v| is at most 3, and a query's score below 2^6 by its values
+  assert plain.within(out, want.cpu(), torch.full_like(want.cpu(), 3.0), 64.0, c["dim"], c["slots"])
+  if c.get("weights"):
+    assert torch.allclose(cache["token_weight"], other["token_weight"], rtol=1e-4, atol=1e-7)
+
+
+def test_offsets_behind_32_bits():
+  """A cache whose last row lies behind 2^31 codes."""
+  b, slots = 5, 1 << 19
+  cache = cache8.init_cache(b, slots, 8, 128, "cuda", block=128, weights=True)
+  cache["cache_index"].copy_(torch.tensor([0, 0, 0, 0, slots - 9]))
+  key = torch.randn(b, 8, 8, 128, device="cuda", dtype=torch.bfloat16)
+  cache8.append_(cache, key, key)
+  codes, most = cache["cached_key"][4, :, slots - 9:slots - 1], cache["key_absmax"][4, :, -1]
+  assert torch.equal(codes, ref.codes_of(key[4].float().transpose(0, 1), 127, most[:, None, None]))
+  cache["cache_index"] += 8
+  cache["cache_index"][4] = slots
+  hide = torch.zeros(b, slots, dtype=torch.bool, device="cuda")
+  hide[:4, :8], hide[4, slots - 9:slots - 1] = True, True
+  q = torch.randn(b, 1, 8, 128, device="cuda", dtype=torch.bfloat16) / 8
+  out = cache8.attention(q, cache, key_mask=hide, causal=False)
+  v = torch.stack([cache["cached_value"][i, :, :8] if i < 4 else cache["cached_value"][4, :, slots - 9:slots - 1]
+                   for i in range(b)]).float() * (key.float().abs().amax((1, 3))[:, :, None, None] / 127)
+  p = torch.softmax(torch.einsum("blhd,bhsd->bhls", q.float(), v), -1)
+  want = torch.einsum("bhls,bhsd->blhd", p, v)
+  assert torch.allclose(out.float(), want, rtol=2.0 ** -8, atol=2.0 ** -9 * v.abs().max().item())
+  cache["token_weight"][4, :, slots - 1] = 1.0
+  small, kept = cache8.evict(cache, 4, recent=0, out=cache8.init_cache(b, 16, 8, 128, "cuda", block=16, weights=True,
+                                                                       positions=True))
+  assert (kept[4] >= slots - 9).all() and (small["dropped"][4] == slots - 4)
