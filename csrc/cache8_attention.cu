@@ -1,7 +1,7 @@
 // Attention over a key/value cache held in 8 bits (cache8.cuh), for a few query rows a key head: a decode step, the beams
 // of a cross attention, a chunk of a prompt.
 //
-// out = sum_s p_s v_s / sum_s p_s, p_s = exp(scale q.k_s + bias - m), with the running maximum m and sum of a streaming
+// out = sum_s p_s v_s / sum_s p_s, p_s = exp(scale q.k_s + bias - m), with the reference m and the sum of a streaming
 // softmax; k and v are codes times their block's largest value / 127. Bytes bound it: 2 * dim a token and head are read
 // once, and a query row does 4 * dim operations on them. So the codes go from global memory straight into the registers
 // of mma.sync (whose operand of 8 columns the query rows of a head fill or nearly fill; a tcgen05 tile has 64 rows at
@@ -10,21 +10,27 @@
 //
 //   * Channels of a dot product may come in any order: lane (g, t) (g = lane / 4, t = lane % 4) loads channels
 //     64 c + 16 t .. + 15 of tokens g and g + 8, sixteen bytes at a time, and MMA step (c, j) takes bytes 4 j .. 4 j + 3 of
-//     them as its k positions {2t, 2t+1, 2t+8, 2t+9}; the query is laid out the same way.
+//     them: the even ones as its k positions 2t and 2t + 1, the odd ones as 2t + 8 and 2t + 9. The query lies the same way.
 //   * In the second product lane (g, t) loads dim / 8 channels, from g * dim / 8 on, of tokens {2t, 2t+1, 2t+8, 2t+9}; row
 //     tile i takes channels 2 i and 2 i + 1 of each lane as its rows g and g + 8. So a lane ends up with adjacent channels.
 //   * The probabilities, tokens by query rows in the first product's result, turn into the second one's operand by
 //     movmatrix.
-//   * A byte u = code + 128 under the exponent of 1024 is the fp16 number 1024 + u; one subtraction gives the code.
+//   * A key byte u = code + 128 alone is the fp16 number u 2^-24 (below the normal ones, which the tensor cores take as
+//     they are); 128 times the sum of the query is subtracted from the score. Value bytes stand under the exponent of
+//     1024, and 1152 is subtracted from each: their sums run over the whole cache, and an offset of all would leave
+//     nothing of a mean near zero.
 //
 // Queries are scaled by a power of two to just below 2^14, where fp16 holds the values of 16-bit types down to 2^-28 of
-// the row's largest without loss; values of 32 bits go in as two fp16 numbers each (22 bits). Probabilities are 2^14 at
-// the maximum, rounded to 11 bits (a quarter of the rounding of a bf16 result, and random in sign), or two numbers
-// again. A value block's scale goes into the probability, relative to the largest scale that the row has met where it saw
-// something, so that the accumulators need no scaling by token. Sums are in 32 bits.
+// the row's largest without loss; values of 32 bits go in as two fp16 numbers each (22 bits). The reference m is raised
+// only where a probability would come to 2^12.6 (it is 2^4 at the reference): raising it costs a maximum over the lanes
+// and a multiplication of all sums. Probabilities are rounded to 11 bits (a quarter of the rounding of a bf16 result, and
+// random in sign), or are two numbers again. A value block's scale goes into the probability, relative to one that the row
+// has met where it saw something (at most four times as large), so that the accumulators need no scaling by token. Sums are
+// in 32 bits.
 //
-// A block of warps takes a stretch of the slots of one (row, head); its warps take tiles in turn and meet at the end in
-// shared memory, the stretches in workspace.
+// Rows may hold any number of tokens, so the work is dealt out by tiles of 16 tokens: all tiles of all (row, head) laid end
+// to end are cut into one equal piece a warp. What a warp has of a (row, head) that it does not have whole goes to
+// workspace, and a second kernel joins the pieces.
 #include <algorithm>
 
 #include "cache8.cuh"
@@ -35,8 +41,13 @@ namespace {
 constexpr int kWarps = 8;
 constexpr int kThreads = kWarps * 32;
 constexpr int kMaxDistances = 1024;
+constexpr int kMaxBatch = 2048;  // rows of one launch
+constexpr int kMaxBiases = 8192;  // values of a bias table
+constexpr int kEntry = 6;        // what beginning a (row, head) costs, in tiles
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kPeak = 14.f;  // exponent of the largest probability, and of the largest query value
+constexpr float kPeak = 4.f;     // exponent of a probability at the reference
+constexpr float kLimit = 12.6f;  // of the largest; times 4 it is still an fp16 number
+constexpr float kNothing = -3e38f;  // the reference of a row that has seen nothing
 
 struct Cache8Attn {
   Cache8 c;
@@ -44,16 +55,19 @@ struct Cache8Attn {
   void* out;
   const float* table;
   const uint8_t* mask;
-  long long q_sb, q_st, q_sh, table_stride, mask_stride;
+  long long q_sb, q_st, q_sh, mask_stride;
+  int table_stride, q_vec;  // q_vec: whole 16 bytes of a query may be loaded
   int count, group, rows;  // queries a row, heads a key head, their product
   int distances, mask_len, causal;
   int appended;            // tokens of this call behind c.index
   float scale;
-  int splits;
-  float* part;             // [batch * heads, splits, rows, dim], with splits
-  float2* stats;           // [batch * heads, splits, rows]: maximum, sum
-  float* scores;           // [batch * heads, rows, slots] where weights are added up, else null
-  float2* final_stats;     // [batch * heads, rows]: maximum, 1 / sum; with scores
+  int warps;               // pieces that the tiles are cut into
+  int least;               // tiles of a piece at least
+  float* part;             // [row tile, warps, 2, rows of a tile, dim]
+  float2* stats;           // [row tile, warps, 2, rows of a tile]: reference, sum
+  long long* first;        // [batch + 1]: cost in front of a row, in tiles; then that of a piece
+  float* scores;           // [batch * heads, rows, slots], times log2 e, where weights are added up; else null
+  float2* final_stats;     // [batch * heads, rows]: reference, 1 / sum; with scores
   uint8_t buckets[kMaxDistances];  // column of the bias table by distance
 };
 
@@ -72,8 +86,11 @@ __device__ __forceinline__ uint32_t transposed(uint32_t x) {
 }
 __device__ __forceinline__ uint32_t as_u32(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
 __device__ __forceinline__ __half2 as_half2(uint32_t u) { return *reinterpret_cast<__half2*>(&u); }
-__device__ __forceinline__ uint32_t less_1152(uint32_t u) {
-  return as_u32(__hsub2(as_half2(u), as_half2(0x64806480u)));
+// bytes 0 and 2 of codes as two numbers (code + 128) 2^-24
+__device__ __forceinline__ uint32_t key_pair(uint32_t w) { return (w & 0x00ff00ffu) ^ 0x00800080u; }
+// bytes 0 and 2 of codes as two numbers
+__device__ __forceinline__ uint32_t value_pair(uint32_t w) {
+  return as_u32(__hsub2(as_half2((w & 0x00ff00ffu) ^ 0x64806480u), as_half2(0x64806480u)));
 }
 __device__ __forceinline__ float exp2_approx(float x) {
   float r;
@@ -89,6 +106,55 @@ __device__ __forceinline__ int last_seen(const Cache8Attn& p, int start, int end
   const long long first = static_cast<long long>(start) + p.appended - p.count;
   return static_cast<int>(min(first + r / p.group, static_cast<long long>(end) - 1));
 }
+__device__ __forceinline__ int end_of(const Cache8Attn& p, int start) {
+  return static_cast<int>(min(static_cast<long long>(start) + p.appended, static_cast<long long>(p.c.slots)));
+}
+template <typename T>
+__device__ __forceinline__ T* out_row(const Cache8Attn& p, int b, int h, int r) {
+  const int tok = r / p.group;
+  return static_cast<T*>(p.out) +
+         ((static_cast<long long>(b) * p.count + tok) * p.c.heads * p.group + h * p.group + r - tok * p.group) * p.c.dim;
+}
+
+// s_first[b]: what all heads of the rows in front of b cost; s_first[batch]: all.
+__device__ __forceinline__ void count_tiles(const Cache8Attn& p, long long* s_first) {
+  __shared__ long long s_sums[kWarps];
+  const int each = (p.c.batch + kThreads - 1) / kThreads, from = threadIdx.x * each;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  auto cost = [&](int b) {
+    const int tiles = (end_of(p, held_of(p.c, b)) + 15) >> 4;
+    return tiles == 0 ? 0LL : static_cast<long long>(tiles + kEntry) * p.c.heads;
+  };
+  long long mine = 0;
+  for (int b = from; b < min(from + each, p.c.batch); ++b) mine += cost(b);
+  long long sum = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const long long u = __shfl_up_sync(0xffffffffu, sum, o);
+    if (lane >= o) sum += u;
+  }
+  if (lane == 31) s_sums[warp] = sum;
+  __syncthreads();
+  for (int w = 0; w < warp; ++w) sum += s_sums[w];
+  long long run = sum - mine;
+  for (int b = from; b < min(from + each, p.c.batch); ++b) {
+    s_first[b] = run;
+    run += cost(b);
+  }
+  if (threadIdx.x == kThreads - 1) s_first[p.c.batch] = run;
+  __syncthreads();
+}
+
+// Where registers are short, the query's operand lies in shared memory.
+template <int D, int NT, bool kTwo>
+__host__ __device__ constexpr bool query_in_smem() {
+  return NT > 1 || D == 128;
+}
+// What a score column needs beside its reference and sums; in shared memory where there are many columns.
+struct Column {
+  float scale, sum;
+  int lim, where, bias;
+};
 
 // NT: tiles of 8 query rows; MT: tiles of 16 tokens a step; kTwo: operands as two fp16 numbers each.
 template <typename T, int D, int NT, int MT, bool kTwo>
@@ -97,485 +163,605 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1) cache8_attention_ke
   constexpr int VB = D / 8;        // channels a lane has in the second product
   constexpr int MI = D / 16;       // row tiles of the second product
   constexpr int Q2 = kTwo ? 2 : 1;
-  extern __shared__ float s_dyn[];  // [kWarps][NT * 8][D] at the end; before: bias by head and distance
-  __shared__ float s_m[kWarps][NT * 8], s_l[kWarps][NT * 8];
+  constexpr bool kQuerySmem = query_in_smem<D, NT, kTwo>();
+  constexpr bool kColSmem = NT > 1;
+  extern __shared__ uint2 s_query[];   // [kWarps][Q2][NT][CH * 4][32] with kQuerySmem; then the bias table, times log2 e
+  float* s_table = reinterpret_cast<float*>(s_query + (kQuerySmem ? kWarps * Q2 * NT * CH * 4 * 32 : 0));
+  __shared__ long long s_first[kMaxBatch + 1];
+  __shared__ uint8_t s_buckets[kMaxDistances];
+  __shared__ Column s_cols[kColSmem ? kWarps * NT * 8 : 1];
   const Cache8& c = p.c;
-  const int bh = blockIdx.x, split = blockIdx.y, row0 = blockIdx.z * NT * 8;
-  const int b = bh / c.heads, h = bh - b * c.heads;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-
-  const int start = held_of(c, b);
-  const int end_all = static_cast<int>(min(static_cast<long long>(start) + p.appended, static_cast<long long>(c.slots)));
-  // the stretch of this CTA: whole tiles of 16 slots
-  const int end = last_seen(p, start, end_all, min(row0 + NT * 8, p.rows) - 1) + 1;
-  const int tiles = (end + 15) >> 4;
-  const int per = (tiles + p.splits - 1) / p.splits;
-  const int tile0 = split * per, tile1 = min(tile0 + per, tiles);
+  const int row0 = blockIdx.y * NT * 8;
+  const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const int warp = blockIdx.x * kWarps + (threadIdx.x >> 5);
 
   if (p.table != nullptr) {
-    for (int i = threadIdx.x; i < p.group * p.distances; i += kThreads) {
-      const int gq = i / p.distances, d = i - gq * p.distances;
-      s_dyn[i] = p.table[static_cast<long long>(h * p.group + gq) * p.table_stride + p.buckets[d]];
+    for (int i = threadIdx.x; i < p.distances; i += kThreads) s_buckets[i] = p.buckets[i];
+    // (finite ones stay finite)
+    for (int i = threadIdx.x; i < c.heads * p.group * p.table_stride; i += kThreads) {
+      const float x = p.table[i];
+      s_table[i] = fabsf(x) < INFINITY ? fminf(fmaxf(x * kLog2e, -0x1p126f), 0x1p126f) : x;
     }
-    __syncthreads();
   }
+  count_tiles(p, s_first);
+  const long long all = s_first[c.batch];
+  const long long piece = max((all + p.warps - 1) / p.warps, static_cast<long long>(p.least));
+  if (blockIdx.x == 0 && blockIdx.y == 0) {
+    for (int b = threadIdx.x; b <= c.batch; b += kThreads) p.first[b] = s_first[b];
+    if (threadIdx.x == 0) p.first[c.batch + 1] = piece;
+  }
+  chain_wait();  // new tokens are written by the kernel in front
+  chain_release();
+  long long at = warp * piece;
+  const long long stop = min(at + piece, all);
+  if (at >= stop) return;
+  int b = 0;
+  for (int step = 1 << 11; step > 0; step >>= 1)  // the last row that begins at or before `at` and holds something
+    if (b + step < c.batch && s_first[b + step] <= at) b += step;
 
-  // ---- this lane's part of the query rows as the first product's second operand ----
-  uint32_t qf[Q2][NT][CH * 4][2];
-  float q_scale[NT][2];   // of the score columns 2t and 2t + 1
-  int lim[NT][2], where[NT][2], head[NT][2];
-  const int dropped = c.position != nullptr ? c.dropped[b] : 0;
-  const int q_first = static_cast<int>(static_cast<long long>(start) + p.appended - p.count);
+  while (at < stop) {
+    while (s_first[b + 1] <= at) ++b;
+    const int start = held_of(c, b), end = end_of(p, start);
+    const int tiles = (end + 15) >> 4;
+    const int h = static_cast<int>((at - s_first[b]) / (tiles + kEntry));
+    const long long seg = s_first[b] + static_cast<long long>(h) * (tiles + kEntry) + kEntry;  // this (row, head)'s first tile
+    const int tile0 = static_cast<int>(max(at - seg, 0LL)), tile1 = static_cast<int>(min(stop - seg, static_cast<long long>(tiles)));
+    if (tile1 <= 0) break;  // (no more than a part of what the beginning costs)
+    const long long bh = static_cast<long long>(b) * c.heads + h;
+
+    const long long slots0 = bh * c.slots;
+    const int8_t* keys = c.codes[0] + slots0 * D + g * D + 16 * t;
+    const int8_t* values = c.codes[1] + slots0 * D + 2 * t * D + VB * g;
+    const float* k_most = c.absmax[0] + bh * (c.slots >> c.block_log2);
+    const float* v_most = c.absmax[1] + bh * (c.slots >> c.block_log2);
+    const uint8_t* mask = p.mask == nullptr ? nullptr : p.mask + b * p.mask_stride;
+
+    uint4 kr[MT][2][CH];         // tokens g, g + 8
+    uint32_t vr[MT][4][VB / 4];  // tokens 2t, 2t + 1, 2t + 8, 2t + 9
+    float ka[MT], va[MT];
+    // (what the kernel in front may have written is read through L2)
+    auto load_k = [&](int tile) {
 #pragma unroll
-  for (int nt = 0; nt < NT; ++nt) {
-    const int r = row0 + nt * 8 + g;
-    float x[CH][16];
-    uint32_t most = 0;
-    const int i = r / p.group;
-    const T* src = static_cast<const T*>(p.q) + b * p.q_sb + i * p.q_st + (h * p.group + r - i * p.group) * p.q_sh;
+      for (int mt = 0; mt < MT; ++mt) {
+        const int s0 = min(tile + mt, tile1 - 1) << 4;  // (a tile past the end is read again, and hidden)
+        const int8_t* src = keys + static_cast<long long>(s0) * D;
+        ka[mt] = __ldcg(k_most + (s0 >> c.block_log2));
 #pragma unroll
-    for (int ch = 0; ch < CH; ++ch)
+        for (int e = 0; e < 2; ++e)
 #pragma unroll
-      for (int k = 0; k < 16; ++k) {
-        x[ch][k] = r < p.rows ? to_float(src[64 * ch + 16 * t + k]) : 0.f;
-        most = max(most, abs_bits(x[ch][k]));
+          for (int ch = 0; ch < CH; ++ch) kr[mt][e][ch] = __ldcg(reinterpret_cast<const uint4*>(src + 8 * e * D + 64 * ch));
       }
-    most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
-    most = max(most, __shfl_xor_sync(0xffffffffu, most, 2));
-    // 2^up brings the largest to [2^13, 2^14)
-    int up = most == 0 || most >= 0x7f800000u ? 0 : 13 - (static_cast<int>(most >> 23) - 127);
-    up = max(min(up, 126), -113);
-    const float by = __uint_as_float(static_cast<uint32_t>(up + 127) << 23);
-    const float back = __uint_as_float(static_cast<uint32_t>(127 - up) << 23) * p.scale;
+    };
+    auto load_v = [&](int tile) {
 #pragma unroll
-    for (int ch = 0; ch < CH; ++ch)
+      for (int mt = 0; mt < MT; ++mt) {
+        const int s0 = min(tile + mt, tile1 - 1) << 4;
+        const int8_t* src = values + static_cast<long long>(s0) * D;
+        va[mt] = __ldcg(v_most + (s0 >> c.block_log2));
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const float lo = x[ch][2 * j] * by, hi = x[ch][2 * j + 1] * by;
-        const __half2 v = __floats2half2_rn(lo, hi);
-        qf[0][nt][ch * 4 + j / 2][j & 1] = as_u32(v);
-        if (kTwo)
-          qf[Q2 - 1][nt][ch * 4 + j / 2][j & 1] = as_u32(__floats2half2_rn(lo - __low2float(v), hi - __high2float(v)));
-      }
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {  // lane 4 * row has that row's
-      q_scale[nt][e] = __shfl_sync(0xffffffffu, back, (2 * t + e) * 4);
-      const int rr = row0 + nt * 8 + 2 * t + e;
-      lim[nt][e] = last_seen(p, start, end_all, rr);
-      where[nt][e] = q_first + rr / p.group + dropped;
-      head[nt][e] = min(rr, p.rows - 1) % p.group * p.distances;
-    }
-  }
-  // slots up to this one are seen by every row of the tile
-  int all_see = end - 1;
-#pragma unroll
-  for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-    for (int e = 0; e < 2; ++e) all_see = min(all_see, lim[nt][e]);
-  all_see = __reduce_min_sync(0xffffffffu, all_see);
-
-  const long long at = static_cast<long long>(bh) * c.slots;
-  const int8_t* keys = c.codes[0] + at * D;
-  const int8_t* values = c.codes[1] + at * D;
-  const float* k_most = c.absmax[0] + static_cast<long long>(bh) * (c.slots >> c.block_log2);
-  const float* v_most = c.absmax[1] + static_cast<long long>(bh) * (c.slots >> c.block_log2);
-  const uint8_t* mask = p.mask == nullptr ? nullptr : p.mask + b * p.mask_stride;
-
-  float o[NT][MI][4];
-  float m[NT][2], l[NT][2];
-#pragma unroll
-  for (int nt = 0; nt < NT; ++nt) {
-#pragma unroll
-    for (int i = 0; i < MI; ++i)
-#pragma unroll
-      for (int k = 0; k < 4; ++k) o[nt][i][k] = 0.f;
-    m[nt][0] = m[nt][1] = -INFINITY;
-    l[nt][0] = l[nt][1] = 0.f;
-  }
-  float v_ref[NT][2];  // largest value scale that a column met where it saw something
-#pragma unroll
-  for (int nt = 0; nt < NT; ++nt) v_ref[nt][0] = v_ref[nt][1] = 0.f;
-
-  uint4 kr[MT][2][CH];                 // tokens g, g + 8
-  uint32_t vr[MT][4][VB / 4];          // tokens 2t, 2t + 1, 2t + 8, 2t + 9
-  float ka[MT], va[MT];
-  auto load_k = [&](int tile) {
-#pragma unroll
-    for (int mt = 0; mt < MT; ++mt) {
-      const int s0 = min(tile + mt, tile1 - 1) << 4;  // (a tile past the end is read again, and hidden)
-      ka[mt] = k_most[s0 >> c.block_log2];
-#pragma unroll
-      for (int e = 0; e < 2; ++e)
-#pragma unroll
-        for (int ch = 0; ch < CH; ++ch)
-          kr[mt][e][ch] =
-              *reinterpret_cast<const uint4*>(keys + static_cast<long long>(s0 + g + 8 * e) * D + 64 * ch + 16 * t);
-    }
-  };
-  auto load_v = [&](int tile) {
-#pragma unroll
-    for (int mt = 0; mt < MT; ++mt) {
-      const int s0 = min(tile + mt, tile1 - 1) << 4;
-      va[mt] = v_most[s0 >> c.block_log2];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int8_t* src = values + static_cast<long long>(s0 + 2 * t + (e & 1) + 8 * (e >> 1)) * D + VB * g;
-        if (VB == 16) {
-          const uint4 u = *reinterpret_cast<const uint4*>(src);
-          vr[mt][e][0] = u.x, vr[mt][e][1] = u.y, vr[mt][e][VB / 4 - 2] = u.z, vr[mt][e][VB / 4 - 1] = u.w;
-        } else {
-          const uint2 u = *reinterpret_cast<const uint2*>(src);
-          vr[mt][e][0] = u.x, vr[mt][e][1] = u.y;
+        for (int e = 0; e < 4; ++e) {
+          const int8_t* from = src + ((e & 1) + 8 * (e >> 1)) * D;
+          if (VB == 16) {
+            const uint4 u = __ldcg(reinterpret_cast<const uint4*>(from));
+            vr[mt][e][0] = u.x, vr[mt][e][1] = u.y, vr[mt][e][VB / 4 - 2] = u.z, vr[mt][e][VB / 4 - 1] = u.w;
+          } else {
+            const uint2 u = __ldcg(reinterpret_cast<const uint2*>(from));
+            vr[mt][e][0] = u.x, vr[mt][e][1] = u.y;
+          }
         }
       }
+    };
+    if (!kColSmem) {
+      load_k(tile0);
+      load_v(tile0);
     }
-  };
 
-  int tile = tile0 + warp * MT;
-  if (tile < tile1) {
-    load_k(tile);
-    load_v(tile);
-  }
-  for (; tile < tile1; tile += kWarps * MT) {
-    const int next = tile + kWarps * MT;
-    // ---- S^T = K Q^T ----
-    float s[MT][NT][4];
+    // ---- this lane's part of the query rows as the first product's second operand ----
+    uint2 qf[kQuerySmem ? 1 : Q2][kQuerySmem ? 1 : NT][kQuerySmem ? 1 : CH * 4];
+    uint2* s_mine = s_query + static_cast<size_t>(threadIdx.x >> 5) * Q2 * NT * CH * 4 * 32 + lane;
+    Column cols[kColSmem ? 1 : NT][2];  // of the score columns 2t and 2t + 1
+    Column* s_col = s_cols + (kColSmem ? (threadIdx.x >> 5) * NT * 8 + 2 * t : 0);
+    auto column = [&](int nt, int e) -> const Column& {
+      if constexpr (kColSmem) return s_col[nt * 8 + e];
+      else return cols[nt][e];
+    };
+    int all_see = end - 1;  // slots up to this one are seen by every row of the tile
+    __syncwarp();
+    const int dropped = c.position != nullptr ? c.dropped[b] : 0;
+    const int q_first = static_cast<int>(static_cast<long long>(start) + p.appended - p.count);
 #pragma unroll
-    for (int mt = 0; mt < MT; ++mt) {
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int k = 0; k < 4; ++k) s[mt][nt][k] = 0.f;
+    for (int nt = 0; nt < NT; ++nt) {
+      const int r = row0 + nt * 8 + g;
+      float x[CH][16];
+      uint32_t most = 0;
+      const int i = r / p.group;
+      const T* src = static_cast<const T*>(p.q) + b * p.q_sb + i * p.q_st + (h * p.group + r - i * p.group) * p.q_sh;
 #pragma unroll
       for (int ch = 0; ch < CH; ++ch) {
-        const uint32_t w0[4] = {kr[mt][0][ch].x, kr[mt][0][ch].y, kr[mt][0][ch].z, kr[mt][0][ch].w};
-        const uint32_t w1[4] = {kr[mt][1][ch].x, kr[mt][1][ch].y, kr[mt][1][ch].z, kr[mt][1][ch].w};
+        constexpr int E = 16 / sizeof(T);
+        alignas(16) T part[16];
+        if (r < p.rows && p.q_vec) {
+#pragma unroll
+          for (int k = 0; k < 16 / E; ++k)
+            *reinterpret_cast<uint4*>(part + k * E) = *reinterpret_cast<const uint4*>(src + 64 * ch + 16 * t + k * E);
+        }
+#pragma unroll
+        for (int k = 0; k < 16; ++k) {
+          x[ch][k] = r >= p.rows ? 0.f : p.q_vec ? to_float(part[k]) : to_float(src[64 * ch + 16 * t + k]);
+          most = max(most, abs_bits(x[ch][k]));
+        }
+      }
+      most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
+      most = max(most, __shfl_xor_sync(0xffffffffu, most, 2));
+      // 2^up brings the largest to [2^13, 2^14)
+      int up = most == 0 || most >= 0x7f800000u ? 0 : 13 - (static_cast<int>(most >> 23) - 127);
+      up = max(min(up, 126), -113);
+      const float by = __uint_as_float(static_cast<uint32_t>(up + 127) << 23);
+      // 2^24 back from the keys' exponent; the scale of a key block is its largest value / 127; scores are times log2 e
+      const float back = __uint_as_float(static_cast<uint32_t>(127 - up) << 23) * p.scale * (0x1p24f / 127.f * kLog2e);
+      float sum = 0.f;
+#pragma unroll
+      for (int ch = 0; ch < CH; ++ch)
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const uint32_t u0 = w0[j] ^ 0x80808080u, u1 = w1[j] ^ 0x80808080u;
-          const uint32_t a0 = less_1152(__byte_perm(u0, 0x64646464u, 0x4140));
-          const uint32_t a2 = less_1152(__byte_perm(u0, 0x64646464u, 0x4342));
-          const uint32_t a1 = less_1152(__byte_perm(u1, 0x64646464u, 0x4140));
-          const uint32_t a3 = less_1152(__byte_perm(u1, 0x64646464u, 0x4342));
+          uint32_t f[Q2][2];
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
+          for (int k = 0; k < 2; ++k) {
+            const float lo = x[ch][4 * j + k] * by, hi = x[ch][4 * j + 2 + k] * by;
+            const __half2 v = __floats2half2_rn(lo, hi);
+            f[0][k] = as_u32(v);
+            sum += __low2float(v) + __high2float(v);
+            if (kTwo) {
+              const __half2 rest = __floats2half2_rn(lo - __low2float(v), hi - __high2float(v));
+              f[Q2 - 1][k] = as_u32(rest);
+              sum += __low2float(rest) + __high2float(rest);
+            }
+          }
 #pragma unroll
-            for (int w = 0; w < Q2; ++w)
-              mma_f16(s[mt][nt], a0, a1, a2, a3, qf[w][nt][ch * 4 + j][0], qf[w][nt][ch * 4 + j][1]);
+          for (int w = 0; w < Q2; ++w) {
+            if constexpr (kQuerySmem) s_mine[((w * NT + nt) * CH * 4 + ch * 4 + j) * 32] = make_uint2(f[w][0], f[w][1]);
+            else qf[w][nt][ch * 4 + j] = make_uint2(f[w][0], f[w][1]);
+          }
         }
+      sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+      sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {  // lane 4 * row has that row's
+        const int rr = row0 + nt * 8 + 2 * t + e;
+        Column col;
+        col.scale = __shfl_sync(0xffffffffu, back, (2 * t + e) * 4);
+        col.sum = __shfl_sync(0xffffffffu, sum, (2 * t + e) * 4) * 0x1p-17f;  // 128 times, at the keys' exponent
+        col.lim = last_seen(p, start, end, rr);
+        col.where = q_first + rr / p.group + dropped;
+        col.bias = (h * p.group + min(rr, p.rows - 1) % p.group) * p.table_stride;
+        all_see = min(all_see, col.lim);
+        if constexpr (kColSmem) s_col[nt * 8 + e] = col;  // (all lanes of a column write the same)
+        else cols[nt][e] = col;
       }
     }
-    float k_scale[MT];
-#pragma unroll
-    for (int mt = 0; mt < MT; ++mt) k_scale[mt] = ka[mt] * (1.f / 127.f);
-    if (next < tile1) load_k(next);
+    all_see = __reduce_min_sync(0xffffffffu, all_see);
+    __syncwarp();
+    if (kColSmem) {
+      load_k(tile0);
+      load_v(tile0);
+    }
 
-    bool some[MT];  // whether the mask shows a token of the tile
-    // ---- scores of tokens g (k = 0, 1) and g + 8 (k = 2, 3), query rows 2t (k = 0, 2) and 2t + 1 ----
+    float o[NT][MI][4];
+    float ref[NT][2], l[NT][2], v_ref[NT][2], v_inv[NT][2];
 #pragma unroll
-    for (int mt = 0; mt < MT; ++mt) {
-      const int s0 = (tile + mt) << 4;
-      const bool inside = tile + mt < tile1;
-      const bool whole = inside && s0 + 15 <= all_see && mask == nullptr;
-      bool shown[2] = {true, true};
-      some[mt] = inside;
-      if (mask != nullptr) {
+    for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
-        for (int e = 0; e < 2; ++e) shown[e] = s0 + g + 8 * e < p.mask_len && mask[s0 + g + 8 * e] != 0;
-        some[mt] = inside && __any_sync(0xffffffffu, shown[0] || shown[1]);
+      for (int i = 0; i < MI; ++i)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) o[nt][i][k] = 0.f;
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        ref[nt][e] = kNothing;
+        l[nt][e] = v_inv[nt][e] = 0.f;
+        v_ref[nt][e] = row0 + nt * 8 + 2 * t + e < p.rows ? 0.f : 3e38f;  // (a column without a row asks for nothing)
       }
-      int place[2] = {s0 + g, s0 + g + 8};
-      if (p.table != nullptr && c.position != nullptr) {
+    }
+
+    for (int tile = tile0; tile < tile1; tile += MT) {
+      // ---- S^T = K Q^T ----
+      float s[MT][NT][4];
 #pragma unroll
-        for (int e = 0; e < 2; ++e) place[e] = c.position[at + min(s0 + g + 8 * e, c.slots - 1)];
-      }
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          float x = s[mt][nt][k] * (k_scale[mt] * q_scale[nt][k & 1]);
-          if (p.table != nullptr) {
-            const int d = where[nt][k & 1] - place[k >> 1];
-            x += s_dyn[head[nt][k & 1] + min(max(d, 0), p.distances - 1)];
-          }
-          if (!whole && !(inside && shown[k >> 1] && s0 + g + 8 * (k >> 1) <= lim[nt][k & 1])) x = -INFINITY;
-          s[mt][nt][k] = x;
-        }
-      if (p.scores != nullptr && inside) {
+      for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            const int r = row0 + nt * 8 + 2 * t + (k & 1);
-            if (r < p.rows)
-              p.scores[(static_cast<long long>(bh) * p.rows + r) * c.slots + s0 + g + 8 * (k >> 1)] = s[mt][nt][k];
-          }
-      }
-    }
-
-    // ---- running maximum, probabilities ----
-    bool moved = false;
-    float shrink[NT][2];
-    uint32_t pf[Q2][MT][NT][2];
+          for (int k = 0; k < 4; ++k) s[mt][nt][k] = 0.f;
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-      float base[2], v_inv[2];
+      for (int ch = 0; ch < CH; ++ch)
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        float x = m[nt][e];
+        for (int j = 0; j < 4; ++j) {
+          uint32_t a[MT][4];
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt) x = fmaxf(x, fmaxf(s[mt][nt][e], s[mt][nt][2 + e]));
-        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
-        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
-        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
-        base[e] = x == -INFINITY ? 0.f : x;
-        const float f = exp2_approx((m[nt][e] - base[e]) * kLog2e);  // (0 at first)
-        float v_new = v_ref[nt][e];
+          for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt)
-          if (some[mt] && lim[nt][e] >= (tile + mt) << 4 && va[mt] < INFINITY) v_new = fmaxf(v_new, va[mt]);
-        moved |= x != m[nt][e] || v_new != v_ref[nt][e];
-        v_inv[e] = v_new > 0.f ? __frcp_rn(v_new) : 0.f;
-        shrink[nt][e] = f * (v_ref[nt][e] * v_inv[e]);  // (0 where nothing had been met)
-        v_ref[nt][e] = v_new;
-        m[nt][e] = x;
-        l[nt][e] *= f;
-      }
-#pragma unroll
-      for (int mt = 0; mt < MT; ++mt) {
-        const float r[2] = {va[mt] * v_inv[0], va[mt] * v_inv[1]};
-        float pr[4];
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const float x = s[mt][nt][k];
-          const float e = exp2_approx(fmaf(x - base[k & 1], kLog2e, kPeak));
-          l[nt][k & 1] += e;
-          // (a hidden token counts for nothing whatever its block holds)
-          pr[k] = x == -INFINITY ? 0.f : e * r[k & 1];
-        }
-        const __half2 v0 = __floats2half2_rn(pr[0], pr[1]), v1 = __floats2half2_rn(pr[2], pr[3]);
-        pf[0][mt][nt][0] = transposed(as_u32(v0));
-        pf[0][mt][nt][1] = transposed(as_u32(v1));
-        if (kTwo) {
-          pf[Q2 - 1][mt][nt][0] =
-              transposed(as_u32(__floats2half2_rn(pr[0] - __low2float(v0), pr[1] - __high2float(v0))));
-          pf[Q2 - 1][mt][nt][1] =
-              transposed(as_u32(__floats2half2_rn(pr[2] - __low2float(v1), pr[3] - __high2float(v1))));
-        }
-      }
-    }
-    if (__any_sync(0xffffffffu, moved)) {
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int i = 0; i < MI; ++i)
-#pragma unroll
-          for (int k = 0; k < 4; ++k) o[nt][i][k] *= shrink[nt][k & 1];
-    }
-
-    // ---- O^T += V^T P^T ----
-#pragma unroll
-    for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-      for (int w = 0; w < VB / 4; ++w) {
-        const uint32_t u0 = vr[mt][0][w] ^ 0x80808080u, u1 = vr[mt][1][w] ^ 0x80808080u;
-        const uint32_t u2 = vr[mt][2][w] ^ 0x80808080u, u3 = vr[mt][3][w] ^ 0x80808080u;
-#pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          const uint32_t x = __byte_perm(u0, u1, half ? 0x7362 : 0x5140), y = __byte_perm(u2, u3, half ? 0x7362 : 0x5140);
-          const uint32_t a0 = less_1152(__byte_perm(x, 0x64646464u, 0x4140));
-          const uint32_t a1 = less_1152(__byte_perm(x, 0x64646464u, 0x4342));
-          const uint32_t a2 = less_1152(__byte_perm(y, 0x64646464u, 0x4140));
-          const uint32_t a3 = less_1152(__byte_perm(y, 0x64646464u, 0x4342));
+            for (int e = 0; e < 2; ++e) {
+              const uint32_t w = j == 0 ? kr[mt][e][ch].x : j == 1 ? kr[mt][e][ch].y : j == 2 ? kr[mt][e][ch].z : kr[mt][e][ch].w;
+              a[mt][e] = key_pair(w);
+              a[mt][2 + e] = key_pair(w >> 8);
+            }
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-            for (int q2 = 0; q2 < Q2; ++q2)
-              mma_f16(o[nt][2 * w + half], a0, a1, a2, a3, pf[q2][mt][nt][0], pf[q2][mt][nt][1]);
+            for (int w = 0; w < Q2; ++w) {
+              uint2 q;
+              if constexpr (kQuerySmem) q = s_mine[((w * NT + nt) * CH * 4 + ch * 4 + j) * 32];
+              else q = qf[w][nt][ch * 4 + j];
+#pragma unroll
+              for (int mt = 0; mt < MT; ++mt) mma_f16(s[mt][nt], a[mt][0], a[mt][1], a[mt][2], a[mt][3], q.x, q.y);
+            }
+        }
+      float k_scale[MT];
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt) k_scale[mt] = ka[mt];
+      if (tile + MT < tile1) load_k(tile + MT);
+
+      // ---- scores of tokens g (k = 0, 1) and g + 8 (k = 2, 3), query rows 2t (k = 0, 2) and 2t + 1 ----
+      bool some[MT];       // whether the mask shows a token of the tile
+      bool raise = false;  // whether a reference has to go up
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt) {
+        const int s0 = (tile + mt) << 4;
+        const bool inside = tile + mt < tile1;
+        some[mt] = inside;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const float sum = column(nt, e).sum, by = k_scale[mt] * column(nt, e).scale;
+            s[mt][nt][e] = (s[mt][nt][e] - sum) * by;
+            s[mt][nt][2 + e] = (s[mt][nt][2 + e] - sum) * by;
+          }
+        }
+        if (p.table != nullptr) {
+          int place[2] = {s0 + g, s0 + g + 8};
+          if (c.position != nullptr) {
+#pragma unroll
+            for (int e = 0; e < 2; ++e) place[e] = __ldcg(c.position + slots0 + min(s0 + g + 8 * e, c.slots - 1));
+          }
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const int d = column(nt, k & 1).where - place[k >> 1];
+              s[mt][nt][k] += s_table[column(nt, k & 1).bias + s_buckets[min(max(d, 0), p.distances - 1)]];
+            }
+        }
+        if (!(inside && s0 + 15 <= all_see && mask == nullptr)) {
+          bool shown[2] = {inside, inside};
+          if (mask != nullptr) {
+#pragma unroll
+            for (int e = 0; e < 2; ++e) shown[e] = inside && s0 + g + 8 * e < p.mask_len && mask[s0 + g + 8 * e] != 0;
+            some[mt] = __any_sync(0xffffffffu, shown[0] || shown[1]);
+          }
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              if (!shown[k >> 1] || s0 + g + 8 * (k >> 1) > column(nt, k & 1).lim) s[mt][nt][k] = -INFINITY;
+        }
+        if (p.scores != nullptr && inside) {
+          float* to = p.scores + bh * p.rows * c.slots;
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const int r = row0 + nt * 8 + 2 * t + e;
+              if (r < p.rows) {
+                to[r * c.slots + s0 + g] = s[mt][nt][e];
+                to[r * c.slots + s0 + g + 8] = s[mt][nt][2 + e];
+              }
+            }
+        }
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            raise |= fmaxf(s[mt][nt][e], s[mt][nt][2 + e]) - ref[nt][e] > kLimit;
+            raise |= va[mt] > 4.f * v_ref[nt][e];
+          }
+      }
+
+      // ---- references ----
+      if (__any_sync(0xffffffffu, raise)) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            float x = -INFINITY, v = v_ref[nt][e];
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt) {
+              x = fmaxf(x, fmaxf(s[mt][nt][e], s[mt][nt][2 + e]));
+              if (some[mt] && column(nt, e).lim >= (tile + mt) << 4 && va[mt] < INFINITY) v = fmaxf(v, va[mt]);
+            }
+            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
+            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
+            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
+            const float up = fmaxf(x - kPeak, ref[nt][e]);
+            const float f = exp2_approx(ref[nt][e] - up);
+            v_inv[nt][e] = v > 0.f ? __frcp_rn(v) : 0.f;
+            const float shrink = f * (v_ref[nt][e] * v_inv[nt][e]);  // (0 where nothing had been met)
+            ref[nt][e] = up;
+            l[nt][e] *= f;
+            v_ref[nt][e] = v;
+#pragma unroll
+            for (int i = 0; i < MI; ++i) o[nt][i][e] *= shrink, o[nt][i][2 + e] *= shrink;
+          }
+      }
+
+      // ---- probabilities ----
+      uint32_t pf[Q2][MT][NT][2];
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          const float r[2] = {va[mt] * v_inv[nt][0], va[mt] * v_inv[nt][1]};
+          float pr[4];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            pr[k] = exp2_approx(s[mt][nt][k] - ref[nt][k & 1]);
+            l[nt][k & 1] += pr[k];
+            pr[k] *= r[k & 1];
+          }
+          if (!(va[mt] < INFINITY)) {  // a block that is not finite: what is hidden counts for nothing all the same
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              if (s[mt][nt][k] == -INFINITY) pr[k] = 0.f;
+          }
+          const __half2 v0 = __floats2half2_rn(pr[0], pr[1]), v1 = __floats2half2_rn(pr[2], pr[3]);
+          pf[0][mt][nt][0] = transposed(as_u32(v0));
+          pf[0][mt][nt][1] = transposed(as_u32(v1));
+          if (kTwo) {
+            pf[Q2 - 1][mt][nt][0] =
+                transposed(as_u32(__floats2half2_rn(pr[0] - __low2float(v0), pr[1] - __high2float(v0))));
+            pf[Q2 - 1][mt][nt][1] =
+                transposed(as_u32(__floats2half2_rn(pr[2] - __low2float(v1), pr[3] - __high2float(v1))));
+          }
+        }
+
+      // ---- O^T += V^T P^T ----
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+        for (int w = 0; w < VB / 4; ++w)
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            const uint32_t x = __byte_perm(vr[mt][0][w], vr[mt][1][w], half ? 0x7632 : 0x5410);
+            const uint32_t y = __byte_perm(vr[mt][2][w], vr[mt][3][w], half ? 0x7632 : 0x5410);
+            const uint32_t a0 = value_pair(x), a1 = value_pair(x >> 8), a2 = value_pair(y), a3 = value_pair(y >> 8);
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+              for (int q2 = 0; q2 < Q2; ++q2)
+                mma_f16(o[nt][2 * w + half], a0, a1, a2, a3, pf[q2][mt][nt][0], pf[q2][mt][nt][1]);
+          }
+      if (tile + MT < tile1) load_v(tile + MT);
+    }
+
+    // ---- the whole (row, head), or a piece of it ----
+    const bool whole = tile0 == 0 && tile1 == tiles;
+    // a warp has one piece that began before its own first tile at most, and one that goes on behind its last
+    const long long slot = ((static_cast<long long>(blockIdx.y) * p.warps + warp) * 2 + (tile0 == 0 ? 1 : 0)) * NT * 8;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        float sum = l[nt][e];
+        sum += __shfl_xor_sync(0xffffffffu, sum, 4);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 8);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 16);
+        const int col = nt * 8 + 2 * t + e, r = row0 + col;
+        if (r >= p.rows) continue;
+        // (a row that nothing was seen of may have sums of 0 * NaN)
+        const float f = v_ref[nt][e] * (1.f / 127.f) * (whole ? 1.f / sum : 1.f);
+        float x[VB];
+#pragma unroll
+        for (int i = 0; i < MI; ++i) {
+          x[2 * i] = sum == 0.f ? 0.f : o[nt][i][e] * f;
+          x[2 * i + 1] = sum == 0.f ? 0.f : o[nt][i][2 + e] * f;
+        }
+        if (whole) {
+          T* dst = out_row<T>(p, b, h, r) + VB * g;
+#pragma unroll
+          for (int i = 0; i < VB; ++i) dst[i] = from_float<T>(x[i]);
+          if (g == 0 && p.scores != nullptr) p.final_stats[bh * p.rows + r] = make_float2(ref[nt][e], sum == 0.f ? 0.f : 1.f / sum);
+        } else {
+          float4* dst = reinterpret_cast<float4*>(p.part + (slot + col) * D + VB * g);
+#pragma unroll
+          for (int i = 0; i < VB / 4; ++i) dst[i] = make_float4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]);
+          if (g == 0) p.stats[slot + col] = make_float2(ref[nt][e], sum);
         }
       }
-    if (next < tile1) load_v(next);
-  }
-
-  // ---- the warps meet ----
-#pragma unroll
-  for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      float x = l[nt][e];
-      x += __shfl_xor_sync(0xffffffffu, x, 4);
-      x += __shfl_xor_sync(0xffffffffu, x, 8);
-      x += __shfl_xor_sync(0xffffffffu, x, 16);
-      if (g == 0) {
-        s_m[warp][nt * 8 + 2 * t + e] = m[nt][e];
-        s_l[warp][nt * 8 + 2 * t + e] = x;
-      }
-    }
-  __syncthreads();  // (and the bias table is read for the last time)
-#pragma unroll
-  for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      const int col = nt * 8 + 2 * t + e;
-      float most = -INFINITY;
-#pragma unroll
-      for (int w = 0; w < kWarps; ++w) most = fmaxf(most, s_m[w][col]);
-      const float f = m[nt][e] == -INFINITY ? 0.f : exp2_approx((m[nt][e] - most) * kLog2e) * (v_ref[nt][e] * (1.f / 127.f));
-      float* dst = s_dyn + (static_cast<long long>(warp) * NT * 8 + col) * D + VB * g;
-#pragma unroll
-      for (int i = 0; i < MI; ++i) {
-        // a row that nothing was seen of has sums of 0, or of 0 * NaN
-        const float x = m[nt][e] == -INFINITY && l[nt][e] == 0.f ? 0.f : o[nt][i][e] * f;
-        const float y = m[nt][e] == -INFINITY && l[nt][e] == 0.f ? 0.f : o[nt][i][2 + e] * f;
-        *reinterpret_cast<float2*>(dst + 2 * i) = make_float2(x, y);
-      }
-    }
-  __syncthreads();
-  for (int i = threadIdx.x; i < NT * 8 * D; i += kThreads) {
-    const int col = i / D, r = row0 + col;
-    if (r >= p.rows) break;
-    float most = -INFINITY, sum = 0.f, x = 0.f;
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) most = fmaxf(most, s_m[w][col]);
-    const float base = most == -INFINITY ? 0.f : most;
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
-      sum += s_l[w][col] * exp2_approx((s_m[w][col] - base) * kLog2e);
-      x += s_dyn[w * NT * 8 * D + i];
-    }
-    const int d = i - col * D;
-    if (p.splits == 1) {
-      const int tok = r / p.group;
-      T* dst = static_cast<T*>(p.out) +
-               ((static_cast<long long>(b) * p.count + tok) * c.heads * p.group + h * p.group + r - tok * p.group) * D + d;
-      *dst = from_float<T>(sum == 0.f ? 0.f : x / sum);
-      if (d == 0 && p.scores != nullptr)
-        p.final_stats[static_cast<long long>(bh) * p.rows + r] = make_float2(base, sum == 0.f ? 0.f : 1.f / sum);
-    } else {
-      const long long part = (static_cast<long long>(bh) * p.splits + split) * p.rows + r;
-      p.part[part * D + d] = x;
-      if (d == 0) p.stats[part] = make_float2(most, sum);
-    }
+    at = seg + tile1;
   }
 }
 
-// One warp a query row: joins the stretches.
-template <typename T>
-__global__ void __launch_bounds__(kThreads) cache8_join_kernel(const __grid_constant__ Cache8Attn p, long long total) {
-  const long long at = static_cast<long long>(blockIdx.x) * kWarps + (threadIdx.x >> 5);
-  if (at >= total) return;
-  const int lane = threadIdx.x & 31, D = p.c.dim;
-  const long long bh = at / p.rows;
-  const int r = static_cast<int>(at - bh * p.rows);
-  const float2* stats = p.stats + bh * p.splits * p.rows + r;
-  float most = -INFINITY;
-  for (int s = lane; s < p.splits; s += 32) most = fmaxf(most, stats[static_cast<long long>(s) * p.rows].x);
-  most = warp_max(most);
-  const float base = most == -INFINITY ? 0.f : most;
-  float sum = 0.f, x[4] = {0.f, 0.f, 0.f, 0.f};
-  const float* part = p.part + (bh * p.splits * p.rows + r) * D;
-  for (int s = 0; s < p.splits; ++s) {
-    const float2 ml = stats[static_cast<long long>(s) * p.rows];
-    const float f = exp2_approx((ml.x - base) * kLog2e);
-    sum += ml.y * f;
+// A block a query row: joins its pieces, where it has several, or none. A lane has four adjacent channels.
+constexpr int kJoinThreads = 128;
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kJoinThreads) cache8_join_kernel(const __grid_constant__ Cache8Attn p, int tile_rows) {
+  constexpr int L = D / 4, S = kJoinThreads / L;  // lanes a piece, pieces at a time
+  __shared__ float4 s_x[S][L];
+  __shared__ float2 s_stat[S];
+  const int bh = blockIdx.x, r = blockIdx.y, b = bh / p.c.heads, h = bh - b * p.c.heads;
+  const int sub = threadIdx.x / L, lane = threadIdx.x % L;
+  chain_wait();
+  chain_release();
+  const long long piece = __ldcg(p.first + p.c.batch + 1), from = __ldcg(p.first + b);
+  const long long cost = (__ldcg(p.first + b + 1) - from) / p.c.heads;  // tiles + kEntry, or 0
+  const long long seg = from + h * cost + kEntry;  // its first tile
+  const int w0 = static_cast<int>(seg / piece), w1 = cost == 0 ? w0 - 1 : static_cast<int>((seg + cost - kEntry - 1) / piece);
+  if (w0 == w1) return;  // one warp had it whole
+  // the first piece is its warp's second, the others are their warps' first ones
+  const long long base = (static_cast<long long>(r / tile_rows) * p.warps) * 2 * tile_rows + r % tile_rows;
+  auto slot = [&](int w) { return base + (w * 2LL + (w == w0 ? 1 : 0)) * tile_rows; };
+  float high = kNothing, sum = 0.f;
+  float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+  constexpr int U = 4;  // pieces requested at a time
+  for (int w = w0 + sub; w <= w1; w += S * U) {
+    float2 st[U];
+    float4 v[U];
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-      if (j * 32 < D) x[j] += f * part[static_cast<long long>(s) * p.rows * D + j * 32 + lane];
+    for (int u = 0; u < U; ++u) {
+      const int at = min(w + u * S, w1);
+      st[u] = __ldcg(p.stats + slot(at));
+      v[u] = __ldcg(reinterpret_cast<const float4*>(p.part + slot(at) * D) + lane);
+      if (w + u * S > w1) st[u] = make_float2(kNothing, 0.f);
+    }
+    float top = high;
+#pragma unroll
+    for (int u = 0; u < U; ++u) top = fmaxf(top, st[u].x);
+    const float f0 = exp2_approx(high - top);
+    high = top;
+    sum *= f0, x.x *= f0, x.y *= f0, x.z *= f0, x.w *= f0;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (st[u].y == 0.f) continue;
+      const float f = exp2_approx(st[u].x - top);
+      sum += st[u].y * f;
+      x.x += v[u].x * f, x.y += v[u].y * f, x.z += v[u].z * f, x.w += v[u].w * f;
+    }
   }
-  const int b = static_cast<int>(bh / p.c.heads), h = static_cast<int>(bh - static_cast<long long>(b) * p.c.heads);
-  const int tok = r / p.group;
-  T* dst = static_cast<T*>(p.out) +
-           ((static_cast<long long>(b) * p.count + tok) * p.c.heads * p.group + h * p.group + r - tok * p.group) * D;
+  s_x[sub][lane] = x;
+  if (lane == 0) s_stat[sub] = make_float2(high, sum);
+  __syncthreads();
+  if (sub != 0) return;
+  float top = kNothing;
 #pragma unroll
-  for (int j = 0; j < 4; ++j)
-    if (j * 32 < D) dst[j * 32 + lane] = from_float<T>(sum == 0.f ? 0.f : x[j] / sum);
-  if (lane == 0 && p.scores != nullptr) p.final_stats[at] = make_float2(base, sum == 0.f ? 0.f : 1.f / sum);
+  for (int i = 0; i < S; ++i) top = fmaxf(top, s_stat[i].x);
+  sum = 0.f;
+  x = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+  for (int i = 0; i < S; ++i) {
+    const float f = s_stat[i].y == 0.f ? 0.f : exp2_approx(s_stat[i].x - top);
+    const float4 v = s_x[i][lane];
+    sum += s_stat[i].y * f;
+    if (f != 0.f) x.x += v.x * f, x.y += v.y * f, x.z += v.z * f, x.w += v.w * f;
+  }
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  T* dst = out_row<T>(p, b, h, r) + 4 * lane;
+  const float o[4] = {x.x * inv, x.y * inv, x.z * inv, x.w * inv};
+#pragma unroll
+  for (int j = 0; j < 4; ++j) dst[j] = from_float<T>(sum == 0.f ? 0.f : o[j]);
+  if (lane == 0 && p.scores != nullptr) p.final_stats[static_cast<long long>(bh) * p.rows + r] = make_float2(top, inv);
 }
 
 // weight[slot] += the probabilities that the query rows gave it
 __global__ void __launch_bounds__(kThreads) cache8_weight_kernel(const __grid_constant__ Cache8Attn p) {
   const int bh = blockIdx.x, b = bh / p.c.heads;
   const int s = blockIdx.y * kThreads + threadIdx.x;
-  const int start = held_of(p.c, b);
-  const int end = static_cast<int>(min(static_cast<long long>(start) + p.appended, static_cast<long long>(p.c.slots)));
+  const int start = held_of(p.c, b), end = end_of(p, start);
+  chain_wait();
+  chain_release();
   if (s >= end) return;
+  float* weight = p.c.weight + static_cast<long long>(bh) * p.c.slots + s;
   float sum = 0.f;
   for (int r = 0; r < p.rows; ++r) {
     if (s > last_seen(p, start, end, r)) continue;  // (no score was written)
-    const float x = p.scores[(static_cast<long long>(bh) * p.rows + r) * p.c.slots + s];
-    const float2 st = p.final_stats[static_cast<long long>(bh) * p.rows + r];
-    // (the sums are of probabilities 2^kPeak times as large)
-    sum += exp2_approx(fmaf(x - st.x, kLog2e, kPeak)) * st.y;
+    const float x = __ldcg(p.scores + (static_cast<long long>(bh) * p.rows + r) * p.c.slots + s);
+    const float2 st = __ldcg(p.final_stats + static_cast<long long>(bh) * p.rows + r);
+    if (x > -INFINITY || x != x) sum += exp2_approx(x - st.x) * st.y;
   }
-  p.c.weight[static_cast<long long>(bh) * p.c.slots + s] += sum;
+  *weight = __ldcg(weight) + sum;
 }
 
+// Launches a kernel that may begin while the one in front of it still runs; it waits for it by itself (chain_wait).
+template <typename... Params, typename... Args>
+cudaError_t launch_behind(bool behind, void (*kernel)(Params...), dim3 grid, int threads, size_t smem,
+                          cudaStream_t stream, Args&&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = behind ? 1 : 0;
+  count_launches(1);
+  return cudaLaunchKernelEx(&cfg, kernel, std::forward<Args>(args)...);
+}
+
+constexpr int tile_rows_of(int rows) { return rows <= 8 ? 8 : 32; }
+
 template <typename T, int D, int NT, int MT, bool kTwo>
-cudaError_t launch_tile(const Cache8Attn& p, cudaStream_t stream) {
-  const size_t smem = std::max(static_cast<size_t>(kWarps) * NT * 8 * D * 4,
-                               p.table == nullptr ? size_t{0} : static_cast<size_t>(p.group) * p.distances * 4);
+cudaError_t launch_tile(const Cache8Attn& p, bool behind, cudaStream_t stream) {
+  constexpr size_t query = !query_in_smem<D, NT, kTwo>() ? 0 : static_cast<size_t>(kWarps) * (kTwo ? 2 : 1) * NT * (D / 64) * 4 * 32 * sizeof(uint2);
+  const size_t smem = query + (p.table == nullptr ? 0 : sizeof(float) * p.c.heads * p.group * p.table_stride);
   static bool set[64] = {false};
   int dev = 0;
   cudaGetDevice(&dev);
   if (!set[dev & 63]) {
     cudaError_t e = cudaFuncSetAttribute(cache8_attention_kernel<T, D, NT, MT, kTwo>,
-                                         cudaFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024);
+                                         cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(query) + kMaxBiases * 4);
     if (e != cudaSuccess) return e;
     set[dev & 63] = true;
   }
-  const int row_tiles = (p.rows + NT * 8 - 1) / (NT * 8);
-  cache8_attention_kernel<T, D, NT, MT, kTwo>
-      <<<dim3(static_cast<unsigned>(p.c.batch) * p.c.heads, p.splits, row_tiles), kThreads, smem, stream>>>(p);
-  count_launches(1);
-  return cudaGetLastError();
+  const dim3 grid(p.warps / kWarps, (p.rows + NT * 8 - 1) / (NT * 8));
+  return launch_behind(behind, cache8_attention_kernel<T, D, NT, MT, kTwo>, grid, kThreads, smem, stream, p);
 }
 
 template <typename T, bool kTwo>
-cudaError_t launch_all(const Cache8Attn& p, int nt, cudaStream_t stream) {
+cudaError_t launch_all(const Cache8Attn& p, bool behind, cudaStream_t stream) {
+  const int tile_rows = tile_rows_of(p.rows);
   cudaError_t e;
   if (p.c.dim == 64)
-    e = nt == 1 ? launch_tile<T, 64, 1, 2, kTwo>(p, stream) : launch_tile<T, 64, 4, 1, kTwo>(p, stream);
+    e = tile_rows == 8 ? launch_tile<T, 64, 1, 2, kTwo>(p, behind, stream) : launch_tile<T, 64, 4, 1, kTwo>(p, behind, stream);
   else
-    e = nt == 1 ? launch_tile<T, 128, 1, 1, kTwo>(p, stream) : launch_tile<T, 128, kTwo ? 2 : 4, 1, kTwo>(p, stream);
+    e = tile_rows == 8 ? launch_tile<T, 128, 1, 1, kTwo>(p, behind, stream) : launch_tile<T, 128, 4, 1, kTwo>(p, behind, stream);
   if (e != cudaSuccess) return e;
-  if (p.splits > 1) {
-    const long long total = static_cast<long long>(p.c.batch) * p.c.heads * p.rows;
-    cache8_join_kernel<T><<<static_cast<unsigned>((total + kWarps - 1) / kWarps), kThreads, 0, stream>>>(p, total);
-    count_launches(1);
-  }
-  if (p.scores != nullptr) {
-    cache8_weight_kernel<<<dim3(static_cast<unsigned>(p.c.batch) * p.c.heads, (p.c.slots + kThreads - 1) / kThreads),
-                           kThreads, 0, stream>>>(p);
-    count_launches(1);
-  }
-  return cudaGetLastError();
+  const dim3 rows(static_cast<unsigned>(p.c.batch) * p.c.heads, p.rows);
+  e = p.c.dim == 64 ? launch_behind(true, cache8_join_kernel<T, 64>, rows, kJoinThreads, 0, stream, p, tile_rows)
+                    : launch_behind(true, cache8_join_kernel<T, 128>, rows, kJoinThreads, 0, stream, p, tile_rows);
+  if (e != cudaSuccess || p.scores == nullptr) return e;
+  return launch_behind(true, cache8_weight_kernel,
+                       dim3(static_cast<unsigned>(p.c.batch) * p.c.heads, (p.c.slots + kThreads - 1) / kThreads),
+                       kThreads, 0, stream, p);
 }
 
-// Tiles of 8 query rows a block takes, and stretches that the slots are cut into.
-void plan(const Cache8& c, int rows, bool two, int& nt, int& splits) {
-  nt = rows <= 8 ? 1 : 4;
-  const int tile_rows = nt == 1 ? 8 : c.dim == 128 && two ? 16 : 32;
-  const long long blocks = static_cast<long long>(c.batch) * c.heads * ((rows + tile_rows - 1) / tile_rows);
-  // enough blocks for a few rounds over the SMs, none of under 256 slots
-  const long long wanted = (4LL * num_sms() + blocks - 1) / blocks;
-  splits = static_cast<int>(std::max(1LL, std::min({wanted, static_cast<long long>(c.slots) / 256, 1024LL})));
+// Rows `from` on of a cache.
+Cache8 rows_of(Cache8 c, int from, int count) {
+  const long long by_head = static_cast<long long>(from) * c.heads;
+  for (int i = 0; i < 2; ++i) {
+    c.codes[i] += by_head * c.slots * c.dim;
+    c.absmax[i] += by_head * (c.slots >> c.block_log2);
+  }
+  c.index += static_cast<long long>(from) * c.index_stride;
+  if (c.weight) c.weight += by_head * c.slots;
+  if (c.position) c.position += by_head * c.slots, c.dropped += from;
+  c.batch = count;
+  return c;
 }
 
-struct Workspace {
-  size_t part = 0, stats = 0, scores = 0, final_stats = 0, total = 0;
+struct Plan {
+  int warps, least;
+  size_t part = 0, stats = 0, first = 0, scores = 0, final_stats = 0, total = 0;
 };
-Workspace workspace(const Cache8& c, int rows, int splits) {
-  Workspace w;
+Plan plan(Cache8 c, int rows) {
+  Plan w;
+  c.batch = std::min(c.batch, kMaxBatch);
+  const int tile_rows = tile_rows_of(rows), row_tiles = (rows + tile_rows - 1) / tile_rows;
+  // the warps that the SMs hold at a time, shared by the tiles of query rows; no piece of under 64 tokens
+  const long long room = static_cast<long long>(num_sms()) * kWarps * (tile_rows == 8 ? 2 : 1) / row_tiles;
+  const long long most = static_cast<long long>(c.batch) * c.heads * (c.slots / 16 + kEntry) / (4 + kEntry) + 1;
+  w.least = 4 + kEntry;
+  w.warps = static_cast<int>(std::max<long long>(1, std::min(room, most) / kWarps)) * kWarps;
   const size_t bh = static_cast<size_t>(c.batch) * c.heads;
   auto take = [&](size_t bytes) {
     const size_t at = w.total;
     w.total += (bytes + 15) / 16 * 16;
     return at;
   };
-  if (splits > 1) {
-    w.part = take(bh * splits * rows * c.dim * 4);
-    w.stats = take(bh * splits * rows * 8);
-  }
+  const size_t parts = static_cast<size_t>(row_tiles) * w.warps * 2 * tile_rows;
+  w.part = take(parts * c.dim * 4);
+  w.stats = take(parts * 8);
+  w.first = take((static_cast<size_t>(c.batch) + 2) * 8);
   if (c.weight != nullptr) {
     w.scores = take(bh * rows * c.slots * 4);
     w.final_stats = take(bh * rows * 8);
@@ -585,15 +771,17 @@ Workspace workspace(const Cache8& c, int rows, int splits) {
 
 int check_query(const Cache8& c, const T5xCache8Query* q, const T5xNewTokens* n) {
   if (q->count < 1 || q->group < 1 || q->type < 0 || q->type > 2 ||
-      static_cast<long long>(q->count) * q->group > (1 << 20) || c.heads * static_cast<long long>(c.batch) > (1 << 24))
+      static_cast<long long>(q->count) * q->group > 65535 || c.heads * static_cast<long long>(c.batch) > (1 << 24))
     return set_error("cache8_attention: %d queries of type %d, %d heads a key head", q->count, q->type, q->group);
   const int bytes = q->type == 2 ? 4 : 2;
   if (!q->query || !q->out || !aligned_to(bytes, {q->query, q->out}) || !aligned_to(4, {q->table}))
     return set_error("cache8_attention: a null or misaligned pointer");
   if (q->table && (!q->buckets || q->distances < 1 || q->distances > kMaxDistances ||
-                   static_cast<long long>(q->group) * q->distances > 40000))
+                   q->table_stride < 1 || q->table_stride * c.heads * q->group > kMaxBiases))
     return set_error("cache8_attention: biases of %d distances for %d heads", q->distances, q->group);
   if (q->key_mask && (q->mask_len < 0 || q->mask_len > c.slots)) return set_error("cache8_attention: a mask of %d slots", q->mask_len);
+  if (c.weight && static_cast<long long>(q->count) * q->group * c.slots > 0x7fffffffLL)
+    return set_error("cache8_attention: %d queries with weights over %d slots", q->count, c.slots);
   if (n && (n->count != q->count || n->lengths)) return set_error("cache8_attention: %d queries, %d new tokens", q->count, n->count);
   return n ? check_new_tokens("cache8_attention", n) : 0;
 }
@@ -607,9 +795,7 @@ T5X_API long long t5x_cache8_attention_bytes(const T5xCache8* cache, const T5xCa
   if (int e = t5x::check_cache8("cache8_attention", c)) return e;
   if (int e = t5x::check_query(c, q, n)) return e;
   if (c.batch == 0) return 0;
-  int nt, splits;
-  t5x::plan(c, q->count * q->group, q->type == 2, nt, splits);
-  return static_cast<long long>(t5x::workspace(c, q->count * q->group, splits).total);
+  return static_cast<long long>(t5x::plan(c, q->count * q->group).total);
 }
 
 T5X_API int t5x_cache8_attention(const T5xCache8* cache, const T5xCache8Query* q, const T5xNewTokens* n, void* workspace,
@@ -628,8 +814,10 @@ T5X_API int t5x_cache8_attention(const T5xCache8* cache, const T5xCache8Query* q
   p.q_sb = q->stride_batch;
   p.q_st = q->stride_token;
   p.q_sh = q->stride_head;
-  p.table_stride = q->table_stride;
+  p.table_stride = static_cast<int>(q->table_stride);
   p.mask_stride = q->mask_stride;
+  const int q_size = q->type == 2 ? 4 : 2;
+  p.q_vec = t5x::aligned_to(16, {q->query}) && ((q->stride_batch | q->stride_token | q->stride_head) * q_size) % 16 == 0;
   p.count = q->count;
   p.group = q->group;
   p.rows = q->count * q->group;
@@ -639,21 +827,33 @@ T5X_API int t5x_cache8_attention(const T5xCache8* cache, const T5xCache8Query* q
   p.causal = q->causal;
   p.appended = n ? n->count : 0;
   p.scale = q->scale;
-  int nt;
-  t5x::plan(c, p.rows, q->type == 2, nt, p.splits);
-  const t5x::Workspace w = t5x::workspace(c, p.rows, p.splits);
-  if (w.total && (!workspace || !t5x::aligned_to(16, {workspace})))
+  const t5x::Plan w = t5x::plan(c, p.rows);
+  if (!workspace || !t5x::aligned_to(16, {workspace}))
     return t5x::set_error("cache8_attention: a null or misaligned workspace");
   uint8_t* ws = static_cast<uint8_t*>(workspace);
+  p.warps = w.warps;
+  p.least = w.least;
   p.part = reinterpret_cast<float*>(ws + w.part);
   p.stats = reinterpret_cast<float2*>(ws + w.stats);
+  p.first = reinterpret_cast<long long*>(ws + w.first);
   p.scores = c.weight ? reinterpret_cast<float*>(ws + w.scores) : nullptr;
   p.final_stats = reinterpret_cast<float2*>(ws + w.final_stats);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (n)
     if (int e = t5x::cache8_append(c, n, st)) return e;
-  const cudaError_t e = q->type == 0   ? t5x::launch_all<__nv_bfloat16, false>(p, nt, st)
-                        : q->type == 1 ? t5x::launch_all<__half, false>(p, nt, st)
-                                       : t5x::launch_all<float, true>(p, nt, st);
-  return e == cudaSuccess ? 0 : t5x::set_error("cache8_attention launch: %s", cudaGetErrorString(e));
+  const int size = q->type == 2 ? 4 : 2;
+  for (int from = 0; from < c.batch; from += t5x::kMaxBatch) {
+    t5x::Cache8Attn part = p;
+    part.c = t5x::rows_of(c, from, std::min(c.batch - from, t5x::kMaxBatch));
+    part.q = static_cast<const char*>(p.q) + from * p.q_sb * size;
+    part.out = static_cast<char*>(p.out) + static_cast<long long>(from) * p.rows * c.heads * c.dim * size;
+    part.mask = p.mask ? p.mask + from * p.mask_stride : nullptr;
+    // (what follows the append alone may begin while it runs; the workspace of a launch is the next one's)
+    const bool behind = n != nullptr && from == 0;
+    const cudaError_t e = q->type == 0   ? t5x::launch_all<__nv_bfloat16, false>(part, behind, st)
+                          : q->type == 1 ? t5x::launch_all<__half, false>(part, behind, st)
+                                         : t5x::launch_all<float, true>(part, behind, st);
+    if (e != cudaSuccess) return t5x::set_error("cache8_attention launch: %s", cudaGetErrorString(e));
+  }
+  return 0;
 }

@@ -149,11 +149,10 @@ def attention(query: torch.Tensor, cache: dict, key: Optional[torch.Tensor] = No
   if key_mask is not None and (key_mask.dim() != 2 or key_mask.shape[0] != b or key_mask.shape[1] > slots or
                                key_mask.device != query.device):
     raise ValueError(f"attention: a mask is [{b}, at most {slots}]; got {tuple(key_mask.shape)}")
-  if query.shape[1] * (query.shape[2] // h) > 1 << 20:
-    raise ValueError("attention: over 2^20 query rows a head")
-  covered = bias_table is None or (max_distance < native.CACHE8_DISTANCES and
-                                   query.shape[2] // h * (max_distance + 1) <= native.CACHE8_BIASES)
-  if not (_native_ok(cache, query.dtype) and covered):
+  if query.shape[1] * (query.shape[2] // h) > 65535:
+    raise ValueError("attention: over 65535 query rows a head")
+  if not (_native_ok(cache, query.dtype) and (bias_table is None or (
+      max_distance < native.CACHE8_DISTANCES and query.shape[2] * num_buckets <= native.CACHE8_BIASES))):
     if key is not None:
       ref.cache8_append(cache, key, value)
     return ref.cache8_attention(query, cache, 0 if key is None else key.shape[1], bias_table, num_buckets, max_distance,

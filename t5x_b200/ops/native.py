@@ -1346,7 +1346,7 @@ register_signature("t5x_linear8", [c_void_p, c_int, c_int, c_int, c_ll, c_void_p
                    [c_void_p] * 3)
 
 CACHE8_TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
-CACHE8_DISTANCES, CACHE8_BIASES = 1024, 40000  # distances of a bias table; distances times heads that share keys
+CACHE8_DISTANCES, CACHE8_BIASES = 1024, 8192  # distances, values of a bias table
 _cache8_buckets: dict = {}
 
 
@@ -1404,7 +1404,7 @@ def cache8_attention(query, cache, key, value, bias_table, num_buckets, max_dist
                    causal=int(causal), scale=scale)
   q.stride_batch, q.stride_token, q.stride_head = query.stride()[:3]
   if bias_table is not None:
-    bias_table = bias_table.detach().float().contiguous()
+    bias_table = bias_table.detach()[:heads, :num_buckets].float().contiguous()
     buckets = _buckets_of(num_buckets, max_distance)
     q.table, q.table_stride, q.distances = bias_table.data_ptr(), bias_table.shape[1], len(buckets)
     q.buckets = ctypes.cast(ctypes.c_char_p(buckets), c_void_p)
