@@ -13,64 +13,21 @@ namespace {
 // ---------------------------------------------------------------------------
 constexpr int kAppendThreads = 128;
 
-template <typename T>
-struct NewTokens {
-  const T* x[2];               // keys, values [batch, token, head, dim]
-  long long sb[2], st[2], sh[2];
-  const int* lengths;          // new tokens by row, or null
-  int count;
-};
-
-template <typename T>
-__global__ void __launch_bounds__(kAppendThreads) cache8_append_kernel(const __grid_constant__ Cache8 c, const __grid_constant__ NewTokens<T> n) {
+template <typename T, int D>
+__global__ void __launch_bounds__(kAppendThreads)
+    cache8_append_kernel(const __grid_constant__ Cache8 c, const __grid_constant__ NewTokens<T> n) {
   __shared__ uint32_t s_most[kAppendThreads / 32];
   const int what = blockIdx.x & 1, b = blockIdx.z, h = blockIdx.y;
-  const int block = 1 << c.block_log2;
+  chain_release();  // (an attention behind this waits for what it reads of it)
   const int start = held_of(c, b);
   const int fresh = n.lengths == nullptr ? n.count : min(max(n.lengths[b], 0), n.count);
   const int blk = (start >> c.block_log2) + static_cast<int>(blockIdx.x >> 1);
   if (blk >= c.slots >> c.block_log2) return;
   const int first = blk << c.block_log2;
   const int lo = max(start, first);
-  const int hi = static_cast<int>(min(min(static_cast<long long>(start) + fresh, static_cast<long long>(first) + block),
+  const int hi = static_cast<int>(min(min(static_cast<long long>(start) + fresh, static_cast<long long>(first) + (1 << c.block_log2)),
                                       static_cast<long long>(c.slots)));
-  if (lo >= hi) return;
-
-  const long long bh = static_cast<long long>(b) * c.heads + h;
-  const T* x = n.x[what] + b * n.sb[what] + h * n.sh[what];
-  int8_t* codes = c.codes[what] + (bh * c.slots + first) * c.dim;
-  float* absmax = c.absmax[what] + bh * (c.slots >> c.block_log2) + blk;
-  const int old = (lo - first) * c.dim, all = (hi - lo) * c.dim;
-
-  uint32_t most = 0;
-  for (int i = threadIdx.x; i < all; i += kAppendThreads) {
-    const int tok = i / c.dim, d = i - tok * c.dim;
-    most = max(most, abs_bits(to_float(x[(lo - start + tok) * n.st[what] + d])));
-  }
-  most = __reduce_max_sync(0xffffffffu, most);
-  if ((threadIdx.x & 31) == 0) s_most[threadIdx.x >> 5] = most;
-  const float before = old > 0 ? *absmax : 0.f;
-  __syncthreads();
-#pragma unroll
-  for (int w = 0; w < kAppendThreads / 32; ++w) most = max(most, s_most[w]);
-  most = max(most, abs_bits(before));
-  const float a = __uint_as_float(most);
-  if (most != abs_bits(before)) {
-    const Coder again(before, a);
-    for (int i = threadIdx.x; i < old; i += kAppendThreads) codes[i] = static_cast<int8_t>(again(codes[i]));
-  }
-  const Coder code(127.f, a);
-  for (int i = threadIdx.x; i < all; i += kAppendThreads) {
-    const int tok = i / c.dim, d = i - tok * c.dim;
-    codes[old + i] = static_cast<int8_t>(code(to_float(x[(lo - start + tok) * n.st[what] + d])));
-  }
-  __syncthreads();  // everyone has read *absmax
-  if (threadIdx.x == 0) *absmax = a;
-  if (what == 0)
-    for (int s = lo + threadIdx.x; s < hi; s += kAppendThreads) {
-      if (c.weight != nullptr) c.weight[bh * c.slots + s] = 0.f;
-      if (c.position != nullptr) c.position[bh * c.slots + s] = s + c.dropped[b];
-    }
+  if (lo < hi) append_block<T, D, kAppendThreads>(c, n, what, b, h, start, lo, hi, threadIdx.x, s_most);
 }
 
 // ---------------------------------------------------------------------------
@@ -258,19 +215,13 @@ namespace {
 
 template <typename T>
 int launch_append(const Cache8& c, const T5xNewTokens* in, cudaStream_t stream) {
-  NewTokens<T> n;
-  for (int i = 0; i < 2; ++i) {
-    n.x[i] = static_cast<const T*>(in->x[i]);
-    n.sb[i] = in->stride_batch[i];
-    n.st[i] = in->stride_token[i];
-    n.sh[i] = in->stride_head[i];
-  }
-  n.lengths = static_cast<const int*>(in->lengths);
-  n.count = in->count;
+  const NewTokens<T> n = make_tokens<T>(in);
   const int block = 1 << c.block_log2;
   const long long touched = std::min((static_cast<long long>(n.count) + block - 2) / block + 1,
                                      static_cast<long long>(c.slots >> c.block_log2));
-  cache8_append_kernel<T><<<dim3(2 * static_cast<unsigned>(touched), c.heads, c.batch), kAppendThreads, 0, stream>>>(c, n);
+  const dim3 grid(2 * static_cast<unsigned>(touched), c.heads, c.batch);
+  if (c.dim == 64) cache8_append_kernel<T, 64><<<grid, kAppendThreads, 0, stream>>>(c, n);
+  else cache8_append_kernel<T, 128><<<grid, kAppendThreads, 0, stream>>>(c, n);
   count_launches(1);
   const cudaError_t e = cudaGetLastError();
   return e == cudaSuccess ? 0 : set_error("cache8_append launch: %s", cudaGetErrorString(e));

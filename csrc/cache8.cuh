@@ -8,6 +8,8 @@
 #pragma once
 #include <cuda_fp16.h>
 
+#include <algorithm>
+
 #include "common.cuh"
 #include "t5x_ops.h"
 
@@ -75,6 +77,102 @@ __device__ __forceinline__ __half from_float(float x) { return __float2half_rn(x
 // tokens that row b holds
 __device__ __forceinline__ int held_of(const Cache8& c, int b) {
   return min(max(c.index[static_cast<long long>(b) * c.index_stride], 0), c.slots);
+}
+
+// New keys and values [batch, token, head, dim].
+template <typename T>
+struct NewTokens {
+  const T* x[2];
+  long long sb[2], st[2], sh[2];
+  const int* lengths;  // tokens by row, or null: `count` each
+  int count;
+  int vec;             // four adjacent values may be loaded at a time
+};
+
+template <typename T>
+__device__ __forceinline__ void load_four(const T* src, bool vec, float (&v)[4]) {
+  alignas(4 * sizeof(T)) T in[4];
+  if (vec) {
+    if constexpr (sizeof(T) == 4) *reinterpret_cast<uint4*>(in) = *reinterpret_cast<const uint4*>(src);
+    else *reinterpret_cast<uint2*>(in) = *reinterpret_cast<const uint2*>(src);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) in[i] = src[i];
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v[i] = to_float(in[i]);
+}
+
+// Slots lo .. hi of one block of a (row, head), its keys (what = 0) or values, get the tokens from lo - start on. By THREADS
+// threads, number `tid`, all of which call it, with s_most[THREADS / 32] of their own; all threads of the CTA meet in it.
+template <typename T, int D, int THREADS>
+__device__ __forceinline__ void append_block(const Cache8& c, const NewTokens<T>& n, int what, int b, int h, int start, int lo,
+                                             int hi, int tid, uint32_t* s_most) {
+  const long long bh = static_cast<long long>(b) * c.heads + h;
+  const int blk = lo >> c.block_log2, first = blk << c.block_log2;
+  const T* x = n.x[what] + b * n.sb[what] + h * n.sh[what];
+  const long long st = n.st[what];
+  int8_t* codes = c.codes[what] + bh * c.slots * D;
+  float* absmax = c.absmax[what] + bh * (c.slots >> c.block_log2) + blk;
+  constexpr int lanes = D / 4, step = THREADS / lanes;
+  const int d = tid % lanes * 4, from = tid / lanes;
+  const bool vec = n.vec != 0;
+
+  const float before = lo > first ? __ldcg(absmax) : 0.f;
+  uint32_t most = 0;
+#pragma unroll 4
+  for (int s = lo + from; s < hi; s += step) {
+    float v[4];
+    load_four(x + (s - start) * st + d, vec, v);
+    most = max(max(most, max(abs_bits(v[0]), abs_bits(v[1]))), max(abs_bits(v[2]), abs_bits(v[3])));
+  }
+  most = __reduce_max_sync(0xffffffffu, most);
+  if ((tid & 31) == 0) s_most[tid >> 5] = most;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < THREADS / 32; ++w) most = max(most, s_most[w]);
+  most = max(most, abs_bits(before));
+  const float a = __uint_as_float(most);
+  if (most != abs_bits(before) && lo > first) {
+    const Coder again(before, a);
+#pragma unroll 2
+    for (int s = first + from; s < lo; s += step) {
+      char4* at = reinterpret_cast<char4*>(codes + static_cast<long long>(s) * D + d);
+      const char4 v = *at;
+      *at = make_char4(again(v.x), again(v.y), again(v.z), again(v.w));
+    }
+  }
+  const Coder code(127.f, a);
+#pragma unroll 2
+  for (int s = lo + from; s < hi; s += step) {
+    float v[4];
+    load_four(x + (s - start) * st + d, vec, v);
+    *reinterpret_cast<char4*>(codes + static_cast<long long>(s) * D + d) = make_char4(code(v[0]), code(v[1]), code(v[2]), code(v[3]));
+  }
+  if (what == 0)
+    for (int s = lo + tid; s < hi; s += THREADS) {
+      if (c.weight != nullptr) c.weight[bh * c.slots + s] = 0.f;
+      if (c.position != nullptr) c.position[bh * c.slots + s] = s + c.dropped[b];
+    }
+  __syncthreads();  // everyone has read *absmax and s_most
+  if (tid == 0) *absmax = a;
+}
+
+template <typename T>
+NewTokens<T> make_tokens(const T5xNewTokens* in) {
+  NewTokens<T> n = {};
+  if (in == nullptr) return n;
+  n.vec = 1;
+  for (int i = 0; i < 2; ++i) {
+    n.x[i] = static_cast<const T*>(in->x[i]);
+    n.sb[i] = in->stride_batch[i];
+    n.st[i] = in->stride_token[i];
+    n.sh[i] = in->stride_head[i];
+    if (!aligned_to(4 * sizeof(T), {in->x[i]}) || (n.sb[i] | n.st[i] | n.sh[i]) % 4 != 0) n.vec = 0;
+  }
+  n.lengths = static_cast<const int*>(in->lengths);
+  n.count = in->count;
+  return n;
 }
 
 Cache8 make_cache8(const T5xCache8* in);

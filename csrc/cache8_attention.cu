@@ -28,9 +28,11 @@
 // has met where it saw something (at most four times as large), so that the accumulators need no scaling by token. Sums are
 // in 32 bits.
 //
-// Rows may hold any number of tokens, so the work is dealt out by tiles of 16 tokens: all tiles of all (row, head) laid end
-// to end are cut into one equal piece a warp. What a warp has of a (row, head) that it does not have whole goes to
-// workspace, and a second kernel joins the pieces.
+// Two ways to deal out the work. Over short caches, and longer ones where there are many (row, head), a CTA takes one: it
+// appends the new tokens, its warps take tiles of 16 tokens in turn and meet in shared memory, and the scores that the
+// weights are made from never leave it: one launch. Over long ones (of all lengths) all tiles of all (row, head) laid end to
+// end are cut into one equal piece a warp; what a warp has of a (row, head) that it does not have whole goes to workspace,
+// and a second kernel joins the pieces.
 #include <algorithm>
 
 #include "cache8.cuh"
@@ -38,8 +40,7 @@
 namespace t5x {
 namespace {
 
-constexpr int kWarps = 8;
-constexpr int kThreads = kWarps * 32;
+constexpr int kPieceWarps = 8;  // warps a CTA, of the kernel by pieces
 constexpr int kMaxDistances = 1024;
 constexpr int kMaxBatch = 2048;  // rows of one launch
 constexpr int kMaxBiases = 8192;  // values of a bias table
@@ -61,6 +62,7 @@ struct Cache8Attn {
   int distances, mask_len, causal;
   int appended;            // tokens of this call behind c.index
   float scale;
+  unsigned long long by_group;  // 2^32 / group, rounded up: r / group for r below 2^16 by one multiplication
   int warps;               // pieces that the tiles are cut into
   int least;               // tiles of a piece at least
   float* part;             // [row tile, warps, 2, rows of a tile, dim]
@@ -98,26 +100,29 @@ __device__ __forceinline__ float exp2_approx(float x) {
   return r;
 }
 
+__device__ __forceinline__ int token_of(const Cache8Attn& p, int r) { return static_cast<int>((r * p.by_group) >> 32); }
+
 // Slots that query row r (token r / group of this call) sees: up to this one.
 __device__ __forceinline__ int last_seen(const Cache8Attn& p, int start, int end, int r) {
   if (r >= p.rows) return -1;
   if (!p.causal) return end - 1;
   // the queries are the last `count` tokens held
   const long long first = static_cast<long long>(start) + p.appended - p.count;
-  return static_cast<int>(min(first + r / p.group, static_cast<long long>(end) - 1));
+  return static_cast<int>(min(first + token_of(p, r), static_cast<long long>(end) - 1));
 }
 __device__ __forceinline__ int end_of(const Cache8Attn& p, int start) {
   return static_cast<int>(min(static_cast<long long>(start) + p.appended, static_cast<long long>(p.c.slots)));
 }
 template <typename T>
 __device__ __forceinline__ T* out_row(const Cache8Attn& p, int b, int h, int r) {
-  const int tok = r / p.group;
+  const int tok = token_of(p, r);
   return static_cast<T*>(p.out) +
          ((static_cast<long long>(b) * p.count + tok) * p.c.heads * p.group + h * p.group + r - tok * p.group) * p.c.dim;
 }
 
 // s_first[b]: what all heads of the rows in front of b cost; s_first[batch]: all.
 __device__ __forceinline__ void count_tiles(const Cache8Attn& p, long long* s_first) {
+  constexpr int kWarps = kPieceWarps, kThreads = kWarps * 32;
   __shared__ long long s_sums[kWarps];
   const int each = (p.c.batch + kThreads - 1) / kThreads, from = threadIdx.x * each;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -157,56 +162,79 @@ struct Column {
 };
 
 // NT: tiles of 8 query rows; MT: tiles of 16 tokens a step; kTwo: operands as two fp16 numbers each.
-template <typename T, int D, int NT, int MT, bool kTwo>
-__global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1) cache8_attention_kernel(const __grid_constant__ Cache8Attn p) {
+// kBlock: a CTA a (row, head), with the append.
+template <typename T, int D, int NT, int MT, bool kTwo, bool kBlock, int kWarps>
+__global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 16 / kWarps : 1)
+    cache8_attention_kernel(const __grid_constant__ Cache8Attn p, const __grid_constant__ NewTokens<T> fresh) {
+  static_assert(!kBlock || NT == 1, "a CTA takes 8 query rows");
+  constexpr int kThreads = kWarps * 32;
   constexpr int CH = D / 64;       // 64-channel pieces
   constexpr int VB = D / 8;        // channels a lane has in the second product
   constexpr int MI = D / 16;       // row tiles of the second product
   constexpr int Q2 = kTwo ? 2 : 1;
   constexpr bool kQuerySmem = query_in_smem<D, NT, kTwo>();
   constexpr bool kColSmem = NT > 1;
-  extern __shared__ uint2 s_query[];   // [kWarps][Q2][NT][CH * 4][32] with kQuerySmem; then the bias table, times log2 e
+  // [kWarps][Q2][NT][CH * 4][32] with kQuerySmem; then the bias table, times log2 e (with kBlock that of the head's rows);
+  // then, with kBlock, sums of the warps [kWarps][rows][D] and scores [rows][slots]
+  extern __shared__ uint2 s_query[];
   float* s_table = reinterpret_cast<float*>(s_query + (kQuerySmem ? kWarps * Q2 * NT * CH * 4 * 32 : 0));
-  __shared__ long long s_first[kMaxBatch + 1];
+  __shared__ long long s_first[kBlock ? 1 : kMaxBatch + 1];
   __shared__ uint8_t s_buckets[kMaxDistances];
   __shared__ Column s_cols[kColSmem ? kWarps * NT * 8 : 1];
   const Cache8& c = p.c;
-  const int row0 = blockIdx.y * NT * 8;
+  const int row0 = kBlock ? 0 : blockIdx.y * NT * 8;
   const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int warp = blockIdx.x * kWarps + (threadIdx.x >> 5);
 
   if (p.table != nullptr) {
     for (int i = threadIdx.x; i < p.distances; i += kThreads) s_buckets[i] = p.buckets[i];
-    // (finite ones stay finite)
-    for (int i = threadIdx.x; i < c.heads * p.group * p.table_stride; i += kThreads) {
-      const float x = p.table[i];
+    const int count = (kBlock ? 1 : c.heads) * p.group * p.table_stride;
+    const float* from = p.table + (kBlock ? blockIdx.x * count : 0);
+    for (int i = threadIdx.x; i < count; i += kThreads) {
+      const float x = from[i];  // (finite ones stay finite)
       s_table[i] = fabsf(x) < INFINITY ? fminf(fmaxf(x * kLog2e, -0x1p126f), 0x1p126f) : x;
     }
   }
-  count_tiles(p, s_first);
-  const long long all = s_first[c.batch];
-  const long long piece = max((all + p.warps - 1) / p.warps, static_cast<long long>(p.least));
-  if (blockIdx.x == 0 && blockIdx.y == 0) {
-    for (int b = threadIdx.x; b <= c.batch; b += kThreads) p.first[b] = s_first[b];
-    if (threadIdx.x == 0) p.first[c.batch + 1] = piece;
-  }
-  chain_wait();  // new tokens are written by the kernel in front
-  chain_release();
-  long long at = warp * piece;
-  const long long stop = min(at + piece, all);
-  if (at >= stop) return;
+  long long at = 0, stop = 1, piece = 0;
   int b = 0;
-  for (int step = 1 << 11; step > 0; step >>= 1)  // the last row that begins at or before `at` and holds something
-    if (b + step < c.batch && s_first[b + step] <= at) b += step;
+  if constexpr (kBlock) {
+    b = blockIdx.y;
+  } else {
+    count_tiles(p, s_first);
+    const long long all = s_first[c.batch];
+    piece = max((all + p.warps - 1) / p.warps, static_cast<long long>(p.least));
+    if (blockIdx.x == 0 && blockIdx.y == 0) {
+      for (int i = threadIdx.x; i <= c.batch; i += kThreads) p.first[i] = s_first[i];
+      if (threadIdx.x == 0) p.first[c.batch + 1] = piece;
+    }
+    chain_wait();  // new tokens are written by the kernel in front
+    chain_release();
+    at = warp * piece;
+    stop = min(at + piece, all);
+    if (at >= stop) return;
+    for (int step = 1 << 11; step > 0; step >>= 1)  // the last row that begins at or before `at` and holds something
+      if (b + step < c.batch && s_first[b + step] <= at) b += step;
+  }
 
   while (at < stop) {
-    while (s_first[b + 1] <= at) ++b;
+    if constexpr (!kBlock)
+      while (s_first[b + 1] <= at) ++b;
     const int start = held_of(c, b), end = end_of(p, start);
     const int tiles = (end + 15) >> 4;
-    const int h = static_cast<int>((at - s_first[b]) / (tiles + kEntry));
-    const long long seg = s_first[b] + static_cast<long long>(h) * (tiles + kEntry) + kEntry;  // this (row, head)'s first tile
-    const int tile0 = static_cast<int>(max(at - seg, 0LL)), tile1 = static_cast<int>(min(stop - seg, static_cast<long long>(tiles)));
-    if (tile1 <= 0) break;  // (no more than a part of what the beginning costs)
+    int h, tile0, tile1;
+    long long seg = 0;
+    if constexpr (kBlock) {
+      h = blockIdx.x;
+      tile0 = (threadIdx.x >> 5) * MT;
+      tile1 = tiles;
+      at = stop;
+    } else {
+      h = static_cast<int>((at - s_first[b]) / (tiles + kEntry));
+      seg = s_first[b] + static_cast<long long>(h) * (tiles + kEntry) + kEntry;  // this (row, head)'s first tile
+      tile0 = static_cast<int>(max(at - seg, 0LL));
+      tile1 = static_cast<int>(min(stop - seg, static_cast<long long>(tiles)));
+      if (tile1 <= 0) break;  // (no more than a part of what the beginning costs)
+    }
     const long long bh = static_cast<long long>(b) * c.heads + h;
 
     const long long slots0 = bh * c.slots;
@@ -251,9 +279,27 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1) cache8_attention_ke
         }
       }
     };
-    if (!kColSmem) {
+    if (!kColSmem && tile0 < tile1) {
       load_k(tile0);
       load_v(tile0);
+    }
+    if constexpr (kBlock) {
+      if (p.appended > 0) {
+        __shared__ uint32_t s_most[kWarps];
+        const int half = threadIdx.x / (kThreads / 2);  // keys by one half of the threads, values by the other
+        for (int lo = start; lo < end;) {
+          const int hi = min(end, ((lo >> c.block_log2) + 1) << c.block_log2);
+          append_block<T, D, kThreads / 2>(c, fresh, half, b, h, start, lo, hi, threadIdx.x % (kThreads / 2),
+                                        s_most + half * (kWarps / 2));
+          lo = hi;
+        }
+      }
+      __syncthreads();
+      // what was requested of a block that got tokens is requested again
+      if (p.appended > 0 && tile0 < tile1 && min(tile0 + MT, tile1) << 4 > start >> c.block_log2 << c.block_log2) {
+        load_k(tile0);
+        load_v(tile0);
+      }
     }
 
     // ---- this lane's part of the query rows as the first product's second operand ----
@@ -274,7 +320,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1) cache8_attention_ke
       const int r = row0 + nt * 8 + g;
       float x[CH][16];
       uint32_t most = 0;
-      const int i = r / p.group;
+      const int i = token_of(p, r);
       const T* src = static_cast<const T*>(p.q) + b * p.q_sb + i * p.q_st + (h * p.group + r - i * p.group) * p.q_sh;
 #pragma unroll
       for (int ch = 0; ch < CH; ++ch) {
@@ -332,8 +378,9 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1) cache8_attention_ke
         col.scale = __shfl_sync(0xffffffffu, back, (2 * t + e) * 4);
         col.sum = __shfl_sync(0xffffffffu, sum, (2 * t + e) * 4) * 0x1p-17f;  // 128 times, at the keys' exponent
         col.lim = last_seen(p, start, end, rr);
-        col.where = q_first + rr / p.group + dropped;
-        col.bias = (h * p.group + min(rr, p.rows - 1) % p.group) * p.table_stride;
+        const int last = min(rr, p.rows - 1), tok = token_of(p, last);
+        col.where = q_first + tok + dropped;
+        col.bias = ((kBlock ? 0 : h * p.group) + last - tok * p.group) * p.table_stride;
         all_see = min(all_see, col.lim);
         if constexpr (kColSmem) s_col[nt * 8 + e] = col;  // (all lanes of a column write the same)
         else cols[nt][e] = col;
@@ -362,7 +409,10 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1) cache8_attention_ke
       }
     }
 
-    for (int tile = tile0; tile < tile1; tile += MT) {
+    float* s_sums = s_table + (p.table == nullptr ? 0 : (p.group * p.table_stride + 3) / 4 * 4);  // (with kBlock)
+    float* s_scores = s_sums + kWarps * p.rows * D;
+    constexpr int kStep = kBlock ? kWarps * MT : MT;
+    for (int tile = tile0; tile < tile1; tile += kStep) {
       // ---- S^T = K Q^T ----
       float s[MT][NT][4];
 #pragma unroll
@@ -398,7 +448,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1) cache8_attention_ke
       float k_scale[MT];
 #pragma unroll
       for (int mt = 0; mt < MT; ++mt) k_scale[mt] = ka[mt];
-      if (tile + MT < tile1) load_k(tile + MT);
+      if (tile + kStep < tile1) load_k(tile + kStep);
 
       // ---- scores of tokens g (k = 0, 1) and g + 8 (k = 2, 3), query rows 2t (k = 0, 2) and 2t + 1 ----
       bool some[MT];       // whether the mask shows a token of the tile
@@ -444,8 +494,8 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1) cache8_attention_ke
             for (int k = 0; k < 4; ++k)
               if (!shown[k >> 1] || s0 + g + 8 * (k >> 1) > column(nt, k & 1).lim) s[mt][nt][k] = -INFINITY;
         }
-        if (p.scores != nullptr && inside) {
-          float* to = p.scores + bh * p.rows * c.slots;
+        if ((kBlock ? c.weight != nullptr : p.scores != nullptr) && inside) {
+          float* to = kBlock ? s_scores : p.scores + bh * p.rows * c.slots;
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -539,9 +589,65 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1) cache8_attention_ke
               for (int q2 = 0; q2 < Q2; ++q2)
                 mma_f16(o[nt][2 * w + half], a0, a1, a2, a3, pf[q2][mt][nt][0], pf[q2][mt][nt][1]);
           }
-      if (tile + MT < tile1) load_v(tile + MT);
+      if (tile + kStep < tile1) load_v(tile + kStep);
     }
 
+    if constexpr (kBlock) {
+      // ---- the warps meet ----
+      __shared__ float2 s_stats[kWarps][8];
+      __shared__ float2 s_rows[8];
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        float sum = l[0][e];
+        sum += __shfl_xor_sync(0xffffffffu, sum, 4);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 8);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 16);
+        const int r = 2 * t + e;
+        if (r < p.rows) {
+          const float f = v_ref[0][e] * (1.f / 127.f);
+          float* dst = s_sums + ((threadIdx.x >> 5) * p.rows + r) * D + VB * g;
+#pragma unroll
+          for (int i = 0; i < MI; i += 2)
+            *reinterpret_cast<float4*>(dst + 2 * i) = make_float4(o[0][i][e] * f, o[0][i][2 + e] * f, o[0][i + 1][e] * f,
+                                                                  o[0][i + 1][2 + e] * f);
+          if (g == 0) s_stats[threadIdx.x >> 5][r] = make_float2(ref[0][e], sum);
+        }
+      }
+      __syncthreads();
+      for (int i = threadIdx.x; i < p.rows * (D / 4); i += kThreads) {
+        const int r = i / (D / 4), d = i % (D / 4) * 4;
+        float high = kNothing, sum = 0.f;
+        float x[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) high = fmaxf(high, s_stats[w][r].x);
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) {
+          const float2 st = s_stats[w][r];
+          if (st.y == 0.f) continue;  // (a warp that saw nothing may have sums of 0 * NaN)
+          const float f = exp2_approx(st.x - high);
+          const float4 v = *reinterpret_cast<const float4*>(s_sums + (w * p.rows + r) * D + d);
+          sum += st.y * f;
+          x[0] += v.x * f, x[1] += v.y * f, x[2] += v.z * f, x[3] += v.w * f;
+        }
+        const float inv = sum == 0.f ? 0.f : 1.f / sum;
+        T* dst = out_row<T>(p, b, h, r) + d;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) dst[k] = from_float<T>(x[k] * inv);
+        if (d == 0) s_rows[r] = make_float2(high, inv);
+      }
+      if (c.weight != nullptr) {
+        __syncthreads();
+        for (int s = threadIdx.x; s < end; s += kThreads) {
+          float sum = 0.f;
+          for (int r = 0; r < p.rows; ++r) {
+            const float x = s_scores[r * c.slots + s];
+            if (x > -INFINITY || x != x) sum += exp2_approx(x - s_rows[r].x) * s_rows[r].y;
+          }
+          float* weight = c.weight + slots0 + s;
+          *weight = (s >= start ? 0.f : *weight) + sum;
+        }
+      }
+    } else {
     // ---- the whole (row, head), or a piece of it ----
     const bool whole = tile0 == 0 && tile1 == tiles;
     // a warp has one piece that began before its own first tile at most, and one that goes on behind its last
@@ -577,6 +683,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1) cache8_attention_ke
         }
       }
     at = seg + tile1;
+    }
   }
 }
 
@@ -652,9 +759,10 @@ __global__ void __launch_bounds__(kJoinThreads) cache8_join_kernel(const __grid_
 }
 
 // weight[slot] += the probabilities that the query rows gave it
-__global__ void __launch_bounds__(kThreads) cache8_weight_kernel(const __grid_constant__ Cache8Attn p) {
+constexpr int kWeightThreads = 256;
+__global__ void __launch_bounds__(kWeightThreads) cache8_weight_kernel(const __grid_constant__ Cache8Attn p) {
   const int bh = blockIdx.x, b = bh / p.c.heads;
-  const int s = blockIdx.y * kThreads + threadIdx.x;
+  const int s = blockIdx.y * kWeightThreads + threadIdx.x;
   const int start = held_of(p.c, b), end = end_of(p, start);
   chain_wait();
   chain_release();
@@ -688,41 +796,71 @@ cudaError_t launch_behind(bool behind, void (*kernel)(Params...), dim3 grid, int
   return cudaLaunchKernelEx(&cfg, kernel, std::forward<Args>(args)...);
 }
 
+// Shared memory of a CTA that takes a whole (row, head), beside the query and the biases.
+constexpr int kMaxBlockBytes = 72 * 1024;
+size_t block_bytes(const Cache8& c, int rows) {
+  return 4ull * rows * (static_cast<size_t>(kPieceWarps) * c.dim + (c.weight != nullptr ? c.slots : 0));
+}
+// Whether a CTA takes a whole (row, head): caches of up to 1024 slots, and longer ones where there are several CTAs' worth
+// for every SM.
+bool whole_blocks(const Cache8& c, int rows) {
+  const long long bh = static_cast<long long>(c.batch) * c.heads;
+  return rows <= 8 && block_bytes(c, rows) <= kMaxBlockBytes && (c.slots <= 1024 || (c.slots <= 8192 && bh >= 6LL * num_sms()));
+}
+
 constexpr int tile_rows_of(int rows) { return rows <= 8 ? 8 : 32; }
 
-template <typename T, int D, int NT, int MT, bool kTwo>
-cudaError_t launch_tile(const Cache8Attn& p, bool behind, cudaStream_t stream) {
+template <typename T, int D, int NT, int MT, bool kTwo, bool kBlock, int kWarps = kPieceWarps>
+cudaError_t launch_tile(const Cache8Attn& p, const NewTokens<T>& fresh, bool behind, cudaStream_t stream) {
   constexpr size_t query = !query_in_smem<D, NT, kTwo>() ? 0 : static_cast<size_t>(kWarps) * (kTwo ? 2 : 1) * NT * (D / 64) * 4 * 32 * sizeof(uint2);
-  const size_t smem = query + (p.table == nullptr ? 0 : sizeof(float) * p.c.heads * p.group * p.table_stride);
+  const size_t table = p.table == nullptr ? 0 : sizeof(float) * (kBlock ? (p.group * p.table_stride + 3) / 4 * 4
+                                                                         : p.c.heads * p.group * p.table_stride);
+  const size_t smem = query + table + (kBlock ? block_bytes(p.c, p.rows) : 0);
   static bool set[64] = {false};
   int dev = 0;
   cudaGetDevice(&dev);
   if (!set[dev & 63]) {
-    cudaError_t e = cudaFuncSetAttribute(cache8_attention_kernel<T, D, NT, MT, kTwo>,
-                                         cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(query) + kMaxBiases * 4);
+    cudaError_t e = cudaFuncSetAttribute(cache8_attention_kernel<T, D, NT, MT, kTwo, kBlock, kWarps>,
+                                         cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                         static_cast<int>(query) + kMaxBiases * 4 + (kBlock ? kMaxBlockBytes : 0));
     if (e != cudaSuccess) return e;
     set[dev & 63] = true;
   }
-  const dim3 grid(p.warps / kWarps, (p.rows + NT * 8 - 1) / (NT * 8));
-  return launch_behind(behind, cache8_attention_kernel<T, D, NT, MT, kTwo>, grid, kThreads, smem, stream, p);
+  const dim3 grid = kBlock ? dim3(p.c.heads, p.c.batch) : dim3(p.warps / kWarps, (p.rows + NT * 8 - 1) / (NT * 8));
+  return launch_behind(behind, cache8_attention_kernel<T, D, NT, MT, kTwo, kBlock, kWarps>, grid, kWarps * 32, smem, stream, p, fresh);
 }
 
 template <typename T, bool kTwo>
-cudaError_t launch_all(const Cache8Attn& p, bool behind, cudaStream_t stream) {
+cudaError_t launch_blocks(const Cache8Attn& p, const T5xNewTokens* tokens, cudaStream_t stream) {
+  const NewTokens<T> fresh = make_tokens<T>(tokens);
+  // half the warps where there are CTAs for all SMs: what a warp does around its tiles is done half as often
+  const bool many = static_cast<long long>(p.c.batch) * p.c.heads >= 2LL * num_sms();
+  if (p.c.dim == 64)
+    return many ? launch_tile<T, 64, 1, 2, kTwo, true, 4>(p, fresh, false, stream)
+                : launch_tile<T, 64, 1, 2, kTwo, true, 8>(p, fresh, false, stream);
+  return many ? launch_tile<T, 128, 1, 1, kTwo, true, 4>(p, fresh, false, stream)
+              : launch_tile<T, 128, 1, 1, kTwo, true, 8>(p, fresh, false, stream);
+}
+
+template <typename T, bool kTwo>
+cudaError_t launch_pieces(const Cache8Attn& p, bool behind, cudaStream_t stream) {
   const int tile_rows = tile_rows_of(p.rows);
+  const NewTokens<T> none = {};
   cudaError_t e;
   if (p.c.dim == 64)
-    e = tile_rows == 8 ? launch_tile<T, 64, 1, 2, kTwo>(p, behind, stream) : launch_tile<T, 64, 4, 1, kTwo>(p, behind, stream);
+    e = tile_rows == 8 ? launch_tile<T, 64, 1, 2, kTwo, false>(p, none, behind, stream)
+                       : launch_tile<T, 64, 4, 1, kTwo, false>(p, none, behind, stream);
   else
-    e = tile_rows == 8 ? launch_tile<T, 128, 1, 1, kTwo>(p, behind, stream) : launch_tile<T, 128, 4, 1, kTwo>(p, behind, stream);
+    e = tile_rows == 8 ? launch_tile<T, 128, 1, 1, kTwo, false>(p, none, behind, stream)
+                       : launch_tile<T, 128, 4, 1, kTwo, false>(p, none, behind, stream);
   if (e != cudaSuccess) return e;
   const dim3 rows(static_cast<unsigned>(p.c.batch) * p.c.heads, p.rows);
   e = p.c.dim == 64 ? launch_behind(true, cache8_join_kernel<T, 64>, rows, kJoinThreads, 0, stream, p, tile_rows)
                     : launch_behind(true, cache8_join_kernel<T, 128>, rows, kJoinThreads, 0, stream, p, tile_rows);
   if (e != cudaSuccess || p.scores == nullptr) return e;
   return launch_behind(true, cache8_weight_kernel,
-                       dim3(static_cast<unsigned>(p.c.batch) * p.c.heads, (p.c.slots + kThreads - 1) / kThreads),
-                       kThreads, 0, stream, p);
+                       dim3(static_cast<unsigned>(p.c.batch) * p.c.heads, (p.c.slots + kWeightThreads - 1) / kWeightThreads),
+                       kWeightThreads, 0, stream, p);
 }
 
 // Rows `from` on of a cache.
@@ -740,18 +878,19 @@ Cache8 rows_of(Cache8 c, int from, int count) {
 }
 
 struct Plan {
-  int warps, least;
+  int warps = 0, least = 0;
   size_t part = 0, stats = 0, first = 0, scores = 0, final_stats = 0, total = 0;
 };
 Plan plan(Cache8 c, int rows) {
-  Plan w;
+  Plan w = {};
+  if (whole_blocks(c, rows)) return w;
   c.batch = std::min(c.batch, kMaxBatch);
   const int tile_rows = tile_rows_of(rows), row_tiles = (rows + tile_rows - 1) / tile_rows;
   // the warps that the SMs hold at a time, shared by the tiles of query rows; no piece of under 64 tokens
-  const long long room = static_cast<long long>(num_sms()) * kWarps * (tile_rows == 8 ? 2 : 1) / row_tiles;
+  const long long room = static_cast<long long>(num_sms()) * kPieceWarps * (tile_rows == 8 ? 2 : 1) / row_tiles;
   const long long most = static_cast<long long>(c.batch) * c.heads * (c.slots / 16 + kEntry) / (4 + kEntry) + 1;
   w.least = 4 + kEntry;
-  w.warps = static_cast<int>(std::max<long long>(1, std::min(room, most) / kWarps)) * kWarps;
+  w.warps = static_cast<int>(std::max<long long>(1, std::min(room, most) / kPieceWarps)) * kPieceWarps;
   const size_t bh = static_cast<size_t>(c.batch) * c.heads;
   auto take = [&](size_t bytes) {
     const size_t at = w.total;
@@ -821,6 +960,7 @@ T5X_API int t5x_cache8_attention(const T5xCache8* cache, const T5xCache8Query* q
   p.count = q->count;
   p.group = q->group;
   p.rows = q->count * q->group;
+  p.by_group = ((1ull << 32) + q->group - 1) / q->group;
   p.distances = q->table ? q->distances : 0;
   if (q->table) std::copy_n(q->buckets, q->distances, p.buckets);
   p.mask_len = q->mask_len;
@@ -828,6 +968,14 @@ T5X_API int t5x_cache8_attention(const T5xCache8* cache, const T5xCache8Query* q
   p.appended = n ? n->count : 0;
   p.scale = q->scale;
   const t5x::Plan w = t5x::plan(c, p.rows);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (t5x::whole_blocks(c, p.rows)) {
+    p.scores = nullptr;
+    const cudaError_t e = q->type == 0   ? t5x::launch_blocks<__nv_bfloat16, false>(p, n, st)
+                          : q->type == 1 ? t5x::launch_blocks<__half, false>(p, n, st)
+                                         : t5x::launch_blocks<float, true>(p, n, st);
+    return e == cudaSuccess ? 0 : t5x::set_error("cache8_attention launch: %s", cudaGetErrorString(e));
+  }
   if (!workspace || !t5x::aligned_to(16, {workspace}))
     return t5x::set_error("cache8_attention: a null or misaligned workspace");
   uint8_t* ws = static_cast<uint8_t*>(workspace);
@@ -838,7 +986,6 @@ T5X_API int t5x_cache8_attention(const T5xCache8* cache, const T5xCache8Query* q
   p.first = reinterpret_cast<long long*>(ws + w.first);
   p.scores = c.weight ? reinterpret_cast<float*>(ws + w.scores) : nullptr;
   p.final_stats = reinterpret_cast<float2*>(ws + w.final_stats);
-  cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (n)
     if (int e = t5x::cache8_append(c, n, st)) return e;
   const int size = q->type == 2 ? 4 : 2;
@@ -850,9 +997,9 @@ T5X_API int t5x_cache8_attention(const T5xCache8* cache, const T5xCache8Query* q
     part.mask = p.mask ? p.mask + from * p.mask_stride : nullptr;
     // (what follows the append alone may begin while it runs; the workspace of a launch is the next one's)
     const bool behind = n != nullptr && from == 0;
-    const cudaError_t e = q->type == 0   ? t5x::launch_all<__nv_bfloat16, false>(part, behind, st)
-                          : q->type == 1 ? t5x::launch_all<__half, false>(part, behind, st)
-                                         : t5x::launch_all<float, true>(part, behind, st);
+    const cudaError_t e = q->type == 0   ? t5x::launch_pieces<__nv_bfloat16, false>(part, behind, st)
+                          : q->type == 1 ? t5x::launch_pieces<__half, false>(part, behind, st)
+                                         : t5x::launch_pieces<float, true>(part, behind, st);
     if (e != cudaSuccess) return t5x::set_error("cache8_attention launch: %s", cudaGetErrorString(e));
   }
   return 0;
