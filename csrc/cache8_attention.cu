@@ -31,8 +31,9 @@
 // Two ways to deal out the work. Over short caches, and longer ones where there are many (row, head), a CTA takes one: it
 // appends the new tokens, its warps take tiles of 16 tokens in turn and meet in shared memory, and the scores that the
 // weights are made from never leave it: one launch. Over long ones (of all lengths) all tiles of all (row, head) laid end to
-// end are cut into one equal piece a warp; what a warp has of a (row, head) that it does not have whole goes to workspace,
-// and a second kernel joins the pieces.
+// end are cut into one equal piece a CTA; what it has of a (row, head) that it does not have whole goes to workspace, and a
+// second kernel joins the pieces. Many query rows go 32 at a time, a warp each, so that the warps of a CTA read the same
+// tiles, from L1.
 #include <algorithm>
 
 #include "cache8.cuh"
@@ -63,10 +64,11 @@ struct Cache8Attn {
   int appended;            // tokens of this call behind c.index
   float scale;
   unsigned long long by_group;  // 2^32 / group, rounded up: r / group for r below 2^16 by one multiplication
-  int warps;               // pieces that the tiles are cut into
+  int pieces;              // that the tiles are cut into
+  int row_warps;           // kRows: warps of a CTA that take different query rows of one piece (1, or all)
   int least;               // tiles of a piece at least
-  float* part;             // [row tile, warps, 2, rows of a tile, dim]
-  float2* stats;           // [row tile, warps, 2, rows of a tile]: reference, sum
+  float* part;             // [row tile, pieces, 2, rows of a tile, dim]
+  float2* stats;           // [row tile, pieces, 2, rows of a tile]: reference, sum
   long long* first;        // [batch + 1]: cost in front of a row, in tiles; then that of a piece
   float* scores;           // [batch * heads, rows, slots], times log2 e, where weights are added up; else null
   float2* final_stats;     // [batch * heads, rows]: reference, 1 / sum; with scores
@@ -150,68 +152,152 @@ __device__ __forceinline__ void count_tiles(const Cache8Attn& p, long long* s_fi
   __syncthreads();
 }
 
-// Where registers are short, the query's operand lies in shared memory.
-template <int D, int NT, bool kTwo>
-__host__ __device__ constexpr bool query_in_smem() {
-  return NT > 1 || D == 128;
-}
-// What a score column needs beside its reference and sums; in shared memory where there are many columns.
+// What a score column needs beside its reference and sums.
 struct Column {
   float scale, sum;
   int lim, where, bias;
 };
 
+// One call's query rows row0 .. row0 + 8 * NT - 1 of a (row, head), by one warp: its lanes' parts of the first product's second
+// operand to s_query[Q2][NT][CH * 4][32], its columns to s_cols[NT * 8].
+template <typename T, int D, int NT, bool kTwo>
+__device__ __forceinline__ void lay_query(const Cache8Attn& p, int b, int h, int row0, int start, int end, int first_bias,
+                                          uint2* s_query, Column* s_cols) {
+  constexpr int CH = D / 64, Q2 = kTwo ? 2 : 1, E = 16 / sizeof(T);
+  const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const int dropped = p.c.position != nullptr ? p.c.dropped[b] : 0;
+  const int q_first = static_cast<int>(static_cast<long long>(start) + p.appended - p.count);
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+    const int r = row0 + nt * 8 + g, i = token_of(p, min(r, p.rows - 1)), in_group = min(r, p.rows - 1) - i * p.group;
+    const T* src = static_cast<const T*>(p.q) + b * p.q_sb + i * p.q_st + (h * p.group + in_group) * p.q_sh + 16 * t;
+    float x[CH][16];
+    uint32_t most = 0;
+#pragma unroll
+    for (int ch = 0; ch < CH; ++ch) {
+      alignas(16) T part[16];
+      if (p.q_vec) {
+#pragma unroll
+        for (int k = 0; k < 16 / E; ++k)
+          *reinterpret_cast<uint4*>(part + k * E) = *reinterpret_cast<const uint4*>(src + 64 * ch + k * E);
+      } else {
+#pragma unroll
+        for (int k = 0; k < 16; ++k) part[k] = src[64 * ch + k];
+      }
+#pragma unroll
+      for (int k = 0; k < 16; ++k) {
+        x[ch][k] = r < p.rows ? to_float(part[k]) : 0.f;
+        most = max(most, abs_bits(x[ch][k]));
+      }
+    }
+    most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
+    most = max(most, __shfl_xor_sync(0xffffffffu, most, 2));
+    // 2^up brings the largest to [2^13, 2^14)
+    int up = most == 0 || most >= 0x7f800000u ? 0 : 13 - (static_cast<int>(most >> 23) - 127);
+    up = max(min(up, 126), -113);
+    const float by = __uint_as_float(static_cast<uint32_t>(up + 127) << 23);
+    float sum = 0.f;
+#pragma unroll
+    for (int ch = 0; ch < CH; ++ch)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        uint32_t f[Q2][2];
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          const float lo = x[ch][4 * j + k] * by, hi = x[ch][4 * j + 2 + k] * by;
+          const __half2 v = __floats2half2_rn(lo, hi);
+          f[0][k] = as_u32(v);
+          sum += __low2float(v) + __high2float(v);
+          if (kTwo) {
+            const __half2 rest = __floats2half2_rn(lo - __low2float(v), hi - __high2float(v));
+            f[Q2 - 1][k] = as_u32(rest);
+            sum += __low2float(rest) + __high2float(rest);
+          }
+        }
+#pragma unroll
+        for (int w = 0; w < Q2; ++w) s_query[((w * NT + nt) * CH * 4 + ch * 4 + j) * 32 + lane] = make_uint2(f[w][0], f[w][1]);
+      }
+    sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+    sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+    if (t == 0) {
+      Column col;
+      // 2^24 back from the keys' exponent; the scale of a key block is its largest value / 127; scores are times log2 e
+      col.scale = __uint_as_float(static_cast<uint32_t>(127 - up) << 23) * p.scale * (0x1p24f / 127.f * kLog2e);
+      col.sum = sum * 0x1p-17f;  // 128 times, at the keys' exponent
+      col.lim = last_seen(p, start, end, r);
+      col.where = q_first + i + dropped;
+      col.bias = first_bias + in_group * p.table_stride;
+      s_cols[nt * 8 + g] = col;
+    }
+  }
+}
+
+enum Deal {
+  kRowHead,  // a CTA takes a (row, head), and appends
+  kPieces,   // a CTA takes a piece of the tiles
+  kRows      // a warp takes a piece of the tiles, or warps of a CTA different query rows of one piece
+};
+
 // NT: tiles of 8 query rows; MT: tiles of 16 tokens a step; kTwo: operands as two fp16 numbers each.
-// kBlock: a CTA a (row, head), with the append.
-template <typename T, int D, int NT, int MT, bool kTwo, bool kBlock, int kWarps>
+template <typename T, int D, int NT, int MT, bool kTwo, Deal kDeal, int kWarps>
 __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 16 / kWarps : 1)
     cache8_attention_kernel(const __grid_constant__ Cache8Attn p, const __grid_constant__ NewTokens<T> fresh) {
-  static_assert(!kBlock || NT == 1, "a CTA takes 8 query rows");
+  constexpr bool kBlock = kDeal == kRowHead, kTeam = kDeal != kRows;  // kTeam: the warps of a CTA share tiles and query rows
+  static_assert(!kTeam || NT == 1, "a team takes 8 query rows");
   constexpr int kThreads = kWarps * 32;
   constexpr int CH = D / 64;       // 64-channel pieces
   constexpr int VB = D / 8;        // channels a lane has in the second product
   constexpr int MI = D / 16;       // row tiles of the second product
   constexpr int Q2 = kTwo ? 2 : 1;
-  constexpr bool kQuerySmem = query_in_smem<D, NT, kTwo>();
-  constexpr bool kColSmem = NT > 1;
-  // [kWarps][Q2][NT][CH * 4][32] with kQuerySmem; then the bias table, times log2 e (with kBlock that of the head's rows);
-  // then, with kBlock, sums of the warps [kWarps][rows][D] and scores [rows][slots]
-  extern __shared__ uint2 s_query[];
-  float* s_table = reinterpret_cast<float*>(s_query + (kQuerySmem ? kWarps * Q2 * NT * CH * 4 * 32 : 0));
+  constexpr bool kQueryRegs = NT == 1 && D == 64;  // the query's operand is kept in registers
+  constexpr int kQuery = Q2 * NT * CH * 4 * 32;
+  // the query's operand of the team or of each warp; the bias table, times log2 e (kRowHead: of the head's rows); the sums
+  // of a team's warps [kWarps][rows][D]; kRowHead: scores [rows][slots]
+  extern __shared__ uint2 s_dyn[];
+  float* s_table = reinterpret_cast<float*>(s_dyn + (kTeam ? 1 : kWarps) * kQuery);
   __shared__ long long s_first[kBlock ? 1 : kMaxBatch + 1];
   __shared__ uint8_t s_buckets[kMaxDistances];
-  __shared__ Column s_cols[kColSmem ? kWarps * NT * 8 : 1];
+  __shared__ Column s_cols[(kTeam ? 1 : kWarps) * NT * 8];
+  __shared__ float2 s_stats[kTeam ? kWarps : 1][8];
+  __shared__ float2 s_rows[8];
   const Cache8& c = p.c;
-  const int row0 = kBlock ? 0 : blockIdx.y * NT * 8;
-  const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  const int warp = blockIdx.x * kWarps + (threadIdx.x >> 5);
+  const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3, wid = threadIdx.x >> 5;
+  // the piece of the tiles, and the first query row
+  const int unit = kTeam ? blockIdx.x : p.row_warps > 1 ? blockIdx.x : blockIdx.x * kWarps + wid;
+  const int row_tile = kTeam ? 0 : p.row_warps > 1 ? blockIdx.y * kWarps + wid : blockIdx.y;
+  const int row0 = row_tile * NT * 8;
+  uint2* s_query = s_dyn + (kTeam ? 0 : wid * kQuery);
+  Column* s_col = s_cols + (kTeam ? 0 : wid * NT * 8);
 
+  const int biases = p.table == nullptr ? 0 : (kBlock ? 1 : c.heads) * p.group * p.table_stride;
   if (p.table != nullptr) {
     for (int i = threadIdx.x; i < p.distances; i += kThreads) s_buckets[i] = p.buckets[i];
-    const int count = (kBlock ? 1 : c.heads) * p.group * p.table_stride;
-    const float* from = p.table + (kBlock ? blockIdx.x * count : 0);
-    for (int i = threadIdx.x; i < count; i += kThreads) {
+    const float* from = p.table + (kBlock ? blockIdx.x * biases : 0);
+    for (int i = threadIdx.x; i < biases; i += kThreads) {
       const float x = from[i];  // (finite ones stay finite)
       s_table[i] = fabsf(x) < INFINITY ? fminf(fmaxf(x * kLog2e, -0x1p126f), 0x1p126f) : x;
     }
   }
-  long long at = 0, stop = 1, piece = 0;
+  float* s_sums = s_table + (biases + 3) / 4 * 4;
+  float* s_scores = s_sums + kWarps * p.rows * D;
+
+  long long at = 0, stop = 1;
   int b = 0;
   if constexpr (kBlock) {
     b = blockIdx.y;
   } else {
     count_tiles(p, s_first);
     const long long all = s_first[c.batch];
-    piece = max((all + p.warps - 1) / p.warps, static_cast<long long>(p.least));
+    const long long piece = max((all + p.pieces - 1) / p.pieces, static_cast<long long>(p.least));
     if (blockIdx.x == 0 && blockIdx.y == 0) {
       for (int i = threadIdx.x; i <= c.batch; i += kThreads) p.first[i] = s_first[i];
       if (threadIdx.x == 0) p.first[c.batch + 1] = piece;
     }
     chain_wait();  // new tokens are written by the kernel in front
     chain_release();
-    at = warp * piece;
+    at = unit * piece;
     stop = min(at + piece, all);
-    if (at >= stop) return;
+    if (at >= stop || row0 >= p.rows) return;
     for (int step = 1 << 11; step > 0; step >>= 1)  // the last row that begins at or before `at` and holds something
       if (b + step < c.batch && s_first[b + step] <= at) b += step;
   }
@@ -225,9 +311,8 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 16 / kWarps : 1)
     long long seg = 0;
     if constexpr (kBlock) {
       h = blockIdx.x;
-      tile0 = (threadIdx.x >> 5) * MT;
+      tile0 = 0;
       tile1 = tiles;
-      at = stop;
     } else {
       h = static_cast<int>((at - s_first[b]) / (tiles + kEntry));
       seg = s_first[b] + static_cast<long long>(h) * (tiles + kEntry) + kEntry;  // this (row, head)'s first tile
@@ -235,6 +320,8 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 16 / kWarps : 1)
       tile1 = static_cast<int>(min(stop - seg, static_cast<long long>(tiles)));
       if (tile1 <= 0) break;  // (no more than a part of what the beginning costs)
     }
+    constexpr int kStep = (kTeam ? kWarps : 1) * MT;
+    const int mine = tile0 + (kTeam ? wid * MT : 0);  // this warp's first tile
     const long long bh = static_cast<long long>(b) * c.heads + h;
 
     const long long slots0 = bh * c.slots;
@@ -243,21 +330,27 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 16 / kWarps : 1)
     const float* k_most = c.absmax[0] + bh * (c.slots >> c.block_log2);
     const float* v_most = c.absmax[1] + bh * (c.slots >> c.block_log2);
     const uint8_t* mask = p.mask == nullptr ? nullptr : p.mask + b * p.mask_stride;
+    const bool placed = p.table != nullptr && c.position != nullptr;
 
     uint4 kr[MT][2][CH];         // tokens g, g + 8
     uint32_t vr[MT][4][VB / 4];  // tokens 2t, 2t + 1, 2t + 8, 2t + 9
     float ka[MT], va[MT];
-    // (what the kernel in front may have written is read through L2)
+    int place[MT][2];
+    // What the kernel in front may have written is read through L2; several rows' warps share lines in L1, and wait for it to
+    // end by their launch.
+    auto get = [](const auto* ptr) { return kTeam ? __ldcg(ptr) : *ptr; };
     auto load_k = [&](int tile) {
 #pragma unroll
       for (int mt = 0; mt < MT; ++mt) {
         const int s0 = min(tile + mt, tile1 - 1) << 4;  // (a tile past the end is read again, and hidden)
         const int8_t* src = keys + static_cast<long long>(s0) * D;
-        ka[mt] = __ldcg(k_most + (s0 >> c.block_log2));
+        ka[mt] = get(k_most + (s0 >> c.block_log2));
 #pragma unroll
-        for (int e = 0; e < 2; ++e)
+        for (int e = 0; e < 2; ++e) {
+          if (placed) place[mt][e] = get(c.position + slots0 + s0 + g + 8 * e);
 #pragma unroll
-          for (int ch = 0; ch < CH; ++ch) kr[mt][e][ch] = __ldcg(reinterpret_cast<const uint4*>(src + 8 * e * D + 64 * ch));
+          for (int ch = 0; ch < CH; ++ch) kr[mt][e][ch] = get(reinterpret_cast<const uint4*>(src + 8 * e * D + 64 * ch));
+        }
       }
     };
     auto load_v = [&](int tile) {
@@ -265,133 +358,116 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 16 / kWarps : 1)
       for (int mt = 0; mt < MT; ++mt) {
         const int s0 = min(tile + mt, tile1 - 1) << 4;
         const int8_t* src = values + static_cast<long long>(s0) * D;
-        va[mt] = __ldcg(v_most + (s0 >> c.block_log2));
+        va[mt] = get(v_most + (s0 >> c.block_log2));
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const int8_t* from = src + ((e & 1) + 8 * (e >> 1)) * D;
           if (VB == 16) {
-            const uint4 u = __ldcg(reinterpret_cast<const uint4*>(from));
+            const uint4 u = get(reinterpret_cast<const uint4*>(from));
             vr[mt][e][0] = u.x, vr[mt][e][1] = u.y, vr[mt][e][VB / 4 - 2] = u.z, vr[mt][e][VB / 4 - 1] = u.w;
           } else {
-            const uint2 u = __ldcg(reinterpret_cast<const uint2*>(from));
+            const uint2 u = get(reinterpret_cast<const uint2*>(from));
             vr[mt][e][0] = u.x, vr[mt][e][1] = u.y;
           }
         }
       }
     };
-    if (!kColSmem && tile0 < tile1) {
-      load_k(tile0);
-      load_v(tile0);
-    }
+
+    const int first_bias = kBlock ? 0 : h * p.group * p.table_stride;
     if constexpr (kBlock) {
-      if (p.appended > 0) {
-        __shared__ uint32_t s_most[kWarps];
-        const int half = threadIdx.x / (kThreads / 2);  // keys by one half of the threads, values by the other
+      // Keys by one half of the threads, values by the other. Tokens of one block that the threads hold at a time are
+      // requested first, the first tiles behind them.
+      __shared__ uint32_t s_most[kWarps];
+      constexpr int kHalf = kThreads / 2, kLanes = D / 4;
+      const int half = threadIdx.x / kHalf, tid = threadIdx.x % kHalf, d = tid % kLanes * 4, own = tid / kLanes;
+      const int blk = start >> c.block_log2, touched = blk << c.block_log2;
+      const bool few = end > start && end - start <= kHalf / kLanes && end <= touched + (1 << c.block_log2);
+      float v[4] = {0.f, 0.f, 0.f, 0.f};
+      float before = 0.f;
+      float* most_at = c.absmax[half] + bh * (c.slots >> c.block_log2) + blk;
+      if (few) {
+        if (own < end - start) load_four(fresh.x[half] + b * fresh.sb[half] + h * fresh.sh[half] + own * fresh.st[half] + d, fresh.vec != 0, v);
+        if (start > touched) before = __ldcg(most_at);
+      }
+      if (mine < tile1) {
+        load_k(mine);
+        load_v(mine);
+      }
+      if (wid == 0) lay_query<T, D, NT, kTwo>(p, b, h, row0, start, end, first_bias, s_query, s_col);
+      if (few) {
+        uint32_t most = max(max(abs_bits(v[0]), abs_bits(v[1])), max(abs_bits(v[2]), abs_bits(v[3])));
+        most = __reduce_max_sync(0xffffffffu, most);
+        if (lane == 0) s_most[wid] = most;
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < kWarps / 2; ++w) most = max(most, s_most[half * (kWarps / 2) + w]);
+        most = max(most, abs_bits(before));
+        const float a = __uint_as_float(most);
+        int8_t* codes = c.codes[half] + slots0 * D + d;
+        if (most != abs_bits(before)) {
+          const Coder again(before, a);
+#pragma unroll 4
+          for (int s = touched + own; s < start; s += kHalf / kLanes) {
+            char4* to = reinterpret_cast<char4*>(codes + static_cast<long long>(s) * D);
+            const char4 u = *to;
+            *to = make_char4(again(u.x), again(u.y), again(u.z), again(u.w));
+          }
+        }
+        if (tid == 0) *most_at = a;
+        if (own < end - start) {
+          const Coder code(127.f, a);
+          *reinterpret_cast<char4*>(codes + static_cast<long long>(start + own) * D) = make_char4(code(v[0]), code(v[1]), code(v[2]), code(v[3]));
+          if (half == 0 && d == 0) {
+            if (c.weight != nullptr) c.weight[slots0 + start + own] = 0.f;
+            if (c.position != nullptr) c.position[slots0 + start + own] = start + own + c.dropped[b];
+          }
+        }
+      } else {
         for (int lo = start; lo < end;) {
           const int hi = min(end, ((lo >> c.block_log2) + 1) << c.block_log2);
-          append_block<T, D, kThreads / 2>(c, fresh, half, b, h, start, lo, hi, threadIdx.x % (kThreads / 2),
-                                        s_most + half * (kWarps / 2));
+          append_block<T, D, kHalf>(c, fresh, half, b, h, start, lo, hi, tid, s_most + half * (kWarps / 2));
           lo = hi;
         }
       }
       __syncthreads();
       // what was requested of a block that got tokens is requested again
-      if (p.appended > 0 && tile0 < tile1 && min(tile0 + MT, tile1) << 4 > start >> c.block_log2 << c.block_log2) {
-        load_k(tile0);
-        load_v(tile0);
+      if (p.appended > 0 && mine < tile1 && min(mine + MT, tile1) << 4 > touched) {
+        load_k(mine);
+        load_v(mine);
+      }
+      at = stop;
+    } else {
+      if (kTeam && mine < tile1) {
+        load_k(mine);
+        load_v(mine);
+      }
+      if (!kTeam || wid == 0) lay_query<T, D, NT, kTwo>(p, b, h, row0, start, end, first_bias, s_query, s_col);
+      if (kTeam) __syncthreads();
+      else __syncwarp();
+      if (!kTeam) {
+        load_k(mine);
+        load_v(mine);
       }
     }
 
-    // ---- this lane's part of the query rows as the first product's second operand ----
-    uint2 qf[kQuerySmem ? 1 : Q2][kQuerySmem ? 1 : NT][kQuerySmem ? 1 : CH * 4];
-    uint2* s_mine = s_query + static_cast<size_t>(threadIdx.x >> 5) * Q2 * NT * CH * 4 * 32 + lane;
-    Column cols[kColSmem ? 1 : NT][2];  // of the score columns 2t and 2t + 1
-    Column* s_col = s_cols + (kColSmem ? (threadIdx.x >> 5) * NT * 8 + 2 * t : 0);
+    // ---- the query: this lane's part of the operand, and what it needs for score columns 2t and 2t + 1 ----
+    uint2 qf[kQueryRegs ? Q2 : 1][kQueryRegs ? CH * 4 : 1];
+    if constexpr (kQueryRegs) {
+#pragma unroll
+      for (int w = 0; w < Q2; ++w)
+#pragma unroll
+        for (int j = 0; j < CH * 4; ++j) qf[w][j] = s_query[(w * CH * 4 + j) * 32 + lane];
+    }
+    Column cols[NT == 1 ? 2 : 1];
+    if constexpr (NT == 1) cols[0] = s_col[2 * t], cols[1] = s_col[2 * t + 1];
     auto column = [&](int nt, int e) -> const Column& {
-      if constexpr (kColSmem) return s_col[nt * 8 + e];
-      else return cols[nt][e];
+      if constexpr (NT == 1) return cols[e];
+      else return s_col[nt * 8 + 2 * t + e];
     };
     int all_see = end - 1;  // slots up to this one are seen by every row of the tile
-    __syncwarp();
-    const int dropped = c.position != nullptr ? c.dropped[b] : 0;
-    const int q_first = static_cast<int>(static_cast<long long>(start) + p.appended - p.count);
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-      const int r = row0 + nt * 8 + g;
-      float x[CH][16];
-      uint32_t most = 0;
-      const int i = token_of(p, r);
-      const T* src = static_cast<const T*>(p.q) + b * p.q_sb + i * p.q_st + (h * p.group + r - i * p.group) * p.q_sh;
-#pragma unroll
-      for (int ch = 0; ch < CH; ++ch) {
-        constexpr int E = 16 / sizeof(T);
-        alignas(16) T part[16];
-        if (r < p.rows && p.q_vec) {
-#pragma unroll
-          for (int k = 0; k < 16 / E; ++k)
-            *reinterpret_cast<uint4*>(part + k * E) = *reinterpret_cast<const uint4*>(src + 64 * ch + 16 * t + k * E);
-        }
-#pragma unroll
-        for (int k = 0; k < 16; ++k) {
-          x[ch][k] = r >= p.rows ? 0.f : p.q_vec ? to_float(part[k]) : to_float(src[64 * ch + 16 * t + k]);
-          most = max(most, abs_bits(x[ch][k]));
-        }
-      }
-      most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
-      most = max(most, __shfl_xor_sync(0xffffffffu, most, 2));
-      // 2^up brings the largest to [2^13, 2^14)
-      int up = most == 0 || most >= 0x7f800000u ? 0 : 13 - (static_cast<int>(most >> 23) - 127);
-      up = max(min(up, 126), -113);
-      const float by = __uint_as_float(static_cast<uint32_t>(up + 127) << 23);
-      // 2^24 back from the keys' exponent; the scale of a key block is its largest value / 127; scores are times log2 e
-      const float back = __uint_as_float(static_cast<uint32_t>(127 - up) << 23) * p.scale * (0x1p24f / 127.f * kLog2e);
-      float sum = 0.f;
-#pragma unroll
-      for (int ch = 0; ch < CH; ++ch)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          uint32_t f[Q2][2];
-#pragma unroll
-          for (int k = 0; k < 2; ++k) {
-            const float lo = x[ch][4 * j + k] * by, hi = x[ch][4 * j + 2 + k] * by;
-            const __half2 v = __floats2half2_rn(lo, hi);
-            f[0][k] = as_u32(v);
-            sum += __low2float(v) + __high2float(v);
-            if (kTwo) {
-              const __half2 rest = __floats2half2_rn(lo - __low2float(v), hi - __high2float(v));
-              f[Q2 - 1][k] = as_u32(rest);
-              sum += __low2float(rest) + __high2float(rest);
-            }
-          }
-#pragma unroll
-          for (int w = 0; w < Q2; ++w) {
-            if constexpr (kQuerySmem) s_mine[((w * NT + nt) * CH * 4 + ch * 4 + j) * 32] = make_uint2(f[w][0], f[w][1]);
-            else qf[w][nt][ch * 4 + j] = make_uint2(f[w][0], f[w][1]);
-          }
-        }
-      sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-      sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {  // lane 4 * row has that row's
-        const int rr = row0 + nt * 8 + 2 * t + e;
-        Column col;
-        col.scale = __shfl_sync(0xffffffffu, back, (2 * t + e) * 4);
-        col.sum = __shfl_sync(0xffffffffu, sum, (2 * t + e) * 4) * 0x1p-17f;  // 128 times, at the keys' exponent
-        col.lim = last_seen(p, start, end, rr);
-        const int last = min(rr, p.rows - 1), tok = token_of(p, last);
-        col.where = q_first + tok + dropped;
-        col.bias = ((kBlock ? 0 : h * p.group) + last - tok * p.group) * p.table_stride;
-        all_see = min(all_see, col.lim);
-        if constexpr (kColSmem) s_col[nt * 8 + e] = col;  // (all lanes of a column write the same)
-        else cols[nt][e] = col;
-      }
-    }
+    for (int nt = 0; nt < NT; ++nt) all_see = min(all_see, min(column(nt, 0).lim, column(nt, 1).lim));
     all_see = __reduce_min_sync(0xffffffffu, all_see);
-    __syncwarp();
-    if (kColSmem) {
-      load_k(tile0);
-      load_v(tile0);
-    }
 
     float o[NT][MI][4];
     float ref[NT][2], l[NT][2], v_ref[NT][2], v_inv[NT][2];
@@ -409,10 +485,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 16 / kWarps : 1)
       }
     }
 
-    float* s_sums = s_table + (p.table == nullptr ? 0 : (p.group * p.table_stride + 3) / 4 * 4);  // (with kBlock)
-    float* s_scores = s_sums + kWarps * p.rows * D;
-    constexpr int kStep = kBlock ? kWarps * MT : MT;
-    for (int tile = tile0; tile < tile1; tile += kStep) {
+    for (int tile = mine; tile < tile1; tile += kStep) {
       // ---- S^T = K Q^T ----
       float s[MT][NT][4];
 #pragma unroll
@@ -439,15 +512,21 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 16 / kWarps : 1)
 #pragma unroll
             for (int w = 0; w < Q2; ++w) {
               uint2 q;
-              if constexpr (kQuerySmem) q = s_mine[((w * NT + nt) * CH * 4 + ch * 4 + j) * 32];
-              else q = qf[w][nt][ch * 4 + j];
+              if constexpr (kQueryRegs) q = qf[w][ch * 4 + j];
+              else q = s_query[((w * NT + nt) * CH * 4 + ch * 4 + j) * 32 + lane];
 #pragma unroll
               for (int mt = 0; mt < MT; ++mt) mma_f16(s[mt][nt], a[mt][0], a[mt][1], a[mt][2], a[mt][3], q.x, q.y);
             }
         }
       float k_scale[MT];
+      int here[MT][2];  // positions of tokens g and g + 8
 #pragma unroll
-      for (int mt = 0; mt < MT; ++mt) k_scale[mt] = ka[mt];
+      for (int mt = 0; mt < MT; ++mt) {
+        k_scale[mt] = ka[mt];
+        const int s0 = (tile + mt) << 4;
+        here[mt][0] = placed ? place[mt][0] : s0 + g;
+        here[mt][1] = placed ? place[mt][1] : s0 + g + 8;
+      }
       if (tile + kStep < tile1) load_k(tile + kStep);
 
       // ---- scores of tokens g (k = 0, 1) and g + 8 (k = 2, 3), query rows 2t (k = 0, 2) and 2t + 1 ----
@@ -468,16 +547,11 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 16 / kWarps : 1)
           }
         }
         if (p.table != nullptr) {
-          int place[2] = {s0 + g, s0 + g + 8};
-          if (c.position != nullptr) {
-#pragma unroll
-            for (int e = 0; e < 2; ++e) place[e] = __ldcg(c.position + slots0 + min(s0 + g + 8 * e, c.slots - 1));
-          }
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
-              const int d = column(nt, k & 1).where - place[k >> 1];
+              const int d = column(nt, k & 1).where - here[mt][k >> 1];
               s[mt][nt][k] += s_table[column(nt, k & 1).bias + s_buckets[min(max(d, 0), p.distances - 1)]];
             }
         }
@@ -592,10 +666,12 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 16 / kWarps : 1)
       if (tile + kStep < tile1) load_v(tile + kStep);
     }
 
-    if constexpr (kBlock) {
+    // The whole (row, head), or a piece of it: a unit has one that began before its own first tile at most, and one that goes
+    // on behind its last.
+    const bool whole = tile0 == 0 && tile1 == tiles;
+    const long long slot = ((static_cast<long long>(row_tile) * p.pieces + unit) * 2 + (tile0 == 0 ? 1 : 0)) * NT * 8;
+    if constexpr (kTeam) {
       // ---- the warps meet ----
-      __shared__ float2 s_stats[kWarps][8];
-      __shared__ float2 s_rows[8];
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         float sum = l[0][e];
@@ -605,12 +681,12 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 16 / kWarps : 1)
         const int r = 2 * t + e;
         if (r < p.rows) {
           const float f = v_ref[0][e] * (1.f / 127.f);
-          float* dst = s_sums + ((threadIdx.x >> 5) * p.rows + r) * D + VB * g;
+          float* dst = s_sums + (wid * p.rows + r) * D + VB * g;
 #pragma unroll
           for (int i = 0; i < MI; i += 2)
             *reinterpret_cast<float4*>(dst + 2 * i) = make_float4(o[0][i][e] * f, o[0][i][2 + e] * f, o[0][i + 1][e] * f,
                                                                   o[0][i + 1][2 + e] * f);
-          if (g == 0) s_stats[threadIdx.x >> 5][r] = make_float2(ref[0][e], sum);
+          if (g == 0) s_stats[wid][r] = make_float2(ref[0][e], sum);
         }
       }
       __syncthreads();
@@ -630,60 +706,67 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 16 / kWarps : 1)
           x[0] += v.x * f, x[1] += v.y * f, x[2] += v.z * f, x[3] += v.w * f;
         }
         const float inv = sum == 0.f ? 0.f : 1.f / sum;
-        T* dst = out_row<T>(p, b, h, r) + d;
+        if (whole || kBlock) {
+          T* dst = out_row<T>(p, b, h, r) + d;
 #pragma unroll
-        for (int k = 0; k < 4; ++k) dst[k] = from_float<T>(x[k] * inv);
-        if (d == 0) s_rows[r] = make_float2(high, inv);
+          for (int k = 0; k < 4; ++k) dst[k] = from_float<T>(x[k] * inv);
+          if (d == 0) {
+            if (kBlock) s_rows[r] = make_float2(high, inv);
+            else if (p.scores != nullptr) p.final_stats[bh * p.rows + r] = make_float2(high, inv);
+          }
+        } else {
+          *reinterpret_cast<float4*>(p.part + (slot + r) * D + d) = make_float4(x[0], x[1], x[2], x[3]);
+          if (d == 0) p.stats[slot + r] = make_float2(high, sum);
+        }
       }
-      if (c.weight != nullptr) {
+      if (kBlock && c.weight != nullptr) {
         __syncthreads();
+#pragma unroll 4
         for (int s = threadIdx.x; s < end; s += kThreads) {
-          float sum = 0.f;
+          float* weight = c.weight + slots0 + s;
+          float sum = s >= start ? 0.f : *weight;
           for (int r = 0; r < p.rows; ++r) {
             const float x = s_scores[r * c.slots + s];
             if (x > -INFINITY || x != x) sum += exp2_approx(x - s_rows[r].x) * s_rows[r].y;
           }
-          float* weight = c.weight + slots0 + s;
-          *weight = (s >= start ? 0.f : *weight) + sum;
+          *weight = sum;
         }
       }
+      if (!kBlock) __syncthreads();  // the next piece's query and sums
     } else {
-    // ---- the whole (row, head), or a piece of it ----
-    const bool whole = tile0 == 0 && tile1 == tiles;
-    // a warp has one piece that began before its own first tile at most, and one that goes on behind its last
-    const long long slot = ((static_cast<long long>(blockIdx.y) * p.warps + warp) * 2 + (tile0 == 0 ? 1 : 0)) * NT * 8;
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
+      for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        float sum = l[nt][e];
-        sum += __shfl_xor_sync(0xffffffffu, sum, 4);
-        sum += __shfl_xor_sync(0xffffffffu, sum, 8);
-        sum += __shfl_xor_sync(0xffffffffu, sum, 16);
-        const int col = nt * 8 + 2 * t + e, r = row0 + col;
-        if (r >= p.rows) continue;
-        // (a row that nothing was seen of may have sums of 0 * NaN)
-        const float f = v_ref[nt][e] * (1.f / 127.f) * (whole ? 1.f / sum : 1.f);
-        float x[VB];
+        for (int e = 0; e < 2; ++e) {
+          float sum = l[nt][e];
+          sum += __shfl_xor_sync(0xffffffffu, sum, 4);
+          sum += __shfl_xor_sync(0xffffffffu, sum, 8);
+          sum += __shfl_xor_sync(0xffffffffu, sum, 16);
+          const int col = nt * 8 + 2 * t + e, r = row0 + col;
+          if (r >= p.rows) continue;
+          // (a row that nothing was seen of may have sums of 0 * NaN)
+          const float f = v_ref[nt][e] * (1.f / 127.f) * (whole ? 1.f / sum : 1.f);
+          float x[VB];
 #pragma unroll
-        for (int i = 0; i < MI; ++i) {
-          x[2 * i] = sum == 0.f ? 0.f : o[nt][i][e] * f;
-          x[2 * i + 1] = sum == 0.f ? 0.f : o[nt][i][2 + e] * f;
+          for (int i = 0; i < MI; ++i) {
+            x[2 * i] = sum == 0.f ? 0.f : o[nt][i][e] * f;
+            x[2 * i + 1] = sum == 0.f ? 0.f : o[nt][i][2 + e] * f;
+          }
+          if (whole) {
+            T* dst = out_row<T>(p, b, h, r) + VB * g;
+#pragma unroll
+            for (int i = 0; i < VB; ++i) dst[i] = from_float<T>(x[i]);
+            if (g == 0 && p.scores != nullptr) p.final_stats[bh * p.rows + r] = make_float2(ref[nt][e], sum == 0.f ? 0.f : 1.f / sum);
+          } else {
+            float4* dst = reinterpret_cast<float4*>(p.part + (slot + col) * D + VB * g);
+#pragma unroll
+            for (int i = 0; i < VB / 4; ++i) dst[i] = make_float4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]);
+            if (g == 0) p.stats[slot + col] = make_float2(ref[nt][e], sum);
+          }
         }
-        if (whole) {
-          T* dst = out_row<T>(p, b, h, r) + VB * g;
-#pragma unroll
-          for (int i = 0; i < VB; ++i) dst[i] = from_float<T>(x[i]);
-          if (g == 0 && p.scores != nullptr) p.final_stats[bh * p.rows + r] = make_float2(ref[nt][e], sum == 0.f ? 0.f : 1.f / sum);
-        } else {
-          float4* dst = reinterpret_cast<float4*>(p.part + (slot + col) * D + VB * g);
-#pragma unroll
-          for (int i = 0; i < VB / 4; ++i) dst[i] = make_float4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]);
-          if (g == 0) p.stats[slot + col] = make_float2(ref[nt][e], sum);
-        }
-      }
-    at = seg + tile1;
+      __syncwarp();  // the next piece's query
     }
+    if constexpr (!kBlock) at = seg + tile1;
   }
 }
 
@@ -703,9 +786,9 @@ __global__ void __launch_bounds__(kJoinThreads) cache8_join_kernel(const __grid_
   const long long cost = (__ldcg(p.first + b + 1) - from) / p.c.heads;  // tiles + kEntry, or 0
   const long long seg = from + h * cost + kEntry;  // its first tile
   const int w0 = static_cast<int>(seg / piece), w1 = cost == 0 ? w0 - 1 : static_cast<int>((seg + cost - kEntry - 1) / piece);
-  if (w0 == w1) return;  // one warp had it whole
-  // the first piece is its warp's second, the others are their warps' first ones
-  const long long base = (static_cast<long long>(r / tile_rows) * p.warps) * 2 * tile_rows + r % tile_rows;
+  if (w0 == w1) return;  // one unit had it whole
+  // the first piece is its unit's second, the others are their units' first ones
+  const long long base = (static_cast<long long>(r / tile_rows) * p.pieces) * 2 * tile_rows + r % tile_rows;
   auto slot = [&](int w) { return base + (w * 2LL + (w == w0 ? 1 : 0)) * tile_rows; };
   float high = kNothing, sum = 0.f;
   float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -796,50 +879,55 @@ cudaError_t launch_behind(bool behind, void (*kernel)(Params...), dim3 grid, int
   return cudaLaunchKernelEx(&cfg, kernel, std::forward<Args>(args)...);
 }
 
-// Shared memory of a CTA that takes a whole (row, head), beside the query and the biases.
-constexpr int kMaxBlockBytes = 72 * 1024;
-size_t block_bytes(const Cache8& c, int rows) {
-  return 4ull * rows * (static_cast<size_t>(kPieceWarps) * c.dim + (c.weight != nullptr ? c.slots : 0));
+// Shared memory of a team, beside the query and the biases.
+constexpr int kMaxTeamBytes = 72 * 1024;
+constexpr int kRowWarps = 8;
+size_t team_bytes(const Cache8& c, int rows, bool scores) {
+  return 4ull * rows * (8ull * c.dim + (scores && c.weight != nullptr ? c.slots : 0));
 }
 // Whether a CTA takes a whole (row, head): caches of up to 1024 slots, and longer ones where there are several CTAs' worth
 // for every SM.
-bool whole_blocks(const Cache8& c, int rows) {
+bool by_row_head(const Cache8& c, int rows) {
   const long long bh = static_cast<long long>(c.batch) * c.heads;
-  return rows <= 8 && block_bytes(c, rows) <= kMaxBlockBytes && (c.slots <= 1024 || (c.slots <= 8192 && bh >= 6LL * num_sms()));
+  return rows <= 8 && team_bytes(c, rows, true) <= kMaxTeamBytes && (c.slots <= 1024 || (c.slots <= 8192 && bh >= 6LL * num_sms()));
 }
 
 constexpr int tile_rows_of(int rows) { return rows <= 8 ? 8 : 32; }
 
-template <typename T, int D, int NT, int MT, bool kTwo, bool kBlock, int kWarps = kPieceWarps>
+template <typename T, int D, int NT, int MT, bool kTwo, Deal kDeal, int kWarps>
 cudaError_t launch_tile(const Cache8Attn& p, const NewTokens<T>& fresh, bool behind, cudaStream_t stream) {
-  constexpr size_t query = !query_in_smem<D, NT, kTwo>() ? 0 : static_cast<size_t>(kWarps) * (kTwo ? 2 : 1) * NT * (D / 64) * 4 * 32 * sizeof(uint2);
-  const size_t table = p.table == nullptr ? 0 : sizeof(float) * (kBlock ? (p.group * p.table_stride + 3) / 4 * 4
-                                                                         : p.c.heads * p.group * p.table_stride);
-  const size_t smem = query + table + (kBlock ? block_bytes(p.c, p.rows) : 0);
+  constexpr bool kBlock = kDeal == kRowHead, kTeam = kDeal != kRows;
+  constexpr size_t query = sizeof(uint2) * (kTeam ? 1 : kWarps) * (kTwo ? 2 : 1) * NT * (D / 64) * 4 * 32;
+  const size_t table = p.table == nullptr ? 0 : static_cast<size_t>((kBlock ? 1 : p.c.heads) * p.group * p.table_stride + 3) / 4 * 16;
+  const size_t smem = query + table + (kTeam ? team_bytes(p.c, p.rows, kBlock) : 0);
   static bool set[64] = {false};
   int dev = 0;
   cudaGetDevice(&dev);
   if (!set[dev & 63]) {
-    cudaError_t e = cudaFuncSetAttribute(cache8_attention_kernel<T, D, NT, MT, kTwo, kBlock, kWarps>,
+    cudaError_t e = cudaFuncSetAttribute(cache8_attention_kernel<T, D, NT, MT, kTwo, kDeal, kWarps>,
                                          cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                         static_cast<int>(query) + kMaxBiases * 4 + (kBlock ? kMaxBlockBytes : 0));
+                                         static_cast<int>(query) + kMaxBiases * 4 + (kTeam ? kMaxTeamBytes : 0));
     if (e != cudaSuccess) return e;
     set[dev & 63] = true;
   }
-  const dim3 grid = kBlock ? dim3(p.c.heads, p.c.batch) : dim3(p.warps / kWarps, (p.rows + NT * 8 - 1) / (NT * 8));
-  return launch_behind(behind, cache8_attention_kernel<T, D, NT, MT, kTwo, kBlock, kWarps>, grid, kWarps * 32, smem, stream, p, fresh);
+  const int row_tiles = (p.rows + NT * 8 - 1) / (NT * 8);
+  const dim3 grid = kBlock            ? dim3(p.c.heads, p.c.batch)
+                    : kTeam           ? dim3(p.pieces)
+                    : p.row_warps > 1 ? dim3(p.pieces, (row_tiles + kWarps - 1) / kWarps)
+                                      : dim3(p.pieces / kWarps, row_tiles);
+  return launch_behind(behind, cache8_attention_kernel<T, D, NT, MT, kTwo, kDeal, kWarps>, grid, kWarps * 32, smem, stream, p, fresh);
 }
 
 template <typename T, bool kTwo>
-cudaError_t launch_blocks(const Cache8Attn& p, const T5xNewTokens* tokens, cudaStream_t stream) {
+cudaError_t launch_row_heads(const Cache8Attn& p, const T5xNewTokens* tokens, cudaStream_t stream) {
   const NewTokens<T> fresh = make_tokens<T>(tokens);
-  // half the warps where there are CTAs for all SMs: what a warp does around its tiles is done half as often
+  // half the warps where there are CTAs for all SMs: what a CTA does around its tiles overlaps more of the others' tiles
   const bool many = static_cast<long long>(p.c.batch) * p.c.heads >= 2LL * num_sms();
   if (p.c.dim == 64)
-    return many ? launch_tile<T, 64, 1, 2, kTwo, true, 4>(p, fresh, false, stream)
-                : launch_tile<T, 64, 1, 2, kTwo, true, 8>(p, fresh, false, stream);
-  return many ? launch_tile<T, 128, 1, 1, kTwo, true, 4>(p, fresh, false, stream)
-              : launch_tile<T, 128, 1, 1, kTwo, true, 8>(p, fresh, false, stream);
+    return many ? launch_tile<T, 64, 1, 2, kTwo, kRowHead, 4>(p, fresh, false, stream)
+                : launch_tile<T, 64, 1, 2, kTwo, kRowHead, 8>(p, fresh, false, stream);
+  return many ? launch_tile<T, 128, 1, 1, kTwo, kRowHead, 4>(p, fresh, false, stream)
+              : launch_tile<T, 128, 1, 1, kTwo, kRowHead, 8>(p, fresh, false, stream);
 }
 
 template <typename T, bool kTwo>
@@ -848,11 +936,11 @@ cudaError_t launch_pieces(const Cache8Attn& p, bool behind, cudaStream_t stream)
   const NewTokens<T> none = {};
   cudaError_t e;
   if (p.c.dim == 64)
-    e = tile_rows == 8 ? launch_tile<T, 64, 1, 2, kTwo, false>(p, none, behind, stream)
-                       : launch_tile<T, 64, 4, 1, kTwo, false>(p, none, behind, stream);
+    e = tile_rows == 8 ? launch_tile<T, 64, 1, 2, kTwo, kPieces, 8>(p, none, behind, stream)
+                       : launch_tile<T, 64, 4, 1, kTwo, kRows, kRowWarps>(p, none, false, stream);
   else
-    e = tile_rows == 8 ? launch_tile<T, 128, 1, 1, kTwo, false>(p, none, behind, stream)
-                       : launch_tile<T, 128, 4, 1, kTwo, false>(p, none, behind, stream);
+    e = tile_rows == 8 ? launch_tile<T, 128, 1, 1, kTwo, kPieces, 8>(p, none, behind, stream)
+                       : launch_tile<T, 128, 4, 1, kTwo, kRows, kRowWarps>(p, none, false, stream);
   if (e != cudaSuccess) return e;
   const dim3 rows(static_cast<unsigned>(p.c.batch) * p.c.heads, p.rows);
   e = p.c.dim == 64 ? launch_behind(true, cache8_join_kernel<T, 64>, rows, kJoinThreads, 0, stream, p, tile_rows)
@@ -878,26 +966,32 @@ Cache8 rows_of(Cache8 c, int from, int count) {
 }
 
 struct Plan {
-  int warps = 0, least = 0;
+  int pieces = 0, least = 0, row_warps = 1;
   size_t part = 0, stats = 0, first = 0, scores = 0, final_stats = 0, total = 0;
 };
 Plan plan(Cache8 c, int rows) {
   Plan w = {};
-  if (whole_blocks(c, rows)) return w;
+  if (by_row_head(c, rows)) return w;
   c.batch = std::min(c.batch, kMaxBatch);
   const int tile_rows = tile_rows_of(rows), row_tiles = (rows + tile_rows - 1) / tile_rows;
-  // the warps that the SMs hold at a time, shared by the tiles of query rows; no piece of under 64 tokens
-  const long long room = static_cast<long long>(num_sms()) * kPieceWarps * (tile_rows == 8 ? 2 : 1) / row_tiles;
-  const long long most = static_cast<long long>(c.batch) * c.heads * (c.slots / 16 + kEntry) / (4 + kEntry) + 1;
-  w.least = 4 + kEntry;
-  w.warps = static_cast<int>(std::max<long long>(1, std::min(room, most) / kPieceWarps)) * kPieceWarps;
+  // the CTAs, or warps, that the SMs hold at a time, shared by the tiles of query rows; no piece of under 64 tokens a warp
+  const bool team = tile_rows == 8;
+  w.row_warps = !team && row_tiles >= 4 ? kRowWarps : 1;
+  const int unit_warps = team ? 8 : 1;
+  w.least = 4 * unit_warps + kEntry;
+  const long long room = team              ? 2LL * num_sms()
+                         : w.row_warps > 1 ? num_sms() / ((row_tiles + kRowWarps - 1) / kRowWarps)
+                                           : static_cast<long long>(num_sms()) * kRowWarps / row_tiles;
+  const long long most = static_cast<long long>(c.batch) * c.heads * (c.slots / 16 + kEntry) / w.least + 1;
+  w.pieces = static_cast<int>(std::max<long long>(1, std::min(room, most)));
+  if (!team && w.row_warps == 1) w.pieces = (w.pieces + kRowWarps - 1) / kRowWarps * kRowWarps;
   const size_t bh = static_cast<size_t>(c.batch) * c.heads;
   auto take = [&](size_t bytes) {
     const size_t at = w.total;
     w.total += (bytes + 15) / 16 * 16;
     return at;
   };
-  const size_t parts = static_cast<size_t>(row_tiles) * w.warps * 2 * tile_rows;
+  const size_t parts = static_cast<size_t>(row_tiles) * w.pieces * 2 * tile_rows;
   w.part = take(parts * c.dim * 4);
   w.stats = take(parts * 8);
   w.first = take((static_cast<size_t>(c.batch) + 2) * 8);
@@ -969,17 +1063,18 @@ T5X_API int t5x_cache8_attention(const T5xCache8* cache, const T5xCache8Query* q
   p.scale = q->scale;
   const t5x::Plan w = t5x::plan(c, p.rows);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (t5x::whole_blocks(c, p.rows)) {
+  if (t5x::by_row_head(c, p.rows)) {
     p.scores = nullptr;
-    const cudaError_t e = q->type == 0   ? t5x::launch_blocks<__nv_bfloat16, false>(p, n, st)
-                          : q->type == 1 ? t5x::launch_blocks<__half, false>(p, n, st)
-                                         : t5x::launch_blocks<float, true>(p, n, st);
+    const cudaError_t e = q->type == 0   ? t5x::launch_row_heads<__nv_bfloat16, false>(p, n, st)
+                          : q->type == 1 ? t5x::launch_row_heads<__half, false>(p, n, st)
+                                         : t5x::launch_row_heads<float, true>(p, n, st);
     return e == cudaSuccess ? 0 : t5x::set_error("cache8_attention launch: %s", cudaGetErrorString(e));
   }
   if (!workspace || !t5x::aligned_to(16, {workspace}))
     return t5x::set_error("cache8_attention: a null or misaligned workspace");
   uint8_t* ws = static_cast<uint8_t*>(workspace);
-  p.warps = w.warps;
+  p.pieces = w.pieces;
+  p.row_warps = w.row_warps;
   p.least = w.least;
   p.part = reinterpret_cast<float*>(ws + w.part);
   p.stats = reinterpret_cast<float2*>(ws + w.stats);

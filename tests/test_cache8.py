@@ -224,6 +224,19 @@ def test_token_by_token_is_a_repeat_of_the_same_blocks():
   assert (whole["cached_key"].int() - single["cached_key"].int()).abs().max() <= 8
 
 
+def check_zeros_into_a_used_block(device="cpu"):
+  """A block that begins anew does not keep the scale that its slots had before."""
+  cache = make(2, 1, 32, 64, 16, [16, 0], device=device)
+  zeros = torch.zeros(2, 1, 1, 64, device=device)
+  out = cache8.attention(zeros, cache, zeros, zeros)
+  assert cache["key_absmax"][0, 0, 1] == 0 and cache["value_absmax"][1, 0, 0] == 0 and (cache["cached_key"][0, 0, 16] == 0).all()
+  assert (out[1] == 0).all() and not out.isnan().any()
+
+
+def test_zeros_into_a_used_block():
+  check_zeros_into_a_used_block()
+
+
 @pytest.mark.parametrize("bad", [math.inf, -math.inf, math.nan])
 def test_values_that_are_not_finite(bad):
   c = dict(b=1, h=1, group=1, dim=64, slots=64, block=16, starts=[20], count=1)

@@ -52,6 +52,10 @@ def test_append(dtype, dim, block, lengths):
     assert torch.equal(cache["cached_" + n].cpu(), codes) and torch.equal(cache[n + "_absmax"].cpu(), most)
 
 
+def test_zeros_into_a_used_block():
+  plain.check_zeros_into_a_used_block("cuda")
+
+
 def test_codes_at_every_border():
   """Values whose quotient lies on a border between two codes, or next to it, in 32 bits."""
   most = torch.tensor([1.0, 127.0, 2.5390625, 0.7071068286895752, 3.0e-39, 2.0e38])
