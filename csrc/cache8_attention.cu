@@ -35,6 +35,7 @@
 // second kernel joins the pieces. Many query rows go 32 at a time, a warp each, so that the warps of a CTA read the same
 // tiles, from L1.
 #include <algorithm>
+#include <type_traits>
 
 #include "cache8.cuh"
 
@@ -160,7 +161,7 @@ struct Column {
 
 // One call's query rows row0 .. row0 + 8 * NT - 1 of a (row, head), by one warp: its lanes' parts of the first product's second
 // operand to s_query[Q2][NT][CH * 4][32], its columns to s_cols[NT * 8].
-template <typename T, int D, int NT, bool kTwo>
+template <typename T, int D, int NT, bool kTwo, bool kFold>
 __device__ __forceinline__ void lay_query(const Cache8Attn& p, int b, int h, int row0, int start, int end, int first_bias,
                                           uint2* s_query, Column* s_cols) {
   constexpr int CH = D / 64, Q2 = kTwo ? 2 : 1, E = 16 / sizeof(T);
@@ -169,7 +170,7 @@ __device__ __forceinline__ void lay_query(const Cache8Attn& p, int b, int h, int
   const int q_first = static_cast<int>(static_cast<long long>(start) + p.appended - p.count);
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
-    const int r = row0 + nt * 8 + g, i = token_of(p, min(r, p.rows - 1)), in_group = min(r, p.rows - 1) - i * p.group;
+    const int r = kFold ? g & 3 : row0 + nt * 8 + g, i = token_of(p, min(r, p.rows - 1)), in_group = min(r, p.rows - 1) - i * p.group;
     const T* src = static_cast<const T*>(p.q) + b * p.q_sb + i * p.q_st + (h * p.group + in_group) * p.q_sh + 16 * t;
     float x[CH][16];
     uint32_t most = 0;
@@ -224,7 +225,7 @@ __device__ __forceinline__ void lay_query(const Cache8Attn& p, int b, int h, int
       // 2^24 back from the keys' exponent; the scale of a key block is its largest value / 127; scores are times log2 e
       col.scale = __uint_as_float(static_cast<uint32_t>(127 - up) << 23) * p.scale * (0x1p24f / 127.f * kLog2e);
       col.sum = sum * 0x1p-17f;  // 128 times, at the keys' exponent
-      col.lim = last_seen(p, start, end, r);
+      col.lim = r < p.rows ? last_seen(p, start, end, r) : 0x7fffffff;  // (a column without a row hinders nobody)
       col.where = q_first + i + dropped;
       col.bias = first_bias + in_group * p.table_stride;
       s_cols[nt * 8 + g] = col;
@@ -239,11 +240,16 @@ enum Deal {
 };
 
 // NT: tiles of 8 query rows; MT: tiles of 16 tokens a step; kTwo: operands as two fp16 numbers each.
-template <typename T, int D, int NT, int MT, bool kTwo, Deal kDeal, int kWarps>
+// kFold: up to four query rows, twice in the 8 columns: of a step's two tiles the first counts in columns 0 to 3 and the second
+// in 4 to 7, so that what is done for scores and probabilities is done once for both.
+template <typename T, int D, int NT, int MT, bool kTwo, Deal kDeal, int kWarps, bool kFold>
 __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 16 / kWarps : 1)
     cache8_attention_kernel(const __grid_constant__ Cache8Attn p, const __grid_constant__ NewTokens<T> fresh) {
   constexpr bool kBlock = kDeal == kRowHead, kTeam = kDeal != kRows;  // kTeam: the warps of a CTA share tiles and query rows
   static_assert(!kTeam || NT == 1, "a team takes 8 query rows");
+  static_assert(!kFold || (kTeam && MT == 2), "two tiles fold");
+  constexpr int MS = kFold ? 1 : MT;           // tiles of scores that a lane has
+  constexpr int kParts = kFold ? 2 : 1;        // columns of a query row
   constexpr int kThreads = kWarps * 32;
   constexpr int CH = D / 64;       // 64-channel pieces
   constexpr int VB = D / 8;        // channels a lane has in the second product
@@ -258,7 +264,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 16 / kWarps : 1)
   __shared__ long long s_first[kBlock ? 1 : kMaxBatch + 1];
   __shared__ uint8_t s_buckets[kMaxDistances];
   __shared__ Column s_cols[(kTeam ? 1 : kWarps) * NT * 8];
-  __shared__ float2 s_stats[kTeam ? kWarps : 1][8];
+  __shared__ float2 s_stats[kTeam ? kWarps * kParts : 1][8];
   __shared__ float2 s_rows[8];
   const Cache8& c = p.c;
   const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3, wid = threadIdx.x >> 5;
@@ -279,7 +285,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 16 / kWarps : 1)
     }
   }
   float* s_sums = s_table + (biases + 3) / 4 * 4;
-  float* s_scores = s_sums + kWarps * p.rows * D;
+  float* s_scores = s_sums + kWarps * kParts * p.rows * D;
 
   long long at = 0, stop = 1;
   int b = 0;
@@ -334,31 +340,35 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 16 / kWarps : 1)
 
     uint4 kr[MT][2][CH];         // tokens g, g + 8
     uint32_t vr[MT][4][VB / 4];  // tokens 2t, 2t + 1, 2t + 8, 2t + 9
-    float ka[MT], va[MT];
-    int place[MT][2];
+    float ka[MS], va[MS];
+    int place[MS][2];
+    const int fold = kFold ? t >> 1 : 0;  // which of the two tiles this lane's columns count
     // What the kernel in front may have written is read through L2; several rows' warps share lines in L1, and wait for it to
     // end by their launch.
     auto get = [](const auto* ptr) { return kTeam ? __ldcg(ptr) : *ptr; };
+    // (a tile past the end is read again, and hidden)
     auto load_k = [&](int tile) {
 #pragma unroll
-      for (int mt = 0; mt < MT; ++mt) {
-        const int s0 = min(tile + mt, tile1 - 1) << 4;  // (a tile past the end is read again, and hidden)
-        const int8_t* src = keys + static_cast<long long>(s0) * D;
-        ka[mt] = get(k_most + (s0 >> c.block_log2));
+      for (int ms = 0; ms < MS; ++ms) {
+        const int s0 = min(tile + ms + fold, tile1 - 1) << 4;
+        ka[ms] = get(k_most + (s0 >> c.block_log2));
+        if (placed) place[ms][0] = get(c.position + slots0 + s0 + g), place[ms][1] = get(c.position + slots0 + s0 + g + 8);
+      }
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          if (placed) place[mt][e] = get(c.position + slots0 + s0 + g + 8 * e);
+      for (int mt = 0; mt < MT; ++mt) {
+        const int8_t* src = keys + static_cast<long long>(min(tile + mt, tile1 - 1)) * (16 * D);
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
 #pragma unroll
           for (int ch = 0; ch < CH; ++ch) kr[mt][e][ch] = get(reinterpret_cast<const uint4*>(src + 8 * e * D + 64 * ch));
-        }
       }
     };
     auto load_v = [&](int tile) {
 #pragma unroll
+      for (int ms = 0; ms < MS; ++ms) va[ms] = get(v_most + (min(tile + ms + fold, tile1 - 1) << 4 >> c.block_log2));
+#pragma unroll
       for (int mt = 0; mt < MT; ++mt) {
-        const int s0 = min(tile + mt, tile1 - 1) << 4;
-        const int8_t* src = values + static_cast<long long>(s0) * D;
-        va[mt] = get(v_most + (s0 >> c.block_log2));
+        const int8_t* src = values + static_cast<long long>(min(tile + mt, tile1 - 1)) * (16 * D);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const int8_t* from = src + ((e & 1) + 8 * (e >> 1)) * D;
@@ -393,7 +403,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 16 / kWarps : 1)
         load_k(mine);
         load_v(mine);
       }
-      if (wid == 0) lay_query<T, D, NT, kTwo>(p, b, h, row0, start, end, first_bias, s_query, s_col);
+      if (wid == 0) lay_query<T, D, NT, kTwo, kFold>(p, b, h, row0, start, end, first_bias, s_query, s_col);
       if (few) {
         uint32_t most = max(max(abs_bits(v[0]), abs_bits(v[1])), max(abs_bits(v[2]), abs_bits(v[3])));
         most = __reduce_max_sync(0xffffffffu, most);
@@ -441,7 +451,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 16 / kWarps : 1)
         load_k(mine);
         load_v(mine);
       }
-      if (!kTeam || wid == 0) lay_query<T, D, NT, kTwo>(p, b, h, row0, start, end, first_bias, s_query, s_col);
+      if (!kTeam || wid == 0) lay_query<T, D, NT, kTwo, kFold>(p, b, h, row0, start, end, first_bias, s_query, s_col);
       if (kTeam) __syncthreads();
       else __syncwarp();
       if (!kTeam) {
@@ -470,7 +480,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 16 / kWarps : 1)
     all_see = __reduce_min_sync(0xffffffffu, all_see);
 
     float o[NT][MI][4];
-    float ref[NT][2], l[NT][2], v_ref[NT][2], v_inv[NT][2];
+    float ref[NT][2], l[NT][2], v_lim[NT][2], v_inv[NT][2];  // v_lim: four times the scale that a value block's is relative to
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
@@ -481,19 +491,19 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 16 / kWarps : 1)
       for (int e = 0; e < 2; ++e) {
         ref[nt][e] = kNothing;
         l[nt][e] = v_inv[nt][e] = 0.f;
-        v_ref[nt][e] = row0 + nt * 8 + 2 * t + e < p.rows ? 0.f : 3e38f;  // (a column without a row asks for nothing)
+        v_lim[nt][e] = (kFold ? (2 * t + e) & 3 : row0 + nt * 8 + 2 * t + e) < p.rows ? 0.f : INFINITY;  // (without a row: none)
       }
     }
 
     for (int tile = mine; tile < tile1; tile += kStep) {
       // ---- S^T = K Q^T ----
-      float s[MT][NT][4];
+      float st[MT][NT][4];
 #pragma unroll
       for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-          for (int k = 0; k < 4; ++k) s[mt][nt][k] = 0.f;
+          for (int k = 0; k < 4; ++k) st[mt][nt][k] = 0.f;
 #pragma unroll
       for (int ch = 0; ch < CH; ++ch)
 #pragma unroll
@@ -515,58 +525,63 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 16 / kWarps : 1)
               if constexpr (kQueryRegs) q = qf[w][ch * 4 + j];
               else q = s_query[((w * NT + nt) * CH * 4 + ch * 4 + j) * 32 + lane];
 #pragma unroll
-              for (int mt = 0; mt < MT; ++mt) mma_f16(s[mt][nt], a[mt][0], a[mt][1], a[mt][2], a[mt][3], q.x, q.y);
+              for (int mt = 0; mt < MT; ++mt) mma_f16(st[mt][nt], a[mt][0], a[mt][1], a[mt][2], a[mt][3], q.x, q.y);
             }
         }
-      float k_scale[MT];
-      int here[MT][2];  // positions of tokens g and g + 8
+      float s[MS][NT][4], k_scale[MS];
+      int here[MS][2];  // positions of tokens g and g + 8
 #pragma unroll
-      for (int mt = 0; mt < MT; ++mt) {
-        k_scale[mt] = ka[mt];
-        const int s0 = (tile + mt) << 4;
-        here[mt][0] = placed ? place[mt][0] : s0 + g;
-        here[mt][1] = placed ? place[mt][1] : s0 + g + 8;
+      for (int ms = 0; ms < MS; ++ms) {
+        k_scale[ms] = ka[ms];
+        here[ms][0] = place[ms][0], here[ms][1] = place[ms][1];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int k = 0; k < 4; ++k) s[ms][nt][k] = kFold && fold ? st[MT - 1][nt][k] : st[ms][nt][k];
       }
       if (tile + kStep < tile1) load_k(tile + kStep);
 
-      // ---- scores of tokens g (k = 0, 1) and g + 8 (k = 2, 3), query rows 2t (k = 0, 2) and 2t + 1 ----
-      bool some[MT];       // whether the mask shows a token of the tile
+      // ---- scores of tokens g (k = 0, 1) and g + 8 (k = 2, 3), columns 2t (k = 0, 2) and 2t + 1 ----
+      bool some[MS];       // whether the mask shows a token of the tile
       bool raise = false;  // whether a reference has to go up
 #pragma unroll
-      for (int mt = 0; mt < MT; ++mt) {
-        const int s0 = (tile + mt) << 4;
-        const bool inside = tile + mt < tile1;
-        some[mt] = inside;
+      for (int ms = 0; ms < MS; ++ms) {
+        const int s0 = (tile + ms + fold) << 4;
+        const bool inside = tile + ms + fold < tile1;
+        some[ms] = inside;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            const float sum = column(nt, e).sum, by = k_scale[mt] * column(nt, e).scale;
-            s[mt][nt][e] = (s[mt][nt][e] - sum) * by;
-            s[mt][nt][2 + e] = (s[mt][nt][2 + e] - sum) * by;
+            const float sum = column(nt, e).sum, by = k_scale[ms] * column(nt, e).scale;
+            s[ms][nt][e] = (s[ms][nt][e] - sum) * by;
+            s[ms][nt][2 + e] = (s[ms][nt][2 + e] - sum) * by;
           }
         }
         if (p.table != nullptr) {
+          if (!placed) here[ms][0] = s0 + g, here[ms][1] = s0 + g + 8;
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
-              const int d = column(nt, k & 1).where - here[mt][k >> 1];
-              s[mt][nt][k] += s_table[column(nt, k & 1).bias + s_buckets[min(max(d, 0), p.distances - 1)]];
+              const int d = column(nt, k & 1).where - here[ms][k >> 1];
+              s[ms][nt][k] += s_table[column(nt, k & 1).bias + s_buckets[min(max(d, 0), p.distances - 1)]];
             }
         }
-        if (!(inside && s0 + 15 <= all_see && mask == nullptr)) {
+        const int last = tile + (kFold ? MT : ms + 1);  // of the step's tiles that are looked at here, and one
+        if (!(last <= tile1 && last * 16 - 1 <= all_see && mask == nullptr)) {
           bool shown[2] = {inside, inside};
           if (mask != nullptr) {
 #pragma unroll
             for (int e = 0; e < 2; ++e) shown[e] = inside && s0 + g + 8 * e < p.mask_len && mask[s0 + g + 8 * e] != 0;
-            some[mt] = __any_sync(0xffffffffu, shown[0] || shown[1]);
+            const uint32_t which = __ballot_sync(0xffffffffu, shown[0] || shown[1]);
+            some[ms] = (which & (!kFold ? 0xffffffffu : fold ? 0xccccccccu : 0x33333333u)) != 0;
           }
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
             for (int k = 0; k < 4; ++k)
-              if (!shown[k >> 1] || s0 + g + 8 * (k >> 1) > column(nt, k & 1).lim) s[mt][nt][k] = -INFINITY;
+              if (!shown[k >> 1] || s0 + g + 8 * (k >> 1) > column(nt, k & 1).lim) s[ms][nt][k] = -INFINITY;
         }
         if ((kBlock ? c.weight != nullptr : p.scores != nullptr) && inside) {
           float* to = kBlock ? s_scores : p.scores + bh * p.rows * c.slots;
@@ -574,10 +589,10 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 16 / kWarps : 1)
           for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-              const int r = row0 + nt * 8 + 2 * t + e;
+              const int r = kFold ? (2 * t + e) & 3 : row0 + nt * 8 + 2 * t + e;
               if (r < p.rows) {
-                to[r * c.slots + s0 + g] = s[mt][nt][e];
-                to[r * c.slots + s0 + g + 8] = s[mt][nt][2 + e];
+                to[r * c.slots + s0 + g] = s[ms][nt][e];
+                to[r * c.slots + s0 + g + 8] = s[ms][nt][2 + e];
               }
             }
         }
@@ -585,8 +600,8 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 16 / kWarps : 1)
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            raise |= fmaxf(s[mt][nt][e], s[mt][nt][2 + e]) - ref[nt][e] > kLimit;
-            raise |= va[mt] > 4.f * v_ref[nt][e];
+            raise |= fmaxf(s[ms][nt][e], s[ms][nt][2 + e]) - ref[nt][e] > kLimit;
+            raise |= va[ms] > v_lim[nt][e];
           }
       }
 
@@ -596,11 +611,11 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 16 / kWarps : 1)
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            float x = -INFINITY, v = v_ref[nt][e];
+            float x = -INFINITY, v = 0.25f * v_lim[nt][e];
 #pragma unroll
-            for (int mt = 0; mt < MT; ++mt) {
-              x = fmaxf(x, fmaxf(s[mt][nt][e], s[mt][nt][2 + e]));
-              if (some[mt] && column(nt, e).lim >= (tile + mt) << 4 && va[mt] < INFINITY) v = fmaxf(v, va[mt]);
+            for (int ms = 0; ms < MS; ++ms) {
+              x = fmaxf(x, fmaxf(s[ms][nt][e], s[ms][nt][2 + e]));
+              if (some[ms] && column(nt, e).lim >= (tile + ms + fold) << 4 && va[ms] < INFINITY) v = fmaxf(v, va[ms]);
             }
             x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
             x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
@@ -608,10 +623,10 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 16 / kWarps : 1)
             const float up = fmaxf(x - kPeak, ref[nt][e]);
             const float f = exp2_approx(ref[nt][e] - up);
             v_inv[nt][e] = v > 0.f ? __frcp_rn(v) : 0.f;
-            const float shrink = f * (v_ref[nt][e] * v_inv[nt][e]);  // (0 where nothing had been met)
+            const float shrink = f * (0.25f * v_lim[nt][e] * v_inv[nt][e]);  // (0 where nothing had been met)
             ref[nt][e] = up;
             l[nt][e] *= f;
-            v_ref[nt][e] = v;
+            v_lim[nt][e] = 4.f * v;
 #pragma unroll
             for (int i = 0; i < MI; ++i) o[nt][i][e] *= shrink, o[nt][i][2 + e] *= shrink;
           }
@@ -620,31 +635,37 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 16 / kWarps : 1)
       // ---- probabilities ----
       uint32_t pf[Q2][MT][NT][2];
 #pragma unroll
-      for (int mt = 0; mt < MT; ++mt)
+      for (int ms = 0; ms < MS; ++ms)
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-          const float r[2] = {va[mt] * v_inv[nt][0], va[mt] * v_inv[nt][1]};
+          const float r[2] = {va[ms] * v_inv[nt][0], va[ms] * v_inv[nt][1]};
           float pr[4];
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
-            pr[k] = exp2_approx(s[mt][nt][k] - ref[nt][k & 1]);
+            pr[k] = exp2_approx(s[ms][nt][k] - ref[nt][k & 1]);
             l[nt][k & 1] += pr[k];
             pr[k] *= r[k & 1];
           }
-          if (!(va[mt] < INFINITY)) {  // a block that is not finite: what is hidden counts for nothing all the same
+          if (!(va[ms] < INFINITY)) {  // a block that is not finite: what is hidden counts for nothing all the same
 #pragma unroll
             for (int k = 0; k < 4; ++k)
-              if (s[mt][nt][k] == -INFINITY) pr[k] = 0.f;
+              if (s[ms][nt][k] == -INFINITY) pr[k] = 0.f;
           }
           const __half2 v0 = __floats2half2_rn(pr[0], pr[1]), v1 = __floats2half2_rn(pr[2], pr[3]);
-          pf[0][mt][nt][0] = transposed(as_u32(v0));
-          pf[0][mt][nt][1] = transposed(as_u32(v1));
+          uint32_t f[Q2][2];
+          f[0][0] = as_u32(v0), f[0][1] = as_u32(v1);
           if (kTwo) {
-            pf[Q2 - 1][mt][nt][0] =
-                transposed(as_u32(__floats2half2_rn(pr[0] - __low2float(v0), pr[1] - __high2float(v0))));
-            pf[Q2 - 1][mt][nt][1] =
-                transposed(as_u32(__floats2half2_rn(pr[2] - __low2float(v1), pr[3] - __high2float(v1))));
+            f[Q2 - 1][0] = as_u32(__floats2half2_rn(pr[0] - __low2float(v0), pr[1] - __high2float(v0)));
+            f[Q2 - 1][1] = as_u32(__floats2half2_rn(pr[2] - __low2float(v1), pr[3] - __high2float(v1)));
           }
+#pragma unroll
+          for (int w = 0; w < Q2; ++w)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const uint32_t turned = transposed(f[w][e]);  // (column g now)
+              if constexpr (kFold) pf[w][0][nt][e] = g < 4 ? turned : 0u, pf[w][1][nt][e] = g < 4 ? 0u : turned;
+              else pf[w][ms][nt][e] = turned;
+            }
         }
 
       // ---- O^T += V^T P^T ----
@@ -671,22 +692,31 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 16 / kWarps : 1)
     const bool whole = tile0 == 0 && tile1 == tiles;
     const long long slot = ((static_cast<long long>(row_tile) * p.pieces + unit) * 2 + (tile0 == 0 ? 1 : 0)) * NT * 8;
     if constexpr (kTeam) {
-      // ---- the warps meet ----
+      // ---- the warps meet; the weights of the first slots are requested ahead ----
+      constexpr int kAhead = 4;
+      float weight[kAhead];
+      if (kBlock && c.weight != nullptr) {
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) {
+          const int at_slot = threadIdx.x + i * kThreads;
+          weight[i] = at_slot < start ? c.weight[slots0 + at_slot] : 0.f;
+        }
+      }
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         float sum = l[0][e];
         sum += __shfl_xor_sync(0xffffffffu, sum, 4);
         sum += __shfl_xor_sync(0xffffffffu, sum, 8);
         sum += __shfl_xor_sync(0xffffffffu, sum, 16);
-        const int r = 2 * t + e;
+        const int r = kFold ? (2 * t + e) & 3 : 2 * t + e, part = wid * kParts + fold;
         if (r < p.rows) {
-          const float f = v_ref[0][e] * (1.f / 127.f);
-          float* dst = s_sums + (wid * p.rows + r) * D + VB * g;
+          const float f = v_lim[0][e] * (0.25f / 127.f);
+          float* dst = s_sums + (part * p.rows + r) * D + VB * g;
 #pragma unroll
           for (int i = 0; i < MI; i += 2)
             *reinterpret_cast<float4*>(dst + 2 * i) = make_float4(o[0][i][e] * f, o[0][i][2 + e] * f, o[0][i + 1][e] * f,
                                                                   o[0][i + 1][2 + e] * f);
-          if (g == 0) s_stats[wid][r] = make_float2(ref[0][e], sum);
+          if (g == 0) s_stats[part][r] = make_float2(ref[0][e], sum);
         }
       }
       __syncthreads();
@@ -695,9 +725,9 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 16 / kWarps : 1)
         float high = kNothing, sum = 0.f;
         float x[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int w = 0; w < kWarps; ++w) high = fmaxf(high, s_stats[w][r].x);
+        for (int w = 0; w < kWarps * kParts; ++w) high = fmaxf(high, s_stats[w][r].x);
 #pragma unroll
-        for (int w = 0; w < kWarps; ++w) {
+        for (int w = 0; w < kWarps * kParts; ++w) {
           const float2 st = s_stats[w][r];
           if (st.y == 0.f) continue;  // (a warp that saw nothing may have sums of 0 * NaN)
           const float f = exp2_approx(st.x - high);
@@ -721,16 +751,22 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 16 / kWarps : 1)
       }
       if (kBlock && c.weight != nullptr) {
         __syncthreads();
-#pragma unroll 4
-        for (int s = threadIdx.x; s < end; s += kThreads) {
-          float* weight = c.weight + slots0 + s;
-          float sum = s >= start ? 0.f : *weight;
+        auto given = [&](int s) {
+          float sum = 0.f;
           for (int r = 0; r < p.rows; ++r) {
             const float x = s_scores[r * c.slots + s];
             if (x > -INFINITY || x != x) sum += exp2_approx(x - s_rows[r].x) * s_rows[r].y;
           }
-          *weight = sum;
+          return sum;
+        };
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) {
+          const int at_slot = threadIdx.x + i * kThreads;
+          if (at_slot < end) c.weight[slots0 + at_slot] = weight[i] + given(at_slot);
         }
+#pragma unroll 4
+        for (int s = threadIdx.x + kAhead * kThreads; s < end; s += kThreads)
+          c.weight[slots0 + s] = (s >= start ? 0.f : c.weight[slots0 + s]) + given(s);
       }
       if (!kBlock) __syncthreads();  // the next piece's query and sums
     } else {
@@ -745,7 +781,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 16 / kWarps : 1)
           const int col = nt * 8 + 2 * t + e, r = row0 + col;
           if (r >= p.rows) continue;
           // (a row that nothing was seen of may have sums of 0 * NaN)
-          const float f = v_ref[nt][e] * (1.f / 127.f) * (whole ? 1.f / sum : 1.f);
+          const float f = v_lim[nt][e] * (0.25f / 127.f) * (whole ? 1.f / sum : 1.f);
           float x[VB];
 #pragma unroll
           for (int i = 0; i < MI; ++i) {
@@ -883,7 +919,7 @@ cudaError_t launch_behind(bool behind, void (*kernel)(Params...), dim3 grid, int
 constexpr int kMaxTeamBytes = 72 * 1024;
 constexpr int kRowWarps = 8;
 size_t team_bytes(const Cache8& c, int rows, bool scores) {
-  return 4ull * rows * (8ull * c.dim + (scores && c.weight != nullptr ? c.slots : 0));
+  return 4ull * rows * ((rows <= 4 && c.dim == 64 ? 16ull : 8ull) * c.dim + (scores && c.weight != nullptr ? c.slots : 0));
 }
 // Whether a CTA takes a whole (row, head): caches of up to 1024 slots, and longer ones where there are several CTAs' worth
 // for every SM.
@@ -894,7 +930,7 @@ bool by_row_head(const Cache8& c, int rows) {
 
 constexpr int tile_rows_of(int rows) { return rows <= 8 ? 8 : 32; }
 
-template <typename T, int D, int NT, int MT, bool kTwo, Deal kDeal, int kWarps>
+template <typename T, int D, int NT, int MT, bool kTwo, Deal kDeal, int kWarps, bool kFold>
 cudaError_t launch_tile(const Cache8Attn& p, const NewTokens<T>& fresh, bool behind, cudaStream_t stream) {
   constexpr bool kBlock = kDeal == kRowHead, kTeam = kDeal != kRows;
   constexpr size_t query = sizeof(uint2) * (kTeam ? 1 : kWarps) * (kTwo ? 2 : 1) * NT * (D / 64) * 4 * 32;
@@ -904,7 +940,7 @@ cudaError_t launch_tile(const Cache8Attn& p, const NewTokens<T>& fresh, bool beh
   int dev = 0;
   cudaGetDevice(&dev);
   if (!set[dev & 63]) {
-    cudaError_t e = cudaFuncSetAttribute(cache8_attention_kernel<T, D, NT, MT, kTwo, kDeal, kWarps>,
+    cudaError_t e = cudaFuncSetAttribute(cache8_attention_kernel<T, D, NT, MT, kTwo, kDeal, kWarps, kFold>,
                                          cudaFuncAttributeMaxDynamicSharedMemorySize,
                                          static_cast<int>(query) + kMaxBiases * 4 + (kTeam ? kMaxTeamBytes : 0));
     if (e != cudaSuccess) return e;
@@ -915,7 +951,7 @@ cudaError_t launch_tile(const Cache8Attn& p, const NewTokens<T>& fresh, bool beh
                     : kTeam           ? dim3(p.pieces)
                     : p.row_warps > 1 ? dim3(p.pieces, (row_tiles + kWarps - 1) / kWarps)
                                       : dim3(p.pieces / kWarps, row_tiles);
-  return launch_behind(behind, cache8_attention_kernel<T, D, NT, MT, kTwo, kDeal, kWarps>, grid, kWarps * 32, smem, stream, p, fresh);
+  return launch_behind(behind, cache8_attention_kernel<T, D, NT, MT, kTwo, kDeal, kWarps, kFold>, grid, kWarps * 32, smem, stream, p, fresh);
 }
 
 template <typename T, bool kTwo>
@@ -923,11 +959,13 @@ cudaError_t launch_row_heads(const Cache8Attn& p, const T5xNewTokens* tokens, cu
   const NewTokens<T> fresh = make_tokens<T>(tokens);
   // half the warps where there are CTAs for all SMs: what a CTA does around its tiles overlaps more of the others' tiles
   const bool many = static_cast<long long>(p.c.batch) * p.c.heads >= 2LL * num_sms();
-  if (p.c.dim == 64)
-    return many ? launch_tile<T, 64, 1, 2, kTwo, kRowHead, 4>(p, fresh, false, stream)
-                : launch_tile<T, 64, 1, 2, kTwo, kRowHead, 8>(p, fresh, false, stream);
-  return many ? launch_tile<T, 128, 1, 1, kTwo, kRowHead, 4>(p, fresh, false, stream)
-              : launch_tile<T, 128, 1, 1, kTwo, kRowHead, 8>(p, fresh, false, stream);
+  auto launch_with = [&](auto kernel_warps) {
+    constexpr int W = decltype(kernel_warps)::value;
+    if (p.c.dim == 128) return launch_tile<T, 128, 1, 1, kTwo, kRowHead, W, false>(p, fresh, false, stream);
+    return p.rows <= 4 ? launch_tile<T, 64, 1, 2, kTwo, kRowHead, W, true>(p, fresh, false, stream)
+                       : launch_tile<T, 64, 1, 2, kTwo, kRowHead, W, false>(p, fresh, false, stream);
+  };
+  return many ? launch_with(std::integral_constant<int, 4>()) : launch_with(std::integral_constant<int, 8>());
 }
 
 template <typename T, bool kTwo>
@@ -936,11 +974,12 @@ cudaError_t launch_pieces(const Cache8Attn& p, bool behind, cudaStream_t stream)
   const NewTokens<T> none = {};
   cudaError_t e;
   if (p.c.dim == 64)
-    e = tile_rows == 8 ? launch_tile<T, 64, 1, 2, kTwo, kPieces, 8>(p, none, behind, stream)
-                       : launch_tile<T, 64, 4, 1, kTwo, kRows, kRowWarps>(p, none, false, stream);
+    e = p.rows <= 4      ? launch_tile<T, 64, 1, 2, kTwo, kPieces, 8, true>(p, none, behind, stream)
+        : tile_rows == 8 ? launch_tile<T, 64, 1, 2, kTwo, kPieces, 8, false>(p, none, behind, stream)
+                         : launch_tile<T, 64, 4, 1, kTwo, kRows, kRowWarps, false>(p, none, false, stream);
   else
-    e = tile_rows == 8 ? launch_tile<T, 128, 1, 1, kTwo, kPieces, 8>(p, none, behind, stream)
-                       : launch_tile<T, 128, 4, 1, kTwo, kRows, kRowWarps>(p, none, false, stream);
+    e = tile_rows == 8 ? launch_tile<T, 128, 1, 1, kTwo, kPieces, 8, false>(p, none, behind, stream)
+                       : launch_tile<T, 128, 4, 1, kTwo, kRows, kRowWarps, false>(p, none, false, stream);
   if (e != cudaSuccess) return e;
   const dim3 rows(static_cast<unsigned>(p.c.batch) * p.c.heads, p.rows);
   e = p.c.dim == 64 ? launch_behind(true, cache8_join_kernel<T, 64>, rows, kJoinThreads, 0, stream, p, tile_rows)
