@@ -33,8 +33,6 @@ __global__ void __launch_bounds__(kAppendThreads)
 // ---------------------------------------------------------------------------
 // Eviction: which slots stay.
 // ---------------------------------------------------------------------------
-constexpr int kSelectThreads = 1024;
-
 // Order of weights as unsigned numbers: NaN above all, -0 as 0.
 __device__ __forceinline__ uint32_t order_of(float w) {
   if (!(w == w)) return 0xffffffffu;
@@ -42,6 +40,158 @@ __device__ __forceinline__ uint32_t order_of(float w) {
   if (u == 0x80000000u) u = 0;
   return u ^ (u >> 31 ? 0xffffffffu : 0x80000000u);
 }
+
+// Of the counts of 16 digits (lanes 0 to 15) the digit at which `need` of the largest are reached; need less those above it.
+__device__ __forceinline__ int border_digit(int count, int& need) {
+  const int lane = threadIdx.x & 31;
+  int from = lane < 16 ? count : 0;  // of this digit and those above
+#pragma unroll
+  for (int o = 1; o < 16; o <<= 1) {
+    const int u = __shfl_down_sync(0xffffffffu, from, o);
+    if (lane + o < 16) from += u;
+  }
+  const int digit = 31 - __clz(__ballot_sync(0xffffffffu, lane < 16 && from >= need) | 1);
+  need -= __shfl_sync(0xffffffffu, from - count, digit);
+  return digit;
+}
+
+__device__ __forceinline__ unsigned long long remote_u64(const unsigned long long* mine, uint32_t cta) {
+  unsigned long long v;
+  asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v) : "r"(mapa_shared(smem_u32(mine), cta)) : "memory");
+  return v;
+}
+__device__ __forceinline__ int remote_int(const int* mine, uint32_t cta) {
+  int v;
+  asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(mapa_shared(smem_u32(mine), cta)) : "memory");
+  return v;
+}
+
+// A CTA, or a cluster, takes the slots of one head of one row and keeps its weights in registers, K a thread. The border is
+// found four bits at a time: a lane of each warp counts one of the 16 digits from the ballots of the four bits (no atomics
+// on a bin that most weights share: many are equal, or zero). A slot's place is the number of larger ones before it, and of
+// those at the border as far as they stay.
+template <int T, int K, bool kCluster>
+__global__ void __launch_bounds__(T)
+    cache8_select_kernel(const __grid_constant__ Cache8 c, int keep, int recent, int ctas, int* __restrict__ kept,
+                         int* __restrict__ index_out, int* __restrict__ dropped_out) {
+  __shared__ int s_hist[8][16];
+  __shared__ unsigned long long s_before[K * T / 32 + 1];  // larger | at the border << 32, by row of T slots and warp
+  constexpr int kWarps = T / 32;
+  const long long bh = kCluster ? blockIdx.x / ctas : blockIdx.x;
+  const uint32_t rank = kCluster ? cluster_ctarank() : 0;
+  const int b = static_cast<int>(bh / c.heads);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int index = max(c.index[static_cast<long long>(b) * c.index_stride], 0), held = min(index, c.slots);
+  const float* w = c.weight + bh * c.slots;
+  int* out = kept + bh * keep;
+  chain_release();
+  if (bh == static_cast<long long>(b) * c.heads && rank == 0 && threadIdx.x == 0) {
+    index_out[b] = min(held, keep);
+    dropped_out[b] = (c.position != nullptr ? c.dropped[b] : 0) + (index - min(held, keep));
+  }
+  if (held <= keep) {
+    for (int i = rank * T + threadIdx.x; i < keep; i += T * ctas) out[i] = i < held ? i : -1;
+    return;
+  }
+  const int old = held - recent, first = static_cast<int>(rank) * (T * K);  // slots to choose from; this CTA's first
+  uint32_t key[K];
+#pragma unroll
+  for (int i = 0; i < K; ++i) {
+    const int s = first + i * T + threadIdx.x;
+    key[i] = s < old ? order_of(w[s]) : 0;
+  }
+  if (threadIdx.x < 128) s_hist[threadIdx.x / 16][threadIdx.x % 16] = 0;
+  __syncthreads();
+
+  int need = keep - recent;
+  uint32_t border = 0;
+  if (need > 0)
+    for (int round = 0; round < 8; ++round) {
+      const int shift = 28 - 4 * round;
+      int count = 0;
+#pragma unroll
+      for (int i = 0; i < K; ++i) {
+        const bool in = first + i * T + static_cast<int>(threadIdx.x) < old && (round == 0 || ((key[i] ^ border) >> (shift + 4)) == 0);
+        uint32_t m = __ballot_sync(0xffffffffu, in);
+        if (m == 0) continue;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const uint32_t set = __ballot_sync(0xffffffffu, (key[i] >> (shift + k)) & 1);
+          m &= (lane >> k) & 1 ? set : ~set;
+        }
+        count += __popc(m);
+      }
+      if (lane < 16 && count > 0) atomicAdd(&s_hist[round][lane], count);
+      if (kCluster) cluster_sync_all();
+      else __syncthreads();
+      int all = 0;
+      if (lane < 16) {
+        if (kCluster)
+          for (int r = 0; r < ctas; ++r) all += remote_int(&s_hist[round][lane], r);
+        else
+          all = s_hist[round][lane];
+      }
+      border |= static_cast<uint32_t>(border_digit(all, need)) << shift;
+    }
+  const int ties = need;  // of the slots at the border, the first so many stay
+  const bool any = keep > recent;
+
+#pragma unroll
+  for (int i = 0; i < K; ++i) {
+    const bool in = any && first + i * T + static_cast<int>(threadIdx.x) < old;
+    const uint32_t above = __ballot_sync(0xffffffffu, in && key[i] > border), tie = __ballot_sync(0xffffffffu, in && key[i] == border);
+    if (lane == 0) s_before[i * kWarps + warp] = __popc(above) | static_cast<unsigned long long>(__popc(tie)) << 32;
+  }
+  __syncthreads();
+  if (warp == 0) {  // sums of what is before each
+    constexpr int kEach = (K * kWarps + 31) / 32;
+    unsigned long long v[kEach], sum = 0;
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+      const int at = lane * kEach + i;
+      v[i] = at < K * kWarps ? s_before[at] : 0;
+      sum += v[i];
+    }
+    unsigned long long run = sum;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const unsigned long long u = __shfl_up_sync(0xffffffffu, run, o);
+      if (lane >= o) run += u;
+    }
+    if (lane == 31) s_before[K * kWarps] = run;
+    run -= sum;
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+      const int at = lane * kEach + i;
+      if (at < K * kWarps) s_before[at] = run;
+      run += v[i];
+    }
+  }
+  unsigned long long base = 0;
+  if (kCluster) {
+    cluster_sync_all();
+    for (int r = 0; r < static_cast<int>(rank); ++r) base += remote_u64(&s_before[K * kWarps], r);
+  } else {
+    __syncthreads();
+  }
+#pragma unroll
+  for (int i = 0; i < K; ++i) {
+    const int s = first + i * T + threadIdx.x;
+    const bool in = any && s < old;
+    const bool is_above = in && key[i] > border, is_tie = in && key[i] == border;
+    const uint32_t under = (1u << lane) - 1;
+    const uint32_t above = __ballot_sync(0xffffffffu, is_above) & under, tie = __ballot_sync(0xffffffffu, is_tie) & under;
+    const unsigned long long before = base + s_before[i * kWarps + warp];
+    const int tie_rank = static_cast<int>(before >> 32) + __popc(tie);
+    const int place = static_cast<int>(before & 0xffffffffu) + __popc(above) + min(tie_rank, ties);
+    if (is_above || (is_tie && tie_rank < ties)) out[place] = s;
+    else if (s >= old && s < held) out[keep - recent + s - old] = s;
+  }
+  if (kCluster) cluster_sync_all();  // nobody leaves while others read its sums
+}
+
+// Over more slots than a cluster's registers hold the weights are read once for each digit.
+constexpr int kWalkThreads = 1024;
 
 __device__ __forceinline__ int block_scan(int v, int* s_sums) {  // sum over the threads before; leaves the total in s_sums[32]
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -69,20 +219,25 @@ __device__ __forceinline__ int block_scan(int v, int* s_sums) {  // sum over the
   return sum - v + s_sums[warp];
 }
 
-// A CTA takes the slots of one head of one row: the border weight digit by digit from counts, then a walk in order.
-__global__ void __launch_bounds__(kSelectThreads)
-    cache8_select_kernel(const __grid_constant__ Cache8 c, int keep, int recent, int* __restrict__ kept) {
+__global__ void __launch_bounds__(kWalkThreads)
+    cache8_select_walk_kernel(const __grid_constant__ Cache8 c, int keep, int recent, int* __restrict__ kept,
+                              int* __restrict__ index_out, int* __restrict__ dropped_out) {
   __shared__ int s_count[256];
   __shared__ int s_sums[33];
   __shared__ uint32_t s_prefix;
   __shared__ int s_need;
   const long long bh = blockIdx.x;
   const int b = static_cast<int>(bh / c.heads);
-  const int held = held_of(c, b);
+  const int index = max(c.index[static_cast<long long>(b) * c.index_stride], 0), held = min(index, c.slots);
   const float* w = c.weight + bh * c.slots;
   int* out = kept + bh * keep;
+  chain_release();
+  if (bh == static_cast<long long>(b) * c.heads && threadIdx.x == 0) {
+    index_out[b] = min(held, keep);
+    dropped_out[b] = (c.position != nullptr ? c.dropped[b] : 0) + (index - min(held, keep));
+  }
   if (held <= keep) {
-    for (int i = threadIdx.x; i < keep; i += kSelectThreads) out[i] = i < held ? i : -1;
+    for (int i = threadIdx.x; i < keep; i += kWalkThreads) out[i] = i < held ? i : -1;
     return;
   }
   const int old = held - recent;  // the slots to choose from
@@ -95,7 +250,7 @@ __global__ void __launch_bounds__(kSelectThreads)
     __syncthreads();
     const uint32_t prefix = s_prefix;
     const int need = s_need;
-    for (int i = threadIdx.x; i < old; i += kSelectThreads) {
+    for (int i = threadIdx.x; i < old; i += kWalkThreads) {
       const uint32_t u = order_of(w[i]);
       if (shift == 24 || (u >> (shift + 8)) == (prefix >> (shift + 8))) atomicAdd(&s_count[(u >> shift) & 255], 1);
     }
@@ -112,7 +267,7 @@ __global__ void __launch_bounds__(kSelectThreads)
   const uint32_t border = s_prefix;
   const int ties = s_need;  // of the slots at the border, the first so many stay
   int at = 0, seen = 0;
-  for (int i0 = 0; i0 < held; i0 += kSelectThreads) {
+  for (int i0 = 0; i0 < held; i0 += kWalkThreads) {
     const int i = i0 + threadIdx.x;
     const uint32_t u = i < old ? order_of(w[i]) : 0;
     const bool tie = i < old && u == border && keep > recent;
@@ -125,52 +280,102 @@ __global__ void __launch_bounds__(kSelectThreads)
   }
 }
 
-// A CTA takes one block of one head of the smaller cache.
-constexpr int kMoveThreads = 128;
+// ---------------------------------------------------------------------------
+// Eviction: the tokens that stay. A CTA takes one block of one head of the smaller cache, 16 codes a thread at a time.
+// Tokens of a new block come from many old ones, so nearly all codes are rounded again; near a border between two codes
+// exactly, by Coder, and else by one product: 16 codes as numbers (a byte under the exponent of 2^23), times the ratio of the
+// scales, back under the exponent of 3 * 2^22, which rounds to whole numbers.
+// ---------------------------------------------------------------------------
+constexpr int kMoveThreads = 256;
 
-__global__ void __launch_bounds__(kMoveThreads)
-    cache8_move_kernel(const __grid_constant__ Cache8 c, const __grid_constant__ Cache8 to, int keep, const int* __restrict__ kept, int* __restrict__ index_out,
-                       int* __restrict__ dropped_out) {
-  const int b = blockIdx.z, h = blockIdx.y, blk = blockIdx.x;
-  const int held = held_of(c, b), n = min(held, keep);
-  if (h == 0 && blk == 0 && threadIdx.x == 0) {
-    index_out[b] = n;
-    dropped_out[b] = (c.position != nullptr ? c.dropped[b] : 0) +
-                     (max(c.index[static_cast<long long>(b) * c.index_stride], 0) - n);
+__device__ __forceinline__ uint32_t round_four(uint32_t w, float ratio, float& off) {
+  uint32_t r[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float x = __uint_as_float(__byte_perm(w ^ 0x80808080u, 0x4b000000u, 0x7440 + i)) - 8388736.f;
+    const float q = x * ratio, up = q + 12582912.f;
+    off = fmaxf(off, fabsf(q - (up - 12582912.f)));
+    r[i] = __float_as_uint(up);
   }
-  const int block = 1 << to.block_log2;
-  const int lo = blk << to.block_log2, hi = min(lo + block, n);
-  if (lo >= hi) return;
+  return __byte_perm(__byte_perm(r[0], r[1], 0x0040), __byte_perm(r[2], r[3], 0x0040), 0x5410);
+}
+
+__device__ __forceinline__ uint32_t round_four_exactly(uint32_t w, const Coder& again) {
+  uint32_t r = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    r |= static_cast<uint32_t>(again(static_cast<float>(static_cast<int8_t>(w >> (8 * i)))) & 0xff) << (8 * i);
+  return r;
+}
+
+template <int D>
+__global__ void __launch_bounds__(kMoveThreads)
+    cache8_move_kernel(const __grid_constant__ Cache8 c, const __grid_constant__ Cache8 to, int keep,
+                       const int* __restrict__ kept) {
+  __shared__ int s_from[128];
+  __shared__ float s_old[2][128], s_ratio[2][128];
+  __shared__ uint32_t s_most[2];
+  const int b = blockIdx.z, h = blockIdx.y, blk = blockIdx.x;
+  const int n = min(held_of(c, b), keep);
+  const int lo = blk << to.block_log2, count = min(1 << to.block_log2, n - lo);
   const long long bh = static_cast<long long>(b) * c.heads + h;
-  const int* from = kept + bh * keep;
-  const int dim = c.dim;
+  chain_wait();
+  if (count <= 0) return;
+  if (threadIdx.x < 2) s_most[threadIdx.x] = 0;
+  if (static_cast<int>(threadIdx.x) < count) s_from[threadIdx.x] = __ldcg(kept + bh * keep + lo + threadIdx.x);
+  __syncthreads();
+
+  constexpr int L = D / 16, kTokens = kMoveThreads / L, U = 128 / kTokens;  // threads a token, tokens at a time, turns
+  const int tok = threadIdx.x / L, part = threadIdx.x % L;
+  uint4 v[U];
+  auto load = [&](int what) {
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (tok + u * kTokens < count)
+        v[u] = *(reinterpret_cast<const uint4*>(c.codes[what] + (bh * c.slots + s_from[tok + u * kTokens]) * D) + part);
+  };
+  load(0);
+  {  // scales: keys' by one half of the threads, values' by the other
+    const int what = threadIdx.x >> 7, i = threadIdx.x & 127;
+    float old = 0.f;
+    if (i < count) old = c.absmax[what][bh * (c.slots >> c.block_log2) + (s_from[i] >> c.block_log2)];
+    s_old[what][i] = old;
+    const uint32_t most = __reduce_max_sync(0xffffffffu, abs_bits(old));
+    if ((threadIdx.x & 31) == 0) atomicMax(&s_most[what], most);
+    __syncthreads();
+    const float a = __uint_as_float(s_most[what]);
+    // -1: as it is; -2: by Coder
+    s_ratio[what][i] = abs_bits(old) == s_most[what] ? -1.f : a >= 0x1p-60f && a <= 0x1p100f ? __fdiv_rn(old, a) : -2.f;
+    if (i == 0) to.absmax[what][bh * (to.slots >> to.block_log2) + blk] = a;
+    if (what == 0 && i < count) {
+      to.weight[bh * to.slots + lo + i] = c.weight[bh * c.slots + s_from[i]];
+      to.position[bh * to.slots + lo + i] = c.position != nullptr ? c.position[bh * c.slots + s_from[i]] : s_from[i];
+    }
+    __syncthreads();
+  }
 #pragma unroll
   for (int what = 0; what < 2; ++what) {
-    const float* absmax = c.absmax[what] + bh * (c.slots >> c.block_log2);
-    uint32_t most = 0;
-    for (int i = lo + (threadIdx.x & 31); i < hi; i += 32) most = max(most, abs_bits(absmax[from[i] >> c.block_log2]));
-    most = __reduce_max_sync(0xffffffffu, most);
-    const float a = __uint_as_float(most);
-    if (threadIdx.x == 0) to.absmax[what][bh * (to.slots >> to.block_log2) + blk] = a;
-    const int8_t* src = c.codes[what] + bh * c.slots * dim;
-    int8_t* dst = to.codes[what] + bh * to.slots * dim;
-    const int words = dim / 4;
-    for (int i = threadIdx.x; i < (hi - lo) * words; i += kMoveThreads) {
-      const int tok = lo + i / words, d = i % words;
-      const int s = from[tok];
-      const float before = absmax[s >> c.block_log2];
-      char4 v = reinterpret_cast<const char4*>(src + static_cast<long long>(s) * dim)[d];
-      if (abs_bits(before) != most) {
-        const Coder again(before, a);
-        v = make_char4(again(v.x), again(v.y), again(v.z), again(v.w));
+    const float a = __uint_as_float(s_most[what]);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int i = tok + u * kTokens;
+      if (i >= count) continue;
+      const float ratio = s_ratio[what][i];
+      if (ratio != -1.f) {
+        float off = ratio < 0.f ? 1.f : 0.f;
+        const uint4 o = make_uint4(round_four(v[u].x, ratio, off), round_four(v[u].y, ratio, off), round_four(v[u].z, ratio, off),
+                                   round_four(v[u].w, ratio, off));
+        if (off < 0.4999f) {
+          v[u] = o;
+        } else {
+          const Coder again(s_old[what][i], a);
+          v[u] = make_uint4(round_four_exactly(v[u].x, again), round_four_exactly(v[u].y, again),
+                            round_four_exactly(v[u].z, again), round_four_exactly(v[u].w, again));
+        }
       }
-      reinterpret_cast<char4*>(dst + static_cast<long long>(tok) * dim)[d] = v;
+      *(reinterpret_cast<uint4*>(to.codes[what] + (bh * to.slots + lo + i) * D) + part) = v[u];
     }
-  }
-  for (int i = lo + threadIdx.x; i < hi; i += kMoveThreads) {
-    const int s = from[i];
-    to.weight[bh * to.slots + i] = c.weight[bh * c.slots + s];
-    to.position[bh * to.slots + i] = c.position != nullptr ? c.position[bh * c.slots + s] : s;
+    if (what == 0) load(1);
   }
 }
 
@@ -227,6 +432,51 @@ int launch_append(const Cache8& c, const T5xNewTokens* in, cudaStream_t stream) 
   return e == cudaSuccess ? 0 : set_error("cache8_append launch: %s", cudaGetErrorString(e));
 }
 
+template <int T, int K>
+cudaError_t launch_select_by(int ctas, const Cache8& c, int keep, int recent, int* kept, int* index_out, int* dropped_out,
+                             cudaStream_t stream) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(c.batch) * c.heads * ctas);
+  cfg.blockDim = dim3(T);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = ctas;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = ctas > 1 ? 1 : 0;
+  count_launches(1);
+  return cudaLaunchKernelEx(&cfg, ctas > 1 ? cache8_select_kernel<T, K, true> : cache8_select_kernel<T, K, false>, c, keep, recent,
+                            ctas, kept, index_out, dropped_out);
+}
+
+// The weights of a head in the registers of one CTA up to 2048 slots, of up to eight up to 65536.
+cudaError_t launch_select(const Cache8& c, int keep, int recent, int* kept, int* index_out, int* dropped_out, cudaStream_t stream) {
+  const int ctas = c.slots <= 2048 ? 1 : c.slots <= 4096 ? 2 : c.slots <= 8192 ? 4 : 8;
+  if (c.slots <= 2048 * 8) return launch_select_by<256, 8>(ctas, c, keep, recent, kept, index_out, dropped_out, stream);
+  if (c.slots <= 8192 * 8) return launch_select_by<1024, 8>(8, c, keep, recent, kept, index_out, dropped_out, stream);
+  cache8_select_walk_kernel<<<static_cast<unsigned>(c.batch) * c.heads, kWalkThreads, 0, stream>>>(c, keep, recent, kept, index_out,
+                                                                                               dropped_out);
+  count_launches(1);
+  return cudaGetLastError();
+}
+
+// The tokens behind the choice: the kernel begins while that still runs, and waits for it by itself.
+template <typename... Args>
+cudaError_t launch_move(void (*kernel)(Args...), dim3 grid, cudaStream_t stream, Args... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(kMoveThreads);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  count_launches(1);
+  return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
 }  // namespace
 
 int check_new_tokens(const char* what, const T5xNewTokens* n) {
@@ -268,12 +518,12 @@ T5X_API int t5x_cache8_evict(const T5xCache8* cache, const T5xCache8* into, int 
     return t5x::set_error("cache8_evict: %d of %d slots (the last %d) do not fit %d", keep, c.slots, recent, to.slots);
   if (c.batch == 0) return 0;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  t5x::cache8_select_kernel<<<static_cast<unsigned>(c.batch) * c.heads, t5x::kSelectThreads, 0, st>>>(
-      c, keep, recent, static_cast<int*>(kept));
-  const int blocks = (keep + (1 << to.block_log2) - 1) >> to.block_log2;
-  t5x::cache8_move_kernel<<<dim3(blocks, c.heads, c.batch), t5x::kMoveThreads, 0, st>>>(
-      c, to, keep, static_cast<const int*>(kept), static_cast<int*>(index_out), static_cast<int*>(dropped_out));
-  t5x::count_launches(2);
-  const cudaError_t e = cudaGetLastError();
+  cudaError_t e = t5x::launch_select(c, keep, recent, static_cast<int*>(kept), static_cast<int*>(index_out),
+                                     static_cast<int*>(dropped_out), st);
+  if (e == cudaSuccess) {
+    const dim3 grid((keep + (1 << to.block_log2) - 1) >> to.block_log2, c.heads, c.batch);
+    e = t5x::launch_move(c.dim == 64 ? t5x::cache8_move_kernel<64> : t5x::cache8_move_kernel<128>, grid, st, c, to, keep,
+                         static_cast<const int*>(kept));
+  }
   return e == cudaSuccess ? 0 : t5x::set_error("cache8_evict launch: %s", cudaGetErrorString(e));
 }

@@ -131,6 +131,14 @@ def test_evict(c, special):
   launches(lambda: plain.check_evict(c, "cuda", special))
 
 
+@pytest.mark.parametrize("slots,keep,recent", [(4096, 700, 33), (8192, 3000, 0), (16384, 129, 128), (20480, 517, 5),
+                                               (65536, 1000, 17), (66048, 257, 100)])
+@pytest.mark.parametrize("special", [False, True])
+def test_evict_from_long_caches(slots, keep, recent, special):
+  launches(lambda: plain.check_evict(dict(b=2, h=1, dim=64, slots=slots, block=64, starts=[slots - 7, slots // 2], keep=keep,
+                                          recent=recent, to_block=128), "cuda", special))
+
+
 @pytest.mark.parametrize("rows,k,n", [(1, 16, 8), (3, 17, 5), (5, 1, 3), (2, 300, 130), (33, 129, 257), (257, 64, 40),
                                       (130, 513, 300)])
 @pytest.mark.parametrize("dtype", TYPES)
