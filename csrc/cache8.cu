@@ -41,18 +41,25 @@ __device__ __forceinline__ uint32_t order_of(float w) {
   return u ^ (u >> 31 ? 0xffffffffu : 0x80000000u);
 }
 
-// Of the counts of 16 digits (lanes 0 to 15) the digit at which `need` of the largest are reached; need less those above it.
-__device__ __forceinline__ int border_digit(int count, int& need) {
-  const int lane = threadIdx.x & 31;
-  int from = lane < 16 ? count : 0;  // of this digit and those above
+// Of the counts of 256 digits the one at which `need` of the largest are reached; need less those above it. By a warp.
+__device__ __forceinline__ int border_digit(const int* counts, int& need) {
+  const int lane = threadIdx.x & 31, top = 255 - 8 * lane;  // this lane's digits: top .. top - 7
+  int mine[8], sum = 0;
 #pragma unroll
-  for (int o = 1; o < 16; o <<= 1) {
-    const int u = __shfl_down_sync(0xffffffffu, from, o);
-    if (lane + o < 16) from += u;
+  for (int i = 0; i < 8; ++i) sum += mine[i] = counts[top - i];
+  int run = sum;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int u = __shfl_up_sync(0xffffffffu, run, o);
+    if (lane >= o) run += u;
   }
-  const int digit = 31 - __clz(__ballot_sync(0xffffffffu, lane < 16 && from >= need) | 1);
-  need -= __shfl_sync(0xffffffffu, from - count, digit);
-  return digit;
+  const int who = __ffs(__ballot_sync(0xffffffffu, run >= need)) - 1;  // (there are so many: the last lane has all)
+  int above = run - sum, digit = top;
+#pragma unroll
+  for (int i = 0; i < 7; ++i)
+    if (digit == top - i && above + mine[i] < need) above += mine[i], --digit;
+  need -= __shfl_sync(0xffffffffu, above, who & 31);
+  return __shfl_sync(0xffffffffu, digit, who & 31);
 }
 
 __device__ __forceinline__ unsigned long long remote_u64(const unsigned long long* mine, uint32_t cta) {
@@ -67,14 +74,15 @@ __device__ __forceinline__ int remote_int(const int* mine, uint32_t cta) {
 }
 
 // A CTA, or a cluster, takes the slots of one head of one row and keeps its weights in registers, K a thread. The border is
-// found four bits at a time: a lane of each warp counts one of the 16 digits from the ballots of the four bits (no atomics
-// on a bin that most weights share: many are equal, or zero). A slot's place is the number of larger ones before it, and of
-// those at the border as far as they stay.
+// found eight bits at a time from counts of the digits; zeros, which may be most, are counted by ballot. A slot's place is the
+// number of larger ones before it, and of those at the border as far as they stay.
+constexpr uint32_t kZero = 0x80000000u;  // order_of(0)
+
 template <int T, int K, bool kCluster>
-__global__ void __launch_bounds__(T)
+__global__ void __launch_bounds__(T, 1024 / T)
     cache8_select_kernel(const __grid_constant__ Cache8 c, int keep, int recent, int ctas, int* __restrict__ kept,
                          int* __restrict__ index_out, int* __restrict__ dropped_out) {
-  __shared__ int s_hist[8][16];
+  __shared__ int s_hist[4][256], s_all[256];
   __shared__ unsigned long long s_before[K * T / 32 + 1];  // larger | at the border << 32, by row of T slots and warp
   constexpr int kWarps = T / 32;
   const long long bh = kCluster ? blockIdx.x / ctas : blockIdx.x;
@@ -100,38 +108,33 @@ __global__ void __launch_bounds__(T)
     const int s = first + i * T + threadIdx.x;
     key[i] = s < old ? order_of(w[s]) : 0;
   }
-  if (threadIdx.x < 128) s_hist[threadIdx.x / 16][threadIdx.x % 16] = 0;
+  for (int i = threadIdx.x; i < 1024; i += T) s_hist[i >> 8][i & 255] = 0;
   __syncthreads();
 
   int need = keep - recent;
   uint32_t border = 0;
   if (need > 0)
-    for (int round = 0; round < 8; ++round) {
-      const int shift = 28 - 4 * round;
-      int count = 0;
+    for (int round = 0; round < 4; ++round) {
+      const int shift = 24 - 8 * round;
+      int zeros = 0;
 #pragma unroll
       for (int i = 0; i < K; ++i) {
-        const bool in = first + i * T + static_cast<int>(threadIdx.x) < old && (round == 0 || ((key[i] ^ border) >> (shift + 4)) == 0);
-        uint32_t m = __ballot_sync(0xffffffffu, in);
-        if (m == 0) continue;
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const uint32_t set = __ballot_sync(0xffffffffu, (key[i] >> (shift + k)) & 1);
-          m &= (lane >> k) & 1 ? set : ~set;
+        const bool in = first + i * T + static_cast<int>(threadIdx.x) < old && (round == 0 || ((key[i] ^ border) >> (shift + 8)) == 0);
+        zeros += __popc(__ballot_sync(0xffffffffu, in && key[i] == kZero));
+        if (in && key[i] != kZero) atomicAdd(&s_hist[round][(key[i] >> shift) & 255], 1);
+      }
+      if (lane == 0 && zeros > 0) atomicAdd(&s_hist[round][(kZero >> shift) & 255], zeros);
+      if (kCluster) {
+        cluster_sync_all();
+        for (int i = threadIdx.x; i < 256; i += T) {
+          int all = 0;
+          for (int r = 0; r < ctas; ++r) all += remote_int(&s_hist[round][i], r);
+          s_all[i] = all;
         }
-        count += __popc(m);
       }
-      if (lane < 16 && count > 0) atomicAdd(&s_hist[round][lane], count);
-      if (kCluster) cluster_sync_all();
-      else __syncthreads();
-      int all = 0;
-      if (lane < 16) {
-        if (kCluster)
-          for (int r = 0; r < ctas; ++r) all += remote_int(&s_hist[round][lane], r);
-        else
-          all = s_hist[round][lane];
-      }
-      border |= static_cast<uint32_t>(border_digit(all, need)) << shift;
+      __syncthreads();
+      border |= static_cast<uint32_t>(border_digit(kCluster ? s_all : s_hist[round], need)) << shift;
+      if (kCluster) __syncthreads();  // (s_all is the next round's)
     }
   const int ties = need;  // of the slots at the border, the first so many stay
   const bool any = keep > recent;
@@ -282,29 +285,42 @@ __global__ void __launch_bounds__(kWalkThreads)
 
 // ---------------------------------------------------------------------------
 // Eviction: the tokens that stay. A CTA takes one block of one head of the smaller cache, 16 codes a thread at a time.
-// Tokens of a new block come from many old ones, so nearly all codes are rounded again; near a border between two codes
-// exactly, by Coder, and else by one product: 16 codes as numbers (a byte under the exponent of 2^23), times the ratio of the
-// scales, back under the exponent of 3 * 2^22, which rounds to whole numbers.
+// Tokens of a new block come from many old ones, so nearly all codes are rounded again, 16 at a time: as numbers (a byte under
+// the exponent of 2^23), times the ratio of the scales, back under the exponent of 3 * 2^22, which rounds to whole numbers. Near a
+// border between two codes as Coder does it.
 // ---------------------------------------------------------------------------
 constexpr int kMoveThreads = 256;
 
+__device__ __forceinline__ uint32_t low_bytes(const uint32_t (&r)[4]) {
+  return __byte_perm(__byte_perm(r[0], r[1], 0x0040), __byte_perm(r[2], r[3], 0x0040), 0x5410);
+}
+__device__ __forceinline__ float code_number(uint32_t w, int i) {
+  return __uint_as_float(__byte_perm(w ^ 0x80808080u, 0x4b000000u, 0x7440 + i)) - 8388736.f;
+}
+// with short scales (Coder)
+__device__ __forceinline__ uint32_t round_four(uint32_t w, float ratio) {
+  uint32_t r[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) r[i] = __float_as_uint(in_21_bits(code_number(w, i) * ratio) + 12582912.f);
+  return low_bytes(r);
+}
+// with any; off: how far a quotient is from its code
 __device__ __forceinline__ uint32_t round_four(uint32_t w, float ratio, float& off) {
   uint32_t r[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const float x = __uint_as_float(__byte_perm(w ^ 0x80808080u, 0x4b000000u, 0x7440 + i)) - 8388736.f;
-    const float q = x * ratio, up = q + 12582912.f;
+    const float q = code_number(w, i) * ratio, up = q + 12582912.f;
     off = fmaxf(off, fabsf(q - (up - 12582912.f)));
     r[i] = __float_as_uint(up);
   }
-  return __byte_perm(__byte_perm(r[0], r[1], 0x0040), __byte_perm(r[2], r[3], 0x0040), 0x5410);
+  return low_bytes(r);
 }
 
 __device__ __forceinline__ uint32_t round_four_exactly(uint32_t w, const Coder& again) {
   uint32_t r = 0;
 #pragma unroll
   for (int i = 0; i < 4; ++i)
-    r |= static_cast<uint32_t>(again(static_cast<float>(static_cast<int8_t>(w >> (8 * i)))) & 0xff) << (8 * i);
+    r |= static_cast<uint32_t>(again.of<true>(static_cast<float>(static_cast<int8_t>(w >> (8 * i)))) & 0xff) << (8 * i);
   return r;
 }
 
@@ -314,14 +330,14 @@ __global__ void __launch_bounds__(kMoveThreads)
                        const int* __restrict__ kept) {
   __shared__ int s_from[128];
   __shared__ float s_old[2][128], s_ratio[2][128];
-  __shared__ uint32_t s_most[2];
+  __shared__ uint32_t s_most[2], s_bits[2];
   const int b = blockIdx.z, h = blockIdx.y, blk = blockIdx.x;
   const int n = min(held_of(c, b), keep);
   const int lo = blk << to.block_log2, count = min(1 << to.block_log2, n - lo);
   const long long bh = static_cast<long long>(b) * c.heads + h;
   chain_wait();
   if (count <= 0) return;
-  if (threadIdx.x < 2) s_most[threadIdx.x] = 0;
+  if (threadIdx.x < 2) s_most[threadIdx.x] = s_bits[threadIdx.x] = 0;
   if (static_cast<int>(threadIdx.x) < count) s_from[threadIdx.x] = __ldcg(kept + bh * keep + lo + threadIdx.x);
   __syncthreads();
 
@@ -340,8 +356,8 @@ __global__ void __launch_bounds__(kMoveThreads)
     float old = 0.f;
     if (i < count) old = c.absmax[what][bh * (c.slots >> c.block_log2) + (s_from[i] >> c.block_log2)];
     s_old[what][i] = old;
-    const uint32_t most = __reduce_max_sync(0xffffffffu, abs_bits(old));
-    if ((threadIdx.x & 31) == 0) atomicMax(&s_most[what], most);
+    const uint32_t most = __reduce_max_sync(0xffffffffu, abs_bits(old)), bits = __reduce_or_sync(0xffffffffu, abs_bits(old));
+    if ((threadIdx.x & 31) == 0) atomicMax(&s_most[what], most), atomicOr(&s_bits[what], bits);
     __syncthreads();
     const float a = __uint_as_float(s_most[what]);
     // -1: as it is; -2: by Coder
@@ -356,6 +372,7 @@ __global__ void __launch_bounds__(kMoveThreads)
 #pragma unroll
   for (int what = 0; what < 2; ++what) {
     const float a = __uint_as_float(s_most[what]);
+    const bool brief = (s_bits[what] & 0x1fffu) == 0;
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int i = tok + u * kTokens;
@@ -363,6 +380,11 @@ __global__ void __launch_bounds__(kMoveThreads)
       const float ratio = s_ratio[what][i];
       if (ratio != -1.f) {
         float off = ratio < 0.f ? 1.f : 0.f;
+        if (brief && ratio >= 0.f) {
+          v[u] = make_uint4(round_four(v[u].x, ratio), round_four(v[u].y, ratio), round_four(v[u].z, ratio), round_four(v[u].w, ratio));
+          *(reinterpret_cast<uint4*>(to.codes[what] + (bh * to.slots + lo + i) * D) + part) = v[u];
+          continue;
+        }
         const uint4 o = make_uint4(round_four(v[u].x, ratio, off), round_four(v[u].y, ratio, off), round_four(v[u].z, ratio, off),
                                    round_four(v[u].w, ratio, off));
         if (off < 0.4999f) {
@@ -454,7 +476,7 @@ cudaError_t launch_select_by(int ctas, const Cache8& c, int keep, int recent, in
 cudaError_t launch_select(const Cache8& c, int keep, int recent, int* kept, int* index_out, int* dropped_out, cudaStream_t stream) {
   const int ctas = c.slots <= 2048 ? 1 : c.slots <= 4096 ? 2 : c.slots <= 8192 ? 4 : 8;
   if (c.slots <= 2048 * 8) return launch_select_by<256, 8>(ctas, c, keep, recent, kept, index_out, dropped_out, stream);
-  if (c.slots <= 8192 * 8) return launch_select_by<1024, 8>(8, c, keep, recent, kept, index_out, dropped_out, stream);
+  if (c.slots <= 8192 * 8) return launch_select_by<512, 16>(8, c, keep, recent, kept, index_out, dropped_out, stream);
   cache8_select_walk_kernel<<<static_cast<unsigned>(c.batch) * c.heads, kWalkThreads, 0, stream>>>(c, keep, recent, kept, index_out,
                                                                                                dropped_out);
   count_launches(1);

@@ -27,16 +27,28 @@ struct Cache8 {
   int block_log2;
 };
 
+// Whether a number has at most 11 bits, as the values of 16-bit types have (and the largest of them).
+__device__ __forceinline__ bool is_short(float x) { return (__float_as_uint(x) & 0x1fffu) == 0; }
+
 // The code of u * num / a, rounded to the nearest whole number (ties to even), in a block of largest value a: of the value
-// u with num = 127, of an older code u with num = the largest value it was relative to. One multiplication by num / a is
-// at most 4e-5 off; where that may decide, the quotient is taken in 64 bits, where it cannot round to the other side of
-// a border (u * num has 31 bits, a has 24, so they differ by 2^-25 at least).
+// u with num = 127, of an older code u with num = the largest value it was relative to. u * (num / a) is at most 4e-5 off.
+//
+// Where u, num and a are short (a code is), a quotient that is not itself on a border between two codes is more than 2^-20 of
+// itself away from it: with whole numbers U, N, A below 2^11 it is U N 2^-s / A, a border is (2 k + 1) / 2, and
+// they differ by 2^-s / 2 A at least, 1 / (2 U N) of the quotient, where 127 or a code is the other factor. The product, two
+// steps of 24 bits off at most, is brought to 21 bits first, which puts those on a border there and leaves the others on
+// their side. Elsewhere a quotient near a border is taken in 64 bits, where it cannot round to the other side (u * num has
+// 31 bits, a has 24: they differ by 2^-25 at least).
+__device__ __forceinline__ float in_21_bits(float q) { return __uint_as_float((__float_as_uint(q) + 4u) & ~7u); }
+
 struct Coder {
   float num, a, factor;
   bool plain;  // a lies where neither the factor nor a product leaves the normal numbers
+  bool brief;  // num and a are short; for u the caller knows
 
   __device__ __forceinline__ Coder(float num_, float a_) : num(num_), a(a_) {
     plain = a >= 0x1p-60f && a <= 0x1p100f;
+    brief = plain && is_short(num) && is_short(a);
     factor = plain ? __fdiv_rn(num, a) : 0.f;
   }
   __device__ __noinline__ static int exactly(float u, float num, float a) {
@@ -47,7 +59,10 @@ struct Coder {
     const double q = x * y / z;
     return q == q ? __double2int_rn(fmin(fmax(q, -127.0), 127.0)) : 0;
   }
-  __device__ __forceinline__ int operator()(float u) const {
+  // kShort: u is short
+  template <bool kShort>
+  __device__ __forceinline__ int of(float u) const {
+    if (kShort && brief) return __float_as_int(in_21_bits(u * factor) + 12582912.f) - 0x4b400000;  // (3 * 2^22: steps of one)
     const float q = u * factor, r = rintf(q);
     if (!plain || fabsf(fabsf(q - r) - 0.5f) < 1e-4f) return exactly(u, num, a);
     return static_cast<int>(r);
@@ -139,15 +154,17 @@ __device__ __forceinline__ void append_block(const Cache8& c, const NewTokens<T>
     for (int s = first + from; s < lo; s += step) {
       char4* at = reinterpret_cast<char4*>(codes + static_cast<long long>(s) * D + d);
       const char4 v = *at;
-      *at = make_char4(again(v.x), again(v.y), again(v.z), again(v.w));
+      *at = make_char4(again.of<true>(v.x), again.of<true>(v.y), again.of<true>(v.z), again.of<true>(v.w));
     }
   }
+  constexpr bool kShort = sizeof(T) == 2;
   const Coder code(127.f, a);
 #pragma unroll 2
   for (int s = lo + from; s < hi; s += step) {
     float v[4];
     load_four(x + (s - start) * st + d, vec, v);
-    *reinterpret_cast<char4*>(codes + static_cast<long long>(s) * D + d) = make_char4(code(v[0]), code(v[1]), code(v[2]), code(v[3]));
+    *reinterpret_cast<char4*>(codes + static_cast<long long>(s) * D + d) = make_char4(code.of<kShort>(v[0]), code.of<kShort>(v[1]), code.of<kShort>(v[2]),
+                                                                                                 code.of<kShort>(v[3]));
   }
   if (what == 0)
     for (int s = lo + tid; s < hi; s += THREADS) {

@@ -420,13 +420,15 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 16 / kWarps : 1)
           for (int s = touched + own; s < start; s += kHalf / kLanes) {
             char4* to = reinterpret_cast<char4*>(codes + static_cast<long long>(s) * D);
             const char4 u = *to;
-            *to = make_char4(again(u.x), again(u.y), again(u.z), again(u.w));
+            *to = make_char4(again.of<true>(u.x), again.of<true>(u.y), again.of<true>(u.z), again.of<true>(u.w));
           }
         }
         if (tid == 0) *most_at = a;
         if (own < end - start) {
+          constexpr bool kShort = sizeof(T) == 2;
           const Coder code(127.f, a);
-          *reinterpret_cast<char4*>(codes + static_cast<long long>(start + own) * D) = make_char4(code(v[0]), code(v[1]), code(v[2]), code(v[3]));
+          *reinterpret_cast<char4*>(codes + static_cast<long long>(start + own) * D) = 
+              make_char4(code.of<kShort>(v[0]), code.of<kShort>(v[1]), code.of<kShort>(v[2]), code.of<kShort>(v[3]));
           if (half == 0 && d == 0) {
             if (c.weight != nullptr) c.weight[slots0 + start + own] = 0.f;
             if (c.position != nullptr) c.position[slots0 + start + own] = start + own + c.dropped[b];

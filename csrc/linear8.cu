@@ -58,7 +58,7 @@ __global__ void __launch_bounds__(kRowThreads)
   const float a = __uint_as_float(most);
   const Coder code(127.f, a);
   for (int i = threadIdx.x; i < ld; i += kRowThreads)
-    codes[row * ld + i] = static_cast<int8_t>(i < k ? code(to_float(src[i])) : 0);
+    codes[row * ld + i] = static_cast<int8_t>(i < k ? code.template of<sizeof(T) == 2>(to_float(src[i])) : 0);
   if (threadIdx.x == 0) absmax[row] = a;
 }
 

@@ -71,6 +71,36 @@ def test_codes_at_every_border():
   assert torch.equal(codes.cpu(), want) and torch.equal(absmax.cpu(), size)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_codes_of_all_short_values(dtype):
+  """Every positive value of a 16-bit type below each of many largest ones, and every code by many ratios of scales: where the
+  quotient is on a border, and next to it."""
+  bits = torch.arange(0x7f80 if dtype == torch.bfloat16 else 0x7c00, dtype=torch.int32)
+  values = bits.to(torch.int16).view(dtype)
+  one = torch.finfo(dtype).eps
+  ends = torch.cat([1 + one * torch.arange(0, int(1 / one), 1 if dtype == torch.bfloat16 else 37), torch.tensor([2.0])]).to(dtype)
+  near = values[(values.float() > 2.0 ** -9) & (values.float() <= 2)]
+  x = torch.where(near[None] <= ends[:, None], near[None], torch.zeros((), dtype=dtype))
+  x[:, -1] = ends
+  codes, most = native.quantize_rows(x.cuda(), x.shape[1])
+  assert torch.equal(most.cpu(), ends.float())
+  assert torch.equal(codes, ref.codes_of(x.cuda().float(), 127, most[:, None]))
+  # one token with each of 127 codes, moved into a block with one of a larger scale
+  n = ends.numel() // 2 * 2
+  cache = cache8.init_cache(n, 32, 1, 128, "cuda", block=16, weights=True)
+  for k in ("key", "value"):
+    cache["cached_" + k][:, 0, 0] = torch.arange(128)
+    cache[k + "_absmax"][:, 0, 0] = ends[:n].float().cuda()
+    cache[k + "_absmax"][:, 0, 1] = ends[:n].float().cuda().roll(n // 3) * 2
+  cache["cache_index"].fill_(17)
+  cache["token_weight"][:, :, 0] = 1.0
+  small, _ = cache8.evict(cache, 2, recent=1)
+  old, new = cache["key_absmax"][:, 0, 0], cache["key_absmax"][:, 0, 1]
+  want = ref.codes_of(old[:, None], cache["cached_key"][:, 0, 0], torch.maximum(old, new)[:, None])
+  want = torch.where((old >= new)[:, None], cache["cached_key"][:, 0, 0], want)
+  assert torch.equal(small["cached_key"][:, 0, 0], want) and torch.equal(small["cached_value"][:, 0, 0], want)
+
+
 @pytest.mark.parametrize("bad", [math.inf, -math.inf, math.nan])
 @pytest.mark.parametrize("dtype", TYPES)
 def test_values_that_are_not_finite(bad, dtype):
