@@ -45,8 +45,11 @@ __device__ __forceinline__ uint32_t order_of(float w) {
 __device__ __forceinline__ int border_digit(const int* counts, int& need) {
   const int lane = threadIdx.x & 31, top = 255 - 8 * lane;  // this lane's digits: top .. top - 7
   int mine[8], sum = 0;
+  const int4 high = reinterpret_cast<const int4*>(counts)[63 - 2 * lane], low = reinterpret_cast<const int4*>(counts)[62 - 2 * lane];
+  mine[0] = high.w, mine[1] = high.z, mine[2] = high.y, mine[3] = high.x;
+  mine[4] = low.w, mine[5] = low.z, mine[6] = low.y, mine[7] = low.x;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) sum += mine[i] = counts[top - i];
+  for (int i = 0; i < 8; ++i) sum += mine[i];
   int run = sum;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -73,19 +76,28 @@ __device__ __forceinline__ int remote_int(const int* mine, uint32_t cta) {
   return v;
 }
 
+__device__ __forceinline__ void remote_add(int* mine, int v) {  // to the cluster's first CTA
+  asm volatile("red.relaxed.cluster.shared::cluster.add.s32 [%0], %1;" ::"r"(mapa_shared(smem_u32(mine), 0)), "r"(v) : "memory");
+}
+
 // A CTA, or a cluster, takes the slots of one head of one row and keeps its weights in registers, K a thread. The border is
-// found eight bits at a time from counts of the digits; zeros, which may be most, are counted by ballot. A slot's place is the
+// found eight bits at a time from counts of the digits, behind the first of those alone that are at the border so far;
+// zeros, which may be most, are counted by ballot. A slot's place is the
 // number of larger ones before it, and of those at the border as far as they stay.
 constexpr uint32_t kZero = 0x80000000u;  // order_of(0)
 
-template <int T, int K, bool kCluster>
+template <int T, int K, int kCtas>
 __global__ void __launch_bounds__(T, 1024 / T)
-    cache8_select_kernel(const __grid_constant__ Cache8 c, int keep, int recent, int ctas, int* __restrict__ kept,
+    cache8_select_kernel(const __grid_constant__ Cache8 c, int keep, int recent, int* __restrict__ kept,
                          int* __restrict__ index_out, int* __restrict__ dropped_out) {
-  __shared__ int s_hist[4][256], s_all[256];
+  __shared__ __align__(16) int s_hist[4][256];
+  __shared__ uint32_t s_list[T * K];
+  __shared__ int s_left;
+  __shared__ __align__(16) int s_all[4][256];  // a cluster's sums, in its first CTA; here the copy that is looked at
   __shared__ unsigned long long s_before[K * T / 32 + 1];  // larger | at the border << 32, by row of T slots and warp
   constexpr int kWarps = T / 32;
-  const long long bh = kCluster ? blockIdx.x / ctas : blockIdx.x;
+  constexpr bool kCluster = kCtas > 1;
+  const long long bh = blockIdx.x / kCtas;
   const uint32_t rank = kCluster ? cluster_ctarank() : 0;
   const int b = static_cast<int>(bh / c.heads);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -98,7 +110,7 @@ __global__ void __launch_bounds__(T, 1024 / T)
     dropped_out[b] = (c.position != nullptr ? c.dropped[b] : 0) + (index - min(held, keep));
   }
   if (held <= keep) {
-    for (int i = rank * T + threadIdx.x; i < keep; i += T * ctas) out[i] = i < held ? i : -1;
+    for (int i = rank * T + threadIdx.x; i < keep; i += T * kCtas) out[i] = i < held ? i : -1;
     return;
   }
   const int old = held - recent, first = static_cast<int>(rank) * (T * K);  // slots to choose from; this CTA's first
@@ -108,8 +120,10 @@ __global__ void __launch_bounds__(T, 1024 / T)
     const int s = first + i * T + threadIdx.x;
     key[i] = s < old ? order_of(w[s]) : 0;
   }
-  for (int i = threadIdx.x; i < 1024; i += T) s_hist[i >> 8][i & 255] = 0;
-  __syncthreads();
+  for (int i = threadIdx.x; i < 1024; i += T) s_hist[i >> 8][i & 255] = s_all[i >> 8][i & 255] = 0;
+  if (threadIdx.x == 0) s_left = 0;
+  if (kCluster) cluster_sync_all();
+  else __syncthreads();
 
   int need = keep - recent;
   uint32_t border = 0;
@@ -117,24 +131,41 @@ __global__ void __launch_bounds__(T, 1024 / T)
     for (int round = 0; round < 4; ++round) {
       const int shift = 24 - 8 * round;
       int zeros = 0;
+      auto count = [&](bool in, uint32_t u) {
+        zeros += __popc(__ballot_sync(0xffffffffu, in && u == kZero));
+        if (in && u != kZero) atomicAdd(&s_hist[round][(u >> shift) & 255], 1);
+      };
+      if (round == 0) {
 #pragma unroll
-      for (int i = 0; i < K; ++i) {
-        const bool in = first + i * T + static_cast<int>(threadIdx.x) < old && (round == 0 || ((key[i] ^ border) >> (shift + 8)) == 0);
-        zeros += __popc(__ballot_sync(0xffffffffu, in && key[i] == kZero));
-        if (in && key[i] != kZero) atomicAdd(&s_hist[round][(key[i] >> shift) & 255], 1);
-      }
-      if (lane == 0 && zeros > 0) atomicAdd(&s_hist[round][(kZero >> shift) & 255], zeros);
-      if (kCluster) {
-        cluster_sync_all();
-        for (int i = threadIdx.x; i < 256; i += T) {
-          int all = 0;
-          for (int r = 0; r < ctas; ++r) all += remote_int(&s_hist[round][i], r);
-          s_all[i] = all;
+        for (int i = 0; i < K; ++i) count(first + i * T + static_cast<int>(threadIdx.x) < old, key[i]);
+      } else {
+        for (int j = threadIdx.x; j - lane < s_left; j += T) {
+          const uint32_t u = j < s_left ? s_list[j] : 0;
+          count(j < s_left && ((u ^ border) >> (shift + 8)) == 0, u);
         }
       }
+      if (lane == 0 && zeros > 0) atomicAdd(&s_hist[round][(kZero >> shift) & 255], zeros);
       __syncthreads();
-      border |= static_cast<uint32_t>(border_digit(kCluster ? s_all : s_hist[round], need)) << shift;
-      if (kCluster) __syncthreads();  // (s_all is the next round's)
+      if (kCluster) {  // the few digits that occur, to the first CTA
+        for (int i = threadIdx.x; i < 256; i += T)
+          if (s_hist[round][i] != 0) remote_add(&s_all[round][i], s_hist[round][i]);
+        cluster_sync_all();
+        for (int i = threadIdx.x; i < 256; i += T) s_hist[round][i] = remote_int(&s_all[round][i], 0);
+        __syncthreads();
+      }
+      border |= static_cast<uint32_t>(border_digit(s_hist[round], need)) << shift;
+      if (round == 0) {  // those at the border so far
+#pragma unroll
+        for (int i = 0; i < K; ++i) {
+          const bool in = first + i * T + static_cast<int>(threadIdx.x) < old && (key[i] ^ border) >> 24 == 0;
+          const uint32_t who = __ballot_sync(0xffffffffu, in);
+          int at = 0;
+          if (who != 0 && lane == 0) at = atomicAdd(&s_left, __popc(who));
+          at = __shfl_sync(0xffffffffu, at, 0) + __popc(who & ((1u << lane) - 1));
+          if (in) s_list[at] = key[i];
+        }
+        __syncthreads();
+      }
     }
   const int ties = need;  // of the slots at the border, the first so many stay
   const bool any = keep > recent;
@@ -173,7 +204,11 @@ __global__ void __launch_bounds__(T, 1024 / T)
   unsigned long long base = 0;
   if (kCluster) {
     cluster_sync_all();
-    for (int r = 0; r < static_cast<int>(rank); ++r) base += remote_u64(&s_before[K * kWarps], r);
+#pragma unroll
+    for (int r = 0; r < kCtas; ++r) {
+      const unsigned long long u = remote_u64(&s_before[K * kWarps], r);
+      if (r < static_cast<int>(rank)) base += u;
+    }
   } else {
     __syncthreads();
   }
@@ -284,12 +319,12 @@ __global__ void __launch_bounds__(kWalkThreads)
 }
 
 // ---------------------------------------------------------------------------
-// Eviction: the tokens that stay. A CTA takes one block of one head of the smaller cache, 16 codes a thread at a time.
+// Eviction: the tokens that stay. A warp takes up to 32 tokens of one block of one head of the smaller cache.
 // Tokens of a new block come from many old ones, so nearly all codes are rounded again, 16 at a time: as numbers (a byte under
 // the exponent of 2^23), times the ratio of the scales, back under the exponent of 3 * 2^22, which rounds to whole numbers. Near a
 // border between two codes as Coder does it.
 // ---------------------------------------------------------------------------
-constexpr int kMoveThreads = 256;
+constexpr int kMoveThreads = 128;
 
 __device__ __forceinline__ uint32_t low_bytes(const uint32_t (&r)[4]) {
   return __byte_perm(__byte_perm(r[0], r[1], 0x0040), __byte_perm(r[2], r[3], 0x0040), 0x5410);
@@ -324,80 +359,92 @@ __device__ __forceinline__ uint32_t round_four_exactly(uint32_t w, const Coder& 
   return r;
 }
 
+// What a token's codes go through: their scale is the block's (kAsIs), else times the ratio of the two.
+constexpr float kAsIs = -1.f, kByCoder = -2.f;
+__device__ __forceinline__ float ratio_of(float old, float a) {
+  if (abs_bits(old) == abs_bits(a)) return kAsIs;
+  return a >= 0x1p-60f && a <= 0x1p100f ? __fdiv_rn(old, a) : kByCoder;
+}
+
 template <int D>
 __global__ void __launch_bounds__(kMoveThreads)
     cache8_move_kernel(const __grid_constant__ Cache8 c, const __grid_constant__ Cache8 to, int keep,
                        const int* __restrict__ kept) {
-  __shared__ int s_from[128];
-  __shared__ float s_old[2][128], s_ratio[2][128];
-  __shared__ uint32_t s_most[2], s_bits[2];
-  const int b = blockIdx.z, h = blockIdx.y, blk = blockIdx.x;
+  constexpr int L = D / 16, kTokens = 32 / L, U = 4;  // lanes a token, tokens at a time, turns requested at a time
+  const int b = blockIdx.z, h = blockIdx.y, lane = threadIdx.x & 31;
+  const int block = 1 << to.block_log2, span = min(block, 32);
+  const int lo = (blockIdx.x * (kMoveThreads / 32) + (threadIdx.x >> 5)) * span;  // this warp's first token
   const int n = min(held_of(c, b), keep);
-  const int lo = blk << to.block_log2, count = min(1 << to.block_log2, n - lo);
-  const long long bh = static_cast<long long>(b) * c.heads + h;
   chain_wait();
-  if (count <= 0) return;
-  if (threadIdx.x < 2) s_most[threadIdx.x] = s_bits[threadIdx.x] = 0;
-  if (static_cast<int>(threadIdx.x) < count) s_from[threadIdx.x] = __ldcg(kept + bh * keep + lo + threadIdx.x);
-  __syncthreads();
+  if (lo >= n) return;
+  const int first = lo & ~(block - 1), count = min(block, n - first), mine = min(span, n - lo);
+  const long long bh = static_cast<long long>(b) * c.heads + h;
+  const int* from = kept + bh * keep + first;
 
-  constexpr int L = D / 16, kTokens = kMoveThreads / L, U = 128 / kTokens;  // threads a token, tokens at a time, turns
-  const int tok = threadIdx.x / L, part = threadIdx.x % L;
-  uint4 v[U];
-  auto load = [&](int what) {
+  // the block's scale; lane i's token is lo + i
+  int slot = 0;
+  float old[2] = {0.f, 0.f};
+  uint32_t most[2] = {0, 0}, bits[2] = {0, 0};
+  for (int j0 = 0; j0 < count; j0 += 32) {
+    const int j = j0 + lane;
+    const int s = j < count ? __ldcg(from + j) : 0;
 #pragma unroll
-    for (int u = 0; u < U; ++u)
-      if (tok + u * kTokens < count)
-        v[u] = *(reinterpret_cast<const uint4*>(c.codes[what] + (bh * c.slots + s_from[tok + u * kTokens]) * D) + part);
-  };
-  load(0);
-  {  // scales: keys' by one half of the threads, values' by the other
-    const int what = threadIdx.x >> 7, i = threadIdx.x & 127;
-    float old = 0.f;
-    if (i < count) old = c.absmax[what][bh * (c.slots >> c.block_log2) + (s_from[i] >> c.block_log2)];
-    s_old[what][i] = old;
-    const uint32_t most = __reduce_max_sync(0xffffffffu, abs_bits(old)), bits = __reduce_or_sync(0xffffffffu, abs_bits(old));
-    if ((threadIdx.x & 31) == 0) atomicMax(&s_most[what], most), atomicOr(&s_bits[what], bits);
-    __syncthreads();
-    const float a = __uint_as_float(s_most[what]);
-    // -1: as it is; -2: by Coder
-    s_ratio[what][i] = abs_bits(old) == s_most[what] ? -1.f : a >= 0x1p-60f && a <= 0x1p100f ? __fdiv_rn(old, a) : -2.f;
-    if (i == 0) to.absmax[what][bh * (to.slots >> to.block_log2) + blk] = a;
-    if (what == 0 && i < count) {
-      to.weight[bh * to.slots + lo + i] = c.weight[bh * c.slots + s_from[i]];
-      to.position[bh * to.slots + lo + i] = c.position != nullptr ? c.position[bh * c.slots + s_from[i]] : s_from[i];
+    for (int what = 0; what < 2; ++what) {
+      const float x = j < count ? c.absmax[what][bh * (c.slots >> c.block_log2) + (s >> c.block_log2)] : 0.f;
+      most[what] = max(most[what], abs_bits(x));
+      bits[what] |= abs_bits(x);
+      if (j0 == ((lo - first) & ~31)) old[what] = x;
     }
-    __syncthreads();
+    if (j0 == ((lo - first) & ~31)) slot = s;
   }
+  float a[2], ratio[2];
+  bool brief[2];
 #pragma unroll
   for (int what = 0; what < 2; ++what) {
-    const float a = __uint_as_float(s_most[what]);
-    const bool brief = (s_bits[what] & 0x1fffu) == 0;
+    a[what] = __uint_as_float(__reduce_max_sync(0xffffffffu, most[what]));
+    brief[what] = (__reduce_or_sync(0xffffffffu, bits[what]) & 0x1fffu) == 0;
+    ratio[what] = ratio_of(old[what], a[what]);
+    if (lo == first && lane == 0) to.absmax[what][bh * (to.slots >> to.block_log2) + (first >> to.block_log2)] = a[what];
+  }
+  if (lane < mine) {
+    to.weight[bh * to.slots + lo + lane] = c.weight[bh * c.slots + slot];
+    to.position[bh * to.slots + lo + lane] = c.position != nullptr ? c.position[bh * c.slots + slot] : slot;
+  }
+
+  const int tok = lane / L, part = lane % L;
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int i = tok + u * kTokens;
-      if (i >= count) continue;
-      const float ratio = s_ratio[what][i];
-      if (ratio != -1.f) {
-        float off = ratio < 0.f ? 1.f : 0.f;
-        if (brief && ratio >= 0.f) {
-          v[u] = make_uint4(round_four(v[u].x, ratio), round_four(v[u].y, ratio), round_four(v[u].z, ratio), round_four(v[u].w, ratio));
-          *(reinterpret_cast<uint4*>(to.codes[what] + (bh * to.slots + lo + i) * D) + part) = v[u];
-          continue;
-        }
-        const uint4 o = make_uint4(round_four(v[u].x, ratio, off), round_four(v[u].y, ratio, off), round_four(v[u].z, ratio, off),
-                                   round_four(v[u].w, ratio, off));
-        if (off < 0.4999f) {
-          v[u] = o;
-        } else {
-          const Coder again(s_old[what][i], a);
-          v[u] = make_uint4(round_four_exactly(v[u].x, again), round_four_exactly(v[u].y, again),
-                            round_four_exactly(v[u].z, again), round_four_exactly(v[u].w, again));
-        }
+  for (int what = 0; what < 2; ++what) {
+    const int8_t* src = c.codes[what] + bh * c.slots * D + 16 * part;
+    int8_t* dst = to.codes[what] + (bh * to.slots + lo) * D + 16 * part;
+    for (int i0 = 0; i0 < mine; i0 += U * kTokens) {
+      uint4 v[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int i = i0 + u * kTokens + tok, s = __shfl_sync(0xffffffffu, slot, i & 31);
+        if (i < mine) v[u] = *reinterpret_cast<const uint4*>(src + static_cast<long long>(s) * D);
       }
-      *(reinterpret_cast<uint4*>(to.codes[what] + (bh * to.slots + lo + i) * D) + part) = v[u];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int i = i0 + u * kTokens + tok;
+        const float r = __shfl_sync(0xffffffffu, ratio[what], i & 31), before = __shfl_sync(0xffffffffu, old[what], i & 31);
+        if (i >= mine) continue;
+        uint4 o = v[u];
+        if (r != kAsIs) {
+          float off = 0.f;
+          if (brief[what] && r != kByCoder) {
+            o = make_uint4(round_four(o.x, r), round_four(o.y, r), round_four(o.z, r), round_four(o.w, r));
+          } else {
+            o = make_uint4(round_four(o.x, r, off), round_four(o.y, r, off), round_four(o.z, r, off), round_four(o.w, r, off));
+            if (r == kByCoder || off >= 0.4999f) {
+              const Coder again(before, a[what]);
+              o = make_uint4(round_four_exactly(v[u].x, again), round_four_exactly(v[u].y, again),
+                             round_four_exactly(v[u].z, again), round_four_exactly(v[u].w, again));
+            }
+          }
+        }
+        *reinterpret_cast<uint4*>(dst + i * D) = o;
+      }
     }
-    if (what == 0) load(1);
   }
 }
 
@@ -454,29 +501,31 @@ int launch_append(const Cache8& c, const T5xNewTokens* in, cudaStream_t stream) 
   return e == cudaSuccess ? 0 : set_error("cache8_append launch: %s", cudaGetErrorString(e));
 }
 
-template <int T, int K>
-cudaError_t launch_select_by(int ctas, const Cache8& c, int keep, int recent, int* kept, int* index_out, int* dropped_out,
+template <int T, int K, int kCtas>
+cudaError_t launch_select_by(const Cache8& c, int keep, int recent, int* kept, int* index_out, int* dropped_out,
                              cudaStream_t stream) {
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(c.batch) * c.heads * ctas);
+  cfg.gridDim = dim3(static_cast<unsigned>(c.batch) * c.heads * kCtas);
   cfg.blockDim = dim3(T);
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = ctas;
+  attr[0].val.clusterDim.x = kCtas;
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = ctas > 1 ? 1 : 0;
+  cfg.numAttrs = kCtas > 1 ? 1 : 0;
   count_launches(1);
-  return cudaLaunchKernelEx(&cfg, ctas > 1 ? cache8_select_kernel<T, K, true> : cache8_select_kernel<T, K, false>, c, keep, recent,
-                            ctas, kept, index_out, dropped_out);
+  return cudaLaunchKernelEx(&cfg, cache8_select_kernel<T, K, kCtas>, c, keep, recent, kept, index_out, dropped_out);
 }
 
 // The weights of a head in the registers of one CTA up to 2048 slots, of up to eight up to 65536.
 cudaError_t launch_select(const Cache8& c, int keep, int recent, int* kept, int* index_out, int* dropped_out, cudaStream_t stream) {
-  const int ctas = c.slots <= 2048 ? 1 : c.slots <= 4096 ? 2 : c.slots <= 8192 ? 4 : 8;
-  if (c.slots <= 2048 * 8) return launch_select_by<256, 8>(ctas, c, keep, recent, kept, index_out, dropped_out, stream);
-  if (c.slots <= 8192 * 8) return launch_select_by<512, 16>(8, c, keep, recent, kept, index_out, dropped_out, stream);
+  auto by = [&](auto launch) { return launch(c, keep, recent, kept, index_out, dropped_out, stream); };
+  if (c.slots <= 2048) return by(launch_select_by<256, 8, 1>);
+  if (c.slots <= 4096) return by(launch_select_by<256, 8, 2>);
+  if (c.slots <= 8192) return by(launch_select_by<256, 8, 4>);
+  if (c.slots <= 16384) return by(launch_select_by<256, 8, 8>);
+  if (c.slots <= 65536) return by(launch_select_by<256, 32, 8>);
   cache8_select_walk_kernel<<<static_cast<unsigned>(c.batch) * c.heads, kWalkThreads, 0, stream>>>(c, keep, recent, kept, index_out,
                                                                                                dropped_out);
   count_launches(1);
@@ -543,7 +592,8 @@ T5X_API int t5x_cache8_evict(const T5xCache8* cache, const T5xCache8* into, int 
   cudaError_t e = t5x::launch_select(c, keep, recent, static_cast<int*>(kept), static_cast<int*>(index_out),
                                      static_cast<int*>(dropped_out), st);
   if (e == cudaSuccess) {
-    const dim3 grid((keep + (1 << to.block_log2) - 1) >> to.block_log2, c.heads, c.batch);
+    const int tokens = std::min(1 << to.block_log2, 32) * (t5x::kMoveThreads / 32);  // of a CTA
+    const dim3 grid((keep + tokens - 1) / tokens, c.heads, c.batch);
     e = t5x::launch_move(c.dim == 64 ? t5x::cache8_move_kernel<64> : t5x::cache8_move_kernel<128>, grid, st, c, to, keep,
                          static_cast<const int*>(kept));
   }

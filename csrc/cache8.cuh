@@ -39,7 +39,10 @@ __device__ __forceinline__ bool is_short(float x) { return (__float_as_uint(x) &
 // steps of 24 bits off at most, is brought to 21 bits first, which puts those on a border there and leaves the others on
 // their side. Elsewhere a quotient near a border is taken in 64 bits, where it cannot round to the other side (u * num has
 // 31 bits, a has 24: they differ by 2^-25 at least).
-__device__ __forceinline__ float in_21_bits(float q) { return __uint_as_float((__float_as_uint(q) + 4u) & ~7u); }
+__device__ __forceinline__ float in_21_bits(float q) {
+  const float high = __fmul_rn(q, 9.f);
+  return __fsub_rn(high, __fsub_rn(high, q));
+}
 
 struct Coder {
   float num, a, factor;
