@@ -14,6 +14,7 @@
 #include <torch/extension.h>
 
 #include <algorithm>
+#include <array>
 #include <cstring>
 #include <functional>
 #include <memory>
@@ -1123,6 +1124,196 @@ std::vector<Tensor> preference_loss(const Tensor& x, const optional<Tensor>& tar
   });
 }
 
+// ---- decoding in 8 bits ----
+
+// Keys of a cache's dict.
+struct Cache8Names {
+  PyObject *key, *value, *key_most, *value_most, *index, *weight, *position, *dropped;
+  Cache8Names() {
+    auto name = [](const char* s) { return PyUnicode_InternFromString(s); };
+    key = name("cached_key"), value = name("cached_value");
+    key_most = name("key_absmax"), value_most = name("value_absmax");
+    index = name("cache_index"), weight = name("token_weight"), position = name("token_position"), dropped = name("dropped");
+  }
+};
+
+// A cache in 8 bits as the kernels take it; not ok for what does not fit.
+struct Cache8Of {
+  T5xCache8 c = {};
+  int64_t b = 0, h = 0, slots = 0, dim = 0;
+  int device = -1;
+  bool ok = false;
+
+  static const Tensor* entry(PyObject* dict, PyObject* name) {
+    PyObject* o = PyDict_GetItem(dict, name);
+    return o != nullptr && THPVariable_Check(o) ? &THPVariable_Unpack(o) : nullptr;
+  }
+  std::array<Tensor, 8> held;  // the tensors, whatever another thread does to the dict meanwhile
+
+  explicit Cache8Of(PyObject* dict) {
+    static const Cache8Names names;
+    if (!PyDict_Check(dict)) return;
+    const Tensor* codes = entry(dict, names.key);
+    if (codes == nullptr || !codes->is_cuda() || codes->dim() != 4) return;
+    device = codes->get_device();
+    b = codes->size(0), h = codes->size(1), slots = codes->size(2), dim = codes->size(3);
+    const Tensor* most = entry(dict, names.key_most);
+    if (device != c10::cuda::current_device() || codes->numel() == 0 || b > 65535 || h > 65535 || !fits(slots) ||
+        (dim != 64 && dim != 128) || most == nullptr || most->dim() != 3 || most->size(2) < 1)
+      return;
+    const int64_t blocks = most->size(2), block = slots / blocks;
+    if (slots % blocks != 0 || (block != 16 && block != 32 && block != 64 && block != 128)) return;
+    auto fit = [&](const Tensor* t, at::ScalarType type, c10::IntArrayRef sizes) {
+      return t != nullptr && t->scalar_type() == type && t->sizes() == sizes && t->is_contiguous() && t->is_cuda() &&
+             t->get_device() == device;
+    };
+    const Tensor *values = entry(dict, names.value), *value_most = entry(dict, names.value_most);
+    if (!fit(codes, at::kChar, codes->sizes()) || !fit(values, at::kChar, codes->sizes()) ||
+        !fit(most, at::kFloat, {b, h, blocks}) || !fit(value_most, at::kFloat, {b, h, blocks}))
+      return;
+    const Tensor* index = entry(dict, names.index);
+    if (index == nullptr || index->scalar_type() != at::kInt || !index->is_cuda() || index->get_device() != device ||
+        !index->is_contiguous() || index->dim() > 1 || (index->dim() == 1 && index->numel() != b && index->numel() != 1))
+      return;
+    const Tensor *weight = entry(dict, names.weight), *position = entry(dict, names.position),
+                 *dropped = entry(dict, names.dropped);
+    if ((weight != nullptr && !fit(weight, at::kFloat, {b, h, slots})) ||
+        (position != nullptr && !fit(position, at::kInt, {b, h, slots})) ||
+        (dropped != nullptr && !fit(dropped, at::kInt, {b})) || (position != nullptr && dropped == nullptr))
+      return;
+    auto data = [](const Tensor* t) { return t == nullptr ? nullptr : t->data_ptr(); };
+    const Tensor* all[8] = {codes, values, most, value_most, index, weight, position, dropped};
+    for (int i = 0; i < 8; ++i)
+      if (all[i] != nullptr) held[i] = *all[i];
+    c.codes[0] = data(codes), c.codes[1] = data(values);
+    c.absmax[0] = data(most), c.absmax[1] = data(value_most);
+    c.index = data(index), c.weight = data(weight), c.position = data(position), c.dropped = data(dropped);
+    c.index_stride = index->numel() == b && b > 1;
+    c.batch = b, c.heads = h, c.slots = slots, c.dim = dim;
+    c.block_log2 = block == 16 ? 4 : block == 32 ? 5 : block == 64 ? 6 : 7;
+    ok = true;
+  }
+  bool has(const Tensor& t) const { return t.is_cuda() && t.get_device() == device; }
+};
+
+int type8(const Tensor& t) {  // -1: none of the kernels'
+  switch (t.scalar_type()) {
+    case at::kBFloat16: return 0;
+    case at::kHalf: return 1;
+    case at::kFloat: return 2;
+    default: return -1;
+  }
+}
+
+bool graph_of(const Tensor& t) { return at::GradMode::is_enabled() && t.requires_grad(); }
+
+// Attention over a cache in 8 bits. None, before doing anything, for what is not covered or not right.
+py::object cache8_attention(const Tensor& query, py::handle cache, const optional<Tensor>& key, const optional<Tensor>& value,
+                            const optional<Tensor>& table, py::handle buckets, const optional<Tensor>& key_mask, bool causal,
+                            double scale) {
+  const Cache8Of c(cache.ptr());
+  const int type = type8(query);
+  if (!c.ok || type < 0 || query.dim() != 4 || !c.has(query) || graph_of(query) || query.size(0) != c.b ||
+      query.size(3) != c.dim || query.size(2) < c.h || query.size(2) % c.h != 0 || query.size(1) < 1 || query.stride(3) != 1 ||
+      query.size(1) * (query.size(2) / c.h) > 65535 || key.has_value() != value.has_value())
+    return py::none();
+  T5xCache8Query q = {};
+  T5xNewTokens n = {};
+  if (key) {
+    for (int i = 0; i < 2; ++i) {
+      const Tensor& x = i == 0 ? *key : *value;
+      if (x.scalar_type() != query.scalar_type() || x.dim() != 4 || !c.has(x) || graph_of(x) || x.size(0) != c.b ||
+          x.size(1) != query.size(1) || x.size(2) != c.h || x.size(3) != c.dim || x.stride(3) != 1)
+        return py::none();
+      n.x[i] = x.data_ptr();
+      n.stride_batch[i] = x.stride(0), n.stride_token[i] = x.stride(1), n.stride_head[i] = x.stride(2);
+    }
+    n.count = query.size(1);
+    n.type = type;
+  }
+  if (table) {
+    char* bytes = nullptr;
+    Py_ssize_t count = 0;
+    if (table->scalar_type() != at::kFloat || table->dim() != 2 || !c.has(*table) || graph_of(*table) ||
+        table->size(0) != query.size(2) || !table->is_contiguous() || PyBytes_AsStringAndSize(buckets.ptr(), &bytes, &count) != 0 ||
+        count > 1024 || table->numel() > 8192) {
+      PyErr_Clear();
+      return py::none();
+    }
+    q.table = table->data_ptr();
+    q.table_stride = table->size(1);
+    q.buckets = reinterpret_cast<const unsigned char*>(bytes);
+    q.distances = static_cast<int>(count);
+  }
+  if (key_mask) {
+    if (key_mask->scalar_type() != at::kBool || key_mask->dim() != 2 || !c.has(*key_mask) || key_mask->size(0) != c.b ||
+        key_mask->size(1) > c.slots || key_mask->size(1) < 1 || !key_mask->is_contiguous())
+      return py::none();
+    q.key_mask = key_mask->data_ptr();
+    q.mask_stride = q.mask_len = key_mask->size(1);
+  }
+  py::gil_scoped_release no_gil;
+  Tensor out = at::empty(query.sizes(), query.options().requires_grad(false).memory_format(at::MemoryFormat::Contiguous));
+  q.query = query.data_ptr();
+  q.out = out.data_ptr();
+  q.stride_batch = query.stride(0), q.stride_token = query.stride(1), q.stride_head = query.stride(2);
+  q.count = query.size(1);
+  q.group = query.size(2) / c.h;
+  q.type = type;
+  q.causal = causal;
+  q.scale = scale;
+  const long long bytes = t5x_cache8_attention_bytes(&c.c, &q, key ? &n : nullptr);
+  if (bytes < 0) check(-1, "cache8_attention");
+  Tensor workspace;
+  if (bytes > 0) workspace = at::empty({bytes}, query.options().dtype(at::kByte).requires_grad(false));
+  check(t5x_cache8_attention(&c.c, &q, key ? &n : nullptr, bytes > 0 ? workspace.data_ptr() : nullptr, stream_of()),
+        "cache8_attention");
+  py::gil_scoped_acquire gil;
+  return py::cast(out);
+}
+
+// The kept slots; None, before doing anything, for what is not covered or not right.
+py::object cache8_evict(py::handle cache, py::handle into, int64_t keep, int64_t recent) {
+  const Cache8Of c(cache.ptr()), to(into.ptr());
+  if (!c.ok || !to.ok || c.device != to.device || c.b != to.b || c.h != to.h || c.dim != to.dim || c.c.weight == nullptr ||
+      to.c.weight == nullptr || to.c.position == nullptr || keep < 1 || keep > to.slots || recent < 0 || recent > keep ||
+      c.c.codes[0] == to.c.codes[0] || c.c.codes[1] == to.c.codes[1] || c.c.absmax[0] == to.c.absmax[0] ||
+      c.c.absmax[1] == to.c.absmax[1] || c.c.weight == to.c.weight || c.c.index == to.c.index ||
+      (c.c.position != nullptr && (c.c.position == to.c.position || c.c.dropped == to.c.dropped)) ||
+      (to.b > 1 && to.c.index_stride == 0))
+    return py::none();
+  py::gil_scoped_release no_gil;
+  Tensor kept = at::empty({c.b, c.h, keep}, at::TensorOptions().dtype(at::kInt).device(at::Device(at::kCUDA, c.device)));
+  check(t5x_cache8_evict(&c.c, &to.c, keep, recent, kept.data_ptr(), const_cast<void*>(to.c.index),
+                         const_cast<void*>(to.c.dropped), stream_of()),
+        "cache8_evict");
+  py::gil_scoped_acquire gil;
+  return py::cast(kept);
+}
+
+// x [..., k] times weights in 8 bits, plus residual.
+optional<Tensor> linear8(const Tensor& x, const Tensor& codes, const Tensor& absmax, int64_t k, const optional<Tensor>& residual) {
+  const int type = type8(x);
+  if (type < 0 || !x.is_cuda() || x.get_device() != c10::cuda::current_device() || x.dim() < 1 || !x.is_contiguous() ||
+      x.numel() == 0 || x.size(-1) != k || k < 1 || k > 131072 || graph_of(x) || codes.dim() != 2 ||
+      codes.scalar_type() != at::kChar || !codes.is_contiguous() || codes.size(1) != (k + 15) / 16 * 16 ||
+      codes.device() != x.device() || !aligned(codes) || absmax.scalar_type() != at::kFloat || absmax.dim() != 1 ||
+      absmax.size(0) != codes.size(0) || !absmax.is_contiguous() || absmax.device() != x.device())
+    return std::nullopt;
+  const int64_t n = codes.size(0), rows = x.numel() / k;
+  const std::vector<int64_t> sizes = with_last(x, n);
+  if (n < 1 || !fits(rows) || !fits(n)) return std::nullopt;
+  if (residual && (residual->scalar_type() != x.scalar_type() || residual->device() != x.device() || graph_of(*residual) ||
+                   residual->sizes() != sizes || !residual->is_contiguous()))
+    return std::nullopt;
+  Tensor y = at::empty(sizes, x.options().requires_grad(false));
+  Tensor workspace = bytes_like(x, t5x_linear8_workspace_bytes(rows, k));
+  check(t5x_linear8(x.data_ptr(), type, rows, k, k, codes.data_ptr(), absmax.data_ptr(), n, data_of(residual), n, y.data_ptr(),
+                    workspace.data_ptr(), stream_of()),
+        "linear8");
+  return y;
+}
+
 }  // namespace
 
 // The GIL is released for the duration of a call: a launch waits when the device's queue is full,
@@ -1151,5 +1342,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("relu_block_bwd", torch::wrap_pybind_function_no_gil(relu_block_bwd));
   m.def("policy_loss", torch::wrap_pybind_function_no_gil(policy_loss));
   m.def("preference_loss", torch::wrap_pybind_function_no_gil(preference_loss));
+  m.def("linear8", torch::wrap_pybind_function_no_gil(linear8));
+  m.def("cache8_attention", cache8_attention);  // (these read Python's dicts, and release the GIL for the launches)
+  m.def("cache8_evict", cache8_evict);
   m.def("adamw_tree", adamw_tree);  // (it reads Python's dicts, and releases the GIL for the launches)
 }

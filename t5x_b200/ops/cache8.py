@@ -126,6 +126,14 @@ def attention(query: torch.Tensor, cache: dict, key: Optional[torch.Tensor] = No
   bias_table [query heads, num_buckets]: learned biases of the T5 buckets of the distance to a token.
   key_mask [rows, n], n <= slots: slots that are seen; those from n on are hidden. A query that sees nothing has zeros and
   gives no weight. With `token_weight` in the cache the softmax of all queries and heads that share keys is added to it."""
+  host = native.host() if query.is_cuda and not F._transformed() else None
+  if host is not None and (bias_table is None or (bias_table.shape[-1] == num_buckets <= 256 and
+                                                  num_buckets // 2 < max_distance < native.CACHE8_DISTANCES)):
+    # (the plain call, checked there; anything else comes back as None)
+    buckets = None if bias_table is None else native.buckets_of(num_buckets, max_distance)
+    out = host.cache8_attention(query, cache, key, value, bias_table, buckets, key_mask, bool(causal), float(scale))
+    if out is not None:
+      return out
   _check_cache(cache, "attention")
   b, h, slots, dim = cache["cached_key"].shape
   if (key is None) != (value is None):
@@ -168,6 +176,11 @@ def evict(cache: dict, keep: int, *, recent: int = 0, out: Optional[dict] = None
   `out`, another cache with weights and positions for at least `keep` tokens, whose slots behind them stay as they were, or
   a new one as large as this. Its blocks take the largest scale that a token brings, and codes from smaller ones are
   rounded again."""
+  if out is not None and not F._transformed() and getattr(cache.get("cached_key"), "is_cuda", False):
+    host = native.host()
+    kept = None if host is None else host.cache8_evict(cache, out, keep, recent)
+    if kept is not None:
+      return out, kept
   _check_cache(cache, "evict")
   if "token_weight" not in cache:
     raise ValueError("evict: the cache adds up no attention weight (init_cache(..., weights=True))")

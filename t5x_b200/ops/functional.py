@@ -276,6 +276,11 @@ def linear8(x: torch.Tensor, weight: Weight8, residual: Optional[torch.Tensor] =
   products are added exactly and the sum is rounded once, to x's type. A row with a value that is not finite is NaN. For
   serving: there is no backward pass."""
   codes, absmax, k = weight
+  if x.is_cuda and not _transformed():
+    host = native.host()
+    y = None if host is None else host.linear8(x, codes, absmax, k, residual)
+    if y is not None:
+      return y
   n = codes.shape[0]
   if torch.is_grad_enabled() and (x.requires_grad or (residual is not None and residual.requires_grad)):
     raise ValueError("linear8 has no backward pass: detach its inputs or call it under torch.no_grad()")

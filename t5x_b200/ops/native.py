@@ -134,7 +134,7 @@ class _HostOps:
            "rmsnorm_bwd", "attention", "attention_bwd", "attention_block_ok", "attention_grads_ok",
            "attention_block", "attention_block_bwd", "mlp_block_ok", "mlp_grads_ok", "mlp_block",
            "mlp_block_bwd", "relu_block_ok", "relu_grads_ok", "relu_block", "relu_block_bwd",
-           "adamw_tree", "policy_loss", "preference_loss")
+           "adamw_tree", "policy_loss", "preference_loss", "linear8", "cache8_attention", "cache8_evict")
 
   def __init__(self, module):
     for name in self.NAMES:
@@ -1383,7 +1383,7 @@ def cache8_append(cache, key, value, lengths=None) -> None:
     _check(lib().t5x_cache8_append(ctypes.byref(c), ctypes.byref(n), stream_ptr()), "cache8_append")
 
 
-def _buckets_of(num_buckets: int, max_distance: int):
+def buckets_of(num_buckets: int, max_distance: int):
   """The bucket of each distance up to `max_distance`, from where on all share the last: bytes on the host."""
   table = _cache8_buckets.get((num_buckets, max_distance))
   if table is None:
@@ -1405,7 +1405,7 @@ def cache8_attention(query, cache, key, value, bias_table, num_buckets, max_dist
   q.stride_batch, q.stride_token, q.stride_head = query.stride()[:3]
   if bias_table is not None:
     bias_table = bias_table.detach()[:heads, :num_buckets].float().contiguous()
-    buckets = _buckets_of(num_buckets, max_distance)
+    buckets = buckets_of(num_buckets, max_distance)
     q.table, q.table_stride, q.distances = bias_table.data_ptr(), bias_table.shape[1], len(buckets)
     q.buckets = ctypes.cast(ctypes.c_char_p(buckets), c_void_p)
   if key_mask is not None:
