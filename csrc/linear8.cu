@@ -2,7 +2,7 @@
 // largest |x| of the row, cx = 127 x / sx rounded) and weights by output channel. The sums of products are whole numbers
 // below 2^31 for up to 131072 channels and exact; one rounding at the end.
 //
-// Two kernels: the rows are turned into codes, and tcgen05 (kind::i8, sums in 32 bits in tensor memory) multiplies them.
+// Two launches: the rows are turned into codes, and tcgen05 (kind::i8, sums in 32 bits in tensor memory) multiplies them.
 // It runs at twice the rate of bf16, so that a large product has half the time of `native.gemm`; over few rows both are
 // bound by the weights' bytes, which are half of bf16's.
 #include <algorithm>
@@ -39,17 +39,35 @@ __host__ __device__ constexpr uint32_t make_idesc_i8(int m, int n) {
 // Rows to codes
 // ---------------------------------------------------------------------------
 constexpr int kRowThreads = 256;
+constexpr int kRowHeld = 8;  // pieces of 16 bytes that a thread keeps
 
-// One CTA a row; `ld` codes a row, those behind the last channel 0.
-template <typename T>
+// One CTA a row, which it reads once where a thread's pieces fit its registers (16384 values of 16 bits) and whole 16 bytes may
+// be loaded (kVec). `ld` codes a row, those behind the last channel 0.
+template <typename T, bool kVec>
 __global__ void __launch_bounds__(kRowThreads)
     quantize_rows_kernel(const T* __restrict__ x, long long stride, int k, int ld, int8_t* __restrict__ codes,
                          float* __restrict__ absmax) {
+  constexpr int E = 16 / sizeof(T);
   __shared__ uint32_t s_most[kRowThreads / 32];
   const long long row = blockIdx.x;
   const T* src = x + row * stride;
+  int8_t* dst = codes + row * ld;
   uint32_t most = 0;
-  for (int i = threadIdx.x; i < k; i += kRowThreads) most = max(most, abs_bits(to_float(src[i])));
+  alignas(16) T held[kVec ? kRowHeld : 1][E];
+  chain_release();
+  if (kVec) {
+#pragma unroll
+    for (int i = 0; i < kRowHeld; ++i) {
+      const int at = (i * kRowThreads + threadIdx.x) * E;
+      if (at < k) {
+        *reinterpret_cast<uint4*>(held[i]) = *reinterpret_cast<const uint4*>(src + at);
+#pragma unroll
+        for (int e = 0; e < E; ++e) most = max(most, abs_bits(to_float(held[i][e])));
+      }
+    }
+  }
+  const int rest = kVec ? min(k, kRowHeld * kRowThreads * E) : 0;  // from here on value by value, and read twice
+  for (int i = rest + threadIdx.x; i < k; i += kRowThreads) most = max(most, abs_bits(to_float(src[i])));
   most = __reduce_max_sync(0xffffffffu, most);
   if ((threadIdx.x & 31) == 0) s_most[threadIdx.x >> 5] = most;
   __syncthreads();
@@ -57,9 +75,31 @@ __global__ void __launch_bounds__(kRowThreads)
   for (int w = 0; w < kRowThreads / 32; ++w) most = max(most, s_most[w]);
   const float a = __uint_as_float(most);
   const Coder code(127.f, a);
-  for (int i = threadIdx.x; i < ld; i += kRowThreads)
-    codes[row * ld + i] = static_cast<int8_t>(i < k ? code.template of<sizeof(T) == 2>(to_float(src[i])) : 0);
+  auto of = [&](T v) { return code.template of<sizeof(T) == 2>(to_float(v)); };
+  if (kVec) {
+#pragma unroll
+    for (int i = 0; i < kRowHeld; ++i) {
+      const int at = (i * kRowThreads + threadIdx.x) * E;
+      if (at < k) {
+#pragma unroll
+        for (int e = 0; e < E; e += 4)
+          *reinterpret_cast<char4*>(dst + at + e) = make_char4(of(held[i][e]), of(held[i][e + 1]), of(held[i][e + 2]), of(held[i][e + 3]));
+      }
+    }
+  }
+  for (int i = rest + threadIdx.x; i < ld; i += kRowThreads) dst[i] = static_cast<int8_t>(i < k ? of(src[i]) : 0);
   if (threadIdx.x == 0) absmax[row] = a;
+}
+
+template <typename T>
+void launch_rows(const void* x, long long stride, unsigned rows, int k, int ld, int8_t* codes, float* absmax, cudaStream_t stream) {
+  const T* src = static_cast<const T*>(x);
+  // (rows of whole pieces at multiples of 16 bytes, codes at multiples of 4)
+  if (k % (16 / sizeof(T)) == 0 && ld % 4 == 0 && aligned_to(16, {x}) && stride * sizeof(T) % 16 == 0 && aligned_to(4, {codes}))
+    quantize_rows_kernel<T, true><<<rows, kRowThreads, 0, stream>>>(src, stride, k, ld, codes, absmax);
+  else
+    quantize_rows_kernel<T, false><<<rows, kRowThreads, 0, stream>>>(src, stride, k, ld, codes, absmax);
+  count_launches(1);
 }
 
 // ---------------------------------------------------------------------------
@@ -281,19 +321,262 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   }
 }
 
-bool map_of(CUtensorMap* map, const void* codes, int rows, int k) {
+// ---------------------------------------------------------------------------
+// Products that have too few tiles of 256 x 256 for the SMs, as of a decode step: bound by the weights' bytes. A cluster takes
+// 128 output channels by NR tokens and cuts the input channels into one piece a CTA, so that all SMs stream weights at the
+// same time. The weights are the 128-row operand (tokens, of which there may be one, the other), and are requested while the
+// rows are still turned into codes (a programmatic dependent launch). The sums, whole numbers, meet through distributed shared
+// memory, in no particular order: they are exact.
+// ---------------------------------------------------------------------------
+constexpr int kFewThreads = 128;
+constexpr int kFewStages = 4;
+template <int NR>
+constexpr int few_smem() { return kFewStages * (kOperand + NR * kBytes) + 1024 + 256; }
+
+__device__ __forceinline__ void umma_i8(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t"
+      ".reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t"
+      "}\n"
+      :
+      : "r"(tmem_d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ int4 remote_int4(const int* mine, uint32_t cta) {
+  int4 v;
+  asm volatile("ld.shared::cluster.v4.s32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "r"(mapa_shared(smem_u32(mine), cta))
+               : "memory");
+  return v;
+}
+// 32 lanes x 16 columns
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+        "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr)
+      : "memory");
+}
+
+template <typename T, int NR>
+__global__ void __launch_bounds__(kFewThreads)
+    linear8_few_kernel(const __grid_constant__ Linear8Maps maps, const __grid_constant__ Linear8 p, int splits) {
+  static_assert(few_smem<NR>() >= 1024 + NR * 128 * 4, "the sums take the place of the stages");
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  uint8_t* s_w = smem;
+  uint8_t* s_x = smem + kFewStages * kOperand;
+  __shared__ uint64_t full[kFewStages], empty[kFewStages], done;
+  __shared__ uint32_t tmem_slot;
+  __shared__ volatile int abort_word;
+  volatile int* abort_flag = &abort_word;
+  constexpr int kColumns = NR < 32 ? 32 : NR;
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int piece = static_cast<int>(cluster_ctarank());
+  const int n0 = static_cast<int>(blockIdx.x / splits) * kRows, m0 = blockIdx.y * NR;
+  const int steps = (p.K + kBytes - 1) / kBytes, per = (steps + splits - 1) / splits;
+  const int k0 = min(piece * per, steps), k1 = min(k0 + per, steps);
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kFewStages; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    mbar_init(&done, 1);
+    abort_word = 0;
+    mbar_fence_init();
+    tma_prefetch_desc(&maps.x);
+    tma_prefetch_desc(&maps.w);
+  }
+  if (warp == 1) {
+    tmem_alloc(&tmem_slot, kColumns);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = tmem_slot;
+
+  if (warp == 0 && lane == 0) {
+    constexpr uint32_t kStage = kOperand + NR * kBytes;
+    const int ahead = min(kFewStages, k1 - k0);
+    for (int i = 0; i < ahead; ++i) {
+      mbar_expect_tx(&full[i], kStage);
+      tma_load_3d(s_w + i * kOperand, &maps.w, &full[i], (k0 + i) * kBytes, n0, 0);
+    }
+    chain_wait();  // the codes are the kernel's in front
+    for (int i = 0; i < ahead; ++i) tma_load_3d(s_x + i * NR * kBytes, &maps.x, &full[i], (k0 + i) * kBytes, m0, 0);
+    for (int i = ahead; i < k1 - k0; ++i) {
+      const int stage = i % kFewStages;
+      if (!mbar_wait(&empty[stage], (i / kFewStages - 1) & 1, abort_flag)) {
+        report_status(p.status, kStatusTimeoutProducer, kKernelIdLinear8, n0, i);
+        *abort_flag = 1;
+        break;
+      }
+      mbar_expect_tx(&full[stage], kStage);
+      tma_load_3d(s_w + stage * kOperand, &maps.w, &full[stage], (k0 + i) * kBytes, n0, 0);
+      tma_load_3d(s_x + stage * NR * kBytes, &maps.x, &full[stage], (k0 + i) * kBytes, m0, 0);
+    }
+  } else if (warp == 1 && lane == 0) {
+    constexpr uint32_t idesc = make_idesc_i8(kRows, NR);
+    bool ok = true;
+    for (int i = 0; i < k1 - k0; ++i) {
+      const int stage = i % kFewStages;
+      if (!mbar_wait(&full[stage], (i / kFewStages) & 1, abort_flag)) {
+        report_status(p.status, kStatusTimeoutMma, kKernelIdLinear8, n0, i);
+        *abort_flag = 1;
+        ok = false;
+        break;
+      }
+      tc_fence_after();
+      const uint32_t wa = smem_u32(s_w + stage * kOperand), xa = smem_u32(s_x + stage * NR * kBytes);
+#pragma unroll
+      for (int s = 0; s < kBytes / 32; ++s)
+        umma_i8(tmem, make_smem_desc_sw128(wa + s * 32, 16, 1024), make_smem_desc_sw128(xa + s * 32, 16, 1024), idesc, i > 0 || s > 0);
+      umma_commit(&empty[stage]);
+    }
+    if (ok) umma_commit(&done);
+  }
+  __syncwarp();
+  chain_wait();  // the rows' scales are read below
+  bool good = true;
+  if (k1 > k0) {
+    good = mbar_wait(&done, 0, abort_flag);
+    if (!good) {
+      if (lane == 0) report_status(p.status, kStatusTimeoutEpilogue, kKernelIdLinear8, n0, 0);
+      *abort_flag = 1;
+    }
+  }
+  tc_fence_after();
+  // The sums by token and channel, over the stages: all of them have been read (`done`). (After a wait that ran out copies may
+  // still land there: nothing is written then.)
+  int* s_sums = reinterpret_cast<int*>(smem);
+  if (good) {
+#pragma unroll
+    for (int c = 0; c < NR; c += 16) {
+      uint32_t r[16];
+      if (k1 > k0) {
+        tmem_ld16(tmem + (static_cast<uint32_t>(warp * 32) << 16) + c, r);
+        tmem_ld_wait();
+      }
+#pragma unroll
+      for (int j = 0; j < 16; ++j) s_sums[(c + j) * 128 + threadIdx.x] = k1 > k0 ? static_cast<int>(r[j]) : 0;
+    }
+  } else if (lane == 0) {
+    for (int it = 0; it < 2000; ++it) __nanosleep(1000);  // ~2 ms for copies in flight to land
+  }
+  tc_fence_before();
+  cluster_sync_all();
+
+  // each CTA of the cluster finishes a share of the tokens
+  T* y = static_cast<T*>(p.y);
+  const T* residual = static_cast<const T*>(p.residual);
+  const int tokens = min(NR, p.M - m0);
+  for (int i = piece * kFewThreads + threadIdx.x; i < tokens * 32; i += splits * kFewThreads) {
+    const int tok = i >> 5, ch = (i & 31) * 4, n = n0 + ch;
+    int4 sum = make_int4(0, 0, 0, 0);
+    for (int r = 0; r < splits; ++r) {
+      const int4 v = remote_int4(s_sums + tok * 128 + ch, r);
+      sum.x += v.x, sum.y += v.y, sum.z += v.z, sum.w += v.w;
+    }
+    if (n >= p.N) continue;
+    const float sx = ld_chained(p.x_absmax + m0 + tok) * (1.f / 127.f);
+    const int of[4] = {sum.x, sum.y, sum.z, sum.w};
+    const long long row = m0 + tok;
+    alignas(16) T o[4];
+    if (p.vec && n + 4 <= p.N) {
+      float v[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] = static_cast<float>(of[e]) * sx * (p.w_absmax[n + e] * (1.f / 127.f));
+      if (residual != nullptr) {
+        float add[4];
+        load_four(residual + row * p.ld_res + n, true, add);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] += add[e];
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[e] = from_float<T>(v[e]);
+      if (sizeof(T) == 4) *reinterpret_cast<uint4*>(y + row * p.N + n) = *reinterpret_cast<uint4*>(o);
+      else *reinterpret_cast<uint2*>(y + row * p.N + n) = *reinterpret_cast<uint2*>(o);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (n + e < p.N) {
+          float v = static_cast<float>(of[e]) * sx * (p.w_absmax[n + e] * (1.f / 127.f));
+          if (residual != nullptr) v += to_float(residual[row * p.ld_res + n + e]);
+          y[row * p.N + n + e] = from_float<T>(v);
+        }
+    }
+  }
+  cluster_sync_all();  // nobody leaves while others read its sums
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, kColumns);
+  }
+}
+
+bool map_of(CUtensorMap* map, const void* codes, int rows, int k, uint32_t box_rows = kRows) {
   const uint64_t dims[3] = {static_cast<uint64_t>(k), static_cast<uint64_t>(rows), 1};
   const uint64_t strides[2] = {static_cast<uint64_t>(k), static_cast<uint64_t>(k) * rows};
-  const uint32_t box[3] = {kBytes, kRows, 1};
+  const uint32_t box[3] = {kBytes, box_rows, 1};
   return get_tensor_map(map, codes, 1, 3, dims, strides, box, 1);
+}
+
+template <typename T, int NR>
+cudaError_t launch_few(const Linear8Maps& maps, const Linear8& p, int splits, cudaStream_t stream) {
+  static bool set[64] = {false};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (!set[dev & 63]) {
+    const cudaError_t e = cudaFuncSetAttribute(linear8_few_kernel<T, NR>, cudaFuncAttributeMaxDynamicSharedMemorySize, few_smem<NR>());
+    if (e != cudaSuccess) return e;
+    set[dev & 63] = true;
+  }
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((p.N + kRows - 1) / kRows * splits, (p.M + NR - 1) / NR);
+  cfg.blockDim = dim3(kFewThreads);
+  cfg.dynamicSmemBytes = few_smem<NR>();
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = splits;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  count_launches(1);
+  return cudaLaunchKernelEx(&cfg, linear8_few_kernel<T, NR>, maps, p, splits);
 }
 
 template <typename T>
 int launch(const void* x, long long stride, int k, int8_t* codes, const void* w, Linear8 p, cudaStream_t stream) {
   float* absmax = const_cast<float*>(p.x_absmax);
-  quantize_rows_kernel<T><<<p.M, kRowThreads, 0, stream>>>(static_cast<const T*>(x), stride, k, p.K, codes, absmax);
-  count_launches(1);
+  launch_rows<T>(x, stride, p.M, k, p.K, codes, absmax, stream);
   Linear8Maps maps;
+  p.tiles_m = (p.M + kTileRows - 1) / kTileRows;
+  p.tiles_n = (p.N + kTileCols - 1) / kTileCols;
+  const long long tiles = static_cast<long long>(p.tiles_m) * p.tiles_n;
+  if (tiles < num_sms() / 2) {  // pairs of SMs would be left without a tile
+    const int nr = p.M <= 16 ? 16 : p.M <= 32 ? 32 : p.M <= 64 ? 64 : 128;
+    if (!map_of(&maps.x, codes, p.M, p.K, nr) || !map_of(&maps.w, w, p.N, p.K)) return -1;
+    // as many pieces of the input channels as there are CTAs for at a time (two an SM), of two steps at least
+    const long long all = static_cast<long long>((p.N + kRows - 1) / kRows) * ((p.M + nr - 1) / nr);
+    const int steps = (p.K + kBytes - 1) / kBytes;
+    int splits = 1;
+    while (splits < 8 && all * splits * 2 <= 2 * num_sms() && steps >= splits * 4) splits *= 2;
+    const cudaError_t e = nr == 16   ? launch_few<T, 16>(maps, p, splits, stream)
+                          : nr == 32 ? launch_few<T, 32>(maps, p, splits, stream)
+                          : nr == 64 ? launch_few<T, 64>(maps, p, splits, stream)
+                                     : launch_few<T, 128>(maps, p, splits, stream);
+    return e == cudaSuccess ? 0 : set_error("linear8 launch: %s", cudaGetErrorString(e));
+  }
   if (!map_of(&maps.x, codes, p.M, p.K) || !map_of(&maps.w, w, p.N, p.K)) return -1;
   static bool set[64] = {false};
   int dev = 0;
@@ -304,9 +587,6 @@ int launch(const void* x, long long stride, int k, int8_t* codes, const void* w,
     if (e != cudaSuccess) return set_error("linear8: %s", cudaGetErrorString(e));
     set[dev & 63] = true;
   }
-  p.tiles_m = (p.M + kTileRows - 1) / kTileRows;
-  p.tiles_n = (p.N + kTileCols - 1) / kTileCols;
-  const long long tiles = static_cast<long long>(p.tiles_m) * p.tiles_n;
   const int pairs = static_cast<int>(std::min<long long>(num_sms() / 2, tiles));
   linear8_kernel<T><<<2 * pairs, kThreads, kSmem, stream>>>(maps, p);
   count_launches(1);
@@ -328,13 +608,9 @@ T5X_API int t5x_quantize_rows(const void* x, int type, long long rows, int k, lo
   int8_t* c = static_cast<int8_t*>(codes);
   float* a = static_cast<float*>(absmax);
   const unsigned grid = static_cast<unsigned>(rows);
-  if (type == 0)
-    t5x::quantize_rows_kernel<<<grid, t5x::kRowThreads, 0, st>>>(static_cast<const __nv_bfloat16*>(x), stride, k, ld, c, a);
-  else if (type == 1)
-    t5x::quantize_rows_kernel<<<grid, t5x::kRowThreads, 0, st>>>(static_cast<const __half*>(x), stride, k, ld, c, a);
-  else
-    t5x::quantize_rows_kernel<<<grid, t5x::kRowThreads, 0, st>>>(static_cast<const float*>(x), stride, k, ld, c, a);
-  t5x::count_launches(1);
+  if (type == 0) t5x::launch_rows<__nv_bfloat16>(x, stride, grid, k, ld, c, a, st);
+  else if (type == 1) t5x::launch_rows<__half>(x, stride, grid, k, ld, c, a, st);
+  else t5x::launch_rows<float>(x, stride, grid, k, ld, c, a, st);
   const cudaError_t e = cudaGetLastError();
   return e == cudaSuccess ? 0 : t5x::set_error("quantize_rows launch: %s", cudaGetErrorString(e));
 }
