@@ -326,18 +326,18 @@ __global__ void __launch_bounds__(kWalkThreads)
 // ---------------------------------------------------------------------------
 constexpr int kMoveThreads = 128;
 
-__device__ __forceinline__ uint32_t low_bytes(const uint32_t (&r)[4]) {
-  return __byte_perm(__byte_perm(r[0], r[1], 0x0040), __byte_perm(r[2], r[3], 0x0040), 0x5410);
-}
 __device__ __forceinline__ float code_number(uint32_t w, int i) {
   return __uint_as_float(__byte_perm(w ^ 0x80808080u, 0x4b000000u, 0x7440 + i)) - 8388736.f;
 }
 // with short scales (Coder)
 __device__ __forceinline__ uint32_t round_four(uint32_t w, float ratio) {
-  uint32_t r[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) r[i] = __float_as_uint(in_21_bits(code_number(w, i) * ratio) + 12582912.f);
-  return low_bytes(r);
+  const uint32_t u = w ^ 0x80808080u;
+  const uint64_t less = pair_of(-8388736.f, -8388736.f), by = pair_of(ratio, ratio);
+  auto two = [&](int i) {
+    return codes_of_two(add2(pair_of(__uint_as_float(__byte_perm(u, 0x4b000000u, 0x7440 + i)),
+                                     __uint_as_float(__byte_perm(u, 0x4b000000u, 0x7441 + i))), less), by);
+  };
+  return low_bytes(two(0), two(2));
 }
 // with any; off: how far a quotient is from its code
 __device__ __forceinline__ uint32_t round_four(uint32_t w, float ratio, float& off) {

@@ -72,6 +72,55 @@ struct Coder {
   }
 };
 
+// Two numbers an instruction.
+__device__ __forceinline__ uint64_t pair_of(float lo, float hi) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+// Codes of two short values (Coder), in the low byte of each half: quotients in 21 bits, then under the exponent of 3 * 2^22.
+__device__ __forceinline__ uint64_t codes_of_two(uint64_t x, uint64_t factor) {
+  const uint64_t minus = pair_of(-1.f, -1.f);
+  const uint64_t q = mul2(x, factor), high = mul2(q, pair_of(9.f, 9.f)), rest = fma2(q, minus, high);
+  return add2(fma2(rest, minus, high), pair_of(12582912.f, 12582912.f));
+}
+__device__ __forceinline__ uint32_t low_bytes(const uint32_t (&r)[4]) {
+  return __byte_perm(__byte_perm(r[0], r[1], 0x0040), __byte_perm(r[2], r[3], 0x0040), 0x5410);
+}
+__device__ __forceinline__ uint32_t low_bytes(uint64_t a, uint64_t b) {
+  uint32_t r[4];
+  asm("mov.b64 {%0, %1}, %2;" : "=r"(r[0]), "=r"(r[1]) : "l"(a));
+  asm("mov.b64 {%0, %1}, %2;" : "=r"(r[2]), "=r"(r[3]) : "l"(b));
+  return low_bytes(r);
+}
+// the two values of a word
+template <typename T>
+__device__ __forceinline__ uint64_t values_of(uint32_t w);
+template <>
+__device__ __forceinline__ uint64_t values_of<__nv_bfloat16>(uint32_t w) {
+  return pair_of(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+}
+template <>
+__device__ __forceinline__ uint64_t values_of<__half>(uint32_t w) {
+  const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w));
+  return pair_of(f.x, f.y);
+}
+
 // NaN counts as larger than any number: the bits of |x| are ordered so
 __device__ __forceinline__ uint32_t abs_bits(float x) { return __float_as_uint(x) & 0x7fffffffu; }
 

@@ -53,17 +53,30 @@ __global__ void __launch_bounds__(kRowThreads)
   const T* src = x + row * stride;
   int8_t* dst = codes + row * ld;
   uint32_t most = 0;
-  alignas(16) T held[kVec ? kRowHeld : 1][E];
+  uint4 held[kVec ? kRowHeld : 1];
   chain_release();
   if (kVec) {
+    uint32_t two = 0;  // of 16-bit values, the largest of each half
+#pragma unroll
+    for (int i = 0; i < kRowHeld; ++i) {
+      const int at = (i * kRowThreads + threadIdx.x) * E;
+      if (at < k) held[i] = *reinterpret_cast<const uint4*>(src + at);
+    }
 #pragma unroll
     for (int i = 0; i < kRowHeld; ++i) {
       const int at = (i * kRowThreads + threadIdx.x) * E;
       if (at < k) {
-        *reinterpret_cast<uint4*>(held[i]) = *reinterpret_cast<const uint4*>(src + at);
+        const uint32_t w[4] = {held[i].x, held[i].y, held[i].z, held[i].w};
 #pragma unroll
-        for (int e = 0; e < E; ++e) most = max(most, abs_bits(to_float(held[i][e])));
+        for (int j = 0; j < 4; ++j) {
+          if (sizeof(T) == 2) two = __vmaxu2(two, w[j] & 0x7fff7fffu);
+          else most = max(most, w[j] & 0x7fffffffu);
+        }
       }
+    }
+    if (sizeof(T) == 2) {
+      const uint16_t half = static_cast<uint16_t>(max(two >> 16, two & 0xffffu));
+      most = abs_bits(to_float(*reinterpret_cast<const T*>(&half)));
     }
   }
   const int rest = kVec ? min(k, kRowHeld * kRowThreads * E) : 0;  // from here on value by value, and read twice
@@ -76,14 +89,29 @@ __global__ void __launch_bounds__(kRowThreads)
   const float a = __uint_as_float(most);
   const Coder code(127.f, a);
   auto of = [&](T v) { return code.template of<sizeof(T) == 2>(to_float(v)); };
-  if (kVec) {
+  if constexpr (kVec && sizeof(T) == 2) {
+    if (code.brief) {
+      const uint64_t factor = pair_of(code.factor, code.factor);
+#pragma unroll
+      for (int i = 0; i < kRowHeld; ++i) {
+        const int at = (i * kRowThreads + threadIdx.x) * E;
+        if (at < k) {
+          const uint4 w = held[i];
+          *reinterpret_cast<uint2*>(dst + at) =
+              make_uint2(low_bytes(codes_of_two(values_of<T>(w.x), factor), codes_of_two(values_of<T>(w.y), factor)),
+                         low_bytes(codes_of_two(values_of<T>(w.z), factor), codes_of_two(values_of<T>(w.w), factor)));
+        }
+      }
+    }
+  }
+  if (kVec && !(sizeof(T) == 2 && code.brief)) {
 #pragma unroll
     for (int i = 0; i < kRowHeld; ++i) {
       const int at = (i * kRowThreads + threadIdx.x) * E;
       if (at < k) {
+        const T* v = reinterpret_cast<const T*>(&held[i]);
 #pragma unroll
-        for (int e = 0; e < E; e += 4)
-          *reinterpret_cast<char4*>(dst + at + e) = make_char4(of(held[i][e]), of(held[i][e + 1]), of(held[i][e + 2]), of(held[i][e + 3]));
+        for (int e = 0; e < E; e += 4) *reinterpret_cast<char4*>(dst + at + e) = make_char4(of(v[e]), of(v[e + 1]), of(v[e + 2]), of(v[e + 3]));
       }
     }
   }
@@ -94,8 +122,9 @@ __global__ void __launch_bounds__(kRowThreads)
 template <typename T>
 void launch_rows(const void* x, long long stride, unsigned rows, int k, int ld, int8_t* codes, float* absmax, cudaStream_t stream) {
   const T* src = static_cast<const T*>(x);
-  // (rows of whole pieces at multiples of 16 bytes, codes at multiples of 4)
-  if (k % (16 / sizeof(T)) == 0 && ld % 4 == 0 && aligned_to(16, {x}) && stride * sizeof(T) % 16 == 0 && aligned_to(4, {codes}))
+  // (rows of whole pieces at multiples of 16 bytes, codes at multiples of 8)
+  if (k % (16 / sizeof(T)) == 0 && aligned_to(16, {x}) && stride * sizeof(T) % 16 == 0 && aligned_to(8, {codes}) &&
+      ld % 8 == 0)
     quantize_rows_kernel<T, true><<<rows, kRowThreads, 0, stream>>>(src, stride, k, ld, codes, absmax);
   else
     quantize_rows_kernel<T, false><<<rows, kRowThreads, 0, stream>>>(src, stride, k, ld, codes, absmax);
@@ -330,6 +359,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 // ---------------------------------------------------------------------------
 constexpr int kFewThreads = 128;
 constexpr int kFewStages = 4;
+constexpr int kMaxSplits = 8;  // CTAs of a cluster
 template <int NR>
 constexpr int few_smem() { return kFewStages * (kOperand + NR * kBytes) + 1024 + 256; }
 
@@ -480,11 +510,13 @@ __global__ void __launch_bounds__(kFewThreads)
   const int tokens = min(NR, p.M - m0);
   for (int i = piece * kFewThreads + threadIdx.x; i < tokens * 32; i += splits * kFewThreads) {
     const int tok = i >> 5, ch = (i & 31) * 4, n = n0 + ch;
-    int4 sum = make_int4(0, 0, 0, 0);
-    for (int r = 0; r < splits; ++r) {
-      const int4 v = remote_int4(s_sums + tok * 128 + ch, r);
-      sum.x += v.x, sum.y += v.y, sum.z += v.z, sum.w += v.w;
-    }
+    int4 v[kMaxSplits], sum = make_int4(0, 0, 0, 0);
+#pragma unroll
+    for (int r = 0; r < kMaxSplits; ++r)
+      if (r < splits) v[r] = remote_int4(s_sums + tok * 128 + ch, r);
+#pragma unroll
+    for (int r = 0; r < kMaxSplits; ++r)
+      if (r < splits) sum.x += v[r].x, sum.y += v[r].y, sum.z += v[r].z, sum.w += v[r].w;
     if (n >= p.N) continue;
     const float sx = ld_chained(p.x_absmax + m0 + tok) * (1.f / 127.f);
     const int of[4] = {sum.x, sum.y, sum.z, sum.w};
@@ -569,8 +601,7 @@ int launch(const void* x, long long stride, int k, int8_t* codes, const void* w,
     // as many pieces of the input channels as there are CTAs for at a time (two an SM), of two steps at least
     const long long all = static_cast<long long>((p.N + kRows - 1) / kRows) * ((p.M + nr - 1) / nr);
     const int steps = (p.K + kBytes - 1) / kBytes;
-    int splits = 1;
-    while (splits < 8 && all * splits * 2 <= 2 * num_sms() && steps >= splits * 4) splits *= 2;
+    const int splits = static_cast<int>(std::max(1LL, std::min({2LL * num_sms() / all, steps / 2LL, static_cast<long long>(kMaxSplits)})));
     const cudaError_t e = nr == 16   ? launch_few<T, 16>(maps, p, splits, stream)
                           : nr == 32 ? launch_few<T, 32>(maps, p, splits, stream)
                           : nr == 64 ? launch_few<T, 64>(maps, p, splits, stream)
