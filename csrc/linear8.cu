@@ -41,8 +41,8 @@ __host__ __device__ constexpr uint32_t make_idesc_i8(int m, int n) {
 constexpr int kRowThreads = 256;
 constexpr int kRowHeld = 8;  // pieces of 16 bytes that a thread keeps
 
-// One CTA a row, which it reads once where a thread's pieces fit its registers (16384 values of 16 bits) and whole 16 bytes may
-// be loaded (kVec). `ld` codes a row, those behind the last channel 0.
+// One CTA a row, which it reads once where a thread's pieces fit its registers: 16384 values of 16 bits where whole 16 bytes may
+// be loaded (kVec), else 4096. `ld` codes a row, those behind the last channel 0.
 template <typename T, bool kVec>
 __global__ void __launch_bounds__(kRowThreads)
     quantize_rows_kernel(const T* __restrict__ x, long long stride, int k, int ld, int8_t* __restrict__ codes,
@@ -54,6 +54,7 @@ __global__ void __launch_bounds__(kRowThreads)
   int8_t* dst = codes + row * ld;
   uint32_t most = 0;
   uint4 held[kVec ? kRowHeld : 1];
+  T single[kVec ? 1 : 2 * kRowHeld];
   chain_release();
   if (kVec) {
     uint32_t two = 0;  // of 16-bit values, the largest of each half
@@ -79,7 +80,15 @@ __global__ void __launch_bounds__(kRowThreads)
       most = abs_bits(to_float(*reinterpret_cast<const T*>(&half)));
     }
   }
-  const int rest = kVec ? min(k, kRowHeld * kRowThreads * E) : 0;  // from here on value by value, and read twice
+  if (!kVec) {
+#pragma unroll
+    for (int i = 0; i < 2 * kRowHeld; ++i)
+      if (i * kRowThreads + static_cast<int>(threadIdx.x) < k) single[i] = src[i * kRowThreads + threadIdx.x];
+#pragma unroll
+    for (int i = 0; i < 2 * kRowHeld; ++i)
+      if (i * kRowThreads + static_cast<int>(threadIdx.x) < k) most = max(most, abs_bits(to_float(single[i])));
+  }
+  const int rest = min(k, kVec ? kRowHeld * kRowThreads * E : 2 * kRowHeld * kRowThreads);  // from here on read twice
   for (int i = rest + threadIdx.x; i < k; i += kRowThreads) most = max(most, abs_bits(to_float(src[i])));
   most = __reduce_max_sync(0xffffffffu, most);
   if ((threadIdx.x & 31) == 0) s_most[threadIdx.x >> 5] = most;
@@ -114,6 +123,11 @@ __global__ void __launch_bounds__(kRowThreads)
         for (int e = 0; e < E; e += 4) *reinterpret_cast<char4*>(dst + at + e) = make_char4(of(v[e]), of(v[e + 1]), of(v[e + 2]), of(v[e + 3]));
       }
     }
+  }
+  if (!kVec) {
+#pragma unroll
+    for (int i = 0; i < 2 * kRowHeld; ++i)
+      if (i * kRowThreads + static_cast<int>(threadIdx.x) < k) dst[i * kRowThreads + threadIdx.x] = static_cast<int8_t>(of(single[i]));
   }
   for (int i = rest + threadIdx.x; i < ld; i += kRowThreads) dst[i] = static_cast<int8_t>(i < k ? of(src[i]) : 0);
   if (threadIdx.x == 0) absmax[row] = a;
@@ -358,10 +372,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 // memory, in no particular order: they are exact.
 // ---------------------------------------------------------------------------
 constexpr int kFewThreads = 128;
-constexpr int kFewStages = 4;
 constexpr int kMaxSplits = 8;  // CTAs of a cluster
+// Two CTAs an SM.
 template <int NR>
-constexpr int few_smem() { return kFewStages * (kOperand + NR * kBytes) + 1024 + 256; }
+constexpr int few_stages() { return NR <= 32 ? 5 : NR <= 64 ? 4 : 3; }
+template <int NR>
+constexpr int few_smem() { return few_stages<NR>() * (kOperand + NR * kBytes) + 1024; }
+static_assert(2 * (few_smem<32>() + 2048) <= 233472 && 2 * (few_smem<64>() + 2048) <= 233472 && 2 * (few_smem<128>() + 2048) <= 233472,
+              "two CTAs an SM");
 
 __device__ __forceinline__ void umma_i8(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
@@ -382,6 +400,11 @@ __device__ __forceinline__ int4 remote_int4(const int* mine, uint32_t cta) {
                : "memory");
   return v;
 }
+__device__ __forceinline__ int remote_int(const int* mine, uint32_t cta) {
+  int v;
+  asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(mapa_shared(smem_u32(mine), cta)) : "memory");
+  return v;
+}
 // 32 lanes x 16 columns
 __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
   asm volatile(
@@ -397,6 +420,7 @@ template <typename T, int NR>
 __global__ void __launch_bounds__(kFewThreads)
     linear8_few_kernel(const __grid_constant__ Linear8Maps maps, const __grid_constant__ Linear8 p, int splits) {
   static_assert(few_smem<NR>() >= 1024 + NR * 128 * 4, "the sums take the place of the stages");
+  constexpr int kFewStages = few_stages<NR>();
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
   uint8_t* s_w = smem;
@@ -508,42 +532,53 @@ __global__ void __launch_bounds__(kFewThreads)
   T* y = static_cast<T*>(p.y);
   const T* residual = static_cast<const T*>(p.residual);
   const int tokens = min(NR, p.M - m0);
-  for (int i = piece * kFewThreads + threadIdx.x; i < tokens * 32; i += splits * kFewThreads) {
-    const int tok = i >> 5, ch = (i & 31) * 4, n = n0 + ch;
-    int4 v[kMaxSplits], sum = make_int4(0, 0, 0, 0);
+  auto value = [&](int sum, float sx, int n) { return static_cast<float>(sum) * sx * (p.w_absmax[n] * (1.f / 127.f)); };
+  if (p.vec) {  // four channels a thread (there are whole fours of them)
+    for (int i = piece * kFewThreads + threadIdx.x; i < tokens * 32; i += splits * kFewThreads) {
+      const int tok = i >> 5, ch = (i & 31) * 4, n = n0 + ch;
+      if (n >= p.N) continue;
+      int4 v[kMaxSplits], sum = make_int4(0, 0, 0, 0);
 #pragma unroll
-    for (int r = 0; r < kMaxSplits; ++r)
-      if (r < splits) v[r] = remote_int4(s_sums + tok * 128 + ch, r);
+      for (int r = 0; r < kMaxSplits; ++r)
+        if (r < splits) v[r] = remote_int4(s_sums + tok * 128 + ch, r);
+      const long long row = m0 + tok;
+      float add[4] = {0.f, 0.f, 0.f, 0.f};
+      if (residual != nullptr) load_four(residual + row * p.ld_res + n, true, add);
+      const float sx = ld_chained(p.x_absmax + row) * (1.f / 127.f);
 #pragma unroll
-    for (int r = 0; r < kMaxSplits; ++r)
-      if (r < splits) sum.x += v[r].x, sum.y += v[r].y, sum.z += v[r].z, sum.w += v[r].w;
-    if (n >= p.N) continue;
-    const float sx = ld_chained(p.x_absmax + m0 + tok) * (1.f / 127.f);
-    const int of[4] = {sum.x, sum.y, sum.z, sum.w};
-    const long long row = m0 + tok;
-    alignas(16) T o[4];
-    if (p.vec && n + 4 <= p.N) {
-      float v[4];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) v[e] = static_cast<float>(of[e]) * sx * (p.w_absmax[n + e] * (1.f / 127.f));
-      if (residual != nullptr) {
-        float add[4];
-        load_four(residual + row * p.ld_res + n, true, add);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] += add[e];
-      }
-#pragma unroll
-      for (int e = 0; e < 4; ++e) o[e] = from_float<T>(v[e]);
+      for (int r = 0; r < kMaxSplits; ++r)
+        if (r < splits) sum.x += v[r].x, sum.y += v[r].y, sum.z += v[r].z, sum.w += v[r].w;
+      alignas(16) T o[4];
+      o[0] = from_float<T>(value(sum.x, sx, n) + add[0]);
+      o[1] = from_float<T>(value(sum.y, sx, n + 1) + add[1]);
+      o[2] = from_float<T>(value(sum.z, sx, n + 2) + add[2]);
+      o[3] = from_float<T>(value(sum.w, sx, n + 3) + add[3]);
       if (sizeof(T) == 4) *reinterpret_cast<uint4*>(y + row * p.N + n) = *reinterpret_cast<uint4*>(o);
       else *reinterpret_cast<uint2*>(y + row * p.N + n) = *reinterpret_cast<uint2*>(o);
-    } else {
+    }
+  } else if (n0 + static_cast<int>(threadIdx.x) < p.N) {  // one channel a thread, four tokens at a time
+    const int n = n0 + threadIdx.x;
+    constexpr int U = 4;
+    for (int tok = piece * U; tok < tokens; tok += splits * U) {
+      int v[U][kMaxSplits];
+      float add[U], sx[U];
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (n + e < p.N) {
-          float v = static_cast<float>(of[e]) * sx * (p.w_absmax[n + e] * (1.f / 127.f));
-          if (residual != nullptr) v += to_float(residual[row * p.ld_res + n + e]);
-          y[row * p.N + n + e] = from_float<T>(v);
-        }
+      for (int u = 0; u < U; ++u) {
+        const long long row = m0 + min(tok + u, tokens - 1);
+#pragma unroll
+        for (int r = 0; r < kMaxSplits; ++r)
+          if (r < splits) v[u][r] = remote_int(s_sums + (tok + u) * 128 + threadIdx.x, r);
+        add[u] = residual != nullptr ? to_float(residual[row * p.ld_res + n]) : 0.f;
+        sx[u] = ld_chained(p.x_absmax + row) * (1.f / 127.f);
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        int sum = 0;
+#pragma unroll
+        for (int r = 0; r < kMaxSplits; ++r)
+          if (r < splits) sum += v[u][r];
+        if (tok + u < tokens) y[(m0 + tok + u) * static_cast<long long>(p.N) + n] = from_float<T>(value(sum, sx[u], n) + add[u]);
+      }
     }
   }
   cluster_sync_all();  // nobody leaves while others read its sums
