@@ -130,6 +130,8 @@ def _write_state(layer, hidden: torch.Tensor, cache: dict) -> None:
   h = layer.pre_self_attention_layer_norm(hidden)
   k, v = attn.project_kv(h)
   idx = cache["cache_index"]
+  if "key_absmax" in cache:
+    raise ValueError("early exits write into caches of the model's type: kv_cache_dtype is not for them")
   max_len = cache["cached_key"].shape[1]
   if idx.dim() == 0:
     i = int(idx)

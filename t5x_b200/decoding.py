@@ -8,7 +8,7 @@ decoding, and results come back sorted ascending so index -1 is the best.
 The loops are host-driven PyTorch: every tensor op runs on the device, and the only
 device->host read per step is the termination flag (optionally every k-th step).
 The KV cache is a nested dict of tensors whose leading dim is batch*beam; leaves named
-`cache_index`, `cached_bias`, `position_embedder_index`, `cross_key`, `cross_value` are not
+`cache_index`, `cached_bias`, `position_embedder_index`, `cross_key`, `cross_value`, `cross_cache`, `cache_room` are not
 expanded or gathered per beam (cross-attention K/V are shared by the beams of an example).
 """
 from __future__ import annotations
@@ -29,7 +29,7 @@ NEG_INF_VALUE = NEG_INF
 MIN_TEMPERATURE = 1e-4    # below this, sampling is greedy
 
 _CACHE_SKIP = ("cache_index", "cached_bias", "position_embedder_index", "cross_key",
-               "cross_value")
+               "cross_value", "cross_cache", "cache_room")
 
 
 @dataclasses.dataclass
@@ -74,7 +74,7 @@ def cache_map(fn, cache, apply_to_index: bool = False):
     if isinstance(node, Mapping):
       out = {}
       for k, v in node.items():
-        if isinstance(v, Mapping):
+        if isinstance(v, Mapping) and k not in _CACHE_SKIP:
           out[k] = rec(v)
         elif k in _CACHE_SKIP and not (apply_to_index and k == "cache_index" and
                                        isinstance(v, torch.Tensor) and v.dim() > 0):

@@ -248,6 +248,9 @@ def supported(module, decoder_input_tokens: torch.Tensor, decode_fn) -> bool:
   if not isinstance(module, network.Transformer) or decode_fn is not decoding.beam_search:
     return False
   c = module.config
+  if getattr(c, "kv_cache_dtype", None) is not None or any(getattr(m, "weight8", None) is not None
+                                                           for m in module.decoder.modules()):
+    return False  # the step holds its caches and weights in bf16
   # the step is written for this decoder (one position bias for all layers) and its own layers
   if type(module.decoder) is not network.Decoder or \
       any(type(getattr(module.decoder, f"layers_{i}")) is not network.DecoderLayer

@@ -43,6 +43,9 @@ class TransformerConfig:
   relpos_max_distance: int = 128
   float32_attention_logits: bool = False
   scale_attn_logits: bool = False
+  kv_cache_dtype: Any = None  # "int8": decode caches in 8 bits
+  kv_cache_keep: int = 0      # tokens that stay in the cache (0: all), the last kv_cache_recent among them
+  kv_cache_recent: int = 0
 
 
 class DecoderLayer(nn.Module):
@@ -55,7 +58,8 @@ class DecoderLayer(nn.Module):
     self.pre_self_attention_layer_norm = layers.LayerNorm(c.emb_dim, dtype=c.dtype, device=device)
     self.self_attention = layers.MultiHeadDotProductAttention(
         c.emb_dim, c.num_heads, c.head_dim, c.dtype, c.dropout_rate, c.float32_attention_logits,
-        c.scale_attn_logits, device=device)
+        c.scale_attn_logits, device=device, kv_cache_dtype=c.kv_cache_dtype, kv_cache_keep=c.kv_cache_keep,
+        kv_cache_recent=c.kv_cache_recent)
     self.pre_mlp_layer_norm = layers.LayerNorm(c.emb_dim, dtype=c.dtype, device=device)
     self.mlp = layers.MlpBlock(c.emb_dim, c.mlp_dim, c.mlp_activations, c.dropout_rate, c.dtype,
                                device=device)

@@ -19,6 +19,7 @@ from typing import Callable, Optional, Sequence, Tuple
 import torch
 from torch import nn
 
+from t5x_b200.ops import cache8
 from t5x_b200.ops import functional as F
 from t5x_b200.ops import reference as ref
 from t5x_b200.parallel import state as pstate
@@ -228,8 +229,35 @@ class DenseGeneral(nn.Module):
     self.kernel = param_with_axes((in_features, out_features), init, kernel_axes,
                                   shard_dim=shard_dim, device=device)
 
+  # weights in 8 bits that `quantize_dense` made, the kernel that they were made from and its version
+  weight8 = None
+
   def forward(self, x: torch.Tensor, residual: Optional[torch.Tensor] = None) -> torch.Tensor:
+    if self.weight8 is not None:
+      weight, kernel, version = self.weight8
+      if kernel is not self.kernel or kernel._version != version:
+        raise ValueError("the kernel has changed since quantize_dense: call it again, or dequantize_dense")
+      return F.linear8(x.to(self.dtype), weight, None if residual is None else residual.to(self.dtype))
     return F.linear(x.to(self.dtype), self.kernel, residual=residual, dtype=self.dtype)
+
+
+def quantize_dense(module: nn.Module) -> int:
+  """Lets every projection of `module` multiply in 8-bit integers (`functional.linear8`), for serving: weights scaled by output
+  channel, activations by token. The kernels stay as they are; a projection whose kernel changes afterwards raises until this
+  is called again. Returns how many projections there are. The embedding and the logits (in 32 bits) are left alone."""
+  if pstate.get().model_size > 1:
+    raise ValueError("quantize_dense: not under a model axis")
+  found = [m for name, m in module.named_modules() if type(m) is DenseGeneral and not name.endswith("logits_dense")]
+  for m in found:
+    m.weight8 = (F.quantize_weight(m.kernel), m.kernel, m.kernel._version)
+  return len(found)
+
+
+def dequantize_dense(module: nn.Module) -> None:
+  """Undoes `quantize_dense`."""
+  for m in module.modules():
+    if isinstance(m, DenseGeneral):
+      m.weight8 = None
 
 
 class LayerNorm(nn.Module):
@@ -329,9 +357,20 @@ class MultiHeadDotProductAttention(nn.Module):
 
   def __init__(self, emb_dim: int, num_heads: int, head_dim: int, dtype=torch.float32,
                dropout_rate: float = 0.0, float32_logits: bool = False,
-               scale_attn_logits: bool = False, device=None):
+               scale_attn_logits: bool = False, device=None, kv_cache_dtype=None,
+               kv_cache_keep: int = 0, kv_cache_recent: int = 0):
+    """kv_cache_dtype "int8": the decode caches are held in 8 bits (`ops.cache8`). kv_cache_keep: of the tokens of a
+    self-attention cache so many stay, the last `kv_cache_recent` and those that got most attention; the others are evicted
+    as the cache fills."""
     super().__init__()
     st = pstate.get()
+    if kv_cache_dtype not in (None, "int8", torch.int8):
+      raise ValueError(f"kv_cache_dtype {kv_cache_dtype!r}: None (the layer's dtype) or int8")
+    if kv_cache_keep and (kv_cache_dtype is None or not 0 <= kv_cache_recent <= kv_cache_keep):
+      raise ValueError(f"kv_cache_keep {kv_cache_keep} wants kv_cache_dtype int8 and at least the {kv_cache_recent} "
+                       "tokens of kv_cache_recent")
+    self.cache8 = kv_cache_dtype is not None
+    self.kv_cache_keep, self.kv_cache_recent = kv_cache_keep, kv_cache_recent
     if num_heads % st.model_size:
       raise ValueError(f"{num_heads} heads are not divisible by model={st.model_size}")
     self.num_heads = num_heads
@@ -351,16 +390,72 @@ class MultiHeadDotProductAttention(nn.Module):
     self.out = DenseGeneral(inner, emb_dim, ("joined_kv", "embed"), kv_init, dtype, 0, device)
 
   # -- cache helpers ----------------------------------------------------------------------
+  EVICT_ROOM = 64  # tokens that a cache takes between two evictions
+  OBSERVED = 32    # queries at a prompt's end whose attention counts for its first eviction
+
   def init_cache(self, batch: int, max_len: int, device) -> dict:
+    if self.cache8:
+      evicts = 0 < self.kv_cache_keep < max_len - self.EVICT_ROOM
+      slots = self.kv_cache_keep + self.EVICT_ROOM if evicts else max_len
+      cache = cache8.init_cache(batch, slots, self.local_heads, self.head_dim, device, weights=evicts, positions=evicts)
+      cache["cache_index"] = torch.zeros((), dtype=torch.int32, device=device)  # (of all rows)
+      if evicts:
+        cache["cache_room"] = slots
+      return cache
     shape = (batch, max_len, self.local_heads, self.head_dim)
     return {"cached_key": torch.zeros(shape, dtype=self.dtype, device=device),
             "cached_value": torch.zeros(shape, dtype=self.dtype, device=device),
             "cache_index": torch.zeros((), dtype=torch.int32, device=device)}
 
+  def _prefill8(self, cache: dict, q, k, v, lengths, bias) -> None:
+    """The prompt's keys and values into a cache in 8 bits; of a prompt longer than what is kept, what its last queries look
+    at."""
+    rows, lk = k.shape[:2]
+    lengths = torch.full((rows,), lk, device=k.device) if lengths is None else lengths.reshape(-1).expand(rows)
+    lengths = lengths.to(torch.int32)
+    if "cache_room" not in cache:
+      cache8.append_(cache, k, v, lengths)
+      cache["cache_index"] = lengths.clone()
+      return
+    whole = cache8.init_cache(rows, lk, self.local_heads, self.head_dim, k.device, weights=True, positions=True)
+    cache8.append_(whole, k, v, lengths)
+    whole["cache_index"] += lengths
+    seen = min(self.OBSERVED, lk)
+    at = (lengths.long()[:, None] - seen + torch.arange(seen, device=k.device)).clamp(min=0)
+    last = q.gather(1, at[:, :, None, None].expand(rows, seen, *q.shape[2:]))
+    cache8.attention(last, whole, **bias)
+    cache["cache_index"] = torch.zeros(rows, dtype=torch.int32, device=k.device)
+    cache8.evict(whole, self.kv_cache_keep, recent=self.kv_cache_recent, out=cache)
+    cache["cache_room"] = self.EVICT_ROOM
+
+  def _decode8(self, cache: dict, q, k, v, bias) -> torch.Tensor:
+    """One step over a cache in 8 bits: its tokens are appended and attended to; a full cache evicts first."""
+    room = cache.get("cache_room")
+    if room is not None:
+      if room < k.shape[1]:
+        kept, _ = cache8.evict(cache, self.kv_cache_keep, recent=self.kv_cache_recent)
+        cache.update(kept)
+        room = self.EVICT_ROOM
+      cache["cache_room"] = room - k.shape[1]
+    x = cache8.attention(q, cache, k, v, **bias)
+    cache["cache_index"] = cache["cache_index"] + k.shape[1]
+    return x
+
+  def cross_cache(self, inputs_kv: torch.Tensor) -> dict:
+    """Keys and values of a cross attention in 8 bits."""
+    k, v = self.project_kv(inputs_kv)
+    cache = cache8.init_cache(k.shape[0], k.shape[1], self.local_heads, self.head_dim, k.device)
+    cache8.append_(cache, k, v)
+    cache["cache_index"] += k.shape[1]
+    return cache
+
   def project_kv(self, inputs_kv: torch.Tensor):
     b, lk, _ = inputs_kv.shape
     kv_in = tp.copy_to_model_parallel(inputs_kv).to(self.dtype)
-    k, v = F.multi_linear(kv_in, [self.key.kernel, self.value.kernel], dtype=self.dtype)
+    if self.key.weight8 is not None:
+      k, v = self.key(kv_in), self.value(kv_in)
+    else:
+      k, v = F.multi_linear(kv_in, [self.key.kernel, self.value.kernel], dtype=self.dtype)
     return (k.view(b, lk, self.local_heads, self.head_dim),
             v.view(b, lk, self.local_heads, self.head_dim))
 
@@ -376,7 +471,14 @@ class MultiHeadDotProductAttention(nn.Module):
               beams_per_kv: int = 1) -> torch.Tensor:
     b, lq, _ = inputs_q.shape
     q_in = tp.copy_to_model_parallel(inputs_q)
-    if (precomputed_kv is None and inputs_kv is inputs_q and not self.scale_attn_logits):
+    if isinstance(precomputed_kv, dict):  # a cross attention's cache in 8 bits, shared by the beams of an example
+      if self.scale_attn_logits:
+        q_in = q_in / math.sqrt(self.head_dim)
+      q = self.query(q_in).view(b // beams_per_kv, beams_per_kv * lq, self.local_heads, self.head_dim)
+      x = cache8.attention(q, precomputed_kv, key_mask=key_mask, causal=False)
+      return self._project_out(x, b, lq, residual)
+    if (precomputed_kv is None and inputs_kv is inputs_q and not self.scale_attn_logits and
+        self.query.weight8 is None):
       # self-attention: the three projections share their input, and one backward builds its
       # gradient by accumulating GEMMs
       q, k, v = F.multi_linear(q_in.to(self.dtype),
@@ -394,7 +496,15 @@ class MultiHeadDotProductAttention(nn.Module):
       else:
         k, v = self.project_kv(inputs_kv)
     q_offset = 0
-    if cache is not None and prefill:
+    if cache is not None and "key_absmax" in cache and (prefill or decode):
+      if bidirectional:
+        raise ValueError("a cache in 8 bits has causal position biases")
+      bias = {} if bias_table is None else dict(bias_table=F.compute_weight(bias_table, torch.float32)[:self.local_heads],
+                                                num_buckets=num_buckets, max_distance=max_distance)
+      if not prefill:
+        return self._project_out(self._decode8(cache, q, k, v, bias), b, lq, residual)
+      self._prefill8(cache, q, k, v, prefill_lengths, bias)
+    elif cache is not None and prefill:
       # Fill the cache with the prompt's keys/values in one pass.
       lk = k.shape[1]
       cache["cached_key"][:, :lk] = k
@@ -600,7 +710,7 @@ class MlpBlock(nn.Module):
   def forward(self, inputs: torch.Tensor, residual: Optional[torch.Tensor] = None,
               enable_dropout: bool = False) -> torch.Tensor:
     x_in = tp.copy_to_model_parallel(inputs.to(self.dtype))
-    if self.activations == ("gelu", "linear"):
+    if self.activations == ("gelu", "linear") and self.wi_0.weight8 is None:
       x = F.gated_gelu_mlp_in(x_in, self.wi_0.kernel, self.wi_1.kernel, dtype=self.dtype)
     elif len(self.activations) == 1:
       x = ref.ACTIVATIONS[self.activations[0]](self.wi(x_in))

@@ -46,6 +46,9 @@ class T5Config:
   scale_attn_logits: bool = False      # t5x/contrib/gpu/t5/layers.py:205-206
   relpos_num_buckets: int = 32
   relpos_max_distance: int = 128
+  kv_cache_dtype: Any = None  # "int8": decode caches in 8 bits
+  kv_cache_keep: int = 0      # tokens that stay in the decoder's cache (0: all), the last kv_cache_recent among them
+  kv_cache_recent: int = 0
 
 
 def _dropout(x, rate, enable, broadcast=True, **kw):
@@ -148,7 +151,8 @@ class DecoderLayer(nn.Module):
     self.config = c
     mk_attn = lambda: layers.MultiHeadDotProductAttention(
         c.emb_dim, c.num_heads, c.head_dim, c.dtype, c.dropout_rate, c.float32_attention_logits,
-        c.scale_attn_logits, device=device)
+        c.scale_attn_logits, device=device, kv_cache_dtype=c.kv_cache_dtype, kv_cache_keep=c.kv_cache_keep,
+        kv_cache_recent=c.kv_cache_recent)
     self.pre_self_attention_layer_norm = layers.LayerNorm(c.emb_dim, dtype=c.dtype, device=device)
     self.self_attention = mk_attn()
     self.pre_cross_attention_layer_norm = layers.LayerNorm(c.emb_dim, dtype=c.dtype,
@@ -189,13 +193,17 @@ class DecoderLayer(nn.Module):
     x, h = self.pre_cross_attention_layer_norm(x, with_residual=True)
     if decode:
       cross = cache["encoder_decoder_attention"]
-      if "cross_key" not in cross:
-        k, v = self.encoder_decoder_attention.project_kv(encoded)
-        cross["cross_key"], cross["cross_value"] = k, v
-      x = self.encoder_decoder_attention(
-          h, None, key_mask=encoder_key_mask,
-          precomputed_kv=(cross["cross_key"], cross["cross_value"]), residual=x,
-          beams_per_kv=beams_per_kv)
+      if self.encoder_decoder_attention.cache8:
+        if "cross_cache" not in cross:
+          cross["cross_cache"] = self.encoder_decoder_attention.cross_cache(encoded)
+        kv = cross["cross_cache"]
+      else:
+        if "cross_key" not in cross:
+          k, v = self.encoder_decoder_attention.project_kv(encoded)
+          cross["cross_key"], cross["cross_value"] = k, v
+        kv = cross["cross_key"], cross["cross_value"]
+      x = self.encoder_decoder_attention(h, None, key_mask=encoder_key_mask, precomputed_kv=kv, residual=x,
+                                         beams_per_kv=beams_per_kv)
     elif drop:
       x = x + _dropout(self.encoder_decoder_attention(h, encoded, enable_dropout=True, **cross_kwargs),
                        rate, True)

@@ -41,7 +41,7 @@ def _kernels(parent, names, dense_cls):
   out = []
   for n in names:
     m = parent._modules.get(n)
-    if type(m) is not dense_cls or m.dtype is not torch.bfloat16 or not _unhooked(m):
+    if type(m) is not dense_cls or m.dtype is not torch.bfloat16 or m.weight8 is not None or not _unhooked(m):
       return None
     out.append(m._parameters["kernel"])
   return out
