@@ -46,7 +46,6 @@ constexpr int kPieceWarps = 8;  // warps a CTA, of the kernel by pieces
 constexpr int kMaxDistances = 1024;
 constexpr int kMaxBatch = 2048;  // rows of one launch
 constexpr int kMaxBiases = 8192;  // values of a bias table
-constexpr int kEntry = 6;        // what beginning a (row, head) costs, in tiles
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kPeak = 4.f;     // exponent of a probability at the reference
 constexpr float kLimit = 12.6f;  // of the largest; times 4 it is still an fp16 number
@@ -64,10 +63,12 @@ struct Cache8Attn {
   int distances, mask_len, causal;
   int appended;            // tokens of this call behind c.index
   float scale;
+  uint32_t low;            // 0x00ff00ff
   unsigned long long by_group;  // 2^32 / group, rounded up: r / group for r below 2^16 by one multiplication
   int pieces;              // that the tiles are cut into
   int row_warps;           // kRows: warps of a CTA that take different query rows of one piece (1, or all)
-  int least;               // tiles of a piece at least
+  int least;               // cost of a piece at least, in tiles
+  int entry;               // what beginning a (row, head) costs, in tiles
   float* part;             // [row tile, pieces, 2, rows of a tile, dim]
   float2* stats;           // [row tile, pieces, 2, rows of a tile]: reference, sum
   long long* first;        // [batch + 1]: cost in front of a row, in tiles; then that of a piece
@@ -91,11 +92,19 @@ __device__ __forceinline__ uint32_t transposed(uint32_t x) {
 }
 __device__ __forceinline__ uint32_t as_u32(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
 __device__ __forceinline__ __half2 as_half2(uint32_t u) { return *reinterpret_cast<__half2*>(&u); }
+// (w & low) ^ kFlip in one instruction, with `low` = 0x00ff00ff in a register (the compiler makes two of two constants: the
+// kernel reads it from its arguments)
+template <uint32_t kFlip>
+__device__ __forceinline__ uint32_t low_flipped(uint32_t w, uint32_t low) {
+  uint32_t r;
+  asm("lop3.b32 %0, %1, %2, %3, 0x6a;" : "=r"(r) : "r"(w), "r"(low), "n"(kFlip));
+  return r;
+}
 // bytes 0 and 2 of codes as two numbers (code + 128) 2^-24
-__device__ __forceinline__ uint32_t key_pair(uint32_t w) { return (w & 0x00ff00ffu) ^ 0x00800080u; }
+__device__ __forceinline__ uint32_t key_pair(uint32_t w, uint32_t low) { return low_flipped<0x00800080u>(w, low); }
 // bytes 0 and 2 of codes as two numbers
-__device__ __forceinline__ uint32_t value_pair(uint32_t w) {
-  return as_u32(__hsub2(as_half2((w & 0x00ff00ffu) ^ 0x64806480u), as_half2(0x64806480u)));
+__device__ __forceinline__ uint32_t value_pair(uint32_t w, uint32_t low) {
+  return as_u32(__hsub2(as_half2(low_flipped<0x64806480u>(w, low)), as_half2(0x64806480u)));
 }
 __device__ __forceinline__ float exp2_approx(float x) {
   float r;
@@ -131,7 +140,7 @@ __device__ __forceinline__ void count_tiles(const Cache8Attn& p, long long* s_fi
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   auto cost = [&](int b) {
     const int tiles = (end_of(p, held_of(p.c, b)) + 15) >> 4;
-    return tiles == 0 ? 0LL : static_cast<long long>(tiles + kEntry) * p.c.heads;
+    return tiles == 0 ? 0LL : static_cast<long long>(tiles + p.entry) * p.c.heads;
   };
   long long mine = 0;
   for (int b = from; b < min(from + each, p.c.batch); ++b) mine += cost(b);
@@ -267,6 +276,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 16 / kWarps : 1)
   __shared__ float2 s_stats[kTeam ? kWarps * kParts : 1][8];
   __shared__ float2 s_rows[8];
   const Cache8& c = p.c;
+  const uint32_t low = p.low;
   const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3, wid = threadIdx.x >> 5;
   // the piece of the tiles, and the first query row
   const int unit = kTeam ? blockIdx.x : p.row_warps > 1 ? blockIdx.x : blockIdx.x * kWarps + wid;
@@ -320,8 +330,8 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 16 / kWarps : 1)
       tile0 = 0;
       tile1 = tiles;
     } else {
-      h = static_cast<int>((at - s_first[b]) / (tiles + kEntry));
-      seg = s_first[b] + static_cast<long long>(h) * (tiles + kEntry) + kEntry;  // this (row, head)'s first tile
+      h = static_cast<int>((at - s_first[b]) / (tiles + p.entry));
+      seg = s_first[b] + static_cast<long long>(h) * (tiles + p.entry) + p.entry;  // this (row, head)'s first tile
       tile0 = static_cast<int>(max(at - seg, 0LL));
       tile1 = static_cast<int>(min(stop - seg, static_cast<long long>(tiles)));
       if (tile1 <= 0) break;  // (no more than a part of what the beginning costs)
@@ -516,8 +526,8 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 16 / kWarps : 1)
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
               const uint32_t w = j == 0 ? kr[mt][e][ch].x : j == 1 ? kr[mt][e][ch].y : j == 2 ? kr[mt][e][ch].z : kr[mt][e][ch].w;
-              a[mt][e] = key_pair(w);
-              a[mt][2 + e] = key_pair(w >> 8);
+              a[mt][e] = key_pair(w, low);
+              a[mt][2 + e] = key_pair(w >> 8, low);
             }
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt)
@@ -679,7 +689,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 16 / kWarps : 1)
           for (int half = 0; half < 2; ++half) {
             const uint32_t x = __byte_perm(vr[mt][0][w], vr[mt][1][w], half ? 0x7632 : 0x5410);
             const uint32_t y = __byte_perm(vr[mt][2][w], vr[mt][3][w], half ? 0x7632 : 0x5410);
-            const uint32_t a0 = value_pair(x), a1 = value_pair(x >> 8), a2 = value_pair(y), a3 = value_pair(y >> 8);
+            const uint32_t a0 = value_pair(x, low), a1 = value_pair(x >> 8, low), a2 = value_pair(y, low), a3 = value_pair(y >> 8, low);
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -821,9 +831,9 @@ __global__ void __launch_bounds__(kJoinThreads) cache8_join_kernel(const __grid_
   chain_wait();
   chain_release();
   const long long piece = __ldcg(p.first + p.c.batch + 1), from = __ldcg(p.first + b);
-  const long long cost = (__ldcg(p.first + b + 1) - from) / p.c.heads;  // tiles + kEntry, or 0
-  const long long seg = from + h * cost + kEntry;  // its first tile
-  const int w0 = static_cast<int>(seg / piece), w1 = cost == 0 ? w0 - 1 : static_cast<int>((seg + cost - kEntry - 1) / piece);
+  const long long cost = (__ldcg(p.first + b + 1) - from) / p.c.heads;  // tiles + p.entry, or 0
+  const long long seg = from + h * cost + p.entry;  // its first tile
+  const int w0 = static_cast<int>(seg / piece), w1 = cost == 0 ? w0 - 1 : static_cast<int>((seg + cost - p.entry - 1) / piece);
   if (w0 == w1) return;  // one unit had it whole
   // the first piece is its unit's second, the others are their units' first ones
   const long long base = (static_cast<long long>(r / tile_rows) * p.pieces) * 2 * tile_rows + r % tile_rows;
@@ -1007,7 +1017,7 @@ Cache8 rows_of(Cache8 c, int from, int count) {
 }
 
 struct Plan {
-  int pieces = 0, least = 0, row_warps = 1;
+  int pieces = 0, least = 0, entry = 0, row_warps = 1;
   size_t part = 0, stats = 0, first = 0, scores = 0, final_stats = 0, total = 0;
 };
 Plan plan(Cache8 c, int rows) {
@@ -1019,11 +1029,14 @@ Plan plan(Cache8 c, int rows) {
   const bool team = tile_rows == 8;
   w.row_warps = !team && row_tiles >= 4 ? kRowWarps : 1;
   const int unit_warps = team ? 8 : 1;
-  w.least = 4 * unit_warps + kEntry;
+  // (a CTA does some four tiles a us; us for long contexts of all lengths / for 4 x 16 heads of 64 channels by up to 16384 tokens
+  // with 8: 101 / 42, 16: 93 / 30, 24: 93 / 26, 40: 93 / 25)
+  w.entry = team ? 24 : 6;
+  w.least = 4 * unit_warps + w.entry;
   const long long room = team              ? 2LL * num_sms()
                          : w.row_warps > 1 ? num_sms() / ((row_tiles + kRowWarps - 1) / kRowWarps)
                                            : static_cast<long long>(num_sms()) * kRowWarps / row_tiles;
-  const long long most = static_cast<long long>(c.batch) * c.heads * (c.slots / 16 + kEntry) / w.least + 1;
+  const long long most = static_cast<long long>(c.batch) * c.heads * (c.slots / 16 + w.entry) / w.least + 1;
   w.pieces = static_cast<int>(std::max<long long>(1, std::min(room, most)));
   if (!team && w.row_warps == 1) w.pieces = (w.pieces + kRowWarps - 1) / kRowWarps * kRowWarps;
   const size_t bh = static_cast<size_t>(c.batch) * c.heads;
@@ -1102,6 +1115,7 @@ T5X_API int t5x_cache8_attention(const T5xCache8* cache, const T5xCache8Query* q
   p.causal = q->causal;
   p.appended = n ? n->count : 0;
   p.scale = q->scale;
+  p.low = 0x00ff00ffu;
   const t5x::Plan w = t5x::plan(c, p.rows);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (t5x::by_row_head(c, p.rows)) {
@@ -1117,6 +1131,7 @@ T5X_API int t5x_cache8_attention(const T5xCache8* cache, const T5xCache8Query* q
   p.pieces = w.pieces;
   p.row_warps = w.row_warps;
   p.least = w.least;
+  p.entry = w.entry;
   p.part = reinterpret_cast<float*>(ws + w.part);
   p.stats = reinterpret_cast<float2*>(ws + w.stats);
   p.first = reinterpret_cast<long long*>(ws + w.first);
