@@ -32,154 +32,26 @@
 // appends the new tokens, its warps take tiles of 16 tokens in turn and meet in shared memory, and the scores that the
 // weights are made from never leave it: one launch. Over long ones (of all lengths) all tiles of all (row, head) laid end to
 // end are cut into one equal piece a CTA; what it has of a (row, head) that it does not have whole goes to workspace, and a
-// second kernel joins the pieces. Many query rows go 32 at a time, a warp each, so that the warps of a CTA read the same
-// tiles, from L1.
+// second kernel joins the pieces. Many query rows have a kernel of their own, cache8_rows.cu.
 #include <algorithm>
 #include <type_traits>
 
-#include "cache8.cuh"
+#include "cache8_attention.cuh"
 
 namespace t5x {
 namespace {
 
-constexpr int kPieceWarps = 8;  // warps a CTA, of the kernel by pieces
-constexpr int kMaxDistances = 1024;
-constexpr int kMaxBatch = 2048;  // rows of one launch
-constexpr int kMaxBiases = 8192;  // values of a bias table
-constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kPeak = 4.f;     // exponent of a probability at the reference
-constexpr float kLimit = 12.6f;  // of the largest; times 4 it is still an fp16 number
-constexpr float kNothing = -3e38f;  // the reference of a row that has seen nothing
-
-struct Cache8Attn {
-  Cache8 c;
-  const void* q;
-  void* out;
-  const float* table;
-  const uint8_t* mask;
-  long long q_sb, q_st, q_sh, mask_stride;
-  int table_stride, q_vec;  // q_vec: whole 16 bytes of a query may be loaded
-  int count, group, rows;  // queries a row, heads a key head, their product
-  int distances, mask_len, causal;
-  int appended;            // tokens of this call behind c.index
-  float scale;
-  uint32_t low;            // 0x00ff00ff
-  unsigned long long by_group;  // 2^32 / group, rounded up: r / group for r below 2^16 by one multiplication
-  int pieces;              // that the tiles are cut into
-  int row_warps;           // kRows: warps of a CTA that take different query rows of one piece (1, or all)
-  int least;               // cost of a piece at least, in tiles
-  int entry;               // what beginning a (row, head) costs, in tiles
-  float* part;             // [row tile, pieces, 2, rows of a tile, dim]
-  float2* stats;           // [row tile, pieces, 2, rows of a tile]: reference, sum
-  long long* first;        // [batch + 1]: cost in front of a row, in tiles; then that of a piece
-  float* scores;           // [batch * heads, rows, slots], times log2 e, where weights are added up; else null
-  float2* final_stats;     // [batch * heads, rows]: reference, 1 / sum; with scores
-  uint8_t buckets[kMaxDistances];  // column of the bias table by distance
-};
-
-__device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
-                                        uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 "
-      "{%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
-__device__ __forceinline__ uint32_t transposed(uint32_t x) {
-  uint32_t r;
-  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
-  return r;
-}
-__device__ __forceinline__ uint32_t as_u32(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
-__device__ __forceinline__ __half2 as_half2(uint32_t u) { return *reinterpret_cast<__half2*>(&u); }
-// (w & low) ^ kFlip in one instruction, with `low` = 0x00ff00ff in a register (the compiler makes two of two constants: the
-// kernel reads it from its arguments)
-template <uint32_t kFlip>
-__device__ __forceinline__ uint32_t low_flipped(uint32_t w, uint32_t low) {
-  uint32_t r;
-  asm("lop3.b32 %0, %1, %2, %3, 0x6a;" : "=r"(r) : "r"(w), "r"(low), "n"(kFlip));
-  return r;
-}
-// bytes 0 and 2 of codes as two numbers (code + 128) 2^-24
-__device__ __forceinline__ uint32_t key_pair(uint32_t w, uint32_t low) { return low_flipped<0x00800080u>(w, low); }
-// bytes 0 and 2 of codes as two numbers
-__device__ __forceinline__ uint32_t value_pair(uint32_t w, uint32_t low) {
-  return as_u32(__hsub2(as_half2(low_flipped<0x64806480u>(w, low)), as_half2(0x64806480u)));
-}
-__device__ __forceinline__ float exp2_approx(float x) {
-  float r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
-  return r;
-}
-
-__device__ __forceinline__ int token_of(const Cache8Attn& p, int r) { return static_cast<int>((r * p.by_group) >> 32); }
-
-// Slots that query row r (token r / group of this call) sees: up to this one.
-__device__ __forceinline__ int last_seen(const Cache8Attn& p, int start, int end, int r) {
-  if (r >= p.rows) return -1;
-  if (!p.causal) return end - 1;
-  // the queries are the last `count` tokens held
-  const long long first = static_cast<long long>(start) + p.appended - p.count;
-  return static_cast<int>(min(first + token_of(p, r), static_cast<long long>(end) - 1));
-}
-__device__ __forceinline__ int end_of(const Cache8Attn& p, int start) {
-  return static_cast<int>(min(static_cast<long long>(start) + p.appended, static_cast<long long>(p.c.slots)));
-}
-template <typename T>
-__device__ __forceinline__ T* out_row(const Cache8Attn& p, int b, int h, int r) {
-  const int tok = token_of(p, r);
-  return static_cast<T*>(p.out) +
-         ((static_cast<long long>(b) * p.count + tok) * p.c.heads * p.group + h * p.group + r - tok * p.group) * p.c.dim;
-}
-
-// s_first[b]: what all heads of the rows in front of b cost; s_first[batch]: all.
-__device__ __forceinline__ void count_tiles(const Cache8Attn& p, long long* s_first) {
-  constexpr int kWarps = kPieceWarps, kThreads = kWarps * 32;
-  __shared__ long long s_sums[kWarps];
-  const int each = (p.c.batch + kThreads - 1) / kThreads, from = threadIdx.x * each;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  auto cost = [&](int b) {
-    const int tiles = (end_of(p, held_of(p.c, b)) + 15) >> 4;
-    return tiles == 0 ? 0LL : static_cast<long long>(tiles + p.entry) * p.c.heads;
-  };
-  long long mine = 0;
-  for (int b = from; b < min(from + each, p.c.batch); ++b) mine += cost(b);
-  long long sum = mine;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const long long u = __shfl_up_sync(0xffffffffu, sum, o);
-    if (lane >= o) sum += u;
-  }
-  if (lane == 31) s_sums[warp] = sum;
-  __syncthreads();
-  for (int w = 0; w < warp; ++w) sum += s_sums[w];
-  long long run = sum - mine;
-  for (int b = from; b < min(from + each, p.c.batch); ++b) {
-    s_first[b] = run;
-    run += cost(b);
-  }
-  if (threadIdx.x == kThreads - 1) s_first[p.c.batch] = run;
-  __syncthreads();
-}
-
-// What a score column needs beside its reference and sums.
-struct Column {
-  float scale, sum;
-  int lim, where, bias;
-};
-
-// One call's query rows row0 .. row0 + 8 * NT - 1 of a (row, head), by one warp: its lanes' parts of the first product's second
-// operand to s_query[Q2][NT][CH * 4][32], its columns to s_cols[NT * 8].
-template <typename T, int D, int NT, bool kTwo, bool kFold>
-__device__ __forceinline__ void lay_query(const Cache8Attn& p, int b, int h, int row0, int start, int end, int first_bias,
+// The query rows of a (row, head), by one warp: the lanes' parts of the first product's second operand to
+// s_query[Q2][CH * 4][32], the columns to s_cols[8].
+template <typename T, int D, bool kTwo, bool kFold>
+__device__ __forceinline__ void lay_query(const Cache8Attn& p, int b, int h, int start, int end, int first_bias,
                                           uint2* s_query, Column* s_cols) {
   constexpr int CH = D / 64, Q2 = kTwo ? 2 : 1, E = 16 / sizeof(T);
   const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int dropped = p.c.position != nullptr ? p.c.dropped[b] : 0;
   const int q_first = static_cast<int>(static_cast<long long>(start) + p.appended - p.count);
-#pragma unroll
-  for (int nt = 0; nt < NT; ++nt) {
-    const int r = kFold ? g & 3 : row0 + nt * 8 + g, i = token_of(p, min(r, p.rows - 1)), in_group = min(r, p.rows - 1) - i * p.group;
+  {
+    const int r = kFold ? g & 3 : g, i = token_of(p, min(r, p.rows - 1)), in_group = min(r, p.rows - 1) - i * p.group;
     const T* src = static_cast<const T*>(p.q) + b * p.q_sb + i * p.q_st + (h * p.group + in_group) * p.q_sh + 16 * t;
     float x[CH][16];
     uint32_t most = 0;
@@ -225,7 +97,7 @@ __device__ __forceinline__ void lay_query(const Cache8Attn& p, int b, int h, int
           }
         }
 #pragma unroll
-        for (int w = 0; w < Q2; ++w) s_query[((w * NT + nt) * CH * 4 + ch * 4 + j) * 32 + lane] = make_uint2(f[w][0], f[w][1]);
+        for (int w = 0; w < Q2; ++w) s_query[(w * CH * 4 + ch * 4 + j) * 32 + lane] = make_uint2(f[w][0], f[w][1]);
       }
     sum += __shfl_xor_sync(0xffffffffu, sum, 1);
     sum += __shfl_xor_sync(0xffffffffu, sum, 2);
@@ -237,26 +109,25 @@ __device__ __forceinline__ void lay_query(const Cache8Attn& p, int b, int h, int
       col.lim = r < p.rows ? last_seen(p, start, end, r) : 0x7fffffff;  // (a column without a row hinders nobody)
       col.where = q_first + i + dropped;
       col.bias = first_bias + in_group * p.table_stride;
-      s_cols[nt * 8 + g] = col;
+      s_cols[g] = col;
     }
   }
 }
 
 enum Deal {
   kRowHead,  // a CTA takes a (row, head), and appends
-  kPieces,   // a CTA takes a piece of the tiles
-  kRows      // a warp takes a piece of the tiles, or warps of a CTA different query rows of one piece
+  kPieces    // a CTA takes a piece of the tiles
 };
 
-// NT: tiles of 8 query rows; MT: tiles of 16 tokens a step; kTwo: operands as two fp16 numbers each.
+// MT: tiles of 16 tokens a step; kTwo: operands as two fp16 numbers each.
 // kFold: up to four query rows, twice in the 8 columns: of a step's two tiles the first counts in columns 0 to 3 and the second
 // in 4 to 7, so that what is done for scores and probabilities is done once for both.
-template <typename T, int D, int NT, int MT, bool kTwo, Deal kDeal, int kWarps, bool kFold>
-__global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 16 / kWarps : 1)
+template <typename T, int D, int MT, bool kTwo, Deal kDeal, int kWarps, bool kFold>
+__global__ void __launch_bounds__(kWarps * 32, 16 / kWarps)
     cache8_attention_kernel(const __grid_constant__ Cache8Attn p, const __grid_constant__ NewTokens<T> fresh) {
-  constexpr bool kBlock = kDeal == kRowHead, kTeam = kDeal != kRows;  // kTeam: the warps of a CTA share tiles and query rows
-  static_assert(!kTeam || NT == 1, "a team takes 8 query rows");
-  static_assert(!kFold || (kTeam && MT == 2), "two tiles fold");
+  constexpr bool kBlock = kDeal == kRowHead;
+  constexpr int NT = 1;  // tiles of 8 query rows
+  static_assert(!kFold || MT == 2, "two tiles fold");
   constexpr int MS = kFold ? 1 : MT;           // tiles of scores that a lane has
   constexpr int kParts = kFold ? 2 : 1;        // columns of a query row
   constexpr int kThreads = kWarps * 32;
@@ -264,26 +135,22 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 16 / kWarps : 1)
   constexpr int VB = D / 8;        // channels a lane has in the second product
   constexpr int MI = D / 16;       // row tiles of the second product
   constexpr int Q2 = kTwo ? 2 : 1;
-  constexpr bool kQueryRegs = NT == 1 && D == 64;  // the query's operand is kept in registers
+  constexpr bool kQueryRegs = D == 64;  // the query's operand is kept in registers
   constexpr int kQuery = Q2 * NT * CH * 4 * 32;
-  // the query's operand of the team or of each warp; the bias table, times log2 e (kRowHead: of the head's rows); the sums
-  // of a team's warps [kWarps][rows][D]; kRowHead: scores [rows][slots]
+  // the query's operand; the bias table, times log2 e (kRowHead: of the head's rows); the sums
+  // of the warps [kWarps][rows][D]; kRowHead: scores [rows][slots]
   extern __shared__ uint2 s_dyn[];
-  float* s_table = reinterpret_cast<float*>(s_dyn + (kTeam ? 1 : kWarps) * kQuery);
+  uint2* s_query = s_dyn;
+  float* s_table = reinterpret_cast<float*>(s_dyn + kQuery);
   __shared__ long long s_first[kBlock ? 1 : kMaxBatch + 1];
   __shared__ uint8_t s_buckets[kMaxDistances];
-  __shared__ Column s_cols[(kTeam ? 1 : kWarps) * NT * 8];
-  __shared__ float2 s_stats[kTeam ? kWarps * kParts : 1][8];
+  __shared__ Column s_cols[8];
+  __shared__ float2 s_stats[kWarps * kParts][8];
   __shared__ float2 s_rows[8];
   const Cache8& c = p.c;
   const uint32_t low = p.low;
   const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3, wid = threadIdx.x >> 5;
-  // the piece of the tiles, and the first query row
-  const int unit = kTeam ? blockIdx.x : p.row_warps > 1 ? blockIdx.x : blockIdx.x * kWarps + wid;
-  const int row_tile = kTeam ? 0 : p.row_warps > 1 ? blockIdx.y * kWarps + wid : blockIdx.y;
-  const int row0 = row_tile * NT * 8;
-  uint2* s_query = s_dyn + (kTeam ? 0 : wid * kQuery);
-  Column* s_col = s_cols + (kTeam ? 0 : wid * NT * 8);
+  const int unit = blockIdx.x;  // (kPieces)
 
   const int biases = p.table == nullptr ? 0 : (kBlock ? 1 : c.heads) * p.group * p.table_stride;
   if (p.table != nullptr) {
@@ -302,7 +169,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 16 / kWarps : 1)
   if constexpr (kBlock) {
     b = blockIdx.y;
   } else {
-    count_tiles(p, s_first);
+    count_tiles<kWarps>(p, s_first);
     const long long all = s_first[c.batch];
     const long long piece = max((all + p.pieces - 1) / p.pieces, static_cast<long long>(p.least));
     if (blockIdx.x == 0 && blockIdx.y == 0) {
@@ -313,7 +180,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 16 / kWarps : 1)
     chain_release();
     at = unit * piece;
     stop = min(at + piece, all);
-    if (at >= stop || row0 >= p.rows) return;
+    if (at >= stop) return;
     for (int step = 1 << 11; step > 0; step >>= 1)  // the last row that begins at or before `at` and holds something
       if (b + step < c.batch && s_first[b + step] <= at) b += step;
   }
@@ -336,8 +203,8 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 16 / kWarps : 1)
       tile1 = static_cast<int>(min(stop - seg, static_cast<long long>(tiles)));
       if (tile1 <= 0) break;  // (no more than a part of what the beginning costs)
     }
-    constexpr int kStep = (kTeam ? kWarps : 1) * MT;
-    const int mine = tile0 + (kTeam ? wid * MT : 0);  // this warp's first tile
+    constexpr int kStep = kWarps * MT;
+    const int mine = tile0 + wid * MT;  // this warp's first tile
     const long long bh = static_cast<long long>(b) * c.heads + h;
 
     const long long slots0 = bh * c.slots;
@@ -353,9 +220,8 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 16 / kWarps : 1)
     float ka[MS], va[MS];
     int place[MS][2];
     const int fold = kFold ? t >> 1 : 0;  // which of the two tiles this lane's columns count
-    // What the kernel in front may have written is read through L2; several rows' warps share lines in L1, and wait for it to
-    // end by their launch.
-    auto get = [](const auto* ptr) { return kTeam ? __ldcg(ptr) : *ptr; };
+    // (what the kernel in front may have written is read through L2)
+    auto get = [](const auto* ptr) { return __ldcg(ptr); };
     // (a tile past the end is read again, and hidden)
     auto load_k = [&](int tile) {
 #pragma unroll
@@ -413,7 +279,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 16 / kWarps : 1)
         load_k(mine);
         load_v(mine);
       }
-      if (wid == 0) lay_query<T, D, NT, kTwo, kFold>(p, b, h, row0, start, end, first_bias, s_query, s_col);
+      if (wid == 0) lay_query<T, D, kTwo, kFold>(p, b, h, start, end, first_bias, s_query, s_cols);
       if (few) {
         uint32_t most = max(max(abs_bits(v[0]), abs_bits(v[1])), max(abs_bits(v[2]), abs_bits(v[3])));
         most = __reduce_max_sync(0xffffffffu, most);
@@ -459,17 +325,12 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 16 / kWarps : 1)
       }
       at = stop;
     } else {
-      if (kTeam && mine < tile1) {
+      if (mine < tile1) {
         load_k(mine);
         load_v(mine);
       }
-      if (!kTeam || wid == 0) lay_query<T, D, NT, kTwo, kFold>(p, b, h, row0, start, end, first_bias, s_query, s_col);
-      if (kTeam) __syncthreads();
-      else __syncwarp();
-      if (!kTeam) {
-        load_k(mine);
-        load_v(mine);
-      }
+      if (wid == 0) lay_query<T, D, kTwo, kFold>(p, b, h, start, end, first_bias, s_query, s_cols);
+      __syncthreads();
     }
 
     // ---- the query: this lane's part of the operand, and what it needs for score columns 2t and 2t + 1 ----
@@ -480,12 +341,8 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 16 / kWarps : 1)
 #pragma unroll
         for (int j = 0; j < CH * 4; ++j) qf[w][j] = s_query[(w * CH * 4 + j) * 32 + lane];
     }
-    Column cols[NT == 1 ? 2 : 1];
-    if constexpr (NT == 1) cols[0] = s_col[2 * t], cols[1] = s_col[2 * t + 1];
-    auto column = [&](int nt, int e) -> const Column& {
-      if constexpr (NT == 1) return cols[e];
-      else return s_col[nt * 8 + 2 * t + e];
-    };
+    const Column cols[2] = {s_cols[2 * t], s_cols[2 * t + 1]};
+    auto column = [&](int, int e) -> const Column& { return cols[e]; };
     int all_see = end - 1;  // slots up to this one are seen by every row of the tile
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) all_see = min(all_see, min(column(nt, 0).lim, column(nt, 1).lim));
@@ -503,7 +360,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 16 / kWarps : 1)
       for (int e = 0; e < 2; ++e) {
         ref[nt][e] = kNothing;
         l[nt][e] = v_inv[nt][e] = 0.f;
-        v_lim[nt][e] = (kFold ? (2 * t + e) & 3 : row0 + nt * 8 + 2 * t + e) < p.rows ? 0.f : INFINITY;  // (without a row: none)
+        v_lim[nt][e] = (kFold ? (2 * t + e) & 3 : 2 * t + e) < p.rows ? 0.f : INFINITY;  // (without a row: none)
       }
     }
 
@@ -535,7 +392,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 16 / kWarps : 1)
             for (int w = 0; w < Q2; ++w) {
               uint2 q;
               if constexpr (kQueryRegs) q = qf[w][ch * 4 + j];
-              else q = s_query[((w * NT + nt) * CH * 4 + ch * 4 + j) * 32 + lane];
+              else q = s_query[(w * CH * 4 + ch * 4 + j) * 32 + lane];
 #pragma unroll
               for (int mt = 0; mt < MT; ++mt) mma_f16(st[mt][nt], a[mt][0], a[mt][1], a[mt][2], a[mt][3], q.x, q.y);
             }
@@ -601,7 +458,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 16 / kWarps : 1)
           for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-              const int r = kFold ? (2 * t + e) & 3 : row0 + nt * 8 + 2 * t + e;
+              const int r = kFold ? (2 * t + e) & 3 : 2 * t + e;
               if (r < p.rows) {
                 to[r * c.slots + s0 + g] = s[ms][nt][e];
                 to[r * c.slots + s0 + g + 8] = s[ms][nt][2 + e];
@@ -702,8 +559,8 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 16 / kWarps : 1)
     // The whole (row, head), or a piece of it: a unit has one that began before its own first tile at most, and one that goes
     // on behind its last.
     const bool whole = tile0 == 0 && tile1 == tiles;
-    const long long slot = ((static_cast<long long>(row_tile) * p.pieces + unit) * 2 + (tile0 == 0 ? 1 : 0)) * NT * 8;
-    if constexpr (kTeam) {
+    const long long slot = (unit * 2LL + (tile0 == 0 ? 1 : 0)) * 8;
+    {
       // ---- the warps meet; the weights of the first slots are requested ahead ----
       constexpr int kAhead = 4;
       float weight[kAhead];
@@ -781,38 +638,6 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 16 / kWarps : 1)
           c.weight[slots0 + s] = (s >= start ? 0.f : c.weight[slots0 + s]) + given(s);
       }
       if (!kBlock) __syncthreads();  // the next piece's query and sums
-    } else {
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          float sum = l[nt][e];
-          sum += __shfl_xor_sync(0xffffffffu, sum, 4);
-          sum += __shfl_xor_sync(0xffffffffu, sum, 8);
-          sum += __shfl_xor_sync(0xffffffffu, sum, 16);
-          const int col = nt * 8 + 2 * t + e, r = row0 + col;
-          if (r >= p.rows) continue;
-          // (a row that nothing was seen of may have sums of 0 * NaN)
-          const float f = v_lim[nt][e] * (0.25f / 127.f) * (whole ? 1.f / sum : 1.f);
-          float x[VB];
-#pragma unroll
-          for (int i = 0; i < MI; ++i) {
-            x[2 * i] = sum == 0.f ? 0.f : o[nt][i][e] * f;
-            x[2 * i + 1] = sum == 0.f ? 0.f : o[nt][i][2 + e] * f;
-          }
-          if (whole) {
-            T* dst = out_row<T>(p, b, h, r) + VB * g;
-#pragma unroll
-            for (int i = 0; i < VB; ++i) dst[i] = from_float<T>(x[i]);
-            if (g == 0 && p.scores != nullptr) p.final_stats[bh * p.rows + r] = make_float2(ref[nt][e], sum == 0.f ? 0.f : 1.f / sum);
-          } else {
-            float4* dst = reinterpret_cast<float4*>(p.part + (slot + col) * D + VB * g);
-#pragma unroll
-            for (int i = 0; i < VB / 4; ++i) dst[i] = make_float4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]);
-            if (g == 0) p.stats[slot + col] = make_float2(ref[nt][e], sum);
-          }
-        }
-      __syncwarp();  // the next piece's query
     }
     if constexpr (!kBlock) at = seg + tile1;
   }
@@ -909,27 +734,8 @@ __global__ void __launch_bounds__(kWeightThreads) cache8_weight_kernel(const __g
   *weight = __ldcg(weight) + sum;
 }
 
-// Launches a kernel that may begin while the one in front of it still runs; it waits for it by itself (chain_wait).
-template <typename... Params, typename... Args>
-cudaError_t launch_behind(bool behind, void (*kernel)(Params...), dim3 grid, int threads, size_t smem,
-                          cudaStream_t stream, Args&&... args) {
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = grid;
-  cfg.blockDim = dim3(threads);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = behind ? 1 : 0;
-  count_launches(1);
-  return cudaLaunchKernelEx(&cfg, kernel, std::forward<Args>(args)...);
-}
-
 // Shared memory of a team, beside the query and the biases.
 constexpr int kMaxTeamBytes = 72 * 1024;
-constexpr int kRowWarps = 8;
 size_t team_bytes(const Cache8& c, int rows, bool scores) {
   return 4ull * rows * ((rows <= 4 && c.dim == 64 ? 16ull : 8ull) * c.dim + (scores && c.weight != nullptr ? c.slots : 0));
 }
@@ -940,30 +746,24 @@ bool by_row_head(const Cache8& c, int rows) {
   return rows <= 8 && team_bytes(c, rows, true) <= kMaxTeamBytes && (c.slots <= 1024 || (c.slots <= 8192 && bh >= 6LL * num_sms()));
 }
 
-constexpr int tile_rows_of(int rows) { return rows <= 8 ? 8 : 32; }
-
-template <typename T, int D, int NT, int MT, bool kTwo, Deal kDeal, int kWarps, bool kFold>
+template <typename T, int D, int MT, bool kTwo, Deal kDeal, int kWarps, bool kFold>
 cudaError_t launch_tile(const Cache8Attn& p, const NewTokens<T>& fresh, bool behind, cudaStream_t stream) {
-  constexpr bool kBlock = kDeal == kRowHead, kTeam = kDeal != kRows;
-  constexpr size_t query = sizeof(uint2) * (kTeam ? 1 : kWarps) * (kTwo ? 2 : 1) * NT * (D / 64) * 4 * 32;
+  constexpr bool kBlock = kDeal == kRowHead;
+  constexpr size_t query = sizeof(uint2) * (kTwo ? 2 : 1) * (D / 64) * 4 * 32;
   const size_t table = p.table == nullptr ? 0 : static_cast<size_t>((kBlock ? 1 : p.c.heads) * p.group * p.table_stride + 3) / 4 * 16;
-  const size_t smem = query + table + (kTeam ? team_bytes(p.c, p.rows, kBlock) : 0);
+  const size_t smem = query + table + team_bytes(p.c, p.rows, kBlock);
   static bool set[64] = {false};
   int dev = 0;
   cudaGetDevice(&dev);
   if (!set[dev & 63]) {
-    cudaError_t e = cudaFuncSetAttribute(cache8_attention_kernel<T, D, NT, MT, kTwo, kDeal, kWarps, kFold>,
+    cudaError_t e = cudaFuncSetAttribute(cache8_attention_kernel<T, D, MT, kTwo, kDeal, kWarps, kFold>,
                                          cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                         static_cast<int>(query) + kMaxBiases * 4 + (kTeam ? kMaxTeamBytes : 0));
+                                         static_cast<int>(query) + kMaxBiases * 4 + kMaxTeamBytes);
     if (e != cudaSuccess) return e;
     set[dev & 63] = true;
   }
-  const int row_tiles = (p.rows + NT * 8 - 1) / (NT * 8);
-  const dim3 grid = kBlock            ? dim3(p.c.heads, p.c.batch)
-                    : kTeam           ? dim3(p.pieces)
-                    : p.row_warps > 1 ? dim3(p.pieces, (row_tiles + kWarps - 1) / kWarps)
-                                      : dim3(p.pieces / kWarps, row_tiles);
-  return launch_behind(behind, cache8_attention_kernel<T, D, NT, MT, kTwo, kDeal, kWarps, kFold>, grid, kWarps * 32, smem, stream, p, fresh);
+  const dim3 grid = kBlock ? dim3(p.c.heads, p.c.batch) : dim3(p.pieces);
+  return launch_behind(behind, cache8_attention_kernel<T, D, MT, kTwo, kDeal, kWarps, kFold>, grid, kWarps * 32, smem, stream, p, fresh);
 }
 
 template <typename T, bool kTwo>
@@ -973,25 +773,22 @@ cudaError_t launch_row_heads(const Cache8Attn& p, const T5xNewTokens* tokens, cu
   const bool many = static_cast<long long>(p.c.batch) * p.c.heads >= 2LL * num_sms();
   auto launch_with = [&](auto kernel_warps) {
     constexpr int W = decltype(kernel_warps)::value;
-    if (p.c.dim == 128) return launch_tile<T, 128, 1, 1, kTwo, kRowHead, W, false>(p, fresh, false, stream);
-    return p.rows <= 4 ? launch_tile<T, 64, 1, 2, kTwo, kRowHead, W, true>(p, fresh, false, stream)
-                       : launch_tile<T, 64, 1, 2, kTwo, kRowHead, W, false>(p, fresh, false, stream);
+    if (p.c.dim == 128) return launch_tile<T, 128, 1, kTwo, kRowHead, W, false>(p, fresh, false, stream);
+    return p.rows <= 4 ? launch_tile<T, 64, 2, kTwo, kRowHead, W, true>(p, fresh, false, stream)
+                       : launch_tile<T, 64, 2, kTwo, kRowHead, W, false>(p, fresh, false, stream);
   };
   return many ? launch_with(std::integral_constant<int, 4>()) : launch_with(std::integral_constant<int, 8>());
 }
 
 template <typename T, bool kTwo>
 cudaError_t launch_pieces(const Cache8Attn& p, bool behind, cudaStream_t stream) {
-  const int tile_rows = tile_rows_of(p.rows);
+  const int type = sizeof(T) == 4 ? 2 : std::is_same<T, __half>::value ? 1 : 0;
+  const int tile_rows = p.rows <= 8 ? 8 : row_tile_of(type);
   const NewTokens<T> none = {};
-  cudaError_t e;
-  if (p.c.dim == 64)
-    e = p.rows <= 4      ? launch_tile<T, 64, 1, 2, kTwo, kPieces, 8, true>(p, none, behind, stream)
-        : tile_rows == 8 ? launch_tile<T, 64, 1, 2, kTwo, kPieces, 8, false>(p, none, behind, stream)
-                         : launch_tile<T, 64, 4, 1, kTwo, kRows, kRowWarps, false>(p, none, false, stream);
-  else
-    e = tile_rows == 8 ? launch_tile<T, 128, 1, 1, kTwo, kPieces, 8, false>(p, none, behind, stream)
-                       : launch_tile<T, 128, 4, 1, kTwo, kRows, kRowWarps, false>(p, none, false, stream);
+  cudaError_t e = p.rows > 8        ? launch_cache8_rows(p, type, behind, stream)
+                         : p.c.dim == 128  ? launch_tile<T, 128, 1, kTwo, kPieces, 8, false>(p, none, behind, stream)
+                         : p.rows <= 4     ? launch_tile<T, 64, 2, kTwo, kPieces, 8, true>(p, none, behind, stream)
+                                           : launch_tile<T, 64, 2, kTwo, kPieces, 8, false>(p, none, behind, stream);
   if (e != cudaSuccess) return e;
   const dim3 rows(static_cast<unsigned>(p.c.batch) * p.c.heads, p.rows);
   e = p.c.dim == 64 ? launch_behind(true, cache8_join_kernel<T, 64>, rows, kJoinThreads, 0, stream, p, tile_rows)
@@ -1020,25 +817,23 @@ struct Plan {
   int pieces = 0, least = 0, entry = 0, row_warps = 1;
   size_t part = 0, stats = 0, first = 0, scores = 0, final_stats = 0, total = 0;
 };
-Plan plan(Cache8 c, int rows) {
+Plan plan(Cache8 c, int rows, int type) {
   Plan w = {};
   if (by_row_head(c, rows)) return w;
   c.batch = std::min(c.batch, kMaxBatch);
-  const int tile_rows = tile_rows_of(rows), row_tiles = (rows + tile_rows - 1) / tile_rows;
-  // the CTAs, or warps, that the SMs hold at a time, shared by the tiles of query rows; no piece of under 64 tokens a warp
-  const bool team = tile_rows == 8;
-  w.row_warps = !team && row_tiles >= 4 ? kRowWarps : 1;
-  const int unit_warps = team ? 8 : 1;
-  // (a CTA does some four tiles a us; us for long contexts of all lengths / for 4 x 16 heads of 64 channels by up to 16384 tokens
-  // with 8: 101 / 42, 16: 93 / 30, 24: 93 / 26, 40: 93 / 25)
-  w.entry = team ? 24 : 6;
-  w.least = 4 * unit_warps + w.entry;
-  const long long room = team              ? 2LL * num_sms()
-                         : w.row_warps > 1 ? num_sms() / ((row_tiles + kRowWarps - 1) / kRowWarps)
-                                           : static_cast<long long>(num_sms()) * kRowWarps / row_tiles;
+  const int tile_rows = rows <= 8 ? 8 : row_tile_of(type), row_tiles = (rows + tile_rows - 1) / tile_rows;
+  // Pieces for all CTAs that the SMs hold at a time, none of under 64 tokens a warp. Beginning a (row, head) costs as much as
+  // 24 tiles where a CTA does some four of them a us (us for long contexts of all lengths / for 4 x 16 heads of 64 channels by
+  // up to 16384 tokens with 8: 101 / 42, 16: 93 / 30, 24: 93 / 26, 40: 93 / 25).
+  w.entry = rows <= 8 ? 24 : 6;
+  w.least = 32 + w.entry;
+  long long room = 2LL * num_sms();
+  if (rows > 8) {
+    w.row_warps = row_tiles <= 2 ? 2 : row_tiles <= 4 ? 4 : kRowWarps;
+    room = num_sms() / ((row_tiles + w.row_warps - 1) / w.row_warps);
+  }
   const long long most = static_cast<long long>(c.batch) * c.heads * (c.slots / 16 + w.entry) / w.least + 1;
   w.pieces = static_cast<int>(std::max<long long>(1, std::min(room, most)));
-  if (!team && w.row_warps == 1) w.pieces = (w.pieces + kRowWarps - 1) / kRowWarps * kRowWarps;
   const size_t bh = static_cast<size_t>(c.batch) * c.heads;
   auto take = [&](size_t bytes) {
     const size_t at = w.total;
@@ -1082,7 +877,7 @@ T5X_API long long t5x_cache8_attention_bytes(const T5xCache8* cache, const T5xCa
   if (int e = t5x::check_cache8("cache8_attention", c)) return e;
   if (int e = t5x::check_query(c, q, n)) return e;
   if (c.batch == 0) return 0;
-  return static_cast<long long>(t5x::plan(c, q->count * q->group).total);
+  return static_cast<long long>(t5x::plan(c, q->count * q->group, q->type).total);
 }
 
 T5X_API int t5x_cache8_attention(const T5xCache8* cache, const T5xCache8Query* q, const T5xNewTokens* n, void* workspace,
@@ -1116,7 +911,7 @@ T5X_API int t5x_cache8_attention(const T5xCache8* cache, const T5xCache8Query* q
   p.appended = n ? n->count : 0;
   p.scale = q->scale;
   p.low = 0x00ff00ffu;
-  const t5x::Plan w = t5x::plan(c, p.rows);
+  const t5x::Plan w = t5x::plan(c, p.rows, q->type);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (t5x::by_row_head(c, p.rows)) {
     p.scores = nullptr;

@@ -1,0 +1,159 @@
+// What the kernels of attention over a cache in 8 bits share: the arguments of a call, the work's division into pieces, and
+// the small operations on codes and fragments (cache8_attention.cu).
+#pragma once
+#include <utility>
+
+#include "cache8.cuh"
+
+namespace t5x {
+
+constexpr int kMaxDistances = 1024;
+constexpr int kMaxBatch = 2048;  // rows of one launch
+constexpr int kMaxBiases = 8192;  // values of a bias table
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kPeak = 4.f;     // exponent of a probability at the reference
+constexpr float kLimit = 12.6f;  // of the largest; times 4 it is still an fp16 number
+constexpr float kNothing = -3e38f;  // the reference of a row that has seen nothing
+
+struct Cache8Attn {
+  Cache8 c;
+  const void* q;
+  void* out;
+  const float* table;
+  const uint8_t* mask;
+  long long q_sb, q_st, q_sh, mask_stride;
+  int table_stride, q_vec;  // q_vec: whole 16 bytes of a query may be loaded
+  int count, group, rows;  // queries a row, heads a key head, their product
+  int distances, mask_len, causal;
+  int appended;            // tokens of this call behind c.index
+  float scale;
+  uint32_t low;            // 0x00ff00ff
+  unsigned long long by_group;  // 2^32 / group, rounded up: r / group for r below 2^16 by one multiplication
+  int pieces;              // that the tiles are cut into
+  int row_warps;           // over many query rows: warps of a CTA that take different rows (2, 4 or all 8)
+  int least;               // cost of a piece at least, in tiles
+  int entry;               // what beginning a (row, head) costs, in tiles
+  float* part;             // [row tile, pieces, 2, rows of a tile, dim]
+  float2* stats;           // [row tile, pieces, 2, rows of a tile]: reference, sum
+  long long* first;        // [batch + 1]: cost in front of a row, in tiles; then that of a piece
+  float* scores;           // [batch * heads, rows, slots], times log2 e, where weights are added up; else null
+  float2* final_stats;     // [batch * heads, rows]: reference, 1 / sum; with scores
+  uint8_t buckets[kMaxDistances];  // column of the bias table by distance
+};
+
+__device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                        uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 "
+      "{%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t transposed(uint32_t x) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
+  return r;
+}
+__device__ __forceinline__ uint32_t as_u32(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
+__device__ __forceinline__ __half2 as_half2(uint32_t u) { return *reinterpret_cast<__half2*>(&u); }
+// (w & low) ^ kFlip in one instruction, with `low` = 0x00ff00ff in a register (the compiler makes two of two constants: the
+// kernel reads it from its arguments)
+template <uint32_t kFlip>
+__device__ __forceinline__ uint32_t low_flipped(uint32_t w, uint32_t low) {
+  uint32_t r;
+  asm("lop3.b32 %0, %1, %2, %3, 0x6a;" : "=r"(r) : "r"(w), "r"(low), "n"(kFlip));
+  return r;
+}
+// bytes 0 and 2 of codes as two numbers (code + 128) 2^-24
+__device__ __forceinline__ uint32_t key_pair(uint32_t w, uint32_t low) { return low_flipped<0x00800080u>(w, low); }
+// bytes 0 and 2 of codes as two numbers
+__device__ __forceinline__ uint32_t value_pair(uint32_t w, uint32_t low) {
+  return as_u32(__hsub2(as_half2(low_flipped<0x64806480u>(w, low)), as_half2(0x64806480u)));
+}
+__device__ __forceinline__ float exp2_approx(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+
+__device__ __forceinline__ int token_of(const Cache8Attn& p, int r) { return static_cast<int>((r * p.by_group) >> 32); }
+
+// Slots that query row r (token r / group of this call) sees: up to this one.
+__device__ __forceinline__ int last_seen(const Cache8Attn& p, int start, int end, int r) {
+  if (r >= p.rows) return -1;
+  if (!p.causal) return end - 1;
+  // the queries are the last `count` tokens held
+  const long long first = static_cast<long long>(start) + p.appended - p.count;
+  return static_cast<int>(min(first + token_of(p, r), static_cast<long long>(end) - 1));
+}
+__device__ __forceinline__ int end_of(const Cache8Attn& p, int start) {
+  return static_cast<int>(min(static_cast<long long>(start) + p.appended, static_cast<long long>(p.c.slots)));
+}
+template <typename T>
+__device__ __forceinline__ T* out_row(const Cache8Attn& p, int b, int h, int r) {
+  const int tok = token_of(p, r);
+  return static_cast<T*>(p.out) +
+         ((static_cast<long long>(b) * p.count + tok) * p.c.heads * p.group + h * p.group + r - tok * p.group) * p.c.dim;
+}
+
+// s_first[b]: what all heads of the rows in front of b cost; s_first[batch]: all.
+template <int kWarps>
+__device__ __forceinline__ void count_tiles(const Cache8Attn& p, long long* s_first) {
+  constexpr int kThreads = kWarps * 32;
+  __shared__ long long s_sums[kWarps];
+  const int each = (p.c.batch + kThreads - 1) / kThreads, from = threadIdx.x * each;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  auto cost = [&](int b) {
+    const int tiles = (end_of(p, held_of(p.c, b)) + 15) >> 4;
+    return tiles == 0 ? 0LL : static_cast<long long>(tiles + p.entry) * p.c.heads;
+  };
+  long long mine = 0;
+  for (int b = from; b < min(from + each, p.c.batch); ++b) mine += cost(b);
+  long long sum = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const long long u = __shfl_up_sync(0xffffffffu, sum, o);
+    if (lane >= o) sum += u;
+  }
+  if (lane == 31) s_sums[warp] = sum;
+  __syncthreads();
+  for (int w = 0; w < warp; ++w) sum += s_sums[w];
+  long long run = sum - mine;
+  for (int b = from; b < min(from + each, p.c.batch); ++b) {
+    s_first[b] = run;
+    run += cost(b);
+  }
+  if (threadIdx.x == kThreads - 1) s_first[p.c.batch] = run;
+  __syncthreads();
+}
+
+// What a score column needs beside its reference and sums.
+struct Column {
+  float scale, sum;
+  int lim, where, bias;
+};
+
+// Launches a kernel that may begin while the one in front of it still runs; it waits for it by itself (chain_wait).
+template <typename... Params, typename... Args>
+cudaError_t launch_behind(bool behind, void (*kernel)(Params...), dim3 grid, int threads, size_t smem,
+                          cudaStream_t stream, Args&&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = behind ? 1 : 0;
+  count_launches(1);
+  return cudaLaunchKernelEx(&cfg, kernel, std::forward<Args>(args)...);
+}
+
+// Attention of many query rows (cache8_rows.cu). type: 0 bf16, 1 fp16, 2 fp32.
+constexpr int kRowWarps = 8;
+constexpr int row_tile_of(int type) { return type == 2 ? 16 : 32; }  // query rows of a warp
+cudaError_t launch_cache8_rows(const Cache8Attn& p, int type, bool behind, cudaStream_t stream);
+
+}  // namespace t5x
