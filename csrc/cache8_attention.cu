@@ -783,7 +783,7 @@ cudaError_t launch_row_heads(const Cache8Attn& p, const T5xNewTokens* tokens, cu
 template <typename T, bool kTwo>
 cudaError_t launch_pieces(const Cache8Attn& p, bool behind, cudaStream_t stream) {
   const int type = sizeof(T) == 4 ? 2 : std::is_same<T, __half>::value ? 1 : 0;
-  const int tile_rows = p.rows <= 8 ? 8 : row_tile_of(type);
+  const int tile_rows = p.rows <= 8 ? 8 : row_tile_of(type, p.rows);
   const NewTokens<T> none = {};
   cudaError_t e = p.rows > 8        ? launch_cache8_rows(p, type, behind, stream)
                          : p.c.dim == 128  ? launch_tile<T, 128, 1, kTwo, kPieces, 8, false>(p, none, behind, stream)
@@ -821,15 +821,15 @@ Plan plan(Cache8 c, int rows, int type) {
   Plan w = {};
   if (by_row_head(c, rows)) return w;
   c.batch = std::min(c.batch, kMaxBatch);
-  const int tile_rows = rows <= 8 ? 8 : row_tile_of(type), row_tiles = (rows + tile_rows - 1) / tile_rows;
+  const int tile_rows = rows <= 8 ? 8 : row_tile_of(type, rows), row_tiles = (rows + tile_rows - 1) / tile_rows;
   // Pieces for all CTAs that the SMs hold at a time, none of under 64 tokens a warp. Beginning a (row, head) costs as much as
   // 24 tiles where a CTA does some four of them a us (us for long contexts of all lengths / for 4 x 16 heads of 64 channels by
   // up to 16384 tokens with 8: 101 / 42, 16: 93 / 30, 24: 93 / 26, 40: 93 / 25).
   w.entry = rows <= 8 ? 24 : 6;
-  w.least = 32 + w.entry;
+  w.least = (rows <= 8 ? 32 : 8) + w.entry;
   long long room = 2LL * num_sms();
   if (rows > 8) {
-    w.row_warps = row_tiles <= 2 ? 2 : row_tiles <= 4 ? 4 : kRowWarps;
+    w.row_warps = row_tiles > 4 ? kRowWarps : row_tiles > 2 || rows > kFewRows ? 4 : 2;
     room = num_sms() / ((row_tiles + w.row_warps - 1) / w.row_warps);
   }
   const long long most = static_cast<long long>(c.batch) * c.heads * (c.slots / 16 + w.entry) / w.least + 1;

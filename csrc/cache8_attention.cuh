@@ -30,7 +30,7 @@ struct Cache8Attn {
   uint32_t low;            // 0x00ff00ff
   unsigned long long by_group;  // 2^32 / group, rounded up: r / group for r below 2^16 by one multiplication
   int pieces;              // that the tiles are cut into
-  int row_warps;           // over many query rows: warps of a CTA that take different rows (2, 4 or all 8)
+  int row_warps;           // over many query rows: warps of a CTA that take different rows (2 or 4 of few rows, else 4 or 8)
   int least;               // cost of a piece at least, in tiles
   int entry;               // what beginning a (row, head) costs, in tiles
   float* part;             // [row tile, pieces, 2, rows of a tile, dim]
@@ -153,7 +153,8 @@ cudaError_t launch_behind(bool behind, void (*kernel)(Params...), dim3 grid, int
 
 // Attention of many query rows (cache8_rows.cu). type: 0 bf16, 1 fp16, 2 fp32.
 constexpr int kRowWarps = 8;
-constexpr int row_tile_of(int type) { return type == 2 ? 16 : 32; }  // query rows of a warp
+constexpr int kFewRows = 64;
+constexpr int row_tile_of(int type, int rows) { return type == 2 || rows <= kFewRows ? 16 : 32; }  // query rows of a warp
 cudaError_t launch_cache8_rows(const Cache8Attn& p, int type, bool behind, cudaStream_t stream);
 
 }  // namespace t5x

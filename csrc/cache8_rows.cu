@@ -39,7 +39,7 @@ __device__ __forceinline__ uint2 numbers(uint32_t codes) {
 // What a query row needs.
 struct Row {
   float scale;
-  int lim, where, bias;
+  int lim, where, bias;  // (the last two are read where there are biases)
 };
 
 // The 16 * M query rows from row0 on of a (row, head), by one warp, a row to 4 lanes: the first operand of Q K^T to
@@ -52,25 +52,33 @@ __device__ __forceinline__ void lay_rows(const Cache8Attn& p, int b, int h, int 
   const int dropped = p.c.position != nullptr ? p.c.dropped[b] : 0;
   const int q_first = static_cast<int>(static_cast<long long>(start) + p.appended - p.count);
   uint32_t* to = reinterpret_cast<uint32_t*>(s_query);
-#pragma unroll 1
-  for (int i = 0; i < 2 * M; ++i) {  // row 8 i + g
-    const int r = row0 + 8 * i + g, real = min(r, p.rows - 1), token = token_of(p, real), in_group = real - token * p.group;
+  using Pair = typename std::conditional<sizeof(T) == 4, uint2, uint32_t>::type;
+  Pair part[2 * M][J][2];  // channels 16 j + 2 t, + 1, + 8, + 9 of row 8 i + g
+#pragma unroll
+  for (int i = 0; i < 2 * M; ++i) {
+    const int r = min(row0 + 8 * i + g, p.rows - 1), token = token_of(p, r), in_group = r - token * p.group;
     const T* src = static_cast<const T*>(p.q) + b * p.q_sb + token * p.q_st + (h * p.group + in_group) * p.q_sh + 2 * t;
-    float x[J][4];  // channels 16 j + 2 t, + 1, + 8, + 9
+#pragma unroll
+    for (int j = 0; j < J; ++j)
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        if (p.q_vec) part[i][j][k] = *reinterpret_cast<const Pair*>(src + 16 * j + 8 * k);
+        else {
+          T* pair = reinterpret_cast<T*>(&part[i][j][k]);
+          pair[0] = src[16 * j + 8 * k], pair[1] = src[16 * j + 8 * k + 1];
+        }
+      }
+  }
+#pragma unroll
+  for (int i = 0; i < 2 * M; ++i) {
+    const int r = row0 + 8 * i + g, real = min(r, p.rows - 1), token = token_of(p, real), in_group = real - token * p.group;
+    float x[J][4];
     uint32_t most = 0;
 #pragma unroll
     for (int j = 0; j < J; ++j) {
-      alignas(8) T part[4];
-      if (p.q_vec) {
-        using Pair = typename std::conditional<sizeof(T) == 4, uint2, uint32_t>::type;
-        *reinterpret_cast<Pair*>(part) = *reinterpret_cast<const Pair*>(src + 16 * j);
-        *reinterpret_cast<Pair*>(part + 2) = *reinterpret_cast<const Pair*>(src + 16 * j + 8);
-      } else {
-        part[0] = src[16 * j], part[1] = src[16 * j + 1], part[2] = src[16 * j + 8], part[3] = src[16 * j + 9];
-      }
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        x[j][k] = r < p.rows ? to_float(part[k]) : 0.f;
+        x[j][k] = r < p.rows ? to_float(reinterpret_cast<const T*>(&part[i][j][k >> 1])[k & 1]) : 0.f;
         most = max(most, abs_bits(x[j][k]));
       }
     }
@@ -102,7 +110,7 @@ __device__ __forceinline__ void lay_rows(const Cache8Attn& p, int b, int h, int 
   }
 }
 
-template <int D, bool kTwo>
+template <int D>
 constexpr size_t fixed_bytes() {  // codes as numbers, the scales of two steps' tiles
   return 2ull * 2 * kTokens * D * 2 + 2 * 2 * (kTokens / 16) * 4;
 }
@@ -199,14 +207,18 @@ __global__ void __launch_bounds__(kThreads, 1) cache8_rows_kernel(const __grid_c
       lay_rows<T, D, M, kTwo>(p, b, h, row0, start, end, s_queries + mine * kQuery, s_rows + mine * R);
     __syncthreads();
 
-    Row row[M][2];
+    struct {
+      float scale;
+      int lim;
+    } row[M][2];
     int all_see = end - 1;  // slots up to this one are seen by every row of the warp
     if (row0 < p.rows) {
 #pragma unroll
       for (int m = 0; m < M; ++m)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          row[m][e] = s_rows[mine * R + 16 * m + 8 * e + g];
+          const Row& r = s_rows[mine * R + 16 * m + 8 * e + g];
+          row[m][e] = {r.scale, r.lim};
           all_see = min(all_see, row[m][e].lim);
         }
     }
@@ -260,23 +272,32 @@ __global__ void __launch_bounds__(kThreads, 1) cache8_rows_kernel(const __grid_c
           for (int m = 0; m < M; ++m)
 #pragma unroll
             for (int k = 0; k < 8; ++k) s[mt][m][k >> 2][k & 3] = 0.f;
-#pragma unroll
-        for (int j = 0; j < J; ++j) {
-          uint32_t k[MT][4];
+        uint32_t kf[2][MT][4];  // (operands are requested a step ahead of their use)
+        uint4 qf[2][Q2][M];
+        auto operands = [&](int j) {
 #pragma unroll
           for (int mt = 0; mt < MT; ++mt) {
             const int token = (part + mt) * 16 + k_token;
-            load_matrices(k[mt], keys_at + (token * kChunks + ((2 * j + k_half) ^ (token & 7))) * 16);
+            load_matrices(kf[j & 1][mt], keys_at + (token * kChunks + ((2 * j + k_half) ^ (token & 7))) * 16);
           }
 #pragma unroll
           for (int w = 0; w < Q2; ++w)
 #pragma unroll
+            for (int m = 0; m < M; ++m) qf[j & 1][w][m] = query[((w * J + j) * M + m) * 32 + lane];
+        };
+        operands(0);
+#pragma unroll
+        for (int j = 0; j < J; ++j) {
+          if (j + 1 < J) operands(j + 1);
+#pragma unroll
+          for (int w = 0; w < Q2; ++w)
+#pragma unroll
             for (int m = 0; m < M; ++m) {
-              const uint4 q = query[((w * J + j) * M + m) * 32 + lane];
+              const uint4 q = qf[j & 1][w][m];
 #pragma unroll
               for (int mt = 0; mt < MT; ++mt) {
-                mma_f16(s[mt][m][0], q.x, q.y, q.z, q.w, k[mt][0], k[mt][1]);
-                mma_f16(s[mt][m][1], q.x, q.y, q.z, q.w, k[mt][2], k[mt][3]);
+                mma_f16(s[mt][m][0], q.x, q.y, q.z, q.w, kf[j & 1][mt][0], kf[j & 1][mt][1]);
+                mma_f16(s[mt][m][1], q.x, q.y, q.z, q.w, kf[j & 1][mt][2], kf[j & 1][mt][3]);
               }
             }
         }
@@ -306,7 +327,7 @@ __global__ void __launch_bounds__(kThreads, 1) cache8_rows_kernel(const __grid_c
             for (int m = 0; m < M; ++m)
 #pragma unroll
               for (int k = 0; k < 8; ++k) {
-                const Row& r = row[m][k >> 1 & 1];
+                const Row& r = s_rows[mine * R + 16 * m + 8 * (k >> 1 & 1) + g];
                 const int d = r.where - here[k >> 2][k & 1];
                 s[mt][m][k >> 2][k & 3] += s_table[r.bias + s_buckets[min(max(d, 0), p.distances - 1)]];
               }
@@ -384,6 +405,7 @@ __global__ void __launch_bounds__(kThreads, 1) cache8_rows_kernel(const __grid_c
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt) {
           uint32_t pf[Q2][M][4];
+          const bool odd = !(va[mt] < INFINITY);  // a block that is not finite: what is hidden counts for nothing all the same
 #pragma unroll
           for (int m = 0; m < M; ++m) {
             const float r[2] = {va[mt] * v_inv[m][0], va[mt] * v_inv[m][1]};
@@ -398,8 +420,7 @@ __global__ void __launch_bounds__(kThreads, 1) cache8_rows_kernel(const __grid_c
                   pr[k] = exp2_approx(x - ref[m][e]);
                   l[m][e] += pr[k];
                   pr[k] *= r[e];
-                  // a block that is not finite: what is hidden counts for nothing all the same
-                  if (!(va[mt] < INFINITY) && x == -INFINITY) pr[k] = 0.f;
+                  if (odd && x == -INFINITY) pr[k] = 0.f;
                 }
                 const __half2 v = __floats2half2_rn(pr[0], pr[1]);
                 pf[0][m][2 * n + e] = as_u32(v);
@@ -407,10 +428,13 @@ __global__ void __launch_bounds__(kThreads, 1) cache8_rows_kernel(const __grid_c
               }
           }
           const int token = min(part + mt, kTiles - 1) * 16 + v_token;
+          uint32_t vf[2][4];
+          auto values = [&](int i) { load_transposed(vf[i & 1], values_at + (token * kChunks + ((2 * i + v_half) ^ (token & 7))) * 16); };
+          values(0);
 #pragma unroll
           for (int i = 0; i < J; ++i) {
-            uint32_t v[4];
-            load_transposed(v, values_at + (token * kChunks + ((2 * i + v_half) ^ (token & 7))) * 16);
+            if (i + 1 < J) values(i + 1);
+            const uint32_t(&v)[4] = vf[i & 1];
 #pragma unroll
             for (int w = 0; w < Q2; ++w)
 #pragma unroll
@@ -514,12 +538,11 @@ __global__ void __launch_bounds__(kThreads, 1) cache8_rows_kernel(const __grid_c
   }
 }
 
-template <typename T, int D>
+template <typename T, int D, int M, int MT>
 cudaError_t launch(const Cache8Attn& p, bool behind, cudaStream_t stream) {
   constexpr bool kTwo = sizeof(T) == 4;
-  constexpr int M = kTwo ? 1 : 2, MT = 1;
   const size_t table = p.table == nullptr ? 0 : static_cast<size_t>(p.c.heads) * p.group * p.table_stride * 4;
-  const size_t fixed = fixed_bytes<D, kTwo>(), query = query_bytes<D, M, kTwo>();
+  const size_t fixed = fixed_bytes<D>(), query = query_bytes<D, M, kTwo>();
   static bool set[64] = {false};
   int dev = 0;
   cudaGetDevice(&dev);
@@ -534,16 +557,22 @@ cudaError_t launch(const Cache8Attn& p, bool behind, cudaStream_t stream) {
   return launch_behind(behind, cache8_rows_kernel<T, D, M, kTwo, MT>, grid, kThreads, fixed + p.row_warps * query + table, stream, p);
 }
 
+// Few rows: 16 a warp, and a tile of tokens at a time (warps that share rows have but one of a step).
+template <typename T, int D>
+cudaError_t launch_for(const Cache8Attn& p, bool behind, cudaStream_t stream) {
+  return p.rows <= kFewRows ? launch<T, D, 1, 1>(p, behind, stream) : launch<T, D, sizeof(T) == 4 ? 1 : 2, 2>(p, behind, stream);
+}
+
 }  // namespace
 
 cudaError_t launch_cache8_rows(const Cache8Attn& p, int type, bool behind, cudaStream_t stream) {
   if (p.c.dim == 64)
-    return type == 0   ? launch<__nv_bfloat16, 64>(p, behind, stream)
-           : type == 1 ? launch<__half, 64>(p, behind, stream)
-                       : launch<float, 64>(p, behind, stream);
-  return type == 0   ? launch<__nv_bfloat16, 128>(p, behind, stream)
-         : type == 1 ? launch<__half, 128>(p, behind, stream)
-                     : launch<float, 128>(p, behind, stream);
+    return type == 0   ? launch_for<__nv_bfloat16, 64>(p, behind, stream)
+           : type == 1 ? launch_for<__half, 64>(p, behind, stream)
+                       : launch_for<float, 64>(p, behind, stream);
+  return type == 0   ? launch_for<__nv_bfloat16, 128>(p, behind, stream)
+         : type == 1 ? launch_for<__half, 128>(p, behind, stream)
+                     : launch_for<float, 128>(p, behind, stream);
 }
 
 }  // namespace t5x
