@@ -813,6 +813,13 @@ Cache8 rows_of(Cache8 c, int from, int count) {
   return c;
 }
 
+// Rows of a launch: no more scores than a gigabyte where weights are added up (a launch of that many fills the SMs for long).
+int rows_at_a_time(const Cache8& c, int rows) {
+  long long most = kMaxBatch;
+  if (c.weight != nullptr) most = std::min(most, (1LL << 28) / (static_cast<long long>(c.heads) * rows * c.slots));
+  return static_cast<int>(std::min<long long>(c.batch, std::max(most, 1LL)));
+}
+
 struct Plan {
   int pieces = 0, least = 0, entry = 0, row_warps = 1;
   size_t part = 0, stats = 0, first = 0, scores = 0, final_stats = 0, total = 0;
@@ -820,7 +827,7 @@ struct Plan {
 Plan plan(Cache8 c, int rows, int type) {
   Plan w = {};
   if (by_row_head(c, rows)) return w;
-  c.batch = std::min(c.batch, kMaxBatch);
+  c.batch = rows_at_a_time(c, rows);
   const int tile_rows = rows <= 8 ? 8 : row_tile_of(type, rows), row_tiles = (rows + tile_rows - 1) / tile_rows;
   // Pieces for all CTAs that the SMs hold at a time, none of under 64 tokens a warp. Beginning a (row, head) costs as much as
   // 24 tiles where a CTA does some four of them a us (us for long contexts of all lengths / for 4 x 16 heads of 64 channels by
@@ -935,9 +942,10 @@ T5X_API int t5x_cache8_attention(const T5xCache8* cache, const T5xCache8Query* q
   if (n)
     if (int e = t5x::cache8_append(c, n, st)) return e;
   const int size = q->type == 2 ? 4 : 2;
-  for (int from = 0; from < c.batch; from += t5x::kMaxBatch) {
+  const int each = t5x::rows_at_a_time(c, p.rows);
+  for (int from = 0; from < c.batch; from += each) {
     t5x::Cache8Attn part = p;
-    part.c = t5x::rows_of(c, from, std::min(c.batch - from, t5x::kMaxBatch));
+    part.c = t5x::rows_of(c, from, std::min(c.batch - from, each));
     part.q = static_cast<const char*>(p.q) + from * p.q_sb * size;
     part.out = static_cast<char*>(p.out) + static_cast<long long>(from) * p.rows * c.heads * c.dim * size;
     part.mask = p.mask ? p.mask + from * p.mask_stride : nullptr;

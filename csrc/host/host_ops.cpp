@@ -1193,6 +1193,15 @@ struct Cache8Of {
     c.block_log2 = block == 16 ? 4 : block == 32 ? 5 : block == 64 ? 6 : 7;
     ok = true;
   }
+  bool overlaps(const Cache8Of& other) const {
+    for (const Tensor& x : held)
+      for (const Tensor& y : other.held) {
+        if (!x.defined() || !y.defined()) continue;
+        const char *at = static_cast<const char*>(x.data_ptr()), *to = static_cast<const char*>(y.data_ptr());
+        if (at < to + y.nbytes() && to < at + x.nbytes()) return true;
+      }
+    return false;
+  }
   bool has(const Tensor& t) const { return t.is_cuda() && t.get_device() == device; }
 };
 
@@ -1277,10 +1286,7 @@ py::object cache8_evict(py::handle cache, py::handle into, int64_t keep, int64_t
   const Cache8Of c(cache.ptr()), to(into.ptr());
   if (!c.ok || !to.ok || c.device != to.device || c.b != to.b || c.h != to.h || c.dim != to.dim || c.c.weight == nullptr ||
       to.c.weight == nullptr || to.c.position == nullptr || keep < 1 || keep > to.slots || recent < 0 || recent > keep ||
-      c.c.codes[0] == to.c.codes[0] || c.c.codes[1] == to.c.codes[1] || c.c.absmax[0] == to.c.absmax[0] ||
-      c.c.absmax[1] == to.c.absmax[1] || c.c.weight == to.c.weight || c.c.index == to.c.index ||
-      (c.c.position != nullptr && (c.c.position == to.c.position || c.c.dropped == to.c.dropped)) ||
-      (to.b > 1 && to.c.index_stride == 0))
+      (to.b > 1 && to.c.index_stride == 0) || c.overlaps(to))
     return py::none();
   py::gil_scoped_release no_gil;
   Tensor kept = at::empty({c.b, c.h, keep}, at::TensorOptions().dtype(at::kInt).device(at::Device(at::kCUDA, c.device)));

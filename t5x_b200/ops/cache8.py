@@ -93,11 +93,18 @@ def _check_tokens(cache, key, value, what: str) -> None:
   _no_graph(what, key, value)
 
 
+def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
+  """Whether two contiguous tensors share memory."""
+  at, to = a.data_ptr(), b.data_ptr()
+  return at < to + b.numel() * b.element_size() and to < at + a.numel() * a.element_size()
+
+
 def _native_ok(cache, dtype) -> bool:
   """Whether the kernels take the call. (A function transform or a trace sees into the statements, not into kernels.)"""
   codes = cache["cached_key"]
   return codes.is_cuda and codes.shape[3] in (64, 128) and dtype in native.CACHE8_TYPES and codes.numel() > 0 and \
-      codes.shape[0] < 65536 and codes.shape[1] < 65536 and not F._transformed()
+      codes.shape[0] < 65536 and codes.shape[1] < 65536 and codes.shape[0] * codes.shape[1] <= 1 << 24 and \
+      not F._transformed()
 
 
 def append_(cache: dict, key: torch.Tensor, value: torch.Tensor, lengths: Optional[torch.Tensor] = None) -> None:
@@ -159,6 +166,8 @@ def attention(query: torch.Tensor, cache: dict, key: Optional[torch.Tensor] = No
     raise ValueError(f"attention: a mask is [{b}, at most {slots}]; got {tuple(key_mask.shape)}")
   if query.shape[1] * (query.shape[2] // h) > 65535:
     raise ValueError("attention: over 65535 query rows a head")
+  if "token_weight" in cache and query.shape[1] * (query.shape[2] // h) * slots >= 1 << 31:
+    raise ValueError(f"attention: {query.shape[1]} queries over {slots} slots whose weight is added up; give fewer at a time")
   if not (_native_ok(cache, query.dtype) and (bias_table is None or (
       max_distance < native.CACHE8_DISTANCES and query.shape[2] * num_buckets <= native.CACHE8_BIASES))):
     if key is not None:
@@ -196,7 +205,7 @@ def evict(cache: dict, keep: int, *, recent: int = 0, out: Optional[dict] = None
     if "token_weight" not in out or "token_position" not in out or out["cache_index"].shape != (b,) or \
         (to.shape[0], to.shape[1], to.shape[3], to.device) != (b, h, dim, cache["cached_key"].device):
       raise ValueError(f"evict: `out` is another cache of {b} rows, {h} heads of {dim}, with weights and positions")
-    if any(out[n].data_ptr() == cache[n].data_ptr() for n in out if n in cache):
+    if any(_overlap(out[n], cache[m]) for n in out if n in _TENSORS for m in cache if m in _TENSORS):
       raise ValueError("evict: `out` shares memory with the cache")
   if keep > out["cached_key"].shape[2]:
     raise ValueError(f"evict: {keep} tokens into {out['cached_key'].shape[2]} slots")

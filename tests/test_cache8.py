@@ -396,6 +396,7 @@ def test_refusals():
   cache = make(2, 2, 64, 64, 16, [3, 4], weights=True)
   q = torch.randn(2, 1, 4, 64)
   k = torch.randn(2, 1, 2, 64)
+  three = make(3, 2, 64, 64, 16, [3, 4, 5], weights=True, positions=True)
   bad = [
       lambda: cache8.init_cache(1, 8, 1, 64, block=24),
       lambda: cache8.init_cache(1, 0, 1, 64),
@@ -426,6 +427,7 @@ def test_refusals():
       lambda: cache8.evict(cache, 65),
       lambda: cache8.evict(cache, 8, out=cache),
       lambda: cache8.evict(cache, 8, out=make(2, 2, 64, 64, 16, [0, 0], weights=True)),
+      lambda: cache8.evict({n: t[:2] for n, t in three.items()}, 8, out={n: t[1:] for n, t in three.items()}),
       lambda: cache8.evict(make(2, 2, 64, 64, 16, [3, 4]), 8),
       lambda: cache8.evict(cache, 33, out=make(2, 2, 32, 64, 16, [0, 0], weights=True, positions=True)),
       lambda: F.quantize_weight(torch.ones(4, 4, dtype=torch.long)),

@@ -1,6 +1,7 @@
 """Kernels of decoding in 8 bits: against loops in 64 bits (test_cache8.py) at the borders of blocks, tiles, rows and masks;
 strides, streams, captures; long caches against the statements in tensor operations."""
 import math
+import threading
 
 import pytest
 import torch
@@ -319,3 +320,119 @@ def test_offsets_behind_32_bits():
   small, kept = cache8.evict(cache, 4, recent=0, out=cache8.init_cache(b, 16, 8, 128, "cuda", block=16, weights=True,
                                                                        positions=True))
   assert (kept[4] >= slots - 9).all() and (small["dropped"][4] == slots - 4)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("c", [
+    dict(b=2, h=1, group=3, dim=64, slots=160, block=32, starts=[120, 0], count=3, mask=True, weights=True),
+    dict(b=2, h=2, group=16, dim=128, slots=96, block=16, starts=[61, 15], count=1, bias=True, positions=True),
+    dict(b=1, h=2, group=11, dim=64, slots=400, block=16, starts=[366], count=3, bias=True, weights=True),
+    dict(b=3, h=1, group=1, dim=128, slots=208, block=16, starts=[200, 0, 77], count=65, weights=True),
+    dict(b=2, h=1, group=2, dim=64, slots=192, block=64, starts=[128, 192], count=32, cross=True, mask=True),
+    dict(b=1, h=1, group=5, dim=128, slots=144, block=16, starts=[17], count=26, mask=True, bias=True),
+    dict(b=2, h=1, group=1, dim=64, slots=272, block=16, starts=[0, 1], count=260, bias=True, weights=True, positions=True),
+    dict(b=2, h=1, group=2, dim=128, slots=80, block=16, starts=[64, 3], count=129, own=True),
+], ids=range(8))
+def test_many_rows(c, dtype):
+  """9 to 520 query rows a key head: below and above what a warp, half of a CTA's warps and all of them take."""
+  launches(lambda: plain.check_attention(c, "cuda", dtype))
+
+
+def check_some_rows(c, rows, dtype=torch.bfloat16):
+  """As check_attention, for some rows of a batch."""
+  cache, query, key, value, kw = plain.inputs(c, "cuda", dtype)
+  before = cache["token_weight"].clone() if c.get("weights") else None
+  out = launches(lambda: cache8.attention(query, cache, key, value, **kw))
+  for i in rows:
+    held = {n: t[i:i + 1] for n, t in cache.items()}
+    mask = None if kw["key_mask"] is None else kw["key_mask"][i:i + 1].cpu()
+    want, size, high, weight = plain.attention_oracle(query[i:i + 1], held, [c["starts"][i]], 0 if key is None else c["count"],
+                                                      kw["bias_table"], mask=mask, causal=kw["causal"], scale=kw["scale"])
+    assert plain.within(out[i:i + 1], want, size, high, c["dim"], c["slots"]), i
+    if before is not None:
+      new = slice(c["starts"][i], c["starts"][i] + (0 if key is None else c["count"]))
+      before[i, :, new] = 0
+      each = 2 * ((c["dim"] + 16) * 2.0 ** -24 + 2.0 ** -21) * high + (c["slots"] + 64) * 2.0 ** -24 + 2.0 ** -20
+      off = (cache["token_weight"][i].cpu().double() - before[i].cpu().double() - weight[0]).abs()
+      assert (off <= each * weight[0] + 2.0 ** -24 * cache["token_weight"][i].cpu().double().abs() + 2.0 ** -120).all(), i
+
+
+def test_more_rows_than_a_launch_takes():
+  starts = [(7 * i) % 1024 for i in range(2050)]
+  for count in (1, 9):
+    check_some_rows(dict(b=2050, h=1, group=1, dim=64, slots=1040, block=16, starts=starts, count=count), [0, 2047, 2048, 2049])
+
+
+def test_more_scores_than_a_launch_takes():
+  """The weights of 34 rows come from 1.06 GiB of scores."""
+  starts = [(397 * i) % 2048 + 100 for i in range(34)]
+  check_some_rows(dict(b=34, h=8, group=8, dim=64, slots=16384, block=128, starts=starts, count=8, weights=True), [0, 31, 32, 33])
+
+
+def test_tables_beyond_the_kernels():
+  """Biases of more heads than shared memory holds, and of longer distances: the statements."""
+  for heads, group, far in ((2, 150, 128), (2, 2, 2000)):
+    cache = plain.make(1, heads, 48, 64, 16, [40], device="cuda")
+    query = torch.randn(1, 1, heads * group, 64, device="cuda") / 8
+    table = torch.randn(heads * group, 32, device="cuda")
+    out = cache8.attention(query, cache, bias_table=table, max_distance=far)
+    want, size, high, _ = plain.attention_oracle(query, cache, [40], 0, table, far=far)
+    # (the statements round each score's and each sum's products in another order: as many roundings at most)
+    assert plain.within(out, want, size, high, 64, 48)
+
+
+def test_evict_and_products_captured_beside_each_other():
+  """Each captured once and replayed on its own stream, while the same calls run on the current one."""
+  cache = plain.make(2, 2, 512, 64, 32, [500, 77], weights=True, positions=True, device="cuda")
+  room = lambda: cache8.init_cache(2, 256, 2, 64, "cuda", block=32, weights=True, positions=True)  # noqa: E731
+  weight = F.quantize_weight(torch.randn(320, 640).cuda())
+  xs = [torch.randn(n, 320).cuda().bfloat16() for n in (1, 40, 700)]
+  small, kept = cache8.evict(cache, 200, recent=20, out=room())
+  want = [F.linear8(x, weight) for x in xs]
+  torch.cuda.synchronize()
+  streams, graphs, got = [torch.cuda.Stream() for _ in range(2)], [], []
+  for _ in range(2):
+    into, g = room(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+      got.append((*cache8.evict(cache, 200, recent=20, out=into), [F.linear8(x, weight) for x in xs]))
+    graphs.append(g)
+  for _ in range(3):
+    for s, g in zip(streams, graphs):
+      with torch.cuda.stream(s):
+        g.replay()
+    again, again_kept = cache8.evict(cache, 200, recent=20, out=room())
+    here = [F.linear8(x, weight) for x in xs]
+  torch.cuda.synchronize()
+  for into, slots, ys in got + [(again, again_kept, here)]:
+    assert torch.equal(slots, kept) and all(torch.equal(into[n], small[n]) for n in small)
+    assert all(torch.equal(y, w) for y, w in zip(ys, want))
+
+
+def test_threads():
+  """Calls of several threads at once, each with a stream and a cache of its own."""
+  c = dict(b=3, h=2, group=2, dim=64, slots=1600, block=32, starts=[1500, 3, 700], count=1, weights=True, bias=True)
+  cache, query, key, value, kw = plain.inputs(c, "cuda", torch.bfloat16)
+  chunk = torch.randn(3, 30, 4, 64, device="cuda", dtype=torch.bfloat16) / 8
+  weight, x = F.quantize_weight(torch.randn(64, 80).cuda()), torch.randn(9, 64).cuda()
+
+  def run():
+    mine = {n: t.clone() for n, t in cache.items()}
+    outs = [cache8.attention(query, mine, key, value, **kw), cache8.attention(chunk, mine, causal=False), F.linear8(x, weight)]
+    return outs + [mine["token_weight"], cache8.evict(mine, 90, recent=3)[1]]
+
+  want = run()
+  torch.cuda.synchronize()
+  got = {}
+
+  def work(i):
+    with torch.cuda.stream(torch.cuda.Stream()):
+      for _ in range(20):
+        got[i] = run()
+      torch.cuda.current_stream().synchronize()
+
+  threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+  for t in threads:
+    t.start()
+  for t in threads:
+    t.join()
+  assert len(got) == 4 and all(torch.equal(a, b) for one in got.values() for a, b in zip(one, want))
