@@ -65,11 +65,6 @@ __device__ __forceinline__ int border_digit(const int* counts, int& need) {
   return __shfl_sync(0xffffffffu, digit, who & 31);
 }
 
-__device__ __forceinline__ unsigned long long remote_u64(const unsigned long long* mine, uint32_t cta) {
-  unsigned long long v;
-  asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v) : "r"(mapa_shared(smem_u32(mine), cta)) : "memory");
-  return v;
-}
 __device__ __forceinline__ int remote_int(const int* mine, uint32_t cta) {
   int v;
   asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(mapa_shared(smem_u32(mine), cta)) : "memory");
@@ -80,23 +75,25 @@ __device__ __forceinline__ void remote_add(int* mine, int v) {  // to the cluste
   asm volatile("red.relaxed.cluster.shared::cluster.add.s32 [%0], %1;" ::"r"(mapa_shared(smem_u32(mine), 0)), "r"(v) : "memory");
 }
 
-// A CTA, or a cluster, takes the slots of one head of one row and keeps its weights in registers, K a thread. The border is
-// found eight bits at a time from counts of the digits, behind the first of those alone that are at the border so far;
-// zeros, which may be most, are counted by ballot. A slot's place is the
-// number of larger ones before it, and of those at the border as far as they stay.
-constexpr uint32_t kZero = 0x80000000u;  // order_of(0)
+// A CTA, or a cluster, takes the slots of one head of one row and keeps its weights in registers, K adjacent ones a thread
+// (through shared memory, so that global reads are of whole lines). The border is found eight bits at a time from counts of
+// the digits, behind the first of those alone that are at the border so far; zeros, which may be most, are counted apart.
+// A slot's place is the number of larger ones before it, and of those at the border as far as they stay.
+constexpr uint32_t kZero = 0x80000000u;  // order_of(0); of no weight 0
 
 template <int T, int K, int kCtas>
 __global__ void __launch_bounds__(T, 1024 / T)
     cache8_select_kernel(const __grid_constant__ Cache8 c, int keep, int recent, int* __restrict__ kept,
                          int* __restrict__ index_out, int* __restrict__ dropped_out) {
-  __shared__ __align__(16) int s_hist[4][256];
-  __shared__ uint32_t s_list[T * K];
-  __shared__ int s_left;
-  __shared__ __align__(16) int s_all[4][256];  // a cluster's sums, in its first CTA; here the copy that is looked at
-  __shared__ unsigned long long s_before[K * T / 32 + 1];  // larger | at the border << 32, by row of T slots and warp
   constexpr int kWarps = T / 32;
   constexpr bool kCluster = kCtas > 1;
+  static_assert(T * K < 65536, "two counts in 32 bits");
+  __shared__ __align__(16) int s_hist[4][256];
+  __shared__ __align__(16) uint32_t s_list[T * K];
+  __shared__ int s_left;
+  __shared__ __align__(16) int s_all[4][256];  // a cluster's sums, in its first CTA; here the copy that is looked at
+  __shared__ uint32_t s_sums[kWarps];
+  __shared__ int s_total;  // larger | at the border << 16
   const long long bh = blockIdx.x / kCtas;
   const uint32_t rank = kCluster ? cluster_ctarank() : 0;
   const int b = static_cast<int>(bh / c.heads);
@@ -114,36 +111,57 @@ __global__ void __launch_bounds__(T, 1024 / T)
     return;
   }
   const int old = held - recent, first = static_cast<int>(rank) * (T * K);  // slots to choose from; this CTA's first
-  uint32_t key[K];
+  const int own = first + static_cast<int>(threadIdx.x) * K;                // this thread's first
+  // 16 bytes a place, places of a thread's by its number: the banks
+  auto place_of = [](int chunk) { return chunk ^ (chunk >> 3 & 7); };
+  const bool whole = (reinterpret_cast<uintptr_t>(w) & 15) == 0;
 #pragma unroll
-  for (int i = 0; i < K; ++i) {
-    const int s = first + i * T + threadIdx.x;
-    key[i] = s < old ? order_of(w[s]) : 0;
+  for (int i = 0; i < K / 4; ++i) {
+    const int chunk = i * T + threadIdx.x, s = first + 4 * chunk;  // (a cache has whole 16 slots)
+    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (s < old) {
+      if (whole) x = *reinterpret_cast<const float4*>(w + s);
+      else x = make_float4(w[s], w[s + 1], w[s + 2], w[s + 3]);
+    }
+    reinterpret_cast<float4*>(s_list)[place_of(chunk)] = x;
   }
   for (int i = threadIdx.x; i < 1024; i += T) s_hist[i >> 8][i & 255] = s_all[i >> 8][i & 255] = 0;
   if (threadIdx.x == 0) s_left = 0;
+  __syncthreads();
+  uint32_t key[K];
+#pragma unroll
+  for (int i = 0; i < K / 4; ++i) {
+    const float4 x = reinterpret_cast<const float4*>(s_list)[place_of(threadIdx.x * (K / 4) + i)];
+    key[4 * i] = own + 4 * i < old ? order_of(x.x) : 0;
+    key[4 * i + 1] = own + 4 * i + 1 < old ? order_of(x.y) : 0;
+    key[4 * i + 2] = own + 4 * i + 2 < old ? order_of(x.z) : 0;
+    key[4 * i + 3] = own + 4 * i + 3 < old ? order_of(x.w) : 0;
+  }
   if (kCluster) cluster_sync_all();
   else __syncthreads();
 
   int need = keep - recent;
+  const bool any = need > 0;
   uint32_t border = 0;
-  if (need > 0)
+  if (any)
     for (int round = 0; round < 4; ++round) {
       const int shift = 24 - 8 * round;
       int zeros = 0;
-      auto count = [&](bool in, uint32_t u) {
-        zeros += __popc(__ballot_sync(0xffffffffu, in && u == kZero));
-        if (in && u != kZero) atomicAdd(&s_hist[round][(u >> shift) & 255], 1);
-      };
       if (round == 0) {
 #pragma unroll
-        for (int i = 0; i < K; ++i) count(first + i * T + static_cast<int>(threadIdx.x) < old, key[i]);
+        for (int i = 0; i < K; ++i) {
+          if (key[i] == kZero) ++zeros;
+          else if (key[i] != 0) atomicAdd(&s_hist[0][key[i] >> 24], 1);
+        }
       } else {
-        for (int j = threadIdx.x; j - lane < s_left; j += T) {
-          const uint32_t u = j < s_left ? s_list[j] : 0;
-          count(j < s_left && ((u ^ border) >> (shift + 8)) == 0, u);
+        for (int j = threadIdx.x; j < s_left; j += T) {
+          const uint32_t u = s_list[j];
+          if ((u ^ border) >> (shift + 8) != 0) continue;
+          if (u == kZero) ++zeros;
+          else atomicAdd(&s_hist[round][(u >> shift) & 255], 1);
         }
       }
+      zeros = __reduce_add_sync(0xffffffffu, zeros);
       if (lane == 0 && zeros > 0) atomicAdd(&s_hist[round][(kZero >> shift) & 255], zeros);
       __syncthreads();
       if (kCluster) {  // the few digits that occur, to the first CTA
@@ -154,77 +172,66 @@ __global__ void __launch_bounds__(T, 1024 / T)
         __syncthreads();
       }
       border |= static_cast<uint32_t>(border_digit(s_hist[round], need)) << shift;
-      if (round == 0) {  // those at the border so far
+      if (round == 0) {  // those at the border so far, in any order
+        int mine = 0;
 #pragma unroll
-        for (int i = 0; i < K; ++i) {
-          const bool in = first + i * T + static_cast<int>(threadIdx.x) < old && (key[i] ^ border) >> 24 == 0;
-          const uint32_t who = __ballot_sync(0xffffffffu, in);
-          int at = 0;
-          if (who != 0 && lane == 0) at = atomicAdd(&s_left, __popc(who));
-          at = __shfl_sync(0xffffffffu, at, 0) + __popc(who & ((1u << lane) - 1));
-          if (in) s_list[at] = key[i];
+        for (int i = 0; i < K; ++i) mine += key[i] != 0 && (key[i] ^ border) >> 24 == 0;
+        int run = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const int u = __shfl_up_sync(0xffffffffu, run, o);
+          if (lane >= o) run += u;
         }
+        int at = 0;
+        if (lane == 31 && run != 0) at = atomicAdd(&s_left, run);
+        at = __shfl_sync(0xffffffffu, at, 31) + run - mine;
+#pragma unroll
+        for (int i = 0; i < K; ++i)
+          if (key[i] != 0 && (key[i] ^ border) >> 24 == 0) s_list[at++] = key[i];
         __syncthreads();
       }
     }
   const int ties = need;  // of the slots at the border, the first so many stay
-  const bool any = keep > recent;
 
+  uint32_t mine = 0;  // larger | at the border << 16
+  if (any) {
 #pragma unroll
-  for (int i = 0; i < K; ++i) {
-    const bool in = any && first + i * T + static_cast<int>(threadIdx.x) < old;
-    const uint32_t above = __ballot_sync(0xffffffffu, in && key[i] > border), tie = __ballot_sync(0xffffffffu, in && key[i] == border);
-    if (lane == 0) s_before[i * kWarps + warp] = __popc(above) | static_cast<unsigned long long>(__popc(tie)) << 32;
+    for (int i = 0; i < K; ++i) mine += key[i] > border ? 1u : key[i] == border && key[i] != 0 ? 0x10000u : 0u;
   }
+  uint32_t run = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const uint32_t u = __shfl_up_sync(0xffffffffu, run, o);
+    if (lane >= o) run += u;
+  }
+  if (lane == 31) s_sums[warp] = run;
   __syncthreads();
-  if (warp == 0) {  // sums of what is before each
-    constexpr int kEach = (K * kWarps + 31) / 32;
-    unsigned long long v[kEach], sum = 0;
+  uint32_t before = run - mine, all = 0;
 #pragma unroll
-    for (int i = 0; i < kEach; ++i) {
-      const int at = lane * kEach + i;
-      v[i] = at < K * kWarps ? s_before[at] : 0;
-      sum += v[i];
-    }
-    unsigned long long run = sum;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const unsigned long long u = __shfl_up_sync(0xffffffffu, run, o);
-      if (lane >= o) run += u;
-    }
-    if (lane == 31) s_before[K * kWarps] = run;
-    run -= sum;
-#pragma unroll
-    for (int i = 0; i < kEach; ++i) {
-      const int at = lane * kEach + i;
-      if (at < K * kWarps) s_before[at] = run;
-      run += v[i];
-    }
+  for (int i = 0; i < kWarps; ++i) {
+    if (i < warp) before += s_sums[i];
+    all += s_sums[i];
   }
-  unsigned long long base = 0;
+  int above = before & 0xffff, tie = before >> 16;
   if (kCluster) {
+    if (threadIdx.x == 0) s_total = static_cast<int>(all);
     cluster_sync_all();
 #pragma unroll
     for (int r = 0; r < kCtas; ++r) {
-      const unsigned long long u = remote_u64(&s_before[K * kWarps], r);
-      if (r < static_cast<int>(rank)) base += u;
+      const uint32_t u = static_cast<uint32_t>(remote_int(&s_total, r));
+      if (r < static_cast<int>(rank)) above += u & 0xffff, tie += u >> 16;
     }
-  } else {
-    __syncthreads();
   }
+  if (any) {
+    int* to = out + above + min(tie, ties);
 #pragma unroll
-  for (int i = 0; i < K; ++i) {
-    const int s = first + i * T + threadIdx.x;
-    const bool in = any && s < old;
-    const bool is_above = in && key[i] > border, is_tie = in && key[i] == border;
-    const uint32_t under = (1u << lane) - 1;
-    const uint32_t above = __ballot_sync(0xffffffffu, is_above) & under, tie = __ballot_sync(0xffffffffu, is_tie) & under;
-    const unsigned long long before = base + s_before[i * kWarps + warp];
-    const int tie_rank = static_cast<int>(before >> 32) + __popc(tie);
-    const int place = static_cast<int>(before & 0xffffffffu) + __popc(above) + min(tie_rank, ties);
-    if (is_above || (is_tie && tie_rank < ties)) out[place] = s;
-    else if (s >= old && s < held) out[keep - recent + s - old] = s;
+    for (int i = 0; i < K; ++i) {
+      const bool at_border = key[i] == border && key[i] != 0;
+      if (key[i] > border || (at_border && tie < ties)) *to++ = own + i;
+      tie += at_border;
+    }
   }
+  for (int i = rank * T + threadIdx.x; i < recent; i += T * kCtas) out[keep - recent + i] = old + i;
   if (kCluster) cluster_sync_all();  // nobody leaves while others read its sums
 }
 
