@@ -18,7 +18,7 @@
 //   * A key byte u = code + 128 alone is the fp16 number u 2^-24 (below the normal ones, which the tensor cores take as
 //     they are); 128 times the sum of the query is subtracted from the score. Value bytes stand under the exponent of
 //     1024, and 1152 is subtracted from each: their sums run over the whole cache, and an offset of all would leave
-//     nothing of a mean near zero.
+//     nothing of a mean near zero. (Keys too where queries have 32 bits.)
 //
 // Queries are scaled by a power of two to just below 2^14, where fp16 holds the values of 16-bit types down to 2^-28 of
 // the row's largest without loss; values of 32 bits go in as two fp16 numbers each (22 bits). The reference m is raised
@@ -104,8 +104,8 @@ __device__ __forceinline__ void lay_query(const Cache8Attn& p, int b, int h, int
     if (t == 0) {
       Column col;
       // 2^24 back from the keys' exponent; the scale of a key block is its largest value / 127; scores are times log2 e
-      col.scale = __uint_as_float(static_cast<uint32_t>(127 - up) << 23) * p.scale * (0x1p24f / 127.f * kLog2e);
-      col.sum = sum * 0x1p-17f;  // 128 times, at the keys' exponent
+      col.scale = __uint_as_float(static_cast<uint32_t>(127 - up) << 23) * p.scale * ((kTwo ? 1.f : 0x1p24f) / 127.f * kLog2e);
+      col.sum = kTwo ? 0.f : sum * 0x1p-17f;  // 128 times, at the keys' exponent
       col.lim = r < p.rows ? last_seen(p, start, end, r) : 0x7fffffff;  // (a column without a row hinders nobody)
       col.where = q_first + i + dropped;
       col.bias = first_bias + in_group * p.table_stride;
@@ -383,19 +383,22 @@ __global__ void __launch_bounds__(kWarps * 32, 16 / kWarps)
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
               const uint32_t w = j == 0 ? kr[mt][e][ch].x : j == 1 ? kr[mt][e][ch].y : j == 2 ? kr[mt][e][ch].z : kr[mt][e][ch].w;
-              a[mt][e] = key_pair(w, low);
-              a[mt][2 + e] = key_pair(w >> 8, low);
+              a[mt][e] = kTwo ? value_pair(w, low) : key_pair(w, low);
+              a[mt][2 + e] = kTwo ? value_pair(w >> 8, low) : key_pair(w >> 8, low);
             }
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
+          for (int nt = 0; nt < NT; ++nt) {
+            uint32_t q0[Q2], q1[Q2];
 #pragma unroll
             for (int w = 0; w < Q2; ++w) {
               uint2 q;
               if constexpr (kQueryRegs) q = qf[w][ch * 4 + j];
               else q = s_query[(w * CH * 4 + ch * 4 + j) * 32 + lane];
-#pragma unroll
-              for (int mt = 0; mt < MT; ++mt) mma_f16(st[mt][nt], a[mt][0], a[mt][1], a[mt][2], a[mt][3], q.x, q.y);
+              q0[w] = q.x, q1[w] = q.y;
             }
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt) mma_sum<Q2>(st[mt][nt], a[mt], q0, q1);
+          }
         }
       float s[MS][NT][4], k_scale[MS];
       int here[MS][2];  // positions of tokens g and g + 8
@@ -546,12 +549,14 @@ __global__ void __launch_bounds__(kWarps * 32, 16 / kWarps)
           for (int half = 0; half < 2; ++half) {
             const uint32_t x = __byte_perm(vr[mt][0][w], vr[mt][1][w], half ? 0x7632 : 0x5410);
             const uint32_t y = __byte_perm(vr[mt][2][w], vr[mt][3][w], half ? 0x7632 : 0x5410);
-            const uint32_t a0 = value_pair(x, low), a1 = value_pair(x >> 8, low), a2 = value_pair(y, low), a3 = value_pair(y >> 8, low);
+            const uint32_t a[4] = {value_pair(x, low), value_pair(x >> 8, low), value_pair(y, low), value_pair(y >> 8, low)};
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
+            for (int nt = 0; nt < NT; ++nt) {
+              uint32_t p0[Q2], p1[Q2];
 #pragma unroll
-              for (int q2 = 0; q2 < Q2; ++q2)
-                mma_f16(o[nt][2 * w + half], a0, a1, a2, a3, pf[q2][mt][nt][0], pf[q2][mt][nt][1]);
+              for (int q2 = 0; q2 < Q2; ++q2) p0[q2] = pf[q2][mt][nt][0], p1[q2] = pf[q2][mt][nt][1];
+              mma_sum<Q2>(o[nt][2 * w + half], a, p0, p1);
+            }
           }
       if (tile + kStep < tile1) load_v(tile + kStep);
     }

@@ -49,6 +49,33 @@ __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1,
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
+// c += a b, b one fp16 number or the sum of two. Tensor cores cut what they add to an accumulator off, toward zero: over a long
+// sum of 32-bit operands (two numbers) that would count more than they do, so theirs are added by an instruction that rounds.
+template <int Q2>
+__device__ __forceinline__ void mma_sum(float (&c)[4], const uint32_t (&a)[4], const uint32_t (&b0)[Q2], const uint32_t (&b1)[Q2]) {
+  if (Q2 == 1) {
+    mma_f16(c, a[0], a[1], a[2], a[3], b0[0], b1[0]);
+  } else {
+    float x[4] = {0.f, 0.f, 0.f, 0.f};
+    mma_f16(x, a[0], a[1], a[2], a[3], b0[Q2 - 1], b1[Q2 - 1]);
+    mma_f16(x, a[0], a[1], a[2], a[3], b0[0], b1[0]);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) c[k] += x[k];
+  }
+}
+// The same with a the sum.
+template <int Q2>
+__device__ __forceinline__ void mma_sum(float (&c)[4], const uint4 (&a)[Q2], uint32_t b0, uint32_t b1) {
+  if (Q2 == 1) {
+    mma_f16(c, a[0].x, a[0].y, a[0].z, a[0].w, b0, b1);
+  } else {
+    float x[4] = {0.f, 0.f, 0.f, 0.f};
+    mma_f16(x, a[Q2 - 1].x, a[Q2 - 1].y, a[Q2 - 1].z, a[Q2 - 1].w, b0, b1);
+    mma_f16(x, a[0].x, a[0].y, a[0].z, a[0].w, b0, b1);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) c[k] += x[k];
+  }
+}
 __device__ __forceinline__ uint32_t transposed(uint32_t x) {
   uint32_t r;
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));

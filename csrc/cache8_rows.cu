@@ -290,16 +290,16 @@ __global__ void __launch_bounds__(kThreads, 1) cache8_rows_kernel(const __grid_c
         for (int j = 0; j < J; ++j) {
           if (j + 1 < J) operands(j + 1);
 #pragma unroll
-          for (int w = 0; w < Q2; ++w)
+          for (int m = 0; m < M; ++m) {
+            uint4 q[Q2];
 #pragma unroll
-            for (int m = 0; m < M; ++m) {
-              const uint4 q = qf[j & 1][w][m];
+            for (int w = 0; w < Q2; ++w) q[w] = qf[j & 1][w][m];
 #pragma unroll
-              for (int mt = 0; mt < MT; ++mt) {
-                mma_f16(s[mt][m][0], q.x, q.y, q.z, q.w, kf[j & 1][mt][0], kf[j & 1][mt][1]);
-                mma_f16(s[mt][m][1], q.x, q.y, q.z, q.w, kf[j & 1][mt][2], kf[j & 1][mt][3]);
-              }
+            for (int mt = 0; mt < MT; ++mt) {
+              mma_sum<Q2>(s[mt][m][0], q, kf[j & 1][mt][0], kf[j & 1][mt][1]);
+              mma_sum<Q2>(s[mt][m][1], q, kf[j & 1][mt][2], kf[j & 1][mt][3]);
             }
+          }
         }
 
         // ---- scores of tokens 2t + {0, 1} and 8 more, rows g (k = 0, 1) and g + 8 (k = 2, 3) ----
@@ -404,11 +404,12 @@ __global__ void __launch_bounds__(kThreads, 1) cache8_rows_kernel(const __grid_c
         // ---- probabilities, and O += P V ----
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt) {
-          uint32_t pf[Q2][M][4];
+          uint4 pf[M][Q2];
           const bool odd = !(va[mt] < INFINITY);  // a block that is not finite: what is hidden counts for nothing all the same
 #pragma unroll
           for (int m = 0; m < M; ++m) {
             const float r[2] = {va[mt] * v_inv[m][0], va[mt] * v_inv[m][1]};
+            uint32_t f[Q2][4];
 #pragma unroll
             for (int n = 0; n < 2; ++n)
 #pragma unroll
@@ -423,9 +424,11 @@ __global__ void __launch_bounds__(kThreads, 1) cache8_rows_kernel(const __grid_c
                   if (odd && x == -INFINITY) pr[k] = 0.f;
                 }
                 const __half2 v = __floats2half2_rn(pr[0], pr[1]);
-                pf[0][m][2 * n + e] = as_u32(v);
-                if (kTwo) pf[Q2 - 1][m][2 * n + e] = as_u32(__floats2half2_rn(pr[0] - __low2float(v), pr[1] - __high2float(v)));
+                f[0][2 * n + e] = as_u32(v);
+                if (kTwo) f[Q2 - 1][2 * n + e] = as_u32(__floats2half2_rn(pr[0] - __low2float(v), pr[1] - __high2float(v)));
               }
+#pragma unroll
+            for (int w = 0; w < Q2; ++w) pf[m][w] = make_uint4(f[w][0], f[w][1], f[w][2], f[w][3]);
           }
           const int token = min(part + mt, kTiles - 1) * 16 + v_token;
           uint32_t vf[2][4];
@@ -436,12 +439,10 @@ __global__ void __launch_bounds__(kThreads, 1) cache8_rows_kernel(const __grid_c
             if (i + 1 < J) values(i + 1);
             const uint32_t(&v)[4] = vf[i & 1];
 #pragma unroll
-            for (int w = 0; w < Q2; ++w)
-#pragma unroll
-              for (int m = 0; m < M; ++m) {
-                mma_f16(o[m][2 * i], pf[w][m][0], pf[w][m][1], pf[w][m][2], pf[w][m][3], v[0], v[1]);
-                mma_f16(o[m][2 * i + 1], pf[w][m][0], pf[w][m][1], pf[w][m][2], pf[w][m][3], v[2], v[3]);
-              }
+            for (int m = 0; m < M; ++m) {
+              mma_sum<Q2>(o[m][2 * i], pf[m], v[0], v[1]);
+              mma_sum<Q2>(o[m][2 * i + 1], pf[m], v[2], v[3]);
+            }
           }
         }
       }
