@@ -744,11 +744,13 @@ constexpr int kMaxTeamBytes = 72 * 1024;
 size_t team_bytes(const Cache8& c, int rows, bool scores) {
   return 4ull * rows * ((rows <= 4 && c.dim == 64 ? 16ull : 8ull) * c.dim + (scores && c.weight != nullptr ? c.slots : 0));
 }
-// Whether a CTA takes a whole (row, head): caches of up to 1024 slots, and longer ones where there are several CTAs' worth
-// for every SM.
+// Whether a CTA takes a whole (row, head): caches of up to 2048 slots, and of up to 8192 where there are three for every two
+// SMs. One query a head, most slots held, us so / in pieces: 12 heads of 64 channels over 2048 slots 11.3 / 14.7, over 4096
+// 17.2 / 14.5; 8 heads of 128 channels, 8 queries each, 16.8 / 17.0 and 28.2 / 16.9; 128 heads of 64 channels over 8192 slots
+// 37.9 / 35.5, 256 of them 47.5 / 55.0; 64 x 32 of them, of all lengths, 237 / 274.
 bool by_row_head(const Cache8& c, int rows) {
   const long long bh = static_cast<long long>(c.batch) * c.heads;
-  return rows <= 8 && team_bytes(c, rows, true) <= kMaxTeamBytes && (c.slots <= 1024 || (c.slots <= 8192 && bh >= 6LL * num_sms()));
+  return rows <= 8 && team_bytes(c, rows, true) <= kMaxTeamBytes && (c.slots <= 2048 || (c.slots <= 8192 && 2 * bh >= 3LL * num_sms()));
 }
 
 template <typename T, int D, int MT, bool kTwo, Deal kDeal, int kWarps, bool kFold>
@@ -774,7 +776,9 @@ cudaError_t launch_tile(const Cache8Attn& p, const NewTokens<T>& fresh, bool beh
 template <typename T, bool kTwo>
 cudaError_t launch_row_heads(const Cache8Attn& p, const T5xNewTokens* tokens, cudaStream_t stream) {
   const NewTokens<T> fresh = make_tokens<T>(tokens);
-  // half the warps where there are CTAs for all SMs: what a CTA does around its tiles overlaps more of the others' tiles
+  // Half the warps where there are two CTAs for every SM: what a CTA does around its tiles overlaps more of the others' tiles.
+  // 1024 slots, heads of 64 channels, all lengths, us with 4 warps / 8: 256 (row, head) 11.4 / 10.4, 512 15.9 / 18.8, 2048
+  // 48.6 / 65.8 (2 warps: 52 to 63 for 45 to 59).
   const bool many = static_cast<long long>(p.c.batch) * p.c.heads >= 2LL * num_sms();
   auto launch_with = [&](auto kernel_warps) {
     constexpr int W = decltype(kernel_warps)::value;
@@ -834,11 +838,13 @@ Plan plan(Cache8 c, int rows, int type) {
   if (by_row_head(c, rows)) return w;
   c.batch = rows_at_a_time(c, rows);
   const int tile_rows = rows <= 8 ? 8 : row_tile_of(type, rows), row_tiles = (rows + tile_rows - 1) / tile_rows;
-  // Pieces for all CTAs that the SMs hold at a time, none of under 64 tokens a warp. Beginning a (row, head) costs as much as
+  // Pieces for all CTAs that the SMs hold at a time, none of under 64 tokens a warp; over many rows, where a CTA has its steps of
+  // 64 tokens to itself, none of under one (8 heads of 128 channels over 512 slots, 64 rows: 16.7 us, 18.3 with two steps, 25.1
+  // with eight; 500 rows: 39, 44, 64; over 8192 slots the same). Beginning a (row, head) costs as much as
   // 24 tiles where a CTA does some four of them a us (us for long contexts of all lengths / for 4 x 16 heads of 64 channels by
   // up to 16384 tokens with 8: 101 / 42, 16: 93 / 30, 24: 93 / 26, 40: 93 / 25).
   w.entry = rows <= 8 ? 24 : 6;
-  w.least = (rows <= 8 ? 32 : 8) + w.entry;
+  w.least = (rows <= 8 ? 32 : 4) + w.entry;
   long long room = 2LL * num_sms();
   if (rows > 8) {
     w.row_warps = row_tiles > 4 ? kRowWarps : row_tiles > 2 || rows > kFewRows ? 4 : 2;

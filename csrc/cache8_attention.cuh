@@ -180,7 +180,9 @@ cudaError_t launch_behind(bool behind, void (*kernel)(Params...), dim3 grid, int
 
 // Attention of many query rows (cache8_rows.cu). type: 0 bf16, 1 fp16, 2 fp32.
 constexpr int kRowWarps = 8;
-constexpr int kFewRows = 64;
+// Few rows are dealt 16 a warp (8 heads of 128 channels over 8192 slots, us with 16 / 32: 16 rows 21 / 33, 64 27 / 35, 128 35 /
+// 39, 192 56 / 50).
+constexpr int kFewRows = 128;
 constexpr int row_tile_of(int type, int rows) { return type == 2 || rows <= kFewRows ? 16 : 32; }  // query rows of a warp
 cudaError_t launch_cache8_rows(const Cache8Attn& p, int type, bool behind, cudaStream_t stream);
 

@@ -338,6 +338,20 @@ def test_many_rows(c, dtype):
   launches(lambda: plain.check_attention(c, "cuda", dtype))
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("c", [
+    dict(b=4, h=2, group=1, dim=64, slots=2064, block=16, starts=[0, 2063, 5, 1030], count=1, bias=True, weights=True),
+    dict(b=3, h=1, group=4, dim=64, slots=2080, block=32, starts=[2000, 0, 700], count=2, weights=True, positions=True, bias=True),
+    dict(b=2, h=3, group=3, dim=64, slots=2064, block=16, starts=[1500, 17], count=1, mask=True, weights=True),
+    dict(b=3, h=2, group=1, dim=128, slots=2176, block=128, starts=[0, 2176, 901], count=3, cross=True, mask=True),
+    dict(b=2, h=1, group=7, dim=128, slots=2112, block=64, starts=[2111, 1], count=1, bias=True, positions=True),
+    dict(b=1, h=1, group=2, dim=128, slots=2064, block=16, starts=[3], count=4, own=True, weights=True),
+], ids=range(6))
+def test_pieces(c, dtype):
+  """Caches that are cut into pieces: rows that hold nothing, a token, all; a piece's border inside a row."""
+  launches(lambda: plain.check_attention(c, "cuda", dtype))
+
+
 def check_some_rows(c, rows, dtype=torch.bfloat16):
   """As check_attention, for some rows of a batch."""
   cache, query, key, value, kw = plain.inputs(c, "cuda", dtype)
@@ -361,6 +375,19 @@ def test_more_rows_than_a_launch_takes():
   starts = [(7 * i) % 1024 for i in range(2050)]
   for count in (1, 9):
     check_some_rows(dict(b=2050, h=1, group=1, dim=64, slots=1040, block=16, starts=starts, count=count), [0, 2047, 2048, 2049])
+  # and in pieces
+  gen = torch.Generator("cuda").manual_seed(0)
+  cache = cache8.init_cache(2050, 8208, 1, 64, "cuda", block=16)
+  for n in ("key", "value"):
+    cache["cached_" + n].copy_(torch.randint(-127, 128, cache["cached_" + n].shape, generator=gen, device="cuda", dtype=torch.int8))
+    cache[n + "_absmax"].fill_(2.0)
+  starts = [(31 * i) % 999 for i in range(2050)]
+  cache["cache_index"].copy_(torch.tensor(starts))
+  query, key, value = [torch.randn(2050, 1, 1, 64, generator=gen, device="cuda").bfloat16() / 4 for _ in range(3)]
+  out = launches(lambda: cache8.attention(query, cache, key, value))
+  for i in (0, 1, 2046, 2047, 2048, 2049):
+    want, size, high, _ = plain.attention_oracle(query[i:i + 1], {n: t[i:i + 1] for n, t in cache.items()}, [starts[i]], 1)
+    assert plain.within(out[i:i + 1], want, size, high, 64, 8208), i
 
 
 def test_more_scores_than_a_launch_takes():
