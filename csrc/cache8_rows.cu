@@ -7,6 +7,11 @@
 // swizzled by token. A warp has 32 query rows (16 of 32-bit types, as two fp16 numbers each): S = Q K^T with the rows in the
 // 16-row operand, whose result is, lane for lane, the first operand of O = P V. Where there are fewer rows than eight warps
 // take, warps share rows, take different tokens of a step, and meet in shared memory at the end.
+//
+// Bound by latency between the products: two warps a scheduler (128 sums a lane leave no room for more) keep the matrix pipe
+// 38 % busy, the issue slots 33 %. Measured, us for 2 x 4 heads of 128 channels with the append and the join: 500 rows over
+// 8192 slots 86, over 32768 277 (242 TFLOP/s); 256 rows over 8192 55, 64 rows 27. Two tiles of tokens at a time instead of
+// one: 90 to 86 and 306 to 277; operands requested a step ahead: 96 to 90.
 #include <algorithm>
 #include <type_traits>
 
