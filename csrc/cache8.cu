@@ -33,6 +33,144 @@ __global__ void __launch_bounds__(kAppendThreads)
 }
 
 // ---------------------------------------------------------------------------
+// Eviction: the tokens that stay. A warp takes up to 32 tokens of one block of one head of the smaller cache.
+// Tokens of a new block come from many old ones, so nearly all codes are rounded again, 16 at a time: as numbers (a byte under
+// the exponent of 2^23), times the ratio of the scales, back under the exponent of 3 * 2^22, which rounds to whole numbers. Near a
+// border between two codes as Coder does it. 64 heads of 128 channels, 4096 tokens each: 33 us for 137 MB, 4.2 TB/s, half of
+// the issue slots; keys and values requested together were no faster.
+// ---------------------------------------------------------------------------
+constexpr int kMoveThreads = 128;
+
+__device__ __forceinline__ float code_number(uint32_t w, int i) {
+  return __uint_as_float(__byte_perm(w ^ 0x80808080u, 0x4b000000u, 0x7440 + i)) - 8388736.f;
+}
+// with short scales (Coder)
+__device__ __forceinline__ uint32_t round_four(uint32_t w, float ratio) {
+  const uint32_t u = w ^ 0x80808080u;
+  const uint64_t less = pair_of(-8388736.f, -8388736.f), by = pair_of(ratio, ratio);
+  auto two = [&](int i) {
+    return codes_of_two(add2(pair_of(__uint_as_float(__byte_perm(u, 0x4b000000u, 0x7440 + i)),
+                                     __uint_as_float(__byte_perm(u, 0x4b000000u, 0x7441 + i))), less), by);
+  };
+  return low_bytes(two(0), two(2));
+}
+// with any; off: how far a quotient is from its code
+__device__ __forceinline__ uint32_t round_four(uint32_t w, float ratio, float& off) {
+  uint32_t r[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float q = code_number(w, i) * ratio, up = q + 12582912.f;
+    off = fmaxf(off, fabsf(q - (up - 12582912.f)));
+    r[i] = __float_as_uint(up);
+  }
+  return low_bytes(r);
+}
+
+__device__ __forceinline__ uint32_t round_four_exactly(uint32_t w, const Coder& again) {
+  uint32_t r = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    r |= static_cast<uint32_t>(again.of<true>(static_cast<float>(static_cast<int8_t>(w >> (8 * i)))) & 0xff) << (8 * i);
+  return r;
+}
+
+// What a token's codes go through: their scale is the block's (kAsIs), else times the ratio of the two.
+constexpr float kAsIs = -1.f, kByCoder = -2.f;
+__device__ __forceinline__ float ratio_of(float old, float a) {
+  if (abs_bits(old) == abs_bits(a)) return kAsIs;
+  return a >= 0x1p-60f && a <= 0x1p100f ? __fdiv_rn(old, a) : kByCoder;
+}
+
+__device__ __forceinline__ int span_of(const Cache8& to) { return min(1 << to.block_log2, 32); }  // tokens of a warp
+
+// Tokens lo on, of the n that stay.
+template <int D>
+__device__ __forceinline__ void move_span(const Cache8& c, const Cache8& to, int keep, const int* kept, int b, int h, int lo, int n) {
+  constexpr int L = D / 16, kTokens = 32 / L, U = 4;  // lanes a token, tokens at a time, turns requested at a time
+  const int lane = threadIdx.x & 31;
+  const int block = 1 << to.block_log2, span = span_of(to);
+  const int first = lo & ~(block - 1), count = min(block, n - first), mine = min(span, n - lo);
+  const long long bh = static_cast<long long>(b) * c.heads + h;
+  const int* from = kept + bh * keep + first;
+
+  // the block's scale; lane i's token is lo + i
+  int slot = 0;
+  float old[2] = {0.f, 0.f};
+  uint32_t most[2] = {0, 0}, bits[2] = {0, 0};
+  for (int j0 = 0; j0 < count; j0 += 32) {
+    const int j = j0 + lane;
+    const int s = j < count ? __ldcg(from + j) : 0;
+#pragma unroll
+    for (int what = 0; what < 2; ++what) {
+      const float x = j < count ? c.absmax[what][bh * (c.slots >> c.block_log2) + (s >> c.block_log2)] : 0.f;
+      most[what] = max(most[what], abs_bits(x));
+      bits[what] |= abs_bits(x);
+      if (j0 == ((lo - first) & ~31)) old[what] = x;
+    }
+    if (j0 == ((lo - first) & ~31)) slot = s;
+  }
+  float a[2], ratio[2];
+  bool brief[2];
+#pragma unroll
+  for (int what = 0; what < 2; ++what) {
+    a[what] = __uint_as_float(__reduce_max_sync(0xffffffffu, most[what]));
+    brief[what] = (__reduce_or_sync(0xffffffffu, bits[what]) & 0x1fffu) == 0;
+    ratio[what] = ratio_of(old[what], a[what]);
+    if (lo == first && lane == 0) to.absmax[what][bh * (to.slots >> to.block_log2) + (first >> to.block_log2)] = a[what];
+  }
+  if (lane < mine) {
+    to.weight[bh * to.slots + lo + lane] = c.weight[bh * c.slots + slot];
+    to.position[bh * to.slots + lo + lane] = c.position != nullptr ? c.position[bh * c.slots + slot] : slot;
+  }
+
+  const int tok = lane / L, part = lane % L;
+#pragma unroll
+  for (int what = 0; what < 2; ++what) {
+    const int8_t* src = c.codes[what] + bh * c.slots * D + 16 * part;
+    int8_t* dst = to.codes[what] + (bh * to.slots + lo) * D + 16 * part;
+    for (int i0 = 0; i0 < mine; i0 += U * kTokens) {
+      uint4 v[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int i = i0 + u * kTokens + tok, s = __shfl_sync(0xffffffffu, slot, i & 31);
+        if (i < mine) v[u] = *reinterpret_cast<const uint4*>(src + static_cast<long long>(s) * D);
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int i = i0 + u * kTokens + tok;
+        const float r = __shfl_sync(0xffffffffu, ratio[what], i & 31), before = __shfl_sync(0xffffffffu, old[what], i & 31);
+        if (i >= mine) continue;
+        uint4 o = v[u];
+        if (r != kAsIs) {
+          float off = 0.f;
+          if (brief[what] && r != kByCoder) {
+            o = make_uint4(round_four(o.x, r), round_four(o.y, r), round_four(o.z, r), round_four(o.w, r));
+          } else {
+            o = make_uint4(round_four(o.x, r, off), round_four(o.y, r, off), round_four(o.z, r, off), round_four(o.w, r, off));
+            if (r == kByCoder || off >= 0.4999f) {
+              const Coder again(before, a[what]);
+              o = make_uint4(round_four_exactly(v[u].x, again), round_four_exactly(v[u].y, again),
+                             round_four_exactly(v[u].z, again), round_four_exactly(v[u].w, again));
+            }
+          }
+        }
+        *reinterpret_cast<uint4*>(dst + i * D) = o;
+      }
+    }
+  }
+}
+
+template <int D>
+__global__ void __launch_bounds__(kMoveThreads)
+    cache8_move_kernel(const __grid_constant__ Cache8 c, const __grid_constant__ Cache8 to, int keep,
+                       const int* __restrict__ kept) {
+  const int b = blockIdx.z, lo = (blockIdx.x * (kMoveThreads / 32) + (threadIdx.x >> 5)) * span_of(to);
+  const int n = min(held_of(c, b), keep);
+  chain_wait();
+  if (lo < n) move_span<D>(c, to, keep, kept, b, blockIdx.y, lo, n);
+}
+
+// ---------------------------------------------------------------------------
 // Eviction: which slots stay.
 // ---------------------------------------------------------------------------
 // Order of weights as unsigned numbers: NaN above all, -0 as 0.
@@ -86,9 +224,7 @@ __device__ __forceinline__ void remote_add(int* mine, int v) {  // to the cluste
 constexpr uint32_t kZero = 0x80000000u;  // order_of(0); of no weight 0
 
 template <int T, int K, int kCtas>
-__global__ void __launch_bounds__(T, 1024 / T)
-    cache8_select_kernel(const __grid_constant__ Cache8 c, int keep, int recent, int* __restrict__ kept,
-                         int* __restrict__ index_out, int* __restrict__ dropped_out) {
+__device__ __forceinline__ void select_slots(const Cache8& c, int keep, int recent, int* kept, int* index_out, int* dropped_out) {
   constexpr int kWarps = T / 32;
   constexpr bool kCluster = kCtas > 1;
   static_assert(T * K < 65536, "two counts in 32 bits");
@@ -239,6 +375,24 @@ __global__ void __launch_bounds__(T, 1024 / T)
   if (kCluster) cluster_sync_all();  // nobody leaves while others read its sums
 }
 
+template <int T, int K, int kCtas>
+__global__ void __launch_bounds__(T, 1024 / T)
+    cache8_select_kernel(const __grid_constant__ Cache8 c, int keep, int recent, int* __restrict__ kept,
+                         int* __restrict__ index_out, int* __restrict__ dropped_out) {
+  select_slots<T, K, kCtas>(c, keep, recent, kept, index_out, dropped_out);
+}
+
+// The choice and the move in one launch.
+template <int T, int K, int D>
+__global__ void __launch_bounds__(T, 1024 / T)
+    cache8_evict_kernel(const __grid_constant__ Cache8 c, const __grid_constant__ Cache8 to, int keep, int recent,
+                        int* kept, int* index_out, int* dropped_out) {
+  const int b = blockIdx.x / c.heads, h = blockIdx.x - b * c.heads, n = min(held_of(c, b), keep), span = span_of(to);
+  select_slots<T, K, 1>(c, keep, recent, kept, index_out, dropped_out);
+  __syncthreads();
+  for (int lo = (threadIdx.x >> 5) * span; lo < n; lo += T / 32 * span) move_span<D>(c, to, keep, kept, b, h, lo, n);
+}
+
 // Over more slots than a cluster's registers hold the weights are read once for each digit.
 constexpr int kWalkThreads = 1024;
 
@@ -329,137 +483,6 @@ __global__ void __launch_bounds__(kWalkThreads)
   }
 }
 
-// ---------------------------------------------------------------------------
-// Eviction: the tokens that stay. A warp takes up to 32 tokens of one block of one head of the smaller cache.
-// Tokens of a new block come from many old ones, so nearly all codes are rounded again, 16 at a time: as numbers (a byte under
-// the exponent of 2^23), times the ratio of the scales, back under the exponent of 3 * 2^22, which rounds to whole numbers. Near a
-// border between two codes as Coder does it. 64 heads of 128 channels, 4096 tokens each: 33 us for 137 MB, 4.2 TB/s, half of
-// the issue slots; keys and values requested together were no faster.
-// ---------------------------------------------------------------------------
-constexpr int kMoveThreads = 128;
-
-__device__ __forceinline__ float code_number(uint32_t w, int i) {
-  return __uint_as_float(__byte_perm(w ^ 0x80808080u, 0x4b000000u, 0x7440 + i)) - 8388736.f;
-}
-// with short scales (Coder)
-__device__ __forceinline__ uint32_t round_four(uint32_t w, float ratio) {
-  const uint32_t u = w ^ 0x80808080u;
-  const uint64_t less = pair_of(-8388736.f, -8388736.f), by = pair_of(ratio, ratio);
-  auto two = [&](int i) {
-    return codes_of_two(add2(pair_of(__uint_as_float(__byte_perm(u, 0x4b000000u, 0x7440 + i)),
-                                     __uint_as_float(__byte_perm(u, 0x4b000000u, 0x7441 + i))), less), by);
-  };
-  return low_bytes(two(0), two(2));
-}
-// with any; off: how far a quotient is from its code
-__device__ __forceinline__ uint32_t round_four(uint32_t w, float ratio, float& off) {
-  uint32_t r[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float q = code_number(w, i) * ratio, up = q + 12582912.f;
-    off = fmaxf(off, fabsf(q - (up - 12582912.f)));
-    r[i] = __float_as_uint(up);
-  }
-  return low_bytes(r);
-}
-
-__device__ __forceinline__ uint32_t round_four_exactly(uint32_t w, const Coder& again) {
-  uint32_t r = 0;
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-    r |= static_cast<uint32_t>(again.of<true>(static_cast<float>(static_cast<int8_t>(w >> (8 * i)))) & 0xff) << (8 * i);
-  return r;
-}
-
-// What a token's codes go through: their scale is the block's (kAsIs), else times the ratio of the two.
-constexpr float kAsIs = -1.f, kByCoder = -2.f;
-__device__ __forceinline__ float ratio_of(float old, float a) {
-  if (abs_bits(old) == abs_bits(a)) return kAsIs;
-  return a >= 0x1p-60f && a <= 0x1p100f ? __fdiv_rn(old, a) : kByCoder;
-}
-
-template <int D>
-__global__ void __launch_bounds__(kMoveThreads)
-    cache8_move_kernel(const __grid_constant__ Cache8 c, const __grid_constant__ Cache8 to, int keep,
-                       const int* __restrict__ kept) {
-  constexpr int L = D / 16, kTokens = 32 / L, U = 4;  // lanes a token, tokens at a time, turns requested at a time
-  const int b = blockIdx.z, h = blockIdx.y, lane = threadIdx.x & 31;
-  const int block = 1 << to.block_log2, span = min(block, 32);
-  const int lo = (blockIdx.x * (kMoveThreads / 32) + (threadIdx.x >> 5)) * span;  // this warp's first token
-  const int n = min(held_of(c, b), keep);
-  chain_wait();
-  if (lo >= n) return;
-  const int first = lo & ~(block - 1), count = min(block, n - first), mine = min(span, n - lo);
-  const long long bh = static_cast<long long>(b) * c.heads + h;
-  const int* from = kept + bh * keep + first;
-
-  // the block's scale; lane i's token is lo + i
-  int slot = 0;
-  float old[2] = {0.f, 0.f};
-  uint32_t most[2] = {0, 0}, bits[2] = {0, 0};
-  for (int j0 = 0; j0 < count; j0 += 32) {
-    const int j = j0 + lane;
-    const int s = j < count ? __ldcg(from + j) : 0;
-#pragma unroll
-    for (int what = 0; what < 2; ++what) {
-      const float x = j < count ? c.absmax[what][bh * (c.slots >> c.block_log2) + (s >> c.block_log2)] : 0.f;
-      most[what] = max(most[what], abs_bits(x));
-      bits[what] |= abs_bits(x);
-      if (j0 == ((lo - first) & ~31)) old[what] = x;
-    }
-    if (j0 == ((lo - first) & ~31)) slot = s;
-  }
-  float a[2], ratio[2];
-  bool brief[2];
-#pragma unroll
-  for (int what = 0; what < 2; ++what) {
-    a[what] = __uint_as_float(__reduce_max_sync(0xffffffffu, most[what]));
-    brief[what] = (__reduce_or_sync(0xffffffffu, bits[what]) & 0x1fffu) == 0;
-    ratio[what] = ratio_of(old[what], a[what]);
-    if (lo == first && lane == 0) to.absmax[what][bh * (to.slots >> to.block_log2) + (first >> to.block_log2)] = a[what];
-  }
-  if (lane < mine) {
-    to.weight[bh * to.slots + lo + lane] = c.weight[bh * c.slots + slot];
-    to.position[bh * to.slots + lo + lane] = c.position != nullptr ? c.position[bh * c.slots + slot] : slot;
-  }
-
-  const int tok = lane / L, part = lane % L;
-#pragma unroll
-  for (int what = 0; what < 2; ++what) {
-    const int8_t* src = c.codes[what] + bh * c.slots * D + 16 * part;
-    int8_t* dst = to.codes[what] + (bh * to.slots + lo) * D + 16 * part;
-    for (int i0 = 0; i0 < mine; i0 += U * kTokens) {
-      uint4 v[U];
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const int i = i0 + u * kTokens + tok, s = __shfl_sync(0xffffffffu, slot, i & 31);
-        if (i < mine) v[u] = *reinterpret_cast<const uint4*>(src + static_cast<long long>(s) * D);
-      }
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const int i = i0 + u * kTokens + tok;
-        const float r = __shfl_sync(0xffffffffu, ratio[what], i & 31), before = __shfl_sync(0xffffffffu, old[what], i & 31);
-        if (i >= mine) continue;
-        uint4 o = v[u];
-        if (r != kAsIs) {
-          float off = 0.f;
-          if (brief[what] && r != kByCoder) {
-            o = make_uint4(round_four(o.x, r), round_four(o.y, r), round_four(o.z, r), round_four(o.w, r));
-          } else {
-            o = make_uint4(round_four(o.x, r, off), round_four(o.y, r, off), round_four(o.z, r, off), round_four(o.w, r, off));
-            if (r == kByCoder || off >= 0.4999f) {
-              const Coder again(before, a[what]);
-              o = make_uint4(round_four_exactly(v[u].x, again), round_four_exactly(v[u].y, again),
-                             round_four_exactly(v[u].z, again), round_four_exactly(v[u].w, again));
-            }
-          }
-        }
-        *reinterpret_cast<uint4*>(dst + i * D) = o;
-      }
-    }
-  }
-}
-
 }  // namespace
 
 // What every entry asks of a cache.
@@ -545,6 +568,19 @@ cudaError_t launch_select(const Cache8& c, int keep, int recent, int* kept, int*
   return cudaGetLastError();
 }
 
+// Both in one launch where a CTA makes the choice and has a turn of its warps to move: the device takes as long (12 heads of 64
+// channels, 640 -> 121, us so / in two 9.4 / 9.4; 2048 -> 250 10.1 / 9.9, -> 512 13.4 / 9.7; 512 heads, -> 512 29 / 30, of 128
+// channels 45 / 40), the host one launch less (11.7 to 10.3 a call).
+bool in_one_launch(const Cache8& c, int keep) { return c.slots <= 2048 && keep <= 256; }
+template <int D>
+cudaError_t launch_both(const Cache8& c, const Cache8& to, int keep, int recent, int* kept, int* index_out, int* dropped_out,
+                        cudaStream_t stream) {
+  cache8_evict_kernel<256, 8, D><<<static_cast<unsigned>(c.batch) * c.heads, 256, 0, stream>>>(c, to, keep, recent, kept, index_out,
+                                                                                          dropped_out);
+  count_launches(1);
+  return cudaGetLastError();
+}
+
 // The tokens behind the choice: the kernel begins while that still runs, and waits for it by itself.
 template <typename... Args>
 cudaError_t launch_move(void (*kernel)(Args...), dim3 grid, cudaStream_t stream, Args... args) {
@@ -602,13 +638,16 @@ T5X_API int t5x_cache8_evict(const T5xCache8* cache, const T5xCache8* into, int 
     return t5x::set_error("cache8_evict: %d of %d slots (the last %d) do not fit %d", keep, c.slots, recent, to.slots);
   if (c.batch == 0) return 0;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  cudaError_t e = t5x::launch_select(c, keep, recent, static_cast<int*>(kept), static_cast<int*>(index_out),
-                                     static_cast<int*>(dropped_out), st);
-  if (e == cudaSuccess) {
+  int *slots = static_cast<int*>(kept), *index = static_cast<int*>(index_out), *dropped = static_cast<int*>(dropped_out);
+  const bool both = t5x::in_one_launch(c, keep);
+  cudaError_t e = !both          ? t5x::launch_select(c, keep, recent, slots, index, dropped, st)
+                  : c.dim == 64 ? t5x::launch_both<64>(c, to, keep, recent, slots, index, dropped, st)
+                                : t5x::launch_both<128>(c, to, keep, recent, slots, index, dropped, st);
+  if (e == cudaSuccess && !both) {
     const int tokens = std::min(1 << to.block_log2, 32) * (t5x::kMoveThreads / 32);  // of a CTA
     const dim3 grid((keep + tokens - 1) / tokens, c.heads, c.batch);
     e = t5x::launch_move(c.dim == 64 ? t5x::cache8_move_kernel<64> : t5x::cache8_move_kernel<128>, grid, st, c, to, keep,
-                         static_cast<const int*>(kept));
+                         static_cast<const int*>(slots));
   }
   return e == cudaSuccess ? 0 : t5x::set_error("cache8_evict launch: %s", cudaGetErrorString(e));
 }

@@ -884,7 +884,8 @@ int check_query(const Cache8& c, const T5xCache8Query* q, const T5xNewTokens* n)
   if (!q->query || !q->out || !aligned_to(bytes, {q->query, q->out}) || !aligned_to(4, {q->table}))
     return set_error("cache8_attention: a null or misaligned pointer");
   if (q->table && (!q->buckets || q->distances < 1 || q->distances > kMaxDistances ||
-                   q->table_stride < 1 || q->table_stride * c.heads * q->group > kMaxBiases))
+                   q->table_stride < 1 || q->table_stride > kMaxBiases || q->table_stride * c.heads * q->group > kMaxBiases ||
+                   *std::max_element(q->buckets, q->buckets + q->distances) >= q->table_stride))
     return set_error("cache8_attention: biases of %d distances for %d heads", q->distances, q->group);
   if (q->key_mask && (q->mask_len < 0 || q->mask_len > c.slots)) return set_error("cache8_attention: a mask of %d slots", q->mask_len);
   if (c.weight && static_cast<long long>(q->count) * q->group * c.slots > 0x7fffffffLL)

@@ -170,6 +170,14 @@ def test_evict_from_long_caches(slots, keep, recent, special):
                                           recent=recent, to_block=128), "cuda", special))
 
 
+@pytest.mark.parametrize("slots,keep,recent", [(2048, 256, 256), (2048, 257, 3), (1024, 1000, 1), (640, 256, 0), (2048, 1, 1)])
+@pytest.mark.parametrize("dim,to_block", [(64, 16), (128, 128)])
+def test_evict_in_one_launch_and_two(slots, keep, recent, dim, to_block):
+  for special in (False, True):
+    launches(lambda: plain.check_evict(dict(b=3, h=2, dim=dim, slots=slots, block=32, starts=[slots, slots - 333, 200], keep=keep,
+                                            recent=recent, to_block=to_block), "cuda", special))
+
+
 @pytest.mark.parametrize("rows,k,n", [(1, 16, 8), (3, 17, 5), (5, 1, 3), (2, 300, 130), (33, 129, 257), (257, 64, 40),
                                       (130, 513, 300)])
 @pytest.mark.parametrize("dtype", TYPES)
