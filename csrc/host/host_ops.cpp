@@ -1313,9 +1313,11 @@ optional<Tensor> linear8(const Tensor& x, const Tensor& codes, const Tensor& abs
                    residual->sizes() != sizes || !residual->is_contiguous()))
     return std::nullopt;
   Tensor y = at::empty(sizes, x.options().requires_grad(false));
-  Tensor workspace = bytes_like(x, t5x_linear8_workspace_bytes(rows, k));
+  const long long bytes = t5x_linear8_workspace_bytes(rows, k);
+  Tensor workspace;
+  if (bytes > 0) workspace = bytes_like(x, bytes);
   check(t5x_linear8(x.data_ptr(), type, rows, k, k, codes.data_ptr(), absmax.data_ptr(), n, data_of(residual), n, y.data_ptr(),
-                    workspace.data_ptr(), stream_of()),
+                    bytes > 0 ? workspace.data_ptr() : nullptr, stream_of()),
         "linear8");
   return y;
 }

@@ -2,7 +2,8 @@
 // largest |x| of the row, cx = 127 x / sx rounded) and weights by output channel. The sums of products are whole numbers
 // below 2^31 for up to 131072 channels and exact; one rounding at the end.
 //
-// Two launches: the rows are turned into codes, and tcgen05 (kind::i8, sums in 32 bits in tensor memory) multiplies them.
+// Two launches, for more than two rows: the rows are turned into codes, and tcgen05 (kind::i8, sums in 32 bits in tensor memory)
+// multiplies them.
 // It runs at twice the rate of bf16, so that a large product has half the time of `native.gemm`; over few rows both are
 // bound by the weights' bytes, which are half of bf16's. 8192 x 10240 x 4096: 274 us, 42 for the codes and 226 for the product
 // (3.04 POP/s; the tensor pipe is 88 % busy), 210 at twice the measured rate of bf16.
@@ -371,7 +372,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 // cuts the input channels into one piece a CTA, so that all SMs stream weights at the same time. The weights are the 128-row
 // operand (tokens, of which there may be one, the other), and are requested while the rows are still turned into codes (a
 // programmatic dependent launch). The sums, whole numbers, meet through distributed shared memory, in no particular order:
-// they are exact. 61 x 4096 x 10240: 14.9 us with the rows' codes, 6.7 at the copy rate; 1 x 4096 x 32128: 26 of 20. What a
+// they are exact. 61 x 4096 x 10240: 14.9 us with the rows' codes, 6.7 at the copy rate. What a
 // CTA begins and ends with (the rows' codes, the sums of a cluster) is as long as the weights take.
 // ---------------------------------------------------------------------------
 constexpr int kFewThreads = 128;
@@ -591,6 +592,153 @@ __global__ void __launch_bounds__(kFewThreads)
   }
 }
 
+// ---------------------------------------------------------------------------
+// One row or two in one launch: each CTA turns them into codes for itself (they are in L2), behind its first requests for
+// weights; two CTAs an SM take output channels in turn, two a warp, 512 bytes of both at a time, by dot products of four bytes. The
+// weights' bytes bound it: 1 x 4096 x 32128 takes 21.9 us, 92 % of the copy rate.
+// ---------------------------------------------------------------------------
+constexpr int kOneThreads = 256;
+constexpr int kOneWarps = kOneThreads / 32;
+constexpr int kOneChannels = 2;          // of a warp
+constexpr int kOneHeld = 4;              // pieces of 16 bytes of a row that a thread keeps
+
+template <typename T, int R>
+__global__ void __launch_bounds__(kOneThreads)
+    linear8_one_kernel(const __grid_constant__ Linear8 p, const T* __restrict__ x, long long stride, int k, int vec,
+                       const int8_t* __restrict__ w) {
+  constexpr int E = 16 / sizeof(T), C = kOneChannels, U = 4;  // steps of 512 bytes requested at a time
+  constexpr int kHeld = kOneHeld;
+  extern __shared__ uint4 s_codes[];                          // [R][K / 16]
+  __shared__ uint32_t s_most[R][kOneWarps];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int pieces = p.K / 16, stride_n = gridDim.x * kOneWarps * C;
+  int n0 = (blockIdx.x * kOneWarps + warp) * C;
+  uint4 next[U][C];
+  auto request = [&](int n, int at) {
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+      const uint4* row = reinterpret_cast<const uint4*>(w + static_cast<long long>(min(n + c, p.N - 1)) * p.K);
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (at + u * 32 + lane < pieces) next[u][c] = __ldcs(row + at + u * 32 + lane);
+    }
+  };
+  if (n0 < p.N) request(n0, 0);
+
+  // ---- codes ----
+  uint4 held[R][kHeld];
+  const int whole = vec ? min(k, kHeld * kOneThreads * E) : 0;  // values in registers; the rest is read twice
+  uint32_t most[R];
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    most[r] = 0;
+    {
+#pragma unroll
+      for (int i = 0; i < kHeld; ++i) {
+        const int at = (i * kOneThreads + threadIdx.x) * E;
+        if (at < whole) held[r][i] = *reinterpret_cast<const uint4*>(x + r * stride + at);
+      }
+    }
+  }
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    {
+#pragma unroll
+      for (int i = 0; i < kHeld; ++i)
+        if ((i * kOneThreads + static_cast<int>(threadIdx.x)) * E < whole) {
+          const T* v = reinterpret_cast<const T*>(&held[r][i]);
+#pragma unroll
+          for (int e = 0; e < E; ++e) most[r] = max(most[r], abs_bits(to_float(v[e])));
+        }
+      for (int i = whole + threadIdx.x; i < k; i += kOneThreads) most[r] = max(most[r], abs_bits(to_float(x[r * stride + i])));
+    }
+    most[r] = __reduce_max_sync(0xffffffffu, most[r]);
+    if (lane == 0) s_most[r][warp] = most[r];
+  }
+  __syncthreads();
+  float scale[R];
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+#pragma unroll
+    for (int i = 0; i < kOneWarps; ++i) most[r] = max(most[r], s_most[r][i]);
+    const float a = __uint_as_float(most[r]);
+    scale[r] = a * (1.f / 127.f);
+    {
+      const Coder code(127.f, a);
+      auto of = [&](T v) { return code.template of<sizeof(T) == 2>(to_float(v)); };
+      int8_t* dst = reinterpret_cast<int8_t*>(s_codes) + r * p.K;
+#pragma unroll
+      for (int i = 0; i < kHeld; ++i) {
+        const int at = (i * kOneThreads + threadIdx.x) * E;
+        if (at < whole) {
+          const T* v = reinterpret_cast<const T*>(&held[r][i]);
+#pragma unroll
+          for (int e = 0; e < E; e += 4) *reinterpret_cast<char4*>(dst + at + e) = make_char4(of(v[e]), of(v[e + 1]), of(v[e + 2]), of(v[e + 3]));
+        }
+      }
+      for (int i = whole + threadIdx.x; i < p.K; i += kOneThreads) dst[i] = static_cast<int8_t>(i < k ? of(x[r * stride + i]) : 0);
+    }
+  }
+  __syncthreads();
+
+  // ---- products ----
+  for (; n0 < p.N; n0 += stride_n) {
+    int sum[R][C];
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+#pragma unroll
+      for (int c = 0; c < C; ++c) sum[r][c] = 0;
+    for (int at = 0; at < pieces; at += U * 32) {
+      uint4 here[U][C];
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int c = 0; c < C; ++c) here[u][c] = next[u][c];
+      if (at + U * 32 < pieces) request(n0, at + U * 32);
+      else if (n0 + stride_n < p.N) request(n0 + stride_n, 0);
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int piece = at + u * 32 + lane;
+        if (piece >= pieces) break;
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+          const uint4 q = s_codes[r * pieces + piece];
+#pragma unroll
+          for (int c = 0; c < C; ++c) {
+            sum[r][c] = __dp4a(static_cast<int>(here[u][c].x), static_cast<int>(q.x), sum[r][c]);
+            sum[r][c] = __dp4a(static_cast<int>(here[u][c].y), static_cast<int>(q.y), sum[r][c]);
+            sum[r][c] = __dp4a(static_cast<int>(here[u][c].z), static_cast<int>(q.z), sum[r][c]);
+            sum[r][c] = __dp4a(static_cast<int>(here[u][c].w), static_cast<int>(q.w), sum[r][c]);
+          }
+        }
+      }
+    }
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+#pragma unroll
+      for (int c = 0; c < C; ++c) {
+        const int all = __reduce_add_sync(0xffffffffu, sum[r][c]), n = n0 + c;
+        if (lane == r * C + c && n < p.N) {
+          const float add = p.residual != nullptr ? to_float(static_cast<const T*>(p.residual)[r * p.ld_res + n]) : 0.f;
+          static_cast<T*>(p.y)[r * static_cast<long long>(p.N) + n] =
+              from_float<T>(static_cast<float>(all) * scale[r] * (p.w_absmax[n] * (1.f / 127.f)) + add);
+        }
+      }
+  }
+}
+
+bool alone(int rows, int k) { return rows == 1 && k <= 32768; }  // a row that needs no workspace, whatever its type
+
+template <typename T, int R>
+cudaError_t launch_one(const T* x, long long stride, int k, const void* w, const Linear8& p, cudaStream_t stream) {
+  const int vec = k % (16 / static_cast<int>(sizeof(T))) == 0 && aligned_to(16, {x}) && stride * static_cast<long long>(sizeof(T)) % 16 == 0;
+  const int channels = kOneWarps * kOneChannels, most = 2 * num_sms();
+  linear8_one_kernel<T, R><<<std::min((p.N + channels - 1) / channels, most), kOneThreads, static_cast<size_t>(R) * p.K, stream>>>(
+      p, x, stride, k, vec, static_cast<const int8_t*>(w));
+  count_launches(1);
+  return cudaGetLastError();
+}
+
 bool map_of(CUtensorMap* map, const void* codes, int rows, int k, uint32_t box_rows = kRows) {
   const uint64_t dims[3] = {static_cast<uint64_t>(k), static_cast<uint64_t>(rows), 1};
   const uint64_t strides[2] = {static_cast<uint64_t>(k), static_cast<uint64_t>(k) * rows};
@@ -627,6 +775,16 @@ cudaError_t launch_few(const Linear8Maps& maps, const Linear8& p, int splits, cu
 
 template <typename T>
 int launch(const void* x, long long stride, int k, int8_t* codes, const void* w, Linear8 p, cudaStream_t stream) {
+  // us in one launch / as below, rows x in x out: 1 x 1024 x 2816 3.1 / 5.4, 1 x 4096 x 10240 9.9 / 12.4, 1 x 10240 x 4096 11.1 /
+  // 12.4, 2 x 1024 x 2816 4.2 / 5.4, 2 x 4096 x 32128 23.5 / 25.8, 2 x 10240 x 4096 (two rows of which a CTA reads a part twice)
+  // 13.8 / 12.3; four rows 6 to 11 / 5.5.
+  constexpr int kOneValues = kOneHeld * kOneThreads * 16 / static_cast<int>(sizeof(T));  // of a row in a CTA's registers
+  if (alone(p.M, p.K) || (p.M == 2 && p.K <= kOneValues)) {
+    const T* rows = static_cast<const T*>(x);
+    const cudaError_t e = p.M == 1   ? launch_one<T, 1>(rows, stride, k, w, p, stream)
+                                     : launch_one<T, 2>(rows, stride, k, w, p, stream);
+    return e == cudaSuccess ? 0 : set_error("linear8 launch: %s", cudaGetErrorString(e));
+  }
   float* absmax = const_cast<float*>(p.x_absmax);
   launch_rows<T>(x, stride, p.M, k, p.K, codes, absmax, stream);
   Linear8Maps maps;
@@ -688,6 +846,7 @@ T5X_API int t5x_quantize_rows(const void* x, int type, long long rows, int k, lo
 }
 
 T5X_API long long t5x_linear8_workspace_bytes(int rows, int k) {
+  if (t5x::alone(rows, (k + 15) / 16 * 16)) return 0;
   return (static_cast<long long>(rows) * ((k + 15) / 16 * 16) + 127) / 128 * 128 + static_cast<long long>(rows) * 4;
 }
 
@@ -698,8 +857,8 @@ T5X_API int t5x_linear8(const void* x, int type, int rows, int k, long long stri
     return t5x::set_error("linear8: %d rows, %d -> %d channels (at most %d), type %d", rows, k, n, t5x::kMaxK, type);
   if (rows == 0) return 0;
   const int size = type == 2 ? 4 : 2;
-  if (!x || !w || !w_absmax || !y || !workspace || !t5x::aligned_to(size, {x, y, residual}) ||
-      !t5x::aligned_to(16, {w, workspace}) || !t5x::aligned_to(4, {w_absmax}))
+  if (!x || !w || !w_absmax || !y || (!workspace && t5x_linear8_workspace_bytes(rows, k) > 0) ||
+      !t5x::aligned_to(size, {x, y, residual}) || !t5x::aligned_to(16, {w, workspace}) || !t5x::aligned_to(4, {w_absmax}))
     return t5x::set_error("linear8: a null or misaligned pointer");
   t5x::Linear8 p = {};
   p.M = rows;

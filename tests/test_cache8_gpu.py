@@ -224,6 +224,25 @@ def test_linear8_of_wide_outputs(rows, k, n, dtype):
     assert bool((off <= size * 2.0 ** -21 * (1 + info.eps) + info.smallest_normal * info.eps / 2).all())
 
 
+@pytest.mark.parametrize("rows,k,n", [(1, 1, 1), (1, 16, 5), (2, 8192, 33), (2, 8208, 33), (2, 4096, 5000), (1, 32768, 70), (1, 32784, 70),
+                                      (1, 2047, 9001), (2, 515, 4799), (1, 12000, 17)])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_linear8_of_one_row_and_two(rows, k, n, dtype):
+  gen = torch.Generator("cuda").manual_seed(rows)
+  randn = lambda *s: torch.randn(*s, generator=gen, device="cuda")  # noqa: E731
+  weight = F.quantize_weight(randn(k, n))
+  x, r = randn(rows, k).to(dtype), randn(rows, n).to(dtype)
+  for residual in (None, r):
+    y = launches(lambda: F.linear8(x, weight, residual))  # noqa: B023
+    want = ref.linear8(x.double(), weight.codes[:, :k], weight.absmax, None if residual is None else residual.double())
+    # eight roundings in 32 bits of the product, and the last one
+    size = (want if residual is None else want - residual.double()).abs() + want.abs()
+    info = torch.finfo(dtype)
+    off = (y.double() - want).abs() - info.eps / 2 * want.abs()
+    # (results below the smallest normal number are a whole number of its steps: half a step is smallest * eps / 2)
+    assert bool((off <= size * 2.0 ** -21 * (1 + info.eps) + info.smallest_normal * info.eps / 2).all())
+
+
 def test_linear8_strides():
   weight = F.quantize_weight(torch.randn(48, 40).cuda())
   x, r = torch.randn(9, 7, 48).cuda().bfloat16(), torch.randn(9, 7, 40).cuda().bfloat16()
