@@ -148,6 +148,13 @@ void launch_rows(const void* x, long long stride, unsigned rows, int k, int ld, 
   count_launches(1);
 }
 
+// 32 bytes at a multiple of 32
+__device__ __forceinline__ void store_sector(void* to, const uint4& lo, const uint4& hi) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(to), "r"(lo.x), "r"(lo.y), "r"(lo.z), "r"(lo.w),
+               "r"(hi.x), "r"(hi.y), "r"(hi.z), "r"(hi.w)
+               : "memory");
+}
+
 // ---------------------------------------------------------------------------
 // The product
 // ---------------------------------------------------------------------------
@@ -159,7 +166,7 @@ struct Linear8 {
   long long ld_res;
   int M, N, K;            // K: channels, filled up to whole 16
   int tiles_m, tiles_n;
-  int vec;                // whole 16 bytes of y and of the residual may be accessed
+  int vec;                // whole 16 bytes of y and of the residual may be accessed; 2: whole 32 bytes of y
   int* status;
 };
 struct Linear8Maps {
@@ -313,38 +320,73 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       for (int cb = 0; cb < kTileCols / 64; ++cb) {
         const int col = part * (kTileCols / 2) + cb * 32, n0 = nt * kTileCols + col;
         if (n0 >= p.N || m0 >= p.M) break;
-        const float sw = n0 + lane < p.N ? p.w_absmax[n0 + lane] * (1.f / 127.f) : 0.f;
+        const long long row = m0 + lane;
         uint32_t r[32];
+        if (p.vec) {  // a lane stores its row's 32 channels, whole sectors
+          constexpr int E = 16 / sizeof(T), L = 32 / E;  // values of 16 bytes, 16 bytes of a lane
+          uint4 add[L];
+#pragma unroll
+          for (int i = 0; i < L; ++i) add[i] = make_uint4(0, 0, 0, 0);
+          if (residual != nullptr && row < p.M) {
+            const T* from = residual + row * p.ld_res + n0;
+#pragma unroll
+            for (int i = 0; i < L; ++i)
+              if (n0 + i * E < p.N) add[i] = *reinterpret_cast<const uint4*>(from + i * E);
+          }
+          tmem_ld32(t_row + col, r);
+          tmem_ld_wait();
+          T* to = y + row * p.N + n0;
+#pragma unroll
+          for (int i = 0; i < L; i += 2) {
+            alignas(16) T o[2 * E];
+#pragma unroll
+            for (int j = 0; j < 2 * E; j += 4) {
+              const int n = n0 + i * E + j;
+              float4 sw = make_float4(0.f, 0.f, 0.f, 0.f);  // (one address for all lanes)
+              if (n + 4 <= p.N) sw = make_float4(p.w_absmax[n], p.w_absmax[n + 1], p.w_absmax[n + 2], p.w_absmax[n + 3]);
+              const float ws[4] = {sw.x, sw.y, sw.z, sw.w};
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                float v = static_cast<float>(static_cast<int>(r[i * E + j + e])) * sx * (ws[e] * (1.f / 127.f));
+                if (residual != nullptr) v += to_float(reinterpret_cast<const T*>(add)[i * E + j + e]);
+                o[j + e] = from_float<T>(v);
+              }
+            }
+            const uint4 *lo = reinterpret_cast<const uint4*>(o), *hi = lo + 1;
+            if (row < p.M) {
+              if (p.vec == 2 && n0 + (i + 2) * E <= p.N) store_sector(to + i * E, *lo, *hi);
+              else {
+                if (n0 + i * E < p.N) *reinterpret_cast<uint4*>(to + i * E) = *lo;
+                if (n0 + (i + 1) * E < p.N) *reinterpret_cast<uint4*>(to + (i + 1) * E) = *hi;
+              }
+            }
+          }
+          continue;
+        }
+        // rows at any address: by patches of 32 x 32, a lane a channel
+        const int rows = min(32, p.M - m0);
+        const bool mine = n0 + lane < p.N;
+        const float sw = mine ? p.w_absmax[n0 + lane] * (1.f / 127.f) : 0.f;
+        T add[32];
+        if (residual != nullptr && mine) {
+#pragma unroll
+          for (int i = 0; i < 32; ++i)
+            if (i < rows) add[i] = residual[(m0 + i) * p.ld_res + n0 + lane];
+        }
         tmem_ld32(t_row + col, r);
         tmem_ld_wait();
         __syncwarp();  // the patch's last readers are done
 #pragma unroll
         for (int j = 0; j < 32; ++j)
-          patch[lane * 33 + j] = static_cast<float>(static_cast<int>(r[j])) * sx * __shfl_sync(0xffffffffu, sw, j);
+          patch[lane * 33 + j] = static_cast<float>(static_cast<int>(r[j])) * sx;
         __syncwarp();
-        const int rows = min(32, p.M - m0);
-        if (p.vec && n0 + 32 <= p.N) {
-          constexpr int E = 16 / sizeof(T), L = 32 / E;  // values a lane stores at a time, lanes a row
-          const int j = lane % L * E;
-          for (int i = lane / L; i < rows; i += 32 / L) {
-            float v[E];
+        if (mine) {
+          T* to = y + static_cast<long long>(m0) * p.N + n0 + lane;
 #pragma unroll
-            for (int e = 0; e < E; ++e) v[e] = patch[i * 33 + j + e];
-            alignas(16) T o[E];
-            if (residual != nullptr) {
-              *reinterpret_cast<uint4*>(o) = *reinterpret_cast<const uint4*>(residual + (m0 + i) * p.ld_res + n0 + j);
-#pragma unroll
-              for (int e = 0; e < E; ++e) v[e] += to_float(o[e]);
-            }
-#pragma unroll
-            for (int e = 0; e < E; ++e) o[e] = from_float<T>(v[e]);
-            *reinterpret_cast<uint4*>(y + static_cast<long long>(m0 + i) * p.N + n0 + j) = *reinterpret_cast<uint4*>(o);
-          }
-        } else if (n0 + lane < p.N) {
-          for (int i = 0; i < rows; ++i) {
-            float v = patch[i * 33 + lane];
-            if (residual != nullptr) v += to_float(residual[(m0 + i) * p.ld_res + n0 + lane]);
-            y[static_cast<long long>(m0 + i) * p.N + n0 + lane] = from_float<T>(v);
+          for (int i = 0; i < 32; ++i) {
+            float v = patch[i * 33 + lane] * sw;
+            if (residual != nullptr) v += to_float(add[i]);
+            if (i < rows) to[static_cast<long long>(i) * p.N] = from_float<T>(v);
           }
         }
       }
@@ -872,6 +914,7 @@ T5X_API int t5x_linear8(const void* x, int type, int rows, int k, long long stri
   p.y = y;
   p.vec = n * static_cast<long long>(size) % 16 == 0 && t5x::aligned_to(16, {y, residual}) &&
           (residual == nullptr || ld_res * size % 16 == 0);
+  if (p.vec && n * static_cast<long long>(size) % 32 == 0 && t5x::aligned_to(32, {y})) p.vec = 2;
   p.status = t5x::device_status_buffer();
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   switch (type) {
