@@ -148,6 +148,11 @@ void launch_rows(const void* x, long long stride, unsigned rows, int k, int ld, 
   count_launches(1);
 }
 
+// Signals a barrier of the cluster that tensor memory has been read. (Relaxed: it is the fence of tcgen05 in front that orders the
+// reads, and a release would wait for all rows that this thread has stored: 7 of 77 us at 4096 x 64 x 16384.)
+__device__ __forceinline__ void arrive_relaxed(uint32_t bar) {
+  asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
 // 32 bytes at a multiple of 32
 __device__ __forceinline__ void store_sector(void* to, const uint4& lo, const uint4& hi) {
   asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(to), "r"(lo.x), "r"(lo.y), "r"(lo.z), "r"(lo.w),
@@ -310,6 +315,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       tile_at(p, tile, mt, nt);
       const int m0 = mt * kTileRows + static_cast<int>(cta) * kRows + q * 32;
       const float sx = m0 + lane < p.M ? p.x_absmax[m0 + lane] * (1.f / 127.f) : 0.f;
+      const long long row = m0 + lane;
+      const int col0 = part * (kTileCols / 2), first = nt * kTileCols + col0;
+      if (p.vec == 2) {  // the channels' scales, in the patch
+        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int n = first + i * 32 + lane;
+          patch[i * 32 + lane] = n < p.N ? p.w_absmax[n] * (1.f / 127.f) : 0.f;
+        }
+        __syncwarp();
+      }
       if (!mbar_wait(&tmem_full[acc], (local >> 1) & 1, abort_flag)) {
         if (lane == 0) report_status(p.status, kStatusTimeoutEpilogue, kKernelIdLinear8, tile, 0);
         *abort_flag = 1;
@@ -317,23 +333,23 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       }
       tc_fence_after();
       const uint32_t t_row = tmem + (static_cast<uint32_t>(q * 32) << 16) + acc * kTileCols;
-      for (int cb = 0; cb < kTileCols / 64; ++cb) {
-        const int col = part * (kTileCols / 2) + cb * 32, n0 = nt * kTileCols + col;
-        if (n0 >= p.N || m0 >= p.M) break;
-        const long long row = m0 + lane;
-        uint32_t r[32];
-        if (p.vec) {  // a lane stores its row's 32 channels, whole sectors
-          constexpr int E = 16 / sizeof(T), L = 32 / E;  // values of 16 bytes, 16 bytes of a lane
+      // A lane stores its row's channels where they are whole sectors. (4096 x 64 outputs of 16384 / 4096 x 57 of 16004, whole 16 bytes
+      // alone, 32 bits: 101 us so, 114 by patches / 176 and 130.)
+      if (p.vec == 2) {
+        constexpr int E = 16 / sizeof(T), W = sizeof(T) == 4 ? 32 : 64, L = W / E;  // values of 16 bytes, channels at a time, 16 bytes of a lane
+#pragma unroll 1
+        for (int c = 0; c < kTileCols / 2; c += W) {
+          const int n0 = first + c;
+          if (n0 >= p.N || m0 >= p.M) break;
           uint4 add[L];
-#pragma unroll
-          for (int i = 0; i < L; ++i) add[i] = make_uint4(0, 0, 0, 0);
-          if (residual != nullptr && row < p.M) {
-            const T* from = residual + row * p.ld_res + n0;
+          if (residual != nullptr) {
 #pragma unroll
             for (int i = 0; i < L; ++i)
-              if (n0 + i * E < p.N) add[i] = *reinterpret_cast<const uint4*>(from + i * E);
+              if (row < p.M && n0 + i * E < p.N) add[i] = *reinterpret_cast<const uint4*>(residual + row * p.ld_res + n0 + i * E);
           }
-          tmem_ld32(t_row + col, r);
+          uint32_t r[W / 32][32];
+          tmem_ld32(t_row + col0 + c, r[0]);
+          if (W == 64) tmem_ld32(t_row + col0 + c + 32, r[W / 32 - 1]);
           tmem_ld_wait();
           T* to = y + row * p.N + n0;
 #pragma unroll
@@ -341,28 +357,25 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             alignas(16) T o[2 * E];
 #pragma unroll
             for (int j = 0; j < 2 * E; j += 4) {
-              const int n = n0 + i * E + j;
-              float4 sw = make_float4(0.f, 0.f, 0.f, 0.f);  // (one address for all lanes)
-              if (n + 4 <= p.N) sw = make_float4(p.w_absmax[n], p.w_absmax[n + 1], p.w_absmax[n + 2], p.w_absmax[n + 3]);
+              const int at = i * E + j;
+              const float4 sw = *reinterpret_cast<const float4*>(patch + c + at);
               const float ws[4] = {sw.x, sw.y, sw.z, sw.w};
 #pragma unroll
               for (int e = 0; e < 4; ++e) {
-                float v = static_cast<float>(static_cast<int>(r[i * E + j + e])) * sx * (ws[e] * (1.f / 127.f));
-                if (residual != nullptr) v += to_float(reinterpret_cast<const T*>(add)[i * E + j + e]);
+                float v = static_cast<float>(static_cast<int>(r[(at + e) / 32][(at + e) % 32])) * sx * ws[e];
+                if (residual != nullptr) v += to_float(reinterpret_cast<const T*>(add)[at + e]);
                 o[j + e] = from_float<T>(v);
               }
             }
             const uint4 *lo = reinterpret_cast<const uint4*>(o), *hi = lo + 1;
-            if (row < p.M) {
-              if (p.vec == 2 && n0 + (i + 2) * E <= p.N) store_sector(to + i * E, *lo, *hi);
-              else {
-                if (n0 + i * E < p.N) *reinterpret_cast<uint4*>(to + i * E) = *lo;
-                if (n0 + (i + 1) * E < p.N) *reinterpret_cast<uint4*>(to + (i + 1) * E) = *hi;
-              }
-            }
+            if (row < p.M && n0 + i * E < p.N) store_sector(to + i * E, *lo, *hi);
           }
-          continue;
         }
+      }
+      for (int cb = 0; cb < kTileCols / 64 && p.vec != 2; ++cb) {
+        const int col = col0 + cb * 32, n0 = nt * kTileCols + col;
+        if (n0 >= p.N || m0 >= p.M) break;
+        uint32_t r[32];
         // rows at any address: by patches of 32 x 32, a lane a channel
         const int rows = min(32, p.M - m0);
         const bool mine = n0 + lane < p.N;
@@ -392,7 +405,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       }
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive_cluster(drained + acc * 8);
+      if (lane == 0) arrive_relaxed(drained + acc * 8);
     }
   }
 
