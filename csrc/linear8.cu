@@ -317,13 +317,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       const float sx = m0 + lane < p.M ? p.x_absmax[m0 + lane] * (1.f / 127.f) : 0.f;
       const long long row = m0 + lane;
       const int col0 = part * (kTileCols / 2), first = nt * kTileCols + col0;
-      if (p.vec == 2) {  // the channels' scales, in the patch
+      constexpr int kBlocks = kTileCols / 64;  // of 32 channels
+      float sw[kBlocks];  // the channels' scales
+#pragma unroll
+      for (int i = 0; i < kBlocks; ++i) {
+        const int n = first + i * 32 + lane;
+        sw[i] = n < p.N ? p.w_absmax[n] * (1.f / 127.f) : 0.f;
+      }
+      if (p.vec == 2) {  // in the patch
         __syncwarp();
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int n = first + i * 32 + lane;
-          patch[i * 32 + lane] = n < p.N ? p.w_absmax[n] * (1.f / 127.f) : 0.f;
-        }
+        for (int i = 0; i < kBlocks; ++i) patch[i * 32 + lane] = sw[i];
         __syncwarp();
       }
       if (!mbar_wait(&tmem_full[acc], (local >> 1) & 1, abort_flag)) {
@@ -372,34 +376,37 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           }
         }
       }
-      for (int cb = 0; cb < kTileCols / 64 && p.vec != 2; ++cb) {
-        const int col = col0 + cb * 32, n0 = nt * kTileCols + col;
-        if (n0 >= p.N || m0 >= p.M) break;
-        uint32_t r[32];
-        // rows at any address: by patches of 32 x 32, a lane a channel
+      // Rows at any address: by patches of 32 x 32, a lane a channel. The next sums are requested before these are stored.
+      if (p.vec != 2 && first < p.N && m0 < p.M) {
         const int rows = min(32, p.M - m0);
-        const bool mine = n0 + lane < p.N;
-        const float sw = mine ? p.w_absmax[n0 + lane] * (1.f / 127.f) : 0.f;
-        T add[32];
-        if (residual != nullptr && mine) {
+        uint32_t r[32];
+        tmem_ld32(t_row + col0, r);
 #pragma unroll
-          for (int i = 0; i < 32; ++i)
-            if (i < rows) add[i] = residual[(m0 + i) * p.ld_res + n0 + lane];
-        }
-        tmem_ld32(t_row + col, r);
-        tmem_ld_wait();
-        __syncwarp();  // the patch's last readers are done
+        for (int cb = 0; cb < kBlocks; ++cb) {
+          const int n0 = first + cb * 32;
+          if (n0 >= p.N) break;
+          const bool mine = n0 + lane < p.N;
+          T add[32];
+          if (residual != nullptr && mine) {
 #pragma unroll
-        for (int j = 0; j < 32; ++j)
-          patch[lane * 33 + j] = static_cast<float>(static_cast<int>(r[j])) * sx;
-        __syncwarp();
-        if (mine) {
-          T* to = y + static_cast<long long>(m0) * p.N + n0 + lane;
+            for (int i = 0; i < 32; ++i)
+              if (i < rows) add[i] = residual[(m0 + i) * p.ld_res + n0 + lane];
+          }
+          tmem_ld_wait();
+          __syncwarp();  // the patch's last readers are done
 #pragma unroll
-          for (int i = 0; i < 32; ++i) {
-            float v = patch[i * 33 + lane] * sw;
-            if (residual != nullptr) v += to_float(add[i]);
-            if (i < rows) to[static_cast<long long>(i) * p.N] = from_float<T>(v);
+          for (int j = 0; j < 32; ++j) patch[lane * 33 + j] = static_cast<float>(static_cast<int>(r[j])) * sx;
+          __syncwarp();
+          if (cb + 1 < kBlocks && n0 + 32 < p.N) tmem_ld32(t_row + col0 + (cb + 1) * 32, r);
+          if (mine) {
+            T* to = y + static_cast<long long>(m0) * p.N + n0 + lane;
+#pragma unroll
+            for (int i = 0; i < 32; ++i) {
+              float v = patch[i * 33 + lane] * sw[cb];
+              if (residual != nullptr) v += to_float(add[i]);
+              if (i < rows) *to = from_float<T>(v);
+              to += p.N;
+            }
           }
         }
       }
