@@ -5,8 +5,9 @@
 // Two launches, for more than two rows: the rows are turned into codes, and tcgen05 (kind::i8, sums in 32 bits in tensor memory)
 // multiplies them.
 // It runs at twice the rate of bf16, so that a large product has half the time of `native.gemm`; over few rows both are
-// bound by the weights' bytes, which are half of bf16's. 8192 x 10240 x 4096: 274 us, 42 for the codes and 226 for the product
-// (3.04 POP/s; the tensor pipe is 88 % busy), 210 at twice the measured rate of bf16.
+// bound by the weights' bytes, which are half of bf16's. 8192 x 10240 x 4096: 268 us, 42 for the codes and some 220 for the product
+// (3.1 POP/s; the tensor pipe is 88 % busy), 210 at twice the measured rate of bf16. 4096 x 64 x 16384: 57 us, 134 MB of outputs at
+// 2.5 TB/s; 16001 outputs 100: what a warp does for a tile is a chain of trips to memory.
 #include <algorithm>
 
 #include "cache8.cuh"
@@ -337,8 +338,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       }
       tc_fence_after();
       const uint32_t t_row = tmem + (static_cast<uint32_t>(q * 32) << 16) + acc * kTileCols;
-      // A lane stores its row's channels where they are whole sectors. (4096 x 64 outputs of 16384 / 4096 x 57 of 16004, whole 16 bytes
-      // alone, 32 bits: 101 us so, 114 by patches / 176 and 130.)
+      // A lane stores its row's channels where they are whole sectors. (In 32 bits, 4096 x 64 x 16384: 101 us so, 114 by patches; 4096 x
+      // 57 x 16004, whole 16 bytes alone: 176 and 130.)
       if (p.vec == 2) {
         constexpr int E = 16 / sizeof(T), W = sizeof(T) == 4 ? 32 : 64, L = W / E;  // values of 16 bytes, channels at a time, 16 bytes of a lane
 #pragma unroll 1
