@@ -498,6 +498,8 @@ __global__ void __launch_bounds__(kWarps * 32, 16 / kWarps)
             x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
             x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
             x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
+            // (only what this row sees raises its own: a result does not hang on what is hidden, nor on other rows)
+            if (!(x - ref[nt][e] > kLimit || v > v_lim[nt][e])) continue;
             const float up = fmaxf(x - kPeak, ref[nt][e]);
             const float f = exp2_approx(ref[nt][e] - up);
             v_inv[nt][e] = v > 0.f ? __frcp_rn(v) : 0.f;

@@ -394,6 +394,8 @@ __global__ void __launch_bounds__(kThreads, 1) cache8_rows_kernel(const __grid_c
               }
               x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
               x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
+              // (only what this row sees raises its own: a result does not hang on what is hidden, nor on other rows)
+              if (!(x - ref[m][e] > kLimit || v > v_lim[m][e])) continue;
               const float up = fmaxf(x - kPeak, ref[m][e]);
               const float f = exp2_approx(ref[m][e] - up);
               v_inv[m][e] = v > 0.f ? __frcp_rn(v) : 0.f;

@@ -263,6 +263,19 @@ def test_linear8_rows_that_are_not_finite():
   assert y[1].isnan().all() and y[3].isnan().all() and torch.equal(y[::2], want[::2])
 
 
+@pytest.mark.parametrize("rows", [1, 2])
+@pytest.mark.parametrize("bad", [math.inf, -math.inf, math.nan])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_linear8_of_a_row_that_is_not_finite(rows, bad, dtype):
+  weight = F.quantize_weight(torch.randn(300, 40).cuda())
+  x = torch.randn(rows, 300).cuda().to(dtype)
+  want = F.linear8(x, weight)
+  x[0, 299] = bad
+  y = F.linear8(x, weight)
+  assert want.isfinite().all() and y[0].isnan().all() and torch.equal(y[1:], want[1:])
+  assert (F.linear8(torch.zeros_like(x), weight) == 0).all()
+
+
 def test_another_stream_and_two_captures():
   """Two graphs of the same cache's steps, replayed in turn, and a call on another stream."""
   c = dict(b=2, h=2, group=1, dim=64, slots=640, block=32, starts=[300, 500], count=1, weights=True, bias=True)
@@ -396,6 +409,50 @@ def test_many_rows(c, dtype):
 def test_pieces(c, dtype):
   """Caches that are cut into pieces: rows that hold nothing, a token, all; a piece's border inside a row."""
   launches(lambda: plain.check_attention(c, "cuda", dtype))
+
+
+@pytest.mark.parametrize("bad", [math.inf, -math.inf, math.nan])
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("dim,count", [(64, 30), (128, 150)])
+def test_many_rows_and_values_that_are_not_finite(bad, dtype, dim, count):
+  """The last token's block is not finite: the queries before it do not see it, and a mask hides it from all."""
+  c = dict(b=1, h=1, group=2, dim=dim, slots=304, block=16, starts=[0], count=count)
+  cache, query, key, value, _ = plain.inputs(c, "cuda", dtype)
+  cache["cache_index"].fill_(289 - count)  # (the last one begins a block)
+  hide = torch.ones(1, 304, dtype=torch.bool, device="cuda")
+  hide[0, 288:] = False
+  fresh = lambda: {n: t.clone() for n, t in cache.items()}  # noqa: E731
+  masked, plainly = cache8.attention(query, fresh(), key, value, key_mask=hide), cache8.attention(query, fresh(), key, value)
+  assert masked.isfinite().all() and plainly.isfinite().all()
+  for which in (key, value):
+    which[0, -1, 0, 3] = bad
+    assert torch.equal(cache8.attention(query, fresh(), key, value, key_mask=hide), masked)
+    out = cache8.attention(query, fresh(), key, value)
+    assert out[:, -1].isnan().all() and torch.equal(out[:, :-1], plainly[:, :-1])
+    which[0, -1, 0, 3] = 1
+
+
+def test_many_rows_and_biases_of_the_lowest_value():
+  c = dict(b=1, h=2, group=1, dim=64, slots=64, block=16, starts=[12], count=20)
+  cache, query, key, value, _ = plain.inputs(c, "cuda", torch.float32)
+  low = torch.full((2, 32), torch.finfo(torch.float32).min, device="cuda")
+  out = cache8.attention(query * 0, cache, key, value, bias_table=low)
+  held = ref.cache8_values(cache, "value", torch.float64)[0]
+  for i in (0, 7, 19):
+    v = held[:, :13 + i].mean(1)
+    assert torch.allclose(out[0, i].double(), v, rtol=0, atol=2.0 ** -20 * held.abs().max().item() * 16)
+  assert (cache8.attention(query, cache, key, value, bias_table=torch.full_like(low, -math.inf)) == 0).all()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_many_rows_of_any_stride(dtype):
+  c = dict(b=2, h=2, group=3, dim=64, slots=128, block=16, starts=[9, 30], count=15)
+  cache, query, _, _, _ = plain.inputs(dict(c, own=True), "cuda", dtype)
+  want = cache8.attention(query, cache)
+  wide = torch.cat([query.flatten(2), torch.zeros(2, 15, 1, device="cuda", dtype=dtype)], 2)
+  for q in (wide[..., :384].unflatten(2, (6, 64)), query.permute(0, 2, 1, 3).contiguous().permute(0, 2, 1, 3),
+            torch.cat([query.flatten(), query.flatten()[:1]])[1:].roll(1).view_as(query)):
+    assert torch.equal(cache8.attention(q, cache), want)
 
 
 def check_some_rows(c, rows, dtype=torch.bfloat16):
