@@ -526,7 +526,8 @@ __global__ void __launch_bounds__(kWarps * 32, 16 / kWarps)
             l[nt][k & 1] += pr[k];
             pr[k] *= r[k & 1];
           }
-          if (!(va[ms] < INFINITY)) {  // a block that is not finite: what is hidden counts for nothing all the same
+          // a block that is not finite, or far larger than what is seen: what is hidden counts for nothing all the same
+          if (!(fmaxf(r[0], r[1]) < INFINITY)) {
 #pragma unroll
             for (int k = 0; k < 4; ++k)
               if (s[ms][nt][k] == -INFINITY) pr[k] = 0.f;

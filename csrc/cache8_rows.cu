@@ -412,10 +412,11 @@ __global__ void __launch_bounds__(kThreads, 1) cache8_rows_kernel(const __grid_c
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt) {
           uint4 pf[M][Q2];
-          const bool odd = !(va[mt] < INFINITY);  // a block that is not finite: what is hidden counts for nothing all the same
 #pragma unroll
           for (int m = 0; m < M; ++m) {
             const float r[2] = {va[mt] * v_inv[m][0], va[mt] * v_inv[m][1]};
+            // a block that is not finite, or far larger than what is seen: what is hidden counts for nothing all the same
+            const bool odd = !(fmaxf(r[0], r[1]) < INFINITY);
             uint32_t f[Q2][4];
 #pragma unroll
             for (int n = 0; n < 2; ++n)

@@ -432,6 +432,21 @@ def test_many_rows_and_values_that_are_not_finite(bad, dtype, dim, count):
     which[0, -1, 0, 3] = 1
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("dim,count,slots", [(64, 1, 64), (128, 2, 2112), (64, 40, 64), (128, 200, 256)])
+def test_a_hidden_block_of_the_largest_values(dtype, dim, count, slots):
+  """Values of 3e38 that a mask hides beside seen ones of 1e-3: their ratio is no number in 32 bits."""
+  c = dict(b=1, h=1, group=2, dim=dim, slots=slots, block=16, starts=[64], count=count, own=True)
+  cache, query, _, _, _ = plain.inputs(c, "cuda", dtype)
+  hide = torch.ones(1, slots, dtype=torch.bool, device="cuda")
+  hide[0, 16:32] = False
+  cache["value_absmax"].fill_(1e-3)
+  want = cache8.attention(query, cache, key_mask=hide, causal=False)
+  cache["value_absmax"][0, 0, 1] = cache["key_absmax"][0, 0, 1] = 3e38
+  assert want.isfinite().all() and (want != 0).any()
+  assert torch.equal(cache8.attention(query, cache, key_mask=hide, causal=False), want)
+
+
 def test_many_rows_and_biases_of_the_lowest_value():
   c = dict(b=1, h=2, group=1, dim=64, slots=64, block=16, starts=[12], count=20)
   cache, query, key, value, _ = plain.inputs(c, "cuda", torch.float32)
