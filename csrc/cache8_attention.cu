@@ -36,8 +36,8 @@
 //
 // Measured, us on the device of a call with its append: 64 rows x 32 heads of 64 channels, up to 1024 slots of all lengths,
 // with biases, positions and weights, 59 (2.5 TB/s; 35 % of the issue slots: a CTA has four steps of tiles, and waits for
-// memory before and behind them as long); 8 rows x 8 heads of 128 channels, 8 queries each, up to 65536 slots of all lengths, 93
-// (4.8 TB/s; full rows run at 89 % of the copy rate, the arithmetic on codes takes 80 to 85 % of its pipe); 12 heads over 640
+// memory before and behind them as long); 8 rows x 8 heads of 128 channels, 8 queries each, up to 65536 slots of all lengths, 95
+// (4.7 TB/s; full rows run at 89 % of the copy rate, the arithmetic on codes takes 80 to 85 % of its pipe); 12 heads over 640
 // slots 8.4, all of it latency.
 #include <algorithm>
 #include <type_traits>
