@@ -420,13 +420,11 @@ __global__ void __launch_bounds__(kWarps * 32, 16 / kWarps)
       if (tile + kStep < tile1) load_k(tile + kStep);
 
       // ---- scores of tokens g (k = 0, 1) and g + 8 (k = 2, 3), columns 2t (k = 0, 2) and 2t + 1 ----
-      bool some[MS];       // whether the mask shows a token of the tile
       bool raise = false;  // whether a reference has to go up
 #pragma unroll
       for (int ms = 0; ms < MS; ++ms) {
         const int s0 = (tile + ms + fold) << 4;
         const bool inside = tile + ms + fold < tile1;
-        some[ms] = inside;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
@@ -452,8 +450,6 @@ __global__ void __launch_bounds__(kWarps * 32, 16 / kWarps)
           if (mask != nullptr) {
 #pragma unroll
             for (int e = 0; e < 2; ++e) shown[e] = inside && s0 + g + 8 * e < p.mask_len && mask[s0 + g + 8 * e] != 0;
-            const uint32_t which = __ballot_sync(0xffffffffu, shown[0] || shown[1]);
-            some[ms] = (which & (!kFold ? 0xffffffffu : fold ? 0xccccccccu : 0x33333333u)) != 0;
           }
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt)
@@ -492,12 +488,13 @@ __global__ void __launch_bounds__(kWarps * 32, 16 / kWarps)
             float x = -INFINITY, v = 0.25f * v_lim[nt][e];
 #pragma unroll
             for (int ms = 0; ms < MS; ++ms) {
-              x = fmaxf(x, fmaxf(s[ms][nt][e], s[ms][nt][2 + e]));
-              if (some[ms] && column(nt, e).lim >= (tile + ms + fold) << 4 && va[ms] < INFINITY) v = fmaxf(v, va[ms]);
+              float high = fmaxf(s[ms][nt][e], s[ms][nt][2 + e]);
+              high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, 4));
+              high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, 8));
+              high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, 16));
+              x = fmaxf(x, high);
+              if (high > -INFINITY && va[ms] < INFINITY) v = fmaxf(v, va[ms]);  // (the row sees a token of the tile)
             }
-            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
-            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
-            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
             // (only what this row sees raises its own: a result does not hang on what is hidden, nor on other rows)
             if (!(x - ref[nt][e] > kLimit || v > v_lim[nt][e])) continue;
             const float up = fmaxf(x - kPeak, ref[nt][e]);

@@ -308,7 +308,6 @@ __global__ void __launch_bounds__(kThreads, 1) cache8_rows_kernel(const __grid_c
         }
 
         // ---- scores of tokens 2t + {0, 1} and 8 more, rows g (k = 0, 1) and g + 8 (k = 2, 3) ----
-        bool some[MT];       // whether the mask shows a token of the tile
         bool raise = false;  // whether a reference has to go up
         float va[MT];
 #pragma unroll
@@ -317,7 +316,6 @@ __global__ void __launch_bounds__(kThreads, 1) cache8_rows_kernel(const __grid_c
           const bool inside = tl < tile1;
           const float ka = s_scale[buffer * 2 * kTiles + min(part + mt, kTiles - 1)];
           va[mt] = s_scale[buffer * 2 * kTiles + kTiles + min(part + mt, kTiles - 1)];
-          some[mt] = inside;
 #pragma unroll
           for (int m = 0; m < M; ++m)
 #pragma unroll
@@ -340,16 +338,13 @@ __global__ void __launch_bounds__(kThreads, 1) cache8_rows_kernel(const __grid_c
           if (!(inside && tl * 16 + 15 <= all_see && mask == nullptr)) {
             bool shown[2][2] = {{inside, inside}, {inside, inside}};
             if (mask != nullptr) {
-              bool any = false;
 #pragma unroll
               for (int n = 0; n < 2; ++n)
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
                   const int slot = s0 + 8 * n + e;
                   shown[n][e] = inside && slot < p.mask_len && mask[slot] != 0;
-                  any |= shown[n][e];
                 }
-              some[mt] = __any_sync(0xffffffffu, any);
             }
 #pragma unroll
             for (int m = 0; m < M; ++m)
@@ -389,11 +384,12 @@ __global__ void __launch_bounds__(kThreads, 1) cache8_rows_kernel(const __grid_c
               float x = -INFINITY, v = 0.25f * v_lim[m][e];
 #pragma unroll
               for (int mt = 0; mt < MT; ++mt) {
-                x = fmaxf(x, fmaxf(fmaxf(s[mt][m][0][2 * e], s[mt][m][0][2 * e + 1]), fmaxf(s[mt][m][1][2 * e], s[mt][m][1][2 * e + 1])));
-                if (some[mt] && row[m][e].lim >= (tile + part + mt) << 4 && va[mt] < INFINITY) v = fmaxf(v, va[mt]);
+                float high = fmaxf(fmaxf(s[mt][m][0][2 * e], s[mt][m][0][2 * e + 1]), fmaxf(s[mt][m][1][2 * e], s[mt][m][1][2 * e + 1]));
+                high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, 1));
+                high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, 2));
+                x = fmaxf(x, high);
+                if (high > -INFINITY && va[mt] < INFINITY) v = fmaxf(v, va[mt]);  // (the row sees a token of the tile)
               }
-              x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
-              x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
               // (only what this row sees raises its own: a result does not hang on what is hidden, nor on other rows)
               if (!(x - ref[m][e] > kLimit || v > v_lim[m][e])) continue;
               const float up = fmaxf(x - kPeak, ref[m][e]);
