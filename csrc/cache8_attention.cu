@@ -15,10 +15,9 @@
 //     tile i takes channels 2 i and 2 i + 1 of each lane as its rows g and g + 8. So a lane ends up with adjacent channels.
 //   * The probabilities, tokens by query rows in the first product's result, turn into the second one's operand by
 //     movmatrix.
-//   * A key byte u = code + 128 alone is the fp16 number u 2^-24 (below the normal ones, which the tensor cores take as
-//     they are); 128 times the sum of the query is subtracted from the score. Value bytes stand under the exponent of
-//     1024, and 1152 is subtracted from each: their sums run over the whole cache, and an offset of all would leave
-//     nothing of a mean near zero. (Keys too where queries have 32 bits.)
+//   * Bytes stand under the exponent of 1024, and 1152 is subtracted from each, which leaves the code itself. (Keys as code + 128,
+//     with 128 times the query's sum taken off the score, were an instruction a pair less and no faster, 95 us for the long
+//     contexts below against 93, and what the two sums had lost stayed in the score, times the scale of its block.)
 //
 // Queries are scaled by a power of two to just below 2^14, where fp16 holds the values of 16-bit types down to 2^-28 of
 // the row's largest without loss; values of 32 bits go in as two fp16 numbers each (22 bits). The reference m is raised
@@ -84,7 +83,6 @@ __device__ __forceinline__ void lay_query(const Cache8Attn& p, int b, int h, int
     int up = most == 0 || most >= 0x7f800000u ? 0 : 13 - (static_cast<int>(most >> 23) - 127);
     up = max(min(up, 126), -113);
     const float by = __uint_as_float(static_cast<uint32_t>(up + 127) << 23);
-    float sum = 0.f;
 #pragma unroll
     for (int ch = 0; ch < CH; ++ch)
 #pragma unroll
@@ -95,23 +93,15 @@ __device__ __forceinline__ void lay_query(const Cache8Attn& p, int b, int h, int
           const float lo = x[ch][4 * j + k] * by, hi = x[ch][4 * j + 2 + k] * by;
           const __half2 v = __floats2half2_rn(lo, hi);
           f[0][k] = as_u32(v);
-          sum += __low2float(v) + __high2float(v);
-          if (kTwo) {
-            const __half2 rest = __floats2half2_rn(lo - __low2float(v), hi - __high2float(v));
-            f[Q2 - 1][k] = as_u32(rest);
-            sum += __low2float(rest) + __high2float(rest);
-          }
+          if (kTwo) f[Q2 - 1][k] = as_u32(__floats2half2_rn(lo - __low2float(v), hi - __high2float(v)));
         }
 #pragma unroll
         for (int w = 0; w < Q2; ++w) s_query[(w * CH * 4 + ch * 4 + j) * 32 + lane] = make_uint2(f[w][0], f[w][1]);
       }
-    sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-    sum += __shfl_xor_sync(0xffffffffu, sum, 2);
     if (t == 0) {
       Column col;
-      // 2^24 back from the keys' exponent; the scale of a key block is its largest value / 127; scores are times log2 e
-      col.scale = __uint_as_float(static_cast<uint32_t>(127 - up) << 23) * p.scale * ((kTwo ? 1.f : 0x1p24f) / 127.f * kLog2e);
-      col.sum = kTwo ? 0.f : sum * 0x1p-17f;  // 128 times, at the keys' exponent
+      // the scale of a key block is its largest value / 127; scores are times log2 e
+      col.scale = __uint_as_float(static_cast<uint32_t>(127 - up) << 23) * p.scale * (kLog2e / 127.f);
       col.lim = r < p.rows ? last_seen(p, start, end, r) : 0x7fffffff;  // (a column without a row hinders nobody)
       col.where = q_first + i + dropped;
       col.bias = first_bias + in_group * p.table_stride;
@@ -389,8 +379,8 @@ __global__ void __launch_bounds__(kWarps * 32, 16 / kWarps)
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
               const uint32_t w = j == 0 ? kr[mt][e][ch].x : j == 1 ? kr[mt][e][ch].y : j == 2 ? kr[mt][e][ch].z : kr[mt][e][ch].w;
-              a[mt][e] = kTwo ? value_pair(w, low) : key_pair(w, low);
-              a[mt][2 + e] = kTwo ? value_pair(w >> 8, low) : key_pair(w >> 8, low);
+              a[mt][e] = number_pair(w, low);
+              a[mt][2 + e] = number_pair(w >> 8, low);
             }
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
@@ -429,9 +419,9 @@ __global__ void __launch_bounds__(kWarps * 32, 16 / kWarps)
         for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            const float sum = column(nt, e).sum, by = k_scale[ms] * column(nt, e).scale;
-            s[ms][nt][e] = (s[ms][nt][e] - sum) * by;
-            s[ms][nt][2 + e] = (s[ms][nt][2 + e] - sum) * by;
+            const float by = k_scale[ms] * column(nt, e).scale;
+            s[ms][nt][e] *= by;
+            s[ms][nt][2 + e] *= by;
           }
         }
         if (p.table != nullptr) {
@@ -555,7 +545,7 @@ __global__ void __launch_bounds__(kWarps * 32, 16 / kWarps)
           for (int half = 0; half < 2; ++half) {
             const uint32_t x = __byte_perm(vr[mt][0][w], vr[mt][1][w], half ? 0x7632 : 0x5410);
             const uint32_t y = __byte_perm(vr[mt][2][w], vr[mt][3][w], half ? 0x7632 : 0x5410);
-            const uint32_t a[4] = {value_pair(x, low), value_pair(x >> 8, low), value_pair(y, low), value_pair(y >> 8, low)};
+            const uint32_t a[4] = {number_pair(x, low), number_pair(x >> 8, low), number_pair(y, low), number_pair(y >> 8, low)};
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
               uint32_t p0[Q2], p1[Q2];

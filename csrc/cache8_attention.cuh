@@ -91,10 +91,8 @@ __device__ __forceinline__ uint32_t low_flipped(uint32_t w, uint32_t low) {
   asm("lop3.b32 %0, %1, %2, %3, 0x6a;" : "=r"(r) : "r"(w), "r"(low), "n"(kFlip));
   return r;
 }
-// bytes 0 and 2 of codes as two numbers (code + 128) 2^-24
-__device__ __forceinline__ uint32_t key_pair(uint32_t w, uint32_t low) { return low_flipped<0x00800080u>(w, low); }
 // bytes 0 and 2 of codes as two numbers
-__device__ __forceinline__ uint32_t value_pair(uint32_t w, uint32_t low) {
+__device__ __forceinline__ uint32_t number_pair(uint32_t w, uint32_t low) {
   return as_u32(__hsub2(as_half2(low_flipped<0x64806480u>(w, low)), as_half2(0x64806480u)));
 }
 __device__ __forceinline__ float exp2_approx(float x) {
@@ -156,7 +154,7 @@ __device__ __forceinline__ void count_tiles(const Cache8Attn& p, long long* s_fi
 
 // What a score column needs beside its reference and sums.
 struct Column {
-  float scale, sum;
+  float scale;
   int lim, where, bias;
 };
 

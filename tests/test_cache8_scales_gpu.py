@@ -1,4 +1,5 @@
-"""Attention over a cache in 8 bits whose blocks have scales far apart, and whose rows see little of a block."""
+"""Attention over a cache in 8 bits whose blocks have scales far apart, and whose rows see little of a block: what is hidden
+changes no bit, a block that is not finite is NaN to all that see it."""
 import math
 
 import pytest
@@ -43,3 +44,26 @@ def test_a_block_of_which_a_row_sees_nothing(dim, group, count, held, slots, dty
     cache["cached_value"][0, 0, 16:32] = 0  # as such a block is held
   got = attend(query, cache, key_mask=shown)[:, :blind]
   assert want.isfinite().all() and (want != 0).any() and torch.equal(got, want)
+
+
+@pytest.mark.parametrize("bad", [math.inf, math.nan])
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("dim,group,count,slots", [(64, 4, 1, 64), (64, 8, 1, 64), (128, 4, 1, 64), (128, 8, 1, 2112), (64, 2, 2, 2112),
+                                                   (64, 20, 1, 64), (128, 50, 4, 64)])
+def test_a_key_block_that_is_not_finite(dim, group, count, slots, dtype, bad):
+  """NaN for each of a thousand queries that see it, nothing to those that a mask hides it from."""
+  rows = -(-1000 // (group * count))
+  gen = torch.Generator("cuda").manual_seed(0)
+  cache = cache8.init_cache(rows, slots, 1, dim, "cuda", block=16)
+  for n in ("key", "value"):
+    cache["cached_" + n].copy_(torch.randint(-127, 128, cache["cached_" + n].shape, generator=gen, device="cuda", dtype=torch.int8))
+    cache[n + "_absmax"].fill_(1.0)
+  cache["cache_index"].fill_(40)
+  query = torch.randn(rows, count, group, dim, generator=gen, device="cuda").to(dtype)
+  shown = torch.ones(rows, slots, dtype=torch.bool, device="cuda")
+  shown[:, 16:32] = False
+  want = attend(query, cache, key_mask=shown)
+  cache["cached_key"][:, :, 16:32] = 0
+  cache["key_absmax"][:, :, 1] = bad
+  assert want.isfinite().all() and torch.equal(attend(query, cache, key_mask=shown), want)
+  assert attend(query, cache).isnan().all()
