@@ -20,12 +20,10 @@
 //     contexts below against 93, and what the two sums had lost stayed in the score, times the scale of its block.)
 //
 // Queries are scaled by a power of two to just below 2^14, where fp16 holds the values of 16-bit types down to 2^-28 of
-// the row's largest without loss; values of 32 bits go in as two fp16 numbers each (22 bits). The reference m is raised
-// only where a probability would come to 2^12.6 (it is 2^4 at the reference): raising it costs a maximum over the lanes
-// and a multiplication of all sums. Probabilities are rounded to 11 bits (a quarter of the rounding of a bf16 result, and
-// random in sign), or are two numbers again. A value block's scale goes into the probability, relative to one that the row
-// has met where it saw something (at most four times as large), so that the accumulators need no scaling by token. Sums are
-// in 32 bits.
+// the row's largest without loss; values of 32 bits go in as two fp16 numbers each (22 bits). A probability goes into the
+// product with its block's largest value, relative to references that are raised seldom (raising costs a maximum over the
+// lanes and a multiplication of all sums; `Reference` has the rule): as one fp16 number, 11 bits (a quarter of the rounding of a bf16
+// result, and random in sign), or as two. Sums are in 32 bits.
 //
 // Two ways to deal out the work. Over short caches, and longer ones where there are many (row, head), a CTA takes one: it
 // appends the new tokens, its warps take tiles of 16 tokens in turn and meet in shared memory, and the scores that the
@@ -345,7 +343,8 @@ __global__ void __launch_bounds__(kWarps * 32, 16 / kWarps)
     all_see = __reduce_min_sync(0xffffffffu, all_see);
 
     float o[NT][MI][4];
-    float ref[NT][2], l[NT][2], v_lim[NT][2], v_inv[NT][2];  // v_lim: four times the scale that a value block's is relative to
+    Reference ref[NT][2];
+    float l[NT][2];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
@@ -353,11 +352,7 @@ __global__ void __launch_bounds__(kWarps * 32, 16 / kWarps)
 #pragma unroll
         for (int k = 0; k < 4; ++k) o[nt][i][k] = 0.f;
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        ref[nt][e] = kNothing;
-        l[nt][e] = v_inv[nt][e] = 0.f;
-        v_lim[nt][e] = (kFold ? (2 * t + e) & 3 : 2 * t + e) < p.rows ? 0.f : INFINITY;  // (without a row: none)
-      }
+      for (int e = 0; e < 2; ++e) ref[nt][e] = {kNothing, 1.f}, l[nt][e] = 0.f;
     }
 
     for (int tile = mine; tile < tile1; tile += kStep) {
@@ -410,7 +405,6 @@ __global__ void __launch_bounds__(kWarps * 32, 16 / kWarps)
       if (tile + kStep < tile1) load_k(tile + kStep);
 
       // ---- scores of tokens g (k = 0, 1) and g + 8 (k = 2, 3), columns 2t (k = 0, 2) and 2t + 1 ----
-      bool raise = false;  // whether a reference has to go up
 #pragma unroll
       for (int ms = 0; ms < MS; ++ms) {
         const int s0 = (tile + ms + fold) << 4;
@@ -460,42 +454,43 @@ __global__ void __launch_bounds__(kWarps * 32, 16 / kWarps)
               }
             }
         }
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            raise |= fmaxf(s[ms][nt][e], s[ms][nt][2 + e]) - ref[nt][e] > kLimit;
-            raise |= va[ms] > v_lim[nt][e];
-          }
       }
 
-      // ---- references ----
+      // ---- references (all tiles of the step in one question: raise_to asks exactly) ----
+      float most = va[0];
+#pragma unroll
+      for (int ms = 1; ms < MS; ++ms) most = fmaxf(most, va[ms]);
+      bool raise = false;
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          float top = -INFINITY;
+#pragma unroll
+          for (int ms = 0; ms < MS; ++ms) top = fmaxf(top, fmaxf(s[ms][nt][e], s[ms][nt][2 + e]));
+          raise |= beyond(ref[nt][e], top, most * ref[nt][e].by);
+        }
       if (__any_sync(0xffffffffu, raise)) {
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            float x = -INFINITY, v = 0.25f * v_lim[nt][e];
+            float x = -INFINITY, x2 = -INFINITY;
 #pragma unroll
             for (int ms = 0; ms < MS; ++ms) {
-              float high = fmaxf(s[ms][nt][e], s[ms][nt][2 + e]);
-              high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, 4));
-              high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, 8));
-              high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, 16));
+              const float high = fmaxf(s[ms][nt][e], s[ms][nt][2 + e]);
               x = fmaxf(x, high);
-              if (high > -INFINITY && va[ms] < INFINITY) v = fmaxf(v, va[ms]);  // (the row sees a token of the tile)
+              x2 = fmaxf(x2, high + log2_approx(va[ms]));
             }
-            // (only what this row sees raises its own: a result does not hang on what is hidden, nor on other rows)
-            if (!(x - ref[nt][e] > kLimit || v > v_lim[nt][e])) continue;
-            const float up = fmaxf(x - kPeak, ref[nt][e]);
-            const float f = exp2_approx(ref[nt][e] - up);
-            v_inv[nt][e] = v > 0.f ? __frcp_rn(v) : 0.f;
-            const float shrink = f * (0.25f * v_lim[nt][e] * v_inv[nt][e]);  // (0 where nothing had been met)
-            ref[nt][e] = up;
-            l[nt][e] *= f;
-            v_lim[nt][e] = 4.f * v;
 #pragma unroll
-            for (int i = 0; i < MI; ++i) o[nt][i][e] *= shrink, o[nt][i][2 + e] *= shrink;
+            for (int lanes = 4; lanes < 32; lanes *= 2) {
+              x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, lanes));
+              x2 = fmaxf(x2, __shfl_xor_sync(0xffffffffu, x2, lanes));
+            }
+            const float2 by = raise_to(ref[nt][e], x, x2);
+            l[nt][e] *= by.x;
+#pragma unroll
+            for (int i = 0; i < MI; ++i) o[nt][i][e] *= by.y, o[nt][i][2 + e] *= by.y;
           }
       }
 
@@ -505,26 +500,34 @@ __global__ void __launch_bounds__(kWarps * 32, 16 / kWarps)
       for (int ms = 0; ms < MS; ++ms)
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-          const float r[2] = {va[ms] * v_inv[nt][0], va[ms] * v_inv[nt][1]};
+          float r[2] = {va[ms] * ref[nt][0].by, va[ms] * ref[nt][1].by};
+          float counts = 1.f;  // in the sum that divides
+          if (!(fmaxf(r[0], r[1]) < kFar)) {
+            counts = 0.f;
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const float2 part = part_of(ref[nt][e], va[ms]);
+              r[e] = part.x;
+#pragma unroll
+              for (int k = e; k < 4; k += 2) {
+                l[nt][e] += exp2_approx(s[ms][nt][k] - ref[nt][e].score);
+                s[ms][nt][k] = far_score(s[ms][nt][k], part.y, va[ms]);
+              }
+            }
+          }
           float pr[4];
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
-            pr[k] = exp2_approx(s[ms][nt][k] - ref[nt][k & 1]);
-            l[nt][k & 1] += pr[k];
+            pr[k] = exp2_approx(s[ms][nt][k] - ref[nt][k & 1].score);
+            l[nt][k & 1] += pr[k] * counts;
             pr[k] *= r[k & 1];
-          }
-          // a block that is not finite, or far larger than what is seen: what is hidden counts for nothing all the same
-          if (!(fmaxf(r[0], r[1]) < INFINITY)) {
-#pragma unroll
-            for (int k = 0; k < 4; ++k)
-              if (s[ms][nt][k] == -INFINITY) pr[k] = 0.f;
           }
           const __half2 v0 = __floats2half2_rn(pr[0], pr[1]), v1 = __floats2half2_rn(pr[2], pr[3]);
           uint32_t f[Q2][2];
           f[0][0] = as_u32(v0), f[0][1] = as_u32(v1);
           if (kTwo) {
-            f[Q2 - 1][0] = as_u32(__floats2half2_rn(pr[0] - __low2float(v0), pr[1] - __high2float(v0)));
-            f[Q2 - 1][1] = as_u32(__floats2half2_rn(pr[2] - __low2float(v1), pr[3] - __high2float(v1)));
+            f[Q2 - 1][0] = rest_of(pr[0], pr[1], v0);
+            f[Q2 - 1][1] = rest_of(pr[2], pr[3], v1);
           }
 #pragma unroll
           for (int w = 0; w < Q2; ++w)
@@ -551,7 +554,7 @@ __global__ void __launch_bounds__(kWarps * 32, 16 / kWarps)
               uint32_t p0[Q2], p1[Q2];
 #pragma unroll
               for (int q2 = 0; q2 < Q2; ++q2) p0[q2] = pf[q2][mt][nt][0], p1[q2] = pf[q2][mt][nt][1];
-              mma_sum<Q2>(o[nt][2 * w + half], a, p0, p1);
+              mma_sum<Q2, true>(o[nt][2 * w + half], a, p0, p1);
             }
           }
       if (tile + kStep < tile1) load_v(tile + kStep);
@@ -580,13 +583,13 @@ __global__ void __launch_bounds__(kWarps * 32, 16 / kWarps)
         sum += __shfl_xor_sync(0xffffffffu, sum, 16);
         const int r = kFold ? (2 * t + e) & 3 : 2 * t + e, part = wid * kParts + fold;
         if (r < p.rows) {
-          const float f = v_lim[0][e] * (0.25f / 127.f);
+          const float f = power_of_two(scale_of(ref[0][e])) * (1.f / 127.f);
           float* dst = s_sums + (part * p.rows + r) * D + VB * g;
 #pragma unroll
           for (int i = 0; i < MI; i += 2)
             *reinterpret_cast<float4*>(dst + 2 * i) = make_float4(o[0][i][e] * f, o[0][i][2 + e] * f, o[0][i + 1][e] * f,
                                                                   o[0][i + 1][2 + e] * f);
-          if (g == 0) s_stats[part][r] = make_float2(ref[0][e], sum);
+          if (g == 0) s_stats[part][r] = make_float2(ref[0][e].score, sum);
         }
       }
       __syncthreads();

@@ -11,8 +11,8 @@ constexpr int kMaxDistances = 1024;
 constexpr int kMaxBatch = 2048;  // rows of one launch
 constexpr int kMaxBiases = 8192;  // values of a bias table
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kPeak = 4.f;     // exponent of a probability at the reference
-constexpr float kLimit = 12.6f;  // of the largest; times 4 it is still an fp16 number
+constexpr float kPeak = 7.f;     // exponent of a probability at the reference
+constexpr float kLimit = 15.6f;  // of the largest: an fp16 number
 constexpr float kNothing = -3e38f;  // the reference of a row that has seen nothing
 
 struct Cache8Attn {
@@ -41,6 +41,8 @@ struct Cache8Attn {
   uint8_t buckets[kMaxDistances];  // column of the bias table by distance
 };
 
+constexpr float kRest = 0x1p-11f;  // what the second number of a 32-bit probability counts: it stands above fp16's smallest
+
 __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                         uint32_t b1) {
   asm volatile(
@@ -49,28 +51,34 @@ __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1,
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-// c += a b, b one fp16 number or the sum of two. Tensor cores cut what they add to an accumulator off, toward zero: over a long
+// c += a b, b one fp16 number or, of 32-bit operands, two: their sum, or (kApart) the second at 2^-11. Tensor cores cut what they add to an accumulator off, toward zero: over a long
 // sum of 32-bit operands (two numbers) that would count more than they do, so theirs are added by an instruction that rounds.
-template <int Q2>
+template <int Q2, bool kApart = false>
 __device__ __forceinline__ void mma_sum(float (&c)[4], const uint32_t (&a)[4], const uint32_t (&b0)[Q2], const uint32_t (&b1)[Q2]) {
   if (Q2 == 1) {
     mma_f16(c, a[0], a[1], a[2], a[3], b0[0], b1[0]);
   } else {
     float x[4] = {0.f, 0.f, 0.f, 0.f};
     mma_f16(x, a[0], a[1], a[2], a[3], b0[Q2 - 1], b1[Q2 - 1]);
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (kApart) x[k] *= kRest;
     mma_f16(x, a[0], a[1], a[2], a[3], b0[0], b1[0]);
 #pragma unroll
     for (int k = 0; k < 4; ++k) c[k] += x[k];
   }
 }
 // The same with a the sum.
-template <int Q2>
+template <int Q2, bool kApart = false>
 __device__ __forceinline__ void mma_sum(float (&c)[4], const uint4 (&a)[Q2], uint32_t b0, uint32_t b1) {
   if (Q2 == 1) {
     mma_f16(c, a[0].x, a[0].y, a[0].z, a[0].w, b0, b1);
   } else {
     float x[4] = {0.f, 0.f, 0.f, 0.f};
     mma_f16(x, a[Q2 - 1].x, a[Q2 - 1].y, a[Q2 - 1].z, a[Q2 - 1].w, b0, b1);
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (kApart) x[k] *= kRest;
     mma_f16(x, a[0].x, a[0].y, a[0].z, a[0].w, b0, b1);
 #pragma unroll
     for (int k = 0; k < 4; ++k) c[k] += x[k];
@@ -95,10 +103,66 @@ __device__ __forceinline__ uint32_t low_flipped(uint32_t w, uint32_t low) {
 __device__ __forceinline__ uint32_t number_pair(uint32_t w, uint32_t low) {
   return as_u32(__hsub2(as_half2(low_flipped<0x64806480u>(w, low)), as_half2(0x64806480u)));
 }
+__device__ __forceinline__ float log2_approx(float x) {
+  float r;
+  asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
 __device__ __forceinline__ float exp2_approx(float x) {
   float r;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
   return r;
+}
+
+// A probability of 32 bits is two fp16 numbers, the second 2^11 times what the first leaves.
+__device__ __forceinline__ uint32_t rest_of(float lo, float hi, __half2 first) {
+  return as_u32(__floats2half2_rn((lo - __low2float(first)) * (1.f / kRest), (hi - __high2float(first)) * (1.f / kRest)));
+}
+
+// ---- What the probabilities of a query row are relative to ----
+//
+// The sum that divides adds 2^(s - score). The product with the values takes 2^(s - score - scale) times the largest value of the
+// token's block, so that one fp16 number holds both and the sums need no scaling by token. Each of the two is raised only where
+// it would come to 2^kLimit, to where its largest is 2^kPeak (the scale to a power of two), and by what the row itself sees, so that
+// neither what is hidden nor another row changes a result. Taking the scale of the product's largest term, not of the largest
+// block, keeps a block of large values but next to no weight from costing the others their bits: below 2^-14 fp16 numbers are
+// steps of 2^-24, at most 2^-30 of the largest term each.
+struct Reference {
+  float score;
+  float by;  // 2^-scale, scale whole, -126 to 126
+};
+__device__ __forceinline__ float power_of_two(int e) { return __uint_as_float(static_cast<uint32_t>(127 + e) << 23); }
+__device__ __forceinline__ int scale_of(const Reference& r) { return 127 - static_cast<int>(__float_as_uint(r.by) >> 23); }
+
+// Whether a score of a block goes over a limit; a: the block's largest value, times r.by.
+__device__ __forceinline__ bool beyond(const Reference& r, float s, float a) {
+  return s - r.score > kLimit - fmaxf(log2_approx(a), 0.f);
+}
+// x: the row's largest score here; x2: the largest with the logarithm of its block's largest value. What the sum that divides
+// and the other ones are multiplied by: 1 where nothing changes.
+__device__ __forceinline__ float2 raise_to(Reference& r, float x, float x2) {
+  const float old = static_cast<float>(scale_of(r));
+  const bool higher = x - r.score > kLimit, wider = x2 - r.score - old > kLimit;
+  const float up = higher ? x - kPeak : r.score;
+  const float to = wider ? x2 - kPeak : r.score + old;
+  const float scale = higher || wider ? fminf(fmaxf(ceilf(to - up), -126.f), 126.f) : old;
+  const float2 by = make_float2(exp2_approx(r.score - up), exp2_approx((r.score - up) + (old - scale)));
+  r.score = up;
+  r.by = power_of_two(-static_cast<int>(scale));
+  return by;
+}
+
+// Where a block's largest value a, relative to the scale, is no factor that 32 bits hold a small probability beside (or no number):
+// its part from 1 to 2 and its exponent, which goes into the scores.
+constexpr float kFar = 0x1p60f;
+__device__ __forceinline__ float2 part_of(const Reference& r, float a) {
+  const uint32_t u = __float_as_uint(a);
+  return make_float2(u < 0x00800000u ? 0.f : __uint_as_float((u & 0x007fffffu) | 0x3f800000u),
+                     static_cast<float>(static_cast<int>(u >> 23) - 127 - scale_of(r)));
+}
+// A score then; of a block that is not finite NaN, unless it is hidden.
+__device__ __forceinline__ float far_score(float s, float exponent, float a) {
+  return s == -INFINITY ? s : s + exponent + (a - a);
 }
 
 __device__ __forceinline__ int token_of(const Cache8Attn& p, int r) { return static_cast<int>((r * p.by_group) >> 32); }

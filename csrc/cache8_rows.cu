@@ -229,7 +229,8 @@ __global__ void __launch_bounds__(kThreads, 1) cache8_rows_kernel(const __grid_c
     }
     all_see = __reduce_min_sync(0xffffffffu, all_see);
     float o[M][D / 8][4];
-    float ref[M][2], l[M][2], v_lim[M][2], v_inv[M][2];  // v_lim: four times the scale that a value block's is relative to
+    Reference ref[M][2];
+    float l[M][2];
 #pragma unroll
     for (int m = 0; m < M; ++m) {
 #pragma unroll
@@ -237,11 +238,7 @@ __global__ void __launch_bounds__(kThreads, 1) cache8_rows_kernel(const __grid_c
 #pragma unroll
         for (int k = 0; k < 4; ++k) o[m][i][k] = 0.f;
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        ref[m][e] = kNothing;
-        l[m][e] = v_inv[m][e] = 0.f;
-        v_lim[m][e] = row0 + 16 * m + 8 * e + g < p.rows ? 0.f : INFINITY;  // (of a row that is none: none)
-      }
+      for (int e = 0; e < 2; ++e) ref[m][e] = {kNothing, 1.f}, l[m][e] = 0.f;
     }
 
     int buffer = 0;
@@ -308,7 +305,6 @@ __global__ void __launch_bounds__(kThreads, 1) cache8_rows_kernel(const __grid_c
         }
 
         // ---- scores of tokens 2t + {0, 1} and 8 more, rows g (k = 0, 1) and g + 8 (k = 2, 3) ----
-        bool raise = false;  // whether a reference has to go up
         float va[MT];
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt) {
@@ -365,42 +361,45 @@ __global__ void __launch_bounds__(kThreads, 1) cache8_rows_kernel(const __grid_c
                 }
               }
           }
-#pragma unroll
-          for (int m = 0; m < M; ++m)
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              const float top = fmaxf(fmaxf(s[mt][m][0][2 * e], s[mt][m][0][2 * e + 1]), fmaxf(s[mt][m][1][2 * e], s[mt][m][1][2 * e + 1]));
-              raise |= top - ref[m][e] > kLimit;
-              raise |= va[mt] > v_lim[m][e];
-            }
         }
 
-        // ---- references ----
+        // ---- references (all tiles of the step in one question: raise_to asks exactly) ----
+        float most = va[0];
+#pragma unroll
+        for (int mt = 1; mt < MT; ++mt) most = fmaxf(most, va[mt]);
+        bool raise = false;
+#pragma unroll
+        for (int m = 0; m < M; ++m)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            float top = -INFINITY;
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+              for (int k = 0; k < 4; ++k) top = fmaxf(top, s[mt][m][k >> 1][2 * e + (k & 1)]);
+            raise |= beyond(ref[m][e], top, most * ref[m][e].by);
+          }
         if (__any_sync(0xffffffffu, raise)) {
 #pragma unroll
           for (int m = 0; m < M; ++m)
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-              float x = -INFINITY, v = 0.25f * v_lim[m][e];
+              float x = -INFINITY, x2 = -INFINITY;
 #pragma unroll
               for (int mt = 0; mt < MT; ++mt) {
-                float high = fmaxf(fmaxf(s[mt][m][0][2 * e], s[mt][m][0][2 * e + 1]), fmaxf(s[mt][m][1][2 * e], s[mt][m][1][2 * e + 1]));
-                high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, 1));
-                high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, 2));
+                const float high = fmaxf(fmaxf(s[mt][m][0][2 * e], s[mt][m][0][2 * e + 1]), fmaxf(s[mt][m][1][2 * e], s[mt][m][1][2 * e + 1]));
                 x = fmaxf(x, high);
-                if (high > -INFINITY && va[mt] < INFINITY) v = fmaxf(v, va[mt]);  // (the row sees a token of the tile)
+                x2 = fmaxf(x2, high + log2_approx(va[mt]));
               }
-              // (only what this row sees raises its own: a result does not hang on what is hidden, nor on other rows)
-              if (!(x - ref[m][e] > kLimit || v > v_lim[m][e])) continue;
-              const float up = fmaxf(x - kPeak, ref[m][e]);
-              const float f = exp2_approx(ref[m][e] - up);
-              v_inv[m][e] = v > 0.f ? __frcp_rn(v) : 0.f;
-              const float shrink = f * (0.25f * v_lim[m][e] * v_inv[m][e]);  // (0 where nothing had been met)
-              ref[m][e] = up;
-              l[m][e] *= f;
-              v_lim[m][e] = 4.f * v;
 #pragma unroll
-              for (int i = 0; i < D / 8; ++i) o[m][i][2 * e] *= shrink, o[m][i][2 * e + 1] *= shrink;
+              for (int lanes = 1; lanes < 4; lanes *= 2) {
+                x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, lanes));
+                x2 = fmaxf(x2, __shfl_xor_sync(0xffffffffu, x2, lanes));
+              }
+              const float2 by = raise_to(ref[m][e], x, x2);
+              l[m][e] *= by.x;
+#pragma unroll
+              for (int i = 0; i < D / 8; ++i) o[m][i][2 * e] *= by.y, o[m][i][2 * e + 1] *= by.y;
             }
         }
 
@@ -410,9 +409,22 @@ __global__ void __launch_bounds__(kThreads, 1) cache8_rows_kernel(const __grid_c
           uint4 pf[M][Q2];
 #pragma unroll
           for (int m = 0; m < M; ++m) {
-            const float r[2] = {va[mt] * v_inv[m][0], va[mt] * v_inv[m][1]};
-            // a block that is not finite, or far larger than what is seen: what is hidden counts for nothing all the same
-            const bool odd = !(fmaxf(r[0], r[1]) < INFINITY);
+            float r[2] = {va[mt] * ref[m][0].by, va[mt] * ref[m][1].by};
+            float counts = 1.f;  // in the sum that divides
+            if (!(fmaxf(r[0], r[1]) < kFar)) {
+              counts = 0.f;
+#pragma unroll
+              for (int e = 0; e < 2; ++e) {
+                const float2 part = part_of(ref[m][e], va[mt]);
+                r[e] = part.x;
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                  float& x = s[mt][m][k >> 1][2 * e + (k & 1)];
+                  l[m][e] += exp2_approx(x - ref[m][e].score);
+                  x = far_score(x, part.y, va[mt]);
+                }
+              }
+            }
             uint32_t f[Q2][4];
 #pragma unroll
             for (int n = 0; n < 2; ++n)
@@ -422,14 +434,13 @@ __global__ void __launch_bounds__(kThreads, 1) cache8_rows_kernel(const __grid_c
 #pragma unroll
                 for (int k = 0; k < 2; ++k) {
                   const float x = s[mt][m][n][2 * e + k];
-                  pr[k] = exp2_approx(x - ref[m][e]);
-                  l[m][e] += pr[k];
+                  pr[k] = exp2_approx(x - ref[m][e].score);
+                  l[m][e] += pr[k] * counts;
                   pr[k] *= r[e];
-                  if (odd && x == -INFINITY) pr[k] = 0.f;
                 }
                 const __half2 v = __floats2half2_rn(pr[0], pr[1]);
                 f[0][2 * n + e] = as_u32(v);
-                if (kTwo) f[Q2 - 1][2 * n + e] = as_u32(__floats2half2_rn(pr[0] - __low2float(v), pr[1] - __high2float(v)));
+                if (kTwo) f[Q2 - 1][2 * n + e] = rest_of(pr[0], pr[1], v);
               }
 #pragma unroll
             for (int w = 0; w < Q2; ++w) pf[m][w] = make_uint4(f[w][0], f[w][1], f[w][2], f[w][3]);
@@ -444,8 +455,8 @@ __global__ void __launch_bounds__(kThreads, 1) cache8_rows_kernel(const __grid_c
             const uint32_t(&v)[4] = vf[i & 1];
 #pragma unroll
             for (int m = 0; m < M; ++m) {
-              mma_sum<Q2>(o[m][2 * i], pf[m], v[0], v[1]);
-              mma_sum<Q2>(o[m][2 * i + 1], pf[m], v[2], v[3]);
+              mma_sum<Q2, true>(o[m][2 * i], pf[m], v[0], v[1]);
+              mma_sum<Q2, true>(o[m][2 * i + 1], pf[m], v[2], v[3]);
             }
           }
         }
@@ -460,7 +471,7 @@ __global__ void __launch_bounds__(kThreads, 1) cache8_rows_kernel(const __grid_c
         float sum = l[m][e];
         sum += __shfl_xor_sync(0xffffffffu, sum, 1);
         l[m][e] = sum + __shfl_xor_sync(0xffffffffu, sum, 2);
-        const float f = v_lim[m][e] * (0.25f / 127.f);
+        const float f = power_of_two(scale_of(ref[m][e])) * (1.f / 127.f);
 #pragma unroll
         for (int i = 0; i < D / 8; ++i)
 #pragma unroll
@@ -480,7 +491,7 @@ __global__ void __launch_bounds__(kThreads, 1) cache8_rows_kernel(const __grid_c
             given[from * kGiven + (m * (D / 8) + i) * 32 + lane] = make_float4(o[m][i][0], o[m][i][1], o[m][i][2], o[m][i][3]);
 #pragma unroll
           for (int e = 0; e < 2; ++e)
-            if (t == 0) s_stats[from][16 * m + 8 * e + g] = make_float2(ref[m][e], l[m][e]);
+            if (t == 0) s_stats[from][16 * m + 8 * e + g] = make_float2(ref[m][e].score, l[m][e]);
         }
       }
       __syncthreads();
@@ -491,10 +502,10 @@ __global__ void __launch_bounds__(kThreads, 1) cache8_rows_kernel(const __grid_c
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
             const float2 st = s_stats[wid][16 * m + 8 * e + g];
-            const float top = fmaxf(ref[m][e], st.x);
-            f[e] = exp2_approx(ref[m][e] - top);
+            const float top = fmaxf(ref[m][e].score, st.x);
+            f[e] = exp2_approx(ref[m][e].score - top);
             other[e] = exp2_approx(st.x - top);
-            ref[m][e] = top;
+            ref[m][e].score = top;
             l[m][e] = l[m][e] * f[e] + st.y * other[e];
           }
 #pragma unroll
@@ -528,13 +539,13 @@ __global__ void __launch_bounds__(kThreads, 1) cache8_rows_kernel(const __grid_c
               dst[8 * i] = from_float<T>(o[m][i][2 * e] * inv);
               dst[8 * i + 1] = from_float<T>(o[m][i][2 * e + 1] * inv);
             }
-            if (t == 0 && p.scores != nullptr) p.final_stats[bh * p.rows + r] = make_float2(ref[m][e], inv);
+            if (t == 0 && p.scores != nullptr) p.final_stats[bh * p.rows + r] = make_float2(ref[m][e].score, inv);
           } else {
             float* dst = p.part + (slot + in_tile) * D + 2 * t;
 #pragma unroll
             for (int i = 0; i < D / 8; ++i)
               *reinterpret_cast<float2*>(dst + 8 * i) = make_float2(o[m][i][2 * e], o[m][i][2 * e + 1]);
-            if (t == 0) p.stats[slot + in_tile] = make_float2(ref[m][e], l[m][e]);
+            if (t == 0) p.stats[slot + in_tile] = make_float2(ref[m][e].score, l[m][e]);
           }
         }
     }

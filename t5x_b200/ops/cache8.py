@@ -5,7 +5,7 @@ gathered as ever), in blocks of 16, 32, 64 or 128 tokens of a head that share a 
 
 * `cached_key`, `cached_value`: int8 [rows, heads, slots, head_dim];
 * `key_absmax`, `value_absmax`: fp32 [rows, heads, slots / block], the largest absolute value of a block. A code c
-  stands for c * absmax / 127. A value that is not finite makes its block NaN. (Attention adds up to a few thousand times a
+  stands for c * absmax / 127. A value that is not finite makes its block NaN. (Attention adds up to 2^32 times a
   value before it divides: seen values beyond 2^96 may come out infinite.);
 * `cache_index`: int32, tokens that a row holds ([rows], or one for all). Slots from there on are not read;
 * `token_weight`, optional: fp32 [rows, heads, slots], the attention that each token got so far;
