@@ -429,9 +429,13 @@ class MultiHeadDotProductAttention(nn.Module):
     cache["cache_room"] = self.EVICT_ROOM
 
   def _decode8(self, cache: dict, q, k, v, bias) -> torch.Tensor:
-    """One step over a cache in 8 bits: its tokens are appended and attended to; a full cache evicts first."""
+    """One step over a cache in 8 bits: its tokens are appended and attended to; a full cache evicts first. Steps of more
+    tokens than an eviction makes room for go in parts of so many."""
     room = cache.get("cache_room")
     if room is not None:
+      if k.shape[1] > self.EVICT_ROOM:
+        parts = zip(*(t.split(self.EVICT_ROOM, 1) for t in (q, k, v)))
+        return torch.cat([self._decode8(cache, *part, bias) for part in parts], 1)
       if room < k.shape[1]:
         kept, _ = cache8.evict(cache, self.kv_cache_keep, recent=self.kv_cache_recent)
         cache.update(kept)

@@ -154,3 +154,24 @@ def test_refusals():
     attn(x, x, cache=cache, decode=True, bidirectional=False)
   with pytest.raises(ValueError, match="causal"), torch.no_grad():
     attn(x, x, cache=cache, decode=True, bias_table=table)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("steps", [[100], [30, 64, 7, 130, 1], [65, 65]])
+@torch.no_grad()
+def test_steps_of_more_tokens_than_an_eviction_makes_room_for(device, steps):
+  """No token is left out: the cache and the results are those of parts of 64 tokens, given one after the other."""
+  attn, table = attention_layer(device, kv_cache_keep=20, kv_cache_recent=5)
+  x = (torch.randn(2, sum(steps), 64, device=device) / 4).to(attn.dtype)
+  kw = dict(bias_table=table, bidirectional=False, decode=True)
+  outs = []
+  for sizes in (steps, [n for step in steps for n in [64] * (step // 64) + [step % 64] if n]):
+    cache = attn.init_cache(2, 400, device)
+    outs.append((torch.cat([attn(p, p, cache=cache, **kw) for p in x.split(sizes, 1)], 1), cache))
+    assert 0 <= cache["cache_room"] <= 96 and cache["cache_index"].max() <= 84
+    held = cache["cache_index"].expand(2) + (cache["dropped"] if "dropped" in cache else 0)
+    assert held.tolist() == [sum(steps)] * 2
+  (got, one), (want, other) = outs
+  # (the projections of parts may round the other way)
+  assert torch.allclose(got, want, rtol=0.03, atol=0.03 if device == "cuda" else 1e-5)
+  assert one["cache_room"] == other["cache_room"] and one["dropped"].tolist() == other["dropped"].tolist()
