@@ -926,6 +926,11 @@ bool adamw_tree(py::handle params, py::handle grads, py::handle mu, py::handle n
       !gather(params.ptr(), grads.ptr(), mu.ptr(), nu.ptr(), mu_most.ptr(), nu_most.ptr(), to) ||
       !to_items(to) || to.overlap())
     return false;
+  // (the kernel writes through pointers: whoever watches a parameter's version learns of the step by this)
+  for (const AdamwItems::Objects& o : to.objects) {
+    const Tensor& p = THPVariable_Unpack(o.p);
+    if (!p.is_inference()) p.unsafeGetTensorImpl()->bump_version();
+  }
   py::gil_scoped_release no_gil;
   void* st = stream_of();
   const int count = static_cast<int>(to.items.size());

@@ -24,7 +24,7 @@ import numpy as np
 import torch
 import torch.distributed as dist
 
-from t5x_b200.optimizers import OptimizerDef, OptimizerState
+from t5x_b200.optimizers import OptimizerDef, OptimizerState, note_update
 from t5x_b200.parallel import state as pstate
 from t5x_b200.utils import tree as tree_utils
 
@@ -619,6 +619,7 @@ class Adafactor(OptimizerDef):
           continue  # already updated while the backward pass was running
         todo.append((p, flat_s[k], flat_g[k], k))
       self.apply_param_gradients(step, hyper_params, todo, pre_reduced=pre_reduced)
+      note_update(flat_p.values())
     finally:
       self.hyper_params = saved_hp
     return params, OptimizerState(step + 1, state.param_states)

@@ -13,6 +13,7 @@ reduction over the `model` axis.
 """
 from __future__ import annotations
 
+import copy
 import math
 from typing import Callable, Optional, Sequence, Tuple
 
@@ -217,6 +218,27 @@ def dot_product_attention(query, key, value, bias=None, dropout_rate=0.0, determ
 # ----------------------------------------------------------------------------
 # Modules
 # ----------------------------------------------------------------------------
+class _Weight8:
+  """A kernel's weights in 8 bits, for as long as the kernel stays as it was."""
+
+  def __init__(self, kernel: torch.Tensor):
+    self.codes, self.kernel, self.version = F.quantize_weight(kernel), kernel, self._version(kernel)
+
+  @staticmethod
+  def _version(kernel: torch.Tensor) -> Optional[int]:
+    return None if kernel.is_inference() else kernel._version  # (made in inference mode: it has none)
+
+  def is_of(self, kernel: torch.Tensor) -> bool:
+    return kernel is self.kernel and self._version(kernel) == self.version
+
+  def __deepcopy__(self, memo):
+    new = object.__new__(type(self))
+    memo[id(self)] = new
+    new.codes, new.kernel = copy.deepcopy(self.codes, memo), copy.deepcopy(self.kernel, memo)
+    new.version = self._version(new.kernel) if self.is_of(self.kernel) else -1
+    return new
+
+
 class DenseGeneral(nn.Module):
   """Bias-free projection y = x @ kernel, kernel [in, out] fp32 (layers.py:364-414)."""
 
@@ -229,27 +251,27 @@ class DenseGeneral(nn.Module):
     self.kernel = param_with_axes((in_features, out_features), init, kernel_axes,
                                   shard_dim=shard_dim, device=device)
 
-  # weights in 8 bits that `quantize_dense` made, the kernel that they were made from and its version
-  weight8 = None
+  weight8: Optional[_Weight8] = None  # what `quantize_dense` made
 
   def forward(self, x: torch.Tensor, residual: Optional[torch.Tensor] = None) -> torch.Tensor:
     if self.weight8 is not None:
-      weight, kernel, version = self.weight8
-      if kernel is not self.kernel or kernel._version != version:
+      if not self.weight8.is_of(self.kernel):
         raise ValueError("the kernel has changed since quantize_dense: call it again, or dequantize_dense")
-      return F.linear8(x.to(self.dtype), weight, None if residual is None else residual.to(self.dtype))
+      return F.linear8(x.to(self.dtype), self.weight8.codes, None if residual is None else residual.to(self.dtype))
     return F.linear(x.to(self.dtype), self.kernel, residual=residual, dtype=self.dtype)
 
 
 def quantize_dense(module: nn.Module) -> int:
   """Lets every projection of `module` multiply in 8-bit integers (`functional.linear8`), for serving: weights scaled by output
   channel, activations by token. The kernels stay as they are; a projection whose kernel changes afterwards raises until this
-  is called again. Returns how many projections there are. The embedding and the logits (in 32 bits) are left alone."""
+  is called again. (It sees what raises the kernel's version: operations in place, a step of the framework's optimizers, loaded
+  state; not what is written through `.data`, in inference mode, by a replayed CUDA graph or by kernels of the user's own: call
+  this again after those.) Returns how many projections there are. The embedding and the logits (in 32 bits) are left alone."""
   if pstate.get().model_size > 1:
     raise ValueError("quantize_dense: not under a model axis")
   found = [m for name, m in module.named_modules() if type(m) is DenseGeneral and not name.endswith("logits_dense")]
   for m in found:
-    m.weight8 = (F.quantize_weight(m.kernel), m.kernel, m.kernel._version)
+    m.weight8 = _Weight8(m.kernel)
   return len(found)
 
 

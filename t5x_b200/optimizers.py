@@ -68,6 +68,12 @@ to_state_dict = _to_state_dict
 from_state_dict = _from_state_dict
 
 
+def note_update(params) -> None:
+  """Raises the versions of parameters that kernels have written through pointers, or that were written through `.data`, as
+  an operation in place does: whoever watches `_version` (a projection with weights in 8 bits) learns of the step by it."""
+  torch.autograd.graph.increment_version([p for p in params if isinstance(p, torch.Tensor) and not p.is_inference()])
+
+
 class OptimizerDef:
   """Base class for an optimizer definition (t5x/optimizers.py:52-118)."""
 
@@ -762,6 +768,7 @@ class OptaxWrapper(OptimizerDef):
             clip_scale = native.grad_clip_scale(items, plan["max_norm"], device)
           factor = clip_scale if clip_scale is None else clip_scale.to(device)
           native.adamw_group_(items, plan["bits"], seed=plan["seed"], clip_scale=factor, **hyper)
+    note_update(flat_p.values())
     adam_state["count"] = adam_state["count"] + 1
     lr_state["count"] = lr_state["count"] + 1
     return params, OptimizerState(step=state.step + 1, param_states=self._nest(opt_state))

@@ -1,4 +1,6 @@
 """Decoding in 8 bits as the models reach it: `kv_cache_dtype`, `kv_cache_keep`, `layers.quantize_dense`."""
+import copy
+
 import numpy as np
 import pytest
 import torch
@@ -7,6 +9,8 @@ from t5x_b200 import adafactor
 from t5x_b200 import decoding
 from t5x_b200 import decoding_fast
 from t5x_b200 import models
+from t5x_b200 import optax_api
+from t5x_b200 import optimizers
 from t5x_b200.data import vocabularies
 from t5x_b200.models.decoder_only import network as decoder_only
 from t5x_b200.models.t5 import layers
@@ -175,3 +179,55 @@ def test_steps_of_more_tokens_than_an_eviction_makes_room_for(device, steps):
   # (the projections of parts may round the other way)
   assert torch.allclose(got, want, rtol=0.03, atol=0.03 if device == "cuda" else 1e-5)
   assert one["cache_room"] == other["cache_room"] and one["dropped"].tolist() == other["dropped"].tolist()
+
+
+STEPS = {"adafactor": lambda: adafactor.Adafactor(min_dim_size_to_factor=0),
+         "adafactor of vectors": lambda: adafactor.Adafactor(min_dim_size_to_factor=1000),
+         "adamw": lambda: optimizers.adamw(0.1),
+         "clipped adamw": lambda: optimizers.chain([optimizers.clip_by_global_norm(0.5), optax_api.adamw(0.1)]),
+         "adamw8": lambda: optimizers.adamw8(0.1), "sgd": lambda: optimizers.sgd(0.1)}
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("name", STEPS)
+def test_a_step_of_an_optimizer_is_seen_by_quantized_projections(device, name):
+  """Its kernels write the parameters through pointers, its statements through `.data`."""
+  torch.manual_seed(0)
+  dense = layers.DenseGeneral(64, 96, ("embed", "mlp"), device=device)
+  layers.quantize_dense(dense)
+  x = torch.randn(3, 64, device=device)
+  before = dense.kernel.detach().clone()
+  with torch.no_grad():
+    stale = dense(x)
+  optimizer = STEPS[name]().create({"mlp": {"kernel": dense.kernel}})
+  optimizer.apply_gradient({"mlp": {"kernel": torch.randn(64, 96, device=device)}}, learning_rate=0.1)
+  assert not torch.equal(dense.kernel, before)
+  with torch.no_grad():
+    with pytest.raises(ValueError, match="quantize_dense"):
+      dense(x)
+    layers.quantize_dense(dense)
+    assert torch.equal(dense(x), F.linear8(x, F.quantize_weight(dense.kernel))) and not torch.equal(dense(x), stale)
+
+
+def test_copies_of_quantized_projections_and_kernels_of_inference_mode():
+  torch.manual_seed(0)
+  dense = layers.DenseGeneral(64, 96, ("embed", "mlp"))
+  x = torch.randn(3, 64)
+  with torch.no_grad():
+    dense.kernel.mul_(2.0)
+    layers.quantize_dense(dense)
+    twin = copy.deepcopy(dense)
+    assert torch.equal(twin(x), dense(x))
+    twin.kernel.add_(1.0)
+    with pytest.raises(ValueError, match="quantize_dense"):
+      twin(x)
+    dense(x)
+    with pytest.raises(ValueError, match="quantize_dense"):
+      copy.deepcopy(twin)(x)
+    dense.kernel = torch.nn.Parameter(dense.kernel.clone())
+    with pytest.raises(ValueError, match="quantize_dense"):
+      dense(x)
+  with torch.inference_mode():
+    dense = layers.DenseGeneral(64, 96, ("embed", "mlp"))
+    layers.quantize_dense(dense)
+    assert torch.equal(dense(x), F.linear8(x, F.quantize_weight(dense.kernel)))
