@@ -257,6 +257,9 @@ class DenseGeneral(nn.Module):
     if self.weight8 is not None:
       if not self.weight8.is_of(self.kernel):
         raise ValueError("the kernel has changed since quantize_dense: call it again, or dequantize_dense")
+      if torch.is_grad_enabled() and self.kernel.requires_grad:
+        raise ValueError("a projection in 8 bits has no backward pass, not to its kernel either: call it under torch.no_grad(), or "
+                         "dequantize_dense")
       return F.linear8(x.to(self.dtype), self.weight8.codes, None if residual is None else residual.to(self.dtype))
     return F.linear(x.to(self.dtype), self.kernel, residual=residual, dtype=self.dtype)
 

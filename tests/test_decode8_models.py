@@ -231,3 +231,20 @@ def test_copies_of_quantized_projections_and_kernels_of_inference_mode():
     dense = layers.DenseGeneral(64, 96, ("embed", "mlp"))
     layers.quantize_dense(dense)
     assert torch.equal(dense(x), F.linear8(x, F.quantize_weight(dense.kernel)))
+
+
+def test_a_quantized_projection_under_grad_mode():
+  """Its kernel would get no gradient: refused, where the kernel wants one."""
+  dense = layers.DenseGeneral(64, 96, ("embed", "mlp"))
+  layers.quantize_dense(dense)
+  x = torch.randn(3, 64)
+  with pytest.raises(ValueError, match="no_grad"):
+    dense(x)
+  with torch.no_grad():
+    want = dense(x)
+  with torch.inference_mode():
+    assert torch.equal(dense(x), want)
+  dense.kernel.requires_grad_(False)
+  assert torch.equal(dense(x), want)
+  with pytest.raises(ValueError, match="no_grad"):
+    dense(x.requires_grad_())
