@@ -481,7 +481,7 @@ class MultiHeadDotProductAttention(nn.Module):
   def project_kv(self, inputs_kv: torch.Tensor):
     b, lk, _ = inputs_kv.shape
     kv_in = tp.copy_to_model_parallel(inputs_kv).to(self.dtype)
-    if self.key.weight8 is not None:
+    if self.key.weight8 is not None or self.value.weight8 is not None:
       k, v = self.key(kv_in), self.value(kv_in)
     else:
       k, v = F.multi_linear(kv_in, [self.key.kernel, self.value.kernel], dtype=self.dtype)
@@ -507,7 +507,7 @@ class MultiHeadDotProductAttention(nn.Module):
       x = cache8.attention(q, precomputed_kv, key_mask=key_mask, causal=False)
       return self._project_out(x, b, lq, residual)
     if (precomputed_kv is None and inputs_kv is inputs_q and not self.scale_attn_logits and
-        self.query.weight8 is None):
+        all(m.weight8 is None for m in (self.query, self.key, self.value))):
       # self-attention: the three projections share their input, and one backward builds its
       # gradient by accumulating GEMMs
       q, k, v = F.multi_linear(q_in.to(self.dtype),
@@ -739,7 +739,7 @@ class MlpBlock(nn.Module):
   def forward(self, inputs: torch.Tensor, residual: Optional[torch.Tensor] = None,
               enable_dropout: bool = False) -> torch.Tensor:
     x_in = tp.copy_to_model_parallel(inputs.to(self.dtype))
-    if self.activations == ("gelu", "linear") and self.wi_0.weight8 is None:
+    if self.activations == ("gelu", "linear") and self.wi_0.weight8 is None and self.wi_1.weight8 is None:
       x = F.gated_gelu_mlp_in(x_in, self.wi_0.kernel, self.wi_1.kernel, dtype=self.dtype)
     elif len(self.activations) == 1:
       x = ref.ACTIVATIONS[self.activations[0]](self.wi(x_in))

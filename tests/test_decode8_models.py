@@ -248,3 +248,25 @@ def test_a_quantized_projection_under_grad_mode():
   assert torch.equal(dense(x), want)
   with pytest.raises(ValueError, match="no_grad"):
     dense(x.requires_grad_())
+
+
+@pytest.mark.parametrize("name", ["query", "key", "value", "out", "wi_0", "wi_1", "wo"])
+@torch.no_grad()
+def test_a_projection_quantized_by_itself(name):
+  """It multiplies in 8 bits where its layer runs, whatever the projections beside it do."""
+  torch.manual_seed(0)
+  attn = layers.MultiHeadDotProductAttention(64, 2, 8, "float32")
+  mlp = layers.MlpBlock(64, 32, ("gelu", "linear"), 0.0, "float32")
+  x = torch.randn(2, 5, 64)
+  run = lambda: (attn(x, x), mlp(x))  # noqa: E731
+  plain = run()
+  module = getattr(attn, name, None) or getattr(mlp, name)
+  assert layers.quantize_dense(module) == 1
+  calls, forward = [], F.linear8
+  F.linear8 = lambda *args, **kw: (calls.append(args[1]), forward(*args, **kw))[1]
+  try:
+    got = run()
+  finally:
+    F.linear8 = forward
+  assert len(calls) == 1 and calls[0] is module.weight8.codes
+  assert [torch.equal(a, b) for a, b in zip(got, plain)] == [hasattr(mlp, name), hasattr(attn, name)]
