@@ -1,6 +1,8 @@
 // Products in 8-bit integers: y = (sum_k cx cw) * sx * sw / 127^2 (+ residual), activations scaled by token (sx, the
 // largest |x| of the row, cx = 127 x / sx rounded) and weights by output channel. The sums of products are whole numbers
-// below 2^31 for up to 131072 channels and exact; one rounding at the end.
+// below 2^31 for up to 131072 channels and exact. The rest is in 32 bits: the sum's conversion, a scale's division and the product
+// with each, the residual's addition, some 2^-21 of the result's parts together; then the rounding to y's type. Scales beyond
+// 2^40 or below 2^-40, with which a part of that could leave the normal numbers where y does not, go through 64 bits.
 //
 // Two launches, for more than two rows: the rows are turned into codes, and tcgen05 (kind::i8, sums in 32 bits in tensor memory)
 // multiplies them.
@@ -17,6 +19,38 @@ namespace {
 
 constexpr int kKernelIdLinear8 = 21;
 constexpr int kMaxK = 131072;
+
+// Whether sums of products times two such scales stay between 2^-94 and 2^97. (0, and what is not finite, need no care.)
+__device__ __forceinline__ bool ordinary(float a) {
+  const uint32_t u = __float_as_uint(a);
+  return u - (87u << 23) <= (80u << 23) || u == 0 || u >= 0x7f800000u;  // 2^-40 to 2^40
+}
+// sum * sx * sw / 127^2 + add
+__device__ __noinline__ float in_64_bits(int sum, float sx, float sw, float add) {
+  double x, w, r;  // (conversions that the build's flags do not let lose numbers below the normal ones)
+  asm("cvt.f64.f32 %0, %1;" : "=d"(x) : "f"(sx));
+  asm("cvt.f64.f32 %0, %1;" : "=d"(w) : "f"(sw));
+  asm("cvt.f64.f32 %0, %1;" : "=d"(r) : "f"(add));
+  r += sum * x * w / 16129.0;
+  float y;
+  asm("cvt.rn.f32.f64 %0, %1;" : "=f"(y) : "d"(r));
+  return y;
+}
+// The same for V values; sx, sw: the largest values of their rows and channels.
+template <int V>
+__device__ __forceinline__ void scaled(const int (&sum)[V], const float (&sx)[V], const float (&sw)[V], const float (&add)[V],
+                                       float (&y)[V]) {
+  bool far = false;
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    far |= !ordinary(sx[i]) || !ordinary(sw[i]);
+    y[i] = static_cast<float>(sum[i]) * (sx[i] * (1.f / 127.f)) * (sw[i] * (1.f / 127.f)) + add[i];
+  }
+  if (far) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) y[i] = in_64_bits(sum[i], sx[i], sw[i], add[i]);
+  }
+}
 
 // D (+)= A * B on signed 8-bit integers over a CTA pair, issued by one thread of the even CTA.
 __device__ __forceinline__ void umma_i8_pair(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
@@ -315,7 +349,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       int mt, nt;
       tile_at(p, tile, mt, nt);
       const int m0 = mt * kTileRows + static_cast<int>(cta) * kRows + q * 32;
-      const float sx = m0 + lane < p.M ? p.x_absmax[m0 + lane] * (1.f / 127.f) : 0.f;
+      const float most = m0 + lane < p.M ? p.x_absmax[m0 + lane] : 0.f, sx = most * (1.f / 127.f);
+      bool far = !ordinary(most);
       const long long row = m0 + lane;
       const int col0 = part * (kTileCols / 2), first = nt * kTileCols + col0;
       constexpr int kBlocks = kTileCols / 64;  // of 32 channels
@@ -323,9 +358,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 #pragma unroll
       for (int i = 0; i < kBlocks; ++i) {
         const int n = first + i * 32 + lane;
-        sw[i] = n < p.N ? p.w_absmax[n] * (1.f / 127.f) : 0.f;
+        const float most_n = n < p.N ? p.w_absmax[n] : 0.f;
+        far |= !ordinary(most_n);
+        sw[i] = most_n * (1.f / 127.f);
       }
-      if (p.vec == 2) {  // in the patch
+      far = __any_sync(0xffffffffu, far);  // (one value at a time then)
+      const bool wide = p.vec == 2 && !far;
+      if (wide) {  // in the patch
         __syncwarp();
 #pragma unroll
         for (int i = 0; i < kBlocks; ++i) patch[i * 32 + lane] = sw[i];
@@ -340,7 +379,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       const uint32_t t_row = tmem + (static_cast<uint32_t>(q * 32) << 16) + acc * kTileCols;
       // A lane stores its row's channels where they are whole sectors. (In 32 bits, 4096 x 64 x 16384: 101 us so, 114 by patches; 4096 x
       // 57 x 16004, whole 16 bytes alone: 176 and 130.)
-      if (p.vec == 2) {
+      if (wide) {
         constexpr int E = 16 / sizeof(T), W = sizeof(T) == 4 ? 32 : 64, L = W / E;  // values of 16 bytes, channels at a time, 16 bytes of a lane
 #pragma unroll 1
         for (int c = 0; c < kTileCols / 2; c += W) {
@@ -378,7 +417,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         }
       }
       // Rows at any address: by patches of 32 x 32, a lane a channel. The next sums are requested before these are stored.
-      if (p.vec != 2 && first < p.N && m0 < p.M) {
+      if (!wide && first < p.N && m0 < p.M) {
         const int rows = min(32, p.M - m0);
         uint32_t r[32];
         tmem_ld32(t_row + col0, r);
@@ -388,7 +427,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           if (n0 >= p.N) break;
           const bool mine = n0 + lane < p.N;
           T add[32];
-          if (residual != nullptr && mine) {
+          if (residual != nullptr && mine && !far) {
 #pragma unroll
             for (int i = 0; i < 32; ++i)
               if (i < rows) add[i] = residual[(m0 + i) * p.ld_res + n0 + lane];
@@ -396,10 +435,19 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           tmem_ld_wait();
           __syncwarp();  // the patch's last readers are done
 #pragma unroll
-          for (int j = 0; j < 32; ++j) patch[lane * 33 + j] = static_cast<float>(static_cast<int>(r[j])) * sx;
+          for (int j = 0; j < 32; ++j)
+            patch[lane * 33 + j] = far ? __uint_as_float(r[j]) : static_cast<float>(static_cast<int>(r[j])) * sx;
           __syncwarp();
           if (cb + 1 < kBlocks && n0 + 32 < p.N) tmem_ld32(t_row + col0 + (cb + 1) * 32, r);
-          if (mine) {
+          if (mine && far) {
+            const float most_n = p.w_absmax[n0 + lane];
+#pragma unroll 1
+            for (int i = 0; i < rows; ++i) {
+              const float plus = residual != nullptr ? to_float(residual[(m0 + i) * p.ld_res + n0 + lane]) : 0.f;
+              y[static_cast<long long>(m0 + i) * p.N + n0 + lane] =
+                  from_float<T>(in_64_bits(__float_as_int(patch[i * 33 + lane]), p.x_absmax[m0 + i], most_n, plus));
+            }
+          } else if (mine) {
             T* to = y + static_cast<long long>(m0) * p.N + n0 + lane;
 #pragma unroll
             for (int i = 0; i < 32; ++i) {
@@ -599,7 +647,6 @@ __global__ void __launch_bounds__(kFewThreads)
   T* y = static_cast<T*>(p.y);
   const T* residual = static_cast<const T*>(p.residual);
   const int tokens = min(NR, p.M - m0);
-  auto value = [&](int sum, float sx, int n) { return static_cast<float>(sum) * sx * (p.w_absmax[n] * (1.f / 127.f)); };
   if (p.vec) {  // four channels a thread (there are whole fours of them)
     for (int i = piece * kFewThreads + threadIdx.x; i < tokens * 32; i += splits * kFewThreads) {
       const int tok = i >> 5, ch = (i & 31) * 4, n = n0 + ch;
@@ -611,24 +658,28 @@ __global__ void __launch_bounds__(kFewThreads)
       const long long row = m0 + tok;
       float add[4] = {0.f, 0.f, 0.f, 0.f};
       if (residual != nullptr) load_four(residual + row * p.ld_res + n, true, add);
-      const float sx = ld_chained(p.x_absmax + row) * (1.f / 127.f);
+      const float most = ld_chained(p.x_absmax + row);
+      const float sx[4] = {most, most, most, most};
+      const float sw[4] = {p.w_absmax[n], p.w_absmax[n + 1], p.w_absmax[n + 2], p.w_absmax[n + 3]};
 #pragma unroll
       for (int r = 0; r < kMaxSplits; ++r)
         if (r < splits) sum.x += v[r].x, sum.y += v[r].y, sum.z += v[r].z, sum.w += v[r].w;
+      const int sums[4] = {sum.x, sum.y, sum.z, sum.w};
+      float out[4];
+      scaled(sums, sx, sw, add, out);
       alignas(16) T o[4];
-      o[0] = from_float<T>(value(sum.x, sx, n) + add[0]);
-      o[1] = from_float<T>(value(sum.y, sx, n + 1) + add[1]);
-      o[2] = from_float<T>(value(sum.z, sx, n + 2) + add[2]);
-      o[3] = from_float<T>(value(sum.w, sx, n + 3) + add[3]);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) o[k] = from_float<T>(out[k]);
       if (sizeof(T) == 4) *reinterpret_cast<uint4*>(y + row * p.N + n) = *reinterpret_cast<uint4*>(o);
       else *reinterpret_cast<uint2*>(y + row * p.N + n) = *reinterpret_cast<uint2*>(o);
     }
   } else if (n0 + static_cast<int>(threadIdx.x) < p.N) {  // one channel a thread, four tokens at a time
     const int n = n0 + threadIdx.x;
+    const float most_n = p.w_absmax[n];
     constexpr int U = 4;
     for (int tok = piece * U; tok < tokens; tok += splits * U) {
-      int v[U][kMaxSplits];
-      float add[U], sx[U];
+      int v[U][kMaxSplits], sum[U];
+      float add[U], sx[U], sw[U], out[U];
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         const long long row = m0 + min(tok + u, tokens - 1);
@@ -636,16 +687,20 @@ __global__ void __launch_bounds__(kFewThreads)
         for (int r = 0; r < kMaxSplits; ++r)
           if (r < splits) v[u][r] = remote_int(s_sums + (tok + u) * 128 + threadIdx.x, r);
         add[u] = residual != nullptr ? to_float(residual[row * p.ld_res + n]) : 0.f;
-        sx[u] = ld_chained(p.x_absmax + row) * (1.f / 127.f);
+        sx[u] = ld_chained(p.x_absmax + row);
+        sw[u] = most_n;
       }
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        int sum = 0;
+        sum[u] = 0;
 #pragma unroll
         for (int r = 0; r < kMaxSplits; ++r)
-          if (r < splits) sum += v[u][r];
-        if (tok + u < tokens) y[(m0 + tok + u) * static_cast<long long>(p.N) + n] = from_float<T>(value(sum, sx[u], n) + add[u]);
+          if (r < splits) sum[u] += v[u][r];
       }
+      scaled(sum, sx, sw, add, out);
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (tok + u < tokens) y[(m0 + tok + u) * static_cast<long long>(p.N) + n] = from_float<T>(out[u]);
     }
   }
   cluster_sync_all();  // nobody leaves while others read its sums
@@ -725,7 +780,7 @@ __global__ void __launch_bounds__(kOneThreads)
 #pragma unroll
     for (int i = 0; i < kOneWarps; ++i) most[r] = max(most[r], s_most[r][i]);
     const float a = __uint_as_float(most[r]);
-    scale[r] = a * (1.f / 127.f);
+    scale[r] = a;
     {
       const Coder code(127.f, a);
       auto of = [&](T v) { return code.template of<sizeof(T) == 2>(to_float(v)); };
@@ -783,8 +838,9 @@ __global__ void __launch_bounds__(kOneThreads)
         const int all = __reduce_add_sync(0xffffffffu, sum[r][c]), n = n0 + c;
         if (lane == r * C + c && n < p.N) {
           const float add = p.residual != nullptr ? to_float(static_cast<const T*>(p.residual)[r * p.ld_res + n]) : 0.f;
-          static_cast<T*>(p.y)[r * static_cast<long long>(p.N) + n] =
-              from_float<T>(static_cast<float>(all) * scale[r] * (p.w_absmax[n] * (1.f / 127.f)) + add);
+          float out[1];
+          scaled({all}, {scale[r]}, {p.w_absmax[n]}, {add}, out);
+          static_cast<T*>(p.y)[r * static_cast<long long>(p.N) + n] = from_float<T>(out[0]);
         }
       }
   }

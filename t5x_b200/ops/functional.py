@@ -273,8 +273,9 @@ def quantize_weight(weight: torch.Tensor) -> Weight8:
 
 def linear8(x: torch.Tensor, weight: Weight8, residual: Optional[torch.Tensor] = None) -> torch.Tensor:
   """y = x @ W (+ residual) in 8-bit integers: x [..., in] is scaled by its rows' largest values, W by its channels', the
-  products are added exactly and the sum is rounded once, to x's type. A row with a value that is not finite is NaN. For
-  serving: there is no backward pass."""
+  products are added exactly. Scales and the residual go on in 32 bits (eight roundings, 2^-21 of the product's and the sum's
+  sizes at most), then comes the rounding to x's type. A row with a value that is not finite is NaN. For serving: there is no
+  backward pass."""
   codes, absmax, k = weight
   if x.is_cuda and not _transformed():
     host = native.host()
