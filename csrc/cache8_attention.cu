@@ -52,7 +52,7 @@ __device__ __forceinline__ void lay_query(const Cache8Attn& p, int b, int h, int
   constexpr int CH = D / 64, Q2 = kTwo ? 2 : 1, E = 16 / sizeof(T);
   const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int dropped = p.c.position != nullptr ? p.c.dropped[b] : 0;
-  const int q_first = static_cast<int>(static_cast<long long>(start) + p.appended - p.count);
+  const int q_first = static_cast<int>(static_cast<long long>(start) + p.appended - p.from_end);
   {
     const int r = kFold ? g & 3 : g, i = token_of(p, min(r, p.rows - 1)), in_group = min(r, p.rows - 1) - i * p.group;
     const T* src = static_cast<const T*>(p.q) + b * p.q_sb + i * p.q_st + (h * p.group + in_group) * p.q_sh + 16 * t;
@@ -808,35 +808,53 @@ cudaError_t launch_pieces(const Cache8Attn& p, bool behind, cudaStream_t stream)
                        kWeightThreads, 0, stream, p);
 }
 
-// Rows `from` on of a cache.
-Cache8 rows_of(Cache8 c, int from, int count) {
-  const long long by_head = static_cast<long long>(from) * c.heads;
+// What a launch has of a call: batch rows, key heads and queries.
+struct Part {
+  int row, rows, head, heads, query, queries;
+};
+
+// That part of a cache. (Of several rows it has all heads.)
+Cache8 cache_of(Cache8 c, const Part& at) {
+  const long long by_head = static_cast<long long>(at.row) * c.heads + at.head;
   for (int i = 0; i < 2; ++i) {
     c.codes[i] += by_head * c.slots * c.dim;
     c.absmax[i] += by_head * (c.slots >> c.block_log2);
   }
-  c.index += static_cast<long long>(from) * c.index_stride;
+  c.index += static_cast<long long>(at.row) * c.index_stride;
   if (c.weight) c.weight += by_head * c.slots;
-  if (c.position) c.position += by_head * c.slots, c.dropped += from;
-  c.batch = count;
+  if (c.position) c.position += by_head * c.slots, c.dropped += at.row;
+  c.batch = at.rows;
+  c.heads = at.heads;
   return c;
 }
 
-// Rows of a launch: no more scores than a gigabyte where weights are added up (a launch of that many fills the SMs for long).
-int rows_at_a_time(const Cache8& c, int rows) {
-  long long most = kMaxBatch;
-  if (c.weight != nullptr) most = std::min(most, (1LL << 28) / (static_cast<long long>(c.heads) * rows * c.slots));
-  return static_cast<int>(std::min<long long>(c.batch, std::max(most, 1LL)));
+// The launches of a call, by f(part) until one is false. Where weights are added up a launch has no more scores than a gigabyte
+// (which fills the SMs for long), or those of one query of one head: several rows, or several heads of a row, or several queries of
+// a head.
+constexpr long long kMaxScores = 1LL << 28;
+template <typename F>
+bool for_parts(const Cache8& c, int count, int group, F&& f) {
+  int rows = kMaxBatch, heads = c.heads, queries = count;
+  if (c.weight != nullptr) {
+    const long long each = static_cast<long long>(group) * c.slots;  // scores of a query
+    auto fitting = [](long long most) { return static_cast<int>(std::max(1LL, std::min<long long>(most, kMaxBatch))); };
+    rows = fitting(kMaxScores / (each * count * c.heads));
+    if (each * count * c.heads > kMaxScores) heads = std::min(heads, fitting(kMaxScores / (each * count)));
+    if (each * count > kMaxScores) queries = std::min(queries, fitting(kMaxScores / each));
+  }
+  for (int r = 0; r < c.batch; r += rows)
+    for (int h = 0; h < c.heads; h += heads)
+      for (int q = 0; q < count; q += queries)
+        if (!f(Part{r, std::min(rows, c.batch - r), h, std::min(heads, c.heads - h), q, std::min(queries, count - q)})) return false;
+  return true;
 }
 
 struct Plan {
   int pieces = 0, least = 0, entry = 0, row_warps = 1;
   size_t part = 0, stats = 0, first = 0, scores = 0, final_stats = 0, total = 0;
 };
-Plan plan(Cache8 c, int rows, int type) {
+Plan plan(const Cache8& c, int rows, int type) {
   Plan w = {};
-  if (by_row_head(c, rows)) return w;
-  c.batch = rows_at_a_time(c, rows);
   const int tile_rows = rows <= 8 ? 8 : row_tile_of(type, rows), row_tiles = (rows + tile_rows - 1) / tile_rows;
   // Pieces for all CTAs that the SMs hold at a time, none of under 64 tokens a warp; over many rows, where a CTA has its steps of
   // 64 tokens to itself, none of under one (8 heads of 128 channels over 512 slots, 64 rows: 16.7 us, 18.3 with two steps, 25.1
@@ -896,7 +914,13 @@ T5X_API long long t5x_cache8_attention_bytes(const T5xCache8* cache, const T5xCa
   if (int e = t5x::check_cache8("cache8_attention", c)) return e;
   if (int e = t5x::check_query(c, q, n)) return e;
   if (c.batch == 0) return 0;
-  return static_cast<long long>(t5x::plan(c, q->count * q->group, q->type).total);
+  if (t5x::by_row_head(c, q->count * q->group)) return 0;
+  size_t most = 0;  // (the launches have the same workspace, one after the other)
+  t5x::for_parts(c, q->count, q->group, [&](const t5x::Part& at) {
+    most = std::max(most, t5x::plan(t5x::cache_of(c, at), at.queries * q->group, q->type).total);
+    return true;
+  });
+  return static_cast<long long>(most);
 }
 
 T5X_API int t5x_cache8_attention(const T5xCache8* cache, const T5xCache8Query* q, const T5xNewTokens* n, void* workspace,
@@ -922,6 +946,8 @@ T5X_API int t5x_cache8_attention(const T5xCache8* cache, const T5xCache8Query* q
   p.count = q->count;
   p.group = q->group;
   p.rows = q->count * q->group;
+  p.from_end = q->count;
+  p.out_heads = c.heads;
   p.by_group = ((1ull << 32) + q->group - 1) / q->group;
   p.distances = q->table ? q->distances : 0;
   if (q->table) std::copy_n(q->buckets, q->distances, p.buckets);
@@ -930,7 +956,6 @@ T5X_API int t5x_cache8_attention(const T5xCache8* cache, const T5xCache8Query* q
   p.appended = n ? n->count : 0;
   p.scale = q->scale;
   p.low = 0x00ff00ffu;
-  const t5x::Plan w = t5x::plan(c, p.rows, q->type);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (t5x::by_row_head(c, p.rows)) {
     p.scores = nullptr;
@@ -942,31 +967,38 @@ T5X_API int t5x_cache8_attention(const T5xCache8* cache, const T5xCache8Query* q
   if (!workspace || !t5x::aligned_to(16, {workspace}))
     return t5x::set_error("cache8_attention: a null or misaligned workspace");
   uint8_t* ws = static_cast<uint8_t*>(workspace);
-  p.pieces = w.pieces;
-  p.row_warps = w.row_warps;
-  p.least = w.least;
-  p.entry = w.entry;
-  p.part = reinterpret_cast<float*>(ws + w.part);
-  p.stats = reinterpret_cast<float2*>(ws + w.stats);
-  p.first = reinterpret_cast<long long*>(ws + w.first);
-  p.scores = c.weight ? reinterpret_cast<float*>(ws + w.scores) : nullptr;
-  p.final_stats = reinterpret_cast<float2*>(ws + w.final_stats);
   if (n)
     if (int e = t5x::cache8_append(c, n, st)) return e;
   const int size = q->type == 2 ? 4 : 2;
-  const int each = t5x::rows_at_a_time(c, p.rows);
-  for (int from = 0; from < c.batch; from += each) {
+  bool behind = n != nullptr;  // (what follows the append alone may begin while it runs)
+  cudaError_t e = cudaSuccess;
+  t5x::for_parts(c, q->count, q->group, [&](const t5x::Part& at) {
     t5x::Cache8Attn part = p;
-    part.c = t5x::rows_of(c, from, std::min(c.batch - from, each));
-    part.q = static_cast<const char*>(p.q) + from * p.q_sb * size;
-    part.out = static_cast<char*>(p.out) + static_cast<long long>(from) * p.rows * c.heads * c.dim * size;
-    part.mask = p.mask ? p.mask + from * p.mask_stride : nullptr;
-    // (what follows the append alone may begin while it runs; the workspace of a launch is the next one's)
-    const bool behind = n != nullptr && from == 0;
-    const cudaError_t e = q->type == 0   ? t5x::launch_pieces<__nv_bfloat16, false>(part, behind, st)
-                          : q->type == 1 ? t5x::launch_pieces<__half, false>(part, behind, st)
-                                         : t5x::launch_pieces<float, true>(part, behind, st);
-    if (e != cudaSuccess) return t5x::set_error("cache8_attention launch: %s", cudaGetErrorString(e));
-  }
-  return 0;
+    part.c = t5x::cache_of(c, at);
+    part.count = at.queries;
+    part.rows = at.queries * q->group;
+    part.from_end = q->count - at.query;
+    const long long head = static_cast<long long>(at.head) * q->group;
+    part.q = static_cast<const char*>(p.q) + (at.row * p.q_sb + at.query * p.q_st + head * p.q_sh) * size;
+    part.out = static_cast<char*>(p.out) +
+               ((static_cast<long long>(at.row) * q->count + at.query) * c.heads * q->group + head) * c.dim * size;
+    part.table = p.table ? p.table + head * p.table_stride : nullptr;
+    part.mask = p.mask ? p.mask + at.row * p.mask_stride : nullptr;
+    const t5x::Plan w = t5x::plan(part.c, part.rows, q->type);
+    part.pieces = w.pieces;
+    part.row_warps = w.row_warps;
+    part.least = w.least;
+    part.entry = w.entry;
+    part.part = reinterpret_cast<float*>(ws + w.part);
+    part.stats = reinterpret_cast<float2*>(ws + w.stats);
+    part.first = reinterpret_cast<long long*>(ws + w.first);
+    part.scores = c.weight ? reinterpret_cast<float*>(ws + w.scores) : nullptr;
+    part.final_stats = reinterpret_cast<float2*>(ws + w.final_stats);
+    e = q->type == 0   ? t5x::launch_pieces<__nv_bfloat16, false>(part, behind, st)
+        : q->type == 1 ? t5x::launch_pieces<__half, false>(part, behind, st)
+                       : t5x::launch_pieces<float, true>(part, behind, st);
+    behind = false;
+    return e == cudaSuccess;
+  });
+  return e == cudaSuccess ? 0 : t5x::set_error("cache8_attention launch: %s", cudaGetErrorString(e));
 }

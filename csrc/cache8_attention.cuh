@@ -24,6 +24,8 @@ struct Cache8Attn {
   long long q_sb, q_st, q_sh, mask_stride;
   int table_stride, q_vec;  // q_vec: whole 16 bytes of a query may be loaded
   int count, group, rows;  // queries a row, heads a key head, their product
+  int from_end;            // the first query's place, counted from the end of the tokens held: `count`, but for a part of them
+  int out_heads;           // key heads of `out`, of which a launch may have a part
   int distances, mask_len, causal;
   int appended;            // tokens of this call behind c.index
   float scale;
@@ -171,8 +173,7 @@ __device__ __forceinline__ int token_of(const Cache8Attn& p, int r) { return sta
 __device__ __forceinline__ int last_seen(const Cache8Attn& p, int start, int end, int r) {
   if (r >= p.rows) return -1;
   if (!p.causal) return end - 1;
-  // the queries are the last `count` tokens held
-  const long long first = static_cast<long long>(start) + p.appended - p.count;
+  const long long first = static_cast<long long>(start) + p.appended - p.from_end;
   return static_cast<int>(min(first + token_of(p, r), static_cast<long long>(end) - 1));
 }
 __device__ __forceinline__ int end_of(const Cache8Attn& p, int start) {
@@ -182,7 +183,7 @@ template <typename T>
 __device__ __forceinline__ T* out_row(const Cache8Attn& p, int b, int h, int r) {
   const int tok = token_of(p, r);
   return static_cast<T*>(p.out) +
-         ((static_cast<long long>(b) * p.count + tok) * p.c.heads * p.group + h * p.group + r - tok * p.group) * p.c.dim;
+         ((static_cast<long long>(b) * p.count + tok) * p.out_heads * p.group + h * p.group + r - tok * p.group) * p.c.dim;
 }
 
 // s_first[b]: what all heads of the rows in front of b cost; s_first[batch]: all.

@@ -55,7 +55,7 @@ __device__ __forceinline__ void lay_rows(const Cache8Attn& p, int b, int h, int 
   constexpr int J = D / 16;
   const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int dropped = p.c.position != nullptr ? p.c.dropped[b] : 0;
-  const int q_first = static_cast<int>(static_cast<long long>(start) + p.appended - p.count);
+  const int q_first = static_cast<int>(static_cast<long long>(start) + p.appended - p.from_end);
   uint32_t* to = reinterpret_cast<uint32_t*>(s_query);
   using Pair = typename std::conditional<sizeof(T) == 4, uint2, uint32_t>::type;
   Pair part[2 * M][J][2];  // channels 16 j + 2 t, + 1, + 8, + 9 of row 8 i + g

@@ -581,3 +581,40 @@ def test_threads():
   for t in threads:
     t.join()
   assert len(got) == 4 and all(torch.equal(a, b) for one in got.values() for a, b in zip(one, want))
+
+
+@pytest.mark.parametrize("heads,group,count,slots,own", [(5, 8, 300, 32768, False), (2, 8, 1100, 32768, False), (1, 3, 20000, 8208, True)])
+def test_one_row_of_more_scores_than_a_launch_takes(heads, group, count, slots, own):
+  """Heads, or queries of a head, go in several launches: with the results and weights of one, and a gigabyte of workspace."""
+  dim, held = 64, slots - count - 5
+  cache = plain.make(1, heads, slots, dim, 16, [held + count if own else held], weights=True, positions=True, device="cuda")
+  gen = torch.Generator("cuda").manual_seed(0)
+  randn = lambda *s: torch.randn(*s, generator=gen, device="cuda").bfloat16()  # noqa: E731
+  query, table = randn(1, count, heads * group, dim) / 4, torch.randn(heads * group, 32, generator=gen, device="cuda")
+  key, value = (None, None) if own else (randn(1, count, heads, dim), randn(1, count, heads, dim))
+  shown = torch.rand(1, slots, generator=gen, device="cuda") > 0.2
+  before = cache["token_weight"].double()
+  torch.cuda.synchronize()
+  start = torch.cuda.memory_allocated()
+  torch.cuda.reset_peak_memory_stats()
+  out = launches(lambda: cache8.attention(query, cache, key, value, bias_table=table, key_mask=shown))
+  assert torch.cuda.max_memory_allocated() - start < 1.25 * 2 ** 30
+  before[:, :, held:held + count] *= own
+  added = torch.zeros_like(before)
+  values = {n: ref.cache8_values(cache, n, torch.float64) for n in ("key", "value")}
+  slot = torch.arange(slots, device="cuda")
+  for i in range(0, count, 500):  # in 64 bits
+    for h in range(heads):
+      q = query[0, i:i + 500, h * group:(h + 1) * group].double()
+      s = torch.einsum("lgd,sd->gls", q, values["key"][0, h])
+      own_at = held + i + torch.arange(q.shape[0], device="cuda")
+      back = cache["token_position"][0, h].long() - (own_at + cache["dropped"].long())[:, None]
+      s += table[h * group:(h + 1) * group].double()[:, ref.relative_position_bucket(back, False, 32, 128)]
+      s.masked_fill_((slot > own_at[:, None]) | ~shown, -math.inf)
+      p = torch.softmax(s, 2).nan_to_num()  # (queries in front of all that is held see nothing)
+      added[0, h] += p.sum((0, 1))
+      want = torch.einsum("gls,sd->lgd", p, values["value"][0, h])
+      # |v| is at most 3; a score's products are below 2^6
+      size = torch.full_like(want, 3.0)
+      assert plain.within(out[0, i:i + 500, h * group:(h + 1) * group], want.cpu(), size.cpu(), 64.0, dim, slots)
+  assert torch.allclose(cache["token_weight"].double(), before + added, rtol=1e-4, atol=1e-6)
