@@ -837,10 +837,12 @@ bool for_parts(const Cache8& c, int count, int group, F&& f) {
   int rows = kMaxBatch, heads = c.heads, queries = count;
   if (c.weight != nullptr) {
     const long long each = static_cast<long long>(group) * c.slots;  // scores of a query
-    auto fitting = [](long long most) { return static_cast<int>(std::max(1LL, std::min<long long>(most, kMaxBatch))); };
-    rows = fitting(kMaxScores / (each * count * c.heads));
-    if (each * count * c.heads > kMaxScores) heads = std::min(heads, fitting(kMaxScores / (each * count)));
-    if (each * count > kMaxScores) queries = std::min(queries, fitting(kMaxScores / each));
+    auto at_most = [&](int all, long long scores) {  // as many of them, of so many scores each, as fit
+      return static_cast<int>(std::min<long long>(all, std::max(1LL, kMaxScores / scores)));
+    };
+    rows = at_most(kMaxBatch, each * count * c.heads);
+    heads = at_most(c.heads, each * count);
+    queries = at_most(count, each);
   }
   for (int r = 0; r < c.batch; r += rows)
     for (int h = 0; h < c.heads; h += heads)
