@@ -120,7 +120,6 @@ template <typename T, int D, int MT, bool kTwo, Deal kDeal, int kWarps, bool kFo
 __global__ void __launch_bounds__(kWarps * 32, 16 / kWarps)
     cache8_attention_kernel(const __grid_constant__ Cache8Attn p, const __grid_constant__ NewTokens<T> fresh) {
   constexpr bool kBlock = kDeal == kRowHead;
-  constexpr int NT = 1;  // tiles of 8 query rows
   static_assert(!kFold || MT == 2, "two tiles fold");
   constexpr int MS = kFold ? 1 : MT;           // tiles of scores that a lane has
   constexpr int kParts = kFold ? 2 : 1;        // columns of a query row
@@ -130,7 +129,7 @@ __global__ void __launch_bounds__(kWarps * 32, 16 / kWarps)
   constexpr int MI = D / 16;       // row tiles of the second product
   constexpr int Q2 = kTwo ? 2 : 1;
   constexpr bool kQueryRegs = D == 64;  // the query's operand is kept in registers
-  constexpr int kQuery = Q2 * NT * CH * 4 * 32;
+  constexpr int kQuery = Q2 * CH * 4 * 32;
   // the query's operand; the bias table, times log2 e (kRowHead: of the head's rows); the sums
   // of the warps [kWarps][rows][D]; kRowHead: scores [rows][slots]
   extern __shared__ uint2 s_dyn[];
@@ -336,34 +335,27 @@ __global__ void __launch_bounds__(kWarps * 32, 16 / kWarps)
         for (int j = 0; j < CH * 4; ++j) qf[w][j] = s_query[(w * CH * 4 + j) * 32 + lane];
     }
     const Column cols[2] = {s_cols[2 * t], s_cols[2 * t + 1]};
-    auto column = [&](int, int e) -> const Column& { return cols[e]; };
     int all_see = end - 1;  // slots up to this one are seen by every row of the tile
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt) all_see = min(all_see, min(column(nt, 0).lim, column(nt, 1).lim));
+    all_see = min(all_see, min(cols[0].lim, cols[1].lim));
     all_see = __reduce_min_sync(0xffffffffu, all_see);
 
-    float o[NT][MI][4];
-    Reference ref[NT][2];
-    float l[NT][2];
+    float o[MI][4];
+    Reference ref[2];
+    float l[2];
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
+    for (int i = 0; i < MI; ++i)
 #pragma unroll
-      for (int i = 0; i < MI; ++i)
+      for (int k = 0; k < 4; ++k) o[i][k] = 0.f;
 #pragma unroll
-        for (int k = 0; k < 4; ++k) o[nt][i][k] = 0.f;
-#pragma unroll
-      for (int e = 0; e < 2; ++e) ref[nt][e] = {kNothing, 1.f}, l[nt][e] = 0.f;
-    }
+    for (int e = 0; e < 2; ++e) ref[e] = {kNothing, 1.f}, l[e] = 0.f;
 
     for (int tile = mine; tile < tile1; tile += kStep) {
       // ---- S^T = K Q^T ----
-      float st[MT][NT][4];
+      float st[MT][4];
 #pragma unroll
       for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-          for (int k = 0; k < 4; ++k) st[mt][nt][k] = 0.f;
+        for (int k = 0; k < 4; ++k) st[mt][k] = 0.f;
 #pragma unroll
       for (int ch = 0; ch < CH; ++ch)
 #pragma unroll
@@ -377,30 +369,25 @@ __global__ void __launch_bounds__(kWarps * 32, 16 / kWarps)
               a[mt][e] = number_pair(w, low);
               a[mt][2 + e] = number_pair(w >> 8, low);
             }
+          uint32_t q0[Q2], q1[Q2];
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt) {
-            uint32_t q0[Q2], q1[Q2];
-#pragma unroll
-            for (int w = 0; w < Q2; ++w) {
-              uint2 q;
-              if constexpr (kQueryRegs) q = qf[w][ch * 4 + j];
-              else q = s_query[(w * CH * 4 + ch * 4 + j) * 32 + lane];
-              q0[w] = q.x, q1[w] = q.y;
-            }
-#pragma unroll
-            for (int mt = 0; mt < MT; ++mt) mma_sum<Q2>(st[mt][nt], a[mt], q0, q1);
+          for (int w = 0; w < Q2; ++w) {
+            uint2 q;
+            if constexpr (kQueryRegs) q = qf[w][ch * 4 + j];
+            else q = s_query[(w * CH * 4 + ch * 4 + j) * 32 + lane];
+            q0[w] = q.x, q1[w] = q.y;
           }
+#pragma unroll
+          for (int mt = 0; mt < MT; ++mt) mma_sum<Q2>(st[mt], a[mt], q0, q1);
         }
-      float s[MS][NT][4], k_scale[MS];
+      float s[MS][4], k_scale[MS];
       int here[MS][2];  // positions of tokens g and g + 8
 #pragma unroll
       for (int ms = 0; ms < MS; ++ms) {
         k_scale[ms] = ka[ms];
         here[ms][0] = place[ms][0], here[ms][1] = place[ms][1];
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-          for (int k = 0; k < 4; ++k) s[ms][nt][k] = kFold && fold ? st[MT - 1][nt][k] : st[ms][nt][k];
+        for (int k = 0; k < 4; ++k) s[ms][k] = kFold && fold ? st[MT - 1][k] : st[ms][k];
       }
       if (tile + kStep < tile1) load_k(tile + kStep);
 
@@ -410,23 +397,18 @@ __global__ void __launch_bounds__(kWarps * 32, 16 / kWarps)
         const int s0 = (tile + ms + fold) << 4;
         const bool inside = tile + ms + fold < tile1;
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const float by = k_scale[ms] * column(nt, e).scale;
-            s[ms][nt][e] *= by;
-            s[ms][nt][2 + e] *= by;
-          }
+        for (int e = 0; e < 2; ++e) {
+          const float by = k_scale[ms] * cols[e].scale;
+          s[ms][e] *= by;
+          s[ms][2 + e] *= by;
         }
         if (p.table != nullptr) {
           if (!placed) here[ms][0] = s0 + g, here[ms][1] = s0 + g + 8;
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              const int d = column(nt, k & 1).where - here[ms][k >> 1];
-              s[ms][nt][k] += s_table[column(nt, k & 1).bias + s_buckets[min(max(d, 0), p.distances - 1)]];
-            }
+          for (int k = 0; k < 4; ++k) {
+            const int d = cols[k & 1].where - here[ms][k >> 1];
+            s[ms][k] += s_table[cols[k & 1].bias + s_buckets[min(max(d, 0), p.distances - 1)]];
+          }
         }
         const int last = tile + (kFold ? MT : ms + 1);  // of the step's tiles that are looked at here, and one
         if (!(last <= tile1 && last * 16 - 1 <= all_see && mask == nullptr)) {
@@ -436,23 +418,19 @@ __global__ void __launch_bounds__(kWarps * 32, 16 / kWarps)
             for (int e = 0; e < 2; ++e) shown[e] = inside && s0 + g + 8 * e < p.mask_len && mask[s0 + g + 8 * e] != 0;
           }
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-            for (int k = 0; k < 4; ++k)
-              if (!shown[k >> 1] || s0 + g + 8 * (k >> 1) > column(nt, k & 1).lim) s[ms][nt][k] = -INFINITY;
+          for (int k = 0; k < 4; ++k)
+            if (!shown[k >> 1] || s0 + g + 8 * (k >> 1) > cols[k & 1].lim) s[ms][k] = -INFINITY;
         }
         if ((kBlock ? c.weight != nullptr : p.scores != nullptr) && inside) {
           float* to = kBlock ? s_scores : p.scores + bh * p.rows * c.slots;
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              const int r = kFold ? (2 * t + e) & 3 : 2 * t + e;
-              if (r < p.rows) {
-                to[r * c.slots + s0 + g] = s[ms][nt][e];
-                to[r * c.slots + s0 + g + 8] = s[ms][nt][2 + e];
-              }
+          for (int e = 0; e < 2; ++e) {
+            const int r = kFold ? (2 * t + e) & 3 : 2 * t + e;
+            if (r < p.rows) {
+              to[r * c.slots + s0 + g] = s[ms][e];
+              to[r * c.slots + s0 + g + 8] = s[ms][2 + e];
             }
+          }
         }
       }
 
@@ -462,82 +440,76 @@ __global__ void __launch_bounds__(kWarps * 32, 16 / kWarps)
       for (int ms = 1; ms < MS; ++ms) most = fmaxf(most, va[ms]);
       bool raise = false;
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
+      for (int e = 0; e < 2; ++e) {
+        float top = -INFINITY;
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          float top = -INFINITY;
-#pragma unroll
-          for (int ms = 0; ms < MS; ++ms) top = fmaxf(top, fmaxf(s[ms][nt][e], s[ms][nt][2 + e]));
-          raise |= beyond(ref[nt][e], top, most * ref[nt][e].by);
-        }
+        for (int ms = 0; ms < MS; ++ms) top = fmaxf(top, fmaxf(s[ms][e], s[ms][2 + e]));
+        raise |= beyond(ref[e], top, most * ref[e].by);
+      }
       if (__any_sync(0xffffffffu, raise)) {
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
+        for (int e = 0; e < 2; ++e) {
+          float x = -INFINITY, x2 = -INFINITY;
 #pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            float x = -INFINITY, x2 = -INFINITY;
-#pragma unroll
-            for (int ms = 0; ms < MS; ++ms) {
-              const float high = fmaxf(s[ms][nt][e], s[ms][nt][2 + e]);
-              x = fmaxf(x, high);
-              x2 = fmaxf(x2, high + log2_approx(va[ms]));
-            }
-#pragma unroll
-            for (int lanes = 4; lanes < 32; lanes *= 2) {
-              x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, lanes));
-              x2 = fmaxf(x2, __shfl_xor_sync(0xffffffffu, x2, lanes));
-            }
-            const float2 by = raise_to(ref[nt][e], x, x2);
-            l[nt][e] *= by.x;
-#pragma unroll
-            for (int i = 0; i < MI; ++i) o[nt][i][e] *= by.y, o[nt][i][2 + e] *= by.y;
+          for (int ms = 0; ms < MS; ++ms) {
+            const float high = fmaxf(s[ms][e], s[ms][2 + e]);
+            x = fmaxf(x, high);
+            x2 = fmaxf(x2, high + log2_approx(va[ms]));
           }
+#pragma unroll
+          for (int lanes = 4; lanes < 32; lanes *= 2) {
+            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, lanes));
+            x2 = fmaxf(x2, __shfl_xor_sync(0xffffffffu, x2, lanes));
+          }
+          const float2 by = raise_to(ref[e], x, x2);
+          l[e] *= by.x;
+#pragma unroll
+          for (int i = 0; i < MI; ++i) o[i][e] *= by.y, o[i][2 + e] *= by.y;
+        }
       }
 
       // ---- probabilities ----
-      uint32_t pf[Q2][MT][NT][2];
+      uint32_t pf[Q2][MT][2];
 #pragma unroll
-      for (int ms = 0; ms < MS; ++ms)
+      for (int ms = 0; ms < MS; ++ms) {
+        float r[2] = {va[ms] * ref[0].by, va[ms] * ref[1].by};
+        float counts = 1.f;  // in the sum that divides
+        if (!(fmaxf(r[0], r[1]) < kFar)) {
+          counts = 0.f;
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          float r[2] = {va[ms] * ref[nt][0].by, va[ms] * ref[nt][1].by};
-          float counts = 1.f;  // in the sum that divides
-          if (!(fmaxf(r[0], r[1]) < kFar)) {
-            counts = 0.f;
+          for (int e = 0; e < 2; ++e) {
+            const float2 part = part_of(ref[e], va[ms]);
+            r[e] = part.x;
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              const float2 part = part_of(ref[nt][e], va[ms]);
-              r[e] = part.x;
-#pragma unroll
-              for (int k = e; k < 4; k += 2) {
-                l[nt][e] += exp2_approx(s[ms][nt][k] - ref[nt][e].score);
-                s[ms][nt][k] = far_score(s[ms][nt][k], part.y, va[ms]);
-              }
+            for (int k = e; k < 4; k += 2) {
+              l[e] += exp2_approx(s[ms][k] - ref[e].score);
+              s[ms][k] = far_score(s[ms][k], part.y, va[ms]);
             }
           }
-          float pr[4];
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            pr[k] = exp2_approx(s[ms][nt][k] - ref[nt][k & 1].score);
-            l[nt][k & 1] += pr[k] * counts;
-            pr[k] *= r[k & 1];
-          }
-          const __half2 v0 = __floats2half2_rn(pr[0], pr[1]), v1 = __floats2half2_rn(pr[2], pr[3]);
-          uint32_t f[Q2][2];
-          f[0][0] = as_u32(v0), f[0][1] = as_u32(v1);
-          if (kTwo) {
-            f[Q2 - 1][0] = rest_of(pr[0], pr[1], v0);
-            f[Q2 - 1][1] = rest_of(pr[2], pr[3], v1);
-          }
-#pragma unroll
-          for (int w = 0; w < Q2; ++w)
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              const uint32_t turned = transposed(f[w][e]);  // (column g now)
-              if constexpr (kFold) pf[w][0][nt][e] = g < 4 ? turned : 0u, pf[w][1][nt][e] = g < 4 ? 0u : turned;
-              else pf[w][ms][nt][e] = turned;
-            }
         }
+        float pr[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          pr[k] = exp2_approx(s[ms][k] - ref[k & 1].score);
+          l[k & 1] += pr[k] * counts;
+          pr[k] *= r[k & 1];
+        }
+        const __half2 v0 = __floats2half2_rn(pr[0], pr[1]), v1 = __floats2half2_rn(pr[2], pr[3]);
+        uint32_t f[Q2][2];
+        f[0][0] = as_u32(v0), f[0][1] = as_u32(v1);
+        if (kTwo) {
+          f[Q2 - 1][0] = rest_of(pr[0], pr[1], v0);
+          f[Q2 - 1][1] = rest_of(pr[2], pr[3], v1);
+        }
+#pragma unroll
+        for (int w = 0; w < Q2; ++w)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const uint32_t turned = transposed(f[w][e]);  // (column g now)
+            if constexpr (kFold) pf[w][0][e] = g < 4 ? turned : 0u, pf[w][1][e] = g < 4 ? 0u : turned;
+            else pf[w][ms][e] = turned;
+          }
+      }
 
       // ---- O^T += V^T P^T ----
 #pragma unroll
@@ -549,13 +521,10 @@ __global__ void __launch_bounds__(kWarps * 32, 16 / kWarps)
             const uint32_t x = __byte_perm(vr[mt][0][w], vr[mt][1][w], half ? 0x7632 : 0x5410);
             const uint32_t y = __byte_perm(vr[mt][2][w], vr[mt][3][w], half ? 0x7632 : 0x5410);
             const uint32_t a[4] = {number_pair(x, low), number_pair(x >> 8, low), number_pair(y, low), number_pair(y >> 8, low)};
+            uint32_t p0[Q2], p1[Q2];
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-              uint32_t p0[Q2], p1[Q2];
-#pragma unroll
-              for (int q2 = 0; q2 < Q2; ++q2) p0[q2] = pf[q2][mt][nt][0], p1[q2] = pf[q2][mt][nt][1];
-              mma_sum<Q2, true>(o[nt][2 * w + half], a, p0, p1);
-            }
+            for (int q2 = 0; q2 < Q2; ++q2) p0[q2] = pf[q2][mt][0], p1[q2] = pf[q2][mt][1];
+            mma_sum<Q2, true>(o[2 * w + half], a, p0, p1);
           }
       if (tile + kStep < tile1) load_v(tile + kStep);
     }
@@ -577,19 +546,19 @@ __global__ void __launch_bounds__(kWarps * 32, 16 / kWarps)
       }
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        float sum = l[0][e];
+        float sum = l[e];
         sum += __shfl_xor_sync(0xffffffffu, sum, 4);
         sum += __shfl_xor_sync(0xffffffffu, sum, 8);
         sum += __shfl_xor_sync(0xffffffffu, sum, 16);
         const int r = kFold ? (2 * t + e) & 3 : 2 * t + e, part = wid * kParts + fold;
         if (r < p.rows) {
-          const float f = power_of_two(scale_of(ref[0][e])) * (1.f / 127.f);
+          const float f = power_of_two(scale_of(ref[e])) * (1.f / 127.f);
           float* dst = s_sums + (part * p.rows + r) * D + VB * g;
 #pragma unroll
           for (int i = 0; i < MI; i += 2)
-            *reinterpret_cast<float4*>(dst + 2 * i) = make_float4(o[0][i][e] * f, o[0][i][2 + e] * f, o[0][i + 1][e] * f,
-                                                                  o[0][i + 1][2 + e] * f);
-          if (g == 0) s_stats[part][r] = make_float2(ref[0][e].score, sum);
+            *reinterpret_cast<float4*>(dst + 2 * i) = make_float4(o[i][e] * f, o[i][2 + e] * f, o[i + 1][e] * f,
+                                                                  o[i + 1][2 + e] * f);
+          if (g == 0) s_stats[part][r] = make_float2(ref[e].score, sum);
         }
       }
       __syncthreads();
@@ -867,7 +836,7 @@ Plan plan(const Cache8& c, int rows, int type) {
   w.least = (rows <= 8 ? 32 : 4) + w.entry;
   long long room = 2LL * num_sms();
   if (rows > 8) {
-    w.row_warps = row_tiles > 4 ? kRowWarps : row_tiles > 2 || rows > kFewRows ? 4 : 2;
+    w.row_warps = row_tiles > 4 ? kRowWarps : row_tiles > 2 ? 4 : 2;
     room = num_sms() / ((row_tiles + w.row_warps - 1) / w.row_warps);
   }
   const long long most = static_cast<long long>(c.batch) * c.heads * (c.slots / 16 + w.entry) / w.least + 1;
