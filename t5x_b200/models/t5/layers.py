@@ -500,7 +500,11 @@ class MultiHeadDotProductAttention(nn.Module):
               beams_per_kv: int = 1) -> torch.Tensor:
     b, lq, _ = inputs_q.shape
     q_in = tp.copy_to_model_parallel(inputs_q)
+    untaken = [name for name, given in (("explicit_bias", explicit_bias), ("extra_mask", extra_mask), ("q_segment_ids", q_segment_ids),
+                                        ("kv_segment_ids", kv_segment_ids)) if given is not None]  # (of caches in 8 bits)
     if isinstance(precomputed_kv, dict):  # a cross attention's cache in 8 bits, shared by the beams of an example
+      if untaken or bias_table is not None or causal:
+        raise ValueError(f"a cross attention's cache in 8 bits takes a key_mask alone: {untaken or 'a bias table or causal'}")
       if self.scale_attn_logits:
         q_in = q_in / math.sqrt(self.head_dim)
       q = self.query(q_in).view(b // beams_per_kv, beams_per_kv * lq, self.local_heads, self.head_dim)
@@ -531,6 +535,8 @@ class MultiHeadDotProductAttention(nn.Module):
       bias = {} if bias_table is None else dict(bias_table=F.compute_weight(bias_table, torch.float32)[:self.local_heads],
                                                 num_buckets=num_buckets, max_distance=max_distance)
       if not prefill:
+        if untaken or key_mask is not None:
+          raise ValueError(f"a step over a cache in 8 bits sees what is held: {untaken or 'key_mask'}")
         return self._project_out(self._decode8(cache, q, k, v, bias), b, lq, residual)
       self._prefill8(cache, q, k, v, prefill_lengths, bias)
     elif cache is not None and prefill:

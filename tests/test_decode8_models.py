@@ -270,3 +270,22 @@ def test_a_projection_quantized_by_itself(name):
     F.linear8 = forward
   assert len(calls) == 1 and calls[0] is module.weight8.codes
   assert [torch.equal(a, b) for a, b in zip(got, plain)] == [hasattr(mlp, name), hasattr(attn, name)]
+
+
+@torch.no_grad()
+def test_masks_and_biases_that_a_cache_in_8_bits_does_not_take():
+  attn, table = attention_layer("cpu")
+  x, ids = torch.randn(2, 1, 64), torch.ones(2, 1, dtype=torch.long)
+  run = lambda **kw: attn(x, x, cache=attn.init_cache(2, 16, "cpu"), decode=True, bidirectional=False, **kw)  # noqa: E731
+  run(bias_table=table)
+  cross = attn.cross_cache(torch.randn(2, 7, 64))
+  over = lambda **kw: attn(x, None, precomputed_kv=cross, **kw)  # noqa: E731
+  over(key_mask=torch.ones(2, 7, dtype=torch.bool))
+  for kw in (dict(extra_mask=torch.ones(2, 1, 1, 1)), dict(explicit_bias=torch.ones(1, 2, 1, 1)), dict(q_segment_ids=ids),
+             dict(kv_segment_ids=ids)):
+    for call in (run, over):
+      with pytest.raises(ValueError, match=next(iter(kw))):
+        call(**kw)
+  for call in (lambda: run(key_mask=torch.ones(2, 16, dtype=torch.bool)), lambda: over(bias_table=table), lambda: over(causal=True)):
+    with pytest.raises(ValueError, match="8 bits"):
+      call()
