@@ -1182,6 +1182,8 @@ struct Cache8Of {
       return;
     const Tensor *weight = entry(dict, names.weight), *position = entry(dict, names.position),
                  *dropped = entry(dict, names.dropped);
+    auto strange = [&](const Tensor* t, PyObject* name) { return t == nullptr && PyDict_GetItem(dict, name) != nullptr; };
+    if (strange(weight, names.weight) || strange(position, names.position) || strange(dropped, names.dropped)) return;
     if ((weight != nullptr && !fit(weight, at::kFloat, {b, h, slots})) ||
         (position != nullptr && !fit(position, at::kInt, {b, h, slots})) ||
         (dropped != nullptr && !fit(dropped, at::kInt, {b})) || (position != nullptr && dropped == nullptr))

@@ -63,9 +63,9 @@ def _check_cache(cache, what: str) -> None:
     shapes = {"cached_key": codes.shape, "cached_value": codes.shape, "key_absmax": (b, h, blocks),
               "value_absmax": (b, h, blocks), "token_weight": (b, h, slots), "token_position": (b, h, slots), "dropped": (b,)}
     for name, dtype in _TENSORS.items():
-      t = cache.get(name)
-      if t is None and name in ("token_weight", "token_position", "dropped"):
+      if name not in cache and name in ("token_weight", "token_position", "dropped"):
         continue
+      t = cache[name]
       fits = t.shape in ((), (1,), (b,)) if name == "cache_index" else t.shape == shapes[name]
       if not fits or t.dtype != dtype or t.device != codes.device or not t.is_contiguous():
         raise ValueError(f"{what}: `{name}` of a cache of {b} rows, {h} heads, {slots} slots is {dtype} on {codes.device}, "

@@ -442,3 +442,18 @@ def test_refusals():
       call()
       pytest.fail(f"call {i} was not refused")
   assert all(torch.equal(cache[n], t) for n, t in before.items())
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)])
+@pytest.mark.parametrize("name", ["token_weight", "token_position", "dropped"])
+def test_entries_that_are_no_tensors(device, name):
+  """They would go without their weights or positions."""
+  whole = make(2, 2, 64, 64, 16, [3, 4], weights=True, positions=True, device=device)
+  other = make(2, 2, 64, 64, 16, [0, 0], weights=True, positions=True, device=device)
+  q, k = torch.randn(2, 1, 4, 64, device=device), torch.randn(2, 1, 2, 64, device=device)
+  for strange in (None, whole[name].cpu().numpy(), whole[name].tolist()):
+    cache = whole | {name: strange}
+    for call in (lambda: cache8.attention(q, cache, k, k), lambda: cache8.append_(cache, k, k),  # noqa: B023
+                 lambda: cache8.evict(cache, 2, out=other), lambda: cache8.evict(whole, 2, out=other | {name: strange})):  # noqa: B023
+      with pytest.raises(ValueError):
+        call()
