@@ -1231,7 +1231,8 @@ py::object cache8_attention(const Tensor& query, py::handle cache, const optiona
   const int type = type8(query);
   if (!c.ok || type < 0 || query.dim() != 4 || !c.has(query) || graph_of(query) || query.size(0) != c.b ||
       query.size(3) != c.dim || query.size(2) < c.h || query.size(2) % c.h != 0 || query.size(1) < 1 || query.stride(3) != 1 ||
-      query.size(1) * (query.size(2) / c.h) > 65535 || key.has_value() != value.has_value())
+      query.size(1) * (query.size(2) / c.h) > 65535 || key.has_value() != value.has_value() ||
+      (c.c.weight != nullptr && query.size(1) * (query.size(2) / c.h) * c.slots > 0x7fffffffLL) || c.b * c.h > 1 << 24)
     return py::none();
   T5xCache8Query q = {};
   T5xNewTokens n = {};
@@ -1293,7 +1294,7 @@ py::object cache8_evict(py::handle cache, py::handle into, int64_t keep, int64_t
   const Cache8Of c(cache.ptr()), to(into.ptr());
   if (!c.ok || !to.ok || c.device != to.device || c.b != to.b || c.h != to.h || c.dim != to.dim || c.c.weight == nullptr ||
       to.c.weight == nullptr || to.c.position == nullptr || keep < 1 || keep > to.slots || recent < 0 || recent > keep ||
-      (to.b > 1 && to.c.index_stride == 0) || c.overlaps(to))
+      to.held[4].dim() != 1 || to.held[4].numel() != to.b || c.overlaps(to))
     return py::none();
   py::gil_scoped_release no_gil;
   Tensor kept = at::empty({c.b, c.h, keep}, at::TensorOptions().dtype(at::kInt).device(at::Device(at::kCUDA, c.device)));

@@ -135,7 +135,7 @@ def attention(query: torch.Tensor, cache: dict, key: Optional[torch.Tensor] = No
   key_mask [rows, n], n <= slots: slots that are seen; those from n on are hidden. A query that sees nothing has zeros and
   gives no weight. With `token_weight` in the cache the softmax of all queries and heads that share keys is added to it."""
   host = native.host() if query.is_cuda and not F._transformed() else None
-  if host is not None and (bias_table is None or (bias_table.shape[-1] == num_buckets <= 256 and
+  if host is not None and (bias_table is None or (bias_table.dim() == 2 and 2 <= bias_table.shape[1] == num_buckets <= 256 and
                                                   num_buckets // 2 < max_distance < native.CACHE8_DISTANCES)):
     # (the plain call, checked there; anything else comes back as None)
     buckets = None if bias_table is None else native.buckets_of(num_buckets, max_distance)

@@ -457,3 +457,20 @@ def test_entries_that_are_no_tensors(device, name):
                  lambda: cache8.evict(cache, 2, out=other), lambda: cache8.evict(whole, 2, out=other | {name: strange})):  # noqa: B023
       with pytest.raises(ValueError):
         call()
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)])
+def test_refusals_are_the_same_on_every_device(device):
+  cache = make(2, 2, 64, 64, 16, [3, 4], weights=True, device=device)
+  one = make(1, 1, 64, 64, 16, [3], weights=True, device=device)
+  into = make(1, 1, 64, 64, 16, [0], weights=True, positions=True, device=device)
+  q, k = torch.randn(2, 1, 4, 64, device=device), torch.randn(2, 1, 2, 64, device=device)
+  long = cache8.init_cache(1, 1 << 17, 1, 64, device, weights=True)
+  for call in (lambda: cache8.attention(q, cache, k, k, bias_table=torch.zeros(4, 1, device=device), num_buckets=1),
+               lambda: cache8.attention(q, cache, k, k, bias_table=torch.zeros(4, 0, device=device), num_buckets=0),
+               lambda: cache8.attention(q, cache, k, k, bias_table=torch.zeros((), device=device)),
+               # 2^31 scores whose weight is added up
+               lambda: cache8.attention(torch.zeros(1, 1, 1 << 14, 64, device=device), long),
+               lambda: cache8.evict(one, 2, out=into | {"cache_index": into["cache_index"][0]})):
+    with pytest.raises(ValueError):
+      call()
