@@ -568,10 +568,13 @@ cudaError_t launch_select(const Cache8& c, int keep, int recent, int* kept, int*
   return cudaGetLastError();
 }
 
-// Both in one launch where a CTA makes the choice and has a turn of its warps to move: the device takes as long (12 heads of 64
-// channels, 640 -> 121, us so / in two 9.4 / 9.4; 2048 -> 250 10.1 / 9.9, -> 512 13.4 / 9.7; 512 heads, -> 512 29 / 30, of 128
-// channels 45 / 40), the host one launch less (11.7 to 10.3 a call).
-bool in_one_launch(const Cache8& c, int keep) { return c.slots <= 2048 && keep <= 256; }
+// Both in one launch where a CTA makes the choice and has a turn of its warps to move, and all CTAs are there at a time (four an
+// SM): the device takes as long, the host one launch less (11.7 to 10.3 a call). us so / in two: 12 heads of 64 channels, 640 -> 121 9.4 / 9.4,
+// 2048 -> 256 10.4 / 9.8, -> 512 13.4 / 9.7; 512 heads of 64, 2048 -> 32 13.5 / 13.5, -> 256 20.9 / 21.9, of 128 16.1 / 16.2 and 27.3 /
+// 27.5, -> 512 45 / 40; 640 heads of 128, -> 32 26.3 / 19.3, -> 256 39.4 / 37.3, 2048 heads 64 / 49 and 90 / 90.
+bool in_one_launch(const Cache8& c, int keep) {
+  return c.slots <= 2048 && keep <= 256 && static_cast<long long>(c.batch) * c.heads <= 4LL * num_sms();
+}
 template <int D>
 cudaError_t launch_both(const Cache8& c, const Cache8& to, int keep, int recent, int* kept, int* index_out, int* dropped_out,
                         cudaStream_t stream) {

@@ -618,3 +618,12 @@ def test_one_row_of_more_scores_than_a_launch_takes(heads, group, count, slots, 
       size = torch.full_like(want, 3.0)
       assert plain.within(out[0, i:i + 500, h * group:(h + 1) * group], want.cpu(), size.cpu(), 64.0, dim, slots)
   assert torch.allclose(cache["token_weight"].double(), before + added, rtol=1e-4, atol=1e-6)
+
+
+@pytest.mark.parametrize("rows", [148, 149, 300])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_evict_of_as_many_heads_as_the_sms_take_at_a_time_and_more(rows, dim):
+  """Four heads a row: 592 CTAs, and more."""
+  starts = [(37 * i) % 96 for i in range(rows)]
+  launches(lambda: plain.check_evict(dict(b=rows, h=4, dim=dim, slots=96, block=16, starts=starts, keep=30, recent=7, to_block=16),
+                                     "cuda", False))
