@@ -691,8 +691,9 @@ __global__ void __launch_bounds__(kJoinThreads) cache8_join_kernel(const __grid_
 // weight[slot] += the probabilities that the query rows gave it, from the scores that are in workspace: their bytes bound it.
 constexpr int kWeightThreads = 256;
 __global__ void __launch_bounds__(kWeightThreads) cache8_weight_kernel(const __grid_constant__ Cache8Attn p) {
-  const int bh = blockIdx.x, b = bh / p.c.heads;
-  const int s = blockIdx.y * kWeightThreads + threadIdx.x;
+  const unsigned blocks = (p.c.slots + kWeightThreads - 1u) / kWeightThreads;
+  const int bh = blockIdx.x / blocks, b = bh / p.c.heads;
+  const int s = (blockIdx.x - bh * blocks) * kWeightThreads + threadIdx.x;
   const int start = held_of(p.c, b), end = end_of(p, start);
   chain_wait();
   chain_release();
@@ -772,9 +773,9 @@ cudaError_t launch_pieces(const Cache8Attn& p, bool behind, cudaStream_t stream)
   e = p.c.dim == 64 ? launch_behind(true, cache8_join_kernel<T, 64>, rows, kJoinThreads, 0, stream, p, tile_rows)
                     : launch_behind(true, cache8_join_kernel<T, 128>, rows, kJoinThreads, 0, stream, p, tile_rows);
   if (e != cudaSuccess || p.scores == nullptr) return e;
-  return launch_behind(true, cache8_weight_kernel,
-                       dim3(static_cast<unsigned>(p.c.batch) * p.c.heads, (p.c.slots + kWeightThreads - 1) / kWeightThreads),
-                       kWeightThreads, 0, stream, p);
+  // (a part has so few scores that these are below 2^31)
+  const unsigned blocks = (p.c.slots + kWeightThreads - 1u) / kWeightThreads;
+  return launch_behind(true, cache8_weight_kernel, dim3(blocks * p.c.batch * p.c.heads), kWeightThreads, 0, stream, p);
 }
 
 // What a launch has of a call: batch rows, key heads and queries.

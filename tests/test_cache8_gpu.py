@@ -627,3 +627,21 @@ def test_evict_of_as_many_heads_as_the_sms_take_at_a_time_and_more(rows, dim):
   starts = [(37 * i) % 96 for i in range(rows)]
   launches(lambda: plain.check_evict(dict(b=rows, h=4, dim=dim, slots=96, block=16, starts=starts, keep=30, recent=7, to_block=16),
                                      "cuda", False))
+
+
+def test_weights_of_more_slots_than_65535_blocks():
+  """16.8 million slots, of which a mask shows a few: the first, one in the middle, those at the end."""
+  slots = 65536 * 256 + 64
+  cache = cache8.init_cache(1, slots, 1, 64, "cuda", block=64, weights=True)
+  at = torch.tensor([0, 12345678, 65535 * 256 + 7, slots - 1], device="cuda")
+  cache["cached_value"][0, 0, at] = torch.randint(-127, 128, (4, 64), device="cuda", dtype=torch.int8)
+  cache["value_absmax"][0, 0, at // 64] = 1.0
+  cache["cache_index"].fill_(slots)
+  shown = torch.zeros(1, slots, dtype=torch.bool, device="cuda")
+  shown[0, at] = True
+  out = launches(lambda: cache8.attention(torch.randn(1, 1, 1, 64, device="cuda"), cache, key_mask=shown))
+  # (keys of 0: each has a quarter)
+  want = cache["cached_value"][0, 0, at].double().mean(0) / 127
+  assert torch.allclose(out[0, 0, 0].double(), want, rtol=0, atol=2.0 ** -21)
+  assert torch.allclose(cache["token_weight"][0, 0, at], torch.full((4,), 0.25, device="cuda"), rtol=2.0 ** -21)
+  assert cache["token_weight"].sum(dtype=torch.float64).item() == pytest.approx(1.0, rel=2.0 ** -20)
