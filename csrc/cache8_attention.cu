@@ -691,9 +691,9 @@ __global__ void __launch_bounds__(kJoinThreads) cache8_join_kernel(const __grid_
 // weight[slot] += the probabilities that the query rows gave it, from the scores that are in workspace: their bytes bound it.
 constexpr int kWeightThreads = 256;
 __global__ void __launch_bounds__(kWeightThreads) cache8_weight_kernel(const __grid_constant__ Cache8Attn p) {
-  const unsigned blocks = (p.c.slots + kWeightThreads - 1u) / kWeightThreads;
-  const int bh = blockIdx.x / blocks, b = bh / p.c.heads;
-  const int s = (blockIdx.x - bh * blocks) * kWeightThreads + threadIdx.x;
+  const unsigned all = p.c.batch * p.c.heads, block = blockIdx.x / all;
+  const int bh = blockIdx.x - block * all, b = bh / p.c.heads;
+  const int s = block * kWeightThreads + threadIdx.x;
   const int start = held_of(p.c, b), end = end_of(p, start);
   chain_wait();
   chain_release();
