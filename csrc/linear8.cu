@@ -362,9 +362,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         far |= !ordinary(most_n);
         sw[i] = most_n * (1.f / 127.f);
       }
-      far = __any_sync(0xffffffffu, far);  // (one value at a time then)
-      const bool wide = p.vec == 2 && !far;
-      if (wide) {  // in the patch
+      if (p.vec == 2) {  // in the patch
         __syncwarp();
 #pragma unroll
         for (int i = 0; i < kBlocks; ++i) patch[i * 32 + lane] = sw[i];
@@ -377,9 +375,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       }
       tc_fence_after();
       const uint32_t t_row = tmem + (static_cast<uint32_t>(q * 32) << 16) + acc * kTileCols;
+      far = __any_sync(0xffffffffu, far);  // (one value at a time then, below)
       // A lane stores its row's channels where they are whole sectors. (In 32 bits, 4096 x 64 x 16384: 101 us so, 114 by patches; 4096 x
       // 57 x 16004, whole 16 bytes alone: 176 and 130.)
-      if (wide) {
+      if (p.vec == 2 && !far) {
         constexpr int E = 16 / sizeof(T), W = sizeof(T) == 4 ? 32 : 64, L = W / E;  // values of 16 bytes, channels at a time, 16 bytes of a lane
 #pragma unroll 1
         for (int c = 0; c < kTileCols / 2; c += W) {
@@ -417,7 +416,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         }
       }
       // Rows at any address: by patches of 32 x 32, a lane a channel. The next sums are requested before these are stored.
-      if (!wide && first < p.N && m0 < p.M) {
+      if (p.vec != 2 && !far && first < p.N && m0 < p.M) {
         const int rows = min(32, p.M - m0);
         uint32_t r[32];
         tmem_ld32(t_row + col0, r);
@@ -427,7 +426,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           if (n0 >= p.N) break;
           const bool mine = n0 + lane < p.N;
           T add[32];
-          if (residual != nullptr && mine && !far) {
+          if (residual != nullptr && mine) {
 #pragma unroll
             for (int i = 0; i < 32; ++i)
               if (i < rows) add[i] = residual[(m0 + i) * p.ld_res + n0 + lane];
@@ -435,19 +434,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           tmem_ld_wait();
           __syncwarp();  // the patch's last readers are done
 #pragma unroll
-          for (int j = 0; j < 32; ++j)
-            patch[lane * 33 + j] = far ? __uint_as_float(r[j]) : static_cast<float>(static_cast<int>(r[j])) * sx;
+          for (int j = 0; j < 32; ++j) patch[lane * 33 + j] = static_cast<float>(static_cast<int>(r[j])) * sx;
           __syncwarp();
           if (cb + 1 < kBlocks && n0 + 32 < p.N) tmem_ld32(t_row + col0 + (cb + 1) * 32, r);
-          if (mine && far) {
-            const float most_n = p.w_absmax[n0 + lane];
-#pragma unroll 1
-            for (int i = 0; i < rows; ++i) {
-              const float plus = residual != nullptr ? to_float(residual[(m0 + i) * p.ld_res + n0 + lane]) : 0.f;
-              y[static_cast<long long>(m0 + i) * p.N + n0 + lane] =
-                  from_float<T>(in_64_bits(__float_as_int(patch[i * 33 + lane]), p.x_absmax[m0 + i], most_n, plus));
-            }
-          } else if (mine) {
+          if (mine) {
             T* to = y + static_cast<long long>(m0) * p.N + n0 + lane;
 #pragma unroll
             for (int i = 0; i < 32; ++i) {
@@ -456,6 +446,26 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
               if (i < rows) *to = from_float<T>(v);
               to += p.N;
             }
+          }
+        }
+      }
+      if (far && m0 < p.M) {
+#pragma unroll 1
+        for (int n0 = first; n0 < min(first + kTileCols / 2, p.N); n0 += 32) {
+          uint32_t r[32];
+          tmem_ld32(t_row + col0 + (n0 - first), r);
+          tmem_ld_wait();
+          __syncwarp();  // the patch's last readers are done
+#pragma unroll
+          for (int j = 0; j < 32; ++j) patch[lane * 33 + j] = __uint_as_float(r[j]);
+          __syncwarp();
+          if (n0 + lane >= p.N) continue;
+          const float most_n = p.w_absmax[n0 + lane];
+#pragma unroll 1
+          for (int i = 0; i < min(32, p.M - m0); ++i) {
+            const float plus = residual != nullptr ? to_float(residual[(m0 + i) * p.ld_res + n0 + lane]) : 0.f;
+            y[static_cast<long long>(m0 + i) * p.N + n0 + lane] =
+                from_float<T>(in_64_bits(__float_as_int(patch[i * 33 + lane]), p.x_absmax[m0 + i], most_n, plus));
           }
         }
       }
