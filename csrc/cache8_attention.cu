@@ -32,10 +32,11 @@
 // second kernel joins the pieces. Many query rows have a kernel of their own, cache8_rows.cu.
 //
 // Measured, us on the device of a call with its append: 64 rows x 32 heads of 64 channels, up to 1024 slots of all lengths,
-// with biases, positions and weights, 59 (2.5 TB/s; 35 % of the issue slots: a CTA has four steps of tiles, and waits for
-// memory before and behind them as long); 8 rows x 8 heads of 128 channels, 8 queries each, up to 65536 slots of all lengths, 95
-// (4.7 TB/s; full rows run at 89 % of the copy rate, the arithmetic on codes takes 80 to 85 % of its pipe); 12 heads over 640
-// slots 8.4, all of it latency.
+// with biases, positions and weights, 59 (2.5 TB/s; 38 % of the issue slots: a CTA has four steps of tiles, and waits for
+// memory before and behind them as long); 8 rows x 8 heads of 128 channels, 8 queries each, up to 65536 slots of all lengths, 94
+// (4.7 TB/s; full rows 197, 5.5 TB/s, 83 % of the copy rate: latency, four warps a scheduler wait for codes 38 % of their time and for
+// an instruction's result 21 %, with 46 % of the issue slots and 41 % of the ALU pipe taken); 12 heads over 640 slots 8.3, all of it
+// latency.
 #include <algorithm>
 #include <type_traits>
 

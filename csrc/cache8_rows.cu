@@ -9,9 +9,10 @@
 // take, warps share rows, take different tokens of a step, and meet in shared memory at the end.
 //
 // Bound by latency between the products: two warps a scheduler (128 sums a lane leave no room for more) keep the matrix pipe
-// 38 % busy, the issue slots 33 %. Measured, us for 2 x 4 heads of 128 channels with the append and the join: 500 rows over
-// 8192 slots 86, over 32768 277 (242 TFLOP/s); 256 rows over 8192 55, 64 rows 27. Two tiles of tokens at a time instead of
-// one: 90 to 86 and 306 to 277; operands requested a step ahead: 96 to 90.
+// 37 % busy, the issue slots 30 %, and wait for an instruction's result 29 % of their time. Measured, us for 2 x 4 heads of 128 channels with
+// the append and the join: 500 rows over 8192 slots, four fifths of them held, 87 (in 32 bits 135), over 32768 242, all held 286 (234
+// TFLOP/s); 256 rows over 8192 55, 64 rows 26. Two tiles of tokens at a time instead of one took 4 and 9 % off, operands requested a step
+// ahead 6.
 #include <algorithm>
 #include <type_traits>
 

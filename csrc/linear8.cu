@@ -7,9 +7,9 @@
 // Two launches, for more than two rows: the rows are turned into codes, and tcgen05 (kind::i8, sums in 32 bits in tensor memory)
 // multiplies them.
 // It runs at twice the rate of bf16, so that a large product has half the time of `native.gemm`; over few rows both are
-// bound by the weights' bytes, which are half of bf16's. 8192 x 10240 x 4096: 268 us, 42 for the codes and some 220 for the product
-// (3.1 POP/s; the tensor pipe is 88 % busy), 210 at twice the measured rate of bf16. 4096 x 64 x 16384: 57 us, 134 MB of outputs at
-// 2.5 TB/s; 16001 outputs 100: what a warp does for a tile is a chain of trips to memory.
+// bound by the weights' bytes, which are half of bf16's. 8192 x 10240 x 4096: 260 us, 41 for the codes and some 217 for the product
+// (3.2 POP/s; the tensor pipe is 91 % busy), 210 at twice the measured rate of bf16. 4096 x 64 x 16384: 58 us, 134 MB of outputs at
+// 2.4 TB/s; 16001 outputs 99: what a warp does for a tile is a chain of trips to memory.
 #include <algorithm>
 
 #include "cache8.cuh"
@@ -493,7 +493,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 // cuts the input channels into one piece a CTA, so that all SMs stream weights at the same time. The weights are the 128-row
 // operand (tokens, of which there may be one, the other), and are requested while the rows are still turned into codes (a
 // programmatic dependent launch). The sums, whole numbers, meet through distributed shared memory, in no particular order:
-// they are exact. 61 x 4096 x 10240: 14.9 us with the rows' codes, 6.7 at the copy rate. What a
+// they are exact. 61 x 4096 x 10240: 15 us with the rows' codes, 6.7 at the copy rate. What a
 // CTA begins and ends with (the rows' codes, the sums of a cluster) is as long as the weights take.
 // ---------------------------------------------------------------------------
 constexpr int kFewThreads = 128;
@@ -723,7 +723,7 @@ __global__ void __launch_bounds__(kFewThreads)
 // ---------------------------------------------------------------------------
 // One row or two in one launch: each CTA turns them into codes for itself (they are in L2), behind its first requests for
 // weights; two CTAs an SM take output channels in turn, two a warp, 512 bytes of both at a time, by dot products of four bytes. The
-// weights' bytes bound it: 1 x 4096 x 32128 takes 21.9 us, 92 % of the copy rate.
+// weights' bytes bound it: 1 x 4096 x 32128 takes 21.8 us, 92 % of the copy rate.
 // ---------------------------------------------------------------------------
 constexpr int kOneThreads = 256;
 constexpr int kOneWarps = kOneThreads / 32;
