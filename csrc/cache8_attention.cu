@@ -450,19 +450,17 @@ __global__ void __launch_bounds__(kWarps * 32, 16 / kWarps)
       if (__any_sync(0xffffffffu, raise)) {
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          float x = -INFINITY, x2 = -INFINITY;
+          float x = -INFINITY, term = -INFINITY;
 #pragma unroll
-          for (int ms = 0; ms < MS; ++ms) {
-            const float high = fmaxf(s[ms][e], s[ms][2 + e]);
-            x = fmaxf(x, high);
-            x2 = fmaxf(x2, high + log2_approx(va[ms]));
-          }
+          for (int ms = 0; ms < MS; ++ms) x = fmaxf(x, fmaxf(s[ms][e], s[ms][2 + e]));
 #pragma unroll
-          for (int lanes = 4; lanes < 32; lanes *= 2) {
-            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, lanes));
-            x2 = fmaxf(x2, __shfl_xor_sync(0xffffffffu, x2, lanes));
-          }
-          const float2 by = raise_to(ref[e], x, x2);
+          for (int lanes = 4; lanes < 32; lanes *= 2) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, lanes));
+          const float score = raised(ref[e], x);
+#pragma unroll
+          for (int ms = 0; ms < MS; ++ms) term = fmaxf(term, fmaxf(s[ms][e], s[ms][2 + e]) - score + log2_approx(va[ms]));
+#pragma unroll
+          for (int lanes = 4; lanes < 32; lanes *= 2) term = fmaxf(term, __shfl_xor_sync(0xffffffffu, term, lanes));
+          const float2 by = raise_to(ref[e], score, term);
           l[e] *= by.x;
 #pragma unroll
           for (int i = 0; i < MI; ++i) o[i][e] *= by.y, o[i][2 + e] *= by.y;
@@ -473,6 +471,8 @@ __global__ void __launch_bounds__(kWarps * 32, 16 / kWarps)
       uint32_t pf[Q2][MT][2];
 #pragma unroll
       for (int ms = 0; ms < MS; ++ms) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) s[ms][k] -= ref[k & 1].score;
         float r[2] = {va[ms] * ref[0].by, va[ms] * ref[1].by};
         float counts = 1.f;  // in the sum that divides
         if (!(fmaxf(r[0], r[1]) < kFar)) {
@@ -483,7 +483,7 @@ __global__ void __launch_bounds__(kWarps * 32, 16 / kWarps)
             r[e] = part.x;
 #pragma unroll
             for (int k = e; k < 4; k += 2) {
-              l[e] += exp2_approx(s[ms][k] - ref[e].score);
+              l[e] += exp2_approx(s[ms][k]);
               s[ms][k] = far_score(s[ms][k], part.y, va[ms]);
             }
           }
@@ -491,7 +491,7 @@ __global__ void __launch_bounds__(kWarps * 32, 16 / kWarps)
         float pr[4];
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-          pr[k] = exp2_approx(s[ms][k] - ref[k & 1].score);
+          pr[k] = exp2_approx(s[ms][k]);
           l[k & 1] += pr[k] * counts;
           pr[k] *= r[k & 1];
         }

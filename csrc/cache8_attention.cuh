@@ -140,18 +140,17 @@ __device__ __forceinline__ int scale_of(const Reference& r) { return 127 - stati
 __device__ __forceinline__ bool beyond(const Reference& r, float s, float a) {
   return s - r.score > kLimit - fmaxf(log2_approx(a), 0.f);
 }
-// x: the row's largest score here; x2: the largest with the logarithm of its block's largest value. What the sum that divides
-// and the other ones are multiplied by: 1 where nothing changes.
-__device__ __forceinline__ float2 raise_to(Reference& r, float x, float x2) {
-  const float old = static_cast<float>(scale_of(r));
-  const bool higher = x - r.score > kLimit, wider = x2 - r.score - old > kLimit;
-  const float up = higher ? x - kPeak : r.score;
-  const float to = wider ? x2 - kPeak : r.score + old;
-  const float scale = higher || wider ? fminf(fmaxf(ceilf(to - up), -126.f), 126.f) : old;
-  const float2 by = make_float2(exp2_approx(r.score - up), exp2_approx((r.score - up) + (old - scale)));
-  r.score = up;
+// The reference of scores of which x is the row's largest here.
+__device__ __forceinline__ float raised(const Reference& r, float x) { return x - r.score > kLimit ? x - kPeak : r.score; }
+// score: what `raised` gave; term: the row's largest score here relative to that, with the logarithm of its block's largest value.
+// (Differences alone: scores may be as large as the lowest masks, beside which a logarithm would vanish.) What the sum that divides and
+// the other ones are multiplied by: 1 where nothing changes.
+__device__ __forceinline__ float2 raise_to(Reference& r, float score, float term) {
+  const float lower = r.score - score, old = lower + static_cast<float>(scale_of(r));  // where the sums are, relative to `score`
+  const float scale = fminf(fmaxf(ceilf(term - old > kLimit ? term - kPeak : old), -126.f), 126.f);
+  r.score = score;
   r.by = power_of_two(-static_cast<int>(scale));
-  return by;
+  return make_float2(exp2_approx(lower), exp2_approx(old - scale));
 }
 
 // Where a block's largest value a, relative to the scale, is no factor that 32 bits hold a small probability beside (or no number):
@@ -162,7 +161,7 @@ __device__ __forceinline__ float2 part_of(const Reference& r, float a) {
   return make_float2(u < 0x00800000u ? 0.f : __uint_as_float((u & 0x007fffffu) | 0x3f800000u),
                      static_cast<float>(static_cast<int>(u >> 23) - 127 - scale_of(r)));
 }
-// A score then; of a block that is not finite NaN, unless it is hidden.
+// A score, relative to the reference, then; of a block that is not finite NaN, unless it is hidden.
 __device__ __forceinline__ float far_score(float s, float exponent, float a) {
   return s == -INFINITY ? s : s + exponent + (a - a);
 }

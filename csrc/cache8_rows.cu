@@ -385,19 +385,20 @@ __global__ void __launch_bounds__(kThreads, 1) cache8_rows_kernel(const __grid_c
           for (int m = 0; m < M; ++m)
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-              float x = -INFINITY, x2 = -INFINITY;
+              auto high = [&](int mt) {
+                return fmaxf(fmaxf(s[mt][m][0][2 * e], s[mt][m][0][2 * e + 1]), fmaxf(s[mt][m][1][2 * e], s[mt][m][1][2 * e + 1]));
+              };
+              float x = -INFINITY, term = -INFINITY;
 #pragma unroll
-              for (int mt = 0; mt < MT; ++mt) {
-                const float high = fmaxf(fmaxf(s[mt][m][0][2 * e], s[mt][m][0][2 * e + 1]), fmaxf(s[mt][m][1][2 * e], s[mt][m][1][2 * e + 1]));
-                x = fmaxf(x, high);
-                x2 = fmaxf(x2, high + log2_approx(va[mt]));
-              }
+              for (int mt = 0; mt < MT; ++mt) x = fmaxf(x, high(mt));
 #pragma unroll
-              for (int lanes = 1; lanes < 4; lanes *= 2) {
-                x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, lanes));
-                x2 = fmaxf(x2, __shfl_xor_sync(0xffffffffu, x2, lanes));
-              }
-              const float2 by = raise_to(ref[m][e], x, x2);
+              for (int lanes = 1; lanes < 4; lanes *= 2) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, lanes));
+              const float score = raised(ref[m][e], x);
+#pragma unroll
+              for (int mt = 0; mt < MT; ++mt) term = fmaxf(term, high(mt) - score + log2_approx(va[mt]));
+#pragma unroll
+              for (int lanes = 1; lanes < 4; lanes *= 2) term = fmaxf(term, __shfl_xor_sync(0xffffffffu, term, lanes));
+              const float2 by = raise_to(ref[m][e], score, term);
               l[m][e] *= by.x;
 #pragma unroll
               for (int i = 0; i < D / 8; ++i) o[m][i][2 * e] *= by.y, o[m][i][2 * e + 1] *= by.y;
@@ -410,6 +411,8 @@ __global__ void __launch_bounds__(kThreads, 1) cache8_rows_kernel(const __grid_c
           uint4 pf[M][Q2];
 #pragma unroll
           for (int m = 0; m < M; ++m) {
+#pragma unroll
+            for (int k = 0; k < 8; ++k) s[mt][m][k >> 2][k & 3] -= ref[m][k >> 1 & 1].score;
             float r[2] = {va[mt] * ref[m][0].by, va[mt] * ref[m][1].by};
             float counts = 1.f;  // in the sum that divides
             if (!(fmaxf(r[0], r[1]) < kFar)) {
@@ -421,7 +424,7 @@ __global__ void __launch_bounds__(kThreads, 1) cache8_rows_kernel(const __grid_c
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
                   float& x = s[mt][m][k >> 1][2 * e + (k & 1)];
-                  l[m][e] += exp2_approx(x - ref[m][e].score);
+                  l[m][e] += exp2_approx(x);
                   x = far_score(x, part.y, va[mt]);
                 }
               }
@@ -435,7 +438,7 @@ __global__ void __launch_bounds__(kThreads, 1) cache8_rows_kernel(const __grid_c
 #pragma unroll
                 for (int k = 0; k < 2; ++k) {
                   const float x = s[mt][m][n][2 * e + k];
-                  pr[k] = exp2_approx(x - ref[m][e].score);
+                  pr[k] = exp2_approx(x);
                   l[m][e] += pr[k] * counts;
                   pr[k] *= r[e];
                 }

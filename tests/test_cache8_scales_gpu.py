@@ -148,3 +148,30 @@ def test_blocks_of_the_largest_and_smallest_values(dim, group, count, dtype):
     for scales in ((2.0 ** 90, 2.0 ** -60), (2.0 ** -60, 2.0 ** 60), (0.0, 1.0)):
       query, cache = scene(dim, group, count, 1024, dtype, -100.0 if scales[0] > 1 else 5.0, scales, at)
       check(query, cache, dtype)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("dim,group,count", FORMS)
+@pytest.mark.parametrize("tokens", [64, 4096])
+@pytest.mark.parametrize("spread", [0, 4, 30])
+def test_biases_of_the_lowest_value_over_blocks_of_any_scale(dim, group, count, tokens, spread, dtype):
+  """All that a row sees has the lowest bias: its softmax is uniform, whatever the blocks' largest values are."""
+  gen = torch.Generator("cuda").manual_seed(5)
+  for size in (2.0 ** -60, 1e-6, 1e6, 2.0 ** 60):
+    cache = cache8.init_cache(1, tokens, 1, dim, "cuda", block=16)
+    cache["cached_value"].copy_(torch.randint(-127, 128, cache["cached_value"].shape, generator=gen, device="cuda", dtype=torch.int8))
+    cache["cached_key"].copy_(torch.randint(-127, 128, cache["cached_key"].shape, generator=gen, device="cuda", dtype=torch.int8))
+    cache["key_absmax"].fill_(1.0)
+    down = torch.randint(-spread, 1, (tokens // 16,), generator=gen, device="cuda")
+    most = torch.ldexp(torch.full_like(down, size, dtype=torch.float32), down)
+    cache["value_absmax"][0, 0] = most
+    cache["cache_index"].fill_(tokens)
+    query = torch.randn(1, count, group, dim, generator=gen, device="cuda").to(dtype)
+    out = attend(query, cache, bias_table=torch.full((group, 32), torch.finfo(torch.float32).min, device="cuda"), causal=False)
+    v = cache["cached_value"][0, 0].double() * most.double().repeat_interleave(16)[:, None] / 127
+    want, each = v.mean(0), v.abs().mean(0)
+    # a probability is rounded once and in 32 bits; the largest term is that of the largest block
+    floor = most.max().double() * (2.0 ** -42 if dtype == torch.float32 else 2.0 ** -31)
+    bound = each * ((0 if dtype == torch.float32 else 2.0 ** -10) + (tokens // 16 + 64) * 2.0 ** -24 + 2.0 ** -21) + floor
+    off = (out[0].double().flatten(0, 1) - want).abs() - torch.finfo(dtype).eps / 2 * want.abs()
+    assert bool((off <= bound).all()), (size, (off / each).max())
