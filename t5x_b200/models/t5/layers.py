@@ -269,7 +269,8 @@ def quantize_dense(module: nn.Module) -> int:
   channel, activations by token. The kernels stay as they are; a projection whose kernel changes afterwards raises until this
   is called again. (It sees what raises the kernel's version: operations in place, a step of the framework's optimizers, loaded
   state; not what is written through `.data`, in inference mode, by a replayed CUDA graph or by kernels of the user's own: call
-  this again after those.) Returns how many projections there are. The embedding and the logits (in 32 bits) are left alone."""
+  this again after those.) Beam search of an encoder-decoder goes step by step then, not through the captured step, which holds
+  weights in bf16. Returns how many projections there are. The embedding and the logits (in 32 bits) are left alone."""
   if pstate.get().model_size > 1:
     raise ValueError("quantize_dense: not under a model axis")
   found = [m for name, m in module.named_modules() if type(m) is DenseGeneral and not name.endswith("logits_dense")]

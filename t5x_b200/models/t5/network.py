@@ -46,7 +46,7 @@ class T5Config:
   scale_attn_logits: bool = False      # t5x/contrib/gpu/t5/layers.py:205-206
   relpos_num_buckets: int = 32
   relpos_max_distance: int = 128
-  kv_cache_dtype: Any = None  # "int8": decode caches in 8 bits
+  kv_cache_dtype: Any = None  # "int8": decode caches in 8 bits (beam search goes step by step then, not captured)
   kv_cache_keep: int = 0      # tokens that stay in the decoder's cache (0: all), the last kv_cache_recent among them
   kv_cache_recent: int = 0
 
